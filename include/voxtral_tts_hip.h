@@ -322,6 +322,48 @@ const char *tts_hip_last_error(void);
  * exported so that the format can be checked bit for bit.  Returns 0, or -1 on error. */
 int tts_hip_split_planes(uint16_t *d_hi, uint16_t *d_lo, const float *d_x, size_t n);
 
+/* ==== 4 bits: linear layers and a key/value cache in microscaled floats ====
+ * No counterpart in the reference.  The format is MXFP4 of the OCP microscaling specification: a block of
+ * 32 consecutive values of a row is 32 codes e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) and one scale
+ * e8m0, 2^(s - 127).  s = floor(log2 of the block's largest magnitude) - 2 + 127, at least 0; a code is the
+ * nearest value's, of two equally near ones the even code, 6 for what lies beyond 6.  A block with an
+ * infinity or a NaN in it is held as s = 255 and stands for 32 NaN.
+ * A matrix [rows, cols] is d_codes [rows, 64 P] and d_scales [rows, 4 P] bytes with P = cols / 128 rounded
+ * up: two codes a byte, the first in its low half, zeros behind the last column.  Codes lie on 16 bytes,
+ * scales on 4.  Device pointers only; asynchronous on the library's stream; 0 / -1. */
+
+/* values [rows, cols], x_stride of them apart from row to row (0: cols), fp32 or, with x_bf16, bf16 -> codes
+ * and scales.  Values may lie on any multiple of their size; cols up to 2^27. */
+int tts_hip_mx4_quantize(uint8_t *d_codes, uint8_t *d_scales, const void *d_x, int x_bf16,
+                         int rows, int cols, int x_stride);
+/* codes and scales -> the values that they stand for, fp32, exactly; the room between rows is left as it was. */
+int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const uint8_t *d_scales,
+                           int rows, int cols, int x_stride);
+/* y[seq_len, out_dim] = x[seq_len, in_dim] W^T, W [out_dim, in_dim] in 4 bits, x and y fp32 and dense: what
+ * tts_hip_linear_bf16 is for bf16 weights. */
+int tts_hip_linear_mx4(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales,
+                       int seq_len, int in_dim, int out_dim);
+
+/* One layer's key/value cache in 4 bits: codes [n_kv_heads, max_rows, head_dim / 2] and scales
+ * [n_kv_heads, max_rows, head_dim / 32], the caller's device memory.  head_dim 64, 128, 192 or 256.  Only the
+ * struct is read from host memory, during the call. */
+typedef struct {
+    uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+    int max_rows, n_kv_heads, head_dim;
+} tts_hip_kv4_t;
+
+/* K and V rows [n_rows, n_kv_heads * head_dim] fp32, `stride` floats apart (0: dense), into the cache's rows
+ * pos .. pos + n_rows - 1; the others stay as they were. */
+int tts_hip_kv4_append(const tts_hip_kv4_t *cache, const float *d_K, const float *d_V, int n_rows, int pos, int stride);
+/* The cache's rows pos .. pos + n_rows - 1 back as the fp32 values that they stand for. */
+int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cache, int n_rows, int pos, int stride);
+/* Causal attention over the cache: query i of Q [seq_len, n_heads * head_dim] sees the rows 0 .. start_pos + i,
+ * which hold its own keys and values too (append first); out like Q, on 16 bytes both.  n_heads is a multiple
+ * of n_kv_heads.  A decode step is seq_len 1; what tts_hip_causal_attention_decode and _prefill are for an
+ * fp32 cache.  Rows that no query sees are not looked at, whatever they hold. */
+int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_hip_kv4_t *cache, int seq_len,
+                          int start_pos, int n_heads, float scale);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,230 @@
+"""The key/value cache in 4 bits through the C ABI: append, read and attention against numpy in 64 bits (mx4support.py), and a
+decoder layer in 4 bits as a program runs it."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import hipsupport as H
+import mx4support as M
+import vtsupport as S
+
+pytestmark = pytest.mark.gpu
+LAYOUTS = [(32, 8, 128), (16, 16, 64), (8, 1, 128), (12, 4, 256), (14, 2, 64), (6, 2, 192), (20, 1, 64)]
+
+
+@pytest.fixture(scope="module")
+def hip():
+    h = H.Hip(kv_max=8)
+    yield h
+    h.close()
+
+
+@pytest.mark.parametrize("kv_heads,hd", [(8, 128), (1, 64), (3, 192), (2, 256)])
+@pytest.mark.parametrize("n,pos,gap,shift", [(1, 0, 0, 0), (1, 301, 0, 0), (37, 5, 12, 0), (200, 100, 3, 1)])
+def test_append_and_read(hip, kv_heads, hd, n, pos, gap, shift):
+    rows, width = 310, kv_heads * hd
+    c = M.Cache(hip, rows, kv_heads, hd)
+    for a in c.host.values():
+        a[:] = np.random.default_rng(a.size).integers(0, 255, a.shape)
+    cache = c.upload()
+    x = [S.f32_normal((n, width + gap), 10 + i) * 3 for i in range(2)]
+    dev = [H.DevBuf(hip.lib, a.nbytes + 64) for a in x]
+    for d, a in zip(dev, x):
+        hip.lib.tts_hip_to_device(d.at(4 * shift), a.ctypes.data, a.nbytes)
+    k, v = (d.at(4 * shift) for d in dev)
+    assert hip.lib.tts_hip_kv4_append(cache, k, v, n, pos, width + gap) == 0
+    got = c.download()
+    c.fill(*[a[:, :width].reshape(n, kv_heads, hd).transpose(1, 0, 2) for a in x], pos)
+    for name in got:
+        assert np.array_equal(got[name], c.host[name]), name                                    # the other rows too
+    for d, a in zip(dev, x):
+        hip.lib.tts_hip_memset(d.ptr, 0x55, a.nbytes + 64)
+    assert hip.lib.tts_hip_kv4_read(k, v, cache, n, pos, width + gap) == 0
+    for d, a, name in zip(dev, x, "kv"):
+        back = d.to_numpy(np.float32, a.size + 16)[shift:shift + a.size].reshape(a.shape)
+        want = M.decode(c.host[name + "c"][:, pos:pos + n], c.host[name + "s"][:, pos:pos + n])
+        assert np.array_equal(back[:, :width], want.transpose(1, 0, 2).reshape(n, width).astype(np.float32))
+        assert np.all(back[:, width:] == np.frombuffer(b"\x55" * 4, np.float32)[0])
+        d.free()
+    hip.check()
+    c.free()
+
+
+def attend(hip, cache, q, pos, heads, scale):
+    dq, do = H.DevBuf.from_numpy(hip.lib, q), H.DevBuf(hip.lib, q.nbytes + 64)
+    hip.lib.tts_hip_memset(do.ptr, 0x55, q.nbytes + 64)
+    assert hip.lib.tts_hip_kv4_attention(do.ptr, dq.ptr, cache, q.shape[0], pos, heads, scale) == 0
+    out = do.to_numpy(np.float32, q.size + 16)
+    hip.check()
+    dq.free()
+    do.free()
+    assert np.all(out[q.size:] == np.frombuffer(b"\x55" * 4, np.float32)[0])
+    return out[:q.size].reshape(q.shape)
+
+
+def oracle(q, k, v, pos, heads, scale):
+    """-> out, tolerance [rows, heads * hd]; k, v [kv_heads, pos + rows, hd]"""
+    rows, hd, n = q.shape[0], k.shape[2], pos + q.shape[0]
+    out, tol = np.zeros((rows, heads, hd)), np.zeros((rows, heads, hd))
+    seen = np.arange(n)[None] <= pos + np.arange(rows)[:, None]
+    for h in range(heads):
+        kh, vh = k[h * len(k) // heads], v[h * len(k) // heads]
+        qh = q.reshape(rows, heads, hd)[:, h].astype(np.float64)
+        s = np.where(seen, qh @ kh.T * scale, -np.inf)
+        m = s.max(1, keepdims=True)
+        p = np.exp(s - m)
+        p /= p.sum(1, keepdims=True)
+        out[:, h] = p @ vh
+        # a score, times the magnitude of the scale (an error has no sign): q enters as five planes, each leaving 2^-4 of its block's largest magnitude, the accumulators are cut at 2^-23
+        # ten times, the scale and the difference to the largest score rounded: 2^-24 of each.  The weights' exponential: 2^-22, and
+        # what the exponent's rounding to 2^-24 of itself makes.  A weight's error e is a relative one, in the sum of the weights and in that
+        # of the values.  Sums over n rows: chains of n / 64 at 2^-24 and the parts'; weights enter as 24 bits, accumulators cut at 2^-23.
+        ds = np.where(seen, abs(scale) * (2.0 ** -20 * (M.block_max(qh) @ np.abs(kh).T) + 2.0 ** -19 * (np.abs(qh) @ np.abs(kh).T)) + 2.0 ** -22 * np.abs(np.where(seen, s, 0)), 0)
+        far = np.where(seen & (p > 1e-12), m - s, 0).max(1, keepdims=True)
+        e = 2 * ds.max(1, keepdims=True) + 2.0 ** -21 + 2.0 ** -23 * far + 2.0 ** -23 * (n / 32 + 40)
+        tol[:, h] = e * (p @ np.abs(vh)) + 1e-37
+    return out.reshape(rows, -1), tol.reshape(rows, -1)
+
+
+def case(hip, heads, kv_heads, hd, rows, pos, spread=1.0, extra=37):
+    c = M.Cache(hip, pos + rows + extra, kv_heads, hd)
+    r = np.random.default_rng(heads + 31 * rows + pos)
+    for a in c.host.values():
+        a[:] = 255                                        # behind the last row: codes of -6, scales of NaN
+    c.fill(*[r.standard_normal((kv_heads, pos + rows, hd)).astype(np.float32) * spread for _ in range(2)])
+    return c, (r.standard_normal((rows, heads * hd)) * spread).astype(np.float32)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", LAYOUTS)
+@pytest.mark.parametrize("rows,pos", [(1, 0), (1, 1), (1, 15), (1, 16), (1, 300), (1, 2999), (3, 5), (5, 1000), (16, 0), (17, 130), (65, 0), (130, 70), (33, 2100)])
+def test_attention(hip, heads, kv_heads, hd, rows, pos):
+    c, q = case(hip, heads, kv_heads, hd, rows, pos)
+    got = attend(hip, c.upload(), q, pos, heads, 1 / np.sqrt(hd))
+    want, tol = oracle(q, *c.values(pos + rows), pos, heads, float(np.float32(1 / np.sqrt(hd))))
+    c.free()
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("rows,pos", [(1, 40000), (9, 33333), (400, 517)])
+def test_attention_long(hip, rows, pos):
+    c, q = case(hip, 8, 2, 128, rows, pos)
+    got = attend(hip, c.upload(), q, pos, 8, 1 / np.sqrt(128))
+    want, tol = oracle(q, *c.values(pos + rows), pos, 8, float(np.float32(1 / np.sqrt(128))))
+    c.free()
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("rows,pos", [(1, 500), (40, 300)])
+@pytest.mark.parametrize("spread,scale", [(8.0, 1.0), (1e-3, 1.0), (1e15, 1e-31), (3.0, -0.5), (1.0, 0.0)])
+def test_attention_scores_far_apart_and_equal(hip, rows, pos, spread, scale):
+    """One weight takes all; all are equal; values near the ends of the range; a scale that turns the order round."""
+    c, q = case(hip, 8, 2, 128, rows, pos, spread)
+    got = attend(hip, c.upload(), q, pos, 8, scale)
+    want, tol = oracle(q, *c.values(pos + rows), pos, 8, float(np.float32(scale)))
+    c.free()
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 192, 256])
+@pytest.mark.parametrize("rows,pos,bad", [(1, 200, 77), (50, 20, 40), (200, 0, 100), (3, 90, 91)])
+@pytest.mark.parametrize("which", ["ks", "vs"])
+def test_attention_nan_reaches_who_sees_it(hip, hd, rows, pos, bad, which):
+    """A NaN in one key's or value's block: the queries that see the row answer NaN (all of it, or the block's values), the others what
+    they answered without it, bit for bit."""
+    c, q = case(hip, 4, 2, hd, rows, pos)
+    clean = attend(hip, c.upload(), q, pos, 4, 0.1).reshape(rows, 4, hd)
+    c.host[which][1, bad, 1] = 255
+    got = attend(hip, c.upload(), q, pos, 4, 0.1).reshape(rows, 4, hd)
+    c.free()
+    sees = pos + np.arange(rows) >= bad
+    assert np.array_equal(got[:, :2], clean[:, :2]) and np.array_equal(got[~sees], clean[~sees])
+    hit = got[sees][:, 2:]
+    if which == "ks":
+        assert np.isnan(hit).all()
+    else:
+        assert np.isnan(hit[..., 32:64]).all()
+        rest = np.delete(np.arange(hd), np.arange(32, 64))
+        assert np.array_equal(hit[..., rest], clean[sees][:, 2:][..., rest])
+
+
+def test_attention_results_do_not_depend_on_the_call(hip):
+    for rows, pos in ((1, 3000), (50, 700)):
+        c, q = case(hip, 32, 8, 128, rows, pos)
+        cache = c.upload()
+        first = attend(hip, cache, q, pos, 32, 0.1)
+        for _ in range(5):
+            assert np.array_equal(first, attend(hip, cache, q, pos, 32, 0.1))
+        c.free()
+
+
+def test_a_layer_in_4_bits(hip):
+    """A prompt and two decode steps through a layer's attention half and its feed-forward half: norms, projections, rotation, cache,
+    attention, residuals, all on the device; against the same in 64 bits on the same 4-bit weights.  The rounding of k and v to
+    4 bits turns differences of the last bit into steps where a value lies on a border, so the oracle reads the cache's bytes."""
+    lib, D, heads, kvh, hd, F, T, n_dec = hip.lib, 512, 8, 2, 64, 768, 21, 2
+    r = np.random.default_rng(3)
+    names = {"q": (heads * hd, D), "k": (kvh * hd, D), "v": (kvh * hd, D), "o": (D, heads * hd), "g": (F, D), "u": (F, D), "d": (D, F)}
+    w, dev = {}, {}
+    for i, (name, (n, k)) in enumerate(names.items()):
+        full = H.DevBuf.from_numpy(lib, (r.standard_normal((n, k)) * 0.05).astype(np.float32))
+        p = M.panels(k)
+        dev[name] = H.DevBuf(lib, n * p * 64), H.DevBuf(lib, n * p * 4)
+        assert lib.tts_hip_mx4_quantize(dev[name][0].ptr, dev[name][1].ptr, full.ptr, 0, n, k, 0) == 0
+        w[name] = M.decode(dev[name][0].to_numpy(np.uint8, (n, 64 * p)), dev[name][1].to_numpy(np.uint8, (n, 4 * p)))[:, :k]
+        full.free()
+    gain = [np.abs(r.standard_normal(D)).astype(np.float32) * 0.5 + 0.75 for _ in range(2)]
+    dgain = [H.DevBuf.from_numpy(lib, g) for g in gain]
+    c = M.Cache(hip, T + n_dec, kvh, hd)
+    cache = c.upload()
+    lin = lambda y, x, name, m: lib.tts_hip_linear_mx4(y.ptr, x.ptr, dev[name][0].ptr, dev[name][1].ptr, m, names[name][1], names[name][0])  # noqa: E731
+    size = {n: H.DevBuf(lib, 4 * T * max(F, D)) for n in "x n q k v a o g u f".split()}
+    b = size
+
+    def norm(x, g):
+        return x / np.sqrt((x * x).mean(1, keepdims=True) + 1e-5) * g
+
+    def turn(x, pos, h):
+        x = x.reshape(len(x), h, hd // 2, 2)
+        f = 1.0 / 1e6 ** (2 * np.arange(hd // 2) / hd)
+        a = (pos + np.arange(len(x)))[:, None, None] * f
+        return np.stack((x[..., 0] * np.cos(a) - x[..., 1] * np.sin(a), x[..., 0] * np.sin(a) + x[..., 1] * np.cos(a)), -1).reshape(len(x), -1)
+
+    freqs = H.DevBuf(lib, 4 * T * hd)
+    for pos, m in ((0, T), (T, 1), (T + 1, 1)):
+        x = r.standard_normal((m, D)).astype(np.float32)
+        lib.tts_hip_to_device(b["x"].ptr, x.ctypes.data, x.nbytes)
+        lib.tts_hip_rms_norm(b["n"].ptr, b["x"].ptr, dgain[0].ptr, m, D, 1e-5)
+        lib.tts_hip_compute_rope_freqs(freqs.ptr, pos, m, hd, 1e6)
+        status = [lin(b[n], b["n"], n, m) for n in "qkv"]
+        lib.tts_hip_apply_rope(b["q"].ptr, freqs.ptr, m, heads, hd)
+        lib.tts_hip_apply_rope(b["k"].ptr, freqs.ptr, m, kvh, hd)
+        status.append(lib.tts_hip_kv4_append(cache, b["k"].ptr, b["v"].ptr, m, pos, 0))
+        status.append(lib.tts_hip_kv4_attention(b["a"].ptr, b["q"].ptr, cache, m, pos, heads, 0.125))
+        status.append(lin(b["o"], b["a"], "o", m))
+        lib.tts_hip_add_inplace(b["x"].ptr, b["o"].ptr, m * D)
+        lib.tts_hip_rms_norm(b["n"].ptr, b["x"].ptr, dgain[1].ptr, m, D, 1e-5)
+        status += [lin(b["g"], b["n"], "g", m), lin(b["u"], b["n"], "u", m)]
+        lib.tts_hip_silu_mul(b["g"].ptr, b["u"].ptr, m * F)
+        status.append(lin(b["f"], b["g"], "d", m))
+        lib.tts_hip_add_inplace(b["x"].ptr, b["f"].ptr, m * D)
+        assert not any(status)
+        got = b["x"].to_numpy(np.float32, (m, D))
+        x = x.astype(np.float64)
+        y = norm(x, gain[0])
+        k = turn(y @ w["k"].T, pos, kvh)
+        held = c.download()
+        c.host = held
+        kv = c.values(pos + m)
+        # what was appended is what the projections gave, to a step of 4 bits (a half, or a whole one on a border)
+        for have, new in zip(kv, (k, y @ w["v"].T)):
+            new = new.reshape(m, kvh, hd).transpose(1, 0, 2)
+            assert np.all(np.abs(have[:, pos:pos + m] - new) <= M.block_max(new) / 4 + 1e-5)
+        a, _ = oracle(turn(y @ w["q"].T, pos, heads), *kv, pos, heads, 0.125)
+        x = x + a @ w["o"].T
+        y = norm(x, gain[1])
+        g = y @ w["g"].T
+        x = x + (g / (1 + np.exp(-g)) * (y @ w["u"].T)) @ w["d"].T
+        assert np.abs(got - x).max() <= 1e-4 * np.sqrt((x * x).mean())      # fp32 sums through eight launches of a few 2^-20 each, five times over
+    hip.check()
+    c.free()

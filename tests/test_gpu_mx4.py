@@ -1,0 +1,162 @@
+"""Quantisation to microscaled 4-bit floats, the way back and the linear layer on such weights, through the C ABI against
+numpy in 64 bits (mx4support.py)."""
+import numpy as np
+import pytest
+
+import hipsupport as H
+import mx4support as M
+import vtsupport as S
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    h = H.Hip(kv_max=8)
+    yield h
+    h.close()
+
+
+def quantize(hip, x, cols, bf16=False, shift=0):
+    """x [rows, stride] on the host; its first `cols` columns -> codes, scales and the values that come back"""
+    rows, stride = x.shape
+    item = 2 if bf16 else 4
+    src = S.f32_to_bf16_trunc(x) if bf16 else x
+    dx = H.DevBuf(hip.lib, x.size * item + 64)
+    hip.lib.tts_hip_to_device(dx.at(shift * item), np.ascontiguousarray(src).ctypes.data, x.size * item)
+    p = M.panels(cols)
+    dc, ds, dy = H.DevBuf(hip.lib, rows * p * 64), H.DevBuf(hip.lib, rows * p * 4), H.DevBuf(hip.lib, x.size * 4 + 64)
+    hip.lib.tts_hip_memset(dy.ptr, 0x55, x.size * 4 + 64)
+    assert hip.lib.tts_hip_mx4_quantize(dc.ptr, ds.ptr, dx.at(shift * item), int(bf16), rows, cols, stride) == 0
+    assert hip.lib.tts_hip_mx4_dequantize(dy.at(4 * shift), dc.ptr, ds.ptr, rows, cols, stride) == 0
+    got = dc.to_numpy(np.uint8, (rows, 64 * p)), ds.to_numpy(np.uint8, (rows, 4 * p)), dy.to_numpy(np.float32, x.size + 16)
+    hip.check()
+    for b in (dx, dc, ds, dy):
+        b.free()
+    return got
+
+
+@pytest.mark.parametrize("rows,cols,gap,shift", [(1, 1, 0, 0), (3, 31, 0, 0), (2, 33, 7, 1), (5, 127, 1, 0), (4, 128, 0, 0), (7, 129, 3, 3), (37, 1000, 24, 0),
+                                                 (300, 96, 0, 0), (9, 3072, 0, 0), (2, 20000, 8, 2), (1, 40000, 0, 0), (1000, 16, 16, 0)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_quantize(hip, rows, cols, gap, shift, bf16):
+    r = np.random.default_rng(rows * 7 + cols)
+    x = (r.standard_normal((rows, cols + gap)) * np.exp2(r.integers(-30, 30, (rows, 1)))).astype(np.float32)
+    if bf16:
+        x = S.bf16_to_f32(S.f32_to_bf16_trunc(x))
+    codes, scales, back = quantize(hip, x, cols, bf16, shift)
+    want = M.encode_matrix(x[:, :cols])
+    assert np.array_equal(scales, want[1]) and np.array_equal(codes, want[0])
+    v = M.decode(*want)[:, :cols].astype(np.float32)
+    whole = back[shift:shift + x.size].reshape(x.shape)
+    assert np.array_equal(whole[:, :cols], v)
+    untouched = np.frombuffer(b"\x55" * 4, np.float32)[0]
+    assert np.all(whole[:, cols:] == untouched) and np.all(back[:shift] == untouched) and np.all(back[shift + x.size:] == untouched)
+
+
+def test_quantize_ties_extremes_and_what_is_not_finite(hip):
+    x = np.zeros((12, 64), np.float32)
+    x[0, :11] = [6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, -0.25, -5, 7]                         # ties go to the even code
+    x[1, :6] = [7.99, 7, 5.01, 1e-30, -0.0, -7.99]                                             # beyond 6, far below half of the first step
+    x[2] = np.exp2(-149.0) * np.arange(1, 65)                                                  # subnormal: scale 2^-127
+    x[3] = np.float32(3.4028235e38) * np.linspace(-1, 1, 64).astype(np.float32)
+    x[4, 3], x[5, 40], x[6, 32], x[7, 31] = np.nan, np.inf, -np.inf, np.nan                    # one block of the two
+    x[8] = np.exp2(-126.0) * np.linspace(-2, 2, 64)
+    x[9] = np.exp2(-120.0) * np.linspace(-2, 2, 64)
+    x[10] = np.exp2(np.linspace(-140, -110, 64))
+    codes, scales, back = quantize(hip, x, 64)
+    want = M.encode_matrix(x)
+    assert np.array_equal(scales, want[1])
+    finite = np.repeat(scales != 255, 16, 1)
+    assert np.array_equal(codes[finite], want[0][finite])
+    v = M.decode(*want)[:, :64].astype(np.float32)
+    assert np.array_equal(back[:x.size].reshape(x.shape), v, equal_nan=True)
+    assert np.isnan(v[4, :32]).all() and not np.isnan(v[4, 32:]).any() and np.isnan(v[5, 32:]).all() and not np.isnan(v[5, :32]).any()
+
+
+def linear(hip, x, codes, scales, n, shift=0):
+    m, k = x.shape
+    dx = H.DevBuf(hip.lib, x.nbytes + 64)
+    hip.lib.tts_hip_to_device(dx.at(4 * shift), np.ascontiguousarray(x).ctypes.data, x.nbytes)
+    dc, ds, dy = H.DevBuf.from_numpy(hip.lib, codes), H.DevBuf.from_numpy(hip.lib, scales), H.DevBuf(hip.lib, 4 * (m * n + 64))
+    hip.lib.tts_hip_memset(dy.ptr, 0x55, 4 * (m * n + 64))
+    assert hip.lib.tts_hip_linear_mx4(dy.at(4 * shift), dx.at(4 * shift), dc.ptr, ds.ptr, m, k, n) == 0
+    y = dy.to_numpy(np.float32, m * n + 64)
+    hip.check()
+    for b in (dx, dc, ds, dy):
+        b.free()
+    untouched = np.frombuffer(b"\x55" * 4, np.float32)[0]
+    assert np.all(y[:shift] == untouched) and np.all(y[shift + m * n:] == untouched)
+    return y[shift:shift + m * n].reshape(m, n)
+
+
+def weights(n, k, seed):
+    r = np.random.default_rng(seed)
+    codes, scales = M.encode_matrix((r.standard_normal((n, k)) * 0.02 * np.exp2(r.integers(-6, 6, (n, 1)))).astype(np.float32))
+    return codes, scales, M.decode(codes, scales)[:, :k]
+
+
+def tolerance(x, w):
+    """x enters as a sum of four planes of e2m1's wider relative e2m3, each of which leaves at most 2^-4 of its block's largest
+    magnitude (half a step of the top binade over its smallest value); the accumulators of a panel of 128 are cut four or eight times
+    at 2^-23, panels and K cuts are added at 2^-24."""
+    k = x.shape[1]
+    return 2.0 ** -16 * (M.block_max(x) @ np.abs(w).T) + (2.0 ** -20 + 2.0 ** -24 * (k / 64 + 24)) * (np.abs(x).astype(np.float64) @ np.abs(w).T)
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (5, 33), (36, 3072), (257, 36), (16, 128), (300, 384), (1000, 1000), (513, 2176), (3072, 9216), (200, 12288)])
+@pytest.mark.parametrize("m", [1, 2, 4, 5, 16, 17, 33, 129])
+def test_linear(hip, m, n, k):
+    codes, scales, w = weights(n, k, n + k)
+    x = S.f32_normal((m, k), 900 + m + k)
+    y = linear(hip, x, codes, scales, n)
+    off = np.abs(y - x.astype(np.float64) @ w.T)
+    assert np.all(off <= tolerance(x, w)), float((off / tolerance(x, w)).max())
+
+
+@pytest.mark.parametrize("m,n,k", [(700, 640, 512), (1531, 300, 1000), (97, 9216, 256)])
+def test_linear_many_rows(hip, m, n, k):
+    codes, scales, w = weights(n, k, 5)
+    x = S.f32_normal((m, k), 77)
+    off = np.abs(linear(hip, x, codes, scales, n) - x.astype(np.float64) @ w.T)
+    assert np.all(off <= tolerance(x, w))
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 70])
+def test_linear_rows_that_lie_on_no_16_bytes(hip, m):
+    codes, scales, w = weights(130, 203, 6)
+    x = S.f32_normal((m, 203), 78)
+    off = np.abs(linear(hip, x, codes, scales, 130, shift=1) - x.astype(np.float64) @ w.T)
+    assert np.all(off <= tolerance(x, w))
+
+
+@pytest.mark.parametrize("m", [1, 4, 6, 40, 200])
+def test_linear_what_is_not_finite_stays_in_its_row_and_its_column(hip, m):
+    n, k = 300, 640
+    codes, scales, w = weights(n, k, 7)
+    x = S.f32_normal((m, k), 79)
+    clean = linear(hip, x, codes, scales, n)
+    x[m // 2, 333] = np.inf
+    scales[17, 6] = 255
+    y = linear(hip, x, codes, scales, n)
+    rows, cols = np.arange(m) != m // 2, np.arange(n) != 17
+    assert np.array_equal(y[rows][:, cols], clean[rows][:, cols])
+    assert not np.isfinite(y[m // 2]).any() and np.isnan(y[:, 17]).all()
+
+
+@pytest.mark.parametrize("m", [1, 7, 50])
+def test_linear_large_and_small_values(hip, m):
+    """Blocks of x across the range of floats; the smallest are held to 2^-127 times their planes' steps."""
+    n, k = 64, 512
+    codes, scales, w = weights(n, k, 8)
+    x = S.f32_normal((m, k), 80) * np.repeat(np.exp2(np.linspace(-140, 100, k // 32)), 32).astype(np.float32)
+    x[:, 64:96] = 0
+    off = np.abs(linear(hip, x, codes, scales, n) - x.astype(np.float64) @ w.T)
+    assert np.all(off <= tolerance(x, w) + 2.0 ** -127 * np.abs(w).sum(1))
+
+
+def test_linear_results_do_not_depend_on_the_call(hip):
+    codes, scales, _ = weights(512, 1024, 9)
+    for m in (1, 16, 64, 300):
+        x = S.f32_normal((m, 1024), 81)
+        assert np.array_equal(linear(hip, x, codes, scales, 512), linear(hip, x, codes, scales, 512))

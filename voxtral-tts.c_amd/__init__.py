@@ -73,6 +73,12 @@ class HipCtx(C.Structure):
                 ("ac_layers_uploaded", C.c_int)]
 
 
+class Kv4(C.Structure):
+    """tts_hip_kv4_t: one layer's key/value cache in 4 bits."""
+    _fields_ = [("k_codes", vp), ("k_scales", vp), ("v_codes", vp), ("v_scales", vp),
+                ("max_rows", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
 # name -> (restype, argtypes); every symbol include/voxtral_tts_hip.h declares
 SIGNATURES = {
     "tts_hip_init": (C.c_int, [C.c_int]),
@@ -129,6 +135,12 @@ SIGNATURES = {
     "tts_hip_default_time_inv_freq": (None, [vp, C.c_int]),
     "tts_hip_safetensors_probe": (C.c_int, [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p,
                                             C.c_void_p, C.c_void_p]),
+    "tts_hip_mx4_quantize": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "tts_hip_mx4_dequantize": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int]),
+    "tts_hip_linear_mx4": (C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int]),
+    "tts_hip_kv4_append": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int]),
+    "tts_hip_kv4_read": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int]),
+    "tts_hip_kv4_attention": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float]),
 }
 
 # every symbol include/voxtral_tts_hip_bench.h declares (csrc/libvoxtral_tts_hip_bench.so, the benchmark
