@@ -83,7 +83,11 @@ def oracle(q, k, v, pos, heads, scale):
         ds = np.where(seen, abs(scale) * (2.0 ** -20 * (M.block_max(qh) @ np.abs(kh).T) + 2.0 ** -19 * (np.abs(qh) @ np.abs(kh).T)) + 2.0 ** -22 * np.abs(np.where(seen, s, 0)), 0)
         far = np.where(seen & (p > 1e-12), m - s, 0).max(1, keepdims=True)
         e = 2 * ds.max(1, keepdims=True) + 2.0 ** -21 + 2.0 ** -23 * far + 2.0 ** -23 * (n / 32 + 40)
-        tol[:, h] = e * (p @ np.abs(vh)) + 1e-37
+        # Besides, in absolute terms: a weight goes in as fp16 planes of p 2^14, p = 1 for the largest, whose smallest step is 2^-24, and so is off by up to
+        # 2^-25 2^-14 = 2^-39 of the largest weight however small it is; the largest weight over the sum is at most 1, and n weights meet
+        # n values: 2^-39 sum |v|.  A value goes in as fp16 of v 2^13 / 2^E with 2^E at most a quarter of the largest value: off by up to 2^-25 2^-13 / 4 =
+        # 2^-40 of that, weights adding up to 1.
+        tol[:, h] = e * (p @ np.abs(vh)) + 2.0 ** -39 * (seen @ np.abs(vh)) + 2.0 ** -40 * np.abs(vh).max() + 1e-37
     return out.reshape(rows, -1), tol.reshape(rows, -1)
 
 

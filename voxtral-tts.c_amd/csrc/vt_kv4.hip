@@ -90,43 +90,328 @@ extern "C" int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cac
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
 
-/* ---- attention ------------------------------------------------------------------------------------------------------- */
+/* ---- attention -------------------------------------------------------------------------------------------------------
+ * The queries of the heads that share a kv head are columns: column c is query c / group, head c % group of the group.  Scores are
+ * S^T[row][column] = K Q^T on the scaled matrix instruction, keys in 4 bits as they lie, queries as five e2m3 planes (vt_mx4.h), the
+ * smallest plane first: the accumulators are cut and not rounded at 2^-23, and so only the last sum meets that.  Results are
+ * O^T[value][column] = V^T P^T in fp16: 4-bit values are exact in fp16 once they are scaled by the largest scale E of the rows at hand,
+ * to 2^13 of it (what is 2^37 times smaller becomes zero), and a weight p 2^14 goes in as two planes of 22 bits in all.  Maximum, sum and
+ * results of a column are fp32, one pass over the rows with the running maximum.  A lane holds the same column of S^T and of O^T, and
+ * the order of keys inside an instruction is free, so that weights go from one product to the next in their registers.
+ * NaN: a key's shows in the scores of who sees it.  A value's scale of 255 is taken for a finite one in the product (a hidden row's weight
+ * is 0, and 0 times NaN would reach who does not see it), and behind the last row NaN goes to the columns that see such a row. */
+typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
+#define KV4_PLANES 5
+#define KV4_P_EXP 14                       /* weights times 2^14 .. */
+#define KV4_V_EXP 13                       /* .. and values up to 6 times 2^13 are fp16 */
+#define KV4_COLS 16
+#define KV4_WAVES 4
+#define KV4_MAX_CHUNKS 64
 
-/* A workgroup per head and query; its waves stride over the rows, a lane owns the values lane, lane + 64, ... of a row. */
-__global__ void __launch_bounds__(256) vt_kv4_attention_kernel(float *out, const float *Q, tts_hip_kv4_t c, int start_pos, int n_heads, float scale) {
-    __shared__ float part[4][2 + 256];
-    const int h = (int)blockIdx.x, i = (int)blockIdx.y, hd = c.head_dim, per = hd / 64, lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const int kvh = h / (n_heads / c.n_kv_heads);
-    const float *q = Q + ((size_t)i * n_heads + h) * hd;
-    float qv[4], o[4], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < 4; e++) { qv[e] = e < per ? q[lane + 64 * e] : 0.f; o[e] = 0.f; }
-    auto value = [&](const uint8_t *codes, const uint8_t *scales, size_t row, int d) {
-        const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((unsigned)codes[(row * hd + d) >> 1], vt_mx4_scale(scales[(row * hd + d) >> 5]), 0);
-        return d & 1 ? p.y : p.x;
-    };
-    for (int j = wave; j <= start_pos + i; j += 4) {
-        const size_t row = (size_t)kvh * c.max_rows + j;
-        float s = 0.f;
-        for (int e = 0; e < per; e++) s = fmaf(qv[e], value(c.k_codes, c.k_scales, row, lane + 64 * e), s);
-        s = vt_wave_sum(s) * scale;
-        const float mn = fmaxf(m, s), old = m == -INFINITY ? 0.f : expf(m - mn), p = expf(s - mn);
-        l = fmaf(l, old, p);
-        for (int e = 0; e < per; e++) o[e] = fmaf(o[e], old, p * value(c.v_codes, c.v_scales, row, lane + 64 * e));
-        m = mn;
+struct kv4_job {
+    float *out;
+    const float *Q;
+    int seq, start, n_heads, cols, per_wave, chunks;     /* columns; tiles of 32 rows per wave; workgroups per head and tile of columns */
+    vt_divisor group;
+    float scale;                                         /* times log2 e */
+    float *part;
+    unsigned *cnt;
+};
+
+/* largest scale byte below 255 of four, and whether one is 255 */
+static __device__ __forceinline__ void kv4_scan4(unsigned w, unsigned &most, unsigned &nan) {
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        const unsigned s = (w >> (8 * b)) & 255u;
+        nan |= s == 255u;
+        most = max(most, s == 255u ? 0u : s);
     }
-    if (lane == 0) { part[wave][0] = m; part[wave][1] = l; }
-    for (int e = 0; e < per; e++) part[wave][2 + lane + 64 * e] = o[e];
-    __syncthreads();
-    for (int d = (int)threadIdx.x; d < hd; d += 256) {
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int w = 0; w < 4; w++) M = fmaxf(M, part[w][0]);
-        for (int w = 0; w < 4; w++) {
-            if (part[w][0] == -INFINITY && part[w][1] == 0.f) continue;
-            const float e = expf(part[w][0] - M);
-            L = fmaf(part[w][1], e, L);
-            O = fmaf(part[w][2 + d], e, O);
+}
+
+/* Few columns: a wave streams 32 rows of K and V at a time into LDS of its own, two such tiles on their way while one is multiplied,
+ * and waits for nobody else; the waves of a workgroup, and then the workgroups of a head, add their parts in a fixed order, the last workgroup
+ * to arrive those of all.  K is the A operand of 16 x 16 x 128, V of 16 x 16 x 32: lane l has the values of column n = l % 16, CD of each
+ * 16 CD, for the eight keys that its group of 16 lanes has weights of. */
+template <int HP>
+__global__ void __launch_bounds__(256, HP <= 2 ? 2 : 1) vt_kv4_stream_kernel(tts_hip_kv4_t c, kv4_job a) {
+    constexpr int HD = 64 * HP, ROW = 32 * HP, KS = (HP + 1) / 2, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4;
+    constexpr int SC = 32 * ROW * 2, STAGE = SC + 512;    /* K rows, V rows, their scales in 256 bytes each */
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[KV4_WAVES * STAGE], buf1[KV4_WAVES * STAGE], buf2[KV4_WAVES * STAGE];
+    __shared__ float ml[KV4_WAVES][KV4_COLS][2], wt[KV4_COLS][KV4_MAX_CHUNKS];
+    __shared__ int last;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int ct = (int)blockIdx.x / a.chunks, chunk = (int)blockIdx.x - ct * a.chunks, h = (int)blockIdx.y;
+    const int c0 = ct * KV4_COLS, nc = min(KV4_COLS, a.cols - c0);
+    const int seen_first = a.start + vt_div(c0, a.group) + 1, seen_last = a.start + vt_div(c0 + nc - 1, a.group) + 1;
+    const int lo = (chunk * KV4_WAVES + wave) * a.per_wave * 32, hi = min(lo + a.per_wave * 32, seen_last), tiles = lo < hi ? (hi - lo + 31) / 32 : 0;
+    const size_t row0 = (size_t)h * c.max_rows + lo;
+    const int rows = max(hi - lo, 0);
+    /* scales come in words; where a row has 2 or 6 bytes of them (HP odd) its first may start in the middle of one, whose other half is
+     * memory that a word of the cache's reaches anyway */
+    const int sub = HP % 2 ? (int)((uintptr_t)(c.v_scales + row0 * 2 * HP) & 3) : 0;
+    /* a stage's requests: unit u of 16 bytes is row u / 2 HP, piece u % 2 HP of it; K's pieces are exchanged so that eight rows' same piece lie in
+     * different banks */
+    const auto swizzle = [](int row, int piece) { return HP == 2 ? piece ^ ((row >> 1) & 3) : HP == 4 ? piece ^ (row & 7) : piece ^ ((row >> 2) & 1); };
+    int k_at[4];                                          /* HP of them (with that size the host pass drops the kernel) */
+#pragma unroll
+    for (int d = 0; d < HP; d++) {
+        const int u = d * 64 + lane, r = u / (2 * HP);
+        k_at[d] = r * ROW + swizzle(r, u - r * 2 * HP) * 16;
+    }
+    auto ask = [&](unsigned char *buf, int t) __attribute__((always_inline)) {
+        const int left = t < tiles ? rows - 32 * t : 0;                       /* none past the last tile: zeros, which nobody reads */
+        const size_t r = row0 + (t < tiles ? 32 * (size_t)t : 0);
+        const __amdgpu_buffer_rsrc_t kd = vt_buffer(c.k_codes + r * ROW, min(left, 32) * ROW), vd = vt_buffer(c.v_codes + r * ROW, min(left, 32) * ROW);
+        const int words = left > 0 ? (min(left, 32) * 2 * HP + sub + 3) & ~3 : 0;
+        const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + r * 2 * HP - sub, words), vsd = vt_buffer(c.v_scales + r * 2 * HP - sub, words);
+        unsigned char *b = buf + wave * STAGE;
+#define LDS(at) (__attribute__((address_space(3))) void *)(b + (at))
+#pragma unroll
+        for (int d = 0; d < HP; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(kd, LDS(d * 1024), 16, k_at[d], 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < HP; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(vd, LDS(32 * ROW + d * 1024), 16, d * 1024 + lane * 16, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ksd, LDS(SC), 4, lane * 4, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vsd, LDS(SC + 256), 4, lane * 4, 0, 0, 0);
+#undef LDS
+    };
+    ask(buf0, 0);
+    ask(buf1, 1);
+    /* largest scale of the wave's values, from 16 bytes a lane at a time */
+    unsigned most = 0, nan = 0;
+    {
+        const uint8_t *vs = c.v_scales + row0 * 2 * HP;
+        const int bytes = rows * 2 * HP;
+        int i = lane * 16;
+        if (((uintptr_t)vs & 3) == 0)
+            for (; i < (bytes & ~15); i += 1024) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) kv4_scan4(reinterpret_cast<const unsigned *>(vs + i)[e], most, nan);
+            }
+        /* the rest, or all of it where rows of two bytes start between words */
+        for (i = (((uintptr_t)vs & 3) == 0 ? bytes & ~15 : 0) + lane; i < bytes; i += 64) kv4_scan4(vs[i], most, nan);
+    }
+    /* queries: lane's column, values 32 g .. of each 128 */
+    const int cc = c0 + n, qi = vt_div(min(cc, a.cols - 1), a.group), see = a.start + qi + 1;
+    vt_u32x6 q[KS][KV4_PLANES];
+    unsigned qs[KS][KV4_PLANES];
+    {
+        const float *src = a.Q + ((size_t)qi * a.n_heads + (size_t)h * a.group.d + (min(cc, a.cols - 1) - qi * a.group.d)) * HD;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            vt_f32x16 even, odd;
+            const bool there = cc < a.cols && 128 * ks + 32 * g < HD;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const f32x4 v = there ? *reinterpret_cast<const f32x4 *>(src + 128 * ks + 32 * g + 4 * i) : f32x4{0.f, 0.f, 0.f, 0.f};
+                even[2 * i] = v.x; odd[2 * i] = v.y; even[2 * i + 1] = v.z; odd[2 * i + 1] = v.w;
+            }
+            vt_mx4_planes<KV4_PLANES>(even, odd, q[ks], qs[ks]);
         }
-        out[((size_t)i * n_heads + h) * hd + d] = O / L;
+    }
+#pragma unroll
+    for (int w = 32; w > 0; w /= 2) {
+        most = max(most, (unsigned)__shfl_xor((int)most, w));
+        nan |= (unsigned)__shfl_xor((int)nan, w);
+    }
+    const int shift = 127 + KV4_V_EXP - (int)most;
+    float m = -3.402823466e38f, l = 0.f;                  /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
+    f32x4 o[CHUNKS * CD];
+#pragma unroll
+    for (int i = 0; i < CHUNKS * CD; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto tile = [&](const unsigned char *buf, int t) __attribute__((always_inline)) {
+        const unsigned char *b = buf + wave * STAGE;
+        f32x4 s[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+            const int row = 16 * kt + n;
+            u32x4 k[KS];
+            int ksc[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const bool half = HP % 2 && ks == KS - 1;        /* 64 values behind the last 128: the other two groups of lanes have zeros */
+                const int p = 4 * ks + (half ? g & 1 : g);
+                k[ks] = *reinterpret_cast<const u32x4 *>(b + row * ROW + swizzle(row, p) * 16);
+                ksc[ks] = b[SC + sub + row * 2 * HP + p];
+                if (half && g >= 2) { k[ks] = u32x4{0u, 0u, 0u, 0u}; ksc[ks] = 0; }
+            }
+            s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = KV4_PLANES - 1; p >= 0; p--)
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+                    s[kt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vt_mfma_e2m1(k[ks]), vt_mfma_e2m3(q[ks][p]), s[kt], VT_MFMA_E2M1, VT_MFMA_E2M3, 0,
+                                                                            ksc[ks], 0, (int)qs[ks][p]);
+        }
+        const int first = lo + 32 * t;
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) s[kt][v] *= a.scale;
+        if (first + 32 > seen_first) {
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) s[kt][v] = first + 16 * kt + 4 * g + v < see ? s[kt][v] : -INFINITY;
+        }
+#pragma unroll
+        for (int v = 0; v < 4; v++) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
+        top = fmaxf(vt_rows_max(top), m);
+        if (__any(top != m)) {
+            const float less = __builtin_amdgcn_exp2f(m - top);
+            l *= less;
+#pragma unroll
+            for (int i = 0; i < CHUNKS * CD; i++) o[i] = o[i] * less;
+            m = top;
+        }
+        u32x4 hi4, lo4;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float p0 = __builtin_amdgcn_exp2f(s[e >> 1][2 * (e & 1)] - m + (float)KV4_P_EXP), p1 = __builtin_amdgcn_exp2f(s[e >> 1][2 * (e & 1) + 1] - m + (float)KV4_P_EXP);
+            l += p0 + p1;
+            const vt_f16x2 hi2 = __builtin_convertvector((f32x2{p0, p1}), vt_f16x2);
+            hi4[e] = __builtin_bit_cast(unsigned, hi2);
+            lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{__fsub_rn(p0, (float)hi2.x), __fsub_rn(p1, (float)hi2.y)}), vt_f16x2));
+        }
+        const vt_f16x8 ph = __builtin_bit_cast(vt_f16x8, hi4), pl = __builtin_bit_cast(vt_f16x8, lo4);
+#pragma unroll
+        for (int ch = 0; ch < CHUNKS; ch++) {
+            unsigned two[8][CD / 2];                           /* key j's values 2 i, 2 i + 1 */
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int row = (j >> 2) * 16 + 4 * g + (j & 3);
+                const unsigned char *at = b + 32 * ROW + row * ROW + ch * 8 * CD + n * (CD / 2);
+                const unsigned w = CD == 8 ? *reinterpret_cast<const unsigned *>(at) : (unsigned)*reinterpret_cast<const uint16_t *>(at);
+                const int sb = b[SC + 256 + sub + row * 2 * HP + (16 * CD * ch + CD * n) / 32];
+                const float f = vt_mx4_scale((unsigned)min(max(sb + shift, 64), 127 + KV4_V_EXP));
+                two[j][0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 0));
+                two[j][1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 1));
+                if constexpr (CD == 8) {
+                    two[j][2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 2));
+                    two[j][3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 3));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < CD; i++) {
+                u32x4 v4;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v4[e] = __builtin_amdgcn_perm(two[2 * e + 1][i / 2], two[2 * e][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                const vt_f16x8 v = __builtin_bit_cast(vt_f16x8, v4);
+                f32x4 &acc = o[ch * CD + i];
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc, 0, 0, 0);
+            }
+        }
+    };
+    auto item = [&](int t, const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0f70 | (2 * HP + 2));       /* vmcnt: the next tile may be on its way */
+        asm volatile("" ::: "memory");
+        ask(later, t + 2);
+        asm volatile("" ::: "memory");
+        tile(here, t);
+    };
+    for (int t = 0; t < tiles; t += 3) {
+        item(t, buf0, buf2);
+        if (t + 1 >= tiles) break;
+        item(t + 1, buf1, buf0);
+        if (t + 2 >= tiles) break;
+        item(t + 2, buf2, buf1);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                          /* nothing arrives in the buffers any more */
+    l = vt_rows_sum(l);
+    if (nan) {
+        /* rare: the first row of the wave's with a NaN in a block of 32 values reaches the columns that see it */
+#pragma unroll 1
+        for (int blk = 0; blk < 2 * HP; blk++) {
+            int at = 0x7fffffff;
+            for (int r = lane; r < rows; r += 64)
+                if (c.v_scales[(row0 + r) * 2 * HP + blk] == 255) { at = lo + r; break; }
+#pragma unroll
+            for (int w = 32; w > 0; w /= 2) at = min(at, __shfl_xor(at, w));
+#pragma unroll
+            for (int ch = 0; ch < CHUNKS; ch++)
+#pragma unroll
+                for (int i = 0; i < CD; i++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+                        if ((16 * CD * ch + CD * (4 * g + v)) / 32 == blk && see > at) o[ch * CD + i][v] = NAN;
+        }
+    }
+    /* the wave's part: weighted mean of its rows' values, largest score, sum of weights.  (A mean: sums of values near the end of the range
+     * would leave it.) */
+    const auto area = [&](int w, int col) { return reinterpret_cast<float *>((col < 8 ? buf0 : buf1) + w * STAGE) + (col & 7) * OD; };
+    {
+        const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+        float *to = area(wave, n);
+#pragma unroll
+        for (int ch = 0; ch < CHUNKS; ch++)
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+#pragma unroll
+                for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * (4 * g + v) + i] = __builtin_amdgcn_ldexpf(o[ch * CD + i][v] * inv, -shift);
+        if (g == 0) { ml[wave][n][0] = m; ml[wave][n][1] = l; }
+    }
+    __syncthreads();
+    const int per = a.chunks, head0 = h * a.group.d;
+    float *part = a.part + ((size_t)(h * (gridDim.x / a.chunks) + ct) * per) * KV4_COLS * (HD + 4);
+    auto store = [&](int col, int d, float v) {
+        const int k = c0 + col, i = vt_div(k, a.group);
+        a.out[((size_t)i * a.n_heads + head0 + (k - i * a.group.d)) * HD + d] = v;
+    };
+    for (int e = (int)threadIdx.x; e < nc * HD; e += 256) {
+        const int col = e / HD, d = e - col * HD;
+        float M = ml[0][col][0], L = 0.f, v = 0.f, w[KV4_WAVES];
+#pragma unroll
+        for (int k = 1; k < KV4_WAVES; k++) M = fmaxf(M, ml[k][col][0]);
+#pragma unroll
+        for (int k = 0; k < KV4_WAVES; k++) { w[k] = ml[k][col][1] * __builtin_amdgcn_exp2f(ml[k][col][0] - M); L += w[k]; }
+        const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
+#pragma unroll
+        for (int k = 0; k < KV4_WAVES; k++) v = fmaf(area(k, col)[d], w[k] * inv, v);
+        if (per == 1) { store(col, d, v); continue; }
+        float *to = part + ((size_t)chunk * KV4_COLS + col) * (HD + 4);
+        vt_stc(to + 4 + d, v);
+        if (d == 0) { vt_stc(to, M); vt_stc(to + 1, L); }
+    }
+    if (per == 1) return;
+    __builtin_amdgcn_s_waitcnt(0x0f70);                          /* the part's stores are acknowledged */
+    __syncthreads();
+    unsigned *cnt = a.cnt + h * (gridDim.x / a.chunks) + ct;
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(per - 1);
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) vt_stc_u32(cnt, 0u);                   /* ready for the next launch */
+    for (int e = (int)threadIdx.x; e < nc * per; e += 256) {
+        const int col = e / per, k = e - col * per;
+        const float *from = part + ((size_t)k * KV4_COLS + col) * (HD + 4);
+        const float pm = vt_ldc(from), pl = vt_ldc(from + 1);
+        wt[col][k] = pm;
+        area(0, 0)[col * KV4_MAX_CHUNKS + k] = pl;               /* 16 x 64 floats: the waves' parts have been read */
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < nc) {
+        const int col = (int)threadIdx.x;
+        float M = wt[col][0], L = 0.f;
+        for (int k = 1; k < per; k++) M = fmaxf(M, wt[col][k]);
+        for (int k = 0; k < per; k++) { const float w = area(0, 0)[col * KV4_MAX_CHUNKS + k] * __builtin_amdgcn_exp2f(wt[col][k] - M); wt[col][k] = w; L += w; }
+        const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
+        for (int k = 0; k < per; k++) wt[col][k] *= inv;
+    }
+    __syncthreads();
+    for (int e = (int)threadIdx.x; e < nc * HD; e += 256) {
+        const int col = e / HD, d = e - col * HD;
+        const float *from = part + (size_t)col * (HD + 4) + 4 + d;
+        float v = 0.f;
+        for (int k0 = 0; k0 < per; k0 += 8) {
+            float p[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) p[k] = vt_ldc(from + (size_t)min(k0 + k, per - 1) * KV4_COLS * (HD + 4));
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k0 + k < per) v = fmaf(p[k], wt[col][k0 + k], v);
+        }
+        store(col, d, v);
     }
 }
 
@@ -136,7 +421,26 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
     if (seq_len < 1 || start_pos < 0) { vt_set_error("%s: %d queries behind %d rows", who, seq_len, start_pos); return -1; }
     if (!cache_ok(who, cache, 0, (long long)start_pos + seq_len)) return -1;
     if (n_heads < 1 || n_heads % cache->n_kv_heads) { vt_set_error("%s: %d heads on %d kv heads", who, n_heads, cache->n_kv_heads); return -1; }
+    const int group = n_heads / cache->n_kv_heads, HP = cache->head_dim / 64;
+    const long long cols = (long long)seq_len * group;
+    if (cols > 1 << 28 || cache->n_kv_heads > 65535 || (long long)start_pos + seq_len > 1 << 28) { vt_set_error("%s: %d queries of %d heads on %d behind %d rows are too many for one call", who, seq_len, n_heads, cache->n_kv_heads, start_pos); return -1; }
     if (!vt_mx4_ready(who)) return -1;
-    hipLaunchKernelGGL(vt_kv4_attention_kernel, dim3(n_heads, seq_len), dim3(256), 0, g_vt.stream, d_out, d_Q, *cache, start_pos, n_heads, scale);
+    kv4_job a = {d_out, d_Q, seq_len, start_pos, n_heads, (int)cols, 0, 1, vt_divisor_of(group, cols), scale * 1.44269504f, NULL, g_vt.d_kv4_cnt};
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
+    const long long cts = (cols + KV4_COLS - 1) / KV4_COLS, heads = cache->n_kv_heads, tiles = ((long long)start_pos + seq_len + 31) / 32;
+    long long chunks = (2 * n_cu + cts * heads - 1) / (cts * heads);
+    if (chunks > KV4_MAX_CHUNKS) chunks = KV4_MAX_CHUNKS;
+    if (chunks > (tiles + KV4_WAVES - 1) / KV4_WAVES) chunks = (tiles + KV4_WAVES - 1) / KV4_WAVES;
+    if (cts * heads > VT_KV4_COUNTERS) chunks = 1;
+    a.per_wave = (int)((tiles + chunks * KV4_WAVES - 1) / (chunks * KV4_WAVES));
+    a.chunks = (int)((tiles + (long long)a.per_wave * KV4_WAVES - 1) / ((long long)a.per_wave * KV4_WAVES));
+    if (a.chunks > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)cts * heads * a.chunks * KV4_COLS * (cache->head_dim + 4)))) return -1;
+    const dim3 grid((unsigned)(cts * a.chunks), (unsigned)heads);
+    switch (HP) {
+    case 1: hipLaunchKernelGGL(vt_kv4_stream_kernel<1>, grid, dim3(256), 0, g_vt.stream, *cache, a); break;
+    case 2: hipLaunchKernelGGL(vt_kv4_stream_kernel<2>, grid, dim3(256), 0, g_vt.stream, *cache, a); break;
+    case 3: hipLaunchKernelGGL(vt_kv4_stream_kernel<3>, grid, dim3(256), 0, g_vt.stream, *cache, a); break;
+    default: hipLaunchKernelGGL(vt_kv4_stream_kernel<4>, grid, dim3(256), 0, g_vt.stream, *cache, a); break;
+    }
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }

@@ -85,4 +85,44 @@ __device__ __forceinline__ void vt_mx4_store8(float *p, int n, bool whole, const
     }
 }
 
+/* ---- fp32 operands of the scaled matrix instructions --------------------------------------------------------------
+ * v_mfma_scale_f32_*_f8f6f4 multiplies blocks of 32 values with a scale each: the 4-bit operand goes in as it lies in memory, and
+ * fp32 values as a sum of NP planes of e2m3 (six bits: 0 .. 2 in steps of 1/8, 2 .. 4 of 1/4, 4 .. 7.5 of 1/2): plane 0 is the nearest
+ * e2m3 of the block, every next one that of what is left, each with a scale of its own that puts the largest magnitude at 3.875 .. 7.75 of
+ * it.  A plane leaves at most 2^-4 of that magnitude, and on values ~N(0, 1) four planes leave 5.2e-7 of their norm, five 9e-9 (three
+ * 2e-5; with scales a fixed ratio apart four leave 1.0e-6).  Subtracting what a plane holds is exact.  With an infinity or a NaN
+ * in it a block's scales say NaN. */
+typedef float vt_f32x16 __attribute__((ext_vector_type(16)));
+typedef float vt_f32x32 __attribute__((ext_vector_type(32)));
+typedef unsigned vt_u32x6 __attribute__((ext_vector_type(6)));
+typedef int vt_i32x8 __attribute__((ext_vector_type(8)));
+#define VT_MFMA_E2M1 4                    /* formats of an operand, as the instruction numbers them */
+#define VT_MFMA_E2M3 2
+
+/* even[i], odd[i]: values 2 i and 2 i + 1 of the block */
+template <int NP>
+__device__ __forceinline__ void vt_mx4_planes(vt_f32x16 even, vt_f32x16 odd, vt_u32x6 (&q)[NP], unsigned (&s)[NP]) {
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) t = __builtin_elementwise_maximum(__builtin_elementwise_maximum(t, fabsf(even[i])), fabsf(odd[i]));
+        const unsigned top = __float_as_uint(t);
+        s[p] = top >= 0x7f800000u ? 255u : (unsigned)max((int)((top + 0x80000u) >> 23) - 2, 0);
+        const float f = vt_mx4_scale(s[p]);
+        q[p] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, f);
+        if (p + 1 < NP) {
+            const vt_f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q[p], f);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                even[i] = __fsub_rn(even[i], held[2 * i]);
+                odd[i] = __fsub_rn(odd[i], held[2 * i + 1]);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ vt_i32x8 vt_mfma_e2m1(const u32x4 &v) { return __builtin_bit_cast(vt_i32x8, __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1)); }
+__device__ __forceinline__ vt_i32x8 vt_mfma_e2m3(const vt_u32x6 &v) { return __builtin_bit_cast(vt_i32x8, __builtin_shufflevector(v, v, 0, 1, 2, 3, 4, 5, -1, -1)); }
+
 #endif /* VT_MX4_H */
