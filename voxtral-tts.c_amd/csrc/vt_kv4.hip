@@ -9,8 +9,6 @@
 
 #include <math.h>
 
-int vt_mx4_ready(const char *who);
-
 static int cache_ok(const char *who, const tts_hip_kv4_t *c, long long first, long long n) {
     if (!c || !c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales) { vt_set_error("%s: no cache, or a NULL pointer in it", who); return 0; }
     if (c->max_rows < 1 || c->n_kv_heads < 1 || c->head_dim < 64 || c->head_dim > 256 || c->head_dim % 64) {

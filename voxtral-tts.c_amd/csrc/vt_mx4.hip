@@ -4,8 +4,11 @@
  * cols / 128 rounded up: panels of 128 columns, 64 bytes of codes and a dword of four scales each, zeros behind the last column.
  */
 #include "vt_state.h"
+#include "vt_gemm.h"
 #include "vt_mx4.h"
 #include "vt_requests.h"
+
+#include <math.h>
 
 static int panels_of(int cols) { return cols / 128 + (cols % 128 != 0); }
 
@@ -110,43 +113,326 @@ extern "C" int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const 
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
 
-/* ---- linear layer ------------------------------------------------------------------------------------------------ */
+/* ---- linear layer: up to four rows ------------------------------------------------------------------------------------
+ * y^T[weight row][column] on v_mfma_scale_f32_16x16x128_f8f6f4: 16 weight rows go in as they lie in memory, and a row of x as four columns, its
+ * four e2m3 planes (vt_mx4.h), so that four rows of x fill an instruction and nothing is decoded.  Every workgroup splits x itself, while its
+ * first weights are on their way.  Its waves share K, a wave's weights come in parts of 16 rows x 2 panels (lines of 128 bytes) straight into
+ * LDS of its own, three parts ahead of the one that is multiplied, and it waits for nothing but its own loads; the waves' sums of 16 rows meet in LDS behind a
+ * bare barrier.  A panel's products start from zero and are added to the sum by the vector unit, which rounds; the matrix unit cuts at 2^-23. */
+#define MXR_ROWS 4
+#define MXR_WAVES 4
+#define MXR_PLANES 4
+#define MXR_PART (16 * 128 + 256)          /* codes, then 16 x 2 words of scales and as much room */
 
-/* A wave per weight row and four rows of x, which share the decoded weights. */
-#define MXL_ROWS 4
-__global__ void __launch_bounds__(256)
-vt_mx4_linear_kernel(float *y, const float *x, const unsigned *codes, const uint8_t *scales, int seq_len, int in_dim, int out_dim, int units, int whole) {
-    const int o = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-    if (o >= out_dim) return;
-    for (int s0 = 0; s0 < seq_len; s0 += MXL_ROWS) {
-        float acc[MXL_ROWS] = {};
-        for (int u = lane; u < units && 8 * u < in_dim; u += 64) {
-            const size_t at = (size_t)o * units + u;
-            f32x4 wa, wb;
-            vt_mx4_decode8(codes[at], scales[at >> 2], wa, wb);
+struct mxr_job { float *y; const float *x; const uint8_t *codes, *scales; int seq_len, in_dim, out_dim, panels, per_wave, rows_per_wg, whole; vt_divisor blocks; };
+
+__global__ void __launch_bounds__(256) vt_mx4_rows_kernel(mxr_job a) {
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[MXR_WAVES * MXR_PART], buf1[MXR_WAVES * MXR_PART], buf2[MXR_WAVES * MXR_PART], buf3[MXR_WAVES * MXR_PART];
+    __shared__ float red[2][MXR_WAVES][16 * MXR_ROWS];
+    extern __shared__ __attribute__((aligned(16))) unsigned char planes[];
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int row0 = (int)blockIdx.x * a.rows_per_wg, rows = min(a.rows_per_wg, a.out_dim - row0);
+    const int p0 = min(wave * a.per_wave, a.panels), p1 = min(p0 + a.per_wave, a.panels), parts = (a.per_wave + 1) / 2, blocks = (rows + 15) / 16, total = blocks * parts;
+    /* codes: lane i brings piece i % 8 of a line, exchanged so that eight rows' same piece lie in different banks; scales: word i % 2 of row i / 2 */
+    int w_at[2];
 #pragma unroll
-            for (int s = 0; s < MXL_ROWS; s++) {
-                if (s0 + s >= seq_len) break;
-                f32x4 a, b;
-                vt_mx4_load8(x + (size_t)(s0 + s) * in_dim + 8 * u, in_dim - 8 * u, whole && 8 * u + 8 <= in_dim, a, b);
+    for (int d = 0; d < 2; d++) { const int r = 8 * d + (lane >> 3); w_at[d] = r * 64 * a.panels + ((lane & 7) ^ (r & 7)) * 16; }
+    const int s_at = lane < 32 ? (lane >> 1) * 4 * a.panels + (lane & 1) * 4 : 0x7ffffff0;
+    int ask_block = 0, ask_part = 0;                      /* where the next request is: no division */
+    auto ask = [&](unsigned char *buf) __attribute__((always_inline)) {
+        const bool live = ask_block < blocks && p0 + 2 * ask_part < p1;         /* else zeros, which nobody reads */
+        const int left = live ? min(16, rows - 16 * ask_block) : 0, panel = live ? p0 + 2 * ask_part : 0;
+        const size_t r = (size_t)row0 + (live ? 16 * ask_block : 0);
+        const __amdgpu_buffer_rsrc_t wd = vt_buffer(a.codes + r * 64 * a.panels, left * 64 * a.panels), sd = vt_buffer(a.scales + r * 4 * a.panels, left * 4 * a.panels);
+        unsigned char *b = buf + wave * MXR_PART;
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[s] = fmaf(wb[i], b[i], fmaf(wa[i], a[i], acc[s]));
-            }
+        for (int d = 0; d < 2; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, (__attribute__((address_space(3))) void *)(b + d * 1024), 16, w_at[d], panel * 64, 0, 2);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, (__attribute__((address_space(3))) void *)(b + 2048), 4, s_at, panel * 4, 0, 2);
+        if (++ask_part >= parts) { ask_part = 0; ask_block++; }
+    };
+    ask(buf0);
+    ask(buf1);
+    ask(buf2);
+    /* x: block u % 4 P of row u / 4 P.  [panel][group of lanes][column] of 16 and of 8 bytes, and the scales; column 4 row + plane */
+    const int nb = 4 * a.panels, nc = 4 * a.seq_len;
+    unsigned char *lo8 = planes + (size_t)nb * nc * 16, *sc = lo8 + (size_t)nb * nc * 8;
+    for (int u = (int)threadIdx.x; u < a.seq_len * nb; u += 256) {
+        const int r = vt_div(u, a.blocks), blk = u - r * nb;
+        const float *src = a.x + (size_t)r * a.in_dim + 32 * (size_t)blk;
+        vt_f32x16 even, odd;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f32x4 v, w;
+            const int left = a.in_dim - 32 * blk - 8 * i;
+            vt_mx4_load8(src + 8 * i, left, a.whole && left >= 8, v, w);
+            even[4 * i] = v.x; odd[4 * i] = v.y; even[4 * i + 1] = v.z; odd[4 * i + 1] = v.w;
+            even[4 * i + 2] = w.x; odd[4 * i + 2] = w.y; even[4 * i + 3] = w.z; odd[4 * i + 3] = w.w;
         }
+        vt_u32x6 q[MXR_PLANES];
+        unsigned s[MXR_PLANES];
+        vt_mx4_planes<MXR_PLANES>(even, odd, q, s);
 #pragma unroll
-        for (int s = 0; s < MXL_ROWS; s++) {
-            const float v = vt_wave_sum(acc[s]);
-            if (lane == 0 && s0 + s < seq_len) y[(size_t)(s0 + s) * out_dim + o] = v;
+        for (int p = 0; p < MXR_PLANES; p++) {
+            const int at = blk * nc + 4 * r + p;
+            *reinterpret_cast<u32x4 *>(planes + (size_t)at * 16) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
+            *reinterpret_cast<u32x2 *>(lo8 + (size_t)at * 8) = u32x2{q[p][4], q[p][5]};
+            sc[at] = (unsigned char)s[p];
         }
     }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);                  /* lgkmcnt(0); weights stay on their way */
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int mine = g * nc + min(n, nc - 1);            /* columns past the last repeat it: nobody looks at their sums */
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    /* the waves' sums: element v of lane l is weight row 4 (l / 16) + v, column l % 16; the planes of a row of x are a quad of lanes */
+    auto finish = [&](int block) __attribute__((always_inline)) {
+        float *to = red[block & 1][wave];
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            float s = acc[v];
+            s += vt_dpp<0xB1>(s);
+            s += vt_dpp<0x4E>(s);
+            if ((n & 3) == 0) to[(n >> 2) * 16 + 4 * g + v] = s;
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        __builtin_amdgcn_s_barrier();                    /* the other half of red is read before a wave is through the next one */
+        asm volatile("" ::: "memory");
+        const int t = (int)threadIdx.x, s = t >> 4, r = 16 * block + (t & 15);
+        if (s < a.seq_len && r < rows) {
+            const float *from = &red[block & 1][0][t];
+            a.y[(size_t)s * a.out_dim + row0 + r] = (from[0] + from[16 * MXR_ROWS]) + (from[2 * 16 * MXR_ROWS] + from[3 * 16 * MXR_ROWS]);
+        }
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    int block = 0, part = 0;
+    auto item = [&](const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0f70 | 6);          /* vmcnt: two later parts may be on their way */
+        asm volatile("" ::: "memory");
+        ask(later);
+        asm volatile("" ::: "memory");
+        const unsigned char *b = here + wave * MXR_PART;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int panel = p0 + 2 * part + k;
+            if (panel >= p1) break;
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(b + n * 128 + ((4 * k + g) ^ (n & 7)) * 16);
+            const int ws = b[2048 + n * 8 + 4 * k + g], at = panel * 4 * nc + mine;
+            const u32x4 x4 = *reinterpret_cast<const u32x4 *>(planes + (size_t)at * 16);
+            const u32x2 x2 = *reinterpret_cast<const u32x2 *>(lo8 + (size_t)at * 8);
+            const vt_u32x6 xq = {x4.x, x4.y, x4.z, x4.w, x2.x, x2.y};
+            acc = acc + __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vt_mfma_e2m1(w), vt_mfma_e2m3(xq), (f32x4{0.f, 0.f, 0.f, 0.f}), VT_MFMA_E2M1, VT_MFMA_E2M3, 0, ws, 0, (int)sc[at]);
+        }
+        if (++part == parts) { part = 0; finish(block++); }
+    };
+    for (int t = 0; t < total; t += 4) {                 /* every wave goes through the same parts and barriers, whatever it has of them */
+        item(buf0, buf3);
+        if (t + 1 >= total) break;
+        item(buf1, buf0);
+        if (t + 2 >= total) break;
+        item(buf2, buf1);
+        if (t + 3 >= total) break;
+        item(buf3, buf2);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                  /* nothing arrives in the buffers any more */
+}
+
+#define MXR_LDS_MOST (160 * 1024)         /* of a workgroup, static and x's planes; from half of it on a CU holds one */
+#define MXR_LDS (MXR_WAVES * MXR_PART * 4 + 2 * MXR_WAVES * 16 * MXR_ROWS * 4)
+static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * panels * 4 * seq_len * 25; }
+
+/* ---- linear layer: more rows -----------------------------------------------------------------------------------------
+ * x is split into its planes first, [column tile of 32 rows][64 columns of W's K][plane] in the order of the matrix instruction's operand, 16
+ * and 8 bytes a lane, and the scales of a lane's four planes in a word.  y[row of x][weight row] then runs on v_mfma_scale_f32_32x32x64_f8f6f4,
+ * x as operand A, weights as they lie as B.  A workgroup's tile of BM weight rows and BN rows of x goes through K by panels of
+ * 128: both operands come straight into LDS, one panel ahead.  A wave has 32 rows of x and FM x 32 weight rows, so that an operand of x, the larger one
+ * (3 bytes a value), is read once for FM products.  Eight products of a panel, the smallest planes first, start from zero and are added by the
+ * vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts are added by a kernel of their own. */
+#define MXT_STEP (MXR_PLANES * 1536 + 256)               /* bytes of 32 rows x 64 columns of x */
+
+__global__ void __launch_bounds__(256) vt_mx4_planes_kernel(unsigned char *out, const float *x, int seq_len, int in_dim, int panels, int tiles, int whole) {
+    const int unit = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = (int)threadIdx.x & 63;
+    if (unit >= tiles * 2 * panels) return;
+    /* [panel][tile][half] */
+    const int panel = unit / (2 * tiles), rest = unit - panel * 2 * tiles, row = (rest >> 1) * 32 + (lane & 31), at = 128 * panel + 64 * (rest & 1) + 32 * (lane >> 5);
+    vt_f32x16 even, odd;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        f32x4 v, w;
+        const int left = row < seq_len ? in_dim - at - 8 * i : 0;
+        vt_mx4_load8(x + (size_t)row * in_dim + at + 8 * i, left, whole && left >= 8, v, w);
+        even[4 * i] = v.x; odd[4 * i] = v.y; even[4 * i + 1] = v.z; odd[4 * i + 1] = v.w;
+        even[4 * i + 2] = w.x; odd[4 * i + 2] = w.y; even[4 * i + 3] = w.z; odd[4 * i + 3] = w.w;
+    }
+    vt_u32x6 q[MXR_PLANES];
+    unsigned s[MXR_PLANES], all = 0;
+    vt_mx4_planes<MXR_PLANES>(even, odd, q, s);
+    unsigned char *to = out + (size_t)unit * MXT_STEP;
+#pragma unroll
+    for (int p = 0; p < MXR_PLANES; p++) {
+        *reinterpret_cast<u32x4 *>(to + p * 1536 + lane * 16) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
+        *reinterpret_cast<u32x2 *>(to + p * 1536 + 1024 + lane * 8) = u32x2{q[p][4], q[p][5]};
+        all |= s[p] << (8 * p);
+    }
+    *reinterpret_cast<unsigned *>(to + MXR_PLANES * 1536 + lane * 4) = all;
+}
+
+struct mxt_job { float *y; const unsigned char *planes; const uint8_t *codes, *scales; int seq_len, out_dim, panels, tiles, cuts, m_tiles; };
+
+/* FM 32 weight rows a wave, NM x NN waves */
+template <int FM, int NM, int NN>
+__global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
+    constexpr int THREADS = 64 * NM * NN, BM = 32 * FM * NM, W_BYTES = BM * 64, X_BYTES = NN * 2 * MXT_STEP;
+    constexpr int BUF = W_BYTES + BM * 4 + (X_BYTES + 1023) / 1024 * 1024;       /* a wave's request brings 1 KB */
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[BUF], buf1[BUF];         /* two arrays: reading one need not wait for what arrives in the other */
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 31, g = lane >> 5, wm = wave % NM, wn = wave / NM;
+    const int cut = (int)blockIdx.x % a.cuts, tile = (int)blockIdx.x / a.cuts, mt = tile % a.m_tiles, nt = tile / a.m_tiles;
+    const int p0 = (int)((long long)a.panels * cut / a.cuts), p1 = (int)((long long)a.panels * (cut + 1) / a.cuts);
+    const size_t row0 = (size_t)mt * BM;
+    const int rows = (int)min((long long)BM, a.out_dim - (long long)row0), t0 = nt * NN, xt = min(NN, a.tiles - t0);
+    const __amdgpu_buffer_rsrc_t wd = vt_buffer(a.codes + row0 * 64 * a.panels, rows * 64 * a.panels), sd = vt_buffer(a.scales + row0 * 4 * a.panels, rows * 4 * a.panels);
+    /* weights: unit u of 16 bytes is row u / 4, piece u % 4, exchanged so that eight rows' same piece lie in different banks */
+    constexpr int WU = W_BYTES / 16 / THREADS, XU = (X_BYTES / 16 + THREADS - 1) / THREADS;
+    static_assert(W_BYTES / 16 % THREADS == 0, "whole requests");
+    int w_at[8];                                         /* WU of them (with that size the host pass drops the kernel) */
+    static_assert(WU <= 8, "w_at");
+#pragma unroll
+    for (int i = 0; i < WU; i++) { const int u = i * THREADS + (int)threadIdx.x, r = u >> 2; w_at[i] = r * 64 * a.panels + ((u & 3) ^ ((r >> 1) & 3)) * 16; }
+    const int s_at = (int)threadIdx.x * 4 * a.panels;
+    auto ask = [&](unsigned char *b, int panel) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t xd = vt_buffer(a.planes + ((size_t)panel * a.tiles + t0) * 2 * MXT_STEP, xt * 2 * MXT_STEP);
+#define LDS(at) (__attribute__((address_space(3))) void *)(b + (at))
+#pragma unroll
+        for (int i = 0; i < WU; i++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, LDS(i * THREADS * 16 + wave * 1024), 16, w_at[i], panel * 64, 0, 0);
+        if (wave * 64 < BM) __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, LDS(W_BYTES + wave * 256), 4, s_at, panel * 4, 0, 0);
+#pragma unroll
+        for (int i = 0; i < XU; i++)
+            if ((i * THREADS + wave * 64) * 16 < X_BYTES)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xd, LDS(W_BYTES + BM * 4 + i * THREADS * 16 + wave * 1024), 16, (i * THREADS + (int)threadIdx.x) * 16, 0, 0, 0);
+#undef LDS
+    };
+    vt_f32x16 acc[FM];
+#pragma unroll
+    for (int f = 0; f < FM; f++) acc[f] = vt_f32x16{};
+    auto step = [&](int panel, const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __syncthreads();                                 /* this panel is there, and everybody is through with the one before */
+        if (panel + 1 < p1) ask(later, panel + 1);
+        u32x4 w[FM][2];
+        int ws[FM], xs[2];
+        const unsigned char *xb = here + W_BYTES + BM * 4 + wn * 2 * MXT_STEP;
+#pragma unroll
+        for (int f = 0; f < FM; f++) {
+            const int r = (wm * FM + f) * 32 + n;
+#pragma unroll
+            for (int h = 0; h < 2; h++) w[f][h] = *reinterpret_cast<const u32x4 *>(here + r * 64 + ((2 * h + g) ^ ((r >> 1) & 3)) * 16);
+            ws[f] = (int)(*reinterpret_cast<const unsigned *>(here + W_BYTES + r * 4) >> (8 * g));       /* bytes 0 and 2: the lane's block of either half */
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) xs[h] = *reinterpret_cast<const int *>(xb + h * MXT_STEP + MXR_PLANES * 1536 + lane * 4);
+        vt_f32x16 sum[FM];
+#pragma unroll
+        for (int f = 0; f < FM; f++) sum[f] = vt_f32x16{};
+#define PRODUCTS(p) \
+        _Pragma("unroll") for (int h = 0; h < 2; h++) { \
+            const u32x4 x4 = *reinterpret_cast<const u32x4 *>(xb + h * MXT_STEP + p * 1536 + lane * 16); \
+            const u32x2 x2 = *reinterpret_cast<const u32x2 *>(xb + h * MXT_STEP + p * 1536 + 1024 + lane * 8); \
+            const vt_u32x6 xq = {x4.x, x4.y, x4.z, x4.w, x2.x, x2.y}; \
+            _Pragma("unroll") for (int f = 0; f < FM; f++) \
+                sum[f] = h ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(xq), vt_mfma_e2m1(w[f][1]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, p, xs[1], 2, ws[f]) \
+                           : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(xq), vt_mfma_e2m1(w[f][0]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, p, xs[0], 0, ws[f]); \
+        }
+        PRODUCTS(3) PRODUCTS(2) PRODUCTS(1) PRODUCTS(0)
+#undef PRODUCTS
+#pragma unroll
+        for (int f = 0; f < FM; f++) acc[f] = acc[f] + sum[f];
+    };
+    ask(buf0, p0);                                       /* every cut has a panel */
+    for (int panel = p0; panel < p1; panel += 2) {
+        step(panel, buf0, buf1);
+        if (panel + 1 >= p1) break;
+        step(panel + 1, buf1, buf0);
+    }
+    /* element v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4 of x, weight row l % 32 */
+    float *y = a.y + (size_t)cut * a.seq_len * a.out_dim;
+#pragma unroll
+    for (int f = 0; f < FM; f++) {
+        const int r = (wm * FM + f) * 32 + n;
+        if (r >= rows) continue;
+#pragma unroll
+        for (int v = 0; v < 16; v++) {
+            const int s = (t0 + wn) * 32 + 8 * (v >> 2) + 4 * g + (v & 3);
+            if (s < a.seq_len) y[(size_t)s * a.out_dim + row0 + r] = acc[f][v];
+        }
+    }
+}
+
+/* Tiles: (weight rows, rows of x, workgroups that a CU holds, us per panel and workgroup when all slots are taken) */
+struct mxt_tile { int bm, bn, per_cu; float panel_us; };
+static const mxt_tile mxt_tiles[] = {{256, 128, 1, 1.25f}, {128, 64, 2, 0.75f}, {128, 32, 3, 0.60f}};
+#define MXT_MAX_CUTS 16
+
+static void mxt_plan(int n_cu, int seq_len, int out_dim, int panels, int *best_tile, int *best_cuts) {
+    double best = 1e30;
+    for (int t = 0; t < 3; t++) {
+        const mxt_tile &k = mxt_tiles[t];
+        const double tiles = (double)((out_dim + k.bm - 1) / k.bm) * ((seq_len + k.bn - 1) / k.bn);
+        for (int cuts = 1; cuts <= MXT_MAX_CUTS && cuts <= panels; cuts++) {
+            const double rounds = ceil(tiles * cuts / ((double)n_cu * k.per_cu)), us = rounds * ((panels + cuts - 1) / cuts * (double)k.panel_us + 2.0) +
+                                  (cuts > 1 ? 3.0 + (double)seq_len * out_dim * 4.0 * (2 * cuts + 1) / 4.0e6 : 0.0);
+            if (us < best) { best = us; *best_tile = t; *best_cuts = cuts; }
+        }
+    }
+}
+
+int vt_mx4_prepare(void) {
+    return vt_check(hipFuncSetAttribute((const void *)vt_mx4_rows_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MXR_LDS_MOST - MXR_LDS), "tts_hip_linear_mx4: LDS");
+}
+
+static int mx4_linear_rows(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim, int whole) {
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = panels_of(in_dim);
+    const size_t lds = mxr_planes_bytes(seq_len, panels);
+    const int wgs = n_cu * (MXR_LDS + lds > MXR_LDS_MOST / 2 ? 1 : 2), rows_per_wg = (int)(((long long)out_dim + wgs - 1) / wgs);
+    mxr_job a = {d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, panels, (panels + MXR_WAVES - 1) / MXR_WAVES, rows_per_wg, whole, vt_divisor_of(4 * panels, 16ll * panels)};
+    hipLaunchKernelGGL(vt_mx4_rows_kernel, dim3((out_dim + rows_per_wg - 1) / rows_per_wg), dim3(256), lds, g_vt.stream, a);
+    return 0;
+}
+
+static int mx4_linear_tiles(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim, int whole) {
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = panels_of(in_dim), tiles = (seq_len + 31) / 32;
+    int t = 0, cuts = 1;
+    mxt_plan(n_cu, seq_len, out_dim, panels, &t, &cuts);
+    const size_t planes = (size_t)tiles * 2 * panels * MXT_STEP, part = cuts > 1 ? sizeof(float) * (size_t)seq_len * out_dim * cuts : 0;
+    unsigned char *area = (unsigned char *)vt_scratch(planes + part);
+    if (!area) return -1;
+    hipLaunchKernelGGL(vt_mx4_planes_kernel, dim3((tiles * 2 * panels + 3) / 4), dim3(256), 0, g_vt.stream, area, d_x, seq_len, in_dim, panels, tiles, whole);
+    const int m_tiles = (out_dim + mxt_tiles[t].bm - 1) / mxt_tiles[t].bm, n_tiles = (seq_len + mxt_tiles[t].bn - 1) / mxt_tiles[t].bn;
+    const mxt_job a = {cuts > 1 ? (float *)(area + planes) : d_y, area, d_codes, d_scales, seq_len, out_dim, panels, tiles, cuts, m_tiles};
+    const long long grid = (long long)m_tiles * n_tiles * cuts;
+    if (grid > 0x7fffffffll) { vt_set_error("tts_hip_linear_mx4: %d x %d x %d is too large for one call", seq_len, out_dim, in_dim); return -1; }
+    if (t == 0) hipLaunchKernelGGL((vt_mx4_tile_kernel<4, 2, 4>), dim3((unsigned)grid), dim3(512), 0, g_vt.stream, a);
+    else if (t == 1) hipLaunchKernelGGL((vt_mx4_tile_kernel<2, 2, 2>), dim3((unsigned)grid), dim3(256), 0, g_vt.stream, a);
+    else hipLaunchKernelGGL((vt_mx4_tile_kernel<1, 4, 1>), dim3((unsigned)grid), dim3(256), 0, g_vt.stream, a);
+    if (cuts > 1) vt_launch_sum_planes(d_y, (float *)(area + planes), cuts, (size_t)seq_len * out_dim, (size_t)seq_len * out_dim);
+    return 0;
 }
 
 extern "C" int tts_hip_linear_mx4(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim) {
     static const char who[] = "tts_hip_linear_mx4";
     if (!d_y || ((uintptr_t)d_y & 3) || seq_len < 1) { vt_set_error("%s: %d rows to %p", who, seq_len, (void *)d_y); return -1; }
-    if (!mx4_shape_ok(who, d_x, d_codes, d_scales, out_dim, in_dim, in_dim, 4) || !vt_mx4_ready(who)) return -1;
+    if (!mx4_shape_ok(who, d_x, d_codes, d_scales, out_dim, in_dim, in_dim, 4)) return -1;
+    if (in_dim > 1 << 23) { vt_set_error("%s: %d columns (1 .. 2^23)", who, in_dim); return -1; }
+    if (!vt_mx4_ready(who)) return -1;
     const int whole = ((uintptr_t)d_x & 15) == 0 && in_dim % 4 == 0;
-    hipLaunchKernelGGL(vt_mx4_linear_kernel, dim3((out_dim + 3) / 4), dim3(256), 0, g_vt.stream, d_y, d_x, (const unsigned *)d_codes, d_scales, seq_len,
-                       in_dim, out_dim, 16 * panels_of(in_dim), whole);
+    if (seq_len <= MXR_ROWS && MXR_LDS + mxr_planes_bytes(seq_len, panels_of(in_dim)) <= MXR_LDS_MOST) {
+        if (mx4_linear_rows(d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, whole)) return -1;
+    } else {
+        /* so many rows at a time that the work area stays small beside the operands, and the tiles in one launch countable */
+        const int most = 1 << 14;
+        for (int s = 0; s < seq_len; s += most)
+            if (mx4_linear_tiles(d_y + (size_t)s * out_dim, d_x + (size_t)s * in_dim, d_codes, d_scales, seq_len - s < most ? seq_len - s : most, in_dim, out_dim, whole)) return -1;
+    }
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }

@@ -127,6 +127,8 @@ void vt_launch_prefill_attention(float *d_out, uint16_t *d_hi, uint16_t *d_lo, c
 /* the model's attention scale, 1/sqrt(head_dim), computed like the CPU path does (voxtral_tts_llm.c:189) */
 #define VT_ATT_SCALE (1.0f / sqrtf((float)VT_HEAD_DIM))
 void vt_codec_free(void);
+int vt_mx4_prepare(void);
+int vt_mx4_ready(const char *who);            /* a context, and its device is the current one; else an error */
 /* single launches for the library's other translation units and its benchmark companion (vt_bench.hip) */
 int vt_codec_probe_buffers(float **x, int **codes);
 void vt_codec_probe_fill(const float *x, int k);
