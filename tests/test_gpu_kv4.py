@@ -152,6 +152,21 @@ def test_attention_nan_reaches_who_sees_it(hip, hd, rows, pos, bad, which):
         assert np.array_equal(hit[..., rest], clean[sees][:, 2:][..., rest])
 
 
+@pytest.mark.parametrize("hd", [64, 128, 192, 256])
+@pytest.mark.parametrize("rows,pos", [(1, 0), (1, 32), (1, 332), (6, 1001), (70, 64)])
+def test_attention_hidden_rows_change_nothing(hip, hd, rows, pos):
+    """Behind the last row, and so in front of the next head's first: zeros, the largest scales, NaN.  The same bits."""
+    outs = []
+    for fill in (0, 254, 255):
+        c, q = case(hip, 6, 3, hd, rows, pos, extra=1 + pos % 2)
+        n = pos + rows
+        for a in c.host.values():
+            a[:, n:] = fill
+        outs.append(attend(hip, c.upload(), q, pos, 6, 0.1))
+        c.free()
+    assert np.isfinite(outs[0]).all() and np.array_equal(outs[0], outs[1]) and np.array_equal(outs[0], outs[2])
+
+
 def test_attention_results_do_not_depend_on_the_call(hip):
     for rows, pos in ((1, 3000), (50, 700)):
         c, q = case(hip, 32, 8, 128, rows, pos)

@@ -103,7 +103,6 @@ typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
 #define KV4_P_EXP 14                       /* weights times 2^14 .. */
 #define KV4_V_EXP 13                       /* .. and values up to 6 times 2^13 are fp16 */
 #define KV4_COLS 16
-#define KV4_WAVES 4
 #define KV4_MAX_CHUNKS 64
 
 struct kv4_job {
@@ -130,18 +129,18 @@ static __device__ __forceinline__ void kv4_scan4(unsigned w, unsigned &most, uns
  * and waits for nobody else; the waves of a workgroup, and then the workgroups of a head, add their parts in a fixed order, the last workgroup
  * to arrive those of all.  K is the A operand of 16 x 16 x 128, V of 16 x 16 x 32: lane l has the values of column n = l % 16, CD of each
  * 16 CD, for the eight keys that its group of 16 lanes has weights of. */
-template <int HP>
-__global__ void __launch_bounds__(256, HP <= 2 ? 2 : 1) vt_kv4_stream_kernel(tts_hip_kv4_t c, kv4_job a) {
+template <int HP, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t c, kv4_job a) {
     constexpr int HD = 64 * HP, ROW = 32 * HP, KS = (HP + 1) / 2, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4;
     constexpr int SC = 32 * ROW * 2, STAGE = SC + 512;    /* K rows, V rows, their scales in 256 bytes each */
-    __shared__ __attribute__((aligned(16))) unsigned char buf0[KV4_WAVES * STAGE], buf1[KV4_WAVES * STAGE], buf2[KV4_WAVES * STAGE];
-    __shared__ float ml[KV4_WAVES][KV4_COLS][2], wt[KV4_COLS][KV4_MAX_CHUNKS];
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[WAVES * STAGE], buf1[WAVES * STAGE], buf2[WAVES * STAGE];
+    __shared__ float ml[WAVES][KV4_COLS][2], wt[KV4_COLS][KV4_MAX_CHUNKS];
     __shared__ int last;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int ct = (int)blockIdx.x / a.chunks, chunk = (int)blockIdx.x - ct * a.chunks, h = (int)blockIdx.y;
     const int c0 = ct * KV4_COLS, nc = min(KV4_COLS, a.cols - c0);
     const int seen_first = a.start + vt_div(c0, a.group) + 1, seen_last = a.start + vt_div(c0 + nc - 1, a.group) + 1;
-    const int lo = (chunk * KV4_WAVES + wave) * a.per_wave * 32, hi = min(lo + a.per_wave * 32, seen_last), tiles = lo < hi ? (hi - lo + 31) / 32 : 0;
+    const int lo = (chunk * WAVES + wave) * a.per_wave * 32, hi = min(lo + a.per_wave * 32, seen_last), tiles = lo < hi ? (hi - lo + 31) / 32 : 0;
     const size_t row0 = (size_t)h * c.max_rows + lo;
     const int rows = max(hi - lo, 0);
     /* scales come in words; where a row has 2 or 6 bytes of them (HP odd) its first may start in the middle of one, whose other half is
@@ -160,8 +159,8 @@ __global__ void __launch_bounds__(256, HP <= 2 ? 2 : 1) vt_kv4_stream_kernel(tts
         const int left = t < tiles ? rows - 32 * t : 0;                       /* none past the last tile: zeros, which nobody reads */
         const size_t r = row0 + (t < tiles ? 32 * (size_t)t : 0);
         const __amdgpu_buffer_rsrc_t kd = vt_buffer(c.k_codes + r * ROW, min(left, 32) * ROW), vd = vt_buffer(c.v_codes + r * ROW, min(left, 32) * ROW);
-        const int words = left > 0 ? (min(left, 32) * 2 * HP + sub + 3) & ~3 : 0;
-        const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + r * 2 * HP - sub, words), vsd = vt_buffer(c.v_scales + r * 2 * HP - sub, words);
+        const int sbytes = left > 0 ? (min(left, 32) * 2 * HP + sub + 3) & ~3 : 0;
+        const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + r * 2 * HP - sub, sbytes), vsd = vt_buffer(c.v_scales + r * 2 * HP - sub, sbytes);
         unsigned char *b = buf + wave * STAGE;
 #define LDS(at) (__attribute__((address_space(3))) void *)(b + (at))
 #pragma unroll
@@ -172,39 +171,46 @@ __global__ void __launch_bounds__(256, HP <= 2 ? 2 : 1) vt_kv4_stream_kernel(tts
         __builtin_amdgcn_raw_ptr_buffer_load_lds(vsd, LDS(SC + 256), 4, lane * 4, 0, 0, 0);
 #undef LDS
     };
-    ask(buf0, 0);
-    ask(buf1, 1);
-    /* largest scale of the wave's values, from 16 bytes a lane at a time */
-    unsigned most = 0, nan = 0;
-    {
-        const uint8_t *vs = c.v_scales + row0 * 2 * HP;
-        const int bytes = rows * 2 * HP;
-        int i = lane * 16;
-        if (((uintptr_t)vs & 3) == 0)
-            for (; i < (bytes & ~15); i += 1024) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) kv4_scan4(reinterpret_cast<const unsigned *>(vs + i)[e], most, nan);
-            }
-        /* the rest, or all of it where rows of two bytes start between words */
-        for (i = (((uintptr_t)vs & 3) == 0 ? bytes & ~15 : 0) + lane; i < bytes; i += 64) kv4_scan4(vs[i], most, nan);
-    }
-    /* queries: lane's column, values 32 g .. of each 128 */
+    /* queries (lane's column, values 32 g .. of each 128) and the scales of the first 1024 / 2 HP rows' values are asked for first: loads return in
+     * order */
     const int cc = c0 + n, qi = vt_div(min(cc, a.cols - 1), a.group), see = a.start + qi + 1;
-    vt_u32x6 q[KS][KV4_PLANES];
-    unsigned qs[KS][KV4_PLANES];
+    vt_f32x16 even[KS], odd[KS];
     {
         const float *src = a.Q + ((size_t)qi * a.n_heads + (size_t)h * a.group.d + (min(cc, a.cols - 1) - qi * a.group.d)) * HD;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-            vt_f32x16 even, odd;
             const bool there = cc < a.cols && 128 * ks + 32 * g < HD;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const f32x4 v = there ? *reinterpret_cast<const f32x4 *>(src + 128 * ks + 32 * g + 4 * i) : f32x4{0.f, 0.f, 0.f, 0.f};
-                even[2 * i] = v.x; odd[2 * i] = v.y; even[2 * i + 1] = v.z; odd[2 * i + 1] = v.w;
+                even[ks][2 * i] = v.x; odd[ks][2 * i] = v.y; even[ks][2 * i + 1] = v.z; odd[ks][2 * i + 1] = v.w;
             }
-            vt_mx4_planes<KV4_PLANES>(even, odd, q[ks], qs[ks]);
         }
+    }
+    const int words = (rows * 2 * HP + sub + 3) / 4;      /* as the requests below take them; zeros behind the last */
+    const unsigned *vs = reinterpret_cast<const unsigned *>(c.v_scales + row0 * 2 * HP - sub);
+    const __amdgpu_buffer_rsrc_t vsd0 = vt_buffer(vs, words * 4);
+    u32x4 scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd0, lane * 16));
+    ask(buf0, 0);
+    ask(buf1, 1);
+    vt_u32x6 q[KS][KV4_PLANES];
+    unsigned qs[KS][KV4_PLANES];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) vt_mx4_planes<KV4_PLANES>(even[ks], odd[ks], q[ks], qs[ks]);
+    /* largest scale of the wave's values */
+    unsigned most = 0, nan = 0;
+    for (int i = lane * 4;;) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (HP % 2) {                                 /* halves of a word that are not this wave's rows */
+                if (i + e == 0 && sub) scan[e] &= 0xffff0000u;
+                if (i + e == words - 1 && ((rows * 2 * HP + sub) & 3)) scan[e] &= 0xffffu;
+            }
+            kv4_scan4(scan[e], most, nan);
+        }
+        i += 256;
+        if (i - lane * 4 >= words) break;
+        scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd0, i * 4));
     }
 #pragma unroll
     for (int w = 32; w > 0; w /= 2) {
@@ -357,16 +363,16 @@ __global__ void __launch_bounds__(256, HP <= 2 ? 2 : 1) vt_kv4_stream_kernel(tts
         const int k = c0 + col, i = vt_div(k, a.group);
         a.out[((size_t)i * a.n_heads + head0 + (k - i * a.group.d)) * HD + d] = v;
     };
-    for (int e = (int)threadIdx.x; e < nc * HD; e += 256) {
+    for (int e = (int)threadIdx.x; e < nc * HD; e += 64 * WAVES) {
         const int col = e / HD, d = e - col * HD;
-        float M = ml[0][col][0], L = 0.f, v = 0.f, w[KV4_WAVES];
+        float M = ml[0][col][0], L = 0.f, v = 0.f, w[WAVES];
 #pragma unroll
-        for (int k = 1; k < KV4_WAVES; k++) M = fmaxf(M, ml[k][col][0]);
+        for (int k = 1; k < WAVES; k++) M = fmaxf(M, ml[k][col][0]);
 #pragma unroll
-        for (int k = 0; k < KV4_WAVES; k++) { w[k] = ml[k][col][1] * __builtin_amdgcn_exp2f(ml[k][col][0] - M); L += w[k]; }
+        for (int k = 0; k < WAVES; k++) { w[k] = ml[k][col][1] * __builtin_amdgcn_exp2f(ml[k][col][0] - M); L += w[k]; }
         const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
 #pragma unroll
-        for (int k = 0; k < KV4_WAVES; k++) v = fmaf(area(k, col)[d], w[k] * inv, v);
+        for (int k = 0; k < WAVES; k++) v = fmaf(area(k, col)[d], w[k] * inv, v);
         if (per == 1) { store(col, d, v); continue; }
         float *to = part + ((size_t)chunk * KV4_COLS + col) * (HD + 4);
         vt_stc(to + 4 + d, v);
@@ -380,37 +386,49 @@ __global__ void __launch_bounds__(256, HP <= 2 ? 2 : 1) vt_kv4_stream_kernel(tts
     __syncthreads();
     if (!last) return;
     if (threadIdx.x == 0) vt_stc_u32(cnt, 0u);                   /* ready for the next launch */
-    for (int e = (int)threadIdx.x; e < nc * per; e += 256) {
-        const int col = e / per, k = e - col * per;
-        const float *from = part + ((size_t)k * KV4_COLS + col) * (HD + 4);
-        const float pm = vt_ldc(from), pl = vt_ldc(from + 1);
-        wt[col][k] = pm;
-        area(0, 0)[col * KV4_MAX_CHUNKS + k] = pl;               /* 16 x 64 floats: the waves' parts have been read */
+    /* a wave per column: lane k has part k's largest score and sum of weights */
+    const __amdgpu_buffer_rsrc_t pd = vt_buffer(part, per * KV4_COLS * (HD + 4) * 4);
+    for (int col = wave; col < nc; col += WAVES) {
+        const int at = ((min(lane, per - 1) * KV4_COLS + col) * (HD + 4)) * 4;
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(pd, at, 0, 16 /* sc1 */);
+        const float pm = __uint_as_float(v.x), pl = lane < per ? __uint_as_float(v.y) : 0.f;
+        const float w = pl * __builtin_amdgcn_exp2f(pm - vt_wave_max(pm)), L = vt_wave_sum(w);
+        wt[col][lane] = L == 0.f ? 0.f : __fdiv_rn(w, L);
     }
     __syncthreads();
-    if ((int)threadIdx.x < nc) {
-        const int col = (int)threadIdx.x;
-        float M = wt[col][0], L = 0.f;
-        for (int k = 1; k < per; k++) M = fmaxf(M, wt[col][k]);
-        for (int k = 0; k < per; k++) { const float w = area(0, 0)[col * KV4_MAX_CHUNKS + k] * __builtin_amdgcn_exp2f(wt[col][k] - M); wt[col][k] = w; L += w; }
-        const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
-        for (int k = 0; k < per; k++) wt[col][k] *= inv;
-    }
-    __syncthreads();
-    for (int e = (int)threadIdx.x; e < nc * HD; e += 256) {
-        const int col = e / HD, d = e - col * HD;
-        const float *from = part + (size_t)col * (HD + 4) + 4 + d;
-        float v = 0.f;
-        for (int k0 = 0; k0 < per; k0 += 8) {
-            float p[8];
+    for (int e = (int)threadIdx.x; e < nc * HD / 4; e += 64 * WAVES) {
+        const int col = e / (HD / 4), d = 4 * (e - col * (HD / 4)), at = (col * (HD + 4) + 4 + d) * 4;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < per; k0 += 16) {
+            u32x4 p[16];
 #pragma unroll
-            for (int k = 0; k < 8; k++) p[k] = vt_ldc(from + (size_t)min(k0 + k, per - 1) * KV4_COLS * (HD + 4));
+            for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_raw_buffer_load_b128(pd, at, min(k0 + k, per - 1) * KV4_COLS * (HD + 4) * 4, 16);
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (k0 + k < per) v = fmaf(p[k], wt[col][k0 + k], v);
+            for (int k = 0; k < 16; k++)
+                if (k0 + k < per) {
+                    const float w = wt[col][k0 + k];
+                    const f32x4 o4 = __builtin_bit_cast(f32x4, p[k]);
+                    v = f32x4{fmaf(o4.x, w, v.x), fmaf(o4.y, w, v.y), fmaf(o4.z, w, v.z), fmaf(o4.w, w, v.w)};
+                }
         }
-        store(col, d, v);
+#pragma unroll
+        for (int i = 0; i < 4; i++) store(col, d + i, v[i]);
     }
+}
+
+template <int HP, int WAVES>
+static int kv4_stream(const tts_hip_kv4_t *cache, kv4_job a) {
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
+    const long long cts = (a.cols + KV4_COLS - 1) / KV4_COLS, heads = cache->n_kv_heads, tiles = ((long long)a.start + a.seq + 31) / 32;
+    long long chunks = (8 * n_cu / WAVES + cts * heads - 1) / (cts * heads);
+    if (chunks > KV4_MAX_CHUNKS) chunks = KV4_MAX_CHUNKS;
+    if (chunks > (tiles + WAVES - 1) / WAVES) chunks = (tiles + WAVES - 1) / WAVES;
+    if (cts * heads > VT_KV4_COUNTERS) chunks = 1;
+    a.per_wave = (int)((tiles + chunks * WAVES - 1) / (chunks * WAVES));
+    a.chunks = (int)((tiles + (long long)a.per_wave * WAVES - 1) / ((long long)a.per_wave * WAVES));
+    if (a.chunks > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)cts * heads * a.chunks * KV4_COLS * (cache->head_dim + 4)))) return -1;
+    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)(cts * a.chunks), (unsigned)heads), dim3(64 * WAVES), 0, g_vt.stream, *cache, a);
+    return 0;
 }
 
 extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_hip_kv4_t *cache, int seq_len, int start_pos, int n_heads, float scale) {
@@ -424,21 +442,6 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
     if (cols > 1 << 28 || cache->n_kv_heads > 65535 || (long long)start_pos + seq_len > 1 << 28) { vt_set_error("%s: %d queries of %d heads on %d behind %d rows are too many for one call", who, seq_len, n_heads, cache->n_kv_heads, start_pos); return -1; }
     if (!vt_mx4_ready(who)) return -1;
     kv4_job a = {d_out, d_Q, seq_len, start_pos, n_heads, (int)cols, 0, 1, vt_divisor_of(group, cols), scale * 1.44269504f, NULL, g_vt.d_kv4_cnt};
-    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
-    const long long cts = (cols + KV4_COLS - 1) / KV4_COLS, heads = cache->n_kv_heads, tiles = ((long long)start_pos + seq_len + 31) / 32;
-    long long chunks = (2 * n_cu + cts * heads - 1) / (cts * heads);
-    if (chunks > KV4_MAX_CHUNKS) chunks = KV4_MAX_CHUNKS;
-    if (chunks > (tiles + KV4_WAVES - 1) / KV4_WAVES) chunks = (tiles + KV4_WAVES - 1) / KV4_WAVES;
-    if (cts * heads > VT_KV4_COUNTERS) chunks = 1;
-    a.per_wave = (int)((tiles + chunks * KV4_WAVES - 1) / (chunks * KV4_WAVES));
-    a.chunks = (int)((tiles + (long long)a.per_wave * KV4_WAVES - 1) / ((long long)a.per_wave * KV4_WAVES));
-    if (a.chunks > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)cts * heads * a.chunks * KV4_COLS * (cache->head_dim + 4)))) return -1;
-    const dim3 grid((unsigned)(cts * a.chunks), (unsigned)heads);
-    switch (HP) {
-    case 1: hipLaunchKernelGGL(vt_kv4_stream_kernel<1>, grid, dim3(256), 0, g_vt.stream, *cache, a); break;
-    case 2: hipLaunchKernelGGL(vt_kv4_stream_kernel<2>, grid, dim3(256), 0, g_vt.stream, *cache, a); break;
-    case 3: hipLaunchKernelGGL(vt_kv4_stream_kernel<3>, grid, dim3(256), 0, g_vt.stream, *cache, a); break;
-    default: hipLaunchKernelGGL(vt_kv4_stream_kernel<4>, grid, dim3(256), 0, g_vt.stream, *cache, a); break;
-    }
+    if (HP == 1 ? kv4_stream<1, 8>(cache, a) : HP == 2 ? kv4_stream<2, 8>(cache, a) : HP == 3 ? kv4_stream<3, 4>(cache, a) : kv4_stream<4, 4>(cache, a)) return -1;
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
