@@ -115,6 +115,9 @@ struct kv4_job {
     unsigned *cnt;
 };
 
+/* column / heads per kv head, for fewer than 2^20 columns: (c + 1/2) / d is no nearer to a whole number than 1 / 2 d, and c 2^-22 / d off */
+static __device__ __forceinline__ int kv4_query(int col, float inv) { return (int)(((float)col + 0.5f) * inv); }
+
 /* largest scale byte below 255 of four, and whether one is 255 */
 static __device__ __forceinline__ void kv4_scan4(unsigned w, unsigned &most, unsigned &nan) {
 #pragma unroll
@@ -128,7 +131,8 @@ static __device__ __forceinline__ void kv4_scan4(unsigned w, unsigned &most, uns
 /* Few columns: a wave streams 32 rows of K and V at a time into LDS of its own, two such tiles on their way while one is multiplied,
  * and waits for nobody else; the waves of a workgroup, and then the workgroups of a head, add their parts in a fixed order, the last workgroup
  * to arrive those of all.  K is the A operand of 16 x 16 x 128, V of 16 x 16 x 32: lane l has the values of column n = l % 16, CD of each
- * 16 CD, for the eight keys that its group of 16 lanes has weights of. */
+ * 16 CD, for the eight keys that its group of 16 lanes has weights of.  Most of a short call is instructions that run once, from a cold instruction cache: the code
+ * in front of the loop and behind it is kept short. */
 template <int HP, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t c, kv4_job a) {
     constexpr int HD = 64 * HP, ROW = 32 * HP, KS = (HP + 1) / 2, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4;
@@ -137,69 +141,71 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
     __shared__ float ml[WAVES][KV4_COLS][2], wt[KV4_COLS][KV4_MAX_CHUNKS];
     __shared__ int last;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const int ct = (int)blockIdx.x / a.chunks, chunk = (int)blockIdx.x - ct * a.chunks, h = (int)blockIdx.y;
+    const int chunk = (int)blockIdx.x, ct = (int)blockIdx.y, h = (int)blockIdx.z, group = a.group.d;
+    const float inv_group = 1.f / (float)group;
     const int c0 = ct * KV4_COLS, nc = min(KV4_COLS, a.cols - c0);
-    const int seen_first = a.start + vt_div(c0, a.group) + 1, seen_last = a.start + vt_div(c0 + nc - 1, a.group) + 1;
-    const int lo = (chunk * WAVES + wave) * a.per_wave * 32, hi = min(lo + a.per_wave * 32, seen_last), tiles = lo < hi ? (hi - lo + 31) / 32 : 0;
+    /* queries (lane's column, values 32 g .. of each 128) are asked for first: loads return in order.  Columns past the last repeat it; the
+     * half of 128 values that a head_dim of 64 or 192 leaves empty repeats the other, against codes of 0. */
+    const int cc = min(c0 + n, a.cols - 1), qi = kv4_query(cc, inv_group), see = a.start + qi + 1;
+    const int seen_first = a.start + kv4_query(c0, inv_group) + 1, seen_last = a.start + kv4_query(c0 + nc - 1, inv_group) + 1;
+    f32x4 q4[KS][8];
+    {
+        const float *src = a.Q + ((size_t)qi * a.n_heads + (size_t)(h * group + cc - qi * group)) * HD;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const float *from = src + 128 * ks + 32 * (HP % 2 && ks == KS - 1 ? g & 1 : g);
+#pragma unroll
+            for (int i = 0; i < 8; i++) q4[ks][i] = *reinterpret_cast<const f32x4 *>(from + 4 * i);
+        }
+    }
+    const int lo = (chunk * WAVES + wave) * a.per_wave * 32, rows = max(min(a.per_wave * 32, seen_last - lo), 0), tiles = (rows + 31) / 32;
     const size_t row0 = (size_t)h * c.max_rows + lo;
-    const int rows = max(hi - lo, 0);
     /* scales come in words; where a row has 2 or 6 bytes of them (HP odd) its first may start in the middle of one, whose other half is
      * memory that a word of the cache's reaches anyway */
-    const int sub = HP % 2 ? (int)((uintptr_t)(c.v_scales + row0 * 2 * HP) & 3) : 0;
-    /* a stage's requests: unit u of 16 bytes is row u / 2 HP, piece u % 2 HP of it; K's pieces are exchanged so that eight rows' same piece lie in
+    const int sub = HP % 2 ? (int)((uintptr_t)(c.v_scales + row0 * 2 * HP) & 3) : 0, words = rows ? (rows * 2 * HP + sub + 3) / 4 : 0;
+    /* what lies past the wave's rows reads as zeros */
+    const __amdgpu_buffer_rsrc_t kd = vt_buffer(c.k_codes + row0 * ROW, rows * ROW), vd = vt_buffer(c.v_codes + row0 * ROW, rows * ROW);
+    const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + row0 * 2 * HP - sub, words * 4), vsd = vt_buffer(c.v_scales + row0 * 2 * HP - sub, words * 4);
+    u32x4 scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd, lane * 16));
+    /* a tile's requests: unit u of 16 bytes is row u / 2 HP, piece u % 2 HP of it; K's pieces are exchanged so that eight rows' same piece lie in
      * different banks */
     const auto swizzle = [](int row, int piece) { return HP == 2 ? piece ^ ((row >> 1) & 3) : HP == 4 ? piece ^ (row & 7) : piece ^ ((row >> 2) & 1); };
-    int k_at[4];                                          /* HP of them (with that size the host pass drops the kernel) */
+    int k_at[4];                                         /* HP of them (with that size the host pass drops the kernel) */
 #pragma unroll
     for (int d = 0; d < HP; d++) {
         const int u = d * 64 + lane, r = u / (2 * HP);
         k_at[d] = r * ROW + swizzle(r, u - r * 2 * HP) * 16;
     }
     auto ask = [&](unsigned char *buf, int t) __attribute__((always_inline)) {
-        const int left = t < tiles ? rows - 32 * t : 0;                       /* none past the last tile: zeros, which nobody reads */
-        const size_t r = row0 + (t < tiles ? 32 * (size_t)t : 0);
-        const __amdgpu_buffer_rsrc_t kd = vt_buffer(c.k_codes + r * ROW, min(left, 32) * ROW), vd = vt_buffer(c.v_codes + r * ROW, min(left, 32) * ROW);
-        const int sbytes = left > 0 ? (min(left, 32) * 2 * HP + sub + 3) & ~3 : 0;
-        const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + r * 2 * HP - sub, sbytes), vsd = vt_buffer(c.v_scales + r * 2 * HP - sub, sbytes);
         unsigned char *b = buf + wave * STAGE;
 #define LDS(at) (__attribute__((address_space(3))) void *)(b + (at))
 #pragma unroll
-        for (int d = 0; d < HP; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(kd, LDS(d * 1024), 16, k_at[d], 0, 0, 0);
+        for (int d = 0; d < HP; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(kd, LDS(d * 1024), 16, k_at[d] + t * 32 * ROW, 0, 0, 0);
 #pragma unroll
-        for (int d = 0; d < HP; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(vd, LDS(32 * ROW + d * 1024), 16, d * 1024 + lane * 16, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(ksd, LDS(SC), 4, lane * 4, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(vsd, LDS(SC + 256), 4, lane * 4, 0, 0, 0);
+        for (int d = 0; d < HP; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(vd, LDS(32 * ROW + d * 1024), 16, d * 1024 + lane * 16 + t * 32 * ROW, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ksd, LDS(SC), 4, lane * 4 + t * 64 * HP, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vsd, LDS(SC + 256), 4, lane * 4 + t * 64 * HP, 0, 0, 0);
 #undef LDS
     };
-    /* queries (lane's column, values 32 g .. of each 128) and the scales of the first 1024 / 2 HP rows' values are asked for first: loads return in
-     * order */
-    const int cc = c0 + n, qi = vt_div(min(cc, a.cols - 1), a.group), see = a.start + qi + 1;
-    vt_f32x16 even[KS], odd[KS];
-    {
-        const float *src = a.Q + ((size_t)qi * a.n_heads + (size_t)h * a.group.d + (min(cc, a.cols - 1) - qi * a.group.d)) * HD;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const bool there = cc < a.cols && 128 * ks + 32 * g < HD;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const f32x4 v = there ? *reinterpret_cast<const f32x4 *>(src + 128 * ks + 32 * g + 4 * i) : f32x4{0.f, 0.f, 0.f, 0.f};
-                even[ks][2 * i] = v.x; odd[ks][2 * i] = v.y; even[ks][2 * i + 1] = v.z; odd[ks][2 * i + 1] = v.w;
-            }
-        }
-    }
-    const int words = (rows * 2 * HP + sub + 3) / 4;      /* as the requests below take them; zeros behind the last */
-    const unsigned *vs = reinterpret_cast<const unsigned *>(c.v_scales + row0 * 2 * HP - sub);
-    const __amdgpu_buffer_rsrc_t vsd0 = vt_buffer(vs, words * 4);
-    u32x4 scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd0, lane * 16));
     ask(buf0, 0);
     ask(buf1, 1);
     vt_u32x6 q[KS][KV4_PLANES];
     unsigned qs[KS][KV4_PLANES];
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) vt_mx4_planes<KV4_PLANES>(even[ks], odd[ks], q[ks], qs[ks]);
+    for (int ks = 0; ks < KS; ks++) {
+        vt_f32x16 even, odd;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const f32x4 v = q4[ks][i] * a.scale;
+            even[2 * i] = v.x; odd[2 * i] = v.y; even[2 * i + 1] = v.z; odd[2 * i + 1] = v.w;
+        }
+        vt_mx4_planes<KV4_PLANES>(even, odd, q[ks], qs[ks]);
+#pragma unroll
+        for (int p = 0; p < KV4_PLANES; p++) asm volatile("" : "+v"(q[ks][p]));       /* here, while the first tiles are on their way, and not behind the loop below */
+    }
     /* largest scale of the wave's values */
     unsigned most = 0, nan = 0;
-    for (int i = lane * 4;;) {
+    auto look = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             if (HP % 2) {                                 /* halves of a word that are not this wave's rows */
@@ -208,34 +214,33 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
             }
             kv4_scan4(scan[e], most, nan);
         }
-        i += 256;
-        if (i - lane * 4 >= words) break;
-        scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd0, i * 4));
+    };
+    look(lane * 4);
+    for (int i = 256; i < words; i += 256) {
+        scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd, (i + lane * 4) * 4));
+        look(i + lane * 4);
     }
-#pragma unroll
-    for (int w = 32; w > 0; w /= 2) {
-        most = max(most, (unsigned)__shfl_xor((int)most, w));
-        nan |= (unsigned)__shfl_xor((int)nan, w);
-    }
+    most = (unsigned)vt_wave_max((float)most);
+    nan = __any((int)nan);
     const int shift = 127 + KV4_V_EXP - (int)most;
     float m = -3.402823466e38f, l = 0.f;                  /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
     f32x4 o[CHUNKS * CD];
 #pragma unroll
     for (int i = 0; i < CHUNKS * CD; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int k_row = wave * STAGE + n * ROW, v_row = wave * STAGE + 32 * ROW + 4 * g * ROW + n * (CD / 2);
+    const int ks_row = wave * STAGE + SC + sub + n * 2 * HP, vs_row = wave * STAGE + SC + 256 + sub + 4 * g * 2 * HP + n * CD / 32;
     auto tile = [&](const unsigned char *buf, int t) __attribute__((always_inline)) {
-        const unsigned char *b = buf + wave * STAGE;
         f32x4 s[2];
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) {
-            const int row = 16 * kt + n;
             u32x4 k[KS];
             int ksc[KS];
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 const bool half = HP % 2 && ks == KS - 1;        /* 64 values behind the last 128: the other two groups of lanes have zeros */
                 const int p = 4 * ks + (half ? g & 1 : g);
-                k[ks] = *reinterpret_cast<const u32x4 *>(b + row * ROW + swizzle(row, p) * 16);
-                ksc[ks] = b[SC + sub + row * 2 * HP + p];
+                k[ks] = *reinterpret_cast<const u32x4 *>(buf + k_row + 16 * kt * ROW + swizzle(n, p) * 16);      /* the exchange is the same 16 rows on */
+                ksc[ks] = buf[ks_row + 16 * kt * 2 * HP + p];
                 if (half && g >= 2) { k[ks] = u32x4{0u, 0u, 0u, 0u}; ksc[ks] = 0; }
             }
             s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -247,20 +252,16 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
                                                                             ksc[ks], 0, (int)qs[ks][p]);
         }
         const int first = lo + 32 * t;
-        float top = -INFINITY;
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) s[kt][v] *= a.scale;
         if (first + 32 > seen_first) {
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
                 for (int v = 0; v < 4; v++) s[kt][v] = first + 16 * kt + 4 * g + v < see ? s[kt][v] : -INFINITY;
         }
+        float top = fmaxf(fmaxf(s[0].x, s[1].x), m);
 #pragma unroll
-        for (int v = 0; v < 4; v++) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
-        top = fmaxf(vt_rows_max(top), m);
+        for (int v = 1; v < 4; v++) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
+        top = vt_rows_max(top);
         if (__any(top != m)) {
             const float less = __builtin_amdgcn_exp2f(m - top);
             l *= less;
@@ -268,10 +269,11 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
             for (int i = 0; i < CHUNKS * CD; i++) o[i] = o[i] * less;
             m = top;
         }
+        const float base = (float)KV4_P_EXP - m;
         u32x4 hi4, lo4;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float p0 = __builtin_amdgcn_exp2f(s[e >> 1][2 * (e & 1)] - m + (float)KV4_P_EXP), p1 = __builtin_amdgcn_exp2f(s[e >> 1][2 * (e & 1) + 1] - m + (float)KV4_P_EXP);
+            const float p0 = __builtin_amdgcn_exp2f(s[e >> 1][2 * (e & 1)] + base), p1 = __builtin_amdgcn_exp2f(s[e >> 1][2 * (e & 1) + 1] + base);
             l += p0 + p1;
             const vt_f16x2 hi2 = __builtin_convertvector((f32x2{p0, p1}), vt_f16x2);
             hi4[e] = __builtin_bit_cast(unsigned, hi2);
@@ -283,11 +285,12 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
             unsigned two[8][CD / 2];                           /* key j's values 2 i, 2 i + 1 */
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int row = (j >> 2) * 16 + 4 * g + (j & 3);
-                const unsigned char *at = b + 32 * ROW + row * ROW + ch * 8 * CD + n * (CD / 2);
+                const int row = (j >> 2) * 16 + (j & 3);       /* and 4 g more */
+                const unsigned char *at = buf + v_row + row * ROW + ch * 8 * CD;
                 const unsigned w = CD == 8 ? *reinterpret_cast<const unsigned *>(at) : (unsigned)*reinterpret_cast<const uint16_t *>(at);
-                const int sb = b[SC + 256 + sub + row * 2 * HP + (16 * CD * ch + CD * n) / 32];
-                const float f = vt_mx4_scale((unsigned)min(max(sb + shift, 64), 127 + KV4_V_EXP));
+                /* a byte of 255 makes the sum wrap or meet the upper end: finite either way */
+                const int e = (int)((unsigned)(buf[vs_row + row * 2 * HP + CD / 2 * ch] + shift) << 23);
+                const float f = __int_as_float(min(max(e, 64 << 23), (127 + KV4_V_EXP) << 23));
                 two[j][0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 0));
                 two[j][1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 1));
                 if constexpr (CD == 8) {
@@ -322,7 +325,6 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
         if (t + 2 >= tiles) break;
         item(t + 2, buf2, buf1);
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);                          /* nothing arrives in the buffers any more */
     l = vt_rows_sum(l);
     if (nan) {
         /* rare: the first row of the wave's with a NaN in a block of 32 values reaches the columns that see it */
@@ -342,77 +344,81 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
                         if ((16 * CD * ch + CD * (4 * g + v)) / 32 == blk && see > at) o[ch * CD + i][v] = NAN;
         }
     }
-    /* the wave's part: weighted mean of its rows' values, largest score, sum of weights.  (A mean: sums of values near the end of the range
-     * would leave it.) */
+    /* The waves' parts, each times its share of the sum of weights, which is a mean of values: a sum of values near the end of the range would
+     * leave it. */
+    ml[wave][n][0] = m;                                          /* four lanes the same */
+    ml[wave][n][1] = l;
+    __builtin_amdgcn_s_waitcnt(0x0f70);                          /* nothing arrives in the buffers any more */
+    __syncthreads();
+    float M = m, L = 0.f;
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) M = fmaxf(M, ml[k][n][0]);
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) L = fmaf(ml[k][n][1], __builtin_amdgcn_exp2f(ml[k][n][0] - M), L);
     const auto area = [&](int w, int col) { return reinterpret_cast<float *>((col < 8 ? buf0 : buf1) + w * STAGE) + (col & 7) * OD; };
     {
-        const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-        float *to = area(wave, n);
+        const float f = L == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - M) / L;
+        float *to = area(wave, n) + 4 * g * CD;
 #pragma unroll
         for (int ch = 0; ch < CHUNKS; ch++)
 #pragma unroll
             for (int v = 0; v < 4; v++)
 #pragma unroll
-                for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * (4 * g + v) + i] = __builtin_amdgcn_ldexpf(o[ch * CD + i][v] * inv, -shift);
-        if (g == 0) { ml[wave][n][0] = m; ml[wave][n][1] = l; }
+                for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * v + i] = __builtin_amdgcn_ldexpf(o[ch * CD + i][v] * f, -shift);
     }
     __syncthreads();
-    const int per = a.chunks, head0 = h * a.group.d;
-    float *part = a.part + ((size_t)(h * (gridDim.x / a.chunks) + ct) * per) * KV4_COLS * (HD + 4);
-    auto store = [&](int col, int d, float v) {
-        const int k = c0 + col, i = vt_div(k, a.group);
-        a.out[((size_t)i * a.n_heads + head0 + (k - i * a.group.d)) * HD + d] = v;
+    const int per = a.chunks;
+    float *part = a.part + ((size_t)h * gridDim.y + ct) * per * KV4_COLS * OD;
+    auto result = [&](int col) {
+        const int k = c0 + col, i = kv4_query(k, inv_group);
+        return a.out + ((size_t)i * a.n_heads + (size_t)(h * group + k - i * group)) * HD;
     };
-    for (int e = (int)threadIdx.x; e < nc * HD; e += 64 * WAVES) {
-        const int col = e / HD, d = e - col * HD;
-        float M = ml[0][col][0], L = 0.f, v = 0.f, w[WAVES];
+    for (int e = (int)threadIdx.x; e < nc * (HD / 4); e += 64 * WAVES) {
+        const int col = e / (HD / 4), d = 4 * (e - col * (HD / 4));
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 1; k < WAVES; k++) M = fmaxf(M, ml[k][col][0]);
+        for (int k = 0; k < WAVES; k++) v = v + *reinterpret_cast<const f32x4 *>(area(k, col) + d);
+        if (per == 1) *reinterpret_cast<f32x4 *>(result(col) + d) = v;
+        else {
+            float *to = part + ((size_t)chunk * KV4_COLS + col) * OD + 4 + d;
 #pragma unroll
-        for (int k = 0; k < WAVES; k++) { w[k] = ml[k][col][1] * __builtin_amdgcn_exp2f(ml[k][col][0] - M); L += w[k]; }
-        const float inv = L == 0.f ? 0.f : __fdiv_rn(1.f, L);
-#pragma unroll
-        for (int k = 0; k < WAVES; k++) v = fmaf(area(k, col)[d], w[k] * inv, v);
-        if (per == 1) { store(col, d, v); continue; }
-        float *to = part + ((size_t)chunk * KV4_COLS + col) * (HD + 4);
-        vt_stc(to + 4 + d, v);
-        if (d == 0) { vt_stc(to, M); vt_stc(to + 1, L); }
+            for (int i = 0; i < 4; i++) vt_stc(to + i, v[i]);
+        }
     }
     if (per == 1) return;
+    if (wave == 0 && lane < nc) {
+        float *to = part + ((size_t)chunk * KV4_COLS + lane) * OD;
+        vt_stc(to, M);
+        vt_stc(to + 1, L);
+    }
     __builtin_amdgcn_s_waitcnt(0x0f70);                          /* the part's stores are acknowledged */
     __syncthreads();
-    unsigned *cnt = a.cnt + h * (gridDim.x / a.chunks) + ct;
+    unsigned *cnt = a.cnt + h * gridDim.y + ct;
     if (threadIdx.x == 0) last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(per - 1);
     __syncthreads();
     if (!last) return;
     if (threadIdx.x == 0) vt_stc_u32(cnt, 0u);                   /* ready for the next launch */
     /* a wave per column: lane k has part k's largest score and sum of weights */
-    const __amdgpu_buffer_rsrc_t pd = vt_buffer(part, per * KV4_COLS * (HD + 4) * 4);
+    const __amdgpu_buffer_rsrc_t pd = vt_buffer(part, per * KV4_COLS * OD * 4);
     for (int col = wave; col < nc; col += WAVES) {
-        const int at = ((min(lane, per - 1) * KV4_COLS + col) * (HD + 4)) * 4;
-        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(pd, at, 0, 16 /* sc1 */);
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(pd, (min(lane, per - 1) * KV4_COLS + col) * OD * 4, 0, 16 /* sc1 */);
         const float pm = __uint_as_float(v.x), pl = lane < per ? __uint_as_float(v.y) : 0.f;
-        const float w = pl * __builtin_amdgcn_exp2f(pm - vt_wave_max(pm)), L = vt_wave_sum(w);
-        wt[col][lane] = L == 0.f ? 0.f : __fdiv_rn(w, L);
+        const float w = pl * __builtin_amdgcn_exp2f(pm - vt_wave_max(pm)), all = vt_wave_sum(w);
+        wt[col][lane] = all == 0.f ? 0.f : w / all;
     }
     __syncthreads();
-    for (int e = (int)threadIdx.x; e < nc * HD / 4; e += 64 * WAVES) {
-        const int col = e / (HD / 4), d = 4 * (e - col * (HD / 4)), at = (col * (HD + 4) + 4 + d) * 4;
+    for (int e = (int)threadIdx.x; e < nc * (HD / 4); e += 64 * WAVES) {
+        const int col = e / (HD / 4), d = 4 * (e - col * (HD / 4)), at = (col * OD + 4 + d) * 4;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (int k0 = 0; k0 < per; k0 += 16) {
-            u32x4 p[16];
+#pragma unroll 1
+        for (int k0 = 0; k0 < per; k0 += 16) {                   /* parts past the last: the last again, times 0 */
+            f32x4 p[16];
 #pragma unroll
-            for (int k = 0; k < 16; k++) p[k] = __builtin_amdgcn_raw_buffer_load_b128(pd, at, min(k0 + k, per - 1) * KV4_COLS * (HD + 4) * 4, 16);
+            for (int k = 0; k < 16; k++) p[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(pd, at + min(k0 + k, per - 1) * (KV4_COLS * OD * 4), 0, 16));
 #pragma unroll
-            for (int k = 0; k < 16; k++)
-                if (k0 + k < per) {
-                    const float w = wt[col][k0 + k];
-                    const f32x4 o4 = __builtin_bit_cast(f32x4, p[k]);
-                    v = f32x4{fmaf(o4.x, w, v.x), fmaf(o4.y, w, v.y), fmaf(o4.z, w, v.z), fmaf(o4.w, w, v.w)};
-                }
+            for (int k = 0; k < 16; k++) v = v + p[k] * wt[col][k0 + k];
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++) store(col, d + i, v[i]);
+        *reinterpret_cast<f32x4 *>(result(col) + d) = v;
     }
 }
 
@@ -427,7 +433,7 @@ static int kv4_stream(const tts_hip_kv4_t *cache, kv4_job a) {
     a.per_wave = (int)((tiles + chunks * WAVES - 1) / (chunks * WAVES));
     a.chunks = (int)((tiles + (long long)a.per_wave * WAVES - 1) / ((long long)a.per_wave * WAVES));
     if (a.chunks > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)cts * heads * a.chunks * KV4_COLS * (cache->head_dim + 4)))) return -1;
-    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)(cts * a.chunks), (unsigned)heads), dim3(64 * WAVES), 0, g_vt.stream, *cache, a);
+    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)a.chunks, (unsigned)cts, (unsigned)heads), dim3(64 * WAVES), 0, g_vt.stream, *cache, a);
     return 0;
 }
 
@@ -439,7 +445,7 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
     if (n_heads < 1 || n_heads % cache->n_kv_heads) { vt_set_error("%s: %d heads on %d kv heads", who, n_heads, cache->n_kv_heads); return -1; }
     const int group = n_heads / cache->n_kv_heads, HP = cache->head_dim / 64;
     const long long cols = (long long)seq_len * group;
-    if (cols > 1 << 28 || cache->n_kv_heads > 65535 || (long long)start_pos + seq_len > 1 << 28) { vt_set_error("%s: %d queries of %d heads on %d behind %d rows are too many for one call", who, seq_len, n_heads, cache->n_kv_heads, start_pos); return -1; }
+    if (cols > 1 << 28 || cache->n_kv_heads > 65535 || (long long)start_pos + seq_len > 1 << 25) { vt_set_error("%s: %d queries of %d heads on %d behind %d rows are too many for one call", who, seq_len, n_heads, cache->n_kv_heads, start_pos); return -1; }
     if (!vt_mx4_ready(who)) return -1;
     kv4_job a = {d_out, d_Q, seq_len, start_pos, n_heads, (int)cols, 0, 1, vt_divisor_of(group, cols), scale * 1.44269504f, NULL, g_vt.d_kv4_cnt};
     if (HP == 1 ? kv4_stream<1, 8>(cache, a) : HP == 2 ? kv4_stream<2, 8>(cache, a) : HP == 3 ? kv4_stream<3, 4>(cache, a) : kv4_stream<4, 4>(cache, a)) return -1;
