@@ -128,7 +128,7 @@ static int init_context(int kv_cache_max) {
         {(void **)&g_vt.d_h, sizeof(float) * VT_FFN},
         {(void **)&g_vt.d_att_part, sizeof(float) * VT_HEADS * max_chunks * VT_ATT_STRIDE},
         {(void **)&g_vt.d_att_cnt, sizeof(unsigned) * TTS_HIP_DEC_LAYERS * VT_KV_HEADS},
-        {(void **)&g_vt.d_kv4_cnt, sizeof(unsigned) * VT_KV4_COUNTERS},
+        {(void **)&g_vt.d_mx4_cnt, sizeof(unsigned) * VT_MX4_COUNTERS},
         {(void **)&g_vt.d_embed, sizeof(float) * VT_DIM},
         {(void **)&g_vt.d_hidden, sizeof(float) * (VT_DIM + 64)},
         {(void **)&g_vt.d_bar_flags, sizeof(unsigned) * (size_t)VT_FLAG_COPIES * VT_FLAG_STRIDE},
@@ -215,7 +215,7 @@ static void teardown(void) {
                     g_vt.ac.time_inv_freq, g_vt.ac.time_tok, g_vt.ac.time_qkv, g_vt.ac.noise_qkv, g_vt.ac.noise_gram, g_vt.ac.audio_emb, g_vt.ac.audio_offsets,
                     g_hip.kv_cache_k_gpu, g_hip.kv_cache_v_gpu,
                     g_vt.d_rope, g_vt.d_x, g_vt.d_q, g_vt.d_attn, g_vt.d_h, g_vt.d_att_part,
-                    g_vt.d_att_cnt, g_vt.d_kv4_cnt, g_vt.d_embed, g_vt.d_hidden, g_vt.d_bar_flags,
+                    g_vt.d_att_cnt, g_vt.d_mx4_cnt, g_vt.d_embed, g_vt.d_hidden, g_vt.d_bar_flags,
                     g_vt.d_abort, g_vt.d_dummy, g_vt.d_scratch, g_vt.d_kv_img};
     for (size_t i = 0; i < sizeof ptrs / sizeof ptrs[0]; i++)
         if (ptrs[i]) (void)hipFree(ptrs[i]);

@@ -104,6 +104,7 @@ typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
 #define KV4_V_EXP 13                       /* .. and values up to 6 times 2^13 are fp16 */
 #define KV4_COLS 16
 #define KV4_MAX_CHUNKS 64
+#define KV4_STREAM_COLS 32                 /* up to so many columns */
 
 struct kv4_job {
     float *out;
@@ -126,6 +127,11 @@ static __device__ __forceinline__ void kv4_scan4(unsigned w, unsigned &most, uns
         nan |= s == 255u;
         most = max(most, s == 255u ? 0u : s);
     }
+}
+
+/* K's pieces of 16 bytes are exchanged within a row in LDS, so that eight rows' same piece lie in different banks */
+template <int HP> static __device__ __forceinline__ int kv4_swizzle(int row, int piece) {
+    return HP == 2 ? piece ^ ((row >> 1) & 3) : HP == 4 ? piece ^ (row & 7) : piece ^ ((row >> 2) & 1);
 }
 
 /* Few columns: a wave streams 32 rows of K and V at a time into LDS of its own, two such tiles on their way while one is multiplied,
@@ -167,14 +173,12 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
     const __amdgpu_buffer_rsrc_t kd = vt_buffer(c.k_codes + row0 * ROW, rows * ROW), vd = vt_buffer(c.v_codes + row0 * ROW, rows * ROW);
     const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + row0 * 2 * HP - sub, words * 4), vsd = vt_buffer(c.v_scales + row0 * 2 * HP - sub, words * 4);
     u32x4 scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd, lane * 16));
-    /* a tile's requests: unit u of 16 bytes is row u / 2 HP, piece u % 2 HP of it; K's pieces are exchanged so that eight rows' same piece lie in
-     * different banks */
-    const auto swizzle = [](int row, int piece) { return HP == 2 ? piece ^ ((row >> 1) & 3) : HP == 4 ? piece ^ (row & 7) : piece ^ ((row >> 2) & 1); };
+    /* a tile's requests: unit u of 16 bytes is row u / 2 HP, piece u % 2 HP of it */
     int k_at[4];                                         /* HP of them (with that size the host pass drops the kernel) */
 #pragma unroll
     for (int d = 0; d < HP; d++) {
         const int u = d * 64 + lane, r = u / (2 * HP);
-        k_at[d] = r * ROW + swizzle(r, u - r * 2 * HP) * 16;
+        k_at[d] = r * ROW + kv4_swizzle<HP>(r, u - r * 2 * HP) * 16;
     }
     auto ask = [&](unsigned char *buf, int t) __attribute__((always_inline)) {
         unsigned char *b = buf + wave * STAGE;
@@ -239,7 +243,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
             for (int ks = 0; ks < KS; ks++) {
                 const bool half = HP % 2 && ks == KS - 1;        /* 64 values behind the last 128: the other two groups of lanes have zeros */
                 const int p = 4 * ks + (half ? g & 1 : g);
-                k[ks] = *reinterpret_cast<const u32x4 *>(buf + k_row + 16 * kt * ROW + swizzle(n, p) * 16);      /* the exchange is the same 16 rows on */
+                k[ks] = *reinterpret_cast<const u32x4 *>(buf + k_row + 16 * kt * ROW + kv4_swizzle<HP>(n, p) * 16);      /* the exchange is the same 16 rows on */
                 ksc[ks] = buf[ks_row + 16 * kt * 2 * HP + p];
                 if (half && g >= 2) { k[ks] = u32x4{0u, 0u, 0u, 0u}; ksc[ks] = 0; }
             }
@@ -422,6 +426,272 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
     }
 }
 
+/* Many columns: a workgroup has KV4_TILE of them, a wave 32, and goes through its rows 64 at a time.  K comes as it lies, V as fp16 in the order of
+ * the matrix instruction's operand (A of 32 x 32 x 16, value 2 HP r + i in row r of instruction i; four keys of a value are 8 bytes): the workgroup
+ * converts the next rows while it multiplies these, each lane four keys of eight values, so that a conversion serves all columns.  Scores are 32 x 32 x 64.
+ * Where there are few columns for the chip, or a prompt's last ones would be behind everybody, several workgroups share a head's rows, `run` tiles
+ * each; the last to arrive adds their parts. */
+#define KV4_TILE_WAVES 4
+#define KV4_TILE (32 * KV4_TILE_WAVES)
+#define KV4_MAX_PARTS 32
+struct kv4_tile_job { kv4_job a; int run, tiles_of_cols, most_parts; };
+
+template <int HP>
+__global__ void __launch_bounds__(64 * KV4_TILE_WAVES, HP <= 2 ? 2 : 1) vt_kv4_tile_kernel(tts_hip_kv4_t c, kv4_tile_job j) {
+    constexpr int HD = 64 * HP, ROW = 32 * HP, THREADS = 64 * KV4_TILE_WAVES, UNITS = 128 * HP, UN = (UNITS + THREADS - 1) / THREADS, DT = 2 * HP;
+    constexpr int KB = 64 * ROW, SB = KB + UNITS, VB = SB;      /* K rows, their scales, V's operands */
+    __shared__ __attribute__((aligned(16))) unsigned char buf[2][VB + 64 * HD * 2];
+    __shared__ unsigned scan_most[KV4_TILE_WAVES], scan_nan[KV4_TILE_WAVES];
+    __shared__ int last;
+    const kv4_job &a = j.a;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5, h = (int)blockIdx.y;
+    /* the columns that see most first */
+    const int ct = j.tiles_of_cols - 1 - (int)blockIdx.x / j.most_parts, part = (int)blockIdx.x % j.most_parts;
+    const int c0 = ct * KV4_TILE, nc = min(KV4_TILE, a.cols - c0);
+    const int end = a.start + vt_div(c0 + nc - 1, a.group) + 1, parts = ((end + 63) / 64 + j.run - 1) / j.run;
+    if (part >= parts) return;
+    const int lo = part * j.run * 64, rows = min(j.run * 64, end - lo), tiles = (rows + 63) / 64;
+    const int w0 = c0 + 32 * wave, wc = min(w0 + 32, a.cols) - w0;               /* this wave's columns: none, perhaps */
+    const int cc = min(w0 + n, a.cols - 1), qi = vt_div(cc, a.group), see = a.start + qi + 1;
+    const int seen_first = a.start + vt_div(min(w0, a.cols - 1), a.group) + 1, seen_last = wc > 0 ? a.start + vt_div(w0 + wc - 1, a.group) + 1 : 0;
+    const size_t row0 = (size_t)h * c.max_rows + lo;
+    const __amdgpu_buffer_rsrc_t kd = vt_buffer(c.k_codes + row0 * ROW, rows * ROW), vd = vt_buffer(c.v_codes + row0 * ROW, rows * ROW);
+    const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + row0 * DT, rows * DT), vsd = vt_buffer(c.v_scales + row0 * DT, rows * DT);
+    /* unit u: 16 bytes of K, row u / 2 HP; a scale of K; V's keys 4 (u / 8 HP) .. + 3, values 8 (u % 8 HP) .. + 7 */
+    u32x4 kr[UN];
+    unsigned vr[UN][4];
+    unsigned char ksr[UN], vsr[UN][4];
+    auto load = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < UN; i++) {
+            const int u = tid + THREADS * i;
+            if (UNITS % THREADS && u >= UNITS) break;
+            kr[i] = __builtin_bit_cast(u32x4, vt_buffer_ld4(kd, t * 64 * ROW + u * 16));
+            ksr[i] = __builtin_amdgcn_raw_buffer_load_b8(ksd, t * 64 * DT + u, 0, 0);
+            const int kg = u / (8 * HP), dg = u - kg * 8 * HP;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                vr[i][k] = __builtin_amdgcn_raw_buffer_load_b32(vd, (t * 64 + 4 * kg + k) * ROW + dg * 4, 0, 0);
+                vsr[i][k] = __builtin_amdgcn_raw_buffer_load_b8(vsd, (t * 64 + 4 * kg + k) * DT + dg / 4, 0, 0);
+            }
+        }
+    };
+    load(0);
+    vt_u32x6 q[HP][KV4_PLANES];
+    unsigned qs[HP][KV4_PLANES];
+    {
+        const float *src = a.Q + ((size_t)qi * a.n_heads + (size_t)h * a.group.d + (cc - qi * a.group.d)) * HD + 32 * g;
+#pragma unroll
+        for (int k = 0; k < HP; k++) {
+            vt_f32x16 even, odd;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(src + 64 * k + 4 * i) * a.scale;
+                even[2 * i] = v.x; odd[2 * i] = v.y; even[2 * i + 1] = v.z; odd[2 * i + 1] = v.w;
+            }
+            vt_mx4_planes<KV4_PLANES>(even, odd, q[k], qs[k]);
+        }
+    }
+    unsigned most = 0, nan = 0;
+    for (int i = tid; i < rows * DT; i += THREADS * 8) {
+        unsigned char b[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) b[e] = __builtin_amdgcn_raw_buffer_load_b8(vsd, i + e * THREADS, 0, 0);      /* zeros past the last */
+#pragma unroll
+        for (int e = 0; e < 8; e++) { nan |= b[e] == 255; most = max(most, b[e] == 255 ? 0u : (unsigned)b[e]); }
+    }
+    most = (unsigned)vt_wave_max((float)most);
+    if (lane == 0) scan_most[wave] = most;
+    nan = __any((int)nan);
+    if (lane == 0) scan_nan[wave] = nan;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < KV4_TILE_WAVES; w++) { most = max(most, scan_most[w]); nan |= scan_nan[w]; }
+    const int shift = __builtin_amdgcn_readfirstlane(127 + KV4_V_EXP - (int)most);
+    /* where value d's four keys go: row r = d / 2 HP of instruction i = d % 2 HP, step t of 16 keys, half h of the lane's eight (step and half by the
+     * unit: its keys are 4 (kg % 4) .. of step kg / 4, i.e. group of lanes kg % 2, half kg / 2 % 2) */
+    int v_to[2][8];                                       /* UN of them (with that size the host pass drops the kernel) */
+#pragma unroll
+    for (int i = 0; i < UN; i++) {
+        const int u = tid + THREADS * i, kg = u / (8 * HP), dg = u - kg * 8 * HP;
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            const int r = (8 * dg + d) / DT, in = (8 * dg + d) - r * DT;
+            v_to[i][d] = VB + (((in * 4 + (kg >> 2)) * 64 + (kg & 1) * 32 + r) * 2 + ((kg >> 1) & 1)) * 8;
+        }
+    }
+    auto put = [&](unsigned char *b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < UN; i++) {
+            const int u = tid + THREADS * i;
+            if (UNITS % THREADS && u >= UNITS) break;
+            const int r = u / DT;
+            *reinterpret_cast<u32x4 *>(b + r * ROW + kv4_swizzle<HP>(r, u - r * DT) * 16) = kr[i];
+            b[KB + u] = ksr[i];
+            unsigned two[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int e = (int)((unsigned)(vsr[i][k] + shift) << 23);
+                const float f = __int_as_float(min(max(e, 64 << 23), (127 + KV4_V_EXP) << 23));
+                two[k][0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(vr[i][k], f, 0));
+                two[k][1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(vr[i][k], f, 1));
+                two[k][2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(vr[i][k], f, 2));
+                two[k][3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(vr[i][k], f, 3));
+            }
+#pragma unroll
+            for (int d = 0; d < 8; d++) {
+                const unsigned pick = d & 1 ? 0x07060302u : 0x05040100u;
+                *reinterpret_cast<u32x2 *>(b + v_to[i][d]) = u32x2{__builtin_amdgcn_perm(two[1][d / 2], two[0][d / 2], pick), __builtin_amdgcn_perm(two[3][d / 2], two[2][d / 2], pick)};
+            }
+        }
+    };
+    float m = -3.402823466e38f, l = 0.f;
+    vt_f32x16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++) o[i] = vt_f32x16{};
+    put(buf[0]);
+    __syncthreads();
+#pragma unroll 1
+    for (int t = 0; t < tiles; t++) {
+        const unsigned char *b = buf[t & 1];
+        if (t + 1 < tiles) load(t + 1);
+        const int first = lo + 64 * t;
+        if (first < seen_last) {                          /* else nobody of this wave sees these rows */
+            vt_f32x16 s[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                const int row = 32 * kt + n;
+                u32x4 k[HP];
+                int ksc[HP];
+#pragma unroll
+                for (int kk = 0; kk < HP; kk++) {
+                    k[kk] = *reinterpret_cast<const u32x4 *>(b + row * ROW + kv4_swizzle<HP>(row, 2 * kk + g) * 16);
+                    ksc[kk] = b[KB + row * DT + 2 * kk + g];
+                }
+                s[kt] = vt_f32x16{};
+#pragma unroll
+                for (int p = KV4_PLANES - 1; p >= 0; p--)
+#pragma unroll
+                    for (int kk = 0; kk < HP; kk++)
+                        s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m1(k[kk]), vt_mfma_e2m3(q[kk][p]), s[kt], VT_MFMA_E2M1, VT_MFMA_E2M3, 0, ksc[kk], 0, (int)qs[kk][p]);
+            }
+            if (first + 64 > seen_first) {
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) s[kt][v] = first + 32 * kt + 8 * (v >> 2) + 4 * g + (v & 3) < see ? s[kt][v] : -INFINITY;
+            }
+            float top = m;
+#pragma unroll
+            for (int v = 0; v < 16; v++) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
+            { const f32x2 r = vt_swap32(top, top); top = fmaxf(r.x, r.y); }
+            if (__any(top != m)) {
+                const float less = __builtin_amdgcn_exp2f(m - top);
+                l *= less;
+#pragma unroll
+                for (int i = 0; i < DT; i++) o[i] = o[i] * less;
+                m = top;
+            }
+            const float base = (float)KV4_P_EXP - m;
+#pragma unroll
+            for (int st = 0; st < 4; st++) {              /* 16 keys: elements 8 (st % 2) .. of scores st / 2 */
+                u32x4 hi4, lo4;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p0 = __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e] + base), p1 = __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e + 1] + base);
+                    l += p0 + p1;
+                    const vt_f16x2 hi2 = __builtin_convertvector((f32x2{p0, p1}), vt_f16x2);
+                    hi4[e] = __builtin_bit_cast(unsigned, hi2);
+                    lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{__fsub_rn(p0, (float)hi2.x), __fsub_rn(p1, (float)hi2.y)}), vt_f16x2));
+                }
+                const vt_f16x8 ph = __builtin_bit_cast(vt_f16x8, hi4), pl = __builtin_bit_cast(vt_f16x8, lo4);
+#pragma unroll
+                for (int i = 0; i < DT; i++) {
+                    const vt_f16x8 v = __builtin_bit_cast(vt_f16x8, *reinterpret_cast<const u32x4 *>(b + VB + ((i * 4 + st) * 64 + lane) * 16));
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[i], 0, 0, 0);
+                }
+            }
+        }
+        if (t + 1 < tiles) put(buf[(t + 1) & 1]);
+        __syncthreads();
+    }
+    { const f32x2 r = vt_swap32(l, l); l = r.x + r.y; }
+    if (nan) {
+#pragma unroll 1
+        for (int blk = 0; blk < DT; blk++) {
+            int at = 0x7fffffff;
+            for (int r = lane; r < rows; r += 64)
+                if (c.v_scales[(row0 + r) * DT + blk] == 255) { at = lo + r; break; }
+#pragma unroll
+            for (int w = 32; w > 0; w /= 2) at = min(at, __shfl_xor(at, w));
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    if ((DT * (8 * (v >> 2) + 4 * g + (v & 3)) + i) / 32 == blk && see > at) o[i][v] = NAN;
+        }
+    }
+    /* the part's mean of values */
+    {
+        const float f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) o[i][v] = __builtin_amdgcn_ldexpf(o[i][v] * f, -shift);
+    }
+    if (parts > 1) {
+        /* a part lies as the lanes hold it: [part][wave][4 HD / 32 vectors of four, then largest score and sum of weights][lane] */
+        constexpr int WAVE_PART = (DT * 4 + 1) * 1024, PART = KV4_TILE_WAVES * WAVE_PART;
+        const __amdgpu_buffer_rsrc_t pd = vt_buffer(reinterpret_cast<unsigned char *>(a.part) + ((size_t)h * j.tiles_of_cols + ct) * j.most_parts * PART, parts * PART);
+        const int mine = wave * WAVE_PART + lane * 16;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, (f32x4{o[i][4 * v], o[i][4 * v + 1], o[i][4 * v + 2], o[i][4 * v + 3]})), pd, mine + part * PART + (4 * i + v) * 1024, 0, 16 /* sc1 */);
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, pd, mine + part * PART + DT * 4 * 1024, 0, 16);
+        __builtin_amdgcn_s_waitcnt(0x0f70);              /* acknowledged */
+        __syncthreads();
+        unsigned *cnt = a.cnt + h * j.tiles_of_cols + ct;
+        if (tid == 0) last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
+        __syncthreads();
+        if (!last) return;
+        if (tid == 0) vt_stc_u32(cnt, 0u);
+        if (wc <= 0) return;
+        float M = -3.402823466e38f, L = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < parts; k++) {
+            const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(pd, mine + k * PART + DT * 4 * 1024, 0, 16);
+            const float pm = __uint_as_float(v.x), top = fmaxf(M, pm);
+            L = fmaf(L, __builtin_amdgcn_exp2f(M - top), __uint_as_float(v.y) * __builtin_amdgcn_exp2f(pm - top));
+            M = top;
+        }
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[i] = vt_f32x16{};
+#pragma unroll 1
+        for (int k = 0; k < parts; k++) {
+            const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(pd, mine + k * PART + DT * 4 * 1024, 0, 16);
+            f32x4 p[DT * 4];
+#pragma unroll
+            for (int x = 0; x < DT * 4; x++) p[x] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(pd, mine + k * PART + x * 1024, 0, 16));
+            const float w = L == 0.f ? 0.f : __uint_as_float(ml.y) * __builtin_amdgcn_exp2f(__uint_as_float(ml.x) - M) / L;
+#pragma unroll
+            for (int x = 0; x < DT * 4; x++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[x / 4][4 * (x % 4) + e] = fmaf(p[x][e], w, o[x / 4][4 * (x % 4) + e]);
+        }
+    }
+    /* element v of lane l is value 2 HP (8 (v / 4) + 4 (l / 32) + v % 4) + i */
+    if (n < wc) {
+        float *to = a.out + ((size_t)qi * a.n_heads + (size_t)h * a.group.d + (cc - qi * a.group.d)) * HD;
+#pragma unroll
+        for (int v = 0; v < 16; v++)
+#pragma unroll
+            for (int i = 0; i < DT; i += 2) *reinterpret_cast<f32x2 *>(to + DT * (8 * (v >> 2) + 4 * g + (v & 3)) + i) = f32x2{o[i][v], o[i + 1][v]};
+    }
+}
+
 template <int HP, int WAVES>
 static int kv4_stream(const tts_hip_kv4_t *cache, kv4_job a) {
     const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
@@ -429,11 +699,33 @@ static int kv4_stream(const tts_hip_kv4_t *cache, kv4_job a) {
     long long chunks = (8 * n_cu / WAVES + cts * heads - 1) / (cts * heads);
     if (chunks > KV4_MAX_CHUNKS) chunks = KV4_MAX_CHUNKS;
     if (chunks > (tiles + WAVES - 1) / WAVES) chunks = (tiles + WAVES - 1) / WAVES;
-    if (cts * heads > VT_KV4_COUNTERS) chunks = 1;
+    if (cts * heads > VT_MX4_COUNTERS) chunks = 1;
     a.per_wave = (int)((tiles + chunks * WAVES - 1) / (chunks * WAVES));
     a.chunks = (int)((tiles + (long long)a.per_wave * WAVES - 1) / ((long long)a.per_wave * WAVES));
     if (a.chunks > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)cts * heads * a.chunks * KV4_COLS * (cache->head_dim + 4)))) return -1;
     hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)a.chunks, (unsigned)cts, (unsigned)heads), dim3(64 * WAVES), 0, g_vt.stream, *cache, a);
+    return 0;
+}
+
+/* `run` tiles of 64 rows a workgroup */
+template <int HP>
+static int kv4_tiles(const tts_hip_kv4_t *cache, const kv4_job &a) {
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, per_cu = HP <= 2 ? 2 : 1;
+    kv4_tile_job j = {a, 0, (a.cols + KV4_TILE - 1) / KV4_TILE, 1};
+    const long long heads = cache->n_kv_heads, last = ((long long)a.start + a.seq + 63) / 64, first = (a.start + 64) / 64;
+    const long long total = heads * j.tiles_of_cols * ((first + last + 1) / 2);
+    long long run = total / ((long long)n_cu * per_cu) + 1;
+    if (run < 4) run = 4;
+    if (heads * j.tiles_of_cols > VT_MX4_COUNTERS) run = last;
+    if (run * KV4_MAX_PARTS < last) run = (last + KV4_MAX_PARTS - 1) / KV4_MAX_PARTS;
+    if (run > 1 << 16) {
+        run = 1 << 16;                                   /* a descriptor's 31 bits */
+        if (heads * j.tiles_of_cols > VT_MX4_COUNTERS && run < last) { vt_set_error("tts_hip_kv4_attention: %d queries behind %d rows are too many for one call", a.seq, a.start); return -1; }
+    }
+    j.run = (int)run;
+    j.most_parts = (int)((last + run - 1) / run);
+    if (j.most_parts > 1 && !(j.a.part = (float *)vt_scratch((size_t)heads * j.tiles_of_cols * j.most_parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
+    hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)(j.tiles_of_cols * (long long)j.most_parts), (unsigned)heads), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, *cache, j);
     return 0;
 }
 
@@ -447,7 +739,9 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
     const long long cols = (long long)seq_len * group;
     if (cols > 1 << 28 || cache->n_kv_heads > 65535 || (long long)start_pos + seq_len > 1 << 25) { vt_set_error("%s: %d queries of %d heads on %d behind %d rows are too many for one call", who, seq_len, n_heads, cache->n_kv_heads, start_pos); return -1; }
     if (!vt_mx4_ready(who)) return -1;
-    kv4_job a = {d_out, d_Q, seq_len, start_pos, n_heads, (int)cols, 0, 1, vt_divisor_of(group, cols), scale * 1.44269504f, NULL, g_vt.d_kv4_cnt};
-    if (HP == 1 ? kv4_stream<1, 8>(cache, a) : HP == 2 ? kv4_stream<2, 8>(cache, a) : HP == 3 ? kv4_stream<3, 4>(cache, a) : kv4_stream<4, 4>(cache, a)) return -1;
+    kv4_job a = {d_out, d_Q, seq_len, start_pos, n_heads, (int)cols, 0, 1, vt_divisor_of(group, cols), scale * 1.44269504f, NULL, g_vt.d_mx4_cnt};
+    if (cols > KV4_STREAM_COLS) {
+        if (HP == 1 ? kv4_tiles<1>(cache, a) : HP == 2 ? kv4_tiles<2>(cache, a) : HP == 3 ? kv4_tiles<3>(cache, a) : kv4_tiles<4>(cache, a)) return -1;
+    } else if (HP == 1 ? kv4_stream<1, 8>(cache, a) : HP == 2 ? kv4_stream<2, 8>(cache, a) : HP == 3 ? kv4_stream<3, 4>(cache, a) : kv4_stream<4, 4>(cache, a)) return -1;
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }

@@ -122,6 +122,24 @@ __device__ __forceinline__ void vt_mx4_planes(vt_f32x16 even, vt_f32x16 odd, vt_
     }
 }
 
+/* 32 values of a row from column `at` on, through a buffer that holds the row `row_at` bytes in; zeros from column `cols` on.  whole: rows lie on 16 bytes.
+ * (No branch around a load: behind one the compiler waits for it, a trip to memory each.) */
+__device__ __forceinline__ void vt_mx4_load32(__amdgpu_buffer_rsrc_t x, int row_at, int at, int cols, int whole, vt_f32x16 &even, vt_f32x16 &odd) {
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const f32x4 v = vt_buffer_ld4(x, at + 4 * i < cols ? row_at + (at + 4 * i) * 4 : 0x7ffffff0);
+            even[2 * i] = v.x; odd[2 * i] = v.y; even[2 * i + 1] = v.z; odd[2 * i + 1] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            even[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(x, at + 2 * i < cols ? row_at + (at + 2 * i) * 4 : 0x7ffffff0, 0, 0));
+            odd[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(x, at + 2 * i + 1 < cols ? row_at + (at + 2 * i + 1) * 4 : 0x7ffffff0, 0, 0));
+        }
+    }
+}
+
 __device__ __forceinline__ vt_i32x8 vt_mfma_e2m1(const u32x4 &v) { return __builtin_bit_cast(vt_i32x8, __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1)); }
 __device__ __forceinline__ vt_i32x8 vt_mfma_e2m3(const vt_u32x6 &v) { return __builtin_bit_cast(vt_i32x8, __builtin_shufflevector(v, v, 0, 1, 2, 3, 4, 5, -1, -1)); }
 

@@ -113,32 +113,49 @@ extern "C" int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const 
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
 
-/* ---- linear layer: up to four rows ------------------------------------------------------------------------------------
- * y^T[weight row][column] on v_mfma_scale_f32_16x16x128_f8f6f4: 16 weight rows go in as they lie in memory, and a row of x as four columns, its
- * four e2m3 planes (vt_mx4.h), so that four rows of x fill an instruction and nothing is decoded.  Every workgroup splits x itself, while its
- * first weights are on their way.  Its waves share K, a wave's weights come in parts of 16 rows x 2 panels (lines of 128 bytes) straight into
- * LDS of its own, three parts ahead of the one that is multiplied, and it waits for nothing but its own loads; the waves' sums of 16 rows meet in LDS behind a
- * bare barrier.  A panel's products start from zero and are added to the sum by the vector unit, which rounds; the matrix unit cuts at 2^-23. */
-#define MXR_ROWS 4
-#define MXR_WAVES 4
+/* ---- linear layer: up to eight rows --------------------------------------------------------------------------------
+ * y^T[weight row][column] on v_mfma_scale_f32_16x16x128_f8f6f4: 16 weight rows go in as they lie in memory, nothing is decoded, and the four e2m3 planes
+ * of x (vt_mx4.h) are columns or instructions: up to four rows of x all planes in one instruction (a row is four columns), up to eight rows two in each of
+ * G = 2, the smaller ones first.  Every workgroup splits x (a cut of K of it) itself, while its first weights are on their way.  Its waves share K, or groups of
+ * four of them share K and take blocks of 16 weight rows in turn where there are several blocks; a wave's weights come in parts of 16 rows x 2 panels
+ * (lines of 128 bytes) straight into LDS of its own, three parts ahead of the one that is multiplied, and it waits for nothing but its own loads; the
+ * waves' sums of 16 rows meet in LDS behind a bare barrier.  A panel's products start from zero and are added to the sum by the vector unit, which
+ * rounds; the matrix unit cuts at 2^-23.  x's planes have to fit LDS: where they do not, K is cut, the cuts' sums go to memory and the last workgroup
+ * of a block of rows to arrive adds them. */
+#define MXR_ROWS 8
+#define MXR_WAVES 8
 #define MXR_PLANES 4
 #define MXR_PART (16 * 128 + 256)          /* codes, then 16 x 2 words of scales and as much room */
 
-struct mxr_job { float *y; const float *x; const uint8_t *codes, *scales; int seq_len, in_dim, out_dim, panels, per_wave, rows_per_wg, whole; vt_divisor blocks; };
+struct mxr_job { float *y; const float *x; const uint8_t *codes, *scales; int seq_len, in_dim, out_dim, panels, cut_panels, cuts, rows_per_wg, share_log, whole; float *part; unsigned *cnt; };      /* 1 << share_log waves share K */
 
-__global__ void __launch_bounds__(256) vt_mx4_rows_kernel(mxr_job a) {
+template <int G>
+__global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) {
+    constexpr int THREADS = 64 * MXR_WAVES, PP = MXR_PLANES / G;      /* planes of an instruction */
     __shared__ __attribute__((aligned(16))) unsigned char buf0[MXR_WAVES * MXR_PART], buf1[MXR_WAVES * MXR_PART], buf2[MXR_WAVES * MXR_PART], buf3[MXR_WAVES * MXR_PART];
-    __shared__ float red[2][MXR_WAVES][16 * MXR_ROWS];
+    __shared__ float red[2][MXR_WAVES][64 * G];                /* [row of x][weight row] */
+    __shared__ int last;
     extern __shared__ __attribute__((aligned(16))) unsigned char planes[];
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int row0 = (int)blockIdx.x * a.rows_per_wg, rows = min(a.rows_per_wg, a.out_dim - row0);
-    const int p0 = min(wave * a.per_wave, a.panels), p1 = min(p0 + a.per_wave, a.panels), parts = (a.per_wave + 1) / 2, blocks = (rows + 15) / 16, total = blocks * parts;
+    const int share = 1 << a.share_log, groups = MXR_WAVES >> a.share_log, group = wave >> a.share_log;        /* waves that share K, and the blocks that are under way at once */
+    const int k0 = (int)blockIdx.y * a.cut_panels, k1 = min(k0 + a.cut_panels, a.panels), per_wave = (a.cut_panels + share - 1) >> a.share_log;
+    const int p0 = min(k0 + (wave & (share - 1)) * per_wave, k1), p1 = min(p0 + per_wave, k1), parts = (per_wave + 1) / 2, blocks = (rows + 15) / 16;
+    const int total = (blocks + groups - 1) / groups * parts;
+    /* x: block u % nb of row u / nb of the cut.  [panel][group of lanes][instruction][column] of 16 and of 8 bytes, and the scales; column PP row +
+     * plane.  The first blocks are asked for in front of the weights, the next ones while these are split: loads return in order. */
+    const int nb = 4 * (k1 - k0), nc = 4 * a.seq_len + 1, units = a.seq_len * nb;       /* a column more: consecutive blocks lie in different banks */
+    unsigned char *lo8 = planes + nb * nc * 16, *sc = lo8 + nb * nc * 8;
+    const __amdgpu_buffer_rsrc_t xd = vt_buffer(a.x, a.seq_len * a.in_dim * 4);
+    int xr = (int)threadIdx.x / nb, xb = (int)threadIdx.x - xr * nb;
+    const int xr_step = THREADS / nb, xb_step = THREADS - xr_step * nb;
+    vt_f32x16 even, odd, next_even, next_odd;
+    auto ask_x = [&](vt_f32x16 &e, vt_f32x16 &o) __attribute__((always_inline)) { vt_mx4_load32(xd, xr * a.in_dim * 4, xr < a.seq_len ? 128 * k0 + 32 * xb : a.in_dim, a.in_dim, a.whole, e, o); };
+    ask_x(even, odd);
     /* codes: lane i brings piece i % 8 of a line, exchanged so that eight rows' same piece lie in different banks; scales: word i % 2 of row i / 2 */
-    int w_at[2];
-#pragma unroll
-    for (int d = 0; d < 2; d++) { const int r = 8 * d + (lane >> 3); w_at[d] = r * 64 * a.panels + ((lane & 7) ^ (r & 7)) * 16; }
+    const int w_at = (lane >> 3) * 64 * a.panels + ((lane & 7) ^ (lane >> 3)) * 16;                /* and 8 rows on: the same exchange */
     const int s_at = lane < 32 ? (lane >> 1) * 4 * a.panels + (lane & 1) * 4 : 0x7ffffff0;
-    int ask_block = 0, ask_part = 0;                      /* where the next request is: no division */
+    int ask_block = group, ask_part = 0;                      /* where the next request is: no division */
     auto ask = [&](unsigned char *buf) __attribute__((always_inline)) {
         const bool live = ask_block < blocks && p0 + 2 * ask_part < p1;         /* else zeros, which nobody reads */
         const int left = live ? min(16, rows - 16 * ask_block) : 0, panel = live ? p0 + 2 * ask_part : 0;
@@ -146,67 +163,75 @@ __global__ void __launch_bounds__(256) vt_mx4_rows_kernel(mxr_job a) {
         const __amdgpu_buffer_rsrc_t wd = vt_buffer(a.codes + r * 64 * a.panels, left * 64 * a.panels), sd = vt_buffer(a.scales + r * 4 * a.panels, left * 4 * a.panels);
         unsigned char *b = buf + wave * MXR_PART;
 #pragma unroll
-        for (int d = 0; d < 2; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, (__attribute__((address_space(3))) void *)(b + d * 1024), 16, w_at[d], panel * 64, 0, 2);
+        for (int d = 0; d < 2; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, (__attribute__((address_space(3))) void *)(b + d * 1024), 16, w_at + d * 8 * 64 * a.panels, panel * 64, 0, 2);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, (__attribute__((address_space(3))) void *)(b + 2048), 4, s_at, panel * 4, 0, 2);
-        if (++ask_part >= parts) { ask_part = 0; ask_block++; }
+        if (++ask_part >= parts) { ask_part = 0; ask_block += groups; }
     };
     ask(buf0);
     ask(buf1);
     ask(buf2);
-    /* x: block u % 4 P of row u / 4 P.  [panel][group of lanes][column] of 16 and of 8 bytes, and the scales; column 4 row + plane */
-    const int nb = 4 * a.panels, nc = 4 * a.seq_len;
-    unsigned char *lo8 = planes + (size_t)nb * nc * 16, *sc = lo8 + (size_t)nb * nc * 8;
-    for (int u = (int)threadIdx.x; u < a.seq_len * nb; u += 256) {
-        const int r = vt_div(u, a.blocks), blk = u - r * nb;
-        const float *src = a.x + (size_t)r * a.in_dim + 32 * (size_t)blk;
-        vt_f32x16 even, odd;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            f32x4 v, w;
-            const int left = a.in_dim - 32 * blk - 8 * i;
-            vt_mx4_load8(src + 8 * i, left, a.whole && left >= 8, v, w);
-            even[4 * i] = v.x; odd[4 * i] = v.y; even[4 * i + 1] = v.z; odd[4 * i + 1] = v.w;
-            even[4 * i + 2] = w.x; odd[4 * i + 2] = w.y; even[4 * i + 3] = w.z; odd[4 * i + 3] = w.w;
-        }
+    for (int u = THREADS;; u += THREADS) {
+        const int row = xr, at0 = xb * nc + row * PP;
+        xr += xr_step;
+        xb += xb_step;
+        if (xb >= nb) { xb -= nb; xr++; }
+        if (u < units) ask_x(next_even, next_odd);
         vt_u32x6 q[MXR_PLANES];
         unsigned s[MXR_PLANES];
         vt_mx4_planes<MXR_PLANES>(even, odd, q, s);
+        if (row < a.seq_len) {
 #pragma unroll
-        for (int p = 0; p < MXR_PLANES; p++) {
-            const int at = blk * nc + 4 * r + p;
-            *reinterpret_cast<u32x4 *>(planes + (size_t)at * 16) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
-            *reinterpret_cast<u32x2 *>(lo8 + (size_t)at * 8) = u32x2{q[p][4], q[p][5]};
-            sc[at] = (unsigned char)s[p];
+            for (int p = 0; p < MXR_PLANES; p++) {
+                const int at = at0 + (G - 1 - p / PP) * PP * a.seq_len + p % PP;
+                *reinterpret_cast<u32x4 *>(planes + at * 16) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
+                *reinterpret_cast<u32x2 *>(lo8 + at * 8) = u32x2{q[p][4], q[p][5]};
+                sc[at] = (unsigned char)s[p];
+            }
         }
+        if (u >= units) break;
+        even = next_even;
+        odd = next_odd;
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xc07f);                  /* lgkmcnt(0); weights stay on their way */
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int mine = g * nc + min(n, nc - 1);            /* columns past the last repeat it: nobody looks at their sums */
+    const int mine = g * nc + min(n, PP * a.seq_len - 1);        /* columns past the last repeat it: nobody looks at their sums */
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    /* the waves' sums: element v of lane l is weight row 4 (l / 16) + v, column l % 16; the planes of a row of x are a quad of lanes */
-    auto finish = [&](int block) __attribute__((always_inline)) {
-        float *to = red[block & 1][wave];
+    float *y = a.cuts > 1 ? a.part + (size_t)blockIdx.y * a.seq_len * a.out_dim : a.y;
+    /* the waves' sums: element v of lane l is weight row 4 (l / 16) + v, column l % 16; a row's planes of an instruction are PP lanes */
+    auto finish = [&](int turn) __attribute__((always_inline)) {
+        f32x4 sum = acc;
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            float s = acc[v];
-            s += vt_dpp<0xB1>(s);
-            s += vt_dpp<0x4E>(s);
-            if ((n & 3) == 0) to[(n >> 2) * 16 + 4 * g + v] = s;
+            if (PP > 1) sum[v] += vt_dpp<0xB1>(sum[v]);
+            if (PP > 2) sum[v] += vt_dpp<0x4E>(sum[v]);
         }
+        if (n % PP == 0) *reinterpret_cast<f32x4 *>(&red[turn & 1][wave][n / PP * 16 + 4 * g]) = sum;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0xc07f);
         __builtin_amdgcn_s_barrier();                    /* the other half of red is read before a wave is through the next one */
         asm volatile("" ::: "memory");
-        const int t = (int)threadIdx.x, s = t >> 4, r = 16 * block + (t & 15);
+        /* the first 64 G threads of a group of waves: row of x, weight row */
+        const int t = (int)threadIdx.x & (64 * share - 1), s = t >> 4, r = 16 * (turn * groups + group) + (t & 15);
         if (s < a.seq_len && r < rows) {
-            const float *from = &red[block & 1][0][t];
-            a.y[(size_t)s * a.out_dim + row0 + r] = (from[0] + from[16 * MXR_ROWS]) + (from[2 * 16 * MXR_ROWS] + from[3 * 16 * MXR_ROWS]);
+            const float *from = &red[turn & 1][group << a.share_log][t];
+            float p[4];
+#pragma unroll
+            for (int w = 0; w < 4; w++) p[w] = from[w * 64 * G];
+            float v = (p[0] + p[2]) + (p[1] + p[3]);
+            if (share > 4) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) p[w] = from[(4 + w) * 64 * G];
+                v += (p[0] + p[2]) + (p[1] + p[3]);
+            }
+            float *at = y + (size_t)s * a.out_dim + row0 + r;
+            if (a.cuts > 1) vt_stc(at, v);
+            else *at = v;
         }
-        acc = f32x4{0.f, 0.f, 0.f, 0.f};
     };
-    int block = 0, part = 0;
+    int turn = 0, part = 0;
     auto item = [&](const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x0f70 | 6);          /* vmcnt: two later parts may be on their way */
@@ -219,13 +244,19 @@ __global__ void __launch_bounds__(256) vt_mx4_rows_kernel(mxr_job a) {
             const int panel = p0 + 2 * part + k;
             if (panel >= p1) break;
             const u32x4 w = *reinterpret_cast<const u32x4 *>(b + n * 128 + ((4 * k + g) ^ (n & 7)) * 16);
-            const int ws = b[2048 + n * 8 + 4 * k + g], at = panel * 4 * nc + mine;
-            const u32x4 x4 = *reinterpret_cast<const u32x4 *>(planes + (size_t)at * 16);
-            const u32x2 x2 = *reinterpret_cast<const u32x2 *>(lo8 + (size_t)at * 8);
-            const vt_u32x6 xq = {x4.x, x4.y, x4.z, x4.w, x2.x, x2.y};
-            acc = acc + __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vt_mfma_e2m1(w), vt_mfma_e2m3(xq), (f32x4{0.f, 0.f, 0.f, 0.f}), VT_MFMA_E2M1, VT_MFMA_E2M3, 0, ws, 0, (int)sc[at]);
+            const int ws = b[2048 + n * 8 + 4 * k + g];
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                const int at = (panel - k0) * 4 * nc + i * PP * a.seq_len + mine;
+                const u32x4 x4 = *reinterpret_cast<const u32x4 *>(planes + at * 16);
+                const u32x2 x2 = *reinterpret_cast<const u32x2 *>(lo8 + at * 8);
+                const vt_u32x6 xq = {x4.x, x4.y, x4.z, x4.w, x2.x, x2.y};
+                sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vt_mfma_e2m1(w), vt_mfma_e2m3(xq), sum, VT_MFMA_E2M1, VT_MFMA_E2M3, 0, ws, 0, (int)sc[at]);
+            }
+            acc = acc + sum;
         }
-        if (++part == parts) { part = 0; finish(block++); }
+        if (++part == parts) { part = 0; finish(turn++); }
     };
     for (int t = 0; t < total; t += 4) {                 /* every wave goes through the same parts and barriers, whatever it has of them */
         item(buf0, buf3);
@@ -236,12 +267,32 @@ __global__ void __launch_bounds__(256) vt_mx4_rows_kernel(mxr_job a) {
         if (t + 3 >= total) break;
         item(buf3, buf2);
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);                  /* nothing arrives in the buffers any more */
+    __builtin_amdgcn_s_waitcnt(0x0f70);                  /* nothing arrives in the buffers any more, and what was stored is acknowledged */
+    if (a.cuts == 1) return;
+    __syncthreads();
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(a.cnt + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(a.cuts - 1);
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) vt_stc_u32(a.cnt + blockIdx.x, 0u);    /* ready for the next launch */
+    for (int s = 0; s < a.seq_len; s++)
+        for (int r = (int)threadIdx.x; r < rows; r += THREADS) {
+            const size_t at = (size_t)s * a.out_dim + row0 + r;
+            float v = 0.f;
+            for (int c = 0; c < a.cuts; c += 4) {
+                float p[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) p[k] = vt_ldc(a.part + (size_t)min(c + k, a.cuts - 1) * a.seq_len * a.out_dim + at);
+#pragma unroll
+                for (int k = 0; k < 4; k++) v = c + k < a.cuts ? __fadd_rn(v, p[k]) : v;
+            }
+            a.y[at] = v;
+        }
 }
 
-#define MXR_LDS_MOST (160 * 1024)         /* of a workgroup, static and x's planes; from half of it on a CU holds one */
-#define MXR_LDS (MXR_WAVES * MXR_PART * 4 + 2 * MXR_WAVES * 16 * MXR_ROWS * 4)
-static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * panels * 4 * seq_len * 25; }
+/* LDS: four buffers and the sums of eight waves, 25 bytes a block of 32 values of x and plane */
+#define MXR_LDS_MOST (160 * 1024)
+static size_t mxr_lds(int g) { return (size_t)MXR_WAVES * (MXR_PART * 4 + 2 * 64 * g * 4) + 256; }
+static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * panels * (4 * seq_len + 1) * 25; }
 
 /* ---- linear layer: more rows -----------------------------------------------------------------------------------------
  * x is split into its planes first, [column tile of 32 rows][64 columns of W's K][plane] in the order of the matrix instruction's operand, 16
@@ -252,19 +303,34 @@ static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * pan
  * vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts are added by a kernel of their own. */
 #define MXT_STEP (MXR_PLANES * 1536 + 256)               /* bytes of 32 rows x 64 columns of x */
 
+/* A wave has 32 rows by 64 columns; they go through LDS so that its loads are lines (a lane's own 128 bytes come in eight pieces, and with twenty waves on a CU the
+ * rest of a line is gone from the first cache by the time of the next piece). */
 __global__ void __launch_bounds__(256) vt_mx4_planes_kernel(unsigned char *out, const float *x, int seq_len, int in_dim, int panels, int tiles, int whole) {
-    const int unit = (int)(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = (int)threadIdx.x & 63;
+    constexpr int ROW = 64 + 4;                          /* floats: eight rows' same piece lie in different banks */
+    __shared__ __attribute__((aligned(16))) float turn[4][32 * ROW];
+    const int wave = (int)(threadIdx.x >> 6), unit = (int)blockIdx.x * 4 + wave, lane = (int)threadIdx.x & 63;
     if (unit >= tiles * 2 * panels) return;
     /* [panel][tile][half] */
-    const int panel = unit / (2 * tiles), rest = unit - panel * 2 * tiles, row = (rest >> 1) * 32 + (lane & 31), at = 128 * panel + 64 * (rest & 1) + 32 * (lane >> 5);
+    const int panel = unit / (2 * tiles), rest = unit - panel * 2 * tiles, at = 128 * panel + 64 * (rest & 1), row0 = (rest >> 1) * 32;
+    const __amdgpu_buffer_rsrc_t xd = vt_buffer(x + (size_t)row0 * in_dim, min(32, seq_len - row0) * in_dim * 4);      /* zeros past the last row */
+    if (whole) {
+        f32x4 v[8];
+        const int c = at + 4 * (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = vt_buffer_ld4(xd, c < in_dim ? ((4 * i + (lane >> 4)) * in_dim + c) * 4 : 0x7ffffff0);
+#pragma unroll
+        for (int i = 0; i < 8; i++) *reinterpret_cast<f32x4 *>(&turn[wave][(4 * i + (lane >> 4)) * ROW + 4 * (lane & 15)]) = v[i];
+    } else {
+#pragma unroll 8
+        for (int i = 0; i < 32; i++)
+            turn[wave][i * ROW + lane] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(xd, at + lane < in_dim ? (i * in_dim + at + lane) * 4 : 0x7ffffff0, 0, 0));
+    }
+    __builtin_amdgcn_wave_barrier();                     /* the wave's own LDS, in order */
     vt_f32x16 even, odd;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        f32x4 v, w;
-        const int left = row < seq_len ? in_dim - at - 8 * i : 0;
-        vt_mx4_load8(x + (size_t)row * in_dim + at + 8 * i, left, whole && left >= 8, v, w);
-        even[4 * i] = v.x; odd[4 * i] = v.y; even[4 * i + 1] = v.z; odd[4 * i + 1] = v.w;
-        even[4 * i + 2] = w.x; odd[4 * i + 2] = w.y; even[4 * i + 3] = w.z; odd[4 * i + 3] = w.w;
+    for (int i = 0; i < 8; i++) {
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(&turn[wave][(lane & 31) * ROW + 32 * (lane >> 5) + 4 * i]);
+        even[2 * i] = v.x; odd[2 * i] = v.y; even[2 * i + 1] = v.z; odd[2 * i + 1] = v.w;
     }
     vt_u32x6 q[MXR_PLANES];
     unsigned s[MXR_PLANES], all = 0;
@@ -369,34 +435,45 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
     }
 }
 
-/* Tiles: (weight rows, rows of x, workgroups that a CU holds, us per panel and workgroup when all slots are taken) */
-struct mxt_tile { int bm, bn, per_cu; float panel_us; };
-static const mxt_tile mxt_tiles[] = {{256, 128, 1, 1.25f}, {128, 64, 2, 0.75f}, {128, 32, 3, 0.60f}};
+/* Tiles: weight rows, rows of x, workgroups that a CU holds, and us per panel with one, two, three of them on it (from runs of one cut on part of the chip and on all of
+ * it: 226 x 3072 x 9216, 1531 x 9216 x 3072). */
+struct mxt_tile { int bm, bn, per_cu; float panel_us[3]; };
+static const mxt_tile mxt_tiles[] = {{256, 128, 1, {1.9f}}, {128, 64, 2, {0.76f, 1.21f}}, {128, 32, 3, {0.55f, 0.85f, 1.25f}}};
 #define MXT_MAX_CUTS 16
 
+/* The tile and the cuts of K with the least time by these figures.  us, measured and (planned): 226 x 3072 x 9216 36 (128 x 64 in 4 cuts; others 37 to 130), 1531 x 9216 x 3072
+ * 112 (256 x 128 in one; 128 to 154 on the others), 64 x 9216 x 3072 19.5 (128 x 32 in 3), 1000 x 3072 x 4096 51 (128 x 64 in one; 53 and more). */
 static void mxt_plan(int n_cu, int seq_len, int out_dim, int panels, int *best_tile, int *best_cuts) {
     double best = 1e30;
     for (int t = 0; t < 3; t++) {
         const mxt_tile &k = mxt_tiles[t];
-        const double tiles = (double)((out_dim + k.bm - 1) / k.bm) * ((seq_len + k.bn - 1) / k.bn);
+        const double tiles = ceil((double)out_dim / k.bm) * ceil((double)seq_len / k.bn);
         for (int cuts = 1; cuts <= MXT_MAX_CUTS && cuts <= panels; cuts++) {
-            const double rounds = ceil(tiles * cuts / ((double)n_cu * k.per_cu)), us = rounds * ((panels + cuts - 1) / cuts * (double)k.panel_us + 2.0) +
-                                  (cuts > 1 ? 3.0 + (double)seq_len * out_dim * 4.0 * (2 * cuts + 1) / 4.0e6 : 0.0);
+            const double wgs = tiles * cuts, full = floor(wgs / ((double)n_cu * k.per_cu)), rest = wgs - full * n_cu * k.per_cu;
+            const int each = (panels + cuts - 1) / cuts, beside = (int)ceil(rest / n_cu);
+            const double us = each * (full * k.panel_us[k.per_cu - 1] + (beside ? k.panel_us[beside - 1] : 0.0)) + full +
+                              (cuts > 1 ? 2.0 + (double)seq_len * out_dim * 4.0 * (2 * cuts + 1) / 5.0e6 : 0.0);
             if (us < best) { best = us; *best_tile = t; *best_cuts = cuts; }
         }
     }
 }
 
-int vt_mx4_prepare(void) {
-    return vt_check(hipFuncSetAttribute((const void *)vt_mx4_rows_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MXR_LDS_MOST - MXR_LDS), "tts_hip_linear_mx4: LDS");
+template <int G> static int mxr_prepare(void) {
+    return vt_check(hipFuncSetAttribute((const void *)vt_mx4_rows_kernel<G>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(MXR_LDS_MOST - mxr_lds(G))), "tts_hip_linear_mx4: LDS");
 }
+int vt_mx4_prepare(void) { return mxr_prepare<1>() || mxr_prepare<2>() ? -1 : 0; }
 
 static int mx4_linear_rows(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim, int whole) {
-    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = panels_of(in_dim);
-    const size_t lds = mxr_planes_bytes(seq_len, panels);
-    const int wgs = n_cu * (MXR_LDS + lds > MXR_LDS_MOST / 2 ? 1 : 2), rows_per_wg = (int)(((long long)out_dim + wgs - 1) / wgs);
-    mxr_job a = {d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, panels, (panels + MXR_WAVES - 1) / MXR_WAVES, rows_per_wg, whole, vt_divisor_of(4 * panels, 16ll * panels)};
-    hipLaunchKernelGGL(vt_mx4_rows_kernel, dim3((out_dim + rows_per_wg - 1) / rows_per_wg), dim3(256), lds, g_vt.stream, a);
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = panels_of(in_dim), g = seq_len <= 4 ? 1 : 2;
+    const int most = (int)((MXR_LDS_MOST - mxr_lds(g)) / mxr_planes_bytes(seq_len, 1)), cuts = (panels + most - 1) / most, wgs = n_cu / cuts > 0 ? n_cu / cuts : 1;
+    mxr_job a = {d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, panels, (panels + cuts - 1) / cuts, cuts, (int)(((long long)out_dim + wgs - 1) / wgs), 2, whole, NULL, g_vt.d_mx4_cnt};
+    if (a.rows_per_wg <= 16) a.share_log = 3;          /* no second block for the other waves */
+    a.cuts = (panels + a.cut_panels - 1) / a.cut_panels;
+    if (a.cuts > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)a.cuts * seq_len * out_dim))) return -1;
+    const dim3 grid((out_dim + a.rows_per_wg - 1) / a.rows_per_wg, a.cuts);
+    const size_t lds = mxr_planes_bytes(seq_len, a.cut_panels);
+    if (g == 1) hipLaunchKernelGGL(vt_mx4_rows_kernel<1>, grid, dim3(64 * MXR_WAVES), lds, g_vt.stream, a);
+    else hipLaunchKernelGGL(vt_mx4_rows_kernel<2>, grid, dim3(64 * MXR_WAVES), lds, g_vt.stream, a);
     return 0;
 }
 
@@ -426,7 +503,7 @@ extern "C" int tts_hip_linear_mx4(float *d_y, const float *d_x, const uint8_t *d
     if (in_dim > 1 << 23) { vt_set_error("%s: %d columns (1 .. 2^23)", who, in_dim); return -1; }
     if (!vt_mx4_ready(who)) return -1;
     const int whole = ((uintptr_t)d_x & 15) == 0 && in_dim % 4 == 0;
-    if (seq_len <= MXR_ROWS && MXR_LDS + mxr_planes_bytes(seq_len, panels_of(in_dim)) <= MXR_LDS_MOST) {
+    if (seq_len <= MXR_ROWS) {
         if (mx4_linear_rows(d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, whole)) return -1;
     } else {
         /* so many rows at a time that the work area stays small beside the operands, and the tiles in one launch countable */

@@ -21,7 +21,7 @@
 #define VT_SEM_PADDED 8320
 #define VT_SEM_VALID_END 8194     /* 2 special + 8192 codes */
 
-#define VT_KV4_COUNTERS 16384     /* heads times tiles of columns whose rows several workgroups share */
+#define VT_MX4_COUNTERS 16384     /* tiles, or heads times tiles of columns, that several workgroups share */
 #define VT_PIN_ROWS 2048          /* 25 MB */
 
 /* Second copy of a backbone layer's four matrices, in the order the 128 x 256 tile product reads them
@@ -88,7 +88,7 @@ struct vt_state {
     /* generic scratch (prefill / acoustic / linear) */
     void *d_scratch;
     size_t scratch_bytes;
-    unsigned *d_kv4_cnt;          /* 4-bit attention: workgroups of a head and tile of columns that have left their part; zero between launches */
+    unsigned *d_mx4_cnt;          /* 4-bit operators: workgroups that have left their part of a tile or head; zero between launches */
     void *d_kv_img;               /* prefill attention: tile images of one layer's K and V */
     size_t kv_img_bytes;
 
