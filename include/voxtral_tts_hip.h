@@ -363,8 +363,8 @@ int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cache, int n_r
 /* Causal attention over the cache: query i of Q [seq_len, n_heads * head_dim] sees the rows 0 .. start_pos + i,
  * which hold its own keys and values too (append first); out like Q, on 16 bytes both.  n_heads is a multiple
  * of n_kv_heads.  A decode step is seq_len 1; what tts_hip_causal_attention_decode and _prefill are for an
- * fp32 cache.  A row that a query does not see changes nothing in its result, whatever it holds.  At most 2^25 rows,
- * 2^28 queries times heads per kv head, and 65535 kv heads.  Where several workgroups share a head's rows
+ * fp32 cache.  A row that a query does not see changes nothing in its result, whatever it holds.  At most 2^24 rows,
+ * 65535 kv heads and 2^19 heads on each.  Where several workgroups share a head's rows
  * their parts meet in the library's work area, which grows by allocation when a call needs more than any before it. */
 int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_hip_kv4_t *cache, int seq_len,
                           int start_pos, int n_heads, float scale);

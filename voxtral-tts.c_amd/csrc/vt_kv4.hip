@@ -104,7 +104,6 @@ typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
 #define KV4_V_EXP 13                       /* .. and values up to 6 times 2^13 are fp16 */
 #define KV4_COLS 16
 #define KV4_MAX_CHUNKS 64
-#define KV4_STREAM_COLS 32                 /* up to so many columns */
 
 struct kv4_job {
     float *out;
@@ -227,6 +226,8 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
     most = (unsigned)vt_wave_max((float)most);
     nan = __any((int)nan);
     const int shift = 127 + KV4_V_EXP - (int)most;
+    float minus = -1.f;                                   /* a number that the compiler does not know: fp16 to fp32 and the difference are one instruction */
+    asm("" : "+v"(minus));
     float m = -3.402823466e38f, l = 0.f;                  /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
     f32x4 o[CHUNKS * CD];
 #pragma unroll
@@ -262,10 +263,15 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
 #pragma unroll
                 for (int v = 0; v < 4; v++) s[kt][v] = first + 16 * kt + 4 * g + v < see ? s[kt][v] : -INFINITY;
         }
-        float top = fmaxf(fmaxf(s[0].x, s[1].x), m);
+        float top = m;                                    /* a NaN stays one: who sees it answers NaN */
 #pragma unroll
-        for (int v = 1; v < 4; v++) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
-        top = vt_rows_max(top);
+        for (int v = 0; v < 4; v++) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][v]), s[1][v]);
+        {
+            f32x2 r = vt_swap16(top, top);
+            top = __builtin_elementwise_maximum(r.x, r.y);
+            r = vt_swap32(top, top);
+            top = __builtin_elementwise_maximum(r.x, r.y);
+        }
         if (__any(top != m)) {
             const float less = __builtin_amdgcn_exp2f(m - top);
             l *= less;
@@ -281,7 +287,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
             l += p0 + p1;
             const vt_f16x2 hi2 = __builtin_convertvector((f32x2{p0, p1}), vt_f16x2);
             hi4[e] = __builtin_bit_cast(unsigned, hi2);
-            lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{__fsub_rn(p0, (float)hi2.x), __fsub_rn(p1, (float)hi2.y)}), vt_f16x2));
+            lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{fmaf((float)hi2.x, minus, p0), fmaf((float)hi2.y, minus, p1)}), vt_f16x2));
         }
         const vt_f16x8 ph = __builtin_bit_cast(vt_f16x8, hi4), pl = __builtin_bit_cast(vt_f16x8, lo4);
 #pragma unroll
@@ -437,7 +443,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
 struct kv4_tile_job { kv4_job a; int run, tiles_of_cols, most_parts; };
 
 template <int HP>
-__global__ void __launch_bounds__(64 * KV4_TILE_WAVES, HP <= 2 ? 2 : 1) vt_kv4_tile_kernel(tts_hip_kv4_t c, kv4_tile_job j) {
+__global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(tts_hip_kv4_t c, kv4_tile_job j) {
     constexpr int HD = 64 * HP, ROW = 32 * HP, THREADS = 64 * KV4_TILE_WAVES, UNITS = 128 * HP, UN = (UNITS + THREADS - 1) / THREADS, DT = 2 * HP;
     constexpr int KB = 64 * ROW, SB = KB + UNITS, VB = SB;      /* K rows, their scales, V's operands */
     __shared__ __attribute__((aligned(16))) unsigned char buf[2][VB + 64 * HD * 2];
@@ -445,8 +451,9 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, HP <= 2 ? 2 : 1) vt_kv4_t
     __shared__ int last;
     const kv4_job &a = j.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5, h = (int)blockIdx.y;
-    /* the columns that see most first */
-    const int ct = j.tiles_of_cols - 1 - (int)blockIdx.x / j.most_parts, part = (int)blockIdx.x % j.most_parts;
+    /* The columns that see most first, and their last parts, which others do not have, before these.  (Neighbours go to different XCDs: with the parts of a tile side by
+     * side every second XCD had half as many.) */
+    const int ahead = (int)blockIdx.x / j.tiles_of_cols, part = j.most_parts - 1 - ahead, ct = (ahead + 1) * j.tiles_of_cols - 1 - (int)blockIdx.x;
     const int c0 = ct * KV4_TILE, nc = min(KV4_TILE, a.cols - c0);
     const int end = a.start + vt_div(c0 + nc - 1, a.group) + 1, parts = ((end + 63) / 64 + j.run - 1) / j.run;
     if (part >= parts) return;
@@ -476,29 +483,40 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, HP <= 2 ? 2 : 1) vt_kv4_t
             }
         }
     };
-    load(0);
-    vt_u32x6 q[HP][KV4_PLANES];
-    unsigned qs[HP][KV4_PLANES];
+    /* queries and the first scales of values are asked for in front of the first rows: loads return in order */
+    f32x4 q4[HP][8];
     {
         const float *src = a.Q + ((size_t)qi * a.n_heads + (size_t)h * a.group.d + (cc - qi * a.group.d)) * HD + 32 * g;
 #pragma unroll
-        for (int k = 0; k < HP; k++) {
-            vt_f32x16 even, odd;
+        for (int k = 0; k < HP; k++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(src + 64 * k + 4 * i) * a.scale;
-                even[2 * i] = v.x; odd[2 * i] = v.y; even[2 * i + 1] = v.z; odd[2 * i + 1] = v.w;
-            }
-            vt_mx4_planes<KV4_PLANES>(even, odd, q[k], qs[k]);
+            for (int i = 0; i < 8; i++) q4[k][i] = *reinterpret_cast<const f32x4 *>(src + 64 * k + 4 * i);
+    }
+    unsigned char seen[8];
+    auto ask_scales = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) seen[e] = __builtin_amdgcn_raw_buffer_load_b8(vsd, i + e * THREADS, 0, 0);      /* zeros past the last */
+    };
+    ask_scales(tid);
+    load(0);
+    vt_u32x6 q[HP][KV4_PLANES];
+    unsigned qs[HP][KV4_PLANES];
+#pragma unroll
+    for (int k = 0; k < HP; k++) {
+        vt_f32x16 even, odd;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const f32x4 v = q4[k][i] * a.scale;
+            even[2 * i] = v.x; odd[2 * i] = v.y; even[2 * i + 1] = v.z; odd[2 * i + 1] = v.w;
         }
+        vt_mx4_planes<KV4_PLANES>(even, odd, q[k], qs[k]);
     }
     unsigned most = 0, nan = 0;
-    for (int i = tid; i < rows * DT; i += THREADS * 8) {
-        unsigned char b[8];
+    for (int i = tid;;) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) b[e] = __builtin_amdgcn_raw_buffer_load_b8(vsd, i + e * THREADS, 0, 0);      /* zeros past the last */
-#pragma unroll
-        for (int e = 0; e < 8; e++) { nan |= b[e] == 255; most = max(most, b[e] == 255 ? 0u : (unsigned)b[e]); }
+        for (int e = 0; e < 8; e++) { nan |= seen[e] == 255; most = max(most, seen[e] == 255 ? 0u : (unsigned)seen[e]); }
+        if ((i += THREADS * 8) - tid >= rows * DT) break;
+        ask_scales(i);
     }
     most = (unsigned)vt_wave_max((float)most);
     if (lane == 0) scan_most[wave] = most;
@@ -545,6 +563,8 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, HP <= 2 ? 2 : 1) vt_kv4_t
             }
         }
     };
+    float minus = -1.f;
+    asm("" : "+v"(minus));
     float m = -3.402823466e38f, l = 0.f;
     vt_f32x16 o[DT];
 #pragma unroll
@@ -581,10 +601,10 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, HP <= 2 ? 2 : 1) vt_kv4_t
 #pragma unroll
                     for (int v = 0; v < 16; v++) s[kt][v] = first + 32 * kt + 8 * (v >> 2) + 4 * g + (v & 3) < see ? s[kt][v] : -INFINITY;
             }
-            float top = m;
+            float top = m;                                /* a NaN stays one: who sees it answers NaN */
 #pragma unroll
-            for (int v = 0; v < 16; v++) top = fmaxf(top, fmaxf(s[0][v], s[1][v]));
-            { const f32x2 r = vt_swap32(top, top); top = fmaxf(r.x, r.y); }
+            for (int v = 0; v < 16; v++) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][v]), s[1][v]);
+            { const f32x2 r = vt_swap32(top, top); top = __builtin_elementwise_maximum(r.x, r.y); }
             if (__any(top != m)) {
                 const float less = __builtin_amdgcn_exp2f(m - top);
                 l *= less;
@@ -602,7 +622,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, HP <= 2 ? 2 : 1) vt_kv4_t
                     l += p0 + p1;
                     const vt_f16x2 hi2 = __builtin_convertvector((f32x2{p0, p1}), vt_f16x2);
                     hi4[e] = __builtin_bit_cast(unsigned, hi2);
-                    lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{__fsub_rn(p0, (float)hi2.x), __fsub_rn(p1, (float)hi2.y)}), vt_f16x2));
+                    lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{fmaf((float)hi2.x, minus, p0), fmaf((float)hi2.y, minus, p1)}), vt_f16x2));
                 }
                 const vt_f16x8 ph = __builtin_bit_cast(vt_f16x8, hi4), pl = __builtin_bit_cast(vt_f16x8, lo4);
 #pragma unroll
@@ -695,36 +715,36 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, HP <= 2 ? 2 : 1) vt_kv4_t
 template <int HP, int WAVES>
 static int kv4_stream(const tts_hip_kv4_t *cache, kv4_job a) {
     const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
-    const long long cts = (a.cols + KV4_COLS - 1) / KV4_COLS, heads = cache->n_kv_heads, tiles = ((long long)a.start + a.seq + 31) / 32;
-    long long chunks = (8 * n_cu / WAVES + cts * heads - 1) / (cts * heads);
-    if (chunks > KV4_MAX_CHUNKS) chunks = KV4_MAX_CHUNKS;
-    if (chunks > (tiles + WAVES - 1) / WAVES) chunks = (tiles + WAVES - 1) / WAVES;
-    if (cts * heads > VT_MX4_COUNTERS) chunks = 1;
-    a.per_wave = (int)((tiles + chunks * WAVES - 1) / (chunks * WAVES));
+    const long long cts = (a.cols + KV4_COLS - 1) / KV4_COLS, heads = cache->n_kv_heads, wgs = cts * heads, tiles = ((long long)a.start + a.seq + 31) / 32, slots = (long long)n_cu * (HP == 1 ? 2 : 1);
+    /* Workgroups per head and tile of columns: the number that takes the least time at 3.5 us a round of workgroups, 1.2 us a tile of 128 values a row and 2.8 us for adding parts.
+     * (us at 1 / 2 / 4 / 8 / 32 of them: 1 query behind 300 rows 7.4 / 8.5 / 8.5 / 8.5 / 8.5, behind 1999 13.4 / 11.8 / 9.8 / 9.1 / 9.0, behind 65535 264 / 137 / 73 / 41 / 20, 37 queries
+     * behind 4000, ten tiles of columns, 24 / 20 / 27 / 35 and at 3 18.) */
+    long long best = 1;
+    float least = 1e30f;
+    for (long long chunks = 1; chunks <= KV4_MAX_CHUNKS && (chunks == 1 || (wgs <= VT_MX4_COUNTERS && chunks <= (tiles + WAVES - 1) / WAVES)); chunks++) {
+        const float each = (float)((tiles + chunks * WAVES - 1) / (chunks * WAVES)), rounds = (float)((wgs * chunks + slots - 1) / slots);
+        const float us = rounds * (3.5f + 0.6f * HP * each) + (chunks > 1 ? 2.8f : 0.f);
+        if (us < least) { least = us; best = chunks; }
+    }
+    a.per_wave = (int)((tiles + best * WAVES - 1) / (best * WAVES));
     a.chunks = (int)((tiles + (long long)a.per_wave * WAVES - 1) / ((long long)a.per_wave * WAVES));
     if (a.chunks > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)cts * heads * a.chunks * KV4_COLS * (cache->head_dim + 4)))) return -1;
     hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)a.chunks, (unsigned)cts, (unsigned)heads), dim3(64 * WAVES), 0, g_vt.stream, *cache, a);
     return 0;
 }
 
-/* `run` tiles of 64 rows a workgroup */
 template <int HP>
 static int kv4_tiles(const tts_hip_kv4_t *cache, const kv4_job &a) {
-    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, per_cu = HP <= 2 ? 2 : 1;
     kv4_tile_job j = {a, 0, (a.cols + KV4_TILE - 1) / KV4_TILE, 1};
-    const long long heads = cache->n_kv_heads, last = ((long long)a.start + a.seq + 63) / 64, first = (a.start + 64) / 64;
-    const long long total = heads * j.tiles_of_cols * ((first + last + 1) / 2);
-    long long run = total / ((long long)n_cu * per_cu) + 1;
+    const long long heads = cache->n_kv_heads, last = ((long long)a.start + a.seq + 63) / 64, wgs = heads * j.tiles_of_cols, slots = 2ll * (g_vt.n_cu > 0 ? g_vt.n_cu : 256);
+    /* as many parts as there is room for at once, of four tiles and more (400 queries and no rows before: 20 us whole or in runs of 8, 21 in runs of 4; 1000 behind 1000 rows: 69 whole,
+     * 66 in runs of 16, two workgroups on a CU each, 74 to 96 in shorter ones) */
+    long long run = wgs < slots && wgs <= VT_MX4_COUNTERS ? (last + slots / wgs - 1) / (slots / wgs) : last;
     if (run < 4) run = 4;
-    if (heads * j.tiles_of_cols > VT_MX4_COUNTERS) run = last;
-    if (run * KV4_MAX_PARTS < last) run = (last + KV4_MAX_PARTS - 1) / KV4_MAX_PARTS;
-    if (run > 1 << 16) {
-        run = 1 << 16;                                   /* a descriptor's 31 bits */
-        if (heads * j.tiles_of_cols > VT_MX4_COUNTERS && run < last) { vt_set_error("tts_hip_kv4_attention: %d queries behind %d rows are too many for one call", a.seq, a.start); return -1; }
-    }
+    if (run * KV4_MAX_PARTS < last && wgs <= VT_MX4_COUNTERS) run = (last + KV4_MAX_PARTS - 1) / KV4_MAX_PARTS;
     j.run = (int)run;
     j.most_parts = (int)((last + run - 1) / run);
-    if (j.most_parts > 1 && !(j.a.part = (float *)vt_scratch((size_t)heads * j.tiles_of_cols * j.most_parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
+    if (j.most_parts > 1 && !(j.a.part = (float *)vt_scratch((size_t)wgs * j.most_parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
     hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)(j.tiles_of_cols * (long long)j.most_parts), (unsigned)heads), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, *cache, j);
     return 0;
 }
@@ -736,12 +756,22 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
     if (!cache_ok(who, cache, 0, (long long)start_pos + seq_len)) return -1;
     if (n_heads < 1 || n_heads % cache->n_kv_heads) { vt_set_error("%s: %d heads on %d kv heads", who, n_heads, cache->n_kv_heads); return -1; }
     const int group = n_heads / cache->n_kv_heads, HP = cache->head_dim / 64;
-    const long long cols = (long long)seq_len * group;
-    if (cols > 1 << 28 || cache->n_kv_heads > 65535 || (long long)start_pos + seq_len > 1 << 25) { vt_set_error("%s: %d queries of %d heads on %d behind %d rows are too many for one call", who, seq_len, n_heads, cache->n_kv_heads, start_pos); return -1; }
+    if (cache->n_kv_heads > 65535 || group > 1 << 19 || (long long)start_pos + seq_len > 1 << 24) {
+        vt_set_error("%s: %d queries of %d heads on %d behind %d rows are too many", who, seq_len, n_heads, cache->n_kv_heads, start_pos);
+        return -1;
+    }
     if (!vt_mx4_ready(who)) return -1;
-    kv4_job a = {d_out, d_Q, seq_len, start_pos, n_heads, (int)cols, 0, 1, vt_divisor_of(group, cols), scale * 1.44269504f, NULL, g_vt.d_mx4_cnt};
-    if (cols > KV4_STREAM_COLS) {
-        if (HP == 1 ? kv4_tiles<1>(cache, a) : HP == 2 ? kv4_tiles<2>(cache, a) : HP == 3 ? kv4_tiles<3>(cache, a) : kv4_tiles<4>(cache, a)) return -1;
-    } else if (HP == 1 ? kv4_stream<1, 8>(cache, a) : HP == 2 ? kv4_stream<2, 8>(cache, a) : HP == 3 ? kv4_stream<3, 4>(cache, a) : kv4_stream<4, 4>(cache, a)) return -1;
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, most = (1 << 19) / group;        /* queries of a launch: their tiles of columns are a dimension of the grid */
+    for (int s = 0; s < seq_len; s += most) {
+        const int n = seq_len - s < most ? seq_len - s : most, cols = n * group;
+        const size_t at = (size_t)s * n_heads * cache->head_dim;
+        const kv4_job a = {d_out + at, d_Q + at, n, start_pos + s, n_heads, cols, 0, 1, vt_divisor_of(group, cols), scale * 1.44269504f, NULL, g_vt.d_mx4_cnt};
+        /* Many columns: from two rounds of the other kernel's workgroups on (200 queries behind 300 rows, 400 of them: 22 us and 16; 400 queries and no rows before, 800: 20 and 28; 1531:
+         * 65 and 120), and for heads of up to 128 values, whose results and queries leave two waves of a SIMD their registers (500 behind 500 rows with 256: 54 and 40). */
+        int bad;
+        if (HP <= 2 && (long long)((cols + KV4_COLS - 1) / KV4_COLS) * cache->n_kv_heads > 2ll * n_cu) bad = HP == 1 ? kv4_tiles<1>(cache, a) : kv4_tiles<2>(cache, a);
+        else bad = HP == 1 ? kv4_stream<1, 8>(cache, a) : HP == 2 ? kv4_stream<2, 8>(cache, a) : HP == 3 ? kv4_stream<3, 4>(cache, a) : kv4_stream<4, 4>(cache, a);
+        if (bad) return -1;
+    }
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
