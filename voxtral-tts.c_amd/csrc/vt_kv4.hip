@@ -105,14 +105,16 @@ typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
 #define KV4_COLS 16
 #define KV4_MAX_CHUNKS 64
 
+/* 104 bytes: a launch with 112 and more, or one that asks for the size of its grid, takes the host 0.9 us longer (of 2.7) */
 struct kv4_job {
+    const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
     float *out;
     const float *Q;
-    int seq, start, n_heads, cols, per_wave, chunks;     /* columns; tiles of 32 rows per wave; workgroups per head and tile of columns */
+    unsigned char *part;
+    unsigned *cnt;
+    int max_rows, start, n_heads, cols, run, parts, tiles;       /* columns, tiles of them; tiles of 32 rows a wave, of 64 a workgroup; workgroups per head and tile of columns */
     vt_divisor group;
     float scale;                                         /* times log2 e */
-    float *part;
-    unsigned *cnt;
 };
 
 /* column / heads per kv head, for fewer than 2^20 columns: (c + 1/2) / d is no nearer to a whole number than 1 / 2 d, and c 2^-22 / d off */
@@ -139,7 +141,7 @@ template <int HP> static __device__ __forceinline__ int kv4_swizzle(int row, int
  * 16 CD, for the eight keys that its group of 16 lanes has weights of.  Most of a short call is instructions that run once, from a cold instruction cache: the code
  * in front of the loop and behind it is kept short. */
 template <int HP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t c, kv4_job a) {
+__global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     constexpr int HD = 64 * HP, ROW = 32 * HP, KS = (HP + 1) / 2, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4;
     constexpr int SC = 32 * ROW * 2, STAGE = SC + 512;    /* K rows, V rows, their scales in 256 bytes each */
     __shared__ __attribute__((aligned(16))) unsigned char buf0[WAVES * STAGE], buf1[WAVES * STAGE], buf2[WAVES * STAGE];
@@ -163,14 +165,14 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
             for (int i = 0; i < 8; i++) q4[ks][i] = *reinterpret_cast<const f32x4 *>(from + 4 * i);
         }
     }
-    const int lo = (chunk * WAVES + wave) * a.per_wave * 32, rows = max(min(a.per_wave * 32, seen_last - lo), 0), tiles = (rows + 31) / 32;
-    const size_t row0 = (size_t)h * c.max_rows + lo;
+    const int lo = (chunk * WAVES + wave) * a.run * 32, rows = max(min(a.run * 32, seen_last - lo), 0), tiles = (rows + 31) / 32;
+    const size_t row0 = (size_t)h * a.max_rows + lo;
     /* scales come in words; where a row has 2 or 6 bytes of them (HP odd) its first may start in the middle of one, whose other half is
      * memory that a word of the cache's reaches anyway */
-    const int sub = HP % 2 ? (int)((uintptr_t)(c.v_scales + row0 * 2 * HP) & 3) : 0, words = rows ? (rows * 2 * HP + sub + 3) / 4 : 0;
+    const int sub = HP % 2 ? (int)((uintptr_t)(a.v_scales + row0 * 2 * HP) & 3) : 0, words = rows ? (rows * 2 * HP + sub + 3) / 4 : 0;
     /* what lies past the wave's rows reads as zeros */
-    const __amdgpu_buffer_rsrc_t kd = vt_buffer(c.k_codes + row0 * ROW, rows * ROW), vd = vt_buffer(c.v_codes + row0 * ROW, rows * ROW);
-    const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + row0 * 2 * HP - sub, words * 4), vsd = vt_buffer(c.v_scales + row0 * 2 * HP - sub, words * 4);
+    const __amdgpu_buffer_rsrc_t kd = vt_buffer(a.k_codes + row0 * ROW, rows * ROW), vd = vt_buffer(a.v_codes + row0 * ROW, rows * ROW);
+    const __amdgpu_buffer_rsrc_t ksd = vt_buffer(a.k_scales + row0 * 2 * HP - sub, words * 4), vsd = vt_buffer(a.v_scales + row0 * 2 * HP - sub, words * 4);
     u32x4 scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd, lane * 16));
     /* a tile's requests: unit u of 16 bytes is row u / 2 HP, piece u % 2 HP of it */
     int k_at[4];                                         /* HP of them (with that size the host pass drops the kernel) */
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
         for (int blk = 0; blk < 2 * HP; blk++) {
             int at = 0x7fffffff;
             for (int r = lane; r < rows; r += 64)
-                if (c.v_scales[(row0 + r) * 2 * HP + blk] == 255) { at = lo + r; break; }
+                if (a.v_scales[(row0 + r) * 2 * HP + blk] == 255) { at = lo + r; break; }
 #pragma unroll
             for (int w = 32; w > 0; w /= 2) at = min(at, __shfl_xor(at, w));
 #pragma unroll
@@ -377,8 +379,8 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
                 for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * v + i] = __builtin_amdgcn_ldexpf(o[ch * CD + i][v] * f, -shift);
     }
     __syncthreads();
-    const int per = a.chunks;
-    float *part = a.part + ((size_t)h * gridDim.y + ct) * per * KV4_COLS * OD;
+    const int per = a.parts;
+    float *part = reinterpret_cast<float *>(a.part) + ((size_t)h * a.tiles + ct) * per * KV4_COLS * OD;
     auto result = [&](int col) {
         const int k = c0 + col, i = kv4_query(k, inv_group);
         return a.out + ((size_t)i * a.n_heads + (size_t)(h * group + k - i * group)) * HD;
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);                          /* the part's stores are acknowledged */
     __syncthreads();
-    unsigned *cnt = a.cnt + h * gridDim.y + ct;
+    unsigned *cnt = a.cnt + h * a.tiles + ct;
     if (threadIdx.x == 0) last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(per - 1);
     __syncthreads();
     if (!last) return;
@@ -440,30 +442,28 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(tts_hip_kv4_t
 #define KV4_TILE_WAVES 4
 #define KV4_TILE (32 * KV4_TILE_WAVES)
 #define KV4_MAX_PARTS 32
-struct kv4_tile_job { kv4_job a; int run, tiles_of_cols, most_parts; };
 
 template <int HP>
-__global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(tts_hip_kv4_t c, kv4_tile_job j) {
+__global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4_job a) {
     constexpr int HD = 64 * HP, ROW = 32 * HP, THREADS = 64 * KV4_TILE_WAVES, UNITS = 128 * HP, UN = (UNITS + THREADS - 1) / THREADS, DT = 2 * HP;
     constexpr int KB = 64 * ROW, SB = KB + UNITS, VB = SB;      /* K rows, their scales, V's operands */
     __shared__ __attribute__((aligned(16))) unsigned char buf[2][VB + 64 * HD * 2];
     __shared__ unsigned scan_most[KV4_TILE_WAVES], scan_nan[KV4_TILE_WAVES];
     __shared__ int last;
-    const kv4_job &a = j.a;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5, h = (int)blockIdx.y;
     /* The columns that see most first, and their last parts, which others do not have, before these.  (Neighbours go to different XCDs: with the parts of a tile side by
      * side every second XCD had half as many.) */
-    const int ahead = (int)blockIdx.x / j.tiles_of_cols, part = j.most_parts - 1 - ahead, ct = (ahead + 1) * j.tiles_of_cols - 1 - (int)blockIdx.x;
+    const int ahead = (int)blockIdx.x / a.tiles, part = a.parts - 1 - ahead, ct = (ahead + 1) * a.tiles - 1 - (int)blockIdx.x;
     const int c0 = ct * KV4_TILE, nc = min(KV4_TILE, a.cols - c0);
-    const int end = a.start + vt_div(c0 + nc - 1, a.group) + 1, parts = ((end + 63) / 64 + j.run - 1) / j.run;
+    const int end = a.start + vt_div(c0 + nc - 1, a.group) + 1, parts = ((end + 63) / 64 + a.run - 1) / a.run;
     if (part >= parts) return;
-    const int lo = part * j.run * 64, rows = min(j.run * 64, end - lo), tiles = (rows + 63) / 64;
+    const int lo = part * a.run * 64, rows = min(a.run * 64, end - lo), tiles = (rows + 63) / 64;
     const int w0 = c0 + 32 * wave, wc = min(w0 + 32, a.cols) - w0;               /* this wave's columns: none, perhaps */
     const int cc = min(w0 + n, a.cols - 1), qi = vt_div(cc, a.group), see = a.start + qi + 1;
     const int seen_first = a.start + vt_div(min(w0, a.cols - 1), a.group) + 1, seen_last = wc > 0 ? a.start + vt_div(w0 + wc - 1, a.group) + 1 : 0;
-    const size_t row0 = (size_t)h * c.max_rows + lo;
-    const __amdgpu_buffer_rsrc_t kd = vt_buffer(c.k_codes + row0 * ROW, rows * ROW), vd = vt_buffer(c.v_codes + row0 * ROW, rows * ROW);
-    const __amdgpu_buffer_rsrc_t ksd = vt_buffer(c.k_scales + row0 * DT, rows * DT), vsd = vt_buffer(c.v_scales + row0 * DT, rows * DT);
+    const size_t row0 = (size_t)h * a.max_rows + lo;
+    const __amdgpu_buffer_rsrc_t kd = vt_buffer(a.k_codes + row0 * ROW, rows * ROW), vd = vt_buffer(a.v_codes + row0 * ROW, rows * ROW);
+    const __amdgpu_buffer_rsrc_t ksd = vt_buffer(a.k_scales + row0 * DT, rows * DT), vsd = vt_buffer(a.v_scales + row0 * DT, rows * DT);
     /* unit u: 16 bytes of K, row u / 2 HP; a scale of K; V's keys 4 (u / 8 HP) .. + 3, values 8 (u % 8 HP) .. + 7 */
     u32x4 kr[UN];
     unsigned vr[UN][4];
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(tts
         for (int blk = 0; blk < DT; blk++) {
             int at = 0x7fffffff;
             for (int r = lane; r < rows; r += 64)
-                if (c.v_scales[(row0 + r) * DT + blk] == 255) { at = lo + r; break; }
+                if (a.v_scales[(row0 + r) * DT + blk] == 255) { at = lo + r; break; }
 #pragma unroll
             for (int w = 32; w > 0; w /= 2) at = min(at, __shfl_xor(at, w));
 #pragma unroll
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(tts
     if (parts > 1) {
         /* a part lies as the lanes hold it: [part][wave][4 HD / 32 vectors of four, then largest score and sum of weights][lane] */
         constexpr int WAVE_PART = (DT * 4 + 1) * 1024, PART = KV4_TILE_WAVES * WAVE_PART;
-        const __amdgpu_buffer_rsrc_t pd = vt_buffer(reinterpret_cast<unsigned char *>(a.part) + ((size_t)h * j.tiles_of_cols + ct) * j.most_parts * PART, parts * PART);
+        const __amdgpu_buffer_rsrc_t pd = vt_buffer(a.part + ((size_t)h * a.tiles + ct) * a.parts * PART, parts * PART);
         const int mine = wave * WAVE_PART + lane * 16;
 #pragma unroll
         for (int i = 0; i < DT; i++)
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(tts
         __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, pd, mine + part * PART + DT * 4 * 1024, 0, 16);
         __builtin_amdgcn_s_waitcnt(0x0f70);              /* acknowledged */
         __syncthreads();
-        unsigned *cnt = a.cnt + h * j.tiles_of_cols + ct;
+        unsigned *cnt = a.cnt + h * a.tiles + ct;
         if (tid == 0) last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
         __syncthreads();
         if (!last) return;
@@ -713,9 +713,10 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(tts
 }
 
 template <int HP, int WAVES>
-static int kv4_stream(const tts_hip_kv4_t *cache, kv4_job a) {
+static int kv4_stream(kv4_job a, int heads, int end) {
     const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
-    const long long cts = (a.cols + KV4_COLS - 1) / KV4_COLS, heads = cache->n_kv_heads, wgs = cts * heads, tiles = ((long long)a.start + a.seq + 31) / 32, slots = (long long)n_cu * (HP == 1 ? 2 : 1);
+    a.tiles = (a.cols + KV4_COLS - 1) / KV4_COLS;
+    const long long wgs = (long long)a.tiles * heads, tiles = ((long long)end + 31) / 32, slots = (long long)n_cu * (HP == 1 ? 2 : 1);
     /* Workgroups per head and tile of columns: the number that takes the least time at 3.5 us a round of workgroups, 1.2 us a tile of 128 values a row and 2.8 us for adding parts.
      * (us at 1 / 2 / 4 / 8 / 32 of them: 1 query behind 300 rows 7.4 / 8.5 / 8.5 / 8.5 / 8.5, behind 1999 13.4 / 11.8 / 9.8 / 9.1 / 9.0, behind 65535 264 / 137 / 73 / 41 / 20, 37 queries
      * behind 4000, ten tiles of columns, 24 / 20 / 27 / 35 and at 3 18.) */
@@ -726,26 +727,27 @@ static int kv4_stream(const tts_hip_kv4_t *cache, kv4_job a) {
         const float us = rounds * (3.5f + 0.6f * HP * each) + (chunks > 1 ? 2.8f : 0.f);
         if (us < least) { least = us; best = chunks; }
     }
-    a.per_wave = (int)((tiles + best * WAVES - 1) / (best * WAVES));
-    a.chunks = (int)((tiles + (long long)a.per_wave * WAVES - 1) / ((long long)a.per_wave * WAVES));
-    if (a.chunks > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)cts * heads * a.chunks * KV4_COLS * (cache->head_dim + 4)))) return -1;
-    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)a.chunks, (unsigned)cts, (unsigned)heads), dim3(64 * WAVES), 0, g_vt.stream, *cache, a);
+    a.run = (int)((tiles + best * WAVES - 1) / (best * WAVES));
+    a.parts = (int)((tiles + (long long)a.run * WAVES - 1) / ((long long)a.run * WAVES));
+    if (a.parts > 1 && !(a.part = (unsigned char *)vt_scratch(sizeof(float) * (size_t)wgs * a.parts * KV4_COLS * (64 * HP + 4)))) return -1;
+    static_assert(sizeof a <= 104, "arguments");
+    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)a.parts, (unsigned)a.tiles, (unsigned)heads), dim3(64 * WAVES), 0, g_vt.stream, a);
     return 0;
 }
 
 template <int HP>
-static int kv4_tiles(const tts_hip_kv4_t *cache, const kv4_job &a) {
-    kv4_tile_job j = {a, 0, (a.cols + KV4_TILE - 1) / KV4_TILE, 1};
-    const long long heads = cache->n_kv_heads, last = ((long long)a.start + a.seq + 63) / 64, wgs = heads * j.tiles_of_cols, slots = 2ll * (g_vt.n_cu > 0 ? g_vt.n_cu : 256);
+static int kv4_tiles(kv4_job a, int heads, int end) {
+    a.tiles = (a.cols + KV4_TILE - 1) / KV4_TILE;
+    const long long last = ((long long)end + 63) / 64, wgs = (long long)heads * a.tiles, slots = 2ll * (g_vt.n_cu > 0 ? g_vt.n_cu : 256);
     /* as many parts as there is room for at once, of four tiles and more (400 queries and no rows before: 20 us whole or in runs of 8, 21 in runs of 4; 1000 behind 1000 rows: 69 whole,
      * 66 in runs of 16, two workgroups on a CU each, 74 to 96 in shorter ones) */
     long long run = wgs < slots && wgs <= VT_MX4_COUNTERS ? (last + slots / wgs - 1) / (slots / wgs) : last;
     if (run < 4) run = 4;
     if (run * KV4_MAX_PARTS < last && wgs <= VT_MX4_COUNTERS) run = (last + KV4_MAX_PARTS - 1) / KV4_MAX_PARTS;
-    j.run = (int)run;
-    j.most_parts = (int)((last + run - 1) / run);
-    if (j.most_parts > 1 && !(j.a.part = (float *)vt_scratch((size_t)wgs * j.most_parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
-    hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)(j.tiles_of_cols * (long long)j.most_parts), (unsigned)heads), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, *cache, j);
+    a.run = (int)run;
+    a.parts = (int)((last + run - 1) / run);
+    if (a.parts > 1 && !(a.part = (unsigned char *)vt_scratch((size_t)wgs * a.parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
+    hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)(a.tiles * (long long)a.parts), (unsigned)heads), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, a);
     return 0;
 }
 
@@ -765,12 +767,14 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
     for (int s = 0; s < seq_len; s += most) {
         const int n = seq_len - s < most ? seq_len - s : most, cols = n * group;
         const size_t at = (size_t)s * n_heads * cache->head_dim;
-        const kv4_job a = {d_out + at, d_Q + at, n, start_pos + s, n_heads, cols, 0, 1, vt_divisor_of(group, cols), scale * 1.44269504f, NULL, g_vt.d_mx4_cnt};
+        const kv4_job a = {cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, d_out + at, d_Q + at, NULL, g_vt.d_mx4_cnt, cache->max_rows, start_pos + s, n_heads, cols, 0, 1, 0,
+                           vt_divisor_of(group, cols), scale * 1.44269504f};
+        const int heads = cache->n_kv_heads, end = start_pos + s + n;
         /* Many columns: from two rounds of the other kernel's workgroups on (200 queries behind 300 rows, 400 of them: 22 us and 16; 400 queries and no rows before, 800: 20 and 28; 1531:
          * 65 and 120), and for heads of up to 128 values, whose results and queries leave two waves of a SIMD their registers (500 behind 500 rows with 256: 54 and 40). */
         int bad;
-        if (HP <= 2 && (long long)((cols + KV4_COLS - 1) / KV4_COLS) * cache->n_kv_heads > 2ll * n_cu) bad = HP == 1 ? kv4_tiles<1>(cache, a) : kv4_tiles<2>(cache, a);
-        else bad = HP == 1 ? kv4_stream<1, 8>(cache, a) : HP == 2 ? kv4_stream<2, 8>(cache, a) : HP == 3 ? kv4_stream<3, 4>(cache, a) : kv4_stream<4, 4>(cache, a);
+        if (HP <= 2 && (long long)((cols + KV4_COLS - 1) / KV4_COLS) * cache->n_kv_heads > 2ll * n_cu) bad = HP == 1 ? kv4_tiles<1>(a, heads, end) : kv4_tiles<2>(a, heads, end);
+        else bad = HP == 1 ? kv4_stream<1, 8>(a, heads, end) : HP == 2 ? kv4_stream<2, 8>(a, heads, end) : HP == 3 ? kv4_stream<3, 4>(a, heads, end) : kv4_stream<4, 4>(a, heads, end);
         if (bad) return -1;
     }
     return vt_check(hipGetLastError(), who) ? -1 : 0;
