@@ -26,14 +26,14 @@ static int cache_ok(const char *who, const tts_hip_kv4_t *c, long long first, lo
     return 1;
 }
 
-/* ---- rows into the cache and back: a lane per eight values, K in blockIdx.y = 0 and V in 1 ----------------------------- */
+/* ---- rows into the cache (a lane per eight values) and back (four); K in blockIdx.y = 0 and V in 1 ----------------------- */
 struct kv4_rows { int n, pos, max_rows, stride, whole; vt_divisor per_row, per_head; };      /* lanes of a row, of a row of one head */
 
-static __device__ __forceinline__ bool kv4_place(const kv4_rows &r, long long &from, size_t &at) {
+static __device__ __forceinline__ bool kv4_place(const kv4_rows &r, int values, long long &from, size_t &at) {
     const int i = (int)(blockIdx.x * 256 + threadIdx.x);
     if (i >= r.n * r.per_row.d) return false;
     const int row = vt_div(i, r.per_row), u = i - row * r.per_row.d, h = vt_div(u, r.per_head), d = u - h * r.per_head.d;
-    from = (long long)row * r.stride + 8 * u;
+    from = (long long)row * r.stride + values * u;
     at = ((size_t)h * r.max_rows + r.pos + row) * r.per_head.d + d;
     return true;
 }
@@ -41,7 +41,7 @@ static __device__ __forceinline__ bool kv4_place(const kv4_rows &r, long long &f
 __global__ void __launch_bounds__(256) vt_kv4_append_kernel(tts_hip_kv4_t c, const float *K, const float *V, kv4_rows r) {
     long long from;
     size_t at;
-    if (!kv4_place(r, from, at)) return;
+    if (!kv4_place(r, 8, from, at)) return;
     f32x4 a, b;
     vt_mx4_load8((blockIdx.y ? V : K) + from, 8, r.whole, a, b);
     unsigned scale;
@@ -53,29 +53,27 @@ __global__ void __launch_bounds__(256) vt_kv4_append_kernel(tts_hip_kv4_t c, con
 __global__ void __launch_bounds__(256) vt_kv4_read_kernel(float *K, float *V, tts_hip_kv4_t c, kv4_rows r) {
     long long to;
     size_t at;
-    if (!kv4_place(r, to, at)) return;
-    f32x4 a, b;
-    vt_mx4_decode8(((const unsigned *)(blockIdx.y ? c.v_codes : c.k_codes))[at], (blockIdx.y ? c.v_scales : c.k_scales)[at >> 2], a, b);
-    vt_mx4_store8((blockIdx.y ? V : K) + to, 8, r.whole, a, b);
+    if (!kv4_place(r, 4, to, at)) return;
+    vt_mx4_store4((blockIdx.y ? V : K) + to, 4, r.whole, vt_mx4_decode4(((const uint16_t *)(blockIdx.y ? c.v_codes : c.k_codes))[at], (blockIdx.y ? c.v_scales : c.k_scales)[at >> 3]));
 }
 
-static int kv4_rows_ok(const char *who, kv4_rows *r, const tts_hip_kv4_t *c, const float *K, const float *V, int n, int pos, int stride) {
+static int kv4_rows_ok(const char *who, kv4_rows *r, const tts_hip_kv4_t *c, const float *K, const float *V, int n, int pos, int stride, int values) {
     if (!cache_ok(who, c, pos, n)) return 0;
     const long long width = (long long)c->n_kv_heads * c->head_dim;
     if (stride == 0) stride = (int)(width > 0x7fffffff ? 0x7fffffff : width);
-    if (!K || !V || (((uintptr_t)K | (uintptr_t)V) & 3) || stride < width || width / 8 * n > 0x7fffff00ll) {
+    if (!K || !V || (((uintptr_t)K | (uintptr_t)V) & 3) || stride < width || width / values * n > 0x7fffff00ll) {
         vt_set_error("%s: %d rows of %lld values %d apart", who, n, width, stride);
         return 0;
     }
     *r = kv4_rows{n, pos, c->max_rows, stride, (((uintptr_t)K | (uintptr_t)V) & 15) == 0 && stride % 4 == 0,
-                  vt_divisor_of((int)(width / 8), width / 8 * n), vt_divisor_of(c->head_dim / 8, width / 8)};
+                  vt_divisor_of((int)(width / values), width / values * n), vt_divisor_of(c->head_dim / values, width / values)};
     return vt_mx4_ready(who);
 }
 
 extern "C" int tts_hip_kv4_append(const tts_hip_kv4_t *cache, const float *d_K, const float *d_V, int n_rows, int pos, int stride) {
     static const char who[] = "tts_hip_kv4_append";
     kv4_rows r;
-    if (!kv4_rows_ok(who, &r, cache, d_K, d_V, n_rows, pos, stride)) return -1;
+    if (!kv4_rows_ok(who, &r, cache, d_K, d_V, n_rows, pos, stride, 8)) return -1;
     hipLaunchKernelGGL(vt_kv4_append_kernel, dim3((r.n * r.per_row.d + 255) / 256, 2), dim3(256), 0, g_vt.stream, *cache, d_K, d_V, r);
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
@@ -83,7 +81,7 @@ extern "C" int tts_hip_kv4_append(const tts_hip_kv4_t *cache, const float *d_K, 
 extern "C" int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cache, int n_rows, int pos, int stride) {
     static const char who[] = "tts_hip_kv4_read";
     kv4_rows r;
-    if (!kv4_rows_ok(who, &r, cache, d_K, d_V, n_rows, pos, stride)) return -1;
+    if (!kv4_rows_ok(who, &r, cache, d_K, d_V, n_rows, pos, stride, 4)) return -1;
     hipLaunchKernelGGL(vt_kv4_read_kernel, dim3((r.n * r.per_row.d + 255) / 256, 2), dim3(256), 0, g_vt.stream, d_K, d_V, *cache, r);
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }

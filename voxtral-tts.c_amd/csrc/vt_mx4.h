@@ -38,12 +38,10 @@ __device__ __forceinline__ unsigned vt_mx4_encode8(const f32x4 &a, const f32x4 &
     return scale == 255u ? 0u : c;
 }
 
-__device__ __forceinline__ void vt_mx4_decode8(unsigned c, unsigned scale, f32x4 &a, f32x4 &b) {
+__device__ __forceinline__ f32x4 vt_mx4_decode4(unsigned c, unsigned scale) {
     const float f = vt_mx4_scale(scale);
     const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, f, 0), q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, f, 1);
-    const f32x2 r = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, f, 2), t = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, f, 3);
-    a = f32x4{p.x, p.y, q.x, q.y};
-    b = f32x4{r.x, r.y, t.x, t.y};
+    return f32x4{p.x, p.y, q.x, q.y};
 }
 
 /* n (at most 8) of eight values at p, zeros behind them; whole: all eight there and p on 16 bytes */
@@ -72,17 +70,15 @@ __device__ __forceinline__ void vt_mx4_load8(const uint16_t *p, int n, bool whol
         b[i] = i + 4 < n ? vt_bf16_lo(p[i + 4]) : 0.f;
     }
 }
-__device__ __forceinline__ void vt_mx4_store8(float *p, int n, bool whole, const f32x4 &a, const f32x4 &b) {
+/* four values back, past the caches where they lie on 16 bytes */
+__device__ __forceinline__ void vt_mx4_store4(float *p, int n, bool whole, const f32x4 &v) {
     if (whole) {
-        *reinterpret_cast<f32x4 *>(p) = a;
-        *reinterpret_cast<f32x4 *>(p + 4) = b;
+        __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(p));
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (i < n) p[i] = a[i];
-        if (i + 4 < n) p[i + 4] = b[i];
-    }
+    for (int i = 0; i < 4; i++)
+        if (i < n) p[i] = v[i];
 }
 
 /* ---- fp32 operands of the scaled matrix instructions --------------------------------------------------------------
