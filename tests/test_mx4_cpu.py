@@ -24,7 +24,7 @@ def refused(name, *args):
 
 @pytest.mark.parametrize("args", [(None, Q, R, 0, 4, 128, 0), (P, None, R, 0, 4, 128, 0), (P, Q, None, 0, 4, 128, 0), (P, Q, R, 0, 0, 128, 0), (P, Q, R, 0, 4, 0, 0),
                                   (P, Q, R, 0, -1, 128, 0), (P, Q, R, 0, 4, 128, 127), (P, Q, R, 0, 4, 128, -128), (P + 8, Q, R, 0, 4, 128, 0), (P, Q + 2, R, 0, 4, 128, 0),
-                                  (P, Q, R + 2, 0, 4, 128, 0), (P, Q, R + 1, 1, 4, 128, 0), (P, Q, R, 0, 4, (1 << 27) + 1, 0)])
+                                  (P, Q, R + 2, 0, 4, 128, 0), (P, Q, R + 1, 1, 4, 128, 0), (P, Q, R, 0, 4, (1 << 27) + 1, 0), (P, Q, R, 0, (1 << 30) + 1, 1, 0)])
 def test_quantize_refuses(args):
     refused("tts_hip_mx4_quantize", *args)
     codes, scales, x, bf16, rows, cols, stride = args
@@ -33,7 +33,8 @@ def test_quantize_refuses(args):
 
 
 @pytest.mark.parametrize("args", [(None, Q, P, R, 1, 8, 8), (P, None, Q, R, 1, 8, 8), (P, Q, None, R, 1, 8, 8), (P, Q, R, None, 1, 8, 8), (P, Q, R, P, 0, 8, 8),
-                                  (P, Q, R, P, 1, 0, 8), (P, Q, R, P, 1, 8, 0), (P + 2, Q, R, P, 1, 8, 8), (P, Q + 1, R, P, 1, 8, 8), (P, Q, R + 4, P, 1, 8, 8), (P, Q, R, P + 1, 1, 8, 8)])
+                                  (P, Q, R, P, 1, 0, 8), (P, Q, R, P, 1, 8, 0), (P + 2, Q, R, P, 1, 8, 8), (P, Q + 1, R, P, 1, 8, 8), (P, Q, R + 4, P, 1, 8, 8), (P, Q, R, P + 1, 1, 8, 8), (P, Q, R, P, 1, (1 << 23) + 1, 8),
+                                  (P, Q, R, P, (1 << 30) + 1, 8, 8), (P, Q, R, P, 1, 8, (1 << 30) + 1)])
 def test_linear_refuses(args):
     refused("tts_hip_linear_mx4", *args)
 
@@ -73,6 +74,9 @@ def test_other_arguments():
     refused("tts_hip_kv4_attention", P, P + 4, cache(), 1, 0, 32, 0.1)
     refused("tts_hip_kv4_attention", P, P, cache(), 1, 0, 33, 0.1)
     refused("tts_hip_kv4_attention", P, P, cache(), 1, 0, 0, 0.1)
+    refused("tts_hip_kv4_attention", P, P, cache(max_rows=2 ** 31 - 1), 1, 1 << 24, 32, 0.1)
+    refused("tts_hip_kv4_attention", P, P, cache(n_kv_heads=65536), 1, 0, 65536, 0.1)
+    refused("tts_hip_kv4_attention", P, P, cache(n_kv_heads=1), 1, 0, (1 << 19) + 1, 0.1)
 
 
 def test_the_oracle_rounds_as_the_format_says():

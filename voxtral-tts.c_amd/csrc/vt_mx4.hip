@@ -81,8 +81,8 @@ static int mx4_grid(mx4_shape *s, const void *x, int item, int rows, int cols, i
 
 static int mx4_shape_ok(const char *who, const void *x, const uint8_t *codes, const uint8_t *scales, int rows, int cols, int stride, int item) {
     if (!x || !codes || !scales) { vt_set_error("%s: NULL pointer", who); return 0; }
-    if (rows < 1 || cols < 1 || cols > 1 << 27 || stride < cols) {
-        vt_set_error("%s: %d rows of %d columns %d apart (columns: 1 .. 2^27)", who, rows, cols, stride);
+    if (rows < 1 || rows > 1 << 30 || cols < 1 || cols > 1 << 27 || stride < cols) {
+        vt_set_error("%s: %d rows (1 .. 2^30) of %d columns (1 .. 2^27) %d apart", who, rows, cols, stride);
         return 0;
     }
     if (((uintptr_t)codes & 15) || ((uintptr_t)scales & 3) || (uintptr_t)x % item) {
@@ -369,15 +369,17 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
 #pragma unroll
     for (int i = 0; i < WU; i++) { const int u = i * THREADS + (int)threadIdx.x, r = u >> 2; w_at[i] = r * 64 * a.panels + ((u & 3) ^ ((r >> 1) & 3)) * 16; }
     const int s_at = (int)threadIdx.x * 4 * a.panels;
-    auto ask = [&](unsigned char *b, int panel) __attribute__((always_inline)) {
-        const __amdgpu_buffer_rsrc_t xd = vt_buffer(a.planes + ((size_t)panel * a.tiles + t0) * 2 * MXT_STEP, xt * 2 * MXT_STEP);
+    /* a quarter q of a panel's requests, or all of them (-1); past the last panel: zeros, which nobody reads */
+    auto ask = [&](unsigned char *b, int panel, int q) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t xd = vt_buffer(a.planes + ((size_t)min(panel, p1 - 1) * a.tiles + t0) * 2 * MXT_STEP, panel < p1 ? xt * 2 * MXT_STEP : 0);
+        const int dead = panel < p1 ? 0 : 0x40000000;
 #define LDS(at) (__attribute__((address_space(3))) void *)(b + (at))
 #pragma unroll
-        for (int i = 0; i < WU; i++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, LDS(i * THREADS * 16 + wave * 1024), 16, w_at[i], panel * 64, 0, 0);
-        if (wave * 64 < BM) __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, LDS(W_BYTES + wave * 256), 4, s_at, panel * 4, 0, 0);
+        for (int i = 0; i < WU; i++) if (q < 0 || i % 4 == q) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, LDS(i * THREADS * 16 + wave * 1024), 16, (w_at[i] + panel * 64) | dead, 0, 0, 0);
+        if ((q < 0 || q == 3) && wave * 64 < BM) __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, LDS(W_BYTES + wave * 256), 4, (s_at + panel * 4) | dead, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < XU; i++)
-            if ((i * THREADS + wave * 64) * 16 < X_BYTES)
+            if ((q < 0 || (i + 2) % 4 == q) && (i * THREADS + wave * 64) * 16 < X_BYTES)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(xd, LDS(W_BYTES + BM * 4 + i * THREADS * 16 + wave * 1024), 16, (i * THREADS + (int)threadIdx.x) * 16, 0, 0, 0);
 #undef LDS
     };
@@ -387,7 +389,6 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
     auto step = [&](int panel, const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(0x0f70);
         __syncthreads();                                 /* this panel is there, and everybody is through with the one before */
-        if (panel + 1 < p1) ask(later, panel + 1);
         u32x4 w[FM][2];
         int ws[FM], xs[2];
         const unsigned char *xb = here + W_BYTES + BM * 4 + wn * 2 * MXT_STEP;
@@ -412,12 +413,16 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
                 sum[f] = h ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(xq), vt_mfma_e2m1(w[f][1]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, p, xs[1], 2, ws[f]) \
                            : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(xq), vt_mfma_e2m1(w[f][0]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, p, xs[0], 0, ws[f]); \
         }
-        PRODUCTS(3) PRODUCTS(2) PRODUCTS(1) PRODUCTS(0)
+/* a quarter of the next panel's requests behind each plane's products: all at once they keep the waves of a CU waiting at its address path, 0.5 us of 1.8 a panel.
+ * Anything but products and requests may cross. */
+#define STAGE(q) __builtin_amdgcn_sched_barrier(0x387); ask(later, panel + 1, q); __builtin_amdgcn_sched_barrier(0x387);
+        PRODUCTS(3) STAGE(0) PRODUCTS(2) STAGE(1) PRODUCTS(1) STAGE(2) PRODUCTS(0) STAGE(3)
+#undef STAGE
 #undef PRODUCTS
 #pragma unroll
         for (int f = 0; f < FM; f++) acc[f] = acc[f] + sum[f];
     };
-    ask(buf0, p0);                                       /* every cut has a panel */
+    ask(buf0, p0, -1);                                       /* every cut has a panel */
     for (int panel = p0; panel < p1; panel += 2) {
         step(panel, buf0, buf1);
         if (panel + 1 >= p1) break;
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
 /* Tiles: weight rows, rows of x, workgroups that a CU holds, and us per panel with one, two, three of them on it (from runs of one cut on part of the chip and on all of
  * it: 226 x 3072 x 9216, 1531 x 9216 x 3072). */
 struct mxt_tile { int bm, bn, per_cu; float panel_us[3]; };
-static const mxt_tile mxt_tiles[] = {{256, 128, 1, {1.9f}}, {128, 64, 2, {0.76f, 1.21f}}, {128, 32, 3, {0.55f, 0.85f, 1.25f}}};
+static const mxt_tile mxt_tiles[] = {{256, 128, 1, {1.8f}}, {128, 64, 2, {0.72f, 1.2f}}, {128, 32, 3, {0.56f, 0.85f, 1.25f}}};
 #define MXT_MAX_CUTS 16
 
 /* The tile and the cuts of K with the least time by these figures.  us, measured and (planned): 226 x 3072 x 9216 36 (128 x 64 in 4 cuts; others 37 to 130), 1531 x 9216 x 3072
@@ -500,7 +505,7 @@ static int mx4_linear_tiles(float *d_y, const float *d_x, const uint8_t *d_codes
 
 extern "C" int tts_hip_linear_mx4(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim) {
     static const char who[] = "tts_hip_linear_mx4";
-    if (!d_y || ((uintptr_t)d_y & 3) || seq_len < 1) { vt_set_error("%s: %d rows to %p", who, seq_len, (void *)d_y); return -1; }
+    if (!d_y || ((uintptr_t)d_y & 3) || seq_len < 1 || seq_len > 1 << 30) { vt_set_error("%s: %d rows (1 .. 2^30) to %p", who, seq_len, (void *)d_y); return -1; }
     if (!mx4_shape_ok(who, d_x, d_codes, d_scales, out_dim, in_dim, in_dim, 4)) return -1;
     if (in_dim > 1 << 23) { vt_set_error("%s: %d columns (1 .. 2^23)", who, in_dim); return -1; }
     if (!vt_mx4_ready(who)) return -1;
