@@ -333,8 +333,7 @@ int tts_hip_split_planes(uint16_t *d_hi, uint16_t *d_lo, const float *d_x, size_
  * scales on 4.  Device pointers only; asynchronous on the library's stream; 0 / -1. */
 
 /* values [rows, cols], x_stride of them apart from row to row (0: cols), fp32 or, with x_bf16, bf16 -> codes
- * and scales.  Values may lie on any multiple of their size; rows up to 2^30, cols up to
- * 2^27. */
+ * and scales.  Values may lie on any multiple of their size; rows up to 2^30, cols up to 2^27. */
 int tts_hip_mx4_quantize(uint8_t *d_codes, uint8_t *d_scales, const void *d_x, int x_bf16,
                          int rows, int cols, int x_stride);
 /* codes and scales -> the values that they stand for, fp32, exactly; the room between rows is left as it was. */
@@ -342,9 +341,10 @@ int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const uint8_t *d_
                            int rows, int cols, int x_stride);
 /* y[seq_len, out_dim] = x[seq_len, in_dim] W^T, W [out_dim, in_dim] in 4 bits, x and y fp32 and dense: what
  * tts_hip_linear_bf16 is for bf16 weights.  x enters to 2^-16 of the largest of its 32 neighbours at the
- * worst, 5e-7 of a row's norm on values of a normal distribution; sums are fp32.  A row of x with an infinity or a NaN in
- * it gives NaN.  seq_len and out_dim up to 2^30, in_dim up to 2^23.  More than a few rows use the library's work area, which grows by
- * allocation when a call needs more than any before it. */
+ * worst, 5e-7 of a row's norm on values of a normal distribution; sums are fp32.  A row of x with an infinity
+ * or a NaN in it gives NaN, a sum that leaves fp32 NaN or an infinity of either sign.  y and x do not overlap.
+ * seq_len and out_dim up to 2^30, in_dim up to 2^23.  More than a few rows use the library's work area, which
+ * grows by allocation when a call needs more than any before it. */
 int tts_hip_linear_mx4(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales,
                        int seq_len, int in_dim, int out_dim);
 
@@ -358,16 +358,19 @@ typedef struct {
 
 /* K and V rows [n_rows, n_kv_heads * head_dim] fp32, `stride` floats apart (0: dense), into the cache's rows
  * pos .. pos + n_rows - 1; the others stay as they were. */
-int tts_hip_kv4_append(const tts_hip_kv4_t *cache, const float *d_K, const float *d_V, int n_rows, int pos, int stride);
+int tts_hip_kv4_append(const tts_hip_kv4_t *cache, const float *d_K, const float *d_V,
+                       int n_rows, int pos, int stride);
 /* The cache's rows pos .. pos + n_rows - 1 back as the fp32 values that they stand for. */
 int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cache, int n_rows, int pos, int stride);
 /* Causal attention over the cache: query i of Q [seq_len, n_heads * head_dim] sees the rows 0 .. start_pos + i,
  * which hold its own keys and values too (append first); out like Q, on 16 bytes both.  n_heads is a multiple
  * of n_kv_heads.  A decode step is seq_len 1; what tts_hip_causal_attention_decode and _prefill are for an
- * fp32 cache.  A row that a query does not see changes nothing in its result, whatever it holds;
- * a query with an infinity or a NaN in it, and one that sees such a key, gives NaN, a value's NaN the 32 values of its block.  At most 2^24 rows,
- * 65535 kv heads and 2^19 heads on each.  Where several workgroups share a head's rows
- * their parts meet in the library's work area, which grows by allocation when a call needs more than any before it. */
+ * fp32 cache.  A row that a query does not see changes nothing in its result, whatever it holds; a query with
+ * an infinity or a NaN in it, and one that sees such a key, gives NaN, a value's NaN the 32 values of its block.
+ * A score whose sum leaves fp32 makes NaN or counts for nothing.  Values whose magnitudes differ by more than
+ * 2^36 within a head are handled exactly, by a far slower way.  out and Q do not overlap.  At most 2^24 rows,
+ * 65535 kv heads and 2^19 heads on each.  Where several workgroups share a head's rows their parts meet in the
+ * library's work area, which grows by allocation when a call needs more than any before it. */
 int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_hip_kv4_t *cache, int seq_len,
                           int start_pos, int n_heads, float scale);
 

@@ -63,7 +63,7 @@ def attend(hip, cache, q, pos, heads, scale):
     return out[:q.size].reshape(q.shape)
 
 
-def oracle(q, k, v, pos, heads, scale):
+def oracle(q, k, v, pos, heads, scale, absolute=True):
     """-> out, tolerance [rows, heads * hd]; k, v [kv_heads, pos + rows, hd]"""
     rows, hd, n = q.shape[0], k.shape[2], pos + q.shape[0]
     out, tol = np.zeros((rows, heads, hd)), np.zeros((rows, heads, hd))
@@ -87,7 +87,7 @@ def oracle(q, k, v, pos, heads, scale):
         # 2^-25 2^-14 = 2^-39 of the largest weight however small it is; the largest weight over the sum is at most 1, and n weights meet
         # n values: 2^-39 sum |v|.  A value goes in as fp16 of v 2^13 / 2^E with 2^E at most a quarter of the largest value: off by up to 2^-25 2^-13 / 4 =
         # 2^-40 of that, weights adding up to 1.
-        tol[:, h] = e * (p @ np.abs(vh)) + 2.0 ** -39 * (seen @ np.abs(vh)) + 2.0 ** -40 * np.abs(vh).max() + 1e-37
+        tol[:, h] = e * (p @ np.abs(vh)) + absolute * (2.0 ** -39 * (seen @ np.abs(vh)) + 2.0 ** -40 * np.abs(vh).max()) + 1e-37
     return out.reshape(rows, -1), tol.reshape(rows, -1)
 
 
@@ -175,6 +175,67 @@ def test_attention_results_do_not_depend_on_the_call(hip):
         for _ in range(5):
             assert np.array_equal(first, attend(hip, cache, q, pos, 32, 0.1))
         c.free()
+
+
+BOTH = [(4, 2, 64, 1, 300), (4, 2, 128, 40, 600), (4, 2, 192, 40, 20), (4, 1, 256, 64, 0), (32, 2, 64, 300, 0), (32, 2, 128, 300, 1500), (32, 2, 128, 700, 0)]      # few columns and many
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
+def test_attention_scores_of_any_size(hip, heads, kv_heads, hd, rows, pos):
+    """All keys the same, queries from 2^-10 to 2^60 and both signs: all weights are the same, results are means of values.  (Products of the
+    same numbers in the same order: the scores differ by nothing.)"""
+    c, q = case(hip, heads, kv_heads, hd, rows, pos)
+    r, n = np.random.default_rng(5), pos + rows
+    k, v = np.repeat(r.standard_normal((kv_heads, 1, hd)), n, 1).astype(np.float32), r.standard_normal((kv_heads, n, hd)).astype(np.float32)
+    c.fill(k, v)
+    q = (q * 2.0 ** (-10 + 70 * (np.arange(rows) + r.random(rows))[:, None] / rows)).astype(np.float32)
+    got = attend(hip, c.upload(), q, pos, heads, 0.1).reshape(rows, heads, hd)
+    _, v = c.values(n)
+    c.free()
+    count = (pos + np.arange(rows) + 1)[:, None]
+    for h in range(heads):
+        vh = v[h * kv_heads // heads]
+        mean, size = np.cumsum(vh, 0)[pos:] / count, np.cumsum(np.abs(vh), 0)[pos:] / count
+        # weights alike to 2^-21 and the sums' rounding, as in the oracle; values and small weights to 2^-39 besides
+        tol = (2.0 ** -20 + 2.0 ** -23 * (n / 32 + 40)) * size + 2.0 ** -39 * np.abs(vh).max() + 2.0 ** -39 * count * size
+        assert np.all(np.abs(got[:, h] - mean) <= tol), (h, float((np.abs(got[:, h] - mean) / tol).max()))
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
+@pytest.mark.parametrize("near", [False, True])
+def test_attention_values_of_any_size(hip, heads, kv_heads, hd, rows, pos, near):
+    """A row 2^100 times as large as the others, and one 2^-60 times: who does not see the first has what it has without it, and so, but for a
+    part in the last binades, has who gives it a weight of 2^-110.  No absolute error: nothing counts beside the values seen, each by its weight."""
+    c, q = case(hip, heads, kv_heads, hd, rows, pos)
+    r, n = np.random.default_rng(6), pos + rows
+    k, v = r.standard_normal((2, kv_heads, n, hd)).astype(np.float32)
+    bad = n - 1 - rows // 3
+    v[:, bad] *= np.float32(2.0 ** 100)
+    v[:, bad // 2] *= np.float32(2.0 ** -60)
+    q = q.reshape(rows, heads, hd)
+    q[..., 0], k[..., 0], k[:, bad, 0] = 8, 0, 0 if near else -96
+    q = q.reshape(rows, -1)
+    c.fill(k, v)
+    got = attend(hip, c.upload(), q, pos, heads, 0.1)
+    want, tol = oracle(q, *c.values(n), pos, heads, float(np.float32(0.1)), absolute=False)
+    c.free()
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
+def test_attention_nan_beside_values_of_any_size(hip, heads, kv_heads, hd, rows, pos):
+    c, q = case(hip, heads, kv_heads, hd, rows, pos)
+    r, n = np.random.default_rng(7), pos + rows
+    k, v = r.standard_normal((2, kv_heads, n, hd)).astype(np.float32)
+    v[:, n // 3] *= np.float32(2.0 ** -90)
+    bad = n - 1 - rows // 3
+    v[0, bad, 33] = np.nan
+    c.fill(k, v)
+    got = attend(hip, c.upload(), q, pos, heads, 0.1).reshape(rows, heads, hd)
+    c.free()
+    nan = np.zeros(got.shape, bool)
+    nan[pos + np.arange(rows) >= bad, :heads // kv_heads, 32:64] = True
+    assert np.array_equal(np.isnan(got), nan)
 
 
 def test_a_layer_in_4_bits(hip):

@@ -91,9 +91,12 @@ extern "C" int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cac
  * S^T[row][column] = K Q^T on the scaled matrix instruction, keys in 4 bits as they lie, queries as five e2m3 planes (vt_mx4.h), the
  * smallest plane first: the accumulators are cut and not rounded at 2^-23, and so only the last sum meets that.  Results are
  * O^T[value][column] = V^T P^T in fp16: 4-bit values are exact in fp16 once they are scaled by the largest scale E of the rows at hand,
- * to 2^13 of it (what is 2^37 times smaller becomes zero), and a weight p 2^14 goes in as two planes of 22 bits in all.  Maximum, sum and
+ * to 2^13 of it, and a weight p 2^14 goes in as two planes of 22 bits in all.  Maximum, sum and
  * results of a column are fp32, one pass over the rows with the running maximum.  A lane holds the same column of S^T and of O^T, and
  * the order of keys inside an instruction is free, so that weights go from one product to the next in their registers.
+ * Rows at hand with scales further apart than fp16 reaches (36 binades) go another way (kv4_column): fp32 all through, rare, and slow: 1 query of 32 heads behind 1999
+ * rows 46 us with the call and the wait for it, 1531 behind none 5.9 ms.
+ * A score beyond fp32 meets the planes one by one, with signs of their own: it makes NaN or an infinity of either sign.
  * NaN: a key's shows in the scores of who sees it.  A value's scale of 255 is taken for a finite one in the product (a hidden row's weight
  * is 0, and 0 times NaN would reach who does not see it), and behind the last row NaN goes to the columns that see such a row. */
 typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
@@ -118,19 +121,78 @@ struct kv4_job {
 /* column / heads per kv head, for fewer than 2^20 columns: (c + 1/2) / d is no nearer to a whole number than 1 / 2 d, and c 2^-22 / d off */
 static __device__ __forceinline__ int kv4_query(int col, float inv) { return (int)(((float)col + 0.5f) * inv); }
 
-/* largest scale byte below 255 of four, and whether one is 255 */
-static __device__ __forceinline__ void kv4_scan4(unsigned w, unsigned &most, unsigned &nan) {
+/* What the scales of the values at hand span: bytes s as t = s + 1 mod 256, pairs of them.  255 is t = 0 and the block of zeros 1; neither counts. */
+typedef unsigned short kv4_u16x2 __attribute__((ext_vector_type(2)));
+struct kv4_span {
+    kv4_u16x2 top = {1, 1}, low = {1, 1}, least = {65535, 65535};         /* largest t, 0 if there is one, smallest t - 2 */
+    __device__ __forceinline__ void add4(unsigned w) {
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
-        const unsigned s = (w >> (8 * b)) & 255u;
-        nan |= s == 255u;
-        most = max(most, s == 255u ? 0u : s);
+        for (int b = 0; b < 2; b++) {
+            const kv4_u16x2 t = __builtin_bit_cast(kv4_u16x2, (((w >> (8 * b)) & 0x00ff00ffu) + 0x00010001u) & 0x00ff00ffu);
+            top = __builtin_elementwise_max(top, t);
+            low = __builtin_elementwise_min(low, t);
+            least = __builtin_elementwise_min(least, (kv4_u16x2)(t - (kv4_u16x2){2, 2}));
+        }
     }
+    __device__ __forceinline__ int most() const { return max((int)top.x, (int)top.y) - 1; }
+    __device__ __forceinline__ int smallest() const { return min((int)least.x, (int)least.y) + 1; }
+    __device__ __forceinline__ bool nan() const { return min((int)low.x, (int)low.y) == 0; }
+};
+#define KV4_SPAN 36                        /* 2^13 2^-36 times half a code is fp16's smallest step */
+
+/* 2^14 less the largest score, in front of an exponential.  Behind 2^25 the difference rounds, up to 16, and 2^16 is no fp16. */
+static __device__ __forceinline__ float kv4_base(float m) {
+    const float b = (float)KV4_P_EXP - m;
+    return m + b > (float)KV4_P_EXP + 1.f ? -m : b;
 }
 
 /* K's pieces of 16 bytes are exchanged within a row in LDS, so that eight rows' same piece lie in different banks */
 template <int HP> static __device__ __forceinline__ int kv4_swizzle(int row, int piece) {
     return HP == 2 ? piece ^ ((row >> 1) & 3) : HP == 4 ? piece ^ (row & 7) : piece ^ ((row >> 2) & 1);
+}
+
+/* One column over `rows` rows, all of which it sees, by a wave in fp32: a lane per row for the scores, per value for the results; -> the largest score, the sum of weights
+ * times 2^14, and the mean of values, value 64 k + lane of it to at[64 k + lane]. */
+template <int HP>
+static __device__ __forceinline__ void kv4_column(const kv4_job &a, const float *q, size_t row0, int rows, int lane, float *at, float &m, float &l) {
+    constexpr int ROW = 32 * HP;
+    float o[HP];
+    m = -3.402823466e38f;
+    l = 0.f;
+#pragma unroll
+    for (int k = 0; k < HP; k++) o[k] = 0.f;
+#pragma unroll 1
+    for (int first = 0; first < rows; first += 64) {
+        const size_t row = row0 + min(first + lane, rows - 1);
+        float s = 0.f;
+#pragma unroll 1
+        for (int u = 0; u < 8 * HP; u++) {               /* eight values */
+            const unsigned w = reinterpret_cast<const unsigned *>(a.k_codes + row * ROW)[u], sc = a.k_scales[row * 2 * HP + u / 4];
+            const f32x4 k0 = vt_mx4_decode4(w & 0xffffu, sc), k1 = vt_mx4_decode4(w >> 16, sc);
+#pragma unroll
+            for (int i = 0; i < 4; i++) s = fmaf(k1[i], q[8 * u + 4 + i] * a.scale, fmaf(k0[i], q[8 * u + i] * a.scale, s));
+        }
+        s = first + lane < rows ? s : -INFINITY;
+        const float top = __any(s != s) ? NAN : fmaxf(m, vt_wave_max(s)), less = __builtin_amdgcn_exp2f(m - top), p = __builtin_amdgcn_exp2f(s - top);
+        l = fmaf(l, less, vt_wave_sum(p));
+        m = m != m ? m : top;
+#pragma unroll
+        for (int k = 0; k < HP; k++) o[k] *= less;
+#pragma unroll 8
+        for (int j = 0; j < 64; j++) {                   /* past the last row: the last again, times 0 */
+            const float w = __shfl(p, j);
+            const size_t r = row0 + min(first + j, rows - 1);
+#pragma unroll
+            for (int k = 0; k < HP; k++) {
+                const int d = 64 * k + lane;
+                const f32x4 v = vt_mx4_decode4((unsigned)a.v_codes[r * ROW + d / 2] >> (4 * (d & 1)), a.v_scales[r * 2 * HP + d / 32]);
+                o[k] = fmaf(w, v.x * 0x1p-24f, o[k]);     /* up to 2^24 rows near the end of the range */
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < HP; k++) at[64 * k + lane] = l == 0.f ? 0.f : __builtin_amdgcn_ldexpf(o[k] / l, 24);
+    l = __builtin_amdgcn_ldexpf(l, KV4_P_EXP);
 }
 
 /* Few columns: a wave streams 32 rows of K and V at a time into LDS of its own, two such tiles on their way while one is multiplied,
@@ -206,8 +268,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
 #pragma unroll
         for (int p = 0; p < KV4_PLANES; p++) asm volatile("" : "+v"(q[ks][p]));       /* here, while the first tiles are on their way, and not behind the loop below */
     }
-    /* largest scale of the wave's values */
-    unsigned most = 0, nan = 0;
+    kv4_span span;                                       /* of the wave's values */
     auto look = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -215,7 +276,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
                 if (i + e == 0 && sub) scan[e] &= 0xffff0000u;
                 if (i + e == words - 1 && ((rows * 2 * HP + sub) & 3)) scan[e] &= 0xffffu;
             }
-            kv4_scan4(scan[e], most, nan);
+            span.add4(scan[e]);
         }
     };
     look(lane * 4);
@@ -223,9 +284,9 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
         scan = __builtin_bit_cast(u32x4, vt_buffer_ld4(vsd, (i + lane * 4) * 4));
         look(i + lane * 4);
     }
-    most = (unsigned)vt_wave_max((float)most);
-    nan = __any((int)nan);
-    const int shift = 127 + KV4_V_EXP - (int)most;
+    const int most = (int)vt_wave_max((float)span.most());
+    const bool nan = __any(span.nan()), wide = __any(most - span.smallest() > KV4_SPAN);
+    const int shift = 127 + KV4_V_EXP - most;
     float minus = -1.f;                                   /* a number that the compiler does not know: fp16 to fp32 and the difference are one instruction */
     asm("" : "+v"(minus));
     float m = -3.402823466e38f, l = 0.f;                  /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
@@ -279,7 +340,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
             for (int i = 0; i < CHUNKS * CD; i++) o[i] = o[i] * less;
             m = top;
         }
-        const float base = (float)KV4_P_EXP - m;
+        const float base = kv4_base(m);
         u32x4 hi4, lo4;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -328,7 +389,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
         asm volatile("" ::: "memory");
         tile(here, t);
     };
-    for (int t = 0; t < tiles; t += 3) {
+    for (int t = wide ? tiles : 0; t < tiles; t += 3) {
         item(t, buf0, buf2);
         if (t + 1 >= tiles) break;
         item(t + 1, buf1, buf0);
@@ -336,7 +397,28 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
         item(t + 2, buf2, buf1);
     }
     l = vt_rows_sum(l);
-    if (nan) {
+    if (wide) {                                          /* o: means of values */
+        __builtin_amdgcn_s_waitcnt(0x0f70);              /* nothing arrives in the buffer any more */
+        float *at = reinterpret_cast<float *>(buf0 + wave * STAGE);
+#pragma unroll 1
+        for (int col = 0; col < nc; col++) {
+            const int c = c0 + col, i = kv4_query(c, inv_group);
+            float cm, cl;
+            kv4_column<HP>(a, a.Q + ((size_t)i * a.n_heads + (size_t)(h * group + c - i * group)) * HD, row0, max(min(rows, a.start + i + 1 - lo), 0), lane, at, cm, cl);
+            __builtin_amdgcn_wave_barrier();             /* the wave's own LDS, in order */
+            if (n == col) {
+                m = cm;
+                l = cl;
+#pragma unroll
+                for (int ch = 0; ch < CHUNKS; ch++)
+#pragma unroll
+                    for (int i = 0; i < CD; i++)
+#pragma unroll
+                        for (int v = 0; v < 4; v++) o[ch * CD + i][v] = at[16 * CD * ch + CD * (4 * g + v) + i];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    } else if (nan) {
         /* rare: the first row of the wave's with a NaN in a block of 32 values reaches the columns that see it */
 #pragma unroll 1
         for (int blk = 0; blk < 2 * HP; blk++) {
@@ -367,14 +449,14 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     for (int k = 0; k < WAVES; k++) L = fmaf(ml[k][n][1], __builtin_amdgcn_exp2f(ml[k][n][0] - M), L);
     const auto area = [&](int w, int col) { return reinterpret_cast<float *>((col < 8 ? buf0 : buf1) + w * STAGE) + (col & 7) * OD; };
     {
-        const float f = L == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - M) / L;
+        const float f = L == 0.f && a.parts > 1 ? 0.f : __builtin_amdgcn_exp2f(m - M) / L * (wide ? l : 1.f);
         float *to = area(wave, n) + 4 * g * CD;
 #pragma unroll
         for (int ch = 0; ch < CHUNKS; ch++)
 #pragma unroll
             for (int v = 0; v < 4; v++)
 #pragma unroll
-                for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * v + i] = __builtin_amdgcn_ldexpf(o[ch * CD + i][v] * f, -shift);
+                for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * v + i] = __builtin_amdgcn_ldexpf(o[ch * CD + i][v] * f, wide ? 0 : -shift);
     }
     __syncthreads();
     const int per = a.parts;
@@ -414,7 +496,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
         const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(pd, (min(lane, per - 1) * KV4_COLS + col) * OD * 4, 0, 16 /* sc1 */);
         const float pm = __uint_as_float(v.x), pl = lane < per ? __uint_as_float(v.y) : 0.f;
         const float w = pl * __builtin_amdgcn_exp2f(pm - vt_wave_max(pm)), all = vt_wave_sum(w);
-        wt[col][lane] = all == 0.f ? 0.f : w / all;
+        wt[col][lane] = w / all;
     }
     __syncthreads();
     for (int e = (int)threadIdx.x; e < nc * (HD / 4); e += 64 * WAVES) {
@@ -446,7 +528,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
     constexpr int HD = 64 * HP, ROW = 32 * HP, THREADS = 64 * KV4_TILE_WAVES, UNITS = 128 * HP, UN = (UNITS + THREADS - 1) / THREADS, DT = 2 * HP;
     constexpr int KB = 64 * ROW, SB = KB + UNITS, VB = SB;      /* K rows, their scales, V's operands */
     __shared__ __attribute__((aligned(16))) unsigned char buf[2][VB + 64 * HD * 2];
-    __shared__ unsigned scan_most[KV4_TILE_WAVES], scan_nan[KV4_TILE_WAVES];
+    __shared__ int scan[KV4_TILE_WAVES][3];
     __shared__ int last;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5, h = (int)blockIdx.y;
     /* The columns that see most first, and their last parts, which others do not have, before these.  (Neighbours go to different XCDs: with the parts of a tile side by
@@ -509,21 +591,21 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
         }
         vt_mx4_planes<KV4_PLANES>(even, odd, q[k], qs[k]);
     }
-    unsigned most = 0, nan = 0;
+    unsigned top = 1, low = 1, least = 0xffffffffu;       /* as in kv4_span */
     for (int i = tid;;) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) { nan |= seen[e] == 255; most = max(most, seen[e] == 255 ? 0u : (unsigned)seen[e]); }
+        for (int e = 0; e < 8; e++) { const unsigned t = (unsigned char)(seen[e] + 1); top = max(top, t); low = min(low, t); least = min(least, t - 2); }
         if ((i += THREADS * 8) - tid >= rows * DT) break;
         ask_scales(i);
     }
-    most = (unsigned)vt_wave_max((float)most);
-    if (lane == 0) scan_most[wave] = most;
-    nan = __any((int)nan);
-    if (lane == 0) scan_nan[wave] = nan;
+    int most = (int)vt_wave_max((float)top) - 1, small = 1 - (int)vt_wave_max(-(float)(int)min(least, 65535u));
+    int nan = __any(low == 0);
+    if (lane == 0) { scan[wave][0] = most; scan[wave][1] = small; scan[wave][2] = nan; }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < KV4_TILE_WAVES; w++) { most = max(most, scan_most[w]); nan |= scan_nan[w]; }
-    const int shift = __builtin_amdgcn_readfirstlane(127 + KV4_V_EXP - (int)most);
+    for (int w = 0; w < KV4_TILE_WAVES; w++) { most = max(most, scan[w][0]); small = min(small, scan[w][1]); nan |= scan[w][2]; }
+    const bool wide = __builtin_amdgcn_readfirstlane(most - small > KV4_SPAN);
+    const int shift = __builtin_amdgcn_readfirstlane(127 + KV4_V_EXP - most);
     /* where value d's four keys go: row r = d / 2 HP of instruction i = d % 2 HP, step t of 16 keys, half h of the lane's eight (step and half by the
      * unit: its keys are 4 (kg % 4) .. of step kg / 4, i.e. group of lanes kg % 2, half kg / 2 % 2) */
     int v_to[2][8];                                       /* UN of them (with that size the host pass drops the kernel) */
@@ -570,7 +652,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
     put(buf[0]);
     __syncthreads();
 #pragma unroll 1
-    for (int t = 0; t < tiles; t++) {
+    for (int t = wide ? tiles : 0; t < tiles; t++) {
         const unsigned char *b = buf[t & 1];
         if (t + 1 < tiles) load(t + 1);
         const int first = lo + 64 * t;
@@ -610,7 +692,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                 for (int i = 0; i < DT; i++) o[i] = o[i] * less;
                 m = top;
             }
-            const float base = (float)KV4_P_EXP - m;
+            const float base = kv4_base(m);
 #pragma unroll
             for (int st = 0; st < 4; st++) {              /* 16 keys: elements 8 (st % 2) .. of scores st / 2 */
                 u32x4 hi4, lo4;
@@ -635,7 +717,25 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
         __syncthreads();
     }
     { const f32x2 r = vt_swap32(l, l); l = r.x + r.y; }
-    if (nan) {
+    if (wide) {                                          /* o: means of values */
+        float *at = reinterpret_cast<float *>(buf[0]) + wave * HD;
+#pragma unroll 1
+        for (int col = 0; col < wc; col++) {
+            const int c = w0 + col, i = vt_div(c, a.group);
+            float cm, cl;
+            kv4_column<HP>(a, a.Q + ((size_t)i * a.n_heads + (size_t)h * a.group.d + (c - i * a.group.d)) * HD, row0, max(min(rows, a.start + i + 1 - lo), 0), lane, at, cm, cl);
+            __builtin_amdgcn_wave_barrier();
+            if (n == col) {
+                m = cm;
+                l = cl;
+#pragma unroll
+                for (int i = 0; i < DT; i++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[i][v] = at[DT * (8 * (v >> 2) + 4 * g + (v & 3)) + i];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    } else if (nan) {
 #pragma unroll 1
         for (int blk = 0; blk < DT; blk++) {
             int at = 0x7fffffff;
@@ -650,9 +750,8 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                     if ((DT * (8 * (v >> 2) + 4 * g + (v & 3)) + i) / 32 == blk && see > at) o[i][v] = NAN;
         }
     }
-    /* the part's mean of values */
-    {
-        const float f = l == 0.f ? 0.f : 1.f / l;
+    if (!wide) {                                         /* the part's mean of values */
+        const float f = l == 0.f && parts > 1 ? 0.f : 1.f / l;
 #pragma unroll
         for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -693,7 +792,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
             f32x4 p[DT * 4];
 #pragma unroll
             for (int x = 0; x < DT * 4; x++) p[x] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(pd, mine + k * PART + x * 1024, 0, 16));
-            const float w = L == 0.f ? 0.f : __uint_as_float(ml.y) * __builtin_amdgcn_exp2f(__uint_as_float(ml.x) - M) / L;
+            const float w = __uint_as_float(ml.y) * __builtin_amdgcn_exp2f(__uint_as_float(ml.x) - M) / L;
 #pragma unroll
             for (int x = 0; x < DT * 4; x++)
 #pragma unroll
