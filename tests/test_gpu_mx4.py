@@ -160,3 +160,19 @@ def test_linear_results_do_not_depend_on_the_call(hip):
     for m in (1, 16, 64, 300):
         x = S.f32_normal((m, 1024), 81)
         assert np.array_equal(linear(hip, x, codes, scales, 512), linear(hip, x, codes, scales, 512))
+
+
+def test_what_is_called_behind_a_memset_runs_behind_it(hip):
+    """Large enough that the memory is still being set when the next call is queued."""
+    lib, rows, k = hip.lib, 4096, 8192
+    dx, dc, ds = H.DevBuf(lib, rows * k * 4), H.DevBuf(lib, rows * k // 2), H.DevBuf(lib, rows * k // 32)
+    for fill in (0x55, 0x3f):
+        lib.tts_hip_memset(dx.ptr, fill, dx.nbytes)
+        assert lib.tts_hip_mx4_quantize(dc.ptr, ds.ptr, dx.ptr, 0, rows, k, 0) == 0
+        lib.tts_hip_memset(dx.ptr, 0, dx.nbytes)
+        assert lib.tts_hip_mx4_dequantize(dx.ptr, dc.ptr, ds.ptr, rows, k, 0) == 0
+        want = M.decode(*M.encode(np.full((1, 32), np.frombuffer(bytes([fill] * 4), np.float32)[0])))
+        assert np.all(dx.to_numpy(np.float32, (rows, k)) == np.float32(want[0, 0]))
+    hip.check()
+    for b in (dx, dc, ds):
+        b.free()

@@ -436,7 +436,9 @@ extern "C" void tts_hip_to_host(void *h_dst, const void *d_src, size_t bytes) {
 extern "C" void tts_hip_memset(void *d_ptr, int value, size_t bytes) {
     (void)hipStreamSynchronize(g_vt.stream);
     (void)vt_step_poll_abort();
-    (void)vt_check(hipMemset(d_ptr, value, bytes), "tts_hip_memset");
+    /* hipMemset returns before the memory is set, and the library's stream does not wait for the null stream */
+    if (vt_check(hipMemset(d_ptr, value, bytes), "tts_hip_memset")) return;
+    (void)vt_check(hipStreamSynchronize(NULL), "tts_hip_memset");
 }
 
 extern "C" void *tts_hip_alloc(size_t bytes) { return vt_dev_alloc(bytes); }
