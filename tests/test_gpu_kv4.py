@@ -238,6 +238,42 @@ def test_attention_nan_beside_values_of_any_size(hip, heads, kv_heads, hd, rows,
     assert np.array_equal(np.isnan(got), nan)
 
 
+@pytest.mark.parametrize("rows,heads", [(3, 4), (1100, 16)])
+def test_a_cache_past_32_bits(hip, rows, heads):
+    """Two heads of 34 million rows, 2.2 GB of codes each: rows at the end of what attention reaches and of the cache; all others are zeros
+    and get the weight of a score of 0."""
+    kv_heads, hd, max_rows, last = 2, 128, 34_000_000, 1 << 24
+    buf = [H.DevBuf(hip.lib, kv_heads * max_rows * n) for n in (hd // 2, hd // 32) * 2]
+    for b in buf:
+        hip.lib.tts_hip_memset(b.ptr, 0, b.nbytes)
+    cache = C.byref(hip.pkg.Kv4(*[b.ptr for b in buf], max_rows, kv_heads, hd))
+    r = np.random.default_rng(11)
+    x = [(r.standard_normal((rows, kv_heads * hd)) * 4).astype(np.float32) for _ in range(2)]
+    dev = [H.DevBuf.from_numpy(hip.lib, a) for a in x]
+    back = [H.DevBuf(hip.lib, a.nbytes) for a in x]
+    decoded = [M.decode(*M.encode(a)) for a in x]
+    for pos in (max_rows - rows, last - rows):
+        assert hip.lib.tts_hip_kv4_append(cache, dev[0].ptr, dev[1].ptr, rows, pos, 0) == 0
+        assert hip.lib.tts_hip_kv4_read(back[0].ptr, back[1].ptr, cache, rows, pos, 0) == 0
+        for b, d in zip(back, decoded):
+            assert np.array_equal(b.to_numpy(np.float32, d.shape), d.astype(np.float32))
+    q = (r.standard_normal((rows, heads * hd)) * 4).astype(np.float32)
+    got = attend(hip, cache, q, last - rows, heads, 1.0).reshape(rows, heads, hd)
+    seen = np.arange(rows)[None] <= np.arange(rows)[:, None]
+    for h in range(heads):
+        kh, vh = (d[:, h * kv_heads // heads * hd:][:, :hd] for d in decoded)
+        s = q.reshape(rows, heads, hd)[:, h].astype(np.float64) @ kh.T
+        m = np.maximum(np.where(seen, s, 0).max(1, keepdims=True), 0)
+        p = np.exp(np.where(seen, s - m, -np.inf))
+        p /= p.sum(1, keepdims=True) + (last - rows) * np.exp(-m)
+        ds = 2.0 ** -20 * (M.block_max(q.reshape(rows, heads, hd)[:, h].astype(np.float64)) @ np.abs(kh).T) + 2.0 ** -18 * (np.abs(q.reshape(rows, heads, hd)[:, h]) @ np.abs(kh).T) + 2.0 ** -21 * np.abs(s)
+        # 2^24 weights of one size are added in 64 parts of 8 waves, 1024 tiles of 32 rows each: chains of 8192 at 2^-24
+        e = 2 * np.where(seen, ds, 0).max(1, keepdims=True) + 2.0 ** -11 + 2.0 ** -23 * m
+        assert np.all(np.abs(got[:, h] - p @ vh) <= e * (p @ np.abs(vh)) + 2.0 ** -38 * np.abs(vh).sum(0)), h
+    for b in buf + dev + back:
+        b.free()
+
+
 def test_a_layer_in_4_bits(hip):
     """A prompt and two decode steps through a layer's attention half and its feed-forward half: norms, projections, rotation, cache,
     attention, residuals, all on the device; against the same in 64 bits on the same 4-bit weights.  The rounding of k and v to

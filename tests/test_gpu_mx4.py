@@ -176,3 +176,43 @@ def test_what_is_called_behind_a_memset_runs_behind_it(hip):
     hip.check()
     for b in (dx, dc, ds):
         b.free()
+
+
+@pytest.mark.parametrize("m", [1, 7, 40, 1100])
+def test_matrices_past_32_bits(hip, m):
+    """4.6 GB of codes, or of results: the last rows are random, the others zeros; quantised from 4.9 GB of values and decoded again."""
+    lib, n, k, tail = hip.lib, 1_100_000, 8192, 70
+    r = np.random.default_rng(13)
+    w = r.standard_normal((tail, k)).astype(np.float32)
+    codes, scales = M.encode_matrix(w)
+    if m == 1:
+        rows = 150_000
+        dx, dc, ds = H.DevBuf(lib, rows * k * 4), H.DevBuf(lib, rows * k // 2), H.DevBuf(lib, rows * k // 32)
+        lib.tts_hip_memset(dx.ptr, 0, dx.nbytes)
+        lib.tts_hip_to_device(dx.at((rows - tail) * k * 4), w.ctypes.data, w.nbytes)
+        assert lib.tts_hip_mx4_quantize(dc.ptr, ds.ptr, dx.ptr, 0, rows, k, 0) == 0
+        lib.tts_hip_memset(dx.ptr, 0x55, dx.nbytes)
+        assert lib.tts_hip_mx4_dequantize(dx.ptr, dc.ptr, ds.ptr, rows, k, 0) == 0
+        for b, want in ((dc, codes), (ds, scales), (dx, M.decode(codes, scales).astype(np.float32))):
+            for at, have in ((b.nbytes - want.nbytes, want), (0, np.zeros_like(want))):
+                got = np.empty_like(want)
+                lib.tts_hip_to_host(got.ctypes.data, b.at(at), got.nbytes)
+                assert np.array_equal(got, have)
+            b.free()
+    dc, ds, dy = H.DevBuf(lib, n * k // 2), H.DevBuf(lib, n * k // 32), H.DevBuf(lib, m * n * 4)
+    x = S.f32_normal((m, k), 90)
+    dx = H.DevBuf.from_numpy(lib, x)
+    for b, tail_bytes in ((dc, codes), (ds, scales)):
+        lib.tts_hip_memset(b.ptr, 0, b.nbytes)
+        lib.tts_hip_to_device(b.at(b.nbytes - tail_bytes.nbytes), tail_bytes.ctypes.data, tail_bytes.nbytes)
+    lib.tts_hip_memset(dy.ptr, 0x55, dy.nbytes)
+    assert lib.tts_hip_linear_mx4(dy.ptr, dx.ptr, dc.ptr, ds.ptr, m, k, n) == 0
+    full = M.decode(codes, scales)
+    for row in (0, m // 2, m - 1):
+        got = np.empty(n, np.float32)
+        lib.tts_hip_to_host(got.ctypes.data, dy.at(row * n * 4), got.nbytes)
+        off = np.abs(got[n - tail:] - x[row].astype(np.float64) @ full.T)
+        assert not got[:n - tail].any() and np.all(off <= tolerance(x[row:row + 1], full)[0])
+    hip.check()
+    for b in (dc, ds, dx, dy):
+        b.free()
