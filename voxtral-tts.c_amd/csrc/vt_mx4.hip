@@ -349,11 +349,15 @@ __global__ void __launch_bounds__(256) vt_mx4_planes_kernel(unsigned char *out, 
 
 struct mxt_job { float *y; const unsigned char *planes; const uint8_t *codes, *scales; int seq_len, out_dim, panels, tiles, cuts, m_tiles; };
 
-/* FM 32 weight rows a wave, NM x NN waves */
-template <int FM, int NM, int NN>
+/* FM 32 weight rows a wave, NM x NN waves.  AHEAD: a workgroup with the CU to itself.  Its barrier stands in front of a panel's last quarter, whose x is in registers by then:
+ * behind it the next panel's operands come from LDS while that quarter is multiplied (else the matrix units wait for them at every panel), half of the panel after that is asked for
+ * there and the other half a quarter later.  Workgroups that share a CU fill such waits for each other and need the longer time to memory: they ask for a quarter of the next
+ * panel behind each of this one's, with the barrier between panels.  us, 512 and 1531 x 9216 x 3072 with AHEAD 48.5 and 108 (without 51.5 and 110), 1000 x 3072 x 4096 and 16 x 131072 x 3072 51 and 80
+ * (without 48 and 73). */
+template <int FM, int NM, int NN, bool AHEAD>
 __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
-    constexpr int THREADS = 64 * NM * NN, BM = 32 * FM * NM, W_BYTES = BM * 64, X_BYTES = NN * 2 * MXT_STEP;
-    constexpr int BUF = W_BYTES + BM * 4 + (X_BYTES + 1023) / 1024 * 1024;       /* a wave's request brings 1 KB */
+    constexpr int THREADS = 64 * NM * NN, BM = 32 * FM * NM, W_BYTES = BM * 64, X_AT = W_BYTES + BM * 4, X_BYTES = NN * 2 * MXT_STEP;
+    constexpr int SPARE = X_AT + (X_BYTES + 1023) / 1024 * 1024, BUF = SPARE + (AHEAD ? 1024 : 0);       /* a wave's request brings 1 KB */
     __shared__ __attribute__((aligned(16))) unsigned char buf0[BUF], buf1[BUF];         /* two arrays: reading one need not wait for what arrives in the other */
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 31, g = lane >> 5, wm = wave % NM, wn = wave / NM;
     const int cut = (int)blockIdx.x % a.cuts, tile = (int)blockIdx.x / a.cuts, mt = tile % a.m_tiles, nt = tile / a.m_tiles;
@@ -369,65 +373,110 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
 #pragma unroll
     for (int i = 0; i < WU; i++) { const int u = i * THREADS + (int)threadIdx.x, r = u >> 2; w_at[i] = r * 64 * a.panels + ((u & 3) ^ ((r >> 1) & 3)) * 16; }
     const int s_at = (int)threadIdx.x * 4 * a.panels;
-    /* a quarter q of a panel's requests, or all of them (-1); past the last panel: zeros, which nobody reads */
-    auto ask = [&](unsigned char *b, int panel, int q) __attribute__((always_inline)) {
+    /* part q of `of` of a panel's requests; past the last panel: zeros, which nobody reads */
+    auto ask = [&](unsigned char *b, int panel, int q, int of) __attribute__((always_inline)) {
         const __amdgpu_buffer_rsrc_t xd = vt_buffer(a.planes + ((size_t)min(panel, p1 - 1) * a.tiles + t0) * 2 * MXT_STEP, panel < p1 ? xt * 2 * MXT_STEP : 0);
         const int dead = panel < p1 ? 0 : 0x40000000;
 #define LDS(at) (__attribute__((address_space(3))) void *)(b + (at))
 #pragma unroll
-        for (int i = 0; i < WU; i++) if (q < 0 || i % 4 == q) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, LDS(i * THREADS * 16 + wave * 1024), 16, (w_at[i] + panel * 64) | dead, 0, 0, 0);
-        if ((q < 0 || q == 3) && wave * 64 < BM) __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, LDS(W_BYTES + wave * 256), 4, (s_at + panel * 4) | dead, 0, 0, 0);
+        for (int i = 0; i < WU; i++) if (i % of == q) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, LDS(i * THREADS * 16 + wave * 1024), 16, (w_at[i] + panel * 64) | dead, 0, 0, 0);
+        /* a wave without a share of a request: AHEAD sends it all the same, for nothing to a spare place, because products move across a branch */
+        const bool has = wave * 64 < BM;
+        if (q == of - 1 && (AHEAD || has))
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, LDS(has ? W_BYTES + wave * 256 : SPARE), 4, has ? (s_at + panel * 4) | dead : 0x40000000, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < XU; i++)
-            if ((q < 0 || (i + 2) % 4 == q) && (i * THREADS + wave * 64) * 16 < X_BYTES)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(xd, LDS(W_BYTES + BM * 4 + i * THREADS * 16 + wave * 1024), 16, (i * THREADS + (int)threadIdx.x) * 16, 0, 0, 0);
+        for (int i = 0; i < XU; i++) {
+            const int at = i * THREADS * 16 + wave * 1024;
+            if ((i + of / 2) % of == q && (AHEAD || at < X_BYTES))
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xd, LDS(at < X_BYTES ? X_AT + at : SPARE), 16, (i * THREADS + (int)threadIdx.x) * 16, 0, 0, 0);
+        }
 #undef LDS
     };
     vt_f32x16 acc[FM];
 #pragma unroll
     for (int f = 0; f < FM; f++) acc[f] = vt_f32x16{};
-    auto step = [&](int panel, const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-        __syncthreads();                                 /* this panel is there, and everybody is through with the one before */
-        u32x4 w[FM][2];
-        int ws[FM], xs[2];
-        const unsigned char *xb = here + W_BYTES + BM * 4 + wn * 2 * MXT_STEP;
+    u32x4 w[FM][2];
+    int ws[FM], xs[2];
+    vt_u32x6 first[2];                                   /* x's smallest plane */
+    const int x_at = wn * 2 * MXT_STEP, x16 = x_at + lane * 16, x8 = x_at + lane * 8, x4_at = x_at + lane * 4;
+    const int w_row = wm * FM * 32 + n, w_piece[2] = {w_row * 64 + (g ^ ((n >> 1) & 3)) * 16, w_row * 64 + ((2 + g) ^ ((n >> 1) & 3)) * 16}, ws_at = w_row * 4;
+    auto x_of = [&](const unsigned char *b, int p, int h) __attribute__((always_inline)) {
+        const u32x4 x4 = *reinterpret_cast<const u32x4 *>(b + x16 + (X_AT + h * MXT_STEP + p * 1536));
+        const u32x2 x2 = *reinterpret_cast<const u32x2 *>(b + x8 + (X_AT + h * MXT_STEP + p * 1536 + 1024));
+        return vt_u32x6{x4.x, x4.y, x4.z, x4.w, x2.x, x2.y};
+    };
+    auto fetch_x = [&](const unsigned char *b) __attribute__((always_inline)) {
+        first[0] = x_of(b, MXR_PLANES - 1, 0);
+        first[1] = x_of(b, MXR_PLANES - 1, 1);
+    };
+    auto fetch_w = [&](const unsigned char *b, int h) __attribute__((always_inline)) {
+        xs[h] = *reinterpret_cast<const int *>(b + x4_at + (X_AT + h * MXT_STEP + MXR_PLANES * 1536));
 #pragma unroll
         for (int f = 0; f < FM; f++) {
-            const int r = (wm * FM + f) * 32 + n;
-#pragma unroll
-            for (int h = 0; h < 2; h++) w[f][h] = *reinterpret_cast<const u32x4 *>(here + r * 64 + ((2 * h + g) ^ ((r >> 1) & 3)) * 16);
-            ws[f] = (int)(*reinterpret_cast<const unsigned *>(here + W_BYTES + r * 4) >> (8 * g));       /* bytes 0 and 2: the lane's block of either half */
+            w[f][h] = *reinterpret_cast<const u32x4 *>(b + w_piece[h] + f * 2048);
         }
+        if (!h) return;
+        int at = ws_at;
+        asm("" : "+v"(at));                              /* else a register for each sum with a buffer's place */
 #pragma unroll
-        for (int h = 0; h < 2; h++) xs[h] = *reinterpret_cast<const int *>(xb + h * MXT_STEP + MXR_PLANES * 1536 + lane * 4);
+        for (int f = 0; f < FM; f++) ws[f] = (int)(*reinterpret_cast<const unsigned *>(b + at + (W_BYTES + f * 128)) >> (8 * g));       /* bytes 0 and 2: the lane's block of either half */
+    };
+    auto meet = [&]() __attribute__((always_inline)) {   /* what was asked for is there, and everybody is through with what the next requests overwrite */
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        __syncthreads();
+    };
+    auto step = [&](int panel, unsigned char *here, unsigned char *other) __attribute__((always_inline)) {
+        constexpr int PIN = AHEAD ? 0 : 0x387;           /* what may not cross: nothing may, or products and requests may not */
+        if (!AHEAD) { meet(); fetch_x(here); fetch_w(here, 0); fetch_w(here, 1); }
         vt_f32x16 sum[FM];
 #pragma unroll
         for (int f = 0; f < FM; f++) sum[f] = vt_f32x16{};
-#define PRODUCTS(p) \
-        _Pragma("unroll") for (int h = 0; h < 2; h++) { \
-            const u32x4 x4 = *reinterpret_cast<const u32x4 *>(xb + h * MXT_STEP + p * 1536 + lane * 16); \
-            const u32x2 x2 = *reinterpret_cast<const u32x2 *>(xb + h * MXT_STEP + p * 1536 + 1024 + lane * 8); \
-            const vt_u32x6 xq = {x4.x, x4.y, x4.z, x4.w, x2.x, x2.y}; \
-            _Pragma("unroll") for (int f = 0; f < FM; f++) \
-                sum[f] = h ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(xq), vt_mfma_e2m1(w[f][1]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, p, xs[1], 2, ws[f]) \
-                           : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(xq), vt_mfma_e2m1(w[f][0]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, p, xs[0], 0, ws[f]); \
-        }
-/* a quarter of the next panel's requests behind each plane's products: all at once they keep the waves of a CU waiting at its address path, 0.5 us of 1.8 a panel.
- * Anything but products and requests may cross. */
-#define STAGE(q) __builtin_amdgcn_sched_barrier(0x387); ask(later, panel + 1, q); __builtin_amdgcn_sched_barrier(0x387);
-        PRODUCTS(3) STAGE(0) PRODUCTS(2) STAGE(1) PRODUCTS(1) STAGE(2) PRODUCTS(0) STAGE(3)
-#undef STAGE
+#define PRODUCTS(p, x, h) \
+        _Pragma("unroll") for (int f = 0; f < FM; f++) \
+            sum[f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(x[h]), vt_mfma_e2m1(w[f][h]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, p, xs[h], 2 * h, ws[f]);
+#define PINNED(...) __builtin_amdgcn_sched_barrier(PIN); __VA_ARGS__ __builtin_amdgcn_sched_barrier(PIN);
+        const vt_u32x6 x2[2] = {x_of(here, 2, 0), x_of(here, 2, 1)};
+        PINNED()
+        PRODUCTS(3, first, 0) PRODUCTS(3, first, 1)
+        PINNED(if (AHEAD) ask(other, panel + 1, 1, 2); else ask(other, panel + 1, 0, 4);)
+        const vt_u32x6 x1[2] = {x_of(here, 1, 0), x_of(here, 1, 1)};
+        PINNED()
+        PRODUCTS(2, x2, 0) PRODUCTS(2, x2, 1)
+        PINNED(if (!AHEAD) ask(other, panel + 1, 1, 4);)
+        const vt_u32x6 x0[2] = {x_of(here, 0, 0), x_of(here, 0, 1)};
+        PINNED()
+        PRODUCTS(1, x1, 0) PRODUCTS(1, x1, 1)
+        PINNED(if (AHEAD) { meet(); fetch_x(other); } else ask(other, panel + 1, 2, 4);)
+        PINNED(if (AHEAD) ask(here, panel + 2, 0, 2);)
+        PRODUCTS(0, x0, 0)
+        PINNED(if (AHEAD) fetch_w(other, 0);)
+        PRODUCTS(0, x0, 1)
+        PINNED(if (AHEAD) fetch_w(other, 1); else ask(other, panel + 1, 3, 4);)
+#undef PINNED
 #undef PRODUCTS
 #pragma unroll
         for (int f = 0; f < FM; f++) acc[f] = acc[f] + sum[f];
+        __builtin_amdgcn_sched_barrier(PIN);
     };
-    ask(buf0, p0, -1);                                       /* every cut has a panel */
+    /* every cut has a panel */
+    if (AHEAD) {
+        ask(buf0, p0, 0, 2);
+        ask(buf0, p0, 1, 2);
+        ask(buf1, p0 + 1, 0, 2);
+        meet();
+        fetch_x(buf0);
+        fetch_w(buf0, 0);
+        fetch_w(buf0, 1);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; q++) ask(buf0, p0, q, 4);
+    }
     for (int panel = p0; panel < p1; panel += 2) {
         step(panel, buf0, buf1);
         if (panel + 1 >= p1) break;
         step(panel + 1, buf1, buf0);
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                  /* nothing arrives in the buffers any more */
     /* element v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4 of x, weight row l % 32 */
     float *y = a.y + (size_t)cut * a.seq_len * a.out_dim;
 #pragma unroll
@@ -448,8 +497,8 @@ struct mxt_tile { int bm, bn, per_cu; float panel_us[3]; };
 static const mxt_tile mxt_tiles[] = {{256, 128, 1, {1.8f}}, {128, 64, 2, {0.72f, 1.2f}}, {128, 32, 3, {0.56f, 0.85f, 1.25f}}};
 #define MXT_MAX_CUTS 16
 
-/* The tile and the cuts of K with the least time by these figures.  us, measured and (planned): 226 x 3072 x 9216 36 (128 x 64 in 4 cuts; others 37 to 130), 1531 x 9216 x 3072
- * 112 (256 x 128 in one; 128 to 154 on the others), 64 x 9216 x 3072 19.5 (128 x 32 in 3), 1000 x 3072 x 4096 51 (128 x 64 in one; 53 and more). */
+/* The tile and the cuts of K with the least time by these figures.  us a call, with the best of the others: 1531 x 9216 x 3072 107 (256 x 128 whole; 131 on 128 x 64), 512 of them 48 (the same;
+ * 57), 400 41 (128 x 64 whole; 47 on 256 x 128), 1000 x 3072 x 4096 47 (128 x 64; 48), 300 x 3072 x 9216 38 (128 x 64 in 4 cuts; 41 in 3), 226 x 3072 x 9216 36, 64 x 9216 x 3072 20 (128 x 32 in 3). */
 static void mxt_plan(int n_cu, int seq_len, int out_dim, int panels, int *best_tile, int *best_cuts) {
     double best = 1e30;
     for (int t = 0; t < 3; t++) {
@@ -496,9 +545,9 @@ static int mx4_linear_tiles(float *d_y, const float *d_x, const uint8_t *d_codes
     const mxt_job a = {cuts > 1 ? (float *)(area + planes) : d_y, area, d_codes, d_scales, seq_len, out_dim, panels, tiles, cuts, m_tiles};
     const long long grid = (long long)m_tiles * n_tiles * cuts;
     if (grid > 0x7fffffffll) { vt_set_error("tts_hip_linear_mx4: %d x %d x %d is too large for one call", seq_len, out_dim, in_dim); return -1; }
-    if (t == 0) hipLaunchKernelGGL((vt_mx4_tile_kernel<4, 2, 4>), dim3((unsigned)grid), dim3(512), 0, g_vt.stream, a);
-    else if (t == 1) hipLaunchKernelGGL((vt_mx4_tile_kernel<2, 2, 2>), dim3((unsigned)grid), dim3(256), 0, g_vt.stream, a);
-    else hipLaunchKernelGGL((vt_mx4_tile_kernel<1, 4, 1>), dim3((unsigned)grid), dim3(256), 0, g_vt.stream, a);
+    if (t == 0) hipLaunchKernelGGL((vt_mx4_tile_kernel<4, 2, 4, true>), dim3((unsigned)grid), dim3(512), 0, g_vt.stream, a);
+    else if (t == 1) hipLaunchKernelGGL((vt_mx4_tile_kernel<2, 2, 2, false>), dim3((unsigned)grid), dim3(256), 0, g_vt.stream, a);
+    else hipLaunchKernelGGL((vt_mx4_tile_kernel<1, 4, 1, false>), dim3((unsigned)grid), dim3(256), 0, g_vt.stream, a);
     if (cuts > 1) vt_launch_sum_planes(d_y, (float *)(area + planes), cuts, (size_t)seq_len * out_dim, (size_t)seq_len * out_dim);
     return 0;
 }
