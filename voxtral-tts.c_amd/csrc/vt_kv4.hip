@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     __shared__ float ml[WAVES][KV4_COLS][2], wt[KV4_COLS][KV4_MAX_CHUNKS];
     __shared__ int last;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const int chunk = (int)blockIdx.x, ct = (int)blockIdx.y, h = (int)blockIdx.z, group = a.group.d;
+    const int chunk = (int)blockIdx.y, ct = (int)blockIdx.z, h = (int)blockIdx.x, group = a.group.d;
     const float inv_group = 1.f / (float)group;
     const int c0 = ct * KV4_COLS, nc = min(KV4_COLS, a.cols - c0);
     /* queries (lane's column, values 32 g .. of each 128) are asked for first: loads return in order.  Columns past the last repeat it; the
@@ -530,10 +530,9 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
     __shared__ __attribute__((aligned(16))) unsigned char buf[2][VB + 64 * HD * 2];
     __shared__ int scan[KV4_TILE_WAVES][3];
     __shared__ int last;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5, h = (int)blockIdx.y;
-    /* The columns that see most first, and their last parts, which others do not have, before these.  (Neighbours go to different XCDs: with the parts of a tile side by
-     * side every second XCD had half as many.) */
-    const int ahead = (int)blockIdx.x / a.tiles, part = a.parts - 1 - ahead, ct = (ahead + 1) * a.tiles - 1 - (int)blockIdx.x;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5, h = (int)blockIdx.x;
+    /* Work is handed out head by head, the columns that see most first, and their last parts, which others do not have, before these. */
+    const int part = a.parts - 1 - (int)blockIdx.z, ct = a.tiles - 1 - (int)blockIdx.y;
     const int c0 = ct * KV4_TILE, nc = min(KV4_TILE, a.cols - c0);
     const int end = a.start + vt_div(c0 + nc - 1, a.group) + 1, parts = ((end + 63) / 64 + a.run - 1) / a.run;
     if (part >= parts) return;
@@ -828,7 +827,7 @@ static int kv4_stream(kv4_job a, int heads, int end) {
     a.parts = (int)((tiles + (long long)a.run * WAVES - 1) / ((long long)a.run * WAVES));
     if (a.parts > 1 && !(a.part = (unsigned char *)vt_scratch(sizeof(float) * (size_t)wgs * a.parts * KV4_COLS * (64 * HP + 4)))) return -1;
     static_assert(sizeof a <= 104, "arguments");
-    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)a.parts, (unsigned)a.tiles, (unsigned)heads), dim3(64 * WAVES), 0, g_vt.stream, a);
+    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)heads, (unsigned)a.parts, (unsigned)a.tiles), dim3(64 * WAVES), 0, g_vt.stream, a);
     return 0;
 }
 
@@ -844,7 +843,7 @@ static int kv4_tiles(kv4_job a, int heads, int end) {
     a.run = (int)run;
     a.parts = (int)((last + run - 1) / run);
     if (a.parts > 1 && !(a.part = (unsigned char *)vt_scratch((size_t)wgs * a.parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
-    hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)(a.tiles * (long long)a.parts), (unsigned)heads), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, a);
+    hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)heads, (unsigned)a.tiles, (unsigned)a.parts), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, a);
     return 0;
 }
 
