@@ -692,23 +692,37 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                 m = top;
             }
             const float base = kv4_base(m);
+            /* 16 keys a step: elements 8 (st % 2) .. of scores st / 2.  The next step's weights are made, and its values read, between this one's products. */
+            u32x4 hi4, lo4;
+            vt_f16x8 v[DT];
+            auto weight = [&](int st, int e) __attribute__((always_inline)) {
+                const float p0 = __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e] + base), p1 = __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e + 1] + base);
+                l += p0 + p1;
+                const vt_f16x2 hi2 = __builtin_convertvector((f32x2{p0, p1}), vt_f16x2);
+                hi4[e] = __builtin_bit_cast(unsigned, hi2);
+                lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{fmaf((float)hi2.x, minus, p0), fmaf((float)hi2.y, minus, p1)}), vt_f16x2));
+            };
+            auto value = [&](int st, int i) __attribute__((always_inline)) { v[i] = __builtin_bit_cast(vt_f16x8, *reinterpret_cast<const u32x4 *>(b + VB + ((i * 4 + st) * 64 + lane) * 16)); };
 #pragma unroll
-            for (int st = 0; st < 4; st++) {              /* 16 keys: elements 8 (st % 2) .. of scores st / 2 */
-                u32x4 hi4, lo4;
+            for (int i = 0; i < DT; i++) value(0, i);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float p0 = __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e] + base), p1 = __builtin_amdgcn_exp2f(s[st >> 1][8 * (st & 1) + 2 * e + 1] + base);
-                    l += p0 + p1;
-                    const vt_f16x2 hi2 = __builtin_convertvector((f32x2{p0, p1}), vt_f16x2);
-                    hi4[e] = __builtin_bit_cast(unsigned, hi2);
-                    lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{fmaf((float)hi2.x, minus, p0), fmaf((float)hi2.y, minus, p1)}), vt_f16x2));
-                }
+            for (int e = 0; e < 4; e++) weight(0, e);
+#pragma unroll
+            for (int st = 0; st < 4; st++) {
                 const vt_f16x8 ph = __builtin_bit_cast(vt_f16x8, hi4), pl = __builtin_bit_cast(vt_f16x8, lo4);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < DT; i++) {
-                    const vt_f16x8 v = __builtin_bit_cast(vt_f16x8, *reinterpret_cast<const u32x4 *>(b + VB + ((i * 4 + st) * 64 + lane) * 16));
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[i], 0, 0, 0);
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i], pl, o[i], 0, 0, 0);
+                    if (st < 3) {
+#pragma unroll
+                        for (int e = 4 * i / DT; e < 4 * (i + 1) / DT; e++) weight(st + 1, e);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i], ph, o[i], 0, 0, 0);
+                    if (st < 3) value(st + 1, i);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -831,17 +845,36 @@ static int kv4_stream(kv4_job a, int heads, int end) {
     return 0;
 }
 
+/* us that a launch takes when its columns' rows, first .. last tiles of them, are cut into runs: 1.75 a tile for a workgroup that has a CU to itself and 2.9 for each of two on one, 3.1 a tile and 12 a
+ * part over all of them, 7 and 1 a part to make one of a column's parts.  Measured and (expected), at runs of 4 / 8 / 12 / 16 / whole: 1531 queries 68 / 53 / 54 / 59 / 55 to 60 (69 / 55 / 51 / 61 / 61),
+ * 2000 of them 104 / 80 / 78 / 68 / 75 (112 / 88 / 79 / 75 / 84), 1000 35 / 36 / 39 / - / 37 (36 / 35 / 40 / - / 37), 1531 behind 2000 207 / 148 / 136 / 136 / 136
+ * (215 / 167 / 153 / 147 / 153), 300 behind 1000 31 / 30 / 33 / 40 / 43 (30 / 31 / 37 / 44 / 46), 300 behind 8000 - / 96 / 95 / 92, in runs of 22 and of 32 82 and 102, 4000 425 / 291 / 262 / 241 / 220
+ * (400 / 306 / 275 / 259 / 218). */
+static float kv4_tiles_us(float run, float first, float last, float wgs, float n_cu) {
+    const float all = 0.5f * (first + last) * wgs;
+    if (run >= last) {                                   /* whole: the longest, and what shares its CU with it */
+        if (wgs > 2.f * n_cu) return 9.f + (3.1f * all + 8.f * wgs) / (2.f * n_cu);
+        const float second = wgs > n_cu ? last - (last - first) * n_cu / wgs : 0.f;
+        return 9.f + 2.9f * second + 1.75f * (last - second);
+    }
+    const float parts = wgs * (0.5f * (first + last) / run + 0.5f), shared = fminf(fmaxf(parts / n_cu - 1.f, 0.f), 1.f);
+    const float behind = parts > 2.f * n_cu ? 0.5f * 1.75f * run * first / last : 0.f;       /* parts of one length in more than one round: half a part on average that has a CU to itself */
+    return 7.f + fmaxf(run * (1.75f + 1.15f * shared) + 7.f + ceilf(last / run), (3.1f * all + 12.f * parts) / (2.f * n_cu) + behind);
+}
+
 template <int HP>
 static int kv4_tiles(kv4_job a, int heads, int end) {
     a.tiles = (a.cols + KV4_TILE - 1) / KV4_TILE;
-    const long long last = ((long long)end + 63) / 64, wgs = (long long)heads * a.tiles, slots = 2ll * (g_vt.n_cu > 0 ? g_vt.n_cu : 256);
-    /* as many parts as there is room for at once, of four tiles and more (400 queries and no rows before: 20 us whole or in runs of 8, 21 in runs of 4; 1000 behind 1000 rows: 69 whole,
-     * 66 in runs of 16, two workgroups on a CU each, 74 to 96 in shorter ones) */
-    long long run = wgs < slots && wgs <= VT_MX4_COUNTERS ? (last + slots / wgs - 1) / (slots / wgs) : last;
-    if (run < 4) run = 4;
-    if (run * KV4_MAX_PARTS < last && wgs <= VT_MX4_COUNTERS) run = (last + KV4_MAX_PARTS - 1) / KV4_MAX_PARTS;
-    a.run = (int)run;
-    a.parts = (int)((last + run - 1) / run);
+    const int last = (end + 63) / 64, first = (a.start + (a.cols < KV4_TILE ? a.cols - 1 : KV4_TILE - 1) / a.group.d + 64) / 64;
+    const long long wgs = (long long)heads * a.tiles;
+    a.run = last;
+    float least = 1e30f;
+    for (int parts = 1; parts <= KV4_MAX_PARTS && (parts == 1 || (wgs <= VT_MX4_COUNTERS && last > 4 * (parts - 1))); parts++) {
+        const int run = (last + parts - 1) / parts;
+        const float us = kv4_tiles_us((float)run, (float)first, (float)last, (float)wgs, g_vt.n_cu > 0 ? (float)g_vt.n_cu : 256.f);
+        if (us < least) { least = us; a.run = run; }
+    }
+    a.parts = (last + a.run - 1) / a.run;
     if (a.parts > 1 && !(a.part = (unsigned char *)vt_scratch((size_t)wgs * a.parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
     hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)heads, (unsigned)a.tiles, (unsigned)a.parts), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, a);
     return 0;
