@@ -26,7 +26,8 @@ static int cache_ok(const char *who, const tts_hip_kv4_t *c, long long first, lo
     return 1;
 }
 
-/* ---- rows into the cache (a lane per eight values) and back (four); K in blockIdx.y = 0 and V in 1 ----------------------- */
+/* ---- rows into the cache (a lane per eight values) and back (four); K in blockIdx.y = 0 and V in 1 -----------------------
+ * Bound by the launch: a row of 8 x 128 takes 1.7 us on the device and 1.5 back, of 4 that a call takes; 1531 rows 4.4 (14 MB, 3.2 TB/s) and 5.3. */
 struct kv4_rows { int n, pos, max_rows, stride, whole; vt_divisor per_row, per_head; };      /* lanes of a row, of a row of one head */
 
 static __device__ __forceinline__ bool kv4_place(const kv4_rows &r, int values, long long &from, size_t &at) {
@@ -199,7 +200,8 @@ static __device__ __forceinline__ void kv4_column(const kv4_job &a, const float 
  * and waits for nobody else; the waves of a workgroup, and then the workgroups of a head, add their parts in a fixed order, the last workgroup
  * to arrive those of all.  K is the A operand of 16 x 16 x 128, V of 16 x 16 x 32: lane l has the values of column n = l % 16, CD of each
  * 16 CD, for the eight keys that its group of 16 lanes has weights of.  Most of a short call is instructions that run once, from a cold instruction cache: the code
- * in front of the loop and behind it is kept short. */
+ * in front of the loop and behind it is kept short.  Bound: one query of 32 heads on 8 with 128 values behind 65535 rows 19.3 us, 71 MB at 3.7 TB/s, of which 7 us do not depend on the rows; behind
+ * 1999 8.7 us, nothing but those. */
 template <int HP, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     constexpr int HD = 64 * HP, ROW = 32 * HP, KS = (HP + 1) / 2, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4;
@@ -518,7 +520,9 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
  * the matrix instruction's operand (A of 32 x 32 x 16, value 2 HP r + i in row r of instruction i; four keys of a value are 8 bytes): the workgroup
  * converts the next rows while it multiplies these, each lane four keys of eight values, so that a conversion serves all columns.  Scores are 32 x 32 x 64.
  * Where there are few columns for the chip, or a prompt's last ones would be behind everybody, several workgroups share a head's rows, `run` tiles
- * each; the last to arrive adds their parts. */
+ * each; the last to arrive adds their parts.  Bound: 4000 queries of 32 heads on 8 with 128 values, 220 us, are 64 tiles for each of 512 workgroups that are there at once, 5000 cycles for the two
+ * of a SIMD, of which 3300 are matrix instructions (20 for scores, 32 for results) and 3600 vector ones, at the clock that their power allows.  Reads of what is multiplied next, and the next weights'
+ * arithmetic, stand between the products, and work is handed out head by head, the longest first: neither 283 us, the one 264, the other 231. */
 #define KV4_TILE_WAVES 4
 #define KV4_TILE (32 * KV4_TILE_WAVES)
 #define KV4_MAX_PARTS 32
@@ -899,8 +903,8 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
         const kv4_job a = {cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, d_out + at, d_Q + at, NULL, g_vt.d_mx4_cnt, cache->max_rows, start_pos + s, n_heads, cols, 0, 1, 0,
                            vt_divisor_of(group, cols), scale * 1.44269504f};
         const int heads = cache->n_kv_heads, end = start_pos + s + n;
-        /* Many columns: from two rounds of the other kernel's workgroups on (200 queries behind 300 rows, 400 of them: 22 us and 16; 400 queries and no rows before, 800: 20 and 28; 1531:
-         * 65 and 120), and for heads of up to 128 values, whose results and queries leave two waves of a SIMD their registers (500 behind 500 rows with 256: 54 and 40). */
+        /* Many columns: from two rounds of the other kernel's workgroups on (us, few columns' kernel and many columns': 100 queries behind 300 rows 8.9 and 20, 200 of them 16 and 22, 250 behind
+         * none 13 and 16, 300 20 and 17), and for heads of up to 128 values, whose results and queries leave two waves of a SIMD their registers (500 behind 500 rows with 256: 40 and 54). */
         int bad;
         if (HP <= 2 && (long long)((cols + KV4_COLS - 1) / KV4_COLS) * cache->n_kv_heads > 2ll * n_cu) bad = HP == 1 ? kv4_tiles<1>(a, heads, end) : kv4_tiles<2>(a, heads, end);
         else bad = HP == 1 ? kv4_stream<1, 8>(a, heads, end) : HP == 2 ? kv4_stream<2, 8>(a, heads, end) : HP == 3 ? kv4_stream<3, 4>(a, heads, end) : kv4_stream<4, 4>(a, heads, end);

@@ -123,7 +123,7 @@ extern "C" int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const 
  * (lines of 128 bytes) straight into LDS of its own, three parts ahead of the one that is multiplied, and it waits for nothing but its own loads; the
  * waves' sums of 16 rows meet in LDS behind a bare barrier.  A panel's products start from zero and are added to the sum by the vector unit, which
  * rounds; the matrix unit cuts at 2^-23.  x's planes have to fit LDS: where they do not, K is cut, the cuts' sums go to memory and the last workgroup
- * of a block of rows to arrive adds them. */
+ * of a block of rows to arrive adds them.  Bound: one row by 131072 x 3072 38.6 us, the stream of the weights at 5.6 TB/s; by 9216 x 3072 7.5 us, launch and first touch. */
 #define MXR_ROWS 8
 #define MXR_WAVES 8
 #define MXR_PLANES 4
@@ -302,7 +302,9 @@ static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * pan
  * x as operand A, weights as they lie as B.  A workgroup's tile of BM weight rows and BN rows of x goes through K by panels of
  * 128: both operands come straight into LDS, one panel ahead.  A wave has 32 rows of x and FM x 32 weight rows, so that an operand of x, the larger one
  * (3 bytes a value), is read once for FM products.  Eight products of a panel, the smallest planes first, start from zero and are added by the
- * vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts are added by a kernel of their own. */
+ * vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts are added by a kernel of their own.  Bound: of 1531 x 9216 x 3072, 103 to 107 us, the planes take 9 and the matrix units 86 with
+ * nothing to wait for (timing-only build without loads; 43 GMAC, four times over), the rest is the operands' way through LDS; of 226 x 3072 x 9216, 34 us, 6 the planes, 4 the sums and 24 the product, whose smaller tiles
+ * bring twice the bytes a product to LDS. */
 #define MXT_STEP (MXR_PLANES * 1536 + 256)               /* bytes of 32 rows x 64 columns of x */
 
 /* A wave has 32 rows by 64 columns; they go through LDS so that its loads are lines (a lane's own 128 bytes come in eight pieces, and with twenty waves on a CU the
