@@ -302,9 +302,9 @@ static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * pan
  * x as operand A, weights as they lie as B.  A workgroup's tile of BM weight rows and BN rows of x goes through K by panels of
  * 128: both operands come straight into LDS, one panel ahead.  A wave has 32 rows of x and FM x 32 weight rows, so that an operand of x, the larger one
  * (3 bytes a value), is read once for FM products.  Eight products of a panel, the smallest planes first, start from zero and are added by the
- * vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts are added by a kernel of their own.  Bound: of 1531 x 9216 x 3072, 103 to 107 us, the planes take 9 and the matrix units 86 with
- * nothing to wait for (timing-only build without loads; 43 GMAC, four times over), the rest is the operands' way through LDS; of 226 x 3072 x 9216, 34 us, 6 the planes, 4 the sums and 24 the product, whose smaller tiles
- * bring twice the bytes a product to LDS. */
+ * vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts are added by a kernel of their own.  Bound: 1531 x 9216 x 3072, 103 to 107 us (9 of
+ * them the planes), would take 86 if the product waited for no load (timing-only build): matrix units, four products of 43 GMAC; the rest is the operands' way through LDS.  226 x 3072 x 9216, 34 us: 6 the
+ * planes, 4 the sums, 24 the product, whose smaller tiles bring twice the bytes to LDS for each. */
 #define MXT_STEP (MXR_PLANES * 1536 + 256)               /* bytes of 32 rows x 64 columns of x */
 
 /* A wave has 32 rows by 64 columns; they go through LDS so that its loads are lines (a lane's own 128 bytes come in eight pieces, and with twenty waves on a CU the
