@@ -354,8 +354,8 @@ struct mxt_job { float *y; const unsigned char *planes; const uint8_t *codes, *s
 /* FM 32 weight rows a wave, NM x NN waves.  AHEAD: a workgroup with the CU to itself.  Its barrier stands in front of a panel's last quarter, whose x is in registers by then:
  * behind it the next panel's operands come from LDS while that quarter is multiplied (else the matrix units wait for them at every panel), half of the panel after that is asked for
  * there and the other half a quarter later.  Workgroups that share a CU fill such waits for each other and need the longer time to memory: they ask for a quarter of the next
- * panel behind each of this one's, with the barrier between panels.  us, 512 and 1531 x 9216 x 3072 with AHEAD 48.5 and 108 (without 51.5 and 110), 1000 x 3072 x 4096 and 16 x 131072 x 3072 51 and 80
- * (without 48 and 73). */
+ * panel behind each of this one's, with the barrier between panels.  us, with AHEAD and without, 512 and 1531 x 9216 x 3072 47.5 and 107 (53 and 114), 1000 x 3072 x 4096 and 16 x 131072 x 3072 51 and 80
+ * (48 and 73). */
 template <int FM, int NM, int NN, bool AHEAD>
 __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
     constexpr int THREADS = 64 * NM * NN, BM = 32 * FM * NM, W_BYTES = BM * 64, X_AT = W_BYTES + BM * 4, X_BYTES = NN * 2 * MXT_STEP;
