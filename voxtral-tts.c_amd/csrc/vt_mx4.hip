@@ -162,11 +162,14 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
         const bool live = ask_block < blocks && p0 + 2 * ask_part < p1;         /* else zeros, which nobody reads */
         const int left = live ? min(16, rows - 16 * ask_block) : 0, panel = live ? p0 + 2 * ask_part : 0;
         const size_t r = (size_t)row0 + (live ? 16 * ask_block : 0);
-        const __amdgpu_buffer_rsrc_t wd = vt_buffer(a.codes + r * 64 * a.panels, left * 64 * a.panels), sd = vt_buffer(a.scales + r * 4 * a.panels, left * 4 * a.panels);
+        /* from the panel on, with no scalar offset: the range check need not know of one.  (Past the last of an odd number of panels the last row's lanes read zeros, others the next row.) */
+        const size_t first = r * a.panels + panel;
+        const int size = max(left * a.panels - panel, 0);
+        const __amdgpu_buffer_rsrc_t wd = vt_buffer(a.codes + first * 64, size * 64), sd = vt_buffer(a.scales + first * 4, size * 4);
         unsigned char *b = buf + wave * MXR_PART;
 #pragma unroll
-        for (int d = 0; d < 2; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, (__attribute__((address_space(3))) void *)(b + d * 1024), 16, w_at + d * 8 * 64 * a.panels, panel * 64, 0, 2);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, (__attribute__((address_space(3))) void *)(b + 2048), 4, s_at, panel * 4, 0, 2);
+        for (int d = 0; d < 2; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, (__attribute__((address_space(3))) void *)(b + d * 1024), 16, w_at + d * 8 * 64 * a.panels, 0, 0, 2);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, (__attribute__((address_space(3))) void *)(b + 2048), 4, s_at, 0, 0, 2);
         if (++ask_part >= parts) { ask_part = 0; ask_block += groups; }
     };
     ask(buf0);
