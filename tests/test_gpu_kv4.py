@@ -202,6 +202,41 @@ def test_attention_scores_of_any_size(hip, heads, kv_heads, hd, rows, pos):
 
 
 @pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
+@pytest.mark.parametrize("top", [2.0 ** 9, 2.0 ** 24, 2.0 ** 25, 1.5 * 2 ** 25, -1.5 * 2 ** 25, 2.0 ** 26, -1.5 * 2 ** 26, 2.0 ** 28])
+@pytest.mark.parametrize("far", [False, True])
+def test_attention_scores_a_step_of_fp32_apart(hip, heads, kv_heads, hd, rows, pos, top, far):
+    """Scores that are fp32 numbers, one and two of fp32's steps u apart (1 where they are smaller), the larger ones in later tiles, waves and
+    parts: weights are 2^-2u, 2^-u and 1, whatever the largest score is.  far: a value 2^-60 times the others, so that some waves go
+    their way through fp32."""
+    n, u = pos + rows, max(float(np.spacing(np.float32(abs(top)))), 1.0)
+    scale = np.float32(0.6931472)
+    assert scale * np.float32(1.44269504) == 1                # scores are in units of log2 e: a whole number's weight is a power of two
+    r = np.random.default_rng(17)
+    step = np.zeros(n)
+    step[n * 6 // 10:], step[n * 9 // 10:] = 1, 2
+    k, v = np.zeros((kv_heads, n, hd), np.float32), r.standard_normal((kv_heads, n, hd)).astype(np.float32)
+    k[..., 0], k[..., 1], k[..., 32] = np.copysign(4, top), 1, step / 2
+    if far:
+        v[:, n // 5] *= np.float32(2.0 ** -60)
+    q = np.zeros((rows, heads, hd), np.float32)
+    q[..., 0], q[..., 1], q[..., 32] = abs(top) / 4, u * (np.arange(rows * heads).reshape(rows, heads) % 4), 2 * u      # neighbouring maxima
+    c = M.Cache(hip, n + 5, kv_heads, hd)
+    c.fill(k, v)
+    got = attend(hip, c.upload(), q.reshape(rows, -1), pos, heads, float(scale)).reshape(rows, heads, hd)
+    kd, vd = c.values(n)
+    c.free()
+    assert np.array_equal(kd, k)
+    seen = np.arange(n)[None] <= pos + np.arange(rows)[:, None]
+    p = np.where(seen, np.exp2(u * step), 0)
+    p /= p.sum(1, keepdims=True)
+    for h in range(heads):
+        vh = vd[h * kv_heads // heads]
+        # weights alike to 2^-21 and the sums' rounding, as in the oracle; small weights and values to 2^-39
+        tol = (2.0 ** -20 + 2.0 ** -23 * (n / 32 + 40)) * (p @ np.abs(vh)) + 2.0 ** -39 * (seen @ np.abs(vh)) + 2.0 ** -39 * np.abs(vh).max()
+        assert np.all(np.abs(got[:, h] - p @ vh) <= tol), (h, float((np.abs(got[:, h] - p @ vh) / tol).max()))
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
 @pytest.mark.parametrize("near", [False, True])
 def test_attention_values_of_any_size(hip, heads, kv_heads, hd, rows, pos, near):
     """A row 2^100 times as large as the others, and one 2^-60 times: who does not see the first has what it has without it, and so, but for a

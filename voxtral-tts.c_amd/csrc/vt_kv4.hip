@@ -141,10 +141,15 @@ struct kv4_span {
 };
 #define KV4_SPAN 36                        /* 2^13 2^-36 times half a code is fp16's smallest step */
 
-/* 2^14 less the largest score, in front of an exponential.  Behind 2^25 the difference rounds, up to 16, and 2^16 is no fp16. */
-static __device__ __forceinline__ float kv4_base(float m) {
-    const float b = (float)KV4_P_EXP - m;
-    return m + b > (float)KV4_P_EXP + 1.f ? -m : b;
+/* What a score has added in front of the exponential: 14 less the column's largest, so that the factor of all weights is 2^14 whatever the
+ * maximum, as the sums' rescaling and joins take it.  From 2^10 on, where rounding 14 - m would show in the factor (behind 2^25 it is off by
+ * up to 4), the maximum is taken off first: the difference to a near score is exact. */
+template <class S, int N>
+static __device__ __forceinline__ float kv4_base(float m, S (&s)[N]) {
+    if (!__any(fabsf(m) >= 0x1p10f)) return (float)KV4_P_EXP - m;
+#pragma unroll
+    for (int i = 0; i < N; i++) s[i] = s[i] - m;
+    return (float)KV4_P_EXP;
 }
 
 /* K's pieces of 16 bytes are exchanged within a row in LDS, so that eight rows' same piece lie in different banks */
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
             for (int i = 0; i < CHUNKS * CD; i++) o[i] = o[i] * less;
             m = top;
         }
-        const float base = kv4_base(m);
+        const float base = kv4_base(m, s);
         u32x4 hi4, lo4;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -695,7 +700,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                 for (int i = 0; i < DT; i++) o[i] = o[i] * less;
                 m = top;
             }
-            const float base = kv4_base(m);
+            const float base = kv4_base(m, s);
             /* 16 keys a step: elements 8 (st % 2) .. of scores st / 2.  The next step's weights are made, and its values read, between this one's products. */
             u32x4 hi4, lo4;
             vt_f16x8 v[DT];
