@@ -258,6 +258,25 @@ def test_attention_values_of_any_size(hip, heads, kv_heads, hd, rows, pos, near)
 
 
 @pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
+@pytest.mark.parametrize("small,large", [(-112, -60), (-118, 0), (-118, 100), (-70, 120)])
+def test_attention_values_that_only_later_queries_see(hip, heads, kv_heads, hd, rows, pos, small, large):
+    """Values of about 2^small, the last row's of 2^large: the queries in front of it have what the small ones make, in 24 bits down to where
+    fp32 has no more, and the last query, who gives the row a weight like the others', has its share of it."""
+    c, q = case(hip, heads, kv_heads, hd, rows, pos)
+    r, n = np.random.default_rng(8), pos + rows
+    k, v = r.standard_normal((2, kv_heads, n, hd)).astype(np.float32)
+    v[:, :-1] *= np.float32(2.0 ** small)
+    v[:, -1] *= np.float32(2.0 ** large)
+    c.fill(k, v)
+    got = attend(hip, c.upload(), q, pos, heads, 0.1)
+    want, tol = oracle(q, *c.values(n), pos, heads, float(np.float32(0.1)), absolute=False)
+    c.free()
+    # besides, a column's parts (8 waves, at most 64 workgroups), their products with their shares and the result are rounded to 2^-149 at the lowest, half a step each
+    tol += 80 * 2.0 ** -150 - 1e-37
+    assert np.all(np.abs(got - want) <= tol), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
 def test_attention_nan_beside_values_of_any_size(hip, heads, kv_heads, hd, rows, pos):
     c, q = case(hip, heads, kv_heads, hd, rows, pos)
     r, n = np.random.default_rng(7), pos + rows

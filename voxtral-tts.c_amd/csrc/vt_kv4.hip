@@ -157,8 +157,9 @@ template <int HP> static __device__ __forceinline__ int kv4_swizzle(int row, int
     return HP == 2 ? piece ^ ((row >> 1) & 3) : HP == 4 ? piece ^ (row & 7) : piece ^ ((row >> 2) & 1);
 }
 
-/* One column over `rows` rows, all of which it sees, by a wave in fp32: a lane per row for the scores, per value for the results; -> the largest score, the sum of weights
- * times 2^14, and the mean of values, value 64 k + lane of it to at[64 k + lane]. */
+/* One column over `rows` rows, all of which it sees, by a wave in fp32: a lane per row for the scores, per value for the results; -> the largest score,
+ * the sum of weights times 2^14, and the mean of values, value 64 k + lane of it to at[64 k + lane].  The mean is kept as
+ * one, row after row: a sum of values near the end of the range would leave it, and scaled down small ones would lose bits. */
 template <int HP>
 static __device__ __forceinline__ void kv4_column(const kv4_job &a, const float *q, size_t row0, int rows, int lane, float *at, float &m, float &l) {
     constexpr int ROW = 32 * HP;
@@ -180,24 +181,24 @@ static __device__ __forceinline__ void kv4_column(const kv4_job &a, const float 
         }
         s = first + lane < rows ? s : -INFINITY;
         const float top = __any(s != s) ? NAN : fmaxf(m, vt_wave_max(s)), less = __builtin_amdgcn_exp2f(m - top), p = __builtin_amdgcn_exp2f(s - top);
-        l = fmaf(l, less, vt_wave_sum(p));
+        const float before = l * less, share = p / (l = before + vt_wave_sum(p));
         m = m != m ? m : top;
 #pragma unroll
-        for (int k = 0; k < HP; k++) o[k] *= less;
+        for (int k = 0; k < HP; k++) o[k] *= before / l;
 #pragma unroll 8
         for (int j = 0; j < 64; j++) {                   /* past the last row: the last again, times 0 */
-            const float w = __shfl(p, j);
+            const float w = __shfl(share, j);
             const size_t r = row0 + min(first + j, rows - 1);
 #pragma unroll
             for (int k = 0; k < HP; k++) {
                 const int d = 64 * k + lane;
                 const f32x4 v = vt_mx4_decode4((unsigned)a.v_codes[r * ROW + d / 2] >> (4 * (d & 1)), a.v_scales[r * 2 * HP + d / 32]);
-                o[k] = fmaf(w, v.x * 0x1p-24f, o[k]);     /* up to 2^24 rows near the end of the range */
+                o[k] = fmaf(w, v.x, o[k]);
             }
         }
     }
 #pragma unroll
-    for (int k = 0; k < HP; k++) at[64 * k + lane] = l == 0.f ? 0.f : __builtin_amdgcn_ldexpf(o[k] / l, 24);
+    for (int k = 0; k < HP; k++) at[64 * k + lane] = o[k];
     l = __builtin_amdgcn_ldexpf(l, KV4_P_EXP);
 }
 
