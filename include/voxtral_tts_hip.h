@@ -368,7 +368,7 @@ int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cache, int n_r
  * of n_kv_heads.  A decode step is seq_len 1; what tts_hip_causal_attention_decode and _prefill are for an
  * fp32 cache.  A row that a query does not see changes nothing in its result, whatever it holds; a query with
  * an infinity or a NaN in it, and one that sees such a key, gives NaN, a value's NaN the 32 values of its block.
- * Q times scale is formed first, in fp32; a score whose sum leaves fp32 makes NaN or counts for nothing.
+ * Q times scale is formed first, in fp32; a score that leaves fp32 makes NaN, also where it is a large negative one.
  * Values whose magnitudes differ by more than 2^36 within a head go through fp32 arithmetic, far slower, with the
  * queries that share their work: rounding, not more, may differ with what a later query of the call sees.  out
  * and Q do not overlap.  At most 2^24 rows, 65535 kv heads and 2^19 heads on each.  Where several workgroups

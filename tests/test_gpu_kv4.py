@@ -277,6 +277,33 @@ def test_attention_values_that_only_later_queries_see(hip, heads, kv_heads, hd, 
 
 
 @pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
+@pytest.mark.parametrize("size", [130, 142, 200, -130, -142])
+@pytest.mark.parametrize("far", [False, True])
+def test_attention_a_score_that_leaves_fp32(hip, heads, kv_heads, hd, rows, pos, size, far):
+    """A key whose score is +-2^|size|, of finite queries: who sees it answers NaN, the others what they answered without it.  far: some waves go their
+    way through fp32."""
+    c, q = case(hip, heads, kv_heads, hd, rows, pos)
+    r, n = np.random.default_rng(9), pos + rows
+    k, v = r.standard_normal((2, kv_heads, n, hd)).astype(np.float32)
+    k[..., 32:] = 0
+    bad = n - 1 - rows // 3
+    if far:
+        v[:, n // 5] *= np.float32(2.0 ** -60)
+    q = q.reshape(rows, heads, hd)
+    q[..., 32:] *= np.float32(2.0 ** 80)                     # against keys of 0
+    q[..., 33] = np.float32(1.375 * 2.0 ** 80)               # more than one plane
+    c.fill(k, v)
+    clean = attend(hip, c.upload(), q.reshape(rows, -1), pos, heads, 1.0).reshape(rows, heads, hd)
+    k[0, bad, 33] = np.copysign(np.float32(2.0 ** (abs(size) - 80)), size)
+    c.fill(k, v)
+    got = attend(hip, c.upload(), q.reshape(rows, -1), pos, heads, 1.0).reshape(rows, heads, hd)
+    c.free()
+    hit = np.zeros(got.shape, bool)
+    hit[pos + np.arange(rows) >= bad, :heads // kv_heads] = True
+    assert np.isfinite(clean).all() and np.isnan(got[hit]).all() and np.array_equal(got[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,pos", BOTH)
 def test_attention_nan_beside_values_of_any_size(hip, heads, kv_heads, hd, rows, pos):
     c, q = case(hip, heads, kv_heads, hd, rows, pos)
     r, n = np.random.default_rng(7), pos + rows

@@ -97,7 +97,7 @@ extern "C" int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cac
  * the order of keys inside an instruction is free, so that weights go from one product to the next in their registers.
  * Rows at hand with scales further apart than fp16 reaches (36 binades) go another way (kv4_column): fp32 all through, rare, and slow: 1 query of 32 heads behind 1999
  * rows 46 us with the call and the wait for it, 1531 behind none 5.9 ms.
- * A score beyond fp32 meets the planes one by one, with signs of their own: it makes NaN or an infinity of either sign.
+ * A score beyond fp32 meets the planes one by one, with signs of their own: what comes out may be an infinity of the wrong sign, and so it counts as NaN.
  * NaN: a key's shows in the scores of who sees it.  A value's scale of 255 is taken for a finite one in the product (a hidden row's weight
  * is 0, and 0 times NaN would reach who does not see it), and behind the last row NaN goes to the columns that see such a row. */
 typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
@@ -152,6 +152,18 @@ static __device__ __forceinline__ float kv4_base(float m, S (&s)[N]) {
     return (float)KV4_P_EXP;
 }
 
+/* Scores are below 2^128 where the largest scales of the queries' planes and of the keys at hand add up to 368 at most: head_dim 256 times 7.75 times 6, times 2^(368 - 254), and the smaller planes'
+ * sixteenths.  Behind that an infinity is one that the sum made: NaN. */
+#define KV4_FINITE 368
+template <class S, int N>
+static __device__ __forceinline__ void kv4_overflow(bool may, S (&s)[N]) {
+    if (!__any(may)) return;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (unsigned v = 0; v < sizeof(S) / sizeof(float); v++) s[i][v] = fabsf(s[i][v]) == INFINITY ? NAN : s[i][v];
+}
+
 /* K's pieces of 16 bytes are exchanged within a row in LDS, so that eight rows' same piece lie in different banks */
 template <int HP> static __device__ __forceinline__ int kv4_swizzle(int row, int piece) {
     return HP == 2 ? piece ^ ((row >> 1) & 3) : HP == 4 ? piece ^ (row & 7) : piece ^ ((row >> 2) & 1);
@@ -179,7 +191,7 @@ static __device__ __forceinline__ void kv4_column(const kv4_job &a, const float 
 #pragma unroll
             for (int i = 0; i < 4; i++) s = fmaf(k1[i], q[8 * u + 4 + i] * a.scale, fmaf(k0[i], q[8 * u + i] * a.scale, s));
         }
-        s = first + lane < rows ? s : -INFINITY;
+        s = first + lane < rows ? (fabsf(s) == INFINITY ? NAN : s) : -INFINITY;
         const float top = __any(s != s) ? NAN : fmaxf(m, vt_wave_max(s)), less = __builtin_amdgcn_exp2f(m - top), p = __builtin_amdgcn_exp2f(s - top);
         const float before = l * less, share = p / (l = before + vt_wave_sum(p));
         m = m != m ? m : top;
@@ -276,6 +288,10 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
 #pragma unroll
         for (int p = 0; p < KV4_PLANES; p++) asm volatile("" : "+v"(q[ks][p]));       /* here, while the first tiles are on their way, and not behind the loop below */
     }
+    unsigned q_scale = 0;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) q_scale = max(q_scale, qs[ks][0]);
+    const int k_most = KV4_FINITE - (int)vt_wave_max((float)q_scale);
     kv4_span span;                                       /* of the wave's values */
     auto look = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
@@ -305,6 +321,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     const int ks_row = wave * STAGE + SC + sub + n * 2 * HP, vs_row = wave * STAGE + SC + 256 + sub + 4 * g * 2 * HP + n * CD / 32;
     auto tile = [&](const unsigned char *buf, int t) __attribute__((always_inline)) {
         f32x4 s[2];
+        int k_scale = 0;
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) {
             u32x4 k[KS];
@@ -316,6 +333,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
                 k[ks] = *reinterpret_cast<const u32x4 *>(buf + k_row + 16 * kt * ROW + kv4_swizzle<HP>(n, p) * 16);      /* the exchange is the same 16 rows on */
                 ksc[ks] = buf[ks_row + 16 * kt * 2 * HP + p];
                 if (half && g >= 2) { k[ks] = u32x4{0u, 0u, 0u, 0u}; ksc[ks] = 0; }
+                k_scale = max(k_scale, ksc[ks]);
             }
             s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -325,6 +343,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
                     s[kt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vt_mfma_e2m1(k[ks]), vt_mfma_e2m3(q[ks][p]), s[kt], VT_MFMA_E2M1, VT_MFMA_E2M3, 0,
                                                                             ksc[ks], 0, (int)qs[ks][p]);
         }
+        kv4_overflow(k_scale > k_most, s);
         const int first = lo + 32 * t;
         if (first + 32 > seen_first) {
 #pragma unroll
@@ -600,6 +619,10 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
         }
         vt_mx4_planes<KV4_PLANES>(even, odd, q[k], qs[k]);
     }
+    unsigned q_scale = 0;
+#pragma unroll
+    for (int k = 0; k < HP; k++) q_scale = max(q_scale, qs[k][0]);
+    const int k_most = KV4_FINITE - (int)vt_wave_max((float)q_scale);
     unsigned top = 1, low = 1, least = 0xffffffffu;       /* as in kv4_span */
     for (int i = tid;;) {
 #pragma unroll
@@ -667,6 +690,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
         const int first = lo + 64 * t;
         if (first < seen_last) {                          /* else nobody of this wave sees these rows */
             vt_f32x16 s[2];
+            int k_scale = 0;
 #pragma unroll
             for (int kt = 0; kt < 2; kt++) {
                 const int row = 32 * kt + n;
@@ -676,6 +700,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                 for (int kk = 0; kk < HP; kk++) {
                     k[kk] = *reinterpret_cast<const u32x4 *>(b + row * ROW + kv4_swizzle<HP>(row, 2 * kk + g) * 16);
                     ksc[kk] = b[KB + row * DT + 2 * kk + g];
+                    k_scale = max(k_scale, ksc[kk]);
                 }
                 s[kt] = vt_f32x16{};
 #pragma unroll
@@ -684,6 +709,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                     for (int kk = 0; kk < HP; kk++)
                         s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m1(k[kk]), vt_mfma_e2m3(q[kk][p]), s[kt], VT_MFMA_E2M1, VT_MFMA_E2M3, 0, ksc[kk], 0, (int)qs[kk][p]);
             }
+            kv4_overflow(k_scale > k_most, s);
             if (first + 64 > seen_first) {
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++)
