@@ -141,28 +141,16 @@ struct kv4_span {
 };
 #define KV4_SPAN 36                        /* 2^13 2^-36 times half a code is fp16's smallest step */
 
-/* What a score has added in front of the exponential: 14 less the column's largest, so that the factor of all weights is 2^14 whatever the
- * maximum, as the sums' rescaling and joins take it.  From 2^10 on, where rounding 14 - m would show in the factor (behind 2^25 it is off by
- * up to 4), the maximum is taken off first: the difference to a near score is exact. */
-template <class S, int N>
-static __device__ __forceinline__ float kv4_base(float m, S (&s)[N]) {
-    if (!__any(fabsf(m) >= 0x1p10f)) return (float)KV4_P_EXP - m;
-#pragma unroll
-    for (int i = 0; i < N; i++) s[i] = s[i] - m;
-    return (float)KV4_P_EXP;
-}
+/* From this largest score m on rounding 14 - m, what a score has added in front of its exponential, would show in the factor 2^14 of all
+ * weights (behind 2^25 it is off by up to 4), which the sums' rescaling and joins take for constant: the maximum is taken off first,
+ * whose difference to a near score is exact. */
+#define KV4_FAR 0x1p10f
 
-/* Scores are below 2^128 where the largest scales of the queries' planes and of the keys at hand add up to 368 at most: head_dim 256 times 7.75 times 6, times 2^(368 - 254), and the smaller planes'
- * sixteenths.  Behind that an infinity is one that the sum made: NaN. */
-#define KV4_FINITE 368
-template <class S, int N>
-static __device__ __forceinline__ void kv4_overflow(bool may, S (&s)[N]) {
-    if (!__any(may)) return;
-#pragma unroll
-    for (int i = 0; i < N; i++)
-#pragma unroll
-        for (unsigned v = 0; v < sizeof(S) / sizeof(float); v++) s[i][v] = fabsf(s[i][v]) == INFINITY ? NAN : s[i][v];
-}
+/* Scores are below 2^128 where neither the queries' planes nor the keys at hand have a larger scale than this: head_dim 256 times 7.75
+ * times 6, times 2^(184 - 127) twice, and the smaller planes' sixteenths.  Else an infinity is one that the sum made: NaN.  (Both of
+ * these looked at where a wave has a branch anyway: with a branch of their own 8.99 us for one query behind 1999 rows, so 8.84.) */
+#define KV4_FINITE 184
+static __device__ __forceinline__ float kv4_seen(float s, bool see) { return !see ? -INFINITY : fabsf(s) == INFINITY ? NAN : s; }
 
 /* K's pieces of 16 bytes are exchanged within a row in LDS, so that eight rows' same piece lie in different banks */
 template <int HP> static __device__ __forceinline__ int kv4_swizzle(int row, int piece) {
@@ -191,7 +179,7 @@ static __device__ __forceinline__ void kv4_column(const kv4_job &a, const float 
 #pragma unroll
             for (int i = 0; i < 4; i++) s = fmaf(k1[i], q[8 * u + 4 + i] * a.scale, fmaf(k0[i], q[8 * u + i] * a.scale, s));
         }
-        s = first + lane < rows ? (fabsf(s) == INFINITY ? NAN : s) : -INFINITY;
+        s = kv4_seen(s, first + lane < rows);
         const float top = __any(s != s) ? NAN : fmaxf(m, vt_wave_max(s)), less = __builtin_amdgcn_exp2f(m - top), p = __builtin_amdgcn_exp2f(s - top);
         const float before = l * less, share = p / (l = before + vt_wave_sum(p));
         m = m != m ? m : top;
@@ -291,7 +279,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     unsigned q_scale = 0;
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) q_scale = max(q_scale, qs[ks][0]);
-    const int k_most = KV4_FINITE - (int)vt_wave_max((float)q_scale);
+    const int k_most = __any(q_scale > KV4_FINITE) ? -1 : KV4_FINITE;
     kv4_span span;                                       /* of the wave's values */
     auto look = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
@@ -313,6 +301,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     const int shift = 127 + KV4_V_EXP - most;
     float minus = -1.f;                                   /* a number that the compiler does not know: fp16 to fp32 and the difference are one instruction */
     asm("" : "+v"(minus));
+    bool far = false;
     float m = -3.402823466e38f, l = 0.f;                  /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
     f32x4 o[CHUNKS * CD];
 #pragma unroll
@@ -343,13 +332,12 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
                     s[kt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vt_mfma_e2m1(k[ks]), vt_mfma_e2m3(q[ks][p]), s[kt], VT_MFMA_E2M1, VT_MFMA_E2M3, 0,
                                                                             ksc[ks], 0, (int)qs[ks][p]);
         }
-        kv4_overflow(k_scale > k_most, s);
         const int first = lo + 32 * t;
-        if (first + 32 > seen_first) {
+        if (first + 32 > seen_first || __any(k_scale > k_most)) {
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-                for (int v = 0; v < 4; v++) s[kt][v] = first + 16 * kt + 4 * g + v < see ? s[kt][v] : -INFINITY;
+                for (int v = 0; v < 4; v++) s[kt][v] = kv4_seen(s[kt][v], first + 16 * kt + 4 * g + v < see);
         }
         float top = m;                                    /* a NaN stays one: who sees it answers NaN */
 #pragma unroll
@@ -366,8 +354,14 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
 #pragma unroll
             for (int i = 0; i < CHUNKS * CD; i++) o[i] = o[i] * less;
             m = top;
+            far = __any(fabsf(m) >= KV4_FAR);
         }
-        const float base = kv4_base(m, s);
+        float base = (float)KV4_P_EXP - m;
+        if (far) {
+            s[0] = s[0] - m;
+            s[1] = s[1] - m;
+            base = (float)KV4_P_EXP;
+        }
         u32x4 hi4, lo4;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -622,7 +616,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
     unsigned q_scale = 0;
 #pragma unroll
     for (int k = 0; k < HP; k++) q_scale = max(q_scale, qs[k][0]);
-    const int k_most = KV4_FINITE - (int)vt_wave_max((float)q_scale);
+    const int k_most = __any(q_scale > KV4_FINITE) ? -1 : KV4_FINITE;
     unsigned top = 1, low = 1, least = 0xffffffffu;       /* as in kv4_span */
     for (int i = tid;;) {
 #pragma unroll
@@ -677,6 +671,7 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
     };
     float minus = -1.f;
     asm("" : "+v"(minus));
+    bool far = false;
     float m = -3.402823466e38f, l = 0.f;
     vt_f32x16 o[DT];
 #pragma unroll
@@ -709,12 +704,11 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                     for (int kk = 0; kk < HP; kk++)
                         s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m1(k[kk]), vt_mfma_e2m3(q[kk][p]), s[kt], VT_MFMA_E2M1, VT_MFMA_E2M3, 0, ksc[kk], 0, (int)qs[kk][p]);
             }
-            kv4_overflow(k_scale > k_most, s);
-            if (first + 64 > seen_first) {
+            if (first + 64 > seen_first || __any(k_scale > k_most)) {
 #pragma unroll
                 for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-                    for (int v = 0; v < 16; v++) s[kt][v] = first + 32 * kt + 8 * (v >> 2) + 4 * g + (v & 3) < see ? s[kt][v] : -INFINITY;
+                    for (int v = 0; v < 16; v++) s[kt][v] = kv4_seen(s[kt][v], first + 32 * kt + 8 * (v >> 2) + 4 * g + (v & 3) < see);
             }
             float top = m;                                /* a NaN stays one: who sees it answers NaN */
 #pragma unroll
@@ -726,8 +720,14 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
 #pragma unroll
                 for (int i = 0; i < DT; i++) o[i] = o[i] * less;
                 m = top;
+                far = __any(fabsf(m) >= KV4_FAR);
             }
-            const float base = kv4_base(m, s);
+            float base = (float)KV4_P_EXP - m;
+            if (far) {
+                s[0] = s[0] - m;
+                s[1] = s[1] - m;
+                base = (float)KV4_P_EXP;
+            }
             /* 16 keys a step: elements 8 (st % 2) .. of scores st / 2.  The next step's weights are made, and its values read, between this one's products. */
             u32x4 hi4, lo4;
             vt_f16x8 v[DT];
