@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     };
     auto item = [&](int t, const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0f70 | (2 * HP + 2));       /* vmcnt: the next tile may be on its way */
+        __builtin_amdgcn_s_waitcnt(0x0070 | (2 * HP + 2));       /* vmcnt: the next tile may be on its way; lgkmcnt(0): what is asked for below overwrites what the last tile read */
         asm volatile("" ::: "memory");
         ask(later, t + 2);
         asm volatile("" ::: "memory");

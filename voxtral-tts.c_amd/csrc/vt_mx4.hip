@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
     int turn = 0, part = 0;
     auto item = [&](const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0f70 | 6);          /* vmcnt: two later parts may be on their way */
+        __builtin_amdgcn_s_waitcnt(0x0070 | 6);          /* vmcnt: two later parts may be on their way; lgkmcnt(0): what is asked for below overwrites what the last part read */
         asm volatile("" ::: "memory");
         ask(later);
         asm volatile("" ::: "memory");
