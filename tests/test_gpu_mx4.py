@@ -216,3 +216,35 @@ def test_matrices_past_32_bits(hip, m):
     hip.check()
     for b in (dc, ds, dx, dy):
         b.free()
+
+
+@pytest.mark.parametrize("cols", [1, 40])
+def test_quantize_more_rows_than_a_launch_has_threads_for(hip, cols):
+    """2^28 rows and a few, 17 GB of codes: rows around the places where a launch ends (2^27 - 8 and 2^28 - 16) and at both
+    ends are random, the others zeros."""
+    lib, rows, wide = hip.lib, (1 << 28) + 3, 48
+    dx, dc, ds = H.DevBuf(lib, rows * cols * 4), H.DevBuf(lib, rows * 64), H.DevBuf(lib, rows * 4)
+    lib.tts_hip_memset(dx.ptr, 0, dx.nbytes)
+    lib.tts_hip_memset(dc.ptr, 0x55, dc.nbytes)
+    lib.tts_hip_memset(ds.ptr, 0x55, ds.nbytes)
+    first = [0, (1 << 27) - 8 - wide // 2, (1 << 28) - 16 - wide // 2]
+    x = [S.f32_normal((min(wide, rows - f), cols), 95 + i) for i, f in enumerate(first)]
+    for f, a in zip(first, x):
+        lib.tts_hip_to_device(dx.at(f * cols * 4), a.ctypes.data, a.nbytes)
+    assert lib.tts_hip_mx4_quantize(dc.ptr, ds.ptr, dx.ptr, 0, rows, cols, 0) == 0
+    lib.tts_hip_memset(dx.ptr, 0x55, dx.nbytes)
+    assert lib.tts_hip_mx4_dequantize(dx.ptr, dc.ptr, ds.ptr, rows, cols, 0) == 0
+    hip.check()
+
+    def rows_of(b, at, width, n, dtype):
+        got = np.empty((n, width), dtype)
+        lib.tts_hip_to_host(got.ctypes.data, b.at(at * got.strides[0]), got.nbytes)
+        return got
+
+    for f, a in list(zip(first, x)) + [(at, np.zeros((wide, cols), np.float32)) for at in (wide, (1 << 27) + wide, (1 << 28) - 1000)]:
+        n = len(a)
+        codes, scales = M.encode_matrix(a)
+        assert np.array_equal(rows_of(dc, f, 64, n, np.uint8), codes) and np.array_equal(rows_of(ds, f, 4, n, np.uint8), scales)
+        assert np.array_equal(rows_of(dx, f, cols, n, np.float32), M.decode(codes, scales)[:, :cols].astype(np.float32))
+    for b in (dx, dc, ds):
+        b.free()

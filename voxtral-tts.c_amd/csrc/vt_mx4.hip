@@ -6,11 +6,10 @@
 #include "vt_state.h"
 #include "vt_gemm.h"
 #include "vt_mx4.h"
+#include "vt_mx4_plans.h"
 #include "vt_requests.h"
 
 #include <math.h>
-
-static int panels_of(int cols) { return cols / 128 + (cols % 128 != 0); }
 
 int vt_mx4_ready(const char *who) {
     if (!g_vt.initialized) { vt_set_error("%s: backend not initialised", who); return 0; }
@@ -22,8 +21,7 @@ int vt_mx4_ready(const char *who) {
 }
 
 /* ---- quantisation and the way back -------------------------------------------------------------------------------
- * A lane takes a unit of a row, eight consecutive values (a quad of lanes a block) on the way in, four on the way back; 2^wide_log lanes lie along a row and the rest of
- * the workgroup on the rows below, whichever width leaves the fewest lanes behind the row's end.  Bound by memory: 9216 x 3072 from bf16 12.3 us, 5.8 TB/s in and out, from
+ * A lane takes a unit of a row, eight consecutive values (a quad of lanes a block) on the way in, four on the way back.  Bound by memory: 9216 x 3072 from bf16 12.3 us, 5.8 TB/s in and out, from
  * fp32 23.3, 5.5 (two, four or eight rows a lane: 12.6 to 26). */
 struct mx4_shape { int rows, cols, stride, units, wide_log; vt_divisor chunks; int whole; };
 
@@ -59,24 +57,11 @@ __global__ void __launch_bounds__(256) vt_mx4_dequantize_kernel(float *x, const 
     vt_mx4_store4(x + (size_t)row * s.stride + 4 * (size_t)unit, left, s.whole && left >= 4, v);
 }
 
-/* Workgroups of a launch over [rows, cols], or 0 where they are too many. */
+/* The launch for as many of `rows` as it has threads for; -> its workgroups */
 static int mx4_grid(mx4_shape *s, const void *x, int item, int rows, int cols, int stride, int values) {
-    s->rows = rows;
-    s->cols = cols;
-    s->stride = stride;
-    s->units = 128 / values * panels_of(cols);
-    s->whole = ((uintptr_t)x & 15) == 0 && (size_t)stride * item % 16 == 0;
-    int best = 8;
-    long long lanes = 0;
-    for (int w = 8; w >= 4; w--) {
-        const long long n = ((long long)(s->units + (1 << w) - 1) >> w) << w;
-        if (lanes == 0 || n < lanes) { best = w; lanes = n; }
-    }
-    s->wide_log = best;
-    const long long chunks = (s->units + (1ll << best) - 1) >> best, tall = ((long long)rows + (256 >> best) - 1) / (256 >> best);
-    if (chunks * tall > 0x7fffffffll) return 0;
-    s->chunks = vt_divisor_of((int)chunks, chunks * tall);
-    return (int)(chunks * tall);
+    const vt_mx4_lanes l = vt_mx4_lanes_of(rows, cols, values);
+    *s = mx4_shape{l.rows, cols, stride, l.units, l.wide_log, vt_divisor_of(l.chunks, l.grid), ((uintptr_t)x & 15) == 0 && (size_t)stride * item % 16 == 0};
+    return l.grid;
 }
 
 static int mx4_shape_ok(const char *who, const void *x, const uint8_t *codes, const uint8_t *scales, int rows, int cols, int stride, int item) {
@@ -96,23 +81,33 @@ extern "C" int tts_hip_mx4_quantize(uint8_t *d_codes, uint8_t *d_scales, const v
     static const char who[] = "tts_hip_mx4_quantize";
     if (x_stride == 0) x_stride = cols;
     if (!mx4_shape_ok(who, d_x, d_codes, d_scales, rows, cols, x_stride, x_bf16 ? 2 : 4) || !vt_mx4_ready(who)) return -1;
+    const size_t row = (size_t)vt_mx4_panels(cols) * 64, item = x_bf16 ? 2 : 4;
     mx4_shape s;
-    const int grid = mx4_grid(&s, d_x, x_bf16 ? 2 : 4, rows, cols, x_stride, 8);
-    if (!grid) { vt_set_error("%s: %d x %d is too large for one call", who, rows, cols); return -1; }
-    if (x_bf16) hipLaunchKernelGGL(vt_mx4_quantize_kernel<uint16_t>, dim3(grid), dim3(256), 0, g_vt.stream, (unsigned *)d_codes, d_scales, (const uint16_t *)d_x, s);
-    else hipLaunchKernelGGL(vt_mx4_quantize_kernel<float>, dim3(grid), dim3(256), 0, g_vt.stream, (unsigned *)d_codes, d_scales, (const float *)d_x, s);
-    return vt_check(hipGetLastError(), who) ? -1 : 0;
+    for (int r = 0; r < rows; r += s.rows) {
+        const char *x = (const char *)d_x + (size_t)r * x_stride * item;
+        unsigned *codes = (unsigned *)(d_codes + r * row);
+        uint8_t *scales = d_scales + r * (row / 16);
+        const int grid = mx4_grid(&s, x, (int)item, rows - r, cols, x_stride, 8);
+        if (x_bf16) hipLaunchKernelGGL(vt_mx4_quantize_kernel<uint16_t>, dim3(grid), dim3(256), 0, g_vt.stream, codes, scales, (const uint16_t *)x, s);
+        else hipLaunchKernelGGL(vt_mx4_quantize_kernel<float>, dim3(grid), dim3(256), 0, g_vt.stream, codes, scales, (const float *)x, s);
+        if (vt_check(hipGetLastError(), who)) return -1;
+    }
+    return 0;
 }
 
 extern "C" int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int rows, int cols, int x_stride) {
     static const char who[] = "tts_hip_mx4_dequantize";
     if (x_stride == 0) x_stride = cols;
     if (!mx4_shape_ok(who, d_x, d_codes, d_scales, rows, cols, x_stride, 4) || !vt_mx4_ready(who)) return -1;
+    const size_t row = (size_t)vt_mx4_panels(cols) * 64;
     mx4_shape s;
-    const int grid = mx4_grid(&s, d_x, 4, rows, cols, x_stride, 4);
-    if (!grid) { vt_set_error("%s: %d x %d is too large for one call", who, rows, cols); return -1; }
-    hipLaunchKernelGGL(vt_mx4_dequantize_kernel, dim3(grid), dim3(256), 0, g_vt.stream, d_x, (const uint16_t *)d_codes, d_scales, s);
-    return vt_check(hipGetLastError(), who) ? -1 : 0;
+    for (int r = 0; r < rows; r += s.rows) {
+        float *x = d_x + (size_t)r * x_stride;
+        const int grid = mx4_grid(&s, x, 4, rows - r, cols, x_stride, 4);
+        hipLaunchKernelGGL(vt_mx4_dequantize_kernel, dim3(grid), dim3(256), 0, g_vt.stream, x, (const uint16_t *)(d_codes + r * row), d_scales + r * (row / 16), s);
+        if (vt_check(hipGetLastError(), who)) return -1;
+    }
+    return 0;
 }
 
 /* ---- linear layer: up to eight rows --------------------------------------------------------------------------------
@@ -496,36 +491,13 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
     }
 }
 
-/* Tiles: weight rows, rows of x, workgroups that a CU holds, and us per panel with one, two, three of them on it (from runs of one cut on part of the chip and on all of
- * it: 226 x 3072 x 9216, 1531 x 9216 x 3072). */
-struct mxt_tile { int bm, bn, per_cu; float panel_us[3]; };
-static const mxt_tile mxt_tiles[] = {{256, 128, 1, {1.8f}}, {128, 64, 2, {0.72f, 1.2f}}, {128, 32, 3, {0.56f, 0.85f, 1.25f}}};
-#define MXT_MAX_CUTS 16
-
-/* The tile and the cuts of K with the least time by these figures.  us a call, with the best of the others: 1531 x 9216 x 3072 107 (256 x 128 whole; 131 on 128 x 64), 512 of them 48 (the same;
- * 57), 400 41 (128 x 64 whole; 47 on 256 x 128), 1000 x 3072 x 4096 47 (128 x 64; 48), 300 x 3072 x 9216 38 (128 x 64 in 4 cuts; 41 in 3), 226 x 3072 x 9216 36, 64 x 9216 x 3072 20 (128 x 32 in 3). */
-static void mxt_plan(int n_cu, int seq_len, int out_dim, int panels, int *best_tile, int *best_cuts) {
-    double best = 1e30;
-    for (int t = 0; t < 3; t++) {
-        const mxt_tile &k = mxt_tiles[t];
-        const double tiles = ceil((double)out_dim / k.bm) * ceil((double)seq_len / k.bn);
-        for (int cuts = 1; cuts <= MXT_MAX_CUTS && cuts <= panels; cuts++) {
-            const double wgs = tiles * cuts, full = floor(wgs / ((double)n_cu * k.per_cu)), rest = wgs - full * n_cu * k.per_cu;
-            const int each = (panels + cuts - 1) / cuts, beside = (int)ceil(rest / n_cu);
-            const double us = each * (full * k.panel_us[k.per_cu - 1] + (beside ? k.panel_us[beside - 1] : 0.0)) + full +
-                              (cuts > 1 ? 2.0 + (double)seq_len * out_dim * 4.0 * (2 * cuts + 1) / 5.0e6 : 0.0);
-            if (us < best) { best = us; *best_tile = t; *best_cuts = cuts; }
-        }
-    }
-}
-
 template <int G> static int mxr_prepare(void) {
     return vt_check(hipFuncSetAttribute((const void *)vt_mx4_rows_kernel<G>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(MXR_LDS_MOST - mxr_lds(G))), "tts_hip_linear_mx4: LDS");
 }
 int vt_mx4_prepare(void) { return mxr_prepare<1>() || mxr_prepare<2>() ? -1 : 0; }
 
 static int mx4_linear_rows(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim, int whole) {
-    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = panels_of(in_dim), g = seq_len <= 4 ? 1 : 2;
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = vt_mx4_panels(in_dim), g = seq_len <= 4 ? 1 : 2;
     const int most = (int)((MXR_LDS_MOST - mxr_lds(g)) / mxr_planes_bytes(seq_len, 1)), cuts = (panels + most - 1) / most, wgs = n_cu / cuts > 0 ? n_cu / cuts : 1;
     mxr_job a = {d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, panels, (panels + cuts - 1) / cuts, cuts, (int)(((long long)out_dim + wgs - 1) / wgs), 2, whole, NULL, g_vt.d_mx4_cnt};
     if (a.rows_per_wg <= 16) a.share_log = 3;          /* no second block for the other waves */
@@ -539,21 +511,18 @@ static int mx4_linear_rows(float *d_y, const float *d_x, const uint8_t *d_codes,
 }
 
 static int mx4_linear_tiles(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim, int whole) {
-    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = panels_of(in_dim), tiles = (seq_len + 31) / 32;
-    int t = 0, cuts = 1;
-    mxt_plan(n_cu, seq_len, out_dim, panels, &t, &cuts);
-    const size_t planes = (size_t)tiles * 2 * panels * MXT_STEP, part = cuts > 1 ? sizeof(float) * (size_t)seq_len * out_dim * cuts : 0;
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = vt_mx4_panels(in_dim), tiles = (seq_len + 31) / 32;
+    const vt_mxt_plan p = vt_mxt_plan_of(n_cu, seq_len, out_dim, panels);
+    const size_t planes = (size_t)tiles * 2 * panels * MXT_STEP, part = p.cuts > 1 ? sizeof(float) * (size_t)seq_len * out_dim * p.cuts : 0;
     unsigned char *area = (unsigned char *)vt_scratch(planes + part);
     if (!area) return -1;
     hipLaunchKernelGGL(vt_mx4_planes_kernel, dim3((tiles * 2 * panels + 3) / 4), dim3(256), 0, g_vt.stream, area, d_x, seq_len, in_dim, panels, tiles, whole);
-    const int m_tiles = (out_dim + mxt_tiles[t].bm - 1) / mxt_tiles[t].bm, n_tiles = (seq_len + mxt_tiles[t].bn - 1) / mxt_tiles[t].bn;
-    const mxt_job a = {cuts > 1 ? (float *)(area + planes) : d_y, area, d_codes, d_scales, seq_len, out_dim, panels, tiles, cuts, m_tiles};
-    const long long grid = (long long)m_tiles * n_tiles * cuts;
-    if (grid > 0x7fffffffll) { vt_set_error("tts_hip_linear_mx4: %d x %d x %d is too large for one call", seq_len, out_dim, in_dim); return -1; }
-    if (t == 0) hipLaunchKernelGGL((vt_mx4_tile_kernel<4, 2, 4, true>), dim3((unsigned)grid), dim3(512), 0, g_vt.stream, a);
-    else if (t == 1) hipLaunchKernelGGL((vt_mx4_tile_kernel<2, 2, 2, false>), dim3((unsigned)grid), dim3(256), 0, g_vt.stream, a);
-    else hipLaunchKernelGGL((vt_mx4_tile_kernel<1, 4, 1, false>), dim3((unsigned)grid), dim3(256), 0, g_vt.stream, a);
-    if (cuts > 1) vt_launch_sum_planes(d_y, (float *)(area + planes), cuts, (size_t)seq_len * out_dim, (size_t)seq_len * out_dim);
+    const mxt_job a = {p.cuts > 1 ? (float *)(area + planes) : d_y, area, d_codes, d_scales, seq_len, out_dim, panels, tiles, p.cuts, p.m_tiles};
+    const dim3 grid((unsigned)p.grid), block(vt_mxt_tiles[p.tile].threads);
+    if (p.tile == 0) hipLaunchKernelGGL((vt_mx4_tile_kernel<4, 2, 4, true>), grid, block, 0, g_vt.stream, a);
+    else if (p.tile == 1) hipLaunchKernelGGL((vt_mx4_tile_kernel<2, 2, 2, false>), grid, block, 0, g_vt.stream, a);
+    else hipLaunchKernelGGL((vt_mx4_tile_kernel<1, 4, 1, false>), grid, block, 0, g_vt.stream, a);
+    if (p.cuts > 1) vt_launch_sum_planes(d_y, (float *)(area + planes), p.cuts, (size_t)seq_len * out_dim, (size_t)seq_len * out_dim);
     return 0;
 }
 
@@ -567,8 +536,7 @@ extern "C" int tts_hip_linear_mx4(float *d_y, const float *d_x, const uint8_t *d
     if (seq_len <= MXR_ROWS) {
         if (mx4_linear_rows(d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, whole)) return -1;
     } else {
-        /* so many rows at a time that the work area stays small beside the operands, and the tiles in one launch countable */
-        const int most = 1 << 14;
+        const int most = vt_mxt_rows(out_dim, vt_mx4_panels(in_dim));
         for (int s = 0; s < seq_len; s += most)
             if (mx4_linear_tiles(d_y + (size_t)s * out_dim, d_x + (size_t)s * in_dim, d_codes, d_scales, seq_len - s < most ? seq_len - s : most, in_dim, out_dim, whole)) return -1;
     }
