@@ -9,6 +9,7 @@
  * into one [18432, 3072] matrix so that a (gate, up) pair is adjacent.
  */
 #include "vt_state.h"
+#include "vt_mx4_plans.h"
 #include "vt_gemm.h"
 
 #include <math.h>

@@ -5,6 +5,7 @@
  */
 #include "vt_state.h"
 #include "vt_mx4.h"
+#include "vt_mx4_plans.h"
 #include "vt_requests.h"
 
 #include <math.h>
@@ -104,8 +105,6 @@ typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
 #define KV4_PLANES 5
 #define KV4_P_EXP 14                       /* weights times 2^14 .. */
 #define KV4_V_EXP 13                       /* .. and values up to 6 times 2^13 are fp16 */
-#define KV4_COLS 16
-#define KV4_MAX_CHUNKS 64
 
 /* 104 bytes: a launch with 112 and more, or one that asks for the size of its grid, takes the host 0.9 us longer (of 2.7) */
 struct kv4_job {
@@ -542,9 +541,6 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
  * each; the last to arrive adds their parts.  Bound: 4000 queries of 32 heads on 8 with 128 values, 220 us, are 64 tiles for each of 512 workgroups that are there at once, 5000 cycles for the two
  * of a SIMD, of which 3300 are matrix instructions (20 for scores, 32 for results) and 3600 vector ones, at the clock that their power allows.  Reads of what is multiplied next, and the next weights'
  * arithmetic, stand between the products, and work is handed out head by head, the longest first: neither 283 us, the one 264, the other 231. */
-#define KV4_TILE_WAVES 4
-#define KV4_TILE (32 * KV4_TILE_WAVES)
-#define KV4_MAX_PARTS 32
 
 template <int HP>
 __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4_job a) {
@@ -858,61 +854,22 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
     }
 }
 
+static_assert(sizeof(kv4_job) <= 104, "arguments");
+
 template <int HP, int WAVES>
-static int kv4_stream(kv4_job a, int heads, int end) {
-    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
-    a.tiles = (a.cols + KV4_COLS - 1) / KV4_COLS;
-    const long long wgs = (long long)a.tiles * heads, tiles = ((long long)end + 31) / 32, slots = (long long)n_cu * (HP == 1 ? 2 : 1);
-    /* Workgroups per head and tile of columns: the number that takes the least time at 3.5 us a round of workgroups, 1.2 us a tile of 128 values a row and 2.8 us for adding parts.
-     * (us at 1 / 2 / 4 / 8 / 32 of them: 1 query behind 300 rows 7.4 / 8.5 / 8.5 / 8.5 / 8.5, behind 1999 13.4 / 11.8 / 9.8 / 9.1 / 9.0, behind 65535 264 / 137 / 73 / 41 / 20, 37 queries
-     * behind 4000, ten tiles of columns, 24 / 20 / 27 / 35 and at 3 18.) */
-    long long best = 1;
-    float least = 1e30f;
-    for (long long chunks = 1; chunks <= KV4_MAX_CHUNKS && (chunks == 1 || (wgs <= VT_MX4_COUNTERS && chunks <= (tiles + WAVES - 1) / WAVES)); chunks++) {
-        const float each = (float)((tiles + chunks * WAVES - 1) / (chunks * WAVES)), rounds = (float)((wgs * chunks + slots - 1) / slots);
-        const float us = rounds * (3.5f + 0.6f * HP * each) + (chunks > 1 ? 2.8f : 0.f);
-        if (us < least) { least = us; best = chunks; }
-    }
-    a.run = (int)((tiles + best * WAVES - 1) / (best * WAVES));
-    a.parts = (int)((tiles + (long long)a.run * WAVES - 1) / ((long long)a.run * WAVES));
-    if (a.parts > 1 && !(a.part = (unsigned char *)vt_scratch(sizeof(float) * (size_t)wgs * a.parts * KV4_COLS * (64 * HP + 4)))) return -1;
-    static_assert(sizeof a <= 104, "arguments");
-    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)heads, (unsigned)a.parts, (unsigned)a.tiles), dim3(64 * WAVES), 0, g_vt.stream, a);
+static int kv4_stream(const kv4_job &a, int heads, long long wgs) {
+    static_assert(WAVES == vt_kv4_waves(HP), "the plan's");
+    kv4_job job = a;
+    if (a.parts > 1 && !(job.part = (unsigned char *)vt_scratch(sizeof(float) * (size_t)wgs * a.parts * KV4_COLS * (64 * HP + 4)))) return -1;
+    hipLaunchKernelGGL((vt_kv4_stream_kernel<HP, WAVES>), dim3((unsigned)heads, (unsigned)a.parts, (unsigned)a.tiles), dim3(64 * WAVES), 0, g_vt.stream, job);
     return 0;
 }
 
-/* us that a launch takes when its columns' rows, first .. last tiles of them, are cut into runs: 1.75 a tile for a workgroup that has a CU to itself and 2.9 for each of two on one, 3.1 a tile and 12 a
- * part over all of them, 7 and 1 a part to make one of a column's parts.  Measured and (expected), at runs of 4 / 8 / 12 / 16 / whole: 1531 queries 68 / 53 / 54 / 59 / 55 to 60 (69 / 55 / 51 / 61 / 61),
- * 2000 of them 104 / 80 / 78 / 68 / 75 (112 / 88 / 79 / 75 / 84), 1000 35 / 36 / 39 / - / 37 (36 / 35 / 40 / - / 37), 1531 behind 2000 207 / 148 / 136 / 136 / 136
- * (215 / 167 / 153 / 147 / 153), 300 behind 1000 31 / 30 / 33 / 40 / 43 (30 / 31 / 37 / 44 / 46), 300 behind 8000 - / 96 / 95 / 92, in runs of 22 and of 32 82 and 102, 4000 425 / 291 / 262 / 241 / 220
- * (400 / 306 / 275 / 259 / 218). */
-static float kv4_tiles_us(float run, float first, float last, float wgs, float n_cu) {
-    const float all = 0.5f * (first + last) * wgs;
-    if (run >= last) {                                   /* whole: the longest, and what shares its CU with it */
-        if (wgs > 2.f * n_cu) return 9.f + (3.1f * all + 8.f * wgs) / (2.f * n_cu);
-        const float second = wgs > n_cu ? last - (last - first) * n_cu / wgs : 0.f;
-        return 9.f + 2.9f * second + 1.75f * (last - second);
-    }
-    const float parts = wgs * (0.5f * (first + last) / run + 0.5f), shared = fminf(fmaxf(parts / n_cu - 1.f, 0.f), 1.f);
-    const float behind = parts > 2.f * n_cu ? 0.5f * 1.75f * run * first / last : 0.f;       /* parts of one length in more than one round: half a part on average that has a CU to itself */
-    return 7.f + fmaxf(run * (1.75f + 1.15f * shared) + 7.f + ceilf(last / run), (3.1f * all + 12.f * parts) / (2.f * n_cu) + behind);
-}
-
 template <int HP>
-static int kv4_tiles(kv4_job a, int heads, int end) {
-    a.tiles = (a.cols + KV4_TILE - 1) / KV4_TILE;
-    const int last = (end + 63) / 64, first = (a.start + (a.cols < KV4_TILE ? a.cols - 1 : KV4_TILE - 1) / a.group.d + 64) / 64;
-    const long long wgs = (long long)heads * a.tiles;
-    a.run = last;
-    float least = 1e30f;
-    for (int parts = 1; parts <= KV4_MAX_PARTS && (parts == 1 || (wgs <= VT_MX4_COUNTERS && last > 4 * (parts - 1))); parts++) {
-        const int run = (last + parts - 1) / parts;
-        const float us = kv4_tiles_us((float)run, (float)first, (float)last, (float)wgs, g_vt.n_cu > 0 ? (float)g_vt.n_cu : 256.f);
-        if (us < least) { least = us; a.run = run; }
-    }
-    a.parts = (last + a.run - 1) / a.run;
-    if (a.parts > 1 && !(a.part = (unsigned char *)vt_scratch((size_t)wgs * a.parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
-    hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)heads, (unsigned)a.tiles, (unsigned)a.parts), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, a);
+static int kv4_tiles(const kv4_job &a, int heads, long long wgs) {
+    kv4_job job = a;
+    if (a.parts > 1 && !(job.part = (unsigned char *)vt_scratch((size_t)wgs * a.parts * KV4_TILE_WAVES * (8 * HP + 1) * 1024))) return -1;
+    hipLaunchKernelGGL(vt_kv4_tile_kernel<HP>, dim3((unsigned)heads, (unsigned)a.tiles, (unsigned)a.parts), dim3(64 * KV4_TILE_WAVES), 0, g_vt.stream, job);
     return 0;
 }
 
@@ -932,14 +889,14 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
     for (int s = 0; s < seq_len; s += most) {
         const int n = seq_len - s < most ? seq_len - s : most, cols = n * group;
         const size_t at = (size_t)s * n_heads * cache->head_dim;
-        const kv4_job a = {cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, d_out + at, d_Q + at, NULL, g_vt.d_mx4_cnt, cache->max_rows, start_pos + s, n_heads, cols, 0, 1, 0,
-                           vt_divisor_of(group, cols), scale * 1.44269504f};
-        const int heads = cache->n_kv_heads, end = start_pos + s + n;
-        /* Many columns: from two rounds of the other kernel's workgroups on (us, few columns' kernel and many columns': 100 queries behind 300 rows 8.9 and 20, 200 of them 16 and 22, 250 behind
-         * none 13 and 16, 300 20 and 17), and for heads of up to 128 values, whose results and queries leave two waves of a SIMD their registers (500 behind 500 rows with 256: 40 and 54). */
+        const int heads = cache->n_kv_heads;
+        const vt_kv4_plan p = vt_kv4_plan_of(n_cu, HP, heads, group, cols, start_pos + s, start_pos + s + n);
+        const kv4_job a = {cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, d_out + at, d_Q + at, NULL, g_vt.d_mx4_cnt, cache->max_rows, start_pos + s, n_heads, cols,
+                           p.run, p.parts, p.tiles, vt_divisor_of(group, cols), scale * 1.44269504f};
+        const long long wgs = (long long)heads * p.tiles;
         int bad;
-        if (HP <= 2 && (long long)((cols + KV4_COLS - 1) / KV4_COLS) * cache->n_kv_heads > 2ll * n_cu) bad = HP == 1 ? kv4_tiles<1>(a, heads, end) : kv4_tiles<2>(a, heads, end);
-        else bad = HP == 1 ? kv4_stream<1, 8>(a, heads, end) : HP == 2 ? kv4_stream<2, 8>(a, heads, end) : HP == 3 ? kv4_stream<3, 4>(a, heads, end) : kv4_stream<4, 4>(a, heads, end);
+        if (p.many) bad = HP == 1 ? kv4_tiles<1>(a, heads, wgs) : kv4_tiles<2>(a, heads, wgs);
+        else bad = HP == 1 ? kv4_stream<1, 8>(a, heads, wgs) : HP == 2 ? kv4_stream<2, 8>(a, heads, wgs) : HP == 3 ? kv4_stream<3, 4>(a, heads, wgs) : kv4_stream<4, 4>(a, heads, wgs);
         if (bad) return -1;
     }
     return vt_check(hipGetLastError(), who) ? -1 : 0;

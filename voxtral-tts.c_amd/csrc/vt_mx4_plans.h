@@ -1,12 +1,14 @@
 /*
  * vt_mx4_plans.h - the 4-bit operators' launches (vt_mx4.hip, vt_kv4.hip) from shapes and the number of CUs: lanes of a conversion,
- * tiles and K cuts of a product.  Host code without HIP, so that a host test can walk it.
+ * tiles and K cuts of a product, workgroups of an attention.  Host code without HIP, so that a host test can walk it.
  */
 #ifndef VT_MX4_PLANS_H
 #define VT_MX4_PLANS_H
 
 #include <math.h>
 #include <stddef.h>
+
+#define VT_MX4_COUNTERS 16384     /* tiles, or heads times tiles of columns, that several workgroups share */
 
 /* A launch has fewer than 2^32 threads in a dimension; workgroups of `threads` of it */
 static inline long long vt_launch_most(int threads) { return 0xffffffffll / threads; }
@@ -68,6 +70,74 @@ static inline vt_mxt_plan vt_mxt_plan_of(int n_cu, int seq_len, int out_dim, int
         }
     }
     return best;
+}
+
+/* ---- attention over a 4-bit cache: columns are queries times heads per kv head --- */
+
+#define KV4_COLS 16                        /* of a workgroup of the kernel for few columns */
+#define KV4_MAX_CHUNKS 64
+#define KV4_TILE_WAVES 4                   /* of the kernel for many, 32 columns a wave */
+#define KV4_TILE (32 * KV4_TILE_WAVES)
+#define KV4_MAX_PARTS 32
+
+/* tiles of columns; tiles of 32 (many: 64) rows to a wave (many: a workgroup), and the workgroups that share a head's rows for a tile of columns */
+struct vt_kv4_plan { int many, tiles, run, parts; };
+
+static constexpr int vt_kv4_waves(int hp) { return hp <= 2 ? 8 : 4; }
+
+/* hp: head_dim / 64; the rows of the columns that see most end at `end` */
+static inline vt_kv4_plan vt_kv4_few(int n_cu, int hp, int heads, int cols, int end) {
+    const int waves = vt_kv4_waves(hp), col_tiles = (cols + KV4_COLS - 1) / KV4_COLS;
+    const long long wgs = (long long)col_tiles * heads, tiles = ((long long)end + 31) / 32, slots = (long long)n_cu * (hp == 1 ? 2 : 1);
+    /* Workgroups per head and tile of columns: the number that takes the least time at 3.5 us a round of workgroups, 1.2 us a tile of 128 values a row and 2.8 us for adding parts.
+     * (us at 1 / 2 / 4 / 8 / 32 of them: 1 query behind 300 rows 7.4 / 8.5 / 8.5 / 8.5 / 8.5, behind 1999 13.4 / 11.8 / 9.8 / 9.1 / 9.0, behind 65535 264 / 137 / 73 / 41 / 20, 37 queries
+     * behind 4000, ten tiles of columns, 24 / 20 / 27 / 35 and at 3 18.) */
+    long long best = 1;
+    float least = 1e30f;
+    for (long long chunks = 1; chunks <= KV4_MAX_CHUNKS && (chunks == 1 || (wgs <= VT_MX4_COUNTERS && chunks <= (tiles + waves - 1) / waves)); chunks++) {
+        const float each = (float)((tiles + chunks * waves - 1) / (chunks * waves)), rounds = (float)((wgs * chunks + slots - 1) / slots);
+        const float us = rounds * (3.5f + 0.6f * hp * each) + (chunks > 1 ? 2.8f : 0.f);
+        if (us < least) { least = us; best = chunks; }
+    }
+    const int run = (int)((tiles + best * waves - 1) / (best * waves));
+    return vt_kv4_plan{0, col_tiles, run, (int)((tiles + (long long)run * waves - 1) / ((long long)run * waves))};
+}
+
+/* us that a launch takes when its columns' rows, first .. last tiles of them, are cut into runs: 1.75 a tile for a workgroup that has a CU to itself and 2.9 for each of two on one, 3.1 a tile and 12 a
+ * part over all of them, 7 and 1 a part to make one of a column's parts.  Measured and (expected), at runs of 4 / 8 / 12 / 16 / whole: 1531 queries 68 / 53 / 54 / 59 / 55 to 60 (69 / 55 / 51 / 61 / 61),
+ * 2000 of them 104 / 80 / 78 / 68 / 75 (112 / 88 / 79 / 75 / 84), 1000 35 / 36 / 39 / - / 37 (36 / 35 / 40 / - / 37), 1531 behind 2000 207 / 148 / 136 / 136 / 136
+ * (215 / 167 / 153 / 147 / 153), 300 behind 1000 31 / 30 / 33 / 40 / 43 (30 / 31 / 37 / 44 / 46), 300 behind 8000 - / 96 / 95 / 92, in runs of 22 and of 32 82 and 102, 4000 425 / 291 / 262 / 241 / 220
+ * (400 / 306 / 275 / 259 / 218). */
+static inline float vt_kv4_tiles_us(float run, float first, float last, float wgs, float n_cu) {
+    const float all = 0.5f * (first + last) * wgs;
+    if (run >= last) {                                   /* whole: the longest, and what shares its CU with it */
+        if (wgs > 2.f * n_cu) return 9.f + (3.1f * all + 8.f * wgs) / (2.f * n_cu);
+        const float second = wgs > n_cu ? last - (last - first) * n_cu / wgs : 0.f;
+        return 9.f + 2.9f * second + 1.75f * (last - second);
+    }
+    const float parts = wgs * (0.5f * (first + last) / run + 0.5f), shared = fminf(fmaxf(parts / n_cu - 1.f, 0.f), 1.f);
+    const float behind = parts > 2.f * n_cu ? 0.5f * 1.75f * run * first / last : 0.f;       /* parts of one length in more than one round: half a part on average that has a CU to itself */
+    return 7.f + fmaxf(run * (1.75f + 1.15f * shared) + 7.f + ceilf(last / run), (3.1f * all + 12.f * parts) / (2.f * n_cu) + behind);
+}
+
+static inline vt_kv4_plan vt_kv4_many(int n_cu, int heads, int group, int cols, int start, int end) {
+    const int col_tiles = (cols + KV4_TILE - 1) / KV4_TILE, last = (end + 63) / 64, first = (start + (cols < KV4_TILE ? cols - 1 : KV4_TILE - 1) / group + 64) / 64;
+    const long long wgs = (long long)heads * col_tiles;
+    int best = last;
+    float least = 1e30f;
+    for (int parts = 1; parts <= KV4_MAX_PARTS && (parts == 1 || (wgs <= VT_MX4_COUNTERS && last > 4 * (parts - 1))); parts++) {
+        const int run = (last + parts - 1) / parts;
+        const float us = vt_kv4_tiles_us((float)run, (float)first, (float)last, (float)wgs, (float)n_cu);
+        if (us < least) { least = us; best = run; }
+    }
+    return vt_kv4_plan{1, col_tiles, best, (last + best - 1) / best};
+}
+
+/* Many columns: from two rounds of the other kernel's workgroups on (us, few columns' kernel and many columns': 100 queries behind 300 rows 8.9 and 20, 200 of them 16 and 22, 250 behind
+ * none 13 and 16, 300 20 and 17), and for heads of up to 128 values, whose results and queries leave two waves of a SIMD their registers (500 behind 500 rows with 256: 40 and 54). */
+static inline vt_kv4_plan vt_kv4_plan_of(int n_cu, int hp, int heads, int group, int cols, int start, int end) {
+    if (hp <= 2 && (long long)((cols + KV4_COLS - 1) / KV4_COLS) * heads > 2ll * n_cu) return vt_kv4_many(n_cu, heads, group, cols, start, end);
+    return vt_kv4_few(n_cu, hp, heads, cols, end);
 }
 
 #endif /* VT_MX4_PLANS_H */

@@ -21,7 +21,6 @@
 #define VT_SEM_PADDED 8320
 #define VT_SEM_VALID_END 8194     /* 2 special + 8192 codes */
 
-#define VT_MX4_COUNTERS 16384     /* tiles, or heads times tiles of columns, that several workgroups share */
 #define VT_PIN_ROWS 2048          /* 25 MB */
 
 /* Second copy of a backbone layer's four matrices, in the order the 128 x 256 tile product reads them
