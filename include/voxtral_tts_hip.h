@@ -341,7 +341,8 @@ int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const uint8_t *d_
                            int rows, int cols, int x_stride);
 /* y[seq_len, out_dim] = x[seq_len, in_dim] W^T, W [out_dim, in_dim] in 4 bits, x and y fp32 and dense: what
  * tts_hip_linear_bf16 is for bf16 weights.  x enters to 2^-16 of the largest of its 32 neighbours at the
- * worst, 5e-7 of a row's norm on values of a normal distribution; sums are fp32.  A row of x with an infinity
+ * worst, 5e-7 of a row's norm on values of a normal distribution (where one of 32 is 1000 times the others, what
+ * is off is 1.3e-4 of these, 8e-7 of the row); sums are fp32.  A row of x with an infinity
  * or a NaN in it gives NaN, a sum that leaves fp32 NaN or an infinity of either sign; blocks of x all below
  * 2^-110 lose bits.  y and x do not overlap.
  * seq_len and out_dim up to 2^30, in_dim up to 2^23.  More than a few rows use the library's work area, which
@@ -368,12 +369,13 @@ int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cache, int n_r
  * of n_kv_heads.  A decode step is seq_len 1; what tts_hip_causal_attention_decode and _prefill are for an
  * fp32 cache.  A row that a query does not see changes nothing in its result, whatever it holds; a query with
  * an infinity or a NaN in it, and one that sees such a key, gives NaN, a value's NaN the 32 values of its block.
- * Q times scale is formed first, in fp32; a score that leaves fp32 makes NaN, also where it is a large negative one.
- * Values whose magnitudes differ by more than 2^36 within a head go through fp32 arithmetic, far slower, with the
- * queries that share their work: rounding, not more, may differ with what a later query of the call sees.  out
- * and Q do not overlap.  At most 2^24 rows, 65535 kv heads and 2^19 heads on each.  Where several workgroups
- * share a head's rows their parts meet in the library's work area, which grows by allocation when a call
- * needs more than any before it. */
+ * Q times scale is formed first, in fp32; a score that leaves fp32 makes NaN, also where it is a large negative
+ * one.  Sums are fp32; a weight enters to 2^-22 of itself and no finer than 2^-39 of the column's largest, and
+ * values below 2^-124 may count as 0.  Values whose magnitudes differ by more than 2^36 within a head go through
+ * fp32 arithmetic, far slower, with the queries that share their work: rounding, not more, may differ with what a
+ * later query of the call sees.  out and Q do not overlap.  At most 2^24 rows, 65535 kv heads and 2^19 heads on
+ * each.  Where several workgroups share a head's rows their parts meet in the library's work area (70 MB for 2000
+ * queries of 32 heads on 8), which grows by allocation when a call needs more than any before it and stays. */
 int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_hip_kv4_t *cache, int seq_len,
                           int start_pos, int n_heads, float scale);
 

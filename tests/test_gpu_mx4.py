@@ -248,3 +248,97 @@ def test_quantize_more_rows_than_a_launch_has_threads_for(hip, cols):
         assert np.array_equal(rows_of(dx, f, cols, n, np.float32), M.decode(codes, scales)[:, :cols].astype(np.float32))
     for b in (dx, dc, ds):
         b.free()
+
+
+# rows of x, weight rows, columns -> tile of vt_mx4_plans.h (weight rows x rows of x) and cuts of K on 256 CUs, which test_mx4_plans_cpu.py asserts: one, two and more panels,
+# odd and even, and ends inside a tile and a panel
+TILES = {(515, 8250, 128): ("256x128", 1), (515, 8250, 200): ("256x128", 1), (515, 8250, 384): ("256x128", 1), (300, 13100, 1300): ("256x128", 1), (515, 8202, 3072): ("256x128", 1),
+         (66, 11514, 3190): ("256x128", 5), (2101, 129, 9216): ("256x128", 15),
+         (97, 9216, 256): ("128x64", 1), (226, 3072, 9216): ("128x64", 5), (64, 9216, 3072): ("128x64", 3), (400, 9000, 1000): ("128x64", 1),
+         (700, 640, 512): ("128x32", 1), (16, 20000, 1000): ("128x32", 1), (9, 9216, 3072): ("128x32", 6)}
+
+
+def random_weights(n, k, seed):
+    """Any codes, scales 2^-12 .. 2^-5: [n, k] -> codes, scales, values"""
+    r = np.random.default_rng(seed)
+    p = M.panels(k)
+    codes, scales = r.integers(0, 256, (n, 64 * p), dtype=np.uint8), r.integers(115, 123, (n, 4 * p), dtype=np.uint8)
+    codes[:, (k + 1) // 2:] = 0
+    if k % 2:
+        codes[:, k // 2] &= 15
+    return codes, scales, M.decode(codes, scales)[:, :k]
+
+
+def sums(x, w):
+    """What is left of tolerance() where x's planes are known: the accumulators and the sums of panels."""
+    return (2.0 ** -20 + 2.0 ** -24 * (x.shape[1] / 64 + 24)) * (np.abs(x) @ np.abs(w).T)
+
+
+@pytest.mark.parametrize("m,n,k", TILES)
+@pytest.mark.parametrize("shift", [0, 1])
+def test_linear_tiles(hip, m, n, k, shift):
+    codes, scales, w = random_weights(n, k, n + k)
+    x = S.f32_normal((m, k), 910 + m + k)
+    y = linear(hip, x, codes, scales, n, shift)
+    off = np.abs(y - x.astype(np.float64) @ w.T)
+    tol = tolerance(x, w)
+    assert np.all(off <= tol), float((off / tol).max())
+    assert np.array_equal(y, linear(hip, x, codes, scales, n, shift))
+
+
+@pytest.mark.parametrize("m,n,k", [(515, 8250, 200), (515, 8250, 384), (66, 11514, 3190), (97, 9216, 256), (16, 20000, 1000)])
+def test_linear_tiles_what_is_not_finite_stays_in_its_row_and_its_column(hip, m, n, k):
+    codes, scales, _ = random_weights(n, k, 17)
+    x = S.f32_normal((m, k), 92)
+    clean = linear(hip, x, codes, scales, n)
+    bad, out = [0, m // 2, m - 1], [5, n // 2, n - 1]
+    for i, (s, r) in enumerate(zip(bad, out)):
+        x[s, (i * k + k // 2) // 3] = (np.inf, np.nan, -np.inf)[i]
+        scales[r, (i * k // 32 + 1) // 3] = 255
+    y = linear(hip, x, codes, scales, n)
+    rows, cols = np.ones(m, bool), np.ones(n, bool)
+    rows[bad], cols[out] = False, False
+    assert np.isfinite(clean).all() and np.array_equal(y[rows][:, cols], clean[rows][:, cols])
+    assert np.isnan(y[~rows]).all() and np.isnan(y[:, ~cols]).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 1000, 3072), (8, 36, 9216), (6, 300, 20000), (8, 513, 12288), (8, 5, 33)])
+def test_linear_eight_rows(hip, m, n, k):
+    codes, scales, w = random_weights(n, k, 18)
+    x = S.f32_normal((m, k), 93)
+    off = np.abs(linear(hip, x, codes, scales, n) - x.astype(np.float64) @ w.T)
+    assert np.all(off <= tolerance(x, w))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 9216, 3072), (8, 3072, 9216), (64, 9216, 3072), (226, 3072, 9216), (515, 8202, 3072), (700, 640, 512)])
+def test_linear_error_of_a_normal_row(hip, m, n, k):
+    """The error as a share of the results' norm on values ~N(0, 1).  Four planes leave 5.24e-7 of x's norm, and so of y's, weights being independent of it.  A panel's sum is
+    cut at 2^-23 in its last product and, of a tile, in the one in front of it: 2^-22 of it at most, 2.4e-7 of the norm of P panels that are independent of each other.  Adding
+    P of them rounds partial sums of sqrt(i) at up to 2^-24, uniformly, i.e. 2^-24 / sqrt(3): sqrt(P / 2) 2^-24 / sqrt(3) of the norm, 2.1e-7 at 72.  Together, as if they all
+    pointed the same way, 9.8e-7; and 2 % for what a finite row's planes are off from 5.24e-7."""
+    codes, scales, w = random_weights(n, k, 19)
+    x = S.f32_normal((m, k), 94)
+    want = x.astype(np.float64) @ w.T
+    off = np.linalg.norm(linear(hip, x, codes, scales, n) - want) / np.linalg.norm(want)
+    bound = 1.02 * 5.24e-7 + 2.0 ** -22 + np.sqrt(M.panels(k) / 2) * 2.0 ** -24 / np.sqrt(3)
+    assert off <= bound, off
+
+
+@pytest.mark.parametrize("m", [1, 4, 7, 40, 300])
+@pytest.mark.parametrize("large", [30.0, 1000.0, 1e6])
+def test_linear_one_value_far_above_its_neighbours(hip, m, large):
+    """A channel of 32 `large` times the others, and no weight on it: what is left of the others by the planes' definition."""
+    n, k = 320, 1024
+    codes, scales, _ = random_weights(n, k, 20)
+    codes = codes.reshape(n, -1, 16)
+    codes[:, :, 2] &= 0x0f                                # value 5 of 32
+    codes = codes.reshape(n, -1)
+    w = M.decode(codes, scales)
+    x = S.f32_normal((m, k), 96)
+    x[:, 5::32] *= np.float32(large)
+    held = M.planes(x, 4)
+    off = np.abs(linear(hip, x, codes, scales, n) - held @ w.T)
+    # a product may be cut at 2^-23 of the largest that the exponents of its 128 columns could make, a large value's with no weight among them
+    top = [np.repeat(np.abs(a).reshape(len(a), -1, 128).max(-1), 128, -1).astype(np.float64) for a in (x, w)]
+    tol = sums(held, w) + 2.0 ** -23 * (top[0] @ top[1].T)
+    assert np.all(off <= tol), float((off / tol).max())

@@ -1,5 +1,8 @@
 """The 4-bit operators' launches (vt_mx4_plans.h), walked on the CPU: the header compiled with g++, 256 CUs."""
 import plansupport as P
+import test_gpu_kv4
+import test_gpu_kv4_many
+import test_gpu_mx4
 
 LANES = r"""
 #include <stdio.h>
@@ -69,3 +72,84 @@ def test_tiles_in_launches_that_the_device_takes():
     out = P.run(TILES)
     checked, halved, bad = map(int, out.splitlines()[-1].split())
     assert checked > 100000 and halved > 100 and bad == 0, out
+
+
+ASK = r"""
+#include <stdio.h>
+#include "vt_mx4_plans.h"
+int main(void) {
+    int m, n, k;
+    while (scanf("%d %d %d", &m, &n, &k) == 3) {
+        const vt_mxt_plan p = vt_mxt_plan_of(256, m, n, vt_mx4_panels(k));
+        printf("%dx%d %d\n", vt_mxt_tiles[p.tile].bm, vt_mxt_tiles[p.tile].bn, p.cuts);
+    }
+    return 0;
+}
+"""
+
+
+def test_the_tiles_that_the_device_tests_are_there_for():
+    cases = test_gpu_mx4.TILES
+    got = [(t, int(c)) for t, c in (line.split() for line in P.run(ASK, "\n".join("%d %d %d" % c for c in cases)).splitlines())]
+    assert got == list(cases.values())
+
+
+ATTENTION = r"""
+#include <stdio.h>
+#include "vt_mx4_plans.h"
+int main(void) {
+    long long checked = 0, many = 0, shared = 0, bad = 0;
+    for (int hp = 1; hp <= 4; hp++)
+        for (long long heads = 1; heads <= 65535; heads += 1 + heads / 2)
+            for (long long group = 1; group <= 1 << 19; group += 1 + group / 2)
+                for (long long rows = 1; rows * group <= 1 << 19; rows += 1 + rows / 2)
+                    for (long long start = 0; start + rows <= 1 << 24; start += 1 + start) {
+                        const int cols = (int)(rows * group), end = (int)(start + rows);
+                        const vt_kv4_plan p = vt_kv4_plan_of(256, hp, (int)heads, (int)group, cols, (int)start, end);
+                        const int wide = p.many ? KV4_TILE : KV4_COLS, tall = p.many ? 64 : 32 * vt_kv4_waves(hp);
+                        const long long covered = (long long)p.parts * p.run * tall, row = 32 * hp;
+                        /* a wave's (many: a workgroup's) codes through one descriptor, and where its requests for the two tiles behind end */
+                        const long long bytes = ((long long)p.run * (p.many ? 64 : 32) + 128) * row;
+                        const int wrong = p.tiles != (cols + wide - 1) / wide || p.run < 1 || p.parts < 1 || p.parts > (p.many ? KV4_MAX_PARTS : KV4_MAX_CHUNKS) || covered < end ||
+                                          covered - (long long)p.run * tall >= end || covered > 0x7fffffff || (p.parts > 1 && heads * p.tiles > VT_MX4_COUNTERS) || bytes > 0x7fffffff ||
+                                          p.tiles > 65535 || p.parts > 65535 || (p.many && hp > 2);
+                        checked++;
+                        many += p.many;
+                        shared += p.parts > 1;
+                        if (wrong && bad++ < 5)
+                            printf("hp %d, %lld heads, group %lld, %lld rows behind %lld: %s, %d tiles, run %d, %d parts\n", hp, heads, group, rows, start, p.many ? "many" : "few", p.tiles, p.run, p.parts);
+                    }
+    printf("%lld %lld %lld %lld\n", checked, many, shared, bad);
+    return 0;
+}
+"""
+
+
+def test_every_row_of_an_attention_in_a_part_and_a_counter_for_every_shared_tile():
+    out = P.run(ATTENTION)
+    checked, many, shared, bad = map(int, out.splitlines()[-1].split())
+    assert checked > 100000 and many > 10000 and shared > 10000 and bad == 0, out
+
+
+ASK_ATTENTION = r"""
+#include <stdio.h>
+#include "vt_mx4_plans.h"
+int main(void) {
+    int heads, kv, hd, rows, pos;
+    while (scanf("%d %d %d %d %d", &heads, &kv, &hd, &rows, &pos) == 5) {
+        const vt_kv4_plan p = vt_kv4_plan_of(256, hd / 64, kv, heads / kv, heads / kv * rows, pos, pos + rows);
+        printf("%d %d\n", p.many, p.parts);
+    }
+    return 0;
+}
+"""
+
+
+def attention(cases):
+    return [tuple(map(int, line.split())) for line in P.run(ASK_ATTENTION, "\n".join("%d %d %d %d %d" % c for c in cases)).splitlines()]
+
+
+def test_the_kernels_that_the_device_tests_are_there_for():
+    many = test_gpu_kv4_many.CASES
+    assert attention(many) == [(1, parts) for parts in many.values()]
+    assert [m for m, _ in attention(test_gpu_kv4.BOTH)] == [0, 0, 0, 0, 1, 1, 1]
