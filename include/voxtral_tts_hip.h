@@ -340,11 +340,10 @@ int tts_hip_mx4_quantize(uint8_t *d_codes, uint8_t *d_scales, const void *d_x, i
 int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const uint8_t *d_scales,
                            int rows, int cols, int x_stride);
 /* y[seq_len, out_dim] = x[seq_len, in_dim] W^T, W [out_dim, in_dim] in 4 bits, x and y fp32 and dense: what
- * tts_hip_linear_bf16 is for bf16 weights.  x enters to 2^-16 of the largest of its 32 neighbours at the
- * worst, 5e-7 of a row's norm on values of a normal distribution (where one of 32 is 1000 times the others, what
- * is off is 1.3e-4 of these, 8e-7 of the row); sums are fp32.  A row of x with an infinity
- * or a NaN in it gives NaN, a sum that leaves fp32 NaN or an infinity of either sign; blocks of x all below
- * 2^-110 lose bits.  y and x do not overlap.
+ * tts_hip_linear_bf16 is for bf16 weights.  x enters to 2^-21 of the largest of its 32 neighbours at the worst,
+ * 2e-8 of a row's norm on values of a normal distribution; sums are fp32: results are off by 1e-7 of their norm.
+ * A row of x with an infinity or a NaN in it gives NaN, a sum that leaves fp32 NaN or an infinity of either sign;
+ * blocks of x all below 2^-106 lose bits.  y and x do not overlap.
  * seq_len and out_dim up to 2^30, in_dim up to 2^23.  More than a few rows use the library's work area, which
  * grows by allocation when a call needs more than any before it. */
 int tts_hip_linear_mx4(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales,

@@ -83,15 +83,16 @@ class Cache:
         self.buf = {}
 
 
-def planes(x, n):
+def planes(x, n=5):
     """What n planes of e2m3 (0 .. 2 in steps of 1/8, 2 .. 4 of 1/4, 4 .. 7.5 of 1/2) hold of [rows, cols] fp32: each the nearest to what the ones before leave of
-    its block of 32, with a scale of its own that puts the largest magnitude at 3.875 .. 7.75."""
+    its block of 32, with a scale of its own that puts the largest magnitude at 3.875 .. 7.75, the fifth's 2^-4 of the fourth's."""
     rows, cols = x.shape
     left = np.concatenate((x, np.zeros((rows, -cols % 32), np.float32)), 1).reshape(rows, -1, 32).astype(np.float32)
     held = np.zeros(left.shape)
-    for _ in range(n):
+    for i in range(n):
         top = np.abs(left).max(-1, keepdims=True).view(np.uint32).astype(np.int64)
-        unit = np.exp2(np.maximum(((top + 0x80000) >> 23) - 2, 0).astype(np.float64) - 127)
+        scale = np.maximum((top + 0x80000 >> 23) - 2 if i < 4 else scale - 4, 0)
+        unit = np.exp2(scale.astype(np.float64) - 127)
         a = np.abs(left) / unit
         step = np.where(a < 2, 0.125, np.where(a < 4, 0.25, 0.5))
         q = np.copysign(np.minimum(np.round(a / step) * step, 7.5), left) * unit

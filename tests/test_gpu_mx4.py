@@ -312,15 +312,15 @@ def test_linear_eight_rows(hip, m, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(1, 9216, 3072), (8, 3072, 9216), (64, 9216, 3072), (226, 3072, 9216), (515, 8202, 3072), (700, 640, 512)])
 def test_linear_error_of_a_normal_row(hip, m, n, k):
-    """The error as a share of the results' norm on values ~N(0, 1).  Four planes leave 5.24e-7 of x's norm, and so of y's, weights being independent of it.  A panel's sum is
+    """The error as a share of the results' norm on values ~N(0, 1).  Five planes leave 2.0e-8 of x's norm, and so of y's, weights being independent of it.  A panel's sum is
     cut at 2^-23 in its last product and, of a tile, in the one in front of it: 2^-22 of it at most, 2.4e-7 of the norm of P panels that are independent of each other.  Adding
     P of them rounds partial sums of sqrt(i) at up to 2^-24, uniformly, i.e. 2^-24 / sqrt(3): sqrt(P / 2) 2^-24 / sqrt(3) of the norm, 2.1e-7 at 72.  Together, as if they all
-    pointed the same way, 9.8e-7; and 2 % for what a finite row's planes are off from 5.24e-7."""
+    pointed the same way, 4.7e-7 (four planes leave 5.2e-7); and 2 % for what a finite row's planes are off from 2.0e-8."""
     codes, scales, w = random_weights(n, k, 19)
     x = S.f32_normal((m, k), 94)
     want = x.astype(np.float64) @ w.T
     off = np.linalg.norm(linear(hip, x, codes, scales, n) - want) / np.linalg.norm(want)
-    bound = 1.02 * 5.24e-7 + 2.0 ** -22 + np.sqrt(M.panels(k) / 2) * 2.0 ** -24 / np.sqrt(3)
+    bound = 1.02 * 2.0e-8 + 2.0 ** -22 + np.sqrt(M.panels(k) / 2) * 2.0 ** -24 / np.sqrt(3)
     assert off <= bound, off
 
 
@@ -336,9 +336,22 @@ def test_linear_one_value_far_above_its_neighbours(hip, m, large):
     w = M.decode(codes, scales)
     x = S.f32_normal((m, k), 96)
     x[:, 5::32] *= np.float32(large)
-    held = M.planes(x, 4)
+    held = M.planes(x)
     off = np.abs(linear(hip, x, codes, scales, n) - held @ w.T)
     # a product may be cut at 2^-23 of the largest that the exponents of its 128 columns could make, a large value's with no weight among them
     top = [np.repeat(np.abs(a).reshape(len(a), -1, 128).max(-1), 128, -1).astype(np.float64) for a in (x, w)]
     tol = sums(held, w) + 2.0 ** -23 * (top[0] @ top[1].T)
     assert np.all(off <= tol), float((off / tol).max())
+
+
+@pytest.mark.parametrize("m", [1, 4, 7, 40, 600])
+def test_linear_holds_every_value(hip, m):
+    """Weights that pick one column each: x comes back to 2^-21 of the largest of its block, as its planes hold it, and each of the five planes' products cut at 2^-23 of
+    what the block's exponents could make."""
+    k = 300
+    w = np.eye(k, dtype=np.float32)
+    codes, scales = M.encode_matrix(w)
+    r = np.random.default_rng(21)
+    x = (r.standard_normal((m, k)) * np.exp2(r.integers(-12, 12, (m, k)))).astype(np.float32)
+    y = linear(hip, x, codes, scales, k)
+    assert np.all(np.abs(y - x.astype(np.float64)) <= (2.0 ** -21 + 5 * 2.0 ** -23) * M.block_max(x))

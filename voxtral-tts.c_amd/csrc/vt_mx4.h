@@ -85,9 +85,10 @@ __device__ __forceinline__ void vt_mx4_store4(float *p, int n, bool whole, const
  * v_mfma_scale_f32_*_f8f6f4 multiplies blocks of 32 values with a scale each: the 4-bit operand goes in as it lies in memory, and
  * fp32 values as a sum of NP planes of e2m3 (six bits: 0 .. 2 in steps of 1/8, 2 .. 4 of 1/4, 4 .. 7.5 of 1/2): plane 0 is the nearest
  * e2m3 of the block, every next one that of what is left, each with a scale of its own that puts the largest magnitude at 3.875 .. 7.75 of
- * it.  A plane leaves at most 2^-4 of that magnitude, and on values ~N(0, 1) four planes leave 5.2e-7 of their norm, five 9e-9 (three
- * 2e-5; with scales a fixed ratio apart four leave 1.0e-6).  Subtracting what a plane holds is exact.  With an infinity or a NaN
- * in it a block's scales say NaN. */
+ * it.  A plane leaves at most 2^-4 of that magnitude; on values ~N(0, 1) five planes leave 9e-9 of their norm, and 2.0e-8 where the fifth's
+ * scale is 2^-4 of the fourth's, each value to 2^-24 of its block's largest (2^-21 at the worst).  Fewer are not enough for fp32: four
+ * leave 5.2e-7 of the norm, and 1.3e-4 of the values beside one that is 1000 times as large.  Subtracting what a plane holds is exact.
+ * With an infinity or a NaN in it a block's scales say NaN. */
 typedef float vt_f32x16 __attribute__((ext_vector_type(16)));
 typedef float vt_f32x32 __attribute__((ext_vector_type(32)));
 typedef unsigned vt_u32x6 __attribute__((ext_vector_type(6)));
@@ -95,26 +96,33 @@ typedef int vt_i32x8 __attribute__((ext_vector_type(8)));
 #define VT_MFMA_E2M1 4                    /* formats of an operand, as the instruction numbers them */
 #define VT_MFMA_E2M3 2
 
-/* even[i], odd[i]: values 2 i and 2 i + 1 of the block */
-template <int NP>
+/* the scale of a plane that stands in a fixed ratio to the one before: 2^-4 of its */
+__device__ __forceinline__ int vt_mx4_below(unsigned s) { return max((int)s - 4, 0); }
+
+/* The next plane of a block, and what it leaves of it; even[i], odd[i]: values 2 i and 2 i + 1.  tied: its scale follows from the one before, `scale`. */
+__device__ __forceinline__ vt_u32x6 vt_mx4_plane(vt_f32x16 &even, vt_f32x16 &odd, bool tied, unsigned &scale) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) t = __builtin_elementwise_maximum(__builtin_elementwise_maximum(t, fabsf(even[i])), fabsf(odd[i]));
+    const unsigned top = __float_as_uint(t);
+    scale = tied ? (unsigned)vt_mx4_below(scale) : top >= 0x7f800000u ? 255u : (unsigned)max((int)((top + 0x80000u) >> 23) - 2, 0);
+    const float f = vt_mx4_scale(scale);
+    const vt_u32x6 q = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, f);
+    const vt_f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q, f);
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        even[i] = __fsub_rn(even[i], held[2 * i]);
+        odd[i] = __fsub_rn(odd[i], held[2 * i + 1]);
+    }
+    return q;
+}
+
+template <int NP, bool TIED = false>
 __device__ __forceinline__ void vt_mx4_planes(vt_f32x16 even, vt_f32x16 odd, vt_u32x6 (&q)[NP], unsigned (&s)[NP]) {
 #pragma unroll
     for (int p = 0; p < NP; p++) {
-        float t = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; i++) t = __builtin_elementwise_maximum(__builtin_elementwise_maximum(t, fabsf(even[i])), fabsf(odd[i]));
-        const unsigned top = __float_as_uint(t);
-        s[p] = top >= 0x7f800000u ? 255u : (unsigned)max((int)((top + 0x80000u) >> 23) - 2, 0);
-        const float f = vt_mx4_scale(s[p]);
-        q[p] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, f);
-        if (p + 1 < NP) {
-            const vt_f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q[p], f);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                even[i] = __fsub_rn(even[i], held[2 * i]);
-                odd[i] = __fsub_rn(odd[i], held[2 * i + 1]);
-            }
-        }
+        s[p] = p ? s[p - 1] : 0u;
+        q[p] = vt_mx4_plane(even, odd, TIED && p == NP - 1, s[p]);
     }
 }
 

@@ -111,26 +111,35 @@ extern "C" int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const 
 }
 
 /* ---- linear layer: up to eight rows --------------------------------------------------------------------------------
- * y^T[weight row][column] on v_mfma_scale_f32_16x16x128_f8f6f4: 16 weight rows go in as they lie in memory, nothing is decoded, and the four e2m3 planes
- * of x (vt_mx4.h) are columns or instructions: up to four rows of x all planes in one instruction (a row is four columns), up to eight rows two in each of
- * G = 2, the smaller ones first.  Every workgroup splits x (a cut of K of it) itself, while its first weights are on their way.  Its waves share K, or groups of
- * four of them share K and take blocks of 16 weight rows in turn where there are several blocks; a wave's weights come in parts of 16 rows x 2 panels
- * (lines of 128 bytes) straight into LDS of its own, three parts ahead of the one that is multiplied, and it waits for nothing but its own loads; the
- * waves' sums of 16 rows meet in LDS behind a bare barrier.  A panel's products start from zero and are added to the sum by the vector unit, which
- * rounds; the matrix unit cuts at 2^-23.  x's planes have to fit LDS: where they do not, K is cut, the cuts' sums go to memory and the last workgroup
- * of a block of rows to arrive adds them.  Bound: one row by 131072 x 3072 38.6 us, the stream of the weights at 5.6 TB/s; by 9216 x 3072 7.5 us, launch and first touch. */
+ * y^T[weight row][column] on v_mfma_scale_f32_16x16x128_f8f6f4: 16 weight rows go in as they lie in memory, nothing is decoded, and the five
+ * e2m3 planes of x (vt_mx4.h) are columns or instructions: the smallest plane in the first of G instructions, the other four in the
+ * columns of the second (up to four rows of x, four columns each) or in those of two more (up to eight rows, two columns each).  Every
+ * workgroup splits x (a cut of K of it) itself, while its first weights are on their way.  Its waves share K, or groups of four of
+ * them share K and take blocks of 16 weight rows in turn where there are several blocks; a wave's weights come in parts of 16 rows x
+ * 2 panels (lines of 128 bytes) straight into LDS of its own, three parts (five rows and more: two) ahead of the one that is
+ * multiplied, and it waits for nothing but its own loads; the waves' sums of 16 rows meet in LDS behind a bare barrier.  A panel's
+ * products start from zero and are added to the sum by the vector unit, which rounds; the matrix unit cuts at 2^-23.  x's planes have
+ * to fit LDS: where they do not, K is cut, the cuts' sums go to memory and the last workgroup of a block of rows to arrive adds them.
+ * Bound: one row by 131072 x 3072 39.0 us, the stream of the weights at 5.5 TB/s; by 9216 x 3072 8.0 us, launch and first touch; eight
+ * rows 45 and 12.7 (78 and 14.3 with a ring of four parts, which leaves no room for the planes of 3072 columns). */
 #define MXR_ROWS 8
 #define MXR_WAVES 8
-#define MXR_PLANES 4
+#define MXR_PLANES 5                       /* the last one's scale follows from the fourth's */
 #define MXR_PART (16 * 128 + 256)          /* codes, then 16 x 2 words of scales and as much room */
 
 struct mxr_job { float *y; const float *x; const uint8_t *codes, *scales; int seq_len, in_dim, out_dim, panels, cut_panels, cuts, rows_per_wg, share_log, whole; float *part; unsigned *cnt; };      /* 1 << share_log waves share K */
 
+/* columns of a block: the planes of all rows, and one of zeros; an odd number, so that consecutive blocks lie in different banks */
+static __host__ __device__ constexpr int mxr_columns(int seq_len) { return (MXR_PLANES * seq_len + 1) | 1; }
+/* parts of a wave's ring: the planes of five and more rows need the room of the fourth */
+static constexpr int mxr_ring(int g) { return g > 2 ? 3 : 4; }
+
 template <int G>
 __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) {
-    constexpr int THREADS = 64 * MXR_WAVES, PP = MXR_PLANES / G;      /* planes of an instruction */
-    __shared__ __attribute__((aligned(16))) unsigned char buf0[MXR_WAVES * MXR_PART], buf1[MXR_WAVES * MXR_PART], buf2[MXR_WAVES * MXR_PART], buf3[MXR_WAVES * MXR_PART];
-    __shared__ float red[2][MXR_WAVES][64 * G];                /* [row of x][weight row] */
+    constexpr int THREADS = 64 * MXR_WAVES, PP = 4 / (G - 1);         /* planes of an instruction but the first */
+    constexpr int RING = mxr_ring(G);
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[MXR_WAVES * MXR_PART], buf1[MXR_WAVES * MXR_PART], buf2[MXR_WAVES * MXR_PART], buf3[RING > 3 ? MXR_WAVES * MXR_PART : 16];
+    __shared__ float red[2][MXR_WAVES][64 * (G - 1)];          /* [row of x][weight row] */
     __shared__ int last;
     extern __shared__ __attribute__((aligned(16))) unsigned char planes[];
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
@@ -141,7 +150,7 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
     const int total = (blocks + groups - 1) / groups * parts;
     /* x: block u % nb of row u / nb of the cut.  [panel][group of lanes][instruction][column] of 16 and of 8 bytes, and the scales; column PP row +
      * plane.  The first blocks are asked for in front of the weights, the next ones while these are split: loads return in order. */
-    const int nb = 4 * (k1 - k0), nc = 4 * a.seq_len + 1, units = a.seq_len * nb;       /* a column more: consecutive blocks lie in different banks */
+    const int nb = 4 * (k1 - k0), nc = mxr_columns(a.seq_len), units = a.seq_len * nb;
     unsigned char *lo8 = planes + nb * nc * 16, *sc = lo8 + nb * nc * 8;
     const __amdgpu_buffer_rsrc_t xd = vt_buffer(a.x, a.seq_len * a.in_dim * 4);
     int xr = (int)threadIdx.x / nb, xb = (int)threadIdx.x - xr * nb;
@@ -169,24 +178,30 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
     };
     ask(buf0);
     ask(buf1);
-    ask(buf2);
+    if (RING > 3) ask(buf2);
     for (int u = THREADS;; u += THREADS) {
-        const int row = xr, at0 = xb * nc + row * PP;
+        const int row = xr, xb_at = xb * nc, at0 = xb_at + a.seq_len + row * PP;
         xr += xr_step;
         xb += xb_step;
         if (xb >= nb) { xb -= nb; xr++; }
         if (u < units) ask_x(next_even, next_odd);
         vt_u32x6 q[MXR_PLANES];
         unsigned s[MXR_PLANES];
-        vt_mx4_planes<MXR_PLANES>(even, odd, q, s);
+        vt_mx4_planes<MXR_PLANES, true>(even, odd, q, s);
         if (row < a.seq_len) {
 #pragma unroll
             for (int p = 0; p < MXR_PLANES; p++) {
-                const int at = at0 + (G - 1 - p / PP) * PP * a.seq_len + p % PP;
+                const int at = p == MXR_PLANES - 1 ? xb_at + row : at0 + (G - 2 - p / PP) * PP * a.seq_len + p % PP;
                 *reinterpret_cast<u32x4 *>(planes + at * 16) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
                 *reinterpret_cast<u32x2 *>(lo8 + at * 8) = u32x2{q[p][4], q[p][5]};
                 sc[at] = (unsigned char)s[p];
             }
+        }
+        if (row == 0) {                                  /* the column of zeros */
+            const int at = xb_at + nc - 1;
+            *reinterpret_cast<u32x4 *>(planes + at * 16) = u32x4{0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x2 *>(lo8 + at * 8) = u32x2{0u, 0u};
+            sc[at] = 0;
         }
         if (u >= units) break;
         even = next_even;
@@ -196,7 +211,8 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
     __builtin_amdgcn_s_waitcnt(0xc07f);                  /* lgkmcnt(0); weights stay on their way */
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int mine = g * nc + min(n, PP * a.seq_len - 1);        /* columns past the last repeat it: nobody looks at their sums */
+    const int col = min(n, PP * a.seq_len - 1), mine = g * nc + a.seq_len + col;        /* columns past the last repeat it: nobody looks at their sums */
+    const int smallest = g * nc + (n % PP == 0 ? col / PP : nc - 1);       /* the smallest plane is in one of a row's columns */
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float *y = a.cuts > 1 ? a.part + (size_t)blockIdx.y * a.seq_len * a.out_dim : a.y;
     /* the waves' sums: element v of lane l is weight row 4 (l / 16) + v, column l % 16; a row's planes of an instruction are PP lanes */
@@ -213,17 +229,17 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
         __builtin_amdgcn_s_waitcnt(0xc07f);
         __builtin_amdgcn_s_barrier();                    /* the other half of red is read before a wave is through the next one */
         asm volatile("" ::: "memory");
-        /* the first 64 G threads of a group of waves: row of x, weight row */
+        /* the first 64 (G - 1) threads of a group of waves: row of x, weight row */
         const int t = (int)threadIdx.x & (64 * share - 1), s = t >> 4, r = 16 * (turn * groups + group) + (t & 15);
         if (s < a.seq_len && r < rows) {
             const float *from = &red[turn & 1][group << a.share_log][t];
             float p[4];
 #pragma unroll
-            for (int w = 0; w < 4; w++) p[w] = from[w * 64 * G];
+            for (int w = 0; w < 4; w++) p[w] = from[w * 64 * (G - 1)];
             float v = (p[0] + p[2]) + (p[1] + p[3]);
             if (share > 4) {
 #pragma unroll
-                for (int w = 0; w < 4; w++) p[w] = from[(4 + w) * 64 * G];
+                for (int w = 0; w < 4; w++) p[w] = from[(4 + w) * 64 * (G - 1)];
                 v += (p[0] + p[2]) + (p[1] + p[3]);
             }
             float *at = y + (size_t)s * a.out_dim + row0 + r;
@@ -234,7 +250,7 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
     int turn = 0, part = 0;
     auto item = [&](const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070 | 6);          /* vmcnt: two later parts may be on their way; lgkmcnt(0): what is asked for below overwrites what the last part read */
+        __builtin_amdgcn_s_waitcnt(0x0070 | 3 * (RING - 2));          /* vmcnt: two later parts, or one, may be on their way; lgkmcnt(0): what is asked for below overwrites what the last part read */
         asm volatile("" ::: "memory");
         ask(later);
         asm volatile("" ::: "memory");
@@ -248,7 +264,7 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
             f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < G; i++) {
-                const int at = (panel - k0) * 4 * nc + i * PP * a.seq_len + mine;
+                const int at = (panel - k0) * 4 * nc + (i ? (i - 1) * PP * a.seq_len + mine : smallest);
                 const u32x4 x4 = *reinterpret_cast<const u32x4 *>(planes + at * 16);
                 const u32x2 x2 = *reinterpret_cast<const u32x2 *>(lo8 + at * 8);
                 const vt_u32x6 xq = {x4.x, x4.y, x4.z, x4.w, x2.x, x2.y};
@@ -258,12 +274,13 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
         }
         if (++part == parts) { part = 0; finish(turn++); }
     };
-    for (int t = 0; t < total; t += 4) {                 /* every wave goes through the same parts and barriers, whatever it has of them */
-        item(buf0, buf3);
+    for (int t = 0; t < total; t += RING) {                 /* every wave goes through the same parts and barriers, whatever it has of them */
+        item(buf0, RING > 3 ? buf3 : buf2);
         if (t + 1 >= total) break;
         item(buf1, buf0);
         if (t + 2 >= total) break;
         item(buf2, buf1);
+        if (RING == 3) continue;
         if (t + 3 >= total) break;
         item(buf3, buf2);
     }
@@ -289,20 +306,22 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
         }
 }
 
-/* LDS: four buffers and the sums of eight waves, 25 bytes a block of 32 values of x and plane */
+/* LDS: the rings and the sums of eight waves, 25 bytes a block of 32 values of x and plane */
 #define MXR_LDS_MOST (160 * 1024)
-static size_t mxr_lds(int g) { return (size_t)MXR_WAVES * (MXR_PART * 4 + 2 * 64 * g * 4) + 256; }
-static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * panels * (4 * seq_len + 1) * 25; }
+static size_t mxr_lds(int g) { return (size_t)MXR_WAVES * (MXR_PART * mxr_ring(g) + 2 * 64 * (g - 1) * 4) + 256; }
+static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * panels * mxr_columns(seq_len) * 25; }
 
 /* ---- linear layer: more rows -----------------------------------------------------------------------------------------
  * x is split into its planes first, [column tile of 32 rows][64 columns of W's K][plane] in the order of the matrix instruction's operand, 16
- * and 8 bytes a lane, and the scales of a lane's four planes in a word.  y[row of x][weight row] then runs on v_mfma_scale_f32_32x32x64_f8f6f4,
- * x as operand A, weights as they lie as B.  A workgroup's tile of BM weight rows and BN rows of x goes through K by panels of
- * 128: both operands come straight into LDS, one panel ahead.  A wave has 32 rows of x and FM x 32 weight rows, so that an operand of x, the larger one
- * (3 bytes a value), is read once for FM products.  Eight products of a panel, the smallest planes first, start from zero and are added by the
- * vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts are added by a kernel of their own.  Bound: 1531 x 9216 x 3072, 103 to 107 us (9 of
- * them the planes), would take 86 if the product waited for no load (timing-only build): matrix units, four products of 43 GMAC; the rest is the operands' way through LDS.  226 x 3072 x 9216, 34 us: 6 the
- * planes, 4 the sums, 24 the product, whose smaller tiles bring twice the bytes to LDS for each. */
+ * and 8 bytes a lane, and the scales of a lane's first four planes in a word (the fifth's follows).  y[row of x][weight row] then runs on
+ * v_mfma_scale_f32_32x32x64_f8f6f4, x as operand A, weights as they lie as B.  A workgroup's tile of BM weight rows and BN rows of x goes
+ * through K by panels of 128: both operands come straight into LDS, one panel ahead.  A wave has 32 rows of x and FM x 32 weight rows, so
+ * that an operand of x, the larger one (3.75 bytes a value), is read once for FM products.  Ten products of a panel, the smallest planes
+ * first, start from zero and are added by the vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts
+ * are added by a kernel of their own.  Bound: 1531 x 9216 x 3072 120 us, 10 of them the planes; the product's 108 are five products of 43
+ * GMAC, which keep the matrix units busy 46 % of the time (in two rounds of which the second is 69 % full), and 190 KB that its
+ * eight waves read from LDS per panel, 1500 cycles of the 2600 that the matrix instructions take, with the next panel's 80 KB on their way
+ * there.  226 x 3072 x 9216 39 us: 6 the planes, 5 the sums, 28 the product, whose smaller tiles bring twice the bytes to LDS for each. */
 #define MXT_STEP (MXR_PLANES * 1536 + 256)               /* bytes of 32 rows x 64 columns of x */
 
 /* A wave has 32 rows by 64 columns; they go through LDS so that its loads are lines (a lane's own 128 bytes come in eight pieces, and with twenty waves on a CU the
@@ -336,13 +355,13 @@ __global__ void __launch_bounds__(256) vt_mx4_planes_kernel(unsigned char *out, 
     }
     vt_u32x6 q[MXR_PLANES];
     unsigned s[MXR_PLANES], all = 0;
-    vt_mx4_planes<MXR_PLANES>(even, odd, q, s);
+    vt_mx4_planes<MXR_PLANES, true>(even, odd, q, s);
     unsigned char *to = out + (size_t)unit * MXT_STEP;
 #pragma unroll
     for (int p = 0; p < MXR_PLANES; p++) {
         *reinterpret_cast<u32x4 *>(to + p * 1536 + lane * 16) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
         *reinterpret_cast<u32x2 *>(to + p * 1536 + 1024 + lane * 8) = u32x2{q[p][4], q[p][5]};
-        all |= s[p] << (8 * p);
+        if (p < 4) all |= s[p] << (8 * p);
     }
     *reinterpret_cast<unsigned *>(to + MXR_PLANES * 1536 + lane * 4) = all;
 }
@@ -431,27 +450,32 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
         vt_f32x16 sum[FM];
 #pragma unroll
         for (int f = 0; f < FM; f++) sum[f] = vt_f32x16{};
-#define PRODUCTS(p, x, h) \
+        const int last[2] = {vt_mx4_below((unsigned)xs[0] >> 24), vt_mx4_below((unsigned)xs[1] >> 24)};
+#define PRODUCTS(x, h, byte, scales) \
         _Pragma("unroll") for (int f = 0; f < FM; f++) \
-            sum[f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(x[h]), vt_mfma_e2m1(w[f][h]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, p, xs[h], 2 * h, ws[f]);
+            sum[f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(x[h]), vt_mfma_e2m1(w[f][h]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, byte, scales[h], 2 * h, ws[f]);
 #define PINNED(...) __builtin_amdgcn_sched_barrier(PIN); __VA_ARGS__ __builtin_amdgcn_sched_barrier(PIN);
+        const vt_u32x6 x3[2] = {x_of(here, 3, 0), x_of(here, 3, 1)};
+        PINNED()
+        PRODUCTS(first, 0, 0, last) PRODUCTS(first, 1, 0, last)
+        PINNED(if (AHEAD) ask(other, panel + 1, 1, 2); else ask(other, panel + 1, 0, 4);)
         const vt_u32x6 x2[2] = {x_of(here, 2, 0), x_of(here, 2, 1)};
         PINNED()
-        PRODUCTS(3, first, 0) PRODUCTS(3, first, 1)
-        PINNED(if (AHEAD) ask(other, panel + 1, 1, 2); else ask(other, panel + 1, 0, 4);)
+        PRODUCTS(x3, 0, 3, xs) PRODUCTS(x3, 1, 3, xs)
+        PINNED(if (!AHEAD) ask(other, panel + 1, 1, 4);)
         const vt_u32x6 x1[2] = {x_of(here, 1, 0), x_of(here, 1, 1)};
         PINNED()
-        PRODUCTS(2, x2, 0) PRODUCTS(2, x2, 1)
-        PINNED(if (!AHEAD) ask(other, panel + 1, 1, 4);)
+        PRODUCTS(x2, 0, 2, xs) PRODUCTS(x2, 1, 2, xs)
+        PINNED(if (!AHEAD) ask(other, panel + 1, 2, 4);)
         const vt_u32x6 x0[2] = {x_of(here, 0, 0), x_of(here, 0, 1)};
         PINNED()
-        PRODUCTS(1, x1, 0) PRODUCTS(1, x1, 1)
-        PINNED(if (AHEAD) { meet(); fetch_x(other); } else ask(other, panel + 1, 2, 4);)
+        PRODUCTS(x1, 0, 1, xs) PRODUCTS(x1, 1, 1, xs)
+        PINNED(if (AHEAD) { meet(); fetch_x(other); } else ask(other, panel + 1, 3, 4);)
         PINNED(if (AHEAD) ask(here, panel + 2, 0, 2);)
-        PRODUCTS(0, x0, 0)
+        PRODUCTS(x0, 0, 0, xs)
         PINNED(if (AHEAD) fetch_w(other, 0);)
-        PRODUCTS(0, x0, 1)
-        PINNED(if (AHEAD) fetch_w(other, 1); else ask(other, panel + 1, 3, 4);)
+        PRODUCTS(x0, 1, 0, xs)
+        PINNED(if (AHEAD) fetch_w(other, 1);)
 #undef PINNED
 #undef PRODUCTS
 #pragma unroll
@@ -494,10 +518,10 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
 template <int G> static int mxr_prepare(void) {
     return vt_check(hipFuncSetAttribute((const void *)vt_mx4_rows_kernel<G>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(MXR_LDS_MOST - mxr_lds(G))), "tts_hip_linear_mx4: LDS");
 }
-int vt_mx4_prepare(void) { return mxr_prepare<1>() || mxr_prepare<2>() ? -1 : 0; }
+int vt_mx4_prepare(void) { return mxr_prepare<2>() || mxr_prepare<3>() ? -1 : 0; }
 
 static int mx4_linear_rows(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim, int whole) {
-    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = vt_mx4_panels(in_dim), g = seq_len <= 4 ? 1 : 2;
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = vt_mx4_panels(in_dim), g = seq_len <= 4 ? 2 : 3;
     const int most = (int)((MXR_LDS_MOST - mxr_lds(g)) / mxr_planes_bytes(seq_len, 1)), cuts = (panels + most - 1) / most, wgs = n_cu / cuts > 0 ? n_cu / cuts : 1;
     mxr_job a = {d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, panels, (panels + cuts - 1) / cuts, cuts, (int)(((long long)out_dim + wgs - 1) / wgs), 2, whole, NULL, g_vt.d_mx4_cnt};
     if (a.rows_per_wg <= 16) a.share_log = 3;          /* no second block for the other waves */
@@ -505,8 +529,8 @@ static int mx4_linear_rows(float *d_y, const float *d_x, const uint8_t *d_codes,
     if (a.cuts > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)a.cuts * seq_len * out_dim))) return -1;
     const dim3 grid((out_dim + a.rows_per_wg - 1) / a.rows_per_wg, a.cuts);
     const size_t lds = mxr_planes_bytes(seq_len, a.cut_panels);
-    if (g == 1) hipLaunchKernelGGL(vt_mx4_rows_kernel<1>, grid, dim3(64 * MXR_WAVES), lds, g_vt.stream, a);
-    else hipLaunchKernelGGL(vt_mx4_rows_kernel<2>, grid, dim3(64 * MXR_WAVES), lds, g_vt.stream, a);
+    if (g == 2) hipLaunchKernelGGL(vt_mx4_rows_kernel<2>, grid, dim3(64 * MXR_WAVES), lds, g_vt.stream, a);
+    else hipLaunchKernelGGL(vt_mx4_rows_kernel<3>, grid, dim3(64 * MXR_WAVES), lds, g_vt.stream, a);
     return 0;
 }
 
