@@ -253,9 +253,10 @@ def test_quantize_more_rows_than_a_launch_has_threads_for(hip, cols):
 # rows of x, weight rows, columns -> tile of vt_mx4_plans.h (weight rows x rows of x) and cuts of K on 256 CUs, which test_mx4_plans_cpu.py asserts: one, two and more panels,
 # odd and even, and ends inside a tile and a panel
 TILES = {(515, 8250, 128): ("256x128", 1), (515, 8250, 200): ("256x128", 1), (515, 8250, 384): ("256x128", 1), (300, 13100, 1300): ("256x128", 1), (515, 8202, 3072): ("256x128", 1),
-         (66, 11514, 3190): ("256x128", 5), (2101, 129, 9216): ("256x128", 15),
-         (97, 9216, 256): ("128x64", 1), (226, 3072, 9216): ("128x64", 5), (64, 9216, 3072): ("128x64", 3), (400, 9000, 1000): ("128x64", 1),
-         (700, 640, 512): ("128x32", 1), (16, 20000, 1000): ("128x32", 1), (9, 9216, 3072): ("128x32", 6)}
+         (130, 13100, 3190): ("256x128", 2), (2101, 129, 9216): ("256x128", 12), (226, 3072, 9216): ("256x128", 8),
+         (200, 11514, 128): ("128x64", 1), (200, 11514, 200): ("128x64", 1), (400, 9000, 300): ("128x64", 1), (400, 9000, 1000): ("128x64", 1), (40, 11514, 3190): ("128x64", 5),
+         (40, 8250, 9216): ("128x64", 7),
+         (97, 9216, 256): ("128x32", 1), (700, 640, 512): ("128x32", 1), (16, 20000, 1000): ("128x32", 1), (9, 9216, 3072): ("128x32", 6), (64, 9216, 3072): ("128x32", 3)}
 
 
 def random_weights(n, k, seed):
@@ -286,7 +287,7 @@ def test_linear_tiles(hip, m, n, k, shift):
     assert np.array_equal(y, linear(hip, x, codes, scales, n, shift))
 
 
-@pytest.mark.parametrize("m,n,k", [(515, 8250, 200), (515, 8250, 384), (66, 11514, 3190), (97, 9216, 256), (16, 20000, 1000)])
+@pytest.mark.parametrize("m,n,k", [(515, 8250, 200), (515, 8250, 384), (130, 13100, 3190), (200, 11514, 200), (400, 9000, 300), (97, 9216, 256), (16, 20000, 1000)])
 def test_linear_tiles_what_is_not_finite_stays_in_its_row_and_its_column(hip, m, n, k):
     codes, scales, _ = random_weights(n, k, 17)
     x = S.f32_normal((m, k), 92)

@@ -38,10 +38,10 @@ static inline vt_mx4_lanes vt_mx4_lanes_of(int rows, int cols, int values) {
 
 /* ---- linear layers of more than a few rows --- */
 
-/* Tiles: weight rows, rows of x, threads, workgroups that a CU holds, and us per panel with one, two, three of them on it (from runs of one cut on
- * part of the chip and on all of it: 226 x 3072 x 9216, 1531 x 9216 x 3072). */
+/* Tiles: weight rows, rows of x, threads, workgroups that a CU holds, and us per panel with one, two, three of them on it.  These, what cuts cost and the
+ * rate of their sums are the numbers that choose best, fitted to 4000 runs of every tile and cut count on 190 shapes of 9 to 1531 rows. */
 struct vt_mxt_tile { int bm, bn, threads, per_cu; float panel_us[3]; };
-static const vt_mxt_tile vt_mxt_tiles[] = {{256, 128, 512, 1, {1.8f}}, {128, 64, 256, 2, {0.72f, 1.2f}}, {128, 32, 256, 3, {0.56f, 0.85f, 1.25f}}};
+static const vt_mxt_tile vt_mxt_tiles[] = {{256, 128, 512, 1, {1.4f}}, {128, 64, 256, 2, {0.95f, 1.35f}}, {128, 32, 256, 3, {0.65f, 0.78f, 1.45f}}};
 #define VT_MXT_MAX_CUTS 16
 #define VT_MXT_ROWS (1 << 14)
 
@@ -53,8 +53,11 @@ static inline int vt_mxt_rows(int out_dim, int panels) {
     return rows;
 }
 
-/* The tile and the cuts of K with the least time by these figures.  us a call, with the best of the others: 1531 x 9216 x 3072 107 (256 x 128 whole; 131 on 128 x 64), 512 of them 48 (the same;
- * 57), 400 41 (128 x 64 whole; 47 on 256 x 128), 1000 x 3072 x 4096 47 (128 x 64; 48), 300 x 3072 x 9216 38 (128 x 64 in 4 cuts; 41 in 3), 226 x 3072 x 9216 36, 64 x 9216 x 3072 20 (128 x 32 in 3). */
+/* The tile and the cuts of K with the least time by these figures (which leave out the split of x and, where there are few rows of x for
+ * many weights, the weights' way from memory: alike for all).  Over those shapes the plan taken is 1.6 % behind the fastest on average, at
+ * worst 12 % (512 x 1024 x 3072).  us a call, with the best of other tiles or cuts: 1531 x 9216 x 3072 123 (256 x 128 whole; 147 on 128 x 64), 512 of
+ * them 52 (the same; 64 on 128 x 32), 400 49 (128 x 64 whole; 52 on 256 x 128), 128 25 (128 x 32 whole; 28 on 128 x 64), 64 20 (128 x 32 in 3; 21 on 128 x 64),
+ * 1000 x 3072 x 4096 54 (256 x 128 in 2; 56 on 128 x 64), 226 x 3072 x 9216 39 (256 x 128 in 8; 40 on 128 x 64 in 5, 43 on 128 x 32), 16 x 131072 x 3072 78 (128 x 32 whole; 81 on 128 x 64). */
 struct vt_mxt_plan { int tile, cuts, m_tiles; long long grid; double us; };
 static inline vt_mxt_plan vt_mxt_plan_of(int n_cu, int seq_len, int out_dim, int panels) {
     vt_mxt_plan best = {0, 1, 0, 0, 1e30};
@@ -65,7 +68,7 @@ static inline vt_mxt_plan vt_mxt_plan_of(int n_cu, int seq_len, int out_dim, int
             const double wgs = (double)tiles * cuts, full = floor(wgs / ((double)n_cu * k.per_cu)), rest = wgs - full * n_cu * k.per_cu;
             const int each = (panels + cuts - 1) / cuts, beside = (int)ceil(rest / n_cu);
             const double us = each * (full * k.panel_us[k.per_cu - 1] + (beside ? k.panel_us[beside - 1] : 0.0)) + full +
-                              (cuts > 1 ? 2.0 + (double)seq_len * out_dim * 4.0 * (2 * cuts + 1) / 5.0e6 : 0.0);
+                              (cuts > 1 ? 4.2 + (double)seq_len * out_dim * 4.0 * (2 * cuts + 1) / 3.9e6 : 0.0);
             if (us < best.us) best = vt_mxt_plan{t, cuts, (int)m_tiles, tiles * cuts, us};
         }
     }
