@@ -56,7 +56,9 @@ __global__ void __launch_bounds__(256) vt_kv4_read_kernel(float *K, float *V, tt
     long long to;
     size_t at;
     if (!kv4_place(r, 4, to, at)) return;
-    vt_mx4_store4((blockIdx.y ? V : K) + to, 4, r.whole, vt_mx4_decode4(((const uint16_t *)(blockIdx.y ? c.v_codes : c.k_codes))[at], (blockIdx.y ? c.v_scales : c.k_scales)[at >> 3]));
+    const uint16_t *codes = (const uint16_t *)(blockIdx.y ? c.v_codes : c.k_codes);
+    const uint8_t *scales = blockIdx.y ? c.v_scales : c.k_scales;
+    vt_mx4_store4((blockIdx.y ? V : K) + to, 4, r.whole, vt_mx4_decode4(codes[at], scales[at >> 3]));
 }
 
 static int kv4_rows_ok(const char *who, kv4_rows *r, const tts_hip_kv4_t *c, const float *K, const float *V, int n, int pos, int stride, int values) {
@@ -93,14 +95,14 @@ extern "C" int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cac
  * S^T[row][column] = K Q^T on the scaled matrix instruction, keys in 4 bits as they lie, queries as five e2m3 planes (vt_mx4.h), the
  * smallest plane first: the accumulators are cut and not rounded at 2^-23, and so only the last sum meets that.  Results are
  * O^T[value][column] = V^T P^T in fp16: 4-bit values are exact in fp16 once they are scaled by the largest scale E of the rows at hand,
- * to 2^13 of it, and a weight p 2^14 goes in as two planes of 22 bits in all.  Maximum, sum and
- * results of a column are fp32, one pass over the rows with the running maximum.  A lane holds the same column of S^T and of O^T, and
- * the order of keys inside an instruction is free, so that weights go from one product to the next in their registers.
- * Rows at hand with scales further apart than fp16 reaches (36 binades) go another way (kv4_column): fp32 all through, rare, and slow: 1 query of 32 heads behind 1999
- * rows 46 us with the call and the wait for it, 1531 behind none 5.9 ms.
- * A score beyond fp32 meets the planes one by one, with signs of their own: what comes out may be an infinity of the wrong sign, and so it counts as NaN.
- * NaN: a key's shows in the scores of who sees it.  A value's scale of 255 is taken for a finite one in the product (a hidden row's weight
- * is 0, and 0 times NaN would reach who does not see it), and behind the last row NaN goes to the columns that see such a row. */
+ * to 2^13 of it, and a weight p 2^14 goes in as two planes of 22 bits in all.  Maximum, sum and results of a column are fp32, one pass
+ * over the rows with the running maximum.  A lane holds the same column of S^T and of O^T, and the order of keys inside an instruction
+ * is free, so that weights go from one product to the next in their registers.  Rows at hand with scales further apart than fp16 reaches
+ * (36 binades) go another way (kv4_column): fp32 all through, rare, and slow: 1 query of 32 heads behind 1999 rows 44 us with the call
+ * and the wait for it, 1531 behind none 3.4 ms where one row of each head is so.  A score beyond fp32 meets the planes one by one, with
+ * signs of their own: what comes out may be an infinity of the wrong sign, and so it counts as NaN.  NaN: a key's shows in the scores of
+ * who sees it.  A value's scale of 255 is taken for a finite one in the product (a hidden row's weight is 0, and 0 times NaN would reach
+ * who does not see it), and behind the last row NaN goes to the columns that see such a row. */
 typedef _Float16 vt_f16x8 __attribute__((ext_vector_type(8)));
 #define KV4_PLANES 5
 #define KV4_P_EXP 14                       /* weights times 2^14 .. */
@@ -113,7 +115,8 @@ struct kv4_job {
     const float *Q;
     unsigned char *part;
     unsigned *cnt;
-    int max_rows, start, n_heads, cols, run, parts, tiles;       /* columns, tiles of them; tiles of 32 rows a wave, of 64 a workgroup; workgroups per head and tile of columns */
+    /* cols, tiles: columns and tiles of them; run: tiles of 32 rows a wave, of 64 a workgroup; parts: workgroups per head and tile of columns */
+    int max_rows, start, n_heads, cols, run, parts, tiles;
     vt_divisor group;
     float scale;                                         /* times log2 e */
 };
@@ -156,8 +159,8 @@ template <int HP> static __device__ __forceinline__ int kv4_swizzle(int row, int
     return HP == 2 ? piece ^ ((row >> 1) & 3) : HP == 4 ? piece ^ (row & 7) : piece ^ ((row >> 2) & 1);
 }
 
-/* One column over `rows` rows, all of which it sees, by a wave in fp32: a lane per row for the scores, per value for the results; -> the largest score,
- * the sum of weights times 2^14, and the mean of values, value 64 k + lane of it to at[64 k + lane].  The mean is kept as
+/* One column over `rows` rows, all of which it sees, by a wave in fp32: a lane per row for the scores, per value for the results; -> the
+ * largest score, the sum of weights times 2^14, and the mean of values, value 64 k + lane of it to at[64 k + lane].  The mean is kept as
  * one, row after row: a sum of values near the end of the range would leave it, and scaled down small ones would lose bits. */
 template <int HP>
 static __device__ __forceinline__ void kv4_column(const kv4_job &a, const float *q, size_t row0, int rows, int lane, float *at, float &m, float &l) {
@@ -201,12 +204,12 @@ static __device__ __forceinline__ void kv4_column(const kv4_job &a, const float 
     l = __builtin_amdgcn_ldexpf(l, KV4_P_EXP);
 }
 
-/* Few columns: a wave streams 32 rows of K and V at a time into LDS of its own, two such tiles on their way while one is multiplied,
- * and waits for nobody else; the waves of a workgroup, and then the workgroups of a head, add their parts in a fixed order, the last workgroup
- * to arrive those of all.  K is the A operand of 16 x 16 x 128, V of 16 x 16 x 32: lane l has the values of column n = l % 16, CD of each
- * 16 CD, for the eight keys that its group of 16 lanes has weights of.  Most of a short call is instructions that run once, from a cold instruction cache: the code
- * in front of the loop and behind it is kept short.  Bound: one query of 32 heads on 8 with 128 values behind 65535 rows 19.3 us, 71 MB at 3.7 TB/s, of which 7 us do not depend on the rows; behind
- * 1999 8.7 us, nothing but those. */
+/* Few columns: a wave streams 32 rows of K and V at a time into LDS of its own, two such tiles on their way while one is multiplied, and
+ * waits for nobody else; the waves of a workgroup, and then the workgroups of a head, add their parts in a fixed order, the last
+ * workgroup to arrive those of all.  K is the A operand of 16 x 16 x 128, V of 16 x 16 x 32: lane l has the values of column n = l % 16,
+ * CD of each 16 CD, for the eight keys that its group of 16 lanes has weights of.  Most of a short call is instructions that run once,
+ * from a cold instruction cache: the code in front of the loop and behind it is kept short.  Bound: one query of 32 heads on 8 with 128
+ * values behind 65535 rows 19.5 us, 71 MB at 3.6 TB/s, of which 7 us do not depend on the rows; behind 1999 8.8 us, nothing but those. */
 template <int HP, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     constexpr int HD = 64 * HP, ROW = 32 * HP, KS = (HP + 1) / 2, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4;
@@ -403,7 +406,8 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     };
     auto item = [&](int t, const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070 | (2 * HP + 2));       /* vmcnt: the next tile may be on its way; lgkmcnt(0): what is asked for below overwrites what the last tile read */
+        /* vmcnt: the next tile may be on its way; lgkmcnt(0): what is asked for below overwrites what the last tile read */
+        __builtin_amdgcn_s_waitcnt(0x0070 | (2 * HP + 2));
         asm volatile("" ::: "memory");
         ask(later, t + 2);
         asm volatile("" ::: "memory");
@@ -534,13 +538,15 @@ __global__ void __launch_bounds__(64 * WAVES) vt_kv4_stream_kernel(kv4_job a) {
     }
 }
 
-/* Many columns: a workgroup has KV4_TILE of them, a wave 32, and goes through its rows 64 at a time.  K comes as it lies, V as fp16 in the order of
- * the matrix instruction's operand (A of 32 x 32 x 16, value 2 HP r + i in row r of instruction i; four keys of a value are 8 bytes): the workgroup
- * converts the next rows while it multiplies these, each lane four keys of eight values, so that a conversion serves all columns.  Scores are 32 x 32 x 64.
- * Where there are few columns for the chip, or a prompt's last ones would be behind everybody, several workgroups share a head's rows, `run` tiles
- * each; the last to arrive adds their parts.  Bound: 4000 queries of 32 heads on 8 with 128 values, 220 us, are 64 tiles for each of 512 workgroups that are there at once, 5000 cycles for the two
- * of a SIMD, of which 3300 are matrix instructions (20 for scores, 32 for results) and 3600 vector ones, at the clock that their power allows.  Reads of what is multiplied next, and the next weights'
- * arithmetic, stand between the products, and work is handed out head by head, the longest first: neither 283 us, the one 264, the other 231. */
+/* Many columns: a workgroup has KV4_TILE of them, a wave 32, and goes through its rows 64 at a time.  K comes as it lies, V as fp16 in
+ * the order of the matrix instruction's operand (A of 32 x 32 x 16, value 2 HP r + i in row r of instruction i; four keys of a value are
+ * 8 bytes): the workgroup converts the next rows while it multiplies these, each lane four keys of eight values, so that a conversion
+ * serves all columns.  Scores are 32 x 32 x 64. Where there are few columns for the chip, or a prompt's last ones would be behind
+ * everybody, several workgroups share a head's rows, `run` tiles each; the last to arrive adds their parts.  Bound: 4000 queries of 32
+ * heads on 8 with 128 values, 220 us, are 64 tiles for each of 512 workgroups that are there at once, 5000 cycles for the two of a SIMD,
+ * of which 3300 are matrix instructions (20 for scores, 32 for results) and 3600 vector ones, at the clock that their power allows.
+ * Reads of what is multiplied next, and the next weights' arithmetic, stand between the products, and work is handed out head by head,
+ * the longest first: neither 283 us, the one 264, the other 231. */
 
 template <int HP>
 __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4_job a) {
@@ -661,7 +667,8 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
 #pragma unroll
             for (int d = 0; d < 8; d++) {
                 const unsigned pick = d & 1 ? 0x07060302u : 0x05040100u;
-                *reinterpret_cast<u32x2 *>(b + v_to[i][d]) = u32x2{__builtin_amdgcn_perm(two[1][d / 2], two[0][d / 2], pick), __builtin_amdgcn_perm(two[3][d / 2], two[2][d / 2], pick)};
+                *reinterpret_cast<u32x2 *>(b + v_to[i][d]) = u32x2{__builtin_amdgcn_perm(two[1][d / 2], two[0][d / 2], pick),
+                                                                  __builtin_amdgcn_perm(two[3][d / 2], two[2][d / 2], pick)};
             }
         }
     };
@@ -698,7 +705,8 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                 for (int p = KV4_PLANES - 1; p >= 0; p--)
 #pragma unroll
                     for (int kk = 0; kk < HP; kk++)
-                        s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m1(k[kk]), vt_mfma_e2m3(q[kk][p]), s[kt], VT_MFMA_E2M1, VT_MFMA_E2M3, 0, ksc[kk], 0, (int)qs[kk][p]);
+                        s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m1(k[kk]), vt_mfma_e2m3(q[kk][p]), s[kt], VT_MFMA_E2M1, VT_MFMA_E2M3,
+                                                                                0, ksc[kk], 0, (int)qs[kk][p]);
             }
             if (first + 64 > seen_first || __any(k_scale > k_most)) {
 #pragma unroll
@@ -724,7 +732,8 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                 s[1] = s[1] - m;
                 base = (float)KV4_P_EXP;
             }
-            /* 16 keys a step: elements 8 (st % 2) .. of scores st / 2.  The next step's weights are made, and its values read, between this one's products. */
+            /* 16 keys a step: elements 8 (st % 2) .. of scores st / 2.  The next step's weights are made, and its values read, between
+             * this one's products. */
             u32x4 hi4, lo4;
             vt_f16x8 v[DT];
             auto weight = [&](int st, int e) __attribute__((always_inline)) {
@@ -734,7 +743,9 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
                 hi4[e] = __builtin_bit_cast(unsigned, hi2);
                 lo4[e] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{fmaf((float)hi2.x, minus, p0), fmaf((float)hi2.y, minus, p1)}), vt_f16x2));
             };
-            auto value = [&](int st, int i) __attribute__((always_inline)) { v[i] = __builtin_bit_cast(vt_f16x8, *reinterpret_cast<const u32x4 *>(b + VB + ((i * 4 + st) * 64 + lane) * 16)); };
+            auto value = [&](int st, int i) __attribute__((always_inline)) {
+                v[i] = __builtin_bit_cast(vt_f16x8, *reinterpret_cast<const u32x4 *>(b + VB + ((i * 4 + st) * 64 + lane) * 16));
+            };
 #pragma unroll
             for (int i = 0; i < DT; i++) value(0, i);
             __builtin_amdgcn_sched_barrier(0);
@@ -811,7 +822,8 @@ __global__ void __launch_bounds__(64 * KV4_TILE_WAVES, 2) vt_kv4_tile_kernel(kv4
         for (int i = 0; i < DT; i++)
 #pragma unroll
             for (int v = 0; v < 4; v++)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, (f32x4{o[i][4 * v], o[i][4 * v + 1], o[i][4 * v + 2], o[i][4 * v + 3]})), pd, mine + part * PART + (4 * i + v) * 1024, 0, 16 /* sc1 */);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, (f32x4{o[i][4 * v], o[i][4 * v + 1], o[i][4 * v + 2], o[i][4 * v + 3]})), pd,
+                                                       mine + part * PART + (4 * i + v) * 1024, 0, 16 /* sc1 */);
         __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, pd, mine + part * PART + DT * 4 * 1024, 0, 16);
         __builtin_amdgcn_s_waitcnt(0x0f70);              /* acknowledged */
         __syncthreads();
@@ -891,12 +903,13 @@ extern "C" int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_h
         const size_t at = (size_t)s * n_heads * cache->head_dim;
         const int heads = cache->n_kv_heads;
         const vt_kv4_plan p = vt_kv4_plan_of(n_cu, HP, heads, group, cols, start_pos + s, start_pos + s + n);
-        const kv4_job a = {cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, d_out + at, d_Q + at, NULL, g_vt.d_mx4_cnt, cache->max_rows, start_pos + s, n_heads, cols,
-                           p.run, p.parts, p.tiles, vt_divisor_of(group, cols), scale * 1.44269504f};
+        const kv4_job a = {cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, d_out + at, d_Q + at, NULL, g_vt.d_mx4_cnt,
+                           cache->max_rows, start_pos + s, n_heads, cols, p.run, p.parts, p.tiles, vt_divisor_of(group, cols), scale * 1.44269504f};
         const long long wgs = (long long)heads * p.tiles;
         int bad;
         if (p.many) bad = HP == 1 ? kv4_tiles<1>(a, heads, wgs) : kv4_tiles<2>(a, heads, wgs);
-        else bad = HP == 1 ? kv4_stream<1, 8>(a, heads, wgs) : HP == 2 ? kv4_stream<2, 8>(a, heads, wgs) : HP == 3 ? kv4_stream<3, 4>(a, heads, wgs) : kv4_stream<4, 4>(a, heads, wgs);
+        else if (HP <= 2) bad = HP == 1 ? kv4_stream<1, 8>(a, heads, wgs) : kv4_stream<2, 8>(a, heads, wgs);
+        else bad = HP == 3 ? kv4_stream<3, 4>(a, heads, wgs) : kv4_stream<4, 4>(a, heads, wgs);
         if (bad) return -1;
     }
     return vt_check(hipGetLastError(), who) ? -1 : 0;

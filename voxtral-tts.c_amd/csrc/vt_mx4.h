@@ -99,7 +99,8 @@ typedef int vt_i32x8 __attribute__((ext_vector_type(8)));
 /* the scale of a plane that stands in a fixed ratio to the one before: 2^-4 of its */
 __device__ __forceinline__ int vt_mx4_below(unsigned s) { return max((int)s - 4, 0); }
 
-/* The next plane of a block, and what it leaves of it; even[i], odd[i]: values 2 i and 2 i + 1.  tied: its scale follows from the one before, `scale`. */
+/* The next plane of a block, and what it leaves of it; even[i], odd[i]: values 2 i and 2 i + 1.  tied: its scale follows from the one
+ * before, `scale`. */
 __device__ __forceinline__ vt_u32x6 vt_mx4_plane(vt_f32x16 &even, vt_f32x16 &odd, bool tied, unsigned &scale) {
     float t = 0.f;
 #pragma unroll
@@ -126,8 +127,8 @@ __device__ __forceinline__ void vt_mx4_planes(vt_f32x16 even, vt_f32x16 odd, vt_
     }
 }
 
-/* 32 values of a row from column `at` on, through a buffer that holds the row `row_at` bytes in; zeros from column `cols` on.  whole: rows lie on 16 bytes.
- * (No branch around a load: behind one the compiler waits for it, a trip to memory each.) */
+/* 32 values of a row from column `at` on, through a buffer that holds the row `row_at` bytes in; zeros from column `cols` on.  whole:
+ * rows lie on 16 bytes. (No branch around a load: behind one the compiler waits for it, a trip to memory each.) */
 __device__ __forceinline__ void vt_mx4_load32(__amdgpu_buffer_rsrc_t x, int row_at, int at, int cols, int whole, vt_f32x16 &even, vt_f32x16 &odd) {
     if (whole) {
 #pragma unroll

@@ -21,8 +21,8 @@ int vt_mx4_ready(const char *who) {
 }
 
 /* ---- quantisation and the way back -------------------------------------------------------------------------------
- * A lane takes a unit of a row, eight consecutive values (a quad of lanes a block) on the way in, four on the way back.  Bound by memory: 9216 x 3072 from bf16 12.3 us, 5.8 TB/s in and out, from
- * fp32 23.3, 5.5 (two, four or eight rows a lane: 12.6 to 26). */
+ * A lane takes a unit of a row, eight consecutive values (a quad of lanes a block) on the way in, four on the way back.  Bound by
+ * memory: 9216 x 3072 from bf16 12.3 us, 5.8 TB/s in and out, from fp32 23.3, 5.5 (two, four or eight rows a lane: 12.6 to 26). */
 struct mx4_shape { int rows, cols, stride, units, wide_log; vt_divisor chunks; int whole; };
 
 static __device__ __forceinline__ bool mx4_place(const mx4_shape &s, int &row, int &unit) {
@@ -45,8 +45,8 @@ __global__ void __launch_bounds__(256) vt_mx4_quantize_kernel(unsigned *codes, u
     if ((unit & 3) == 0) scales[((size_t)row * s.units + unit) >> 2] = (uint8_t)scale;
 }
 
-/* The way back: four values a lane, so that a wave's store is one piece of memory, past the caches, which do not hold what is bigger than they are anyway: 9216 x 3072
- * 19.0 us (6.8 TB/s), through them 28, and 29.5 with eight values and two stores a lane. */
+/* The way back: four values a lane, so that a wave's store is one piece of memory, past the caches, which do not hold what is bigger
+ * than they are anyway: 9216 x 3072 19.0 us (6.8 TB/s), through them 28, and 29.5 with eight values and two stores a lane. */
 __global__ void __launch_bounds__(256) vt_mx4_dequantize_kernel(float *x, const uint16_t *codes, const uint8_t *scales, mx4_shape s) {
     int row, unit;
     if (!mx4_place(s, row, unit)) return;
@@ -127,7 +127,14 @@ extern "C" int tts_hip_mx4_dequantize(float *d_x, const uint8_t *d_codes, const 
 #define MXR_PLANES 5                       /* the last one's scale follows from the fourth's */
 #define MXR_PART (16 * 128 + 256)          /* codes, then 16 x 2 words of scales and as much room */
 
-struct mxr_job { float *y; const float *x; const uint8_t *codes, *scales; int seq_len, in_dim, out_dim, panels, cut_panels, cuts, rows_per_wg, share_log, whole; float *part; unsigned *cnt; };      /* 1 << share_log waves share K */
+struct mxr_job {
+    float *y;
+    const float *x;
+    const uint8_t *codes, *scales;
+    int seq_len, in_dim, out_dim, panels, cut_panels, cuts, rows_per_wg, share_log, whole;       /* 1 << share_log waves share K */
+    float *part;
+    unsigned *cnt;
+};
 
 /* columns of a block: the planes of all rows, and one of zeros; an odd number, so that consecutive blocks lie in different banks */
 static __host__ __device__ constexpr int mxr_columns(int seq_len) { return (MXR_PLANES * seq_len + 1) | 1; }
@@ -138,13 +145,15 @@ template <int G>
 __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) {
     constexpr int THREADS = 64 * MXR_WAVES, PP = 4 / (G - 1);         /* planes of an instruction but the first */
     constexpr int RING = mxr_ring(G);
-    __shared__ __attribute__((aligned(16))) unsigned char buf0[MXR_WAVES * MXR_PART], buf1[MXR_WAVES * MXR_PART], buf2[MXR_WAVES * MXR_PART], buf3[RING > 3 ? MXR_WAVES * MXR_PART : 16];
+    constexpr int BUF = MXR_WAVES * MXR_PART;
+    __shared__ __attribute__((aligned(16))) unsigned char buf0[BUF], buf1[BUF], buf2[BUF], buf3[RING > 3 ? BUF : 16];
     __shared__ float red[2][MXR_WAVES][64 * (G - 1)];          /* [row of x][weight row] */
     __shared__ int last;
     extern __shared__ __attribute__((aligned(16))) unsigned char planes[];
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int row0 = (int)blockIdx.x * a.rows_per_wg, rows = min(a.rows_per_wg, a.out_dim - row0);
-    const int share = 1 << a.share_log, groups = MXR_WAVES >> a.share_log, group = wave >> a.share_log;        /* waves that share K, and the blocks that are under way at once */
+    /* waves that share K, and the blocks that are under way at once */
+    const int share = 1 << a.share_log, groups = MXR_WAVES >> a.share_log, group = wave >> a.share_log;
     const int k0 = (int)blockIdx.y * a.cut_panels, k1 = min(k0 + a.cut_panels, a.panels), per_wave = (a.cut_panels + share - 1) >> a.share_log;
     const int p0 = min(k0 + (wave & (share - 1)) * per_wave, k1), p1 = min(p0 + per_wave, k1), parts = (per_wave + 1) / 2, blocks = (rows + 15) / 16;
     const int total = (blocks + groups - 1) / groups * parts;
@@ -156,7 +165,9 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
     int xr = (int)threadIdx.x / nb, xb = (int)threadIdx.x - xr * nb;
     const int xr_step = THREADS / nb, xb_step = THREADS - xr_step * nb;
     vt_f32x16 even, odd, next_even, next_odd;
-    auto ask_x = [&](vt_f32x16 &e, vt_f32x16 &o) __attribute__((always_inline)) { vt_mx4_load32(xd, xr * a.in_dim * 4, xr < a.seq_len ? 128 * k0 + 32 * xb : a.in_dim, a.in_dim, a.whole, e, o); };
+    auto ask_x = [&](vt_f32x16 &e, vt_f32x16 &o) __attribute__((always_inline)) {
+        vt_mx4_load32(xd, xr * a.in_dim * 4, xr < a.seq_len ? 128 * k0 + 32 * xb : a.in_dim, a.in_dim, a.whole, e, o);
+    };
     ask_x(even, odd);
     /* codes: lane i brings piece i % 8 of a line, exchanged so that eight rows' same piece lie in different banks; scales: word i % 2 of row i / 2 */
     const int w_at = (lane >> 3) * 64 * a.panels + ((lane & 7) ^ (lane >> 3)) * 16;                /* and 8 rows on: the same exchange */
@@ -166,13 +177,15 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
         const bool live = ask_block < blocks && p0 + 2 * ask_part < p1;         /* else zeros, which nobody reads */
         const int left = live ? min(16, rows - 16 * ask_block) : 0, panel = live ? p0 + 2 * ask_part : 0;
         const size_t r = (size_t)row0 + (live ? 16 * ask_block : 0);
-        /* from the panel on, with no scalar offset: the range check need not know of one.  (Past the last of an odd number of panels the last row's lanes read zeros, others the next row.) */
+        /* from the panel on, with no scalar offset: the range check need not know of one.  (Past the last of an odd number of panels the
+         * last row's lanes read zeros, others the next row.) */
         const size_t first = r * a.panels + panel;
         const int size = max(left * a.panels - panel, 0);
         const __amdgpu_buffer_rsrc_t wd = vt_buffer(a.codes + first * 64, size * 64), sd = vt_buffer(a.scales + first * 4, size * 4);
         unsigned char *b = buf + wave * MXR_PART;
 #pragma unroll
-        for (int d = 0; d < 2; d++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, (__attribute__((address_space(3))) void *)(b + d * 1024), 16, w_at + d * 8 * 64 * a.panels, 0, 0, 2);
+        for (int d = 0; d < 2; d++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, (__attribute__((address_space(3))) void *)(b + d * 1024), 16, w_at + d * 8 * 64 * a.panels, 0, 0, 2);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(sd, (__attribute__((address_space(3))) void *)(b + 2048), 4, s_at, 0, 0, 2);
         if (++ask_part >= parts) { ask_part = 0; ask_block += groups; }
     };
@@ -250,7 +263,8 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) vt_mx4_rows_kernel(mxr_job a) 
     int turn = 0, part = 0;
     auto item = [&](const unsigned char *here, unsigned char *later) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070 | 3 * (RING - 2));          /* vmcnt: two later parts, or one, may be on their way; lgkmcnt(0): what is asked for below overwrites what the last part read */
+        /* vmcnt: two later parts, or one, may be on their way; lgkmcnt(0): what is asked for below overwrites what the last part read */
+        __builtin_amdgcn_s_waitcnt(0x0070 | 3 * (RING - 2));
         asm volatile("" ::: "memory");
         ask(later);
         asm volatile("" ::: "memory");
@@ -324,8 +338,8 @@ static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * pan
  * there.  226 x 3072 x 9216 39 us: 6 the planes, 5 the sums, 28 the product, whose smaller tiles bring twice the bytes to LDS for each. */
 #define MXT_STEP (MXR_PLANES * 1536 + 256)               /* bytes of 32 rows x 64 columns of x */
 
-/* A wave has 32 rows by 64 columns; they go through LDS so that its loads are lines (a lane's own 128 bytes come in eight pieces, and with twenty waves on a CU the
- * rest of a line is gone from the first cache by the time of the next piece). */
+/* A wave has 32 rows by 64 columns; they go through LDS so that its loads are lines (a lane's own 128 bytes come in eight pieces, and
+ * with twenty waves on a CU the rest of a line is gone from the first cache by the time of the next piece). */
 __global__ void __launch_bounds__(256) vt_mx4_planes_kernel(unsigned char *out, const float *x, int seq_len, int in_dim, int panels, int tiles, int whole) {
     constexpr int ROW = 64 + 4;                          /* floats: eight rows' same piece lie in different banks */
     __shared__ __attribute__((aligned(16))) float turn[4][32 * ROW];
@@ -368,11 +382,13 @@ __global__ void __launch_bounds__(256) vt_mx4_planes_kernel(unsigned char *out, 
 
 struct mxt_job { float *y; const unsigned char *planes; const uint8_t *codes, *scales; int seq_len, out_dim, panels, tiles, cuts, m_tiles; };
 
-/* FM 32 weight rows a wave, NM x NN waves.  AHEAD: a workgroup with the CU to itself.  Its barrier stands in front of a panel's last quarter, whose x is in registers by then:
- * behind it the next panel's operands come from LDS while that quarter is multiplied (else the matrix units wait for them at every panel), half of the panel after that is asked for
- * there and the other half a quarter later.  Workgroups that share a CU fill such waits for each other and need the longer time to memory: they ask for a quarter of the next
- * panel behind each of this one's, with the barrier between panels.  us, with AHEAD and without, 512 and 1531 x 9216 x 3072 47.5 and 107 (53 and 114), 1000 x 3072 x 4096 and 16 x 131072 x 3072 51 and 80
- * (48 and 73). */
+/* FM 32 weight rows a wave, NM x NN waves.  AHEAD: a workgroup with the CU to itself.  Its barrier stands in front of the products of a
+ * panel's first plane, the last of five, whose x is in registers by then: behind it the next panel's operands come from LDS while these
+ * are multiplied (else the matrix units wait for them at every panel), half of the panel after that is asked for there and the other
+ * half a plane later.  Workgroups that share a CU fill such waits for each other and need the longer time to memory: they ask for a
+ * quarter of the next panel behind each of this one's first four planes, with the barrier between panels.  us, with AHEAD and without, as
+ * measured with four planes of x: 512 and 1531 x 9216 x 3072 47.5 and 107 (53 and 114), 1000 x 3072 x 4096 and 16 x 131072 x 3072 51 and
+ * 80 (48 and 73). */
 template <int FM, int NM, int NN, bool AHEAD>
 __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
     constexpr int THREADS = 64 * NM * NN, BM = 32 * FM * NM, W_BYTES = BM * 64, X_AT = W_BYTES + BM * 4, X_BYTES = NN * 2 * MXT_STEP;
@@ -398,7 +414,8 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
         const int dead = panel < p1 ? 0 : 0x40000000;
 #define LDS(at) (__attribute__((address_space(3))) void *)(b + (at))
 #pragma unroll
-        for (int i = 0; i < WU; i++) if (i % of == q) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, LDS(i * THREADS * 16 + wave * 1024), 16, (w_at[i] + panel * 64) | dead, 0, 0, 0);
+        for (int i = 0; i < WU; i++)
+            if (i % of == q) __builtin_amdgcn_raw_ptr_buffer_load_lds(wd, LDS(i * THREADS * 16 + wave * 1024), 16, (w_at[i] + panel * 64) | dead, 0, 0, 0);
         /* a wave without a share of a request: AHEAD sends it all the same, for nothing to a spare place, because products move across a branch */
         const bool has = wave * 64 < BM;
         if (q == of - 1 && (AHEAD || has))
@@ -437,8 +454,9 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
         if (!h) return;
         int at = ws_at;
         asm("" : "+v"(at));                              /* else a register for each sum with a buffer's place */
+        /* bytes 0 and 2: the lane's block of either half */
 #pragma unroll
-        for (int f = 0; f < FM; f++) ws[f] = (int)(*reinterpret_cast<const unsigned *>(b + at + (W_BYTES + f * 128)) >> (8 * g));       /* bytes 0 and 2: the lane's block of either half */
+        for (int f = 0; f < FM; f++) ws[f] = (int)(*reinterpret_cast<const unsigned *>(b + at + (W_BYTES + f * 128)) >> (8 * g));
     };
     auto meet = [&]() __attribute__((always_inline)) {   /* what was asked for is there, and everybody is through with what the next requests overwrite */
         __builtin_amdgcn_s_waitcnt(0x0070);
@@ -453,7 +471,8 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
         const int last[2] = {vt_mx4_below((unsigned)xs[0] >> 24), vt_mx4_below((unsigned)xs[1] >> 24)};
 #define PRODUCTS(x, h, byte, scales) \
         _Pragma("unroll") for (int f = 0; f < FM; f++) \
-            sum[f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(x[h]), vt_mfma_e2m1(w[f][h]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, byte, scales[h], 2 * h, ws[f]);
+            sum[f] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vt_mfma_e2m3(x[h]), vt_mfma_e2m1(w[f][h]), sum[f], VT_MFMA_E2M3, VT_MFMA_E2M1, \
+                                                                    byte, scales[h], 2 * h, ws[f]);
 #define PINNED(...) __builtin_amdgcn_sched_barrier(PIN); __VA_ARGS__ __builtin_amdgcn_sched_barrier(PIN);
         const vt_u32x6 x3[2] = {x_of(here, 3, 0), x_of(here, 3, 1)};
         PINNED()
@@ -516,14 +535,16 @@ __global__ void __launch_bounds__(64 * NM * NN) vt_mx4_tile_kernel(mxt_job a) {
 }
 
 template <int G> static int mxr_prepare(void) {
-    return vt_check(hipFuncSetAttribute((const void *)vt_mx4_rows_kernel<G>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(MXR_LDS_MOST - mxr_lds(G))), "tts_hip_linear_mx4: LDS");
+    return vt_check(hipFuncSetAttribute((const void *)vt_mx4_rows_kernel<G>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(MXR_LDS_MOST - mxr_lds(G))),
+                    "tts_hip_linear_mx4: LDS");
 }
 int vt_mx4_prepare(void) { return mxr_prepare<2>() || mxr_prepare<3>() ? -1 : 0; }
 
 static int mx4_linear_rows(float *d_y, const float *d_x, const uint8_t *d_codes, const uint8_t *d_scales, int seq_len, int in_dim, int out_dim, int whole) {
     const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256, panels = vt_mx4_panels(in_dim), g = seq_len <= 4 ? 2 : 3;
     const int most = (int)((MXR_LDS_MOST - mxr_lds(g)) / mxr_planes_bytes(seq_len, 1)), cuts = (panels + most - 1) / most, wgs = n_cu / cuts > 0 ? n_cu / cuts : 1;
-    mxr_job a = {d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, panels, (panels + cuts - 1) / cuts, cuts, (int)(((long long)out_dim + wgs - 1) / wgs), 2, whole, NULL, g_vt.d_mx4_cnt};
+    mxr_job a = {d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, panels, (panels + cuts - 1) / cuts, cuts,
+                 (int)(((long long)out_dim + wgs - 1) / wgs), 2, whole, NULL, g_vt.d_mx4_cnt};
     if (a.rows_per_wg <= 16) a.share_log = 3;          /* no second block for the other waves */
     a.cuts = (panels + a.cut_panels - 1) / a.cut_panels;
     if (a.cuts > 1 && !(a.part = (float *)vt_scratch(sizeof(float) * (size_t)a.cuts * seq_len * out_dim))) return -1;
@@ -561,8 +582,10 @@ extern "C" int tts_hip_linear_mx4(float *d_y, const float *d_x, const uint8_t *d
         if (mx4_linear_rows(d_y, d_x, d_codes, d_scales, seq_len, in_dim, out_dim, whole)) return -1;
     } else {
         const int most = vt_mxt_rows(out_dim, vt_mx4_panels(in_dim));
-        for (int s = 0; s < seq_len; s += most)
-            if (mx4_linear_tiles(d_y + (size_t)s * out_dim, d_x + (size_t)s * in_dim, d_codes, d_scales, seq_len - s < most ? seq_len - s : most, in_dim, out_dim, whole)) return -1;
+        for (int s = 0; s < seq_len; s += most) {
+            const int n = seq_len - s < most ? seq_len - s : most;
+            if (mx4_linear_tiles(d_y + (size_t)s * out_dim, d_x + (size_t)s * in_dim, d_codes, d_scales, n, in_dim, out_dim, whole)) return -1;
+        }
     }
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
