@@ -332,10 +332,10 @@ static size_t mxr_planes_bytes(int seq_len, int panels) { return (size_t)4 * pan
  * through K by panels of 128: both operands come straight into LDS, one panel ahead.  A wave has 32 rows of x and FM x 32 weight rows, so
  * that an operand of x, the larger one (3.75 bytes a value), is read once for FM products.  Ten products of a panel, the smallest planes
  * first, start from zero and are added by the vector unit (the matrix unit's sums are cut at 2^-23).  Few tiles: K is cut and the parts
- * are added by a kernel of their own.  Bound: 1531 x 9216 x 3072 120 us, 10 of them the planes; the product's 108 are five products of 43
- * GMAC, which keep the matrix units busy 46 % of the time (in two rounds of which the second is 69 % full), and 190 KB that its
- * eight waves read from LDS per panel, 1500 cycles of the 2600 that the matrix instructions take, with the next panel's 80 KB on their way
- * there.  226 x 3072 x 9216 39 us: 6 the planes, 5 the sums, 28 the product, whose smaller tiles bring twice the bytes to LDS for each. */
+ * are added by a kernel of their own.  Bound: 1531 x 9216 x 3072 119 to 127 us, 10 of them the planes; the product's 108 to 117 are five
+ * products of 43 GMAC, which keep the matrix units busy 47 % of the time (in two rounds of which the second is 69 % full), and 190 KB that its
+ * eight waves read from LDS per panel, 1500 cycles of the 2600 that the matrix instructions take, with the next panel's 80 KB on their
+ * way there.  226 x 3072 x 9216 38 to 40 us: 6 the planes, 6 the sums of 8 cuts, 27 the product, 192 workgroups. */
 #define MXT_STEP (MXR_PLANES * 1536 + 256)               /* bytes of 32 rows x 64 columns of x */
 
 /* A wave has 32 rows by 64 columns; they go through LDS so that its loads are lines (a lane's own 128 bytes come in eight pieces, and
