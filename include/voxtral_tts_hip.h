@@ -378,6 +378,69 @@ int tts_hip_kv4_read(float *d_K, float *d_V, const tts_hip_kv4_t *cache, int n_r
 int tts_hip_kv4_attention(float *d_out, const float *d_Q, const tts_hip_kv4_t *cache, int seq_len,
                           int start_pos, int n_heads, float scale);
 
+/* ==== several sequences over one paged key/value cache ====
+ * No counterpart in the reference, which serves one utterance at a time.  A pool is bf16 [n_pages, n_kv_heads, page_rows, head_dim], one for K
+ * and one for V, the caller's device memory on 16 bytes, a pair of them for every layer.  Row p of a sequence lies in row p % page_rows of
+ * the page that the sequence's table names at p / page_rows.  A batch is a number of sequences with their new rows, one token each or a chunk, one
+ * sequence's rows behind the other's in every matrix that a call takes; rows behind the last one are left as they were.  A program describes
+ * a step once (tts_hip_paged_set) and runs every layer's calls on that.  Values x are fp32 or, with x_bf16, bf16. */
+typedef struct {
+    int n_pages, page_rows;              /* page_rows: a power of two, 16 .. 2^20 */
+    int n_heads, n_kv_heads, head_dim;   /* head_dim 64, 128, 192 or 256; up to 4096 heads on a kv head */
+    int window;                          /* a query sees the last `window` rows, its own among them; 0: all */
+} tts_hip_paged_shape_t;
+typedef struct tts_hip_paged tts_hip_paged_t;
+
+/* A handle for batches of up to max_seqs sequences with max_rows new rows and max_table pages in all.  NULL: refused.  Touches no GPU
+ * state; the first tts_hip_paged_set allocates.  tts_hip_paged_free waits for the device. */
+tts_hip_paged_t *tts_hip_paged_create(const tts_hip_paged_shape_t *shape, int max_seqs, int max_rows, int max_table);
+void tts_hip_paged_free(tts_hip_paged_t *batch);
+/* The batch to come: sequence i has rows[i] new rows (none is allowed) behind past[i] cached ones and the pages tables[i * table_stride] ..,
+ * host memory that is read during the call.  Page numbers are checked, up to 2^30 rows a sequence; entries of pages that no new row sees are not looked at.
+ * Sequences may share pages that they read; a page that new rows go into twice is refused.  The description is on its way to the device when the call returns,
+ * behind everything that was queued before; a refused one leaves the handle without a batch. */
+int tts_hip_paged_set(tts_hip_paged_t *batch, int n_seqs, const int *past, const int *rows, const int *tables, int table_stride);
+/* The new rows' positions, one after the other (device memory of the handle), for tts_hip_rotary; NULL: no batch. */
+const int *tts_hip_paged_positions(const tts_hip_paged_t *batch);
+
+/* How heads are turned by their positions.  rot_dim values of each head turn, the first ones, in pairs: (2 i, 2 i + 1), or with half
+ * (i, i + rot_dim / 2); the others pass.  Pair i turns by 2 pi position d_turns[i] (device memory, rot_dim / 2 of them), times
+ * `magnitude`.  With d_gain (fp32 [head_dim], device) a head is divided by its root mean square first, sqrt(mean of squares + eps), and
+ * multiplied by the gains.  rot_dim 0: only that.  The struct is read from host memory during the call. */
+typedef struct {
+    const double *d_turns;
+    const float *d_gain;
+    int rot_dim, half;
+    float magnitude, eps;
+} tts_hip_rotary_t;
+
+/* d_turns[i] = theta^(-2 i / rot_dim) / 2 pi for i < rot_dim / 2, stretched by `factor` (1: not): a pair that makes fewer than low_turns
+ * turns in original_rows positions is divided by it, one that makes more than high_turns is not, in between the share goes with the turns.  original_rows 0
+ * and a low_turns above 0 divide all of them. */
+int tts_hip_rotary_turns(double *d_turns, int rot_dim, double theta, double factor, int original_rows, double low_turns, double high_turns);
+/* x [rows, n_heads, head_dim] -> out of the same type, x_stride and out_stride values from row to row (0: dense); row r at position
+ * d_positions[r] (any int; device).  out may be x with the same stride, else they do not overlap.  Any alignment that the type allows; rows on
+ * four values, head_dim a multiple of 8 and, with half, rot_dim too are fastest.  head_dim even, 2 .. 512.  Angles are as exact as fp32 holds them at
+ * any position, sums fp32, bf16 results are rounded once.  Values that do not turn and are not normed come out bit for bit. */
+int tts_hip_rotary(void *d_out, const void *d_x, int x_bf16, int rows, int n_heads, int head_dim, int out_stride, int x_stride,
+                   const int *d_positions, const tts_hip_rotary_t *how);
+
+/* The new rows' keys and values [rows, n_kv_heads * head_dim], `stride` values from row to row for both (0: dense), into their pages: keys
+ * turned and normed as `how` says (NULL: as they are), values as they are, each rounded to bf16 once.  Nothing else in a page changes. */
+int tts_hip_paged_append(const tts_hip_paged_t *batch, void *d_k_pages, void *d_v_pages, const void *d_K, const void *d_V, int x_bf16,
+                         int stride, const tts_hip_rotary_t *how);
+/* Causal attention of the new rows over their sequences: the query at position p sees the rows 0 .. p, or the last `window` of them, its own
+ * among them (append first).  Q [rows, n_heads * head_dim], q_stride values from row to row (0: dense, else a multiple of 8), out dense and of Q's type, both on 16 bytes;
+ * they do not overlap.  scale > 0.  What a query does not see changes nothing in its result, whatever it holds: rows of its pages behind the
+ * last one are not even read.  A query with an infinity or a NaN in it, and one that sees a key with a NaN, gives NaN; a key's infinity
+ * makes NaN too, or, where the score is -infinity, may leave the key without weight.  A value's infinity or NaN that a
+ * query sees makes that value of its result infinite or NaN.  Sums and softmax statistics are fp32.  fp32: queries (times scale) and
+ * weights enter to 24 bits, results are off by some 1e-7 of their norm; a score that leaves fp32 makes NaN.  bf16: a weight is rounded to bf16 once for more
+ * than 64 queries times heads on a kv head, and results once.  Where several workgroups share a sequence's rows their parts meet in the library's work
+ * area, which grows by allocation when a call needs more than any before it and stays. */
+int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16, int q_stride, const tts_hip_paged_t *batch, const void *d_k_pages,
+                            const void *d_v_pages, float scale);
+
 #ifdef __cplusplus
 }
 #endif

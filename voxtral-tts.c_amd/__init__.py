@@ -79,6 +79,18 @@ class Kv4(C.Structure):
                 ("max_rows", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
 
 
+class PagedShape(C.Structure):
+    """tts_hip_paged_shape_t: what the layers' pools and attention have in common."""
+    _fields_ = [("n_pages", C.c_int), ("page_rows", C.c_int), ("n_heads", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("window", C.c_int)]
+
+
+class Rotary(C.Structure):
+    """tts_hip_rotary_t: how heads are normed and turned by their positions."""
+    _fields_ = [("d_turns", vp), ("d_gain", vp), ("rot_dim", C.c_int), ("half", C.c_int),
+                ("magnitude", C.c_float), ("eps", C.c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/voxtral_tts_hip.h declares
 SIGNATURES = {
     "tts_hip_init": (C.c_int, [C.c_int]),
@@ -141,6 +153,14 @@ SIGNATURES = {
     "tts_hip_kv4_append": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int]),
     "tts_hip_kv4_read": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int]),
     "tts_hip_kv4_attention": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float]),
+    "tts_hip_paged_create": (vp, [vp, C.c_int, C.c_int, C.c_int]),
+    "tts_hip_paged_free": (None, [vp]),
+    "tts_hip_paged_set": (C.c_int, [vp, C.c_int, vp, vp, vp, C.c_int]),
+    "tts_hip_paged_positions": (vp, [vp]),
+    "tts_hip_rotary_turns": (C.c_int, [vp, C.c_int, C.c_double, C.c_double, C.c_int, C.c_double, C.c_double]),
+    "tts_hip_rotary": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]),
+    "tts_hip_paged_append": (C.c_int, [vp, vp, vp, vp, vp, C.c_int, C.c_int, vp]),
+    "tts_hip_paged_attention": (C.c_int, [vp, vp, C.c_int, C.c_int, vp, vp, vp, C.c_float]),
 }
 
 # every symbol include/voxtral_tts_hip_bench.h declares (csrc/libvoxtral_tts_hip_bench.so, the benchmark

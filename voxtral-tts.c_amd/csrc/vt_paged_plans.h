@@ -1,0 +1,199 @@
+/*
+ * vt_paged_plans.h - a batch of sequences over a paged cache (vt_paged.hip): what is refused, and the attention's work items from
+ * shapes and the number of CUs.  Host code without HIP, so that a host test can walk it.
+ */
+#ifndef VT_PAGED_PLANS_H
+#define VT_PAGED_PLANS_H
+
+#include <limits.h>
+#include <stdint.h>
+#include <stdlib.h>
+
+#define PAGED_MAX_POS (1 << 30)            /* rows of a sequence */
+#define PAGED_MAX_ROWS (1 << 22)           /* new rows of a batch */
+#define PAGED_MAX_GROUP 4096               /* heads on a kv head */
+#define PAGED_COUNTERS 16384               /* heads times tiles of columns that several workgroups share */
+
+/* Columns are a sequence's new rows times the heads that share a kv head: column c is row c / group, head c % group of the group.
+ * Few columns: 16 to a workgroup, whose waves take 32 rows of the cache each in turn.  Many: 128 to a workgroup, 64 rows at a time. */
+#define PAGED_FEW_COLS 16
+#define PAGED_FEW_ROWS 32
+#define PAGED_FEW_WAVES 4
+#define PAGED_MANY_COLS 128
+#define PAGED_MANY_ROWS 64
+#define PAGED_MAX_PARTS 64
+#define PAGED_SPLIT_ITEMS 4096             /* items that a launch may have beyond one for each tile of columns */
+
+/* What a workgroup does for every kv head: columns c0 .. of a sequence whose new rows are `row` .. of the batch and lie behind `past`
+ * rows, over the cache's rows lo .. end - 1; `parts` of them make up the columns' result, in slots `slot` .. */
+struct vt_paged_item { int row, past, cols, table, c0, lo, end, slot, part, parts, counter, spare; };
+
+struct vt_paged_shape { int n_pages, page_rows, n_heads, n_kv_heads, head_dim, window; };
+
+/* NULL, or why the shape is none */
+static inline const char *vt_paged_shape_bad(const vt_paged_shape &s) {
+    if (s.page_rows < 16 || s.page_rows > 1 << 20 || (s.page_rows & (s.page_rows - 1))) return "page_rows is a power of two from 16 to 2^20";
+    if (s.n_pages < 1) return "no pages";
+    if (s.head_dim < 64 || s.head_dim > 256 || s.head_dim % 64) return "head_dim is 64, 128, 192 or 256";
+    if (s.n_kv_heads < 1 || s.n_kv_heads > 65535 || s.n_heads < 1 || s.n_heads % s.n_kv_heads) return "n_heads is a multiple of n_kv_heads, which are at most 65535";
+    if (s.n_heads / s.n_kv_heads > PAGED_MAX_GROUP) return "more than 4096 heads on a kv head";
+    if ((long long)s.n_heads * s.head_dim > INT_MAX / 4) return "rows of more values than 2^29";
+    if (s.window < 0) return "a negative window";
+    return NULL;
+}
+
+/* rows of the cache that the new rows q0 .. q1 of a sequence see: from first on, up to past + q1 */
+static inline int vt_paged_first(int window, int past, int q0) { return window && past + q0 >= window ? past + q0 - window + 1 : 0; }
+
+static int vt_paged_by_value(const void *a, const void *b) {
+    const int x = *(const int *)a, y = *(const int *)b;
+    return x < y ? -1 : x > y;
+}
+
+/* The batch as the kernels read it: of each new row its position, page and row in the page, of each sequence its pages' numbers one behind
+ * the other from `starts` on. */
+struct vt_paged_rows { int *pos, *place, *tables, *starts, *written; };
+
+enum { PAGED_OK, PAGED_COUNT, PAGED_SEQUENCE, PAGED_TOO_MANY_ROWS, PAGED_TABLE, PAGED_PAGE, PAGED_WRITTEN };
+struct vt_paged_fault { int what, seq, at, value; };
+
+/* Checks a batch and lays it out; `tables` [n_seqs, stride].  Entries of pages that no new row sees are not looked at. */
+static inline vt_paged_fault vt_paged_lay_out(const vt_paged_shape &s, int max_seqs, int max_rows, int max_table, int n_seqs, const int *past, const int *rows,
+                                              const int *tables, int stride, const vt_paged_rows &to, int *n_rows, int *n_table) {
+    int at = 0, entry = 0, written = 0, log = 0;
+    while (1 << log < s.page_rows) log++;
+    if (n_seqs < 0 || n_seqs > max_seqs || stride < 0) return vt_paged_fault{PAGED_COUNT, 0, 0, 0};
+    for (int i = 0; i < n_seqs; i++) {
+        if (past[i] < 0 || rows[i] < 0 || (long long)past[i] + rows[i] > PAGED_MAX_POS) return vt_paged_fault{PAGED_SEQUENCE, i, 0, 0};
+        if (rows[i] > max_rows - at) return vt_paged_fault{PAGED_TOO_MANY_ROWS, i, 0, 0};
+        to.starts[i] = entry;
+        if (rows[i] == 0) continue;
+        const int pages = ((past[i] + rows[i] - 1) >> log) + 1, seen = vt_paged_first(s.window, past[i], 0) >> log, fresh = past[i] >> log;
+        if (pages > stride || pages > max_table - entry) return vt_paged_fault{PAGED_TABLE, i, pages, 0};
+        const int *from = tables + (size_t)i * stride;
+        for (int p = 0; p < pages; p++) {
+            if (p >= seen && (from[p] < 0 || from[p] >= s.n_pages)) return vt_paged_fault{PAGED_PAGE, i, p, from[p]};
+            to.tables[entry + p] = p >= seen ? from[p] : 0;
+            if (p >= fresh) to.written[written++] = from[p];
+        }
+        for (int r = 0; r < rows[i]; r++, at++) {
+            const int pos = past[i] + r;
+            to.pos[at] = pos;
+            to.place[2 * at] = from[pos >> log];
+            to.place[2 * at + 1] = pos & (s.page_rows - 1);
+        }
+        entry += pages;
+    }
+    /* a page that two sequences write to, or one twice, would hold whichever came last */
+    qsort(to.written, written, sizeof(int), vt_paged_by_value);
+    for (int i = 1; i < written; i++)
+        if (to.written[i] == to.written[i - 1]) return vt_paged_fault{PAGED_WRITTEN, 0, 0, to.written[i]};
+    *n_rows = at;
+    *n_table = entry;
+    return vt_paged_fault{PAGED_OK, 0, 0, 0};
+}
+
+/* ---- work items --- */
+
+struct vt_paged_plan { int few, many, few_slots, many_slots; };       /* items of either kernel (the few's first), parts that they leave */
+
+/* a launch's tiles of columns: how many, how many rows of the cache they read in all, and the most that one reads */
+struct vt_paged_sum { long long tiles, rows, longest; };
+
+static inline long long vt_paged_max_items(int max_seqs, int max_rows, int group) {
+    return (long long)max_rows * group / PAGED_FEW_COLS + max_seqs + 2 * PAGED_SPLIT_ITEMS;
+}
+
+static inline bool vt_paged_is_many(int hp, long long cols) { return hp <= 2 && cols > 64; }
+
+/* calls f(sequence, c0, first row, end) for every tile of columns of one kernel's sequences */
+template <class F>
+static inline void vt_paged_tiles(const vt_paged_shape &s, bool many, int n_seqs, const int *past, const int *rows, F f) {
+    const int group = s.n_heads / s.n_kv_heads, wide = many ? PAGED_MANY_COLS : PAGED_FEW_COLS, hp = s.head_dim / 64;
+    for (int i = 0; i < n_seqs; i++) {
+        const long long cols = (long long)rows[i] * group;
+        if (vt_paged_is_many(hp, cols) != many) continue;
+        for (long long c0 = 0; c0 < cols; c0 += wide) {
+            const long long last = (c0 + wide < cols ? c0 + wide : cols) - 1;
+            f(i, (int)c0, vt_paged_first(s.window, past[i], (int)(c0 / group)), past[i] + (int)(last / group) + 1);
+        }
+    }
+}
+
+/* rows of the cache that a part has: `run` steps of `unit` */
+static inline int vt_paged_parts(int first, int end, int unit, int run) {
+    const long long units = ((long long)end + unit - 1) / unit - first / unit;
+    return (int)((units + run - 1) / run);
+}
+
+/* The run with the least time, by figures of one item: `alone` us and `step` us a unit with a CU's other workgroups beside it, `merge` where
+ * parts meet; workgroups are handed out as they come, the longest first. */
+static inline int vt_paged_run(const vt_paged_shape &s, bool many, int n_cu, int n_seqs, const int *past, const int *rows, int unit, double fixed, double step, double merge) {
+    const double slots = 2.0 * n_cu;
+    long long longest = 1;
+    vt_paged_tiles(s, many, n_seqs, past, rows, [&](int, int, int first, int end) {
+        const long long n = vt_paged_parts(first, end, unit, 1);
+        longest = n > longest ? n : longest;
+    });
+    int best = (int)longest;
+    double least = 1e300;
+    for (long long run = longest, parts = 1; parts <= PAGED_MAX_PARTS; parts++) {
+        run = (longest + parts - 1) / parts;
+        long long items = 0, extra = 0, split = 0, most = 0;
+        double work = 0;
+        vt_paged_tiles(s, many, n_seqs, past, rows, [&](int, int, int first, int end) {
+            const int n = vt_paged_parts(first, end, unit, 1), p = (int)((n + run - 1) / run), each = (n + p - 1) / p;
+            items += p;
+            extra += p > 1 ? p : 0;
+            split += p > 1;
+            most = each > most ? each : most;
+            work += p * fixed + n * step;
+        });
+        if (extra > PAGED_SPLIT_ITEMS || split * s.n_kv_heads > PAGED_COUNTERS) break;
+        const double wgs = (double)items * s.n_kv_heads, share = wgs < slots ? 0.5 + 0.5 * wgs / slots : 1.0;
+        const double one = fixed + most * step * share, all = work * s.n_kv_heads / slots;
+        const double us = (one > all ? one : all) + (wgs > slots ? 0.5 * one : 0.0) + (split ? merge : 0.0);
+        if (us < least) { least = us; best = (int)run; }
+        if (run == 1) break;
+    }
+    return best;
+}
+
+static int vt_paged_longest(const void *a, const void *b) {
+    const vt_paged_item *x = (const vt_paged_item *)a, *y = (const vt_paged_item *)b;
+    const int n = x->end - x->lo, m = y->end - y->lo;
+    if (n != m) return n > m ? -1 : 1;
+    if (x->row != y->row) return x->row < y->row ? -1 : 1;
+    if (x->c0 != y->c0) return x->c0 < y->c0 ? -1 : 1;
+    return x->part < y->part ? -1 : x->part > y->part;
+}
+
+/* Items of one kernel into `to`, the longest first; -> how many, and their slots */
+static inline int vt_paged_items(const vt_paged_shape &s, bool many, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to, int *n_slots) {
+    const int unit = many ? PAGED_MANY_ROWS : PAGED_FEW_ROWS * PAGED_FEW_WAVES, group = s.n_heads / s.n_kv_heads;
+    const double hp = s.head_dim / 64;
+    const int run = many ? vt_paged_run(s, true, n_cu, n_seqs, past, rows, unit, 6.0, 1.5 * hp, 4.0) : vt_paged_run(s, false, n_cu, n_seqs, past, rows, unit, 4.0, 0.6 * hp, 3.0);
+    int n = 0, slots = 0, counters = 0, row = 0, seq = 0;
+    vt_paged_tiles(s, many, n_seqs, past, rows, [&](int i, int c0, int first, int end) {
+        while (seq < i) row += rows[seq++];
+        const int units = vt_paged_parts(first, end, unit, 1), parts = (units + run - 1) / run, u0 = first / unit;
+        for (int p = 0; p < parts; p++) {
+            const int from = (int)((long long)units * p / parts), till = (int)((long long)units * (p + 1) / parts);
+            to[n++] = vt_paged_item{row, past[i], rows[i] * group, starts[i], c0, p ? (u0 + from) * unit : first, p + 1 < parts ? (u0 + till) * unit : end,
+                                    slots, p, parts, counters, 0};
+        }
+        if (parts > 1) { slots += parts; counters++; }
+    });
+    qsort(to, n, sizeof *to, vt_paged_longest);
+    *n_slots = slots;
+    return n;
+}
+
+static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to) {
+    vt_paged_plan p;
+    p.few = vt_paged_items(s, false, n_cu, n_seqs, past, rows, starts, to, &p.few_slots);
+    p.many = vt_paged_items(s, true, n_cu, n_seqs, past, rows, starts, to + p.few, &p.many_slots);
+    return p;
+}
+
+#endif /* VT_PAGED_PLANS_H */

@@ -155,3 +155,31 @@ class Hip:
         self.lib.tts_hip_acoustic_frame(codes.ctypes.data, h.ctypes.data, x0.ctypes.data, x.ctypes.data)
         self.check()
         return codes, x
+
+
+class PagedBatch:
+    """A batch of sequences over a paged cache (tts_hip_paged_t): the handle, and what the calls read of it."""
+
+    def __init__(self, n_pages, page_rows, n_heads, n_kv_heads, head_dim, window=0, max_seqs=64, max_rows=4096, max_table=65536):
+        from . import PagedShape
+        self.lib = lib()
+        self.shape = PagedShape(n_pages, page_rows, n_heads, n_kv_heads, head_dim, window)
+        self.ptr = self.lib.tts_hip_paged_create(C.byref(self.shape), max_seqs, max_rows, max_table)
+        if not self.ptr:
+            raise ValueError(self.lib.tts_hip_last_error().decode())
+
+    def set(self, past, rows, tables):
+        """Sequence i has rows[i] new rows behind past[i] and the pages tables[i]; 0, or -1 where the library refuses."""
+        past, rows = np.ascontiguousarray(past, np.int32), np.ascontiguousarray(rows, np.int32)
+        wide = np.full((len(tables), max([1] + [len(t) for t in tables])), -1, np.int32)
+        for i, t in enumerate(tables):
+            wide[i, :len(t)] = t
+        return self.lib.tts_hip_paged_set(self.ptr, len(past), past.ctypes.data, rows.ctypes.data, wide.ctypes.data, wide.shape[1])
+
+    def positions(self):
+        return self.lib.tts_hip_paged_positions(self.ptr)
+
+    def free(self):
+        if self.ptr:
+            self.lib.tts_hip_paged_free(self.ptr)
+            self.ptr = None
