@@ -67,6 +67,17 @@ static __device__ __forceinline__ void pa_query(const void *Q, size_t at, float 
     } else to[0] = *reinterpret_cast<const u32x4 *>((const uint16_t *)Q + at);
 }
 
+template <bool F32>
+static __device__ __forceinline__ void pa_store4(void *out, size_t at, const f32x4 &v) {
+    if constexpr (F32) *reinterpret_cast<f32x4 *>((float *)out + at) = v;
+    else {
+        unsigned w0[1], w1[1];
+        pa_planes2<1>(v.x, v.y, w0);
+        pa_planes2<1>(v.z, v.w, w1);
+        *reinterpret_cast<u32x2 *>((uint16_t *)out + at) = u32x2{w0[0], w1[0]};
+    }
+}
+
 /* pairs of bf16 of which one is not finite */
 typedef unsigned short pa_u16x2 __attribute__((ext_vector_type(2)));
 static __device__ __forceinline__ pa_u16x2 pa_larger(pa_u16x2 most, unsigned w) { return __builtin_elementwise_max(most, __builtin_bit_cast(pa_u16x2, w & 0x7fff7fffu)); }
@@ -77,11 +88,25 @@ static __device__ __forceinline__ unsigned pa_finite(unsigned w) { return ((w & 
 
 static __device__ __forceinline__ float pa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+/* A column's weights are relative to m, which follows the largest score only where that is further above than this: weights up to 2^8 are as exact as ones below 1,
+ * and what was summed so far is scaled anew in the first tile and hardly ever after it (with 32 columns to a wave one of them has a new largest score in nearly every tile). */
+#define PA_SLACK 8.f
+template <bool F32>
+static __device__ __forceinline__ float pa_weight(float s, float m, float scale) { return pa_exp2(F32 ? s - m : fmaf(s, scale, -m)); }
+
+/* What the batch's description holds is the same for a whole workgroup: scalar loads, which the kernel's own stores cannot touch */
+typedef __attribute__((address_space(4))) const int pa_const_int;
+static __device__ __forceinline__ vt_paged_item pa_item(const vt_paged_item *items) {
+    static_assert(sizeof(vt_paged_item) == 48, "words");
+    const pa_const_int *w = (const pa_const_int *)(uintptr_t)(items + blockIdx.y);
+    return vt_paged_item{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9], w[10], 0};
+}
+
 /* 16 rows from `at` on, a multiple of 16, of those lo .. end - 1: where they lie, and the bytes of them that are there */
 struct pa_rows { size_t row; int bytes; };
-static __device__ __forceinline__ pa_rows pa_place(const int *table, int at, int lo, int end, int page_log, int heads, int head, int row_bytes) {
+static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, int at, int lo, int end, int page_log, int heads, int head, int row_bytes) {
     const int seen = min(at, end - 1), n = at + 16 > lo ? min(max(end - at, 0), 16) : 0;
-    const int page = __builtin_amdgcn_readfirstlane(table[max(seen, lo) >> page_log]);
+    const int page = table[max(seen, lo) >> page_log];
     return pa_rows{((((size_t)(unsigned)page * heads + head) << page_log) + (at & ((1 << page_log) - 1))), n * row_bytes};
 }
 
@@ -98,8 +123,9 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
     __shared__ float ml[WAVES][COLS][2], wt[COLS][PAGED_MAX_PARTS];
     __shared__ int last;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4, h = (int)blockIdx.x, heads = (int)gridDim.x;
-    const vt_paged_item it = a.items[blockIdx.y];
-    const int nc = min(COLS, it.cols - it.c0), *table = a.tables + it.table;
+    const vt_paged_item it = pa_item(a.items);
+    const int nc = min(COLS, it.cols - it.c0);
+    const pa_const_int *table = (const pa_const_int *)(uintptr_t)(a.tables + it.table);
     const int cc = min(it.c0 + n, it.cols - 1), qi = vt_div(cc, a.group), pos = it.past + qi;
     const int see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_hi = pos + 1;
     const int q_first = it.past + vt_div(it.c0, a.group), q_last = it.past + vt_div(it.c0 + nc - 1, a.group);
@@ -152,6 +178,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
     for (int t = wave; t < tiles; t += WAVES) {
         const int first = base + PAGED_FEW_ROWS * t;
         const bool hidden = first < all_lo || first + PAGED_FEW_ROWS > all_hi || first < it.lo || first + PAGED_FEW_ROWS > it.end;
+        place(t + WAVES);
         f32x4 s[2];
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) {
@@ -160,9 +187,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
             for (int p = NQ - 1; p >= 0; p--)
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(kr[kt][ks]), pa_operand(q[ks][p]), s[kt], 0, 0, 0);
-            if constexpr (!F32) s[kt] = s[kt] * a.scale;
         }
-        place(t + WAVES);
         ask_k();
         auto sees = [&](int kt, int v) { const int key = first + 16 * kt + 4 * g + v; return key >= max(see_lo, it.lo) && key < min(see_hi, it.end); };
         bool bad = false;
@@ -180,16 +205,18 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
                     for (int e = 0; e < CD / 2; e++) most = pa_larger(most, vr[j][ch][e]);
             bad = __any(pa_not_finite(most));
         }
-        float top = m;                                   /* a NaN stays one: who sees it answers NaN */
+        float top = __builtin_elementwise_maximum(s[0][0], s[1][0]);                /* a NaN stays one: who sees it answers NaN */
 #pragma unroll
-        for (int v = 0; v < 4; v++) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][v]), s[1][v]);
+        for (int v = 1; v < 4; v++) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][v]), s[1][v]);
         {
             f32x2 r = vt_swap16(top, top);
             top = __builtin_elementwise_maximum(r.x, r.y);
             r = vt_swap32(top, top);
             top = __builtin_elementwise_maximum(r.x, r.y);
         }
-        if (__any(top != m)) {
+        if constexpr (!F32) top = top * a.scale;
+        if (__any(!(top <= m + PA_SLACK))) {
+            top = __builtin_elementwise_maximum(top, m);
             const float less = pa_exp2(m - top);
             l *= less;
 #pragma unroll
@@ -199,7 +226,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
         u32x4 w4[NP];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float p0 = pa_exp2(s[e >> 1][2 * (e & 1)] - m), p1 = pa_exp2(s[e >> 1][2 * (e & 1) + 1] - m);
+            const float p0 = pa_weight<F32>(s[e >> 1][2 * (e & 1)], m, a.scale), p1 = pa_weight<F32>(s[e >> 1][2 * (e & 1) + 1], m, a.scale);
             l += p0 + p1;
             unsigned w[NP];
             pa_planes2<NP>(p0, p1, w);
@@ -266,13 +293,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
     auto result = [&](int col, int d, const f32x4 &v) {
         const int k = it.c0 + col, i = vt_div(k, a.group);
         const size_t to = ((size_t)(it.row + i) * a.n_heads + (size_t)h * a.group.d + (k - i * a.group.d)) * HD + d;
-        if constexpr (F32) *reinterpret_cast<f32x4 *>((float *)a.out + to) = v;
-        else {
-            unsigned w0[1], w1[1];
-            pa_planes2<1>(v.x, v.y, w0);
-            pa_planes2<1>(v.z, v.w, w1);
-            *reinterpret_cast<u32x2 *>((uint16_t *)a.out + to) = u32x2{w0[0], w1[0]};
-        }
+        pa_store4<F32>(a.out, to, v);
     };
     for (int e = (int)threadIdx.x; e < nc * (HD / 4); e += 64 * WAVES) {
         const int col = e / (HD / 4), d = 4 * (e - col * (HD / 4));
@@ -324,182 +345,255 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
 }
 
 /* ---- many columns ------------------------------------------------------------------------------------------------
- * A workgroup has 128 columns, a wave 32, and goes through its rows 64 at a time, 16 of them each wave's to bring: K through requests that write LDS, V as the matrix
- * instruction's operand (A of 32 x 32 x 16, value 2 HP r + i in row r of instruction i; four rows of a value are 8 bytes), put together in registers while the rows before are multiplied. */
+ * A workgroup has 128 columns, a wave 32, and goes through its rows 64 at a time, 16 of them each wave's to ask for, by requests that write LDS.  K's rows are the A operand of
+ * 32 x 32 x 16 as they lie; of V, whose rows are that operand's columns, the transposing reads of LDS give a lane four rows' values of one column.
+ *
+ * A unit is 32 rows.  While unit u's weights are made and multiplied, the matrix cores make unit u + 1's scores, so that K's tiles lie half a tile behind V's: beside V's rows
+ * 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95. */
+typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
+
 template <int HP, bool F32>
 __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
-    constexpr int HD = 64 * HP, ROW = 2 * HD, WAVES = 4, DT = 2 * HP, KS = 4 * HP, PIECES = HD / 8, VD = 4 * HP, VW = VD / 2;
+    constexpr int HD = 64 * HP, ROW = 2 * HD, WAVES = 4, DT = 2 * HP, KS = 4 * HP, PIECES = HD / 8;
     constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 1, KB = 64 * ROW;
-    constexpr int SUB = 2;                               /* 32 rows: tiles of scores that are worked on together */
-    __shared__ __attribute__((aligned(16))) unsigned char buf[2][2 * KB];
-    __shared__ int odd[2][WAVES];                        /* values at hand that are not finite */
-    __shared__ int last;
+    /* objects of their own: a read waits for the requests that write the same one */
+    __shared__ __attribute__((aligned(16))) unsigned char k0[KB], k1[KB], v0[KB], v1[KB];
+    /* Tiles with rows that some column does not see: at most 3 where the columns' rows begin to be seen and 3 where they end (fewer queries than 128 apart), or 5 with a window of less */
+    constexpr int EDGES = 6;
+    __shared__ unsigned marks[EDGES][64][DT];            /* of such a tile the values that are not finite, 32 of a row's to a word; where there are any: .. */
+    __shared__ int odd[EDGES][WAVES], last;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5, h = (int)blockIdx.x, heads = (int)gridDim.x;
-    const vt_paged_item it = a.items[blockIdx.y];
-    const int *table = a.tables + it.table;
+    const vt_paged_item it = pa_item(a.items);
+    const pa_const_int *table = (const pa_const_int *)(uintptr_t)(a.tables + it.table);
     const int w0 = it.c0 + 32 * wave, wc = min(w0 + 32, it.cols) - w0;                   /* this wave's columns: none, perhaps */
     const int cc = min(w0 + n, it.cols - 1), qi = vt_div(cc, a.group), pos = it.past + qi;
     const int see_lo = max(a.window && pos >= a.window ? pos - a.window + 1 : 0, it.lo), see_hi = min(pos + 1, it.end);
     const int q_first = it.past + vt_div(min(w0, it.cols - 1), a.group), q_last = it.past + vt_div(min(w0 + 31, it.cols - 1), a.group);
     const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);     /* rows that every column of the wave sees */
-    const int any_lo = a.window && q_first >= a.window ? q_first - a.window + 1 : 0, any_hi = wc > 0 ? q_last + 1 : 0;                 /* .. that any does */
+    const int any_lo = a.window && q_first >= a.window ? q_first - a.window + 1 : 0, any_hi = wc > 0 ? min(q_last + 1, it.end) : 0;   /* .. that any does */
+    const int wg_last = it.past + vt_div(min(it.c0 + PAGED_MANY_COLS, it.cols) - 1, a.group);
+    const int wg_lo = max(a.window && wg_last >= a.window ? wg_last - a.window + 1 : 0, it.lo), wg_hi = min(it.past + vt_div(it.c0, a.group) + 1, it.end);         /* rows that every column sees */
     const int base = it.lo & ~(PAGED_MANY_ROWS - 1), tiles = (it.end - base + PAGED_MANY_ROWS - 1) / PAGED_MANY_ROWS;
     const size_t head_at = (size_t)h * a.group.d + (cc - qi * a.group.d);
     u32x4 q[KS][NQ];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) pa_query<F32, NQ>(a.Q, (size_t)(it.row + qi) * a.q_stride + head_at * HD + 16 * ks + 8 * g, a.scale, q[ks]);
-    /* K's pieces of 16 bytes are exchanged within a row, so that 16 (8) rows' same piece lie in different banks */
-    constexpr int SWAP = PIECES % 16 ? 7 : 15;
-    int k_at[4];                                         /* DT of them (with that size the host pass drops the kernel) */
+    /* Pieces of 16 bytes change places within a row, so that what is read at once lies in different banks: K's with the row's last bits, so that 16 (8) rows' same piece do; V's fours of
+     * them, so that four rows' same 64 bytes do. */
+    constexpr int SWAP = PIECES - 1;
+    auto v_swap = [](int r) { return HP == 1 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
+    int k_at[4], v_at[4];                                /* DT of them (with that size the host pass drops the kernel) */
 #pragma unroll
     for (int d = 0; d < DT; d++) {
         const int u = d * 64 + lane, r = u / PIECES;
         k_at[d] = r * ROW + ((u - r * PIECES) ^ (r & SWAP)) * 16;
+        v_at[d] = r * ROW + ((u - r * PIECES) ^ v_swap(r)) * 16;
     }
-    const int v_at = 4 * (lane >> 4) * ROW + (lane & 15) * 2 * VD;
-    unsigned vr[4][4];                                   /* VW of each */
-    pa_rows at = pa_place(table, base + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW);
-    auto load = [&](unsigned char *b) __attribute__((always_inline)) {
-        const __amdgpu_buffer_rsrc_t kd = vt_buffer(a.K + at.row * HD, at.bytes), vd = vt_buffer(a.V + at.row * HD, at.bytes);
+    auto place = [&](int from) __attribute__((always_inline)) { return pa_place(table, from + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW); };
+    auto load = [&](const uint16_t *pool, const pa_rows &at, const int (&from)[4], unsigned char *to) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t d = vt_buffer(pool + at.row * HD, at.bytes);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-#pragma unroll
-            for (int e = 0; e < VW; e += VW % 4 ? 2 : 4) {
-                if constexpr (VW % 4) {
-                    const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(vd, v_at + k * ROW + 4 * e, 0, 0);
-                    vr[k][e] = w.x; vr[k][e + 1] = w.y;
-                } else {
-                    const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(vd, v_at + k * ROW + 4 * e, 0, 0);
-                    vr[k][e] = w.x; vr[k][e + 1] = w.y; vr[k][e + 2] = w.z; vr[k][e + 3] = w.w;
-                }
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(kd, (__attribute__((address_space(3))) void *)(b + wave * 16 * ROW + d * 1024), 16, k_at[d], 0, 0, 0);
-    };
-    /* value d's four rows (kg = 4 wave + lane / 16 of the tile's 16 fours) go to row r = d / DT of instruction i = d % DT, step kg / 4, group of lanes kg % 2, half kg / 2 % 2 */
-    const int v_to = KB + ((wave * 64 + ((lane >> 4) & 1) * 32 + 2 * (lane & 15)) * 2 + (lane >> 5)) * 8;
-    auto put = [&](int which) __attribute__((always_inline)) {
-        pa_u16x2 most = {0, 0};
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-            for (int e = 0; e < VW; e++) most = pa_larger(most, vr[k][e]);
-        const int bad = __any(pa_not_finite(most));
-        if (lane == 0) odd[which][wave] = bad;
-#pragma unroll
-        for (int d = 0; d < VD; d++) {
-            const unsigned pick = d & 1 ? 0x07060302u : 0x05040100u;
-            *reinterpret_cast<u32x2 *>(buf[which] + v_to + (d % DT) * 4096 + (d / DT) * 16) =
-                u32x2{__builtin_amdgcn_perm(vr[1][d / 2], vr[0][d / 2], pick), __builtin_amdgcn_perm(vr[3][d / 2], vr[2][d / 2], pick)};
-        }
+        for (int i = 0; i < DT; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void *)(to + wave * 16 * ROW + i * 1024), 16, from[i], 0, 0, 0);
     };
     float m = -3.402823466e38f, l = 0.f;
     pa_f32x16 o[DT];
 #pragma unroll
     for (int i = 0; i < DT; i++) o[i] = pa_f32x16{};
-    load(buf[0]);
-    put(0);
-    __builtin_amdgcn_s_waitcnt(0x0f70);                  /* K has arrived */
-    __syncthreads();
-#pragma unroll 1
-    for (int t = 0; t < tiles; t++) {
-        const unsigned char *b = buf[t & 1];
-        const int first = base + PAGED_MANY_ROWS * t;
-        at = pa_place(table, first + PAGED_MANY_ROWS + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW);
-        if (t + 1 < tiles) load(buf[(t + 1) & 1]);
-#pragma unroll 1
-        for (int sub = 0; sub < 2; sub += SUB) {
-            const int from = first + 32 * sub;
-            if (from >= any_hi || from + 32 * SUB <= any_lo) continue;               /* nobody of this wave sees these rows */
-            pa_f32x16 s[SUB];
+    /* addresses in LDS: one for all of K's pieces and one for all of V's, which differ from them in bits of their own.  (Through an empty asm in each unit: else each piece's, for each
+     * buffer, is kept in a register.) */
+    const int k_base = n * ROW + (g ^ (n & SWAP)) * 16, r4 = (n & 15) >> 2;
+    const int v_base = (4 * g + r4) * ROW + (v_swap(r4) + 2 * (n >> 4) + ((n & 3) >> 1)) * 16 + (n & 1) * 8;
+    auto read_k = [&](const unsigned char *kb, int half, int ks, int from) __attribute__((always_inline)) {
+        return pa_operand(*reinterpret_cast<const u32x4 *>(kb + 32 * half * ROW + (from ^ (32 * ks))));
+    };
+    /* values 32 i + n of rows 16 st + 8 (j / 4) + 4 g + j % 4 */
+    auto read_v = [&](const unsigned char *vb, int st, int i, int from) __attribute__((always_inline)) {
+        const unsigned char *p = vb + 16 * st * ROW + (from ^ (64 * i));
+        const pa_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4 *)p);
+        const pa_s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4 *)(p + 8 * ROW));
+        return __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto visible = [&](int u) { const int from = base + 32 * u; return from < any_hi && from + 32 > any_lo; };
+    auto hidden = [&](int u) { const int from = base + 32 * u; return from < all_lo || from + 32 > all_hi; };          /* from some column */
+    auto sees = [&](int u, int v) { const int key = base + 32 * u + 8 * (v >> 2) + 4 * g + (v & 3); return key >= see_lo && key < see_hi; };
+    auto hide = [&](int u, pa_f32x16 &s) __attribute__((always_inline)) {
+        if (hidden(u)) {
 #pragma unroll
-            for (int kt = 0; kt < SUB; kt++) {
-                const int row = 32 * (sub + kt) + n;
-                s[kt] = pa_f32x16{};
+            for (int v = 0; v < 16; v++) s[v] = sees(u, v) ? s[v] : -INFINITY;
+        }
+    };
+    auto follow = [&](float top) __attribute__((always_inline)) {         /* the running maximum; a NaN stays one: who sees it answers NaN */
+        { const f32x2 r = vt_swap32(top, top); top = __builtin_elementwise_maximum(r.x, r.y); }
+        if constexpr (!F32) top = top * a.scale;
+        if (__any(!(top <= m + PA_SLACK))) {
+            top = __builtin_elementwise_maximum(top, m);
+            const float less = pa_exp2(m - top);
+            l *= less;
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    const u32x4 k = *reinterpret_cast<const u32x4 *>(b + row * ROW + ((2 * ks + g) ^ (row & SWAP)) * 16);
+            for (int i = 0; i < DT; i++) o[i] = o[i] * less;
+            m = top;
+        }
+    };
+    /* Where rows of a V tile are hidden from some column, values that are not finite become 0, and are remembered.  All waves come here or none. */
+    int edges = 0;                                       /* tiles that were looked at: the first ones up to the rows that all columns see, and the last ones */
+    auto look = [&](int t, unsigned char *vb) __attribute__((always_inline)) {
+        if ((base + 64 * t >= wg_lo && base + 64 * t + 64 <= wg_hi) || edges == EDGES) return;
+        pa_u16x2 most = {0, 0};
+        unsigned char *mine = vb + 16 * wave * ROW;
 #pragma unroll
-                    for (int p = NQ - 1; p >= 0; p--) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa_operand(k), pa_operand(q[ks][p]), s[kt], 0, 0, 0);
-                }
-                if constexpr (!F32) s[kt] = s[kt] * a.scale;
-            }
-            auto sees = [&](int kt, int v) { const int key = from + 32 * kt + 8 * (v >> 2) + 4 * g + (v & 3); return key >= see_lo && key < see_hi; };
-            bool bad = false;
-            if (from < all_lo || from + 32 * SUB > all_hi) {
+        for (int i = 0; i < DT; i++) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(mine + (i * 64 + lane) * 16);
 #pragma unroll
-                for (int kt = 0; kt < SUB; kt++)
+            for (int e = 0; e < 4; e++) most = pa_larger(most, w[e]);
+        }
+        const int bad = __any(pa_not_finite(most));
+        if (lane == 0) odd[edges][wave] = bad;
+        if (bad) {                                       /* rare; what it derives from the lane is not kept in registers for it */
+            int own = lane;
+            asm volatile("" : "+v"(own));
 #pragma unroll
-                    for (int v = 0; v < 16; v++) s[kt][v] = sees(kt, v) ? s[kt][v] : -INFINITY;
-                bad = __any(odd[t & 1][lane & 3]);
-            }
-            float top = m;                                /* a NaN stays one: who sees it answers NaN */
-#pragma unroll
-            for (int kt = 0; kt < SUB; kt++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) top = __builtin_elementwise_maximum(top, s[kt][v]);
-            { const f32x2 r = vt_swap32(top, top); top = __builtin_elementwise_maximum(r.x, r.y); }
-            if (__any(top != m)) {
-                const float less = pa_exp2(m - top);
-                l *= less;
-#pragma unroll
-                for (int i = 0; i < DT; i++) o[i] = o[i] * less;
-                m = top;
-            }
-            if (bad) {                                   /* rare */
-#pragma unroll 1
-                for (int st = 0; st < 2 * SUB; st++) {
-                    u32x4 ones;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) ones[e] = (sees(st >> 1, 8 * (st & 1) + 2 * e) ? 0x3f80u : 0u) | (sees(st >> 1, 8 * (st & 1) + 2 * e + 1) ? 0x3f800000u : 0u);
-#pragma unroll
-                    for (int i = 0; i < DT; i++) {
-                        u32x4 v4 = *reinterpret_cast<const u32x4 *>(b + KB + ((i * 4 + 2 * sub + st) * 64 + lane) * 16);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) v4[e] = pa_marks(v4[e]);
-                        const pa_f32x16 hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa_operand(v4), pa_operand(ones), pa_f32x16{}, 0, 0, 0);
-#pragma unroll
-                        for (int v = 0; v < 16; v++) o[i][v] = hit[v] > 0.f ? NAN : o[i][v];
-                    }
-                }
-            }
-#pragma unroll
-            for (int st = 0; st < 2 * SUB; st++) {       /* 16 rows a step: elements 8 (st % 2) .. of scores st / 2 */
-                u32x4 w4[NP];
+            for (int i = 0; i < DT; i++) {
+                const int u = i * 64 + own, r = u / PIECES, piece = (u - r * PIECES) ^ v_swap(r);
+                u32x4 w = *reinterpret_cast<const u32x4 *>(mine + u * 16);
+                unsigned bits = 0;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float p0 = pa_exp2(s[st >> 1][8 * (st & 1) + 2 * e] - m), p1 = pa_exp2(s[st >> 1][8 * (st & 1) + 2 * e + 1] - m);
-                    l += p0 + p1;
-                    unsigned w[NP];
-                    pa_planes2<NP>(p0, p1, w);
-#pragma unroll
-                    for (int p = 0; p < NP; p++) w4[p][e] = w[p];
+                    const unsigned x = pa_marks(w[e]);
+                    bits |= (x & 0x3f80u ? 1u : 0u) << (2 * e) | (x & 0x3f800000u ? 2u : 0u) << (2 * e);
+                    w[e] = pa_finite(w[e]);
                 }
-#pragma unroll
-                for (int i = 0; i < DT; i++) {
-                    u32x4 v4 = *reinterpret_cast<const u32x4 *>(b + KB + ((i * 4 + 2 * sub + st) * 64 + lane) * 16);
-                    if (bad) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) v4[e] = pa_finite(v4[e]);
-                    }
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; p--) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa_operand(v4), pa_operand(w4[p]), o[i], 0, 0, 0);
-                }
+                *reinterpret_cast<u32x4 *>(mine + u * 16) = w;
+                reinterpret_cast<unsigned char *>(&marks[edges][16 * wave + r][0])[piece] = (unsigned char)bits;
             }
         }
-        if (t + 1 < tiles) {
-            put((t + 1) & 1);
-            __builtin_amdgcn_s_waitcnt(0x0f70);
-        }
         __syncthreads();
+        edges++;
+    };
+    /* pairs of weights that are made beside the scores; the others beside the first products with values.  An instruction takes the matrix cores 32 cycles, a pair 50 (fp32, with
+     * three times the instructions: 90) of the vector unit. */
+    constexpr int EARLY = F32 ? 8 : HP == 1 ? 6 : 5, AHEAD = F32 ? 1 : 3;        /* operands that are asked for ahead of their instruction */
+    auto unit = [&](int u, const unsigned char *kb, int khalf, pa_f32x16 &next, pa_f32x16 &s, const unsigned char *vb, int vhalf) __attribute__((always_inline)) {
+        if (!visible(u)) {
+            if (!visible(u + 1)) return;
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[v] = -INFINITY;
+        }
+        int k_from = k_base, v_from = v_base;
+        asm volatile("" : "+v"(k_from), "+v"(v_from));
+        u32x4 w4[2][NP];
+        auto weigh = [&](int e) __attribute__((always_inline)) {
+            const float p0 = pa_weight<F32>(s[2 * e], m, a.scale), p1 = pa_weight<F32>(s[2 * e + 1], m, a.scale);
+            l += p0 + p1;
+            unsigned w[NP];
+            pa_planes2<NP>(p0, p1, w);
+#pragma unroll
+            for (int p = 0; p < NP; p++) w4[e >> 2][p][e & 3] = w[p];
+        };
+        next = pa_f32x16{};
+        pa_bf16x8 k[KS];
+        u32x4 v[2 * DT];
+#pragma unroll
+        for (int ks = 0; ks < AHEAD; ks++) k[ks] = read_k(kb, khalf, ks, k_from);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int then = ks + AHEAD;
+            if (then < KS) k[then] = read_k(kb, khalf, then, k_from);
+            else v[then - KS] = read_v(vb, 2 * vhalf + (then - KS) / DT, (then - KS) % DT, v_from);
+#pragma unroll
+            for (int p = NQ - 1; p >= 0; p--) next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[ks], pa_operand(q[ks][p]), next, 0, 0, 0);
+#pragma unroll
+            for (int e = EARLY * ks / KS; e < EARLY * (ks + 1) / KS; e++) weigh(e);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        hide(u + 1, next);
+        float top = next[0];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < 2 * DT; x++) {               /* 16 rows a step: elements 8 st .. of the scores */
+            const int st = x / DT, i = x % DT;
+            const int then = x + AHEAD;
+            if (then < 2 * DT) v[then] = read_v(vb, 2 * vhalf + then / DT, then % DT, v_from);
+#pragma unroll
+            for (int p = NP - 1; p >= 0; p--) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pa_operand(v[x]), pa_operand(w4[st][p]), o[i], 0, 0, 0);
+            if (st == 0) {
+#pragma unroll
+                for (int e = EARLY + (8 - EARLY) * i / DT; e < EARLY + (8 - EARLY) * (i + 1) / DT; e++) weigh(e);
+            } else {
+#pragma unroll
+                for (int e = 16 * i / DT; e < 16 * (i + 1) / DT; e += 2) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, next[e]), next[e + 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        follow(top);
+    };
+    pa_f32x16 sa, sb;
+    load(a.K, place(base - 32), k_at, k1);
+    load(a.V, place(base), v_at, v0);
+    load(a.K, place(base + 32), k_at, k0);
+    pa_rows next_k = place(base + 96), next_v = place(base + 64);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    if (visible(0)) {                                    /* the first unit's scores */
+        sa = pa_f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const pa_bf16x8 k = read_k(k1, 1, ks, k_base);
+#pragma unroll
+            for (int p = NQ - 1; p >= 0; p--) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, pa_operand(q[ks][p]), sa, 0, 0, 0);
+        }
+        hide(0, sa);
+        float top = sa[0];
+#pragma unroll
+        for (int v = 1; v < 16; v++) top = __builtin_elementwise_maximum(top, sa[v]);
+        follow(top);
+    }
+    __syncthreads();
+    auto step = [&](int t, const unsigned char *kb, unsigned char *vb, unsigned char *k_to, unsigned char *v_to) __attribute__((always_inline)) {
+        const pa_rows here_k = next_k, here_v = next_v;
+        next_k = place(base + 64 * t + 160);
+        next_v = place(base + 64 * t + 128);
+        if (t + 1 < tiles) {
+            load(a.K, here_k, k_at, k_to);
+            load(a.V, here_v, v_at, v_to);
+        }
+        look(t, vb);
+        unit(2 * t, kb, 0, sb, sa, vb, 0);
+        unit(2 * t + 1, kb, 1, sa, sb, vb, 1);
+        __builtin_amdgcn_s_waitcnt(0x0f70);              /* the next tiles have arrived */
+        __syncthreads();
+    };
+#pragma unroll 1
+    for (int t = 0; t < tiles; t += 2) {
+        step(t, k0, v0, k1, v1);
+        if (t + 1 >= tiles) break;
+        step(t + 1, k1, v1, k0, v0);
     }
     { const f32x2 r = vt_swap32(l, l); l = r.x + r.y; }
     {
         const float f = l == 0.f && it.parts > 1 ? 0.f : 1.f / l;
 #pragma unroll
         for (int i = 0; i < DT; i++) o[i] = o[i] * f;
+    }
+    /* results of who sees a value that is not finite */
+#pragma unroll 1
+    for (int x = 0, t = 0; x < edges; x++, t++) {
+        while (base + 64 * t >= wg_lo && base + 64 * t + 64 <= wg_hi) t++;         /* the x-th tile that was looked at */
+#pragma unroll 1
+        for (int r = 0; r < 64; r++) {
+            if (!odd[x][r / 16]) { r += 15; continue; }
+            const int key = base + 64 * t + r;
+            const bool see = key >= see_lo && key < see_hi;
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                const unsigned w = see ? marks[x][r][i] >> (4 * g) : 0u;
+                if (__any(w)) {
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[i][v] = w >> (8 * (v >> 2) + (v & 3)) & 1u ? NAN : o[i][v];
+                }
+            }
+        }
     }
     if (it.parts > 1) {
         /* a part lies as the lanes hold it: [part][wave][4 DT vectors of four, then largest score and sum of weights][lane] */
@@ -544,21 +638,13 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
                 for (int e = 0; e < 4; e++) o[x / 4][4 * (x % 4) + e] = fmaf(p[x][e], w, o[x / 4][4 * (x % 4) + e]);
         }
     }
-    /* element v of lane l is value DT (8 (v / 4) + 4 (l / 32) + v % 4) + i */
+    /* element v of lane l in o[i] is value 32 i + 8 (v / 4) + 4 (l / 32) + v % 4 */
     if (n < wc) {
         const size_t to = ((size_t)(it.row + qi) * a.n_heads + head_at) * HD;
 #pragma unroll
-        for (int v = 0; v < 16; v++)
+        for (int i = 0; i < DT; i++)
 #pragma unroll
-            for (int i = 0; i < DT; i += 2) {
-                const size_t x = to + DT * (8 * (v >> 2) + 4 * g + (v & 3)) + i;
-                if constexpr (F32) *reinterpret_cast<f32x2 *>((float *)a.out + x) = f32x2{o[i][v], o[i + 1][v]};
-                else {
-                    unsigned w[1];
-                    pa_planes2<1>(o[i][v], o[i + 1][v], w);
-                    *reinterpret_cast<unsigned *>((uint16_t *)a.out + x) = w[0];
-                }
-            }
+            for (int v = 0; v < 16; v += 4) pa_store4<F32>(a.out, to + 32 * i + 2 * v + 4 * g, f32x4{o[i][v], o[i][v + 1], o[i][v + 2], o[i][v + 3]});
     }
 }
 
