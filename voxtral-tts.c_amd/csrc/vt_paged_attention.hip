@@ -104,10 +104,13 @@ static __device__ __forceinline__ vt_paged_item pa_item(const vt_paged_item *ite
 
 /* 16 rows from `at` on, a multiple of 16, of those lo .. end - 1: where they lie, and the bytes of them that are there */
 struct pa_rows { size_t row; int bytes; };
-static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, int at, int lo, int end, int page_log, int heads, int head, int row_bytes) {
-    const int seen = min(at, end - 1), n = at + 16 > lo ? min(max(end - at, 0), 16) : 0;
-    const int page = table[max(seen, lo) >> page_log];
+static __device__ __forceinline__ int pa_entry(int at, int lo, int end, int page_log) { return max(min(at, end - 1), lo) >> page_log; }
+static __device__ __forceinline__ pa_rows pa_rows_of(int page, int at, int lo, int end, int page_log, int heads, int head, int row_bytes) {
+    const int n = at + 16 > lo ? min(max(end - at, 0), 16) : 0;
     return pa_rows{((((size_t)(unsigned)page * heads + head) << page_log) + (at & ((1 << page_log) - 1))), n * row_bytes};
+}
+static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, int at, int lo, int end, int page_log, int heads, int head, int row_bytes) {
+    return pa_rows_of(table[pa_entry(at, lo, end, page_log)], at, lo, end, page_log, heads, head, row_bytes);
 }
 
 /* ---- few columns -------------------------------------------------------------------------------------------------
@@ -389,7 +392,19 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
         k_at[d] = r * ROW + ((u - r * PIECES) ^ (r & SWAP)) * 16;
         v_at[d] = r * ROW + ((u - r * PIECES) ^ v_swap(r)) * 16;
     }
-    auto place = [&](int from) __attribute__((always_inline)) { return pa_place(table, from + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW); };
+    /* The wave's pages of the next 64 tiles, a lane each: scalar loads on their way would turn every wait for LDS into one for all of LDS and for them. */
+    int k_page, v_page;
+    auto pages = [&](int t) __attribute__((always_inline)) {
+        const int own = base + 64 * (t + lane) + 16 * wave;
+        k_page = table[pa_entry(own + 32, it.lo, it.end, a.page_log)];
+        v_page = table[pa_entry(own, it.lo, it.end, a.page_log)];
+    };
+    auto k_place = [&](int t) __attribute__((always_inline)) {
+        return pa_rows_of(__builtin_amdgcn_readlane(k_page, t & 63), base + 64 * t + 32 + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW);
+    };
+    auto v_place = [&](int t) __attribute__((always_inline)) {
+        return pa_rows_of(__builtin_amdgcn_readlane(v_page, t & 63), base + 64 * t + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW);
+    };
     auto load = [&](const uint16_t *pool, const pa_rows &at, const int (&from)[4], unsigned char *to) __attribute__((always_inline)) {
         const __amdgpu_buffer_rsrc_t d = vt_buffer(pool + at.row * HD, at.bytes);
 #pragma unroll
@@ -472,12 +487,15 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     };
     /* pairs of weights that are made beside the scores; the others beside the first products with values.  An instruction takes the matrix cores 32 cycles, a pair 50 (fp32, with
      * three times the instructions: 90) of the vector unit. */
-    constexpr int EARLY = F32 ? 8 : HP == 1 ? 6 : 5, AHEAD = F32 ? 1 : 3;        /* operands that are asked for ahead of their instruction */
+    constexpr int EARLY = F32 ? 8 : HP == 1 ? 6 : 5, AHEAD = F32 ? 1 : 3, BEFORE = F32 ? 1 : 2;
+    /* (AHEAD: operands that are asked for ahead of their instruction; BEFORE: those in front of what depends on the maximum) */
+    float top = -INFINITY;                               /* the largest score of the unit at hand, in a lane's rows */
     auto unit = [&](int u, const unsigned char *kb, int khalf, pa_f32x16 &next, pa_f32x16 &s, const unsigned char *vb, int vhalf) __attribute__((always_inline)) {
         if (!visible(u)) {
             if (!visible(u + 1)) return;
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = -INFINITY;
+            top = -INFINITY;
         }
         int k_from = k_base, v_from = v_base;
         asm volatile("" : "+v"(k_from), "+v"(v_from));
@@ -503,12 +521,15 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
             else v[then - KS] = read_v(vb, 2 * vhalf + (then - KS) / DT, (then - KS) % DT, v_from);
 #pragma unroll
             for (int p = NQ - 1; p >= 0; p--) next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[ks], pa_operand(q[ks][p]), next, 0, 0, 0);
+            if (ks == BEFORE - 1) follow(top);
+            if (ks >= BEFORE) {
 #pragma unroll
-            for (int e = EARLY * ks / KS; e < EARLY * (ks + 1) / KS; e++) weigh(e);
+                for (int e = EARLY * (ks - BEFORE) / (KS - BEFORE); e < EARLY * (ks - BEFORE + 1) / (KS - BEFORE); e++) weigh(e);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
         hide(u + 1, next);
-        float top = next[0];
+        top = next[0];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < 2 * DT; x++) {               /* 16 rows a step: elements 8 st .. of the scores */
@@ -526,13 +547,12 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        follow(top);
     };
     pa_f32x16 sa, sb;
-    load(a.K, place(base - 32), k_at, k1);
-    load(a.V, place(base), v_at, v0);
-    load(a.K, place(base + 32), k_at, k0);
-    pa_rows next_k = place(base + 96), next_v = place(base + 64);
+    pages(0);
+    load(a.K, pa_place(table, base - 32 + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW), k_at, k1);
+    load(a.V, v_place(0), v_at, v0);
+    load(a.K, k_place(0), k_at, k0);
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
     if (visible(0)) {                                    /* the first unit's scores */
@@ -544,19 +564,15 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
             for (int p = NQ - 1; p >= 0; p--) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, pa_operand(q[ks][p]), sa, 0, 0, 0);
         }
         hide(0, sa);
-        float top = sa[0];
 #pragma unroll
-        for (int v = 1; v < 16; v++) top = __builtin_elementwise_maximum(top, sa[v]);
-        follow(top);
+        for (int v = 0; v < 16; v++) top = __builtin_elementwise_maximum(top, sa[v]);
     }
     __syncthreads();
     auto step = [&](int t, const unsigned char *kb, unsigned char *vb, unsigned char *k_to, unsigned char *v_to) __attribute__((always_inline)) {
-        const pa_rows here_k = next_k, here_v = next_v;
-        next_k = place(base + 64 * t + 160);
-        next_v = place(base + 64 * t + 128);
         if (t + 1 < tiles) {
-            load(a.K, here_k, k_at, k_to);
-            load(a.V, here_v, v_at, v_to);
+            if (((t + 1) & 63) == 0) pages(t + 1);
+            load(a.K, k_place(t + 1), k_at, k_to);
+            load(a.V, v_place(t + 1), v_at, v_to);
         }
         look(t, vb);
         unit(2 * t, kb, 0, sb, sa, vb, 0);
