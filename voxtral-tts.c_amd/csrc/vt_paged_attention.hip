@@ -51,12 +51,19 @@ static __device__ __forceinline__ void pa_planes2(float a, float b, unsigned (&w
     }
 }
 
-/* 8 values of a query -> operands, one for each plane.  fp32 ones are scaled first; bf16 ones are the operand, and their scores are scaled. */
-template <bool F32, int NQ>
-static __device__ __forceinline__ void pa_query(const void *Q, size_t at, float scale, u32x4 (&to)[NQ]) {
+/* 8 values of a query as they lie, and as operands, one for each plane.  fp32 ones are scaled first; bf16 ones are the operand, and their scores are scaled. */
+template <bool F32>
+static __device__ __forceinline__ void pa_query_load(const void *Q, size_t at, u32x4 (&raw)[2]) {
     if constexpr (F32) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>((const float *)Q + at);
-        const f32x4 a = p[0] * scale, b = p[1] * scale;
+        const u32x4 *p = reinterpret_cast<const u32x4 *>((const float *)Q + at);
+        raw[0] = p[0];
+        raw[1] = p[1];
+    } else raw[0] = *reinterpret_cast<const u32x4 *>((const uint16_t *)Q + at);
+}
+template <bool F32, int NQ>
+static __device__ __forceinline__ void pa_query_planes(const u32x4 (&raw)[2], float scale, u32x4 (&to)[NQ]) {
+    if constexpr (F32) {
+        const f32x4 a = __builtin_bit_cast(f32x4, raw[0]) * scale, b = __builtin_bit_cast(f32x4, raw[1]) * scale;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             unsigned w[NQ];
@@ -64,7 +71,7 @@ static __device__ __forceinline__ void pa_query(const void *Q, size_t at, float 
 #pragma unroll
             for (int k = 0; k < NQ; k++) to[k][e] = w[k];
         }
-    } else to[0] = *reinterpret_cast<const u32x4 *>((const uint16_t *)Q + at);
+    } else to[0] = raw[0];
 }
 
 template <bool F32>
@@ -114,32 +121,25 @@ static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, in
 }
 
 /* ---- few columns -------------------------------------------------------------------------------------------------
- * A wave has 32 rows of K and V in registers at a time, asks for the next as soon as these are used, and waits for nobody; the waves of a workgroup, and then the
- * workgroups that share the columns' rows, add their parts in a fixed order, the last workgroup to arrive those of all.  K is the A operand of 16 x 16 x 32, a lane's 16
+ * A wave has 32 rows of K and V in registers at a time, asks for the next as soon as these are used, and waits for nobody; the waves of a workgroup,
+ * and then the workgroups that share the columns' rows, add their parts in a fixed order, the last workgroup to arrive those of all.  K is the A operand of 16 x 16 x 32, a lane's 16
  * bytes from its own row.  V's rows are its columns: a lane loads CD values each of the eight rows that it has weights of, 16 lanes a whole row, and pairs of rows are
- * put together two values at a time. */
-template <int HP, bool F32>
+ * put together two values at a time.  Queries, the same for all waves, wait in LDS as operands.  ONCE: no other workgroup reads these rows, and there are more than a cache holds. */
+template <int HP, bool F32, bool ONCE>
 __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(pa_job a) {
     constexpr int HD = 64 * HP, ROW = 2 * HD, KS = 2 * HP, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4, WAVES = PAGED_FEW_WAVES;
-    constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 2, COLS = PAGED_FEW_COLS;
-    __shared__ __attribute__((aligned(16))) float area[WAVES][COLS][OD];
+    constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 2, COLS = PAGED_FEW_COLS, HOW = ONCE ? 2 /* nt */ : 0;
+    __shared__ __attribute__((aligned(16))) float area[WAVES][COLS][OD];                /* the queries' operands, then the waves' parts */
     __shared__ float ml[WAVES][COLS][2], wt[COLS][PAGED_MAX_PARTS];
     __shared__ int last;
+    static_assert(sizeof area >= KS * NQ * 1024, "operands");
+    u32x4 *queries = reinterpret_cast<u32x4 *>(area);
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4, h = (int)blockIdx.x, heads = (int)gridDim.x;
     const vt_paged_item it = pa_item(a.items);
-    const int nc = min(COLS, it.cols - it.c0);
     const pa_const_int *table = (const pa_const_int *)(uintptr_t)(a.tables + it.table);
-    const int cc = min(it.c0 + n, it.cols - 1), qi = vt_div(cc, a.group), pos = it.past + qi;
-    const int see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_hi = pos + 1;
-    const int q_first = it.past + vt_div(it.c0, a.group), q_last = it.past + vt_div(it.c0 + nc - 1, a.group);
-    const int all_lo = a.window && q_last >= a.window ? q_last - a.window + 1 : 0, all_hi = q_first + 1;       /* rows that every column sees */
     const int base = it.lo & ~(PAGED_FEW_ROWS - 1), tiles = (it.end - base + PAGED_FEW_ROWS - 1) / PAGED_FEW_ROWS;
-    const size_t head_at = (size_t)h * a.group.d + (cc - qi * a.group.d);
-    u32x4 q[KS][NQ];
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) pa_query<F32, NQ>(a.Q, (size_t)(it.row + qi) * a.q_stride + head_at * HD + 32 * ks + 8 * g, a.scale, q[ks]);
-    u32x4 kr[2][KS];
-    u32x4 vr[8][CHUNKS];                                 /* CD == 4: the first half of each */
+    u32x4 k[2][KS];
+    u32x4 v[8][CHUNKS];                                  /* CD == 4: the first half of each */
     pa_rows at[2];
     auto place = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
         for (int kt = 0; kt < 2; kt++) {
             const __amdgpu_buffer_rsrc_t d = vt_buffer(a.K + at[kt].row * HD, at[kt].bytes);
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) kr[kt][ks] = __builtin_amdgcn_raw_buffer_load_b128(d, n * ROW + 64 * ks + 16 * g, 0, 0);
+            for (int ks = 0; ks < KS; ks++) k[kt][ks] = __builtin_amdgcn_raw_buffer_load_b128(d, n * ROW + 64 * ks + 16 * g, 0, HOW);
         }
     };
     auto ask_v = [&]() __attribute__((always_inline)) {
@@ -161,38 +161,61 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int ch = 0; ch < CHUNKS; ch++) {
-                    const int from = (4 * g + j) * ROW + ch * 32 * CD + n * 2 * CD;
-                    if constexpr (CD == 8) vr[4 * kt + j][ch] = __builtin_amdgcn_raw_buffer_load_b128(d, from, 0, 0);
+                    const int in = (4 * g + j) * ROW + ch * 32 * CD + n * 2 * CD;
+                    if constexpr (CD == 8) v[4 * kt + j][ch] = __builtin_amdgcn_raw_buffer_load_b128(d, in, 0, HOW);
                     else {
-                        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(d, from, 0, 0);
-                        vr[4 * kt + j][ch] = u32x4{w.x, w.y, 0u, 0u};
+                        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(d, in, 0, HOW);
+                        v[4 * kt + j][ch] = u32x4{w.x, w.y, 0u, 0u};
                     }
                 }
         }
     };
+    const int nc = min(COLS, it.cols - it.c0), cc = min(it.c0 + n, it.cols - 1), qi = vt_div(cc, a.group), pos = it.past + qi;
+    const size_t head_at = (size_t)h * a.group.d + (cc - qi * a.group.d);
+    /* queries first: loads return in order */
+    constexpr int MINE = (KS + WAVES - 1) / WAVES;       /* steps of the product that a wave brings the queries' operands of */
+    u32x4 raw[MINE][2];
+#pragma unroll
+    for (int x = 0; x < MINE; x++)
+        pa_query_load<F32>(a.Q, (size_t)(it.row + qi) * a.q_stride + head_at * HD + 32 * min(wave + WAVES * x, KS - 1) + 8 * g, raw[x]);
     place(wave);
     ask_k();
     ask_v();
+#pragma unroll
+    for (int x = 0; x < MINE; x++) {
+        const int ks = wave + WAVES * x;
+        if (KS % WAVES && ks >= KS) break;
+        u32x4 q[NQ];
+        pa_query_planes<F32, NQ>(raw[x], a.scale, q);
+#pragma unroll
+        for (int p = 0; p < NQ; p++) queries[(ks * NQ + p) * 64 + lane] = q[p];
+    }
+    const int see_lo = max(a.window && pos >= a.window ? pos - a.window + 1 : 0, it.lo), see_hi = min(pos + 1, it.end);
+    const int q_first = it.past + vt_div(it.c0, a.group), q_last = it.past + vt_div(it.c0 + nc - 1, a.group);
+    const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);       /* rows that every column sees */
     float m = -3.402823466e38f, l = 0.f;                 /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
     f32x4 o[CHUNKS * CD];
 #pragma unroll
     for (int i = 0; i < CHUNKS * CD; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
 #pragma unroll 1
     for (int t = wave; t < tiles; t += WAVES) {
         const int first = base + PAGED_FEW_ROWS * t;
-        const bool hidden = first < all_lo || first + PAGED_FEW_ROWS > all_hi || first < it.lo || first + PAGED_FEW_ROWS > it.end;
+        const bool hidden = first < all_lo || first + PAGED_FEW_ROWS > all_hi;
         place(t + WAVES);
-        f32x4 s[2];
+        int own = lane;                                  /* (through an empty asm: else the queries are kept in registers after all) */
+        asm volatile("" : "+v"(own));
+        f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-            s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int p = NQ - 1; p >= 0; p--)
+            for (int p = NQ - 1; p >= 0; p--) {
+                const pa_bf16x8 q = pa_operand(queries[(ks * NQ + p) * 64 + own]);
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(kr[kt][ks]), pa_operand(q[ks][p]), s[kt], 0, 0, 0);
-        }
+                for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(k[kt][ks]), q, s[kt], 0, 0, 0);
+            }
         ask_k();
-        auto sees = [&](int kt, int v) { const int key = first + 16 * kt + 4 * g + v; return key >= max(see_lo, it.lo) && key < min(see_hi, it.end); };
+        auto sees = [&](int kt, int v) { const int key = first + 16 * kt + 4 * g + v; return key >= see_lo && key < see_hi; };
         bool bad = false;
         if (hidden) {
 #pragma unroll
@@ -205,7 +228,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
 #pragma unroll
                 for (int ch = 0; ch < CHUNKS; ch++)
 #pragma unroll
-                    for (int e = 0; e < CD / 2; e++) most = pa_larger(most, vr[j][ch][e]);
+                    for (int e = 0; e < CD / 2; e++) most = pa_larger(most, v[j][ch][e]);
             bad = __any(pa_not_finite(most));
         }
         float top = __builtin_elementwise_maximum(s[0][0], s[1][0]);                /* a NaN stays one: who sees it answers NaN */
@@ -246,17 +269,17 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
                 for (int i = 0; i < CD; i++) {
                     u32x4 v4;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v4[e] = pa_marks(__builtin_amdgcn_perm(vr[2 * e + 1][ch][i / 2], vr[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u));
+                    for (int e = 0; e < 4; e++) v4[e] = pa_marks(__builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u));
                     const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(ones), (f32x4{0.f, 0.f, 0.f, 0.f}), 0, 0, 0);
 #pragma unroll
-                    for (int v = 0; v < 4; v++) o[ch * CD + i][v] = hit[v] > 0.f ? NAN : o[ch * CD + i][v];
+                    for (int e = 0; e < 4; e++) o[ch * CD + i][e] = hit[e] > 0.f ? NAN : o[ch * CD + i][e];
                 }
 #pragma unroll
             for (int j = 0; j < 8; j++)
 #pragma unroll
                 for (int ch = 0; ch < CHUNKS; ch++)
 #pragma unroll
-                    for (int e = 0; e < CD / 2; e++) vr[j][ch][e] = pa_finite(vr[j][ch][e]);
+                    for (int e = 0; e < CD / 2; e++) v[j][ch][e] = pa_finite(v[j][ch][e]);
         }
 #pragma unroll
         for (int ch = 0; ch < CHUNKS; ch++)
@@ -264,7 +287,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
             for (int i = 0; i < CD; i++) {
                 u32x4 v4;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v4[e] = __builtin_amdgcn_perm(vr[2 * e + 1][ch][i / 2], vr[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                for (int e = 0; e < 4; e++) v4[e] = __builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
                 f32x4 &acc = o[ch * CD + i];
 #pragma unroll
                 for (int p = NP - 1; p >= 0; p--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[p]), acc, 0, 0, 0);
@@ -292,7 +315,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
                 for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * v + i] = o[ch * CD + i][v] * f;
     }
     __syncthreads();
-    float *part = a.part + (size_t)(it.slot * heads + h * it.parts) * COLS * OD;
+    const __amdgpu_buffer_rsrc_t pd = vt_buffer(a.part + (size_t)(it.slot * heads + h * it.parts) * COLS * OD, it.parts * COLS * OD * 4);
     auto result = [&](int col, int d, const f32x4 &v) {
         const int k = it.c0 + col, i = vt_div(k, a.group);
         const size_t to = ((size_t)(it.row + i) * a.n_heads + (size_t)h * a.group.d + (k - i * a.group.d)) * HD + d;
@@ -305,17 +328,11 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
         for (int k = 0; k < WAVES; k++) v = v + *reinterpret_cast<const f32x4 *>(&area[k][col][d]);
         if (it.parts == 1) result(col, d, v);
         else {
-            float *to = part + ((size_t)it.part * COLS + col) * OD + 4 + d;
-#pragma unroll
-            for (int i = 0; i < 4; i++) vt_stc(to + i, v[i]);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), pd, ((it.part * COLS + col) * OD + 4 + d) * 4, 0, 16 /* sc1 */);
         }
     }
     if (it.parts == 1) return;
-    if (wave == 0 && lane < nc) {
-        float *to = part + ((size_t)it.part * COLS + lane) * OD;
-        vt_stc(to, M);
-        vt_stc(to + 1, L);
-    }
+    if (wave == 0 && lane < nc) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, pd, (it.part * COLS + lane) * OD * 4, 0, 16);
     __builtin_amdgcn_s_waitcnt(0x0f70);                  /* the part's stores are acknowledged */
     __syncthreads();
     unsigned *cnt = a.cnt + it.counter * heads + h;
@@ -324,7 +341,6 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
     if (!last) return;
     if (threadIdx.x == 0) vt_stc_u32(cnt, 0u);           /* ready for the next launch */
     /* a wave per column: lane k has part k's largest score and sum of weights */
-    const __amdgpu_buffer_rsrc_t pd = vt_buffer(part, it.parts * COLS * OD * 4);
     for (int col = wave; col < nc; col += WAVES) {
         const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(pd, (min(lane, it.parts - 1) * COLS + col) * OD * 4, 0, 16 /* sc1 */);
         const float pm = __uint_as_float(v.x), pl = lane < it.parts ? __uint_as_float(v.y) : 0.f;
@@ -378,9 +394,9 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     const int wg_lo = max(a.window && wg_last >= a.window ? wg_last - a.window + 1 : 0, it.lo), wg_hi = min(it.past + vt_div(it.c0, a.group) + 1, it.end);         /* rows that every column sees */
     const int base = it.lo & ~(PAGED_MANY_ROWS - 1), tiles = (it.end - base + PAGED_MANY_ROWS - 1) / PAGED_MANY_ROWS;
     const size_t head_at = (size_t)h * a.group.d + (cc - qi * a.group.d);
-    u32x4 q[KS][NQ];
+    u32x4 raw[KS][2];
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) pa_query<F32, NQ>(a.Q, (size_t)(it.row + qi) * a.q_stride + head_at * HD + 16 * ks + 8 * g, a.scale, q[ks]);
+    for (int ks = 0; ks < KS; ks++) pa_query_load<F32>(a.Q, (size_t)(it.row + qi) * a.q_stride + head_at * HD + 16 * ks + 8 * g, raw[ks]);
     /* Pieces of 16 bytes change places within a row, so that what is read at once lies in different banks: K's with the row's last bits, so that 16 (8) rows' same piece do; V's fours of
      * them, so that four rows' same 64 bytes do. */
     constexpr int SWAP = PIECES - 1;
@@ -411,6 +427,13 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
         for (int i = 0; i < DT; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void *)(to + wave * 16 * ROW + i * 1024), 16, from[i], 0, 0, 0);
     };
+    pages(0);
+    load(a.K, pa_place(table, base - 32 + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW), k_at, k1);
+    load(a.V, v_place(0), v_at, v0);
+    load(a.K, k_place(0), k_at, k0);
+    u32x4 q[KS][NQ];                                     /* (made while the first tiles are on their way) */
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) pa_query_planes<F32, NQ>(raw[ks], a.scale, q[ks]);
     float m = -3.402823466e38f, l = 0.f;
     pa_f32x16 o[DT];
 #pragma unroll
@@ -549,10 +572,6 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
         }
     };
     pa_f32x16 sa, sb;
-    pages(0);
-    load(a.K, pa_place(table, base - 32 + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW), k_at, k1);
-    load(a.V, v_place(0), v_at, v0);
-    load(a.K, k_place(0), k_at, k0);
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
     if (visible(0)) {                                    /* the first unit's scores */
@@ -667,9 +686,11 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
 template <int HP>
 static void pa_launch(const pa_job &job, const vt_paged_plan &p, int heads, bool f32) {
     if (p.few) {
-        const dim3 grid((unsigned)heads, (unsigned)p.few);
-        if (f32) hipLaunchKernelGGL((vt_paged_few_kernel<HP, true>), grid, dim3(64 * PAGED_FEW_WAVES), 0, g_vt.stream, job);
-        else hipLaunchKernelGGL((vt_paged_few_kernel<HP, false>), grid, dim3(64 * PAGED_FEW_WAVES), 0, g_vt.stream, job);
+        const dim3 grid((unsigned)heads, (unsigned)p.few), threads(64 * PAGED_FEW_WAVES);
+        if (f32 && p.once) hipLaunchKernelGGL((vt_paged_few_kernel<HP, true, true>), grid, threads, 0, g_vt.stream, job);
+        else if (f32) hipLaunchKernelGGL((vt_paged_few_kernel<HP, true, false>), grid, threads, 0, g_vt.stream, job);
+        else if (p.once) hipLaunchKernelGGL((vt_paged_few_kernel<HP, false, true>), grid, threads, 0, g_vt.stream, job);
+        else hipLaunchKernelGGL((vt_paged_few_kernel<HP, false, false>), grid, threads, 0, g_vt.stream, job);
     }
     if constexpr (HP <= 2) {
         if (p.many) {
