@@ -128,20 +128,25 @@ class Cache:
             if r == 0:
                 continue
             kb, vb = self.sequence(i)
-            age = np.arange(p, p + r)[:, None] - np.arange(p + r)[None, :]
-            hidden = (age < 0) | (age >= self.window if self.window else False)
-            for h in range(self.heads):
-                k, v = value16(kb[h // group]).astype(np.float64), value16(vb[h // group]).astype(np.float64)
-                x = q[at:at + r, h].astype(np.float64)
-                with np.errstate(invalid="ignore"):
-                    w = np.where(hidden, -np.inf, x @ k.T * scale)
-                    w = np.exp(w - w.max(-1, keepdims=True))
-                    w = w / w.sum(-1, keepdims=True)
-                    clean = np.where(np.isfinite(v), v, 0)
-                    out[at:at + r, h] = w @ clean
-                    size[at:at + r, h] = w @ np.abs(clean)
-                    out[at:at + r, h][((~hidden).astype(float) @ (~np.isfinite(v))) > 0] = np.nan
-                most = max(most, float((np.abs(x) @ np.where(np.isfinite(k), np.abs(k), 0).T * scale).max()))
+            for h in range(self.kv_heads):
+                k, v = value16(kb[h]).astype(np.float64), value16(vb[h]).astype(np.float64)
+                clean, odd = np.where(np.isfinite(v), v, 0), ~np.isfinite(v)
+                for r0 in range(0, r, 256):                                        # queries r0 .., of all heads on this one, over what they see
+                    n = min(256, r - r0)
+                    lo, hi = max(0, p + r0 - self.window + 1 if self.window else 0), p + r0 + n
+                    age = np.arange(p + r0, hi)[:, None] - np.arange(lo, hi)[None, :]
+                    hidden = (age < 0) | (age >= self.window if self.window else False)
+                    to = (slice(at + r0, at + r0 + n), slice(h * group, (h + 1) * group))
+                    x = q[to].astype(np.float64).transpose(1, 0, 2)
+                    with np.errstate(invalid="ignore"):
+                        w = np.where(hidden, -np.inf, x @ k[lo:hi].T * scale)
+                        w = np.exp(w - w.max(-1, keepdims=True))
+                        w = w / w.sum(-1, keepdims=True)
+                        y = w @ clean[lo:hi]
+                        out[to], size[to] = y.transpose(1, 0, 2), (w @ np.abs(clean[lo:hi])).transpose(1, 0, 2)
+                        if odd[lo:hi].any():
+                            out[to][((~hidden).astype(float) @ odd[lo:hi] > 0)[:, None, :].repeat(group, 1)] = np.nan
+                    most = max(most, float((np.abs(x) @ np.where(np.isfinite(k[lo:hi]), np.abs(k[lo:hi]), 0).T * scale).max()))
             at += r
         return out, size, most
 
@@ -167,8 +172,12 @@ def attention(cache, q, bf16, scale, q_gap=0):
 
 
 def is_many(cache, i):
-    """The kernel that rounds a bf16 batch's weights to bf16 (vt_paged_is_many)."""
-    return cache.hd <= 128 and cache.rows[i] * cache.heads // cache.kv_heads > 64
+    """The kernel that rounds a bf16 batch's weights to bf16 (vt_paged_any_many)."""
+    group = cache.heads // cache.kv_heads
+    if cache.hd > 128:
+        return False
+    all_of_them = sum(r * group * min(p + r / 2, cache.window or math.inf) * cache.kv_heads * cache.hd for r, p in zip(cache.rows, cache.past) if r * group > 64)
+    return all_of_them >= 7e8 and cache.rows[i] * group > 64
 
 
 def check(cache, got, want, size, most, bf16):

@@ -161,9 +161,24 @@ def test_attention(hip, batch, page, window, layout, bf16):
     c.free()
 
 
+MANY = [  # layout, batch, page, window: enough for the kernel for many columns
+    ((32, 8, 128), "700@0 3@50", 16, 0), ((32, 8, 128), "130@500 1@700 64@64 0@9 600@300", 64, 0), ((32, 8, 128), "2000@0", 16, 90), ((32, 8, 128), "37@3000 100@2000", 32, 0),
+    ((16, 16, 64), "333@700 500@100 1@40 700@0", 256, 0), ((16, 16, 64), "65@6000 300@2000", 16, 0), ((8, 1, 128), "300@8000", 16, 0), ((8, 1, 128), "1500@100 17@800", 32, 500), ((8, 1, 128), "3000@33", 64, 260),
+    ((14, 2, 64), "1000@400", 1024, 0), ((20, 1, 64), "800@333 9@9", 16, 0)]
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("layout,batch,page,window", MANY)
+def test_attention_of_many_columns(hip, layout, batch, page, window, bf16):
+    test_attention(hip, batch, page, window, layout, bf16)
+    c = P.Cache(hip, batch, page, *layout, window=window)
+    assert any(P.is_many(c, i) for i in range(len(c.rows)))
+    c.free()
+
+
 @pytest.mark.parametrize("bf16", [0, 1])
 @pytest.mark.parametrize("layout", [(8, 2, 128), (6, 2, 192), (16, 2, 64)])
-@pytest.mark.parametrize("batch,window", [("40@100", 0), ("9@7", 0), ("40@100 1@200", 30), ("300@10", 40)])
+@pytest.mark.parametrize("batch,window", [("40@100", 0), ("9@7", 0), ("40@100 1@200", 30), ("300@10", 40), ("900@500", 0), ("2500@10", 300), ("1700@0 1@500", 130), ("8000@0", 100)])
 def test_what_a_query_does_not_see_changes_nothing(hip, batch, window, layout, bf16):
     """Infinities and NaN in keys and values: who sees a key's NaN answers NaN, who sees a value's in that value; nobody else notices.  Who sees a key's infinity answers NaN
     where its score is +infinity or no number, and may where it is -infinity, a weight of 0."""
@@ -200,7 +215,7 @@ def test_what_a_query_does_not_see_changes_nothing(hip, batch, window, layout, b
 
 
 @pytest.mark.parametrize("bf16", [0, 1])
-@pytest.mark.parametrize("batch", ["1@700", "100@300"])
+@pytest.mark.parametrize("batch", ["1@700", "100@300", "1000@300"])
 def test_scores_far_apart(hip, batch, bf16):
     """Scores of hundreds: a weight's error is that of its score, and the largest takes all."""
     c = P.Cache(hip, batch, 16, 8, 2, 128, seed=2)

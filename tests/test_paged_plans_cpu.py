@@ -67,7 +67,7 @@ int main(void) {
         }
         for (int i = 0; i < n_seqs; i++) {
             long long all = 0;
-            const bool many = vt_paged_is_many(lay[2] / 64, (long long)rows[i] * group);
+            const bool many = vt_paged_any_many(s, n_seqs, past.data(), rows.data()) && vt_paged_may_be_many(lay[2] / 64, (long long)rows[i] * group);
             const int cols = many ? PAGED_MANY_COLS : PAGED_FEW_COLS;
             for (int c = 0; c < rows[i] * group; c += cols) all++;
             if (got[i] != want[i] || (rows[i] && !got[i])) { bad++; printf("sequence %d of %d: %lld of %lld\n", i, n_seqs, got[i], want[i]); }

@@ -103,15 +103,31 @@ static inline long long vt_paged_max_items(int max_seqs, int max_rows, int group
     return (long long)max_rows * group / PAGED_FEW_COLS + max_seqs + 2 * PAGED_SPLIT_ITEMS;
 }
 
-static inline bool vt_paged_is_many(int hp, long long cols) { return hp <= 2 && cols > 900; }
+/* Which sequences go to the kernel for many columns: those of more than 64 whose heads of up to 128 values leave it registers, where there is enough for it to do, as columns times
+ * the rows that they see on average times kv heads times values.  A workgroup of it does twice as much for what it reads, but there are few of them.  Measured, us with the kernel
+ * for few columns and for many (fp32 / bf16), 32 heads on 8 of 128: 300 rows behind none (0.18e9) 11 / 10 and 17 / 13, 37 behind 4000 (0.61e9) 21 / 21 and 34 / 26, 450 behind 200 (0.78e9) 22 / 21
+ * and 26 / 19, 700 behind none (1.0e9) 27 / 25 and 27 / 19, 200 behind 2000 (1.7e9) 42 / 41 and 38 / 26, 50 behind 16000 (3.3e9) 75 / 74 and 60 / 43; 16 heads of 64: 700 behind none
+ * (0.25e9) 11 / 11 and 16 / 13, 512 behind 1500 (0.92e9) 24 / 23 and 25 / 18, 100 behind 500 sixteen times (0.90e9) 28 / 27 and 25 / 18. */
+#define PAGED_MANY_FROM 7e8
+static inline bool vt_paged_may_be_many(int hp, long long cols) { return hp <= 2 && cols > 64; }
+static inline bool vt_paged_any_many(const vt_paged_shape &s, int n_seqs, const int *past, const int *rows) {
+    const int group = s.n_heads / s.n_kv_heads, hp = s.head_dim / 64;
+    double all = 0;
+    for (int i = 0; i < n_seqs; i++)
+        if (vt_paged_may_be_many(hp, (long long)rows[i] * group)) {
+            const double seen = past[i] + 0.5 * rows[i];
+            all += (double)rows[i] * group * (s.window && seen > s.window ? s.window : seen) * s.n_kv_heads * s.head_dim;
+        }
+    return all >= PAGED_MANY_FROM;
+}
 
-/* calls f(sequence, c0, first row, end) for every tile of columns of one kernel's sequences */
+/* A kernel's part of a batch: `any`, whether there are sequences for the one for many columns.  Calls f(sequence, c0, first row, end) for every tile of columns. */
 template <class F>
-static inline void vt_paged_tiles(const vt_paged_shape &s, bool many, int n_seqs, const int *past, const int *rows, F f) {
+static inline void vt_paged_tiles(const vt_paged_shape &s, bool any, bool many, int n_seqs, const int *past, const int *rows, F f) {
     const int group = s.n_heads / s.n_kv_heads, wide = many ? PAGED_MANY_COLS : PAGED_FEW_COLS, hp = s.head_dim / 64;
     for (int i = 0; i < n_seqs; i++) {
         const long long cols = (long long)rows[i] * group;
-        if (vt_paged_is_many(hp, cols) != many) continue;
+        if ((any && vt_paged_may_be_many(hp, cols)) != many) continue;
         for (long long c0 = 0; c0 < cols; c0 += wide) {
             const long long last = (c0 + wide < cols ? c0 + wide : cols) - 1;
             f(i, (int)c0, vt_paged_first(s.window, past[i], (int)(c0 / group)), past[i] + (int)(last / group) + 1);
@@ -125,34 +141,42 @@ static inline int vt_paged_parts(int first, int end, int unit, int run) {
     return (int)((units + run - 1) / run);
 }
 
-/* The run with the least time, by figures of one item: `alone` us and `step` us a unit with a CU's other workgroups beside it, `merge` where
- * parts meet; workgroups are handed out as they come, the longest first. */
-static inline int vt_paged_run(const vt_paged_shape &s, bool many, int n_cu, int n_seqs, const int *past, const int *rows, int unit, double fixed, double step, double merge) {
-    const double slots = 2.0 * n_cu;
+/* What a workgroup takes: `fixed` us, `step` for a unit of its rows, alone on its CU and with `beside` of them on it, `part` more where it leaves a part, and `merge` for each of
+ * the parts that the last one adds; `tail`: the share of the longest that a launch of more than fit at once ends with.  By head_dim / 64; fitted to 25 batches at every run.  The run that
+ * these choose is behind the best one by 2 % on average (many columns: 5 %).  us at some of them: 1531 rows behind none, many columns, in runs of 4 / 8 / 12 / 16 / whole (fp32) 76 / 67
+ * / 61 / 65 / 72, 4000 of them 502 / 381 / 350 / 343 / 310, 512 behind 1500 62 / 50 / 54 / 51 / 83; few columns: one row behind 1999 in runs of 1 / 2 / 4 / 8 / 16 7.8 / 8.0 / 9.3 / 13 / 20, behind 65535 of 8 /
+ * 16 / 32 / 64 47 / 45 / 53 / 96, 37 behind 4000 of 2 / 6 / 12 / 32 31 / 23 / 21 / 42. */
+struct vt_paged_cost { int beside; float fixed, alone, step, part, merge, tail; };
+static const vt_paged_cost vt_paged_few_cost[4] = {{4, 1.3f, 0.27f, 0.75f, 1.6f, 0.12f, 0.27f}, {3, 2.3f, 0.58f, 2.4f, 3.1f, 0.12f, 0.2f}, {2, 2.3f, 0.95f, 2.1f, 4.2f, 0.12f, 0.18f}, {2, 2.3f, 1.35f, 1.8f, 5.2f, 0.11f, 0.16f}};
+static const vt_paged_cost vt_paged_many_cost[2] = {{2, 9.1f, 1.94f, 3.3f, 6.0f, 0.9f, 0.54f}, {2, 5.4f, 2.0f, 3.5f, 4.1f, 1.9f, 0.25f}};
+
+static inline int vt_paged_run(const vt_paged_shape &s, bool any, bool many, int n_cu, int n_seqs, const int *past, const int *rows, int unit) {
+    const vt_paged_cost &c = many ? vt_paged_many_cost[s.head_dim / 64 - 1] : vt_paged_few_cost[s.head_dim / 64 - 1];
     long long longest = 1;
-    vt_paged_tiles(s, many, n_seqs, past, rows, [&](int, int, int first, int end) {
+    vt_paged_tiles(s, any, many, n_seqs, past, rows, [&](int, int, int first, int end) {
         const long long n = vt_paged_parts(first, end, unit, 1);
         longest = n > longest ? n : longest;
     });
     int best = (int)longest;
     double least = 1e300;
-    for (long long run = longest, parts = 1; parts <= PAGED_MAX_PARTS; parts++) {
-        run = (longest + parts - 1) / parts;
-        long long items = 0, extra = 0, split = 0, most = 0;
-        double work = 0;
-        vt_paged_tiles(s, many, n_seqs, past, rows, [&](int, int, int first, int end) {
-            const int n = vt_paged_parts(first, end, unit, 1), p = (int)((n + run - 1) / run), each = (n + p - 1) / p;
+    for (int parts = 1; parts <= PAGED_MAX_PARTS; parts++) {
+        const int run = (int)((longest + parts - 1) / parts);
+        long long items = 0, extra = 0, split = 0, most = 0, all = 0;
+        int late = 0;
+        vt_paged_tiles(s, any, many, n_seqs, past, rows, [&](int, int, int first, int end) {
+            const int n = vt_paged_parts(first, end, unit, 1), p = (n + run - 1) / run, each = (n + p - 1) / p;
             items += p;
-            extra += p > 1 ? p : 0;
-            split += p > 1;
-            most = each > most ? each : most;
-            work += p * fixed + n * step;
+            all += n;
+            if (p > 1) { extra += p; split++; }
+            if (each > most || (each == most && p > 1)) { late = p > 1; most = each; }
         });
         if (extra > PAGED_SPLIT_ITEMS || split * s.n_kv_heads > PAGED_COUNTERS) break;
-        const double wgs = (double)items * s.n_kv_heads, share = wgs < slots ? 0.5 + 0.5 * wgs / slots : 1.0;
-        const double one = fixed + most * step * share, all = work * s.n_kv_heads / slots;
-        const double us = (one > all ? one : all) + (wgs > slots ? 0.5 * one : 0.0) + (split ? merge : 0.0);
-        if (us < least) { least = us; best = (int)run; }
+        const double wgs = (double)items * s.n_kv_heads, room = (double)n_cu * c.beside;
+        const double share = wgs < n_cu ? 0.0 : wgs < room ? (wgs - n_cu) / (room - n_cu) : 1.0;
+        const double one = c.fixed + most * (c.alone + (c.step - c.alone) * share) + late * c.part;
+        const double sum = (items * c.fixed + all * c.step + extra * c.part) * s.n_kv_heads / room + (wgs > room ? c.tail * one : 0.0);
+        const double us = (one > sum ? one : sum) + (split ? c.merge * parts : 0.0);
+        if (us < least) { least = us; best = run; }
         if (run == 1) break;
     }
     return best;
@@ -168,12 +192,11 @@ static int vt_paged_longest(const void *a, const void *b) {
 }
 
 /* Items of one kernel into `to`, the longest first; -> how many, and their slots */
-static inline int vt_paged_items(const vt_paged_shape &s, bool many, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to, int *n_slots) {
+static inline int vt_paged_items(const vt_paged_shape &s, bool any, bool many, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to, int *n_slots) {
     const int unit = many ? PAGED_MANY_ROWS : PAGED_FEW_ROWS * PAGED_FEW_WAVES, group = s.n_heads / s.n_kv_heads;
-    const double hp = s.head_dim / 64;
-    const int run = many ? vt_paged_run(s, true, n_cu, n_seqs, past, rows, unit, 6.0, 1.5 * hp, 4.0) : vt_paged_run(s, false, n_cu, n_seqs, past, rows, unit, 4.0, 0.6 * hp, 3.0);
+    const int run = vt_paged_run(s, any, many, n_cu, n_seqs, past, rows, unit);
     int n = 0, slots = 0, counters = 0, row = 0, seq = 0;
-    vt_paged_tiles(s, many, n_seqs, past, rows, [&](int i, int c0, int first, int end) {
+    vt_paged_tiles(s, any, many, n_seqs, past, rows, [&](int i, int c0, int first, int end) {
         while (seq < i) row += rows[seq++];
         const int units = vt_paged_parts(first, end, unit, 1), parts = (units + run - 1) / run, u0 = first / unit;
         for (int p = 0; p < parts; p++) {
@@ -190,13 +213,14 @@ static inline int vt_paged_items(const vt_paged_shape &s, bool many, int n_cu, i
 
 static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to) {
     vt_paged_plan p;
-    p.few = vt_paged_items(s, false, n_cu, n_seqs, past, rows, starts, to, &p.few_slots);
-    p.many = vt_paged_items(s, true, n_cu, n_seqs, past, rows, starts, to + p.few, &p.many_slots);
+    const bool any = vt_paged_any_many(s, n_seqs, past, rows);
+    p.few = vt_paged_items(s, any, false, n_cu, n_seqs, past, rows, starts, to, &p.few_slots);
+    p.many = vt_paged_items(s, any, true, n_cu, n_seqs, past, rows, starts, to + p.few, &p.many_slots);
     /* Requests that leave nothing behind in the caches: 65535 rows of 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows, which the caches
      * (32 MB of L2) keep for the next call on them, 6.8 -> 7.2. */
     long long read = 0;
     p.once = 1;
-    vt_paged_tiles(s, false, n_seqs, past, rows, [&](int i, int, int first, int end) {
+    vt_paged_tiles(s, any, false, n_seqs, past, rows, [&](int i, int, int first, int end) {
         if ((long long)rows[i] * (s.n_heads / s.n_kv_heads) > PAGED_FEW_COLS) p.once = 0;
         read += end - first;
     });
