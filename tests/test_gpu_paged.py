@@ -162,23 +162,45 @@ def test_attention(hip, batch, page, window, layout, bf16):
 
 
 MANY = [  # layout, batch, page, window: enough for the kernel for many columns
-    ((32, 8, 128), "700@0 3@50", 16, 0), ((32, 8, 128), "130@500 1@700 64@64 0@9 600@300", 64, 0), ((32, 8, 128), "2000@0", 16, 90), ((32, 8, 128), "37@3000 100@2000", 32, 0),
-    ((16, 16, 64), "333@700 500@100 1@40 700@0", 256, 0), ((16, 16, 64), "65@6000 300@2000", 16, 0), ((8, 1, 128), "300@8000", 16, 0), ((8, 1, 128), "1500@100 17@800", 32, 500), ((8, 1, 128), "3000@33", 64, 260),
-    ((14, 2, 64), "1000@400", 1024, 0), ((20, 1, 64), "800@333 9@9", 16, 0)]
+    ((32, 8, 128), "1300@0 3@50", 16, 0), ((32, 8, 128), "130@500 1@700 64@64 0@9 900@450", 64, 0), ((32, 8, 128), "7000@0", 16, 90), ((32, 8, 128), "37@9000 100@4000", 32, 0),
+    ((16, 16, 64), "333@3700 900@1100 1@40 700@0", 256, 0), ((16, 16, 64), "65@36000 300@2000", 16, 0), ((8, 1, 128), "300@9000", 16, 0), ((8, 1, 128), "5300@100 17@800", 32, 500), ((8, 1, 128), "10000@33", 64, 260),
+    ((14, 2, 64), "2000@800", 1024, 0), ((20, 1, 64), "1500@733 9@9", 16, 0)]
+WIDE = [  # enough for 32 columns at a time
+    ((32, 8, 128), "37@5100 1@300", 16, 0), ((32, 8, 128), "300@700 5@5 0@1", 64, 650), ((32, 8, 128), "90@1111 7@2000", 32, 1000), ((16, 16, 64), "512@1500", 16, 0), ((20, 1, 64), "100@4000 2@9000", 256, 0),
+    ((8, 1, 128), "70@9999", 16, 0)]
+
+
+def large(hip, layout, batch, page, window, bf16, scale=None, size=1.0):
+    c = P.Cache(hip, batch, page, *layout, window=window, seed=len(batch))
+    c.fill(size=size)
+    c.upload()
+    q = normal(np.random.default_rng(7), (sum(c.rows), layout[0], layout[2]), bf16)
+    scale = scale or 1 / math.sqrt(layout[2])
+    keep = c.some()
+    got = P.attention(c, q, bf16, scale, q_gap=8)
+    assert np.isfinite(got).all()
+    assert P.check(c, got, *c.attend(q, scale, keep), bf16, keep)
+    assert np.array_equal(got, P.attention(c, q, bf16, scale))
+    many = any(P.is_many(c, i) for i in range(len(c.rows)))
+    c.free()
+    return many
 
 
 @pytest.mark.parametrize("bf16", [0, 1])
 @pytest.mark.parametrize("layout,batch,page,window", MANY)
 def test_attention_of_many_columns(hip, layout, batch, page, window, bf16):
-    test_attention(hip, batch, page, window, layout, bf16)
-    c = P.Cache(hip, batch, page, *layout, window=window)
-    assert any(P.is_many(c, i) for i in range(len(c.rows)))
-    c.free()
+    assert large(hip, layout, batch, page, window, bf16)
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("layout,batch,page,window", WIDE)
+def test_attention_of_32_columns_at_a_time(hip, layout, batch, page, window, bf16):
+    assert not large(hip, layout, batch, page, window, bf16)
 
 
 @pytest.mark.parametrize("bf16", [0, 1])
 @pytest.mark.parametrize("layout", [(8, 2, 128), (6, 2, 192), (16, 2, 64)])
-@pytest.mark.parametrize("batch,window", [("40@100", 0), ("9@7", 0), ("40@100 1@200", 30), ("300@10", 40), ("900@500", 0), ("2500@10", 300), ("1700@0 1@500", 130), ("8000@0", 100)])
+@pytest.mark.parametrize("batch,window", [("40@100", 0), ("9@7", 0), ("40@100 1@200", 30), ("300@10", 40), ("200@3000", 0), ("2000@800", 0), ("7500@10", 300), ("3700@0 1@500", 600), ("25000@0", 100)])
 def test_what_a_query_does_not_see_changes_nothing(hip, batch, window, layout, bf16):
     """Infinities and NaN in keys and values: who sees a key's NaN answers NaN, who sees a value's in that value; nobody else notices.  Who sees a key's infinity answers NaN
     where its score is +infinity or no number, and may where it is -infinity, a weight of 0."""
@@ -200,7 +222,11 @@ def test_what_a_query_does_not_see_changes_nothing(hip, batch, window, layout, b
     q = normal(np.random.default_rng(7), (sum(c.rows), layout[0], layout[2]), bf16)
     scale = 1 / math.sqrt(layout[2])
     got = P.attention(c, q, bf16, scale)
-    want, size, most = c.attend(q, scale)
+    keep = c.some()
+    keep[rows // 2 - 5:rows // 2 + 45] = True
+    keep[:60] = keep[max(0, rows - window - 10):rows - window + 40] = keep[rows - 20:rows] = True
+    want, size, most = c.attend(q, scale, keep)
+    got, want, size = (np.where(keep[:, None, None], x, 0) for x in (got, want, size))
     assert np.isnan(want).any() and not np.isnan(want).all()
     inf = np.isinf(got)
     assert not (inf & ~np.isnan(want)).any()
@@ -210,12 +236,12 @@ def test_what_a_query_does_not_see_changes_nothing(hip, batch, window, layout, b
         sees[:rows, :layout[0] // layout[1]] = ((age >= 0) & (age < window))[:, None, None]
         assert sees.any() and not sees.all()
         want[sees & np.isnan(got)] = np.nan
-    assert P.check(c, np.where(inf, np.nan, got), want, size, most, bf16)
+    assert P.check(c, np.where(inf, np.nan, got), want, size, most, bf16, keep)
     c.free()
 
 
 @pytest.mark.parametrize("bf16", [0, 1])
-@pytest.mark.parametrize("batch", ["1@700", "100@300", "1000@300"])
+@pytest.mark.parametrize("batch", ["1@700", "100@300", "300@1500", "1500@1000"])
 def test_scores_far_apart(hip, batch, bf16):
     """Scores of hundreds: a weight's error is that of its score, and the largest takes all."""
     c = P.Cache(hip, batch, 16, 8, 2, 128, seed=2)

@@ -32,11 +32,12 @@ int main(void) {
         if (vt_paged_shape_bad(s) || f.what) { bad++; printf("refused %d\n", f.what); continue; }
         std::vector<vt_paged_item> items(vt_paged_max_items(n_seqs, max_rows, group));
         const vt_paged_plan plan = vt_paged_plan_of(s, 256, n_seqs, past.data(), rows.data(), starts.data(), items.data());
+        const vt_paged_kinds kinds = vt_paged_kinds_of(s, 256, n_seqs, past.data(), rows.data());
         if (plan.few + plan.many > (int)items.size()) { bad++; printf("items %d %d\n", plan.few, plan.many); }
         /* every column's rows are read once, by the parts of one group, in slots of its own */
         std::vector<long long> want(n_seqs), got(n_seqs);
         for (int k = 0; k < 2; k++) {
-            const int from = k ? plan.few : 0, n = k ? plan.many : plan.few, cols = k ? PAGED_MANY_COLS : PAGED_FEW_COLS, unit = k ? 64 : 32, n_slots = k ? plan.many_slots : plan.few_slots;
+            const int from = k ? plan.few : 0, n = k ? plan.many : plan.few, cols = k ? PAGED_MANY_COLS : kinds.few_cols, unit = k ? 64 : 32, n_slots = k ? plan.many_slots : plan.few_slots;
             std::vector<char> slot(n_slots);
             std::vector<int> left(PAGED_COUNTERS);
             for (int j = from; j < from + n; j++) {
@@ -67,8 +68,8 @@ int main(void) {
         }
         for (int i = 0; i < n_seqs; i++) {
             long long all = 0;
-            const bool many = vt_paged_any_many(s, n_seqs, past.data(), rows.data()) && vt_paged_may_be_many(lay[2] / 64, (long long)rows[i] * group);
-            const int cols = many ? PAGED_MANY_COLS : PAGED_FEW_COLS;
+            const bool many = kinds.any && vt_paged_may_be_many(lay[2] / 64, (long long)rows[i] * group);
+            const int cols = many ? PAGED_MANY_COLS : kinds.few_cols;
             for (int c = 0; c < rows[i] * group; c += cols) all++;
             if (got[i] != want[i] || (rows[i] && !got[i])) { bad++; printf("sequence %d of %d: %lld of %lld\n", i, n_seqs, got[i], want[i]); }
         }

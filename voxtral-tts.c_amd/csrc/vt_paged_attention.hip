@@ -125,14 +125,14 @@ static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, in
  * and then the workgroups that share the columns' rows, add their parts in a fixed order, the last workgroup to arrive those of all.  K is the A operand of 16 x 16 x 32, a lane's 16
  * bytes from its own row.  V's rows are its columns: a lane loads CD values each of the eight rows that it has weights of, 16 lanes a whole row, and pairs of rows are
  * put together two values at a time.  Queries, the same for all waves, wait in LDS as operands.  ONCE: no other workgroup reads these rows, and there are more than a cache holds. */
-template <int HP, bool F32, bool ONCE>
+template <int HP, bool F32, bool ONCE, int CT>
 __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(pa_job a) {
     constexpr int HD = 64 * HP, ROW = 2 * HD, KS = 2 * HP, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4, WAVES = PAGED_FEW_WAVES;
-    constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 2, COLS = PAGED_FEW_COLS, HOW = ONCE ? 2 /* nt */ : 0;
+    constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 2, COLS = 16 * CT, HOW = ONCE ? 2 /* nt */ : 0;
     __shared__ __attribute__((aligned(16))) float area[WAVES][COLS][OD];                /* the queries' operands, then the waves' parts */
     __shared__ float ml[WAVES][COLS][2], wt[COLS][PAGED_MAX_PARTS];
     __shared__ int last;
-    static_assert(sizeof area >= KS * NQ * 1024, "operands");
+    static_assert(sizeof area >= KS * NQ * CT * 1024, "operands");
     u32x4 *queries = reinterpret_cast<u32x4 *>(area);
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4, h = (int)blockIdx.x, heads = (int)gridDim.x;
     const vt_paged_item it = pa_item(a.items);
@@ -170,33 +170,50 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
                 }
         }
     };
-    const int nc = min(COLS, it.cols - it.c0), cc = min(it.c0 + n, it.cols - 1), qi = vt_div(cc, a.group), pos = it.past + qi;
-    const size_t head_at = (size_t)h * a.group.d + (cc - qi * a.group.d);
+    const int nc = min(COLS, it.cols - it.c0);
+    const bool two = CT == 2 && nc > 16;
+    int qi[2], see_lo[2], see_hi[2];                     /* CT of them */
+    size_t q_at[2];
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const int cc = min(it.c0 + 16 * c + n, it.cols - 1);
+        qi[c] = vt_div(cc, a.group);
+        const int pos = it.past + qi[c];
+        see_lo[c] = max(a.window && pos >= a.window ? pos - a.window + 1 : 0, it.lo);
+        see_hi[c] = min(pos + 1, it.end);
+        q_at[c] = (size_t)(it.row + qi[c]) * a.q_stride + ((size_t)h * a.group.d + (cc - qi[c] * a.group.d)) * HD;
+    }
     /* queries first: loads return in order */
-    constexpr int MINE = (KS + WAVES - 1) / WAVES;       /* steps of the product that a wave brings the queries' operands of */
+    constexpr int MINE = (KS * CT + WAVES - 1) / WAVES;  /* operands of queries that a wave brings: step x / CT of the product, columns 16 (x % CT) .. */
     u32x4 raw[MINE][2];
 #pragma unroll
-    for (int x = 0; x < MINE; x++)
-        pa_query_load<F32>(a.Q, (size_t)(it.row + qi) * a.q_stride + head_at * HD + 32 * min(wave + WAVES * x, KS - 1) + 8 * g, raw[x]);
+    for (int x = 0; x < MINE; x++) {
+        const int y = min(wave + WAVES * x, KS * CT - 1);
+        pa_query_load<F32>(a.Q, (CT == 2 && y % CT ? q_at[1] : q_at[0]) + 32 * (y / CT) + 8 * g, raw[x]);
+    }
     place(wave);
     ask_k();
     ask_v();
 #pragma unroll
     for (int x = 0; x < MINE; x++) {
-        const int ks = wave + WAVES * x;
-        if (KS % WAVES && ks >= KS) break;
+        const int y = wave + WAVES * x;
+        if (KS * CT % WAVES && y >= KS * CT) break;
         u32x4 q[NQ];
         pa_query_planes<F32, NQ>(raw[x], a.scale, q);
 #pragma unroll
-        for (int p = 0; p < NQ; p++) queries[(ks * NQ + p) * 64 + lane] = q[p];
+        for (int p = 0; p < NQ; p++) queries[(y * NQ + p) * 64 + lane] = q[p];
     }
-    const int see_lo = max(a.window && pos >= a.window ? pos - a.window + 1 : 0, it.lo), see_hi = min(pos + 1, it.end);
     const int q_first = it.past + vt_div(it.c0, a.group), q_last = it.past + vt_div(it.c0 + nc - 1, a.group);
     const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);       /* rows that every column sees */
-    float m = -3.402823466e38f, l = 0.f;                 /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
-    f32x4 o[CHUNKS * CD];
+    float m[2], l[2];
+    f32x4 o[CT][CHUNKS * CD];
 #pragma unroll
-    for (int i = 0; i < CHUNKS * CD; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < CT; c++) {
+        m[c] = -3.402823466e38f;                         /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
+        l[c] = 0.f;
+#pragma unroll
+        for (int i = 0; i < CHUNKS * CD; i++) o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     __syncthreads();
 #pragma unroll 1
     for (int t = wave; t < tiles; t += WAVES) {
@@ -205,23 +222,30 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
         place(t + WAVES);
         int own = lane;                                  /* (through an empty asm: else the queries are kept in registers after all) */
         asm volatile("" : "+v"(own));
-        f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        f32x4 s[CT][2];
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+        for (int c = 0; c < CT; c++) {
+            s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (c && !two) break;
 #pragma unroll
-            for (int p = NQ - 1; p >= 0; p--) {
-                const pa_bf16x8 q = pa_operand(queries[(ks * NQ + p) * 64 + own]);
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(k[kt][ks]), q, s[kt], 0, 0, 0);
-            }
+                for (int p = NQ - 1; p >= 0; p--) {
+                    const pa_bf16x8 q = pa_operand(queries[((ks * CT + c) * NQ + p) * 64 + own]);
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++) s[c][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(k[kt][ks]), q, s[c][kt], 0, 0, 0);
+                }
+        }
         ask_k();
-        auto sees = [&](int kt, int v) { const int key = first + 16 * kt + 4 * g + v; return key >= see_lo && key < see_hi; };
+        auto sees = [&](int c, int kt, int v) { const int key = first + 16 * kt + 4 * g + v; return key >= see_lo[c] && key < see_hi[c]; };
         bool bad = false;
         if (hidden) {
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++)
+            for (int c = 0; c < CT; c++)
 #pragma unroll
-                for (int v = 0; v < 4; v++) s[kt][v] = sees(kt, v) ? s[kt][v] : -INFINITY;
+                for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) s[c][kt][v] = sees(c, kt, v) ? s[c][kt][v] : -INFINITY;
             pa_u16x2 most = {0, 0};
 #pragma unroll
             for (int j = 0; j < 8; j++)
@@ -231,49 +255,56 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
                     for (int e = 0; e < CD / 2; e++) most = pa_larger(most, v[j][ch][e]);
             bad = __any(pa_not_finite(most));
         }
-        float top = __builtin_elementwise_maximum(s[0][0], s[1][0]);                /* a NaN stays one: who sees it answers NaN */
+        u32x4 w4[CT][NP];
 #pragma unroll
-        for (int v = 1; v < 4; v++) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[0][v]), s[1][v]);
-        {
-            f32x2 r = vt_swap16(top, top);
-            top = __builtin_elementwise_maximum(r.x, r.y);
-            r = vt_swap32(top, top);
-            top = __builtin_elementwise_maximum(r.x, r.y);
-        }
-        if constexpr (!F32) top = top * a.scale;
-        if (__any(!(top <= m + PA_SLACK))) {
-            top = __builtin_elementwise_maximum(top, m);
-            const float less = pa_exp2(m - top);
-            l *= less;
+        for (int c = 0; c < CT; c++) {
+            if (c && !two) break;
+            float top = __builtin_elementwise_maximum(s[c][0][0], s[c][1][0]);                /* a NaN stays one: who sees it answers NaN */
 #pragma unroll
-            for (int i = 0; i < CHUNKS * CD; i++) o[i] = o[i] * less;
-            m = top;
-        }
-        u32x4 w4[NP];
+            for (int v = 1; v < 4; v++) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[c][0][v]), s[c][1][v]);
+            {
+                f32x2 r = vt_swap16(top, top);
+                top = __builtin_elementwise_maximum(r.x, r.y);
+                r = vt_swap32(top, top);
+                top = __builtin_elementwise_maximum(r.x, r.y);
+            }
+            if constexpr (!F32) top = top * a.scale;
+            if (__any(!(top <= m[c] + PA_SLACK))) {
+                top = __builtin_elementwise_maximum(top, m[c]);
+                const float less = pa_exp2(m[c] - top);
+                l[c] *= less;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float p0 = pa_weight<F32>(s[e >> 1][2 * (e & 1)], m, a.scale), p1 = pa_weight<F32>(s[e >> 1][2 * (e & 1) + 1], m, a.scale);
-            l += p0 + p1;
-            unsigned w[NP];
-            pa_planes2<NP>(p0, p1, w);
+                for (int i = 0; i < CHUNKS * CD; i++) o[c][i] = o[c][i] * less;
+                m[c] = top;
+            }
 #pragma unroll
-            for (int p = 0; p < NP; p++) w4[p][e] = w[p];
+            for (int e = 0; e < 4; e++) {
+                const float p0 = pa_weight<F32>(s[c][e >> 1][2 * (e & 1)], m[c], a.scale), p1 = pa_weight<F32>(s[c][e >> 1][2 * (e & 1) + 1], m[c], a.scale);
+                l[c] += p0 + p1;
+                unsigned w[NP];
+                pa_planes2<NP>(p0, p1, w);
+#pragma unroll
+                for (int p = 0; p < NP; p++) w4[c][p][e] = w[p];
+            }
         }
         if (bad) {                                       /* rare */
-            u32x4 ones;
 #pragma unroll
-            for (int e = 0; e < 4; e++) ones[e] = (sees(e >> 1, 2 * (e & 1)) ? 0x3f80u : 0u) | (sees(e >> 1, 2 * (e & 1) + 1) ? 0x3f800000u : 0u);
+            for (int c = 0; c < CT; c++) {
+                u32x4 ones;
 #pragma unroll
-            for (int ch = 0; ch < CHUNKS; ch++)
+                for (int e = 0; e < 4; e++) ones[e] = (sees(c, e >> 1, 2 * (e & 1)) ? 0x3f80u : 0u) | (sees(c, e >> 1, 2 * (e & 1) + 1) ? 0x3f800000u : 0u);
 #pragma unroll
-                for (int i = 0; i < CD; i++) {
-                    u32x4 v4;
+                for (int ch = 0; ch < CHUNKS; ch++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v4[e] = pa_marks(__builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u));
-                    const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(ones), (f32x4{0.f, 0.f, 0.f, 0.f}), 0, 0, 0);
+                    for (int i = 0; i < CD; i++) {
+                        u32x4 v4;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[ch * CD + i][e] = hit[e] > 0.f ? NAN : o[ch * CD + i][e];
-                }
+                        for (int e = 0; e < 4; e++) v4[e] = pa_marks(__builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u));
+                        const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(ones), (f32x4{0.f, 0.f, 0.f, 0.f}), 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[c][ch * CD + i][e] = hit[e] > 0.f ? NAN : o[c][ch * CD + i][e];
+                    }
+            }
 #pragma unroll
             for (int j = 0; j < 8; j++)
 #pragma unroll
@@ -288,31 +319,41 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
                 u32x4 v4;
 #pragma unroll
                 for (int e = 0; e < 4; e++) v4[e] = __builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
-                f32x4 &acc = o[ch * CD + i];
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[p]), acc, 0, 0, 0);
+                for (int p = NP - 1; p >= 0; p--) o[0][ch * CD + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[0][p]), o[0][ch * CD + i], 0, 0, 0);
+                if constexpr (CT == 2) {                 /* (also where there is no second: a branch for each would cost more) */
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; p--) o[CT - 1][ch * CD + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[CT - 1][p]), o[CT - 1][ch * CD + i], 0, 0, 0);
+                }
             }
         ask_v();
     }
-    l = vt_rows_sum(l);
     /* The waves' parts, each times its share of the sum of weights: a mean of values */
-    ml[wave][n][0] = m;                                  /* four lanes the same */
-    ml[wave][n][1] = l;
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        l[c] = vt_rows_sum(l[c]);
+        ml[wave][16 * c + n][0] = m[c];                  /* four lanes the same */
+        ml[wave][16 * c + n][1] = l[c];
+    }
     __syncthreads();
-    float M = m, L = 0.f;
+    float M[2], L[2];
 #pragma unroll
-    for (int k = 0; k < WAVES; k++) M = fmaxf(M, ml[k][n][0]);
+    for (int c = 0; c < CT; c++) {
+        const int col = 16 * c + n;
+        M[c] = m[c];
+        L[c] = 0.f;
 #pragma unroll
-    for (int k = 0; k < WAVES; k++) L = fmaf(ml[k][n][1], pa_exp2(ml[k][n][0] - M), L);
-    {
-        const float f = L == 0.f && it.parts > 1 ? 0.f : pa_exp2(m - M) / L;
-        float *to = &area[wave][n][4 * g * CD];
+        for (int k = 0; k < WAVES; k++) M[c] = fmaxf(M[c], ml[k][col][0]);
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) L[c] = fmaf(ml[k][col][1], pa_exp2(ml[k][col][0] - M[c]), L[c]);
+        const float f = L[c] == 0.f && it.parts > 1 ? 0.f : pa_exp2(m[c] - M[c]) / L[c];
+        float *to = &area[wave][col][4 * g * CD];
 #pragma unroll
         for (int ch = 0; ch < CHUNKS; ch++)
 #pragma unroll
             for (int v = 0; v < 4; v++)
 #pragma unroll
-                for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * v + i] = o[ch * CD + i][v] * f;
+                for (int i = 0; i < CD; i++) to[16 * CD * ch + CD * v + i] = o[c][ch * CD + i][v] * f;
     }
     __syncthreads();
     const __amdgpu_buffer_rsrc_t pd = vt_buffer(a.part + (size_t)(it.slot * heads + h * it.parts) * COLS * OD, it.parts * COLS * OD * 4);
@@ -332,7 +373,10 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
         }
     }
     if (it.parts == 1) return;
-    if (wave == 0 && lane < nc) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, pd, (it.part * COLS + lane) * OD * 4, 0, 16);
+    if (wave == 0 && g < CT && 16 * g + n < nc) {
+        const float most = CT == 2 && g ? M[CT - 1] : M[0], sum = CT == 2 && g ? L[CT - 1] : L[0];
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(most), __float_as_uint(sum)}, pd, (it.part * COLS + lane) * OD * 4, 0, 16);
+    }
     __builtin_amdgcn_s_waitcnt(0x0f70);                  /* the part's stores are acknowledged */
     __syncthreads();
     unsigned *cnt = a.cnt + it.counter * heads + h;
@@ -683,22 +727,23 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     }
 }
 
-template <int HP>
-static void pa_launch(const pa_job &job, const vt_paged_plan &p, int heads, bool f32) {
+template <int HP, bool F32>
+static void pa_launch(const pa_job &job, const vt_paged_plan &p, int heads) {
     if (p.few) {
         const dim3 grid((unsigned)heads, (unsigned)p.few), threads(64 * PAGED_FEW_WAVES);
-        if (f32 && p.once) hipLaunchKernelGGL((vt_paged_few_kernel<HP, true, true>), grid, threads, 0, g_vt.stream, job);
-        else if (f32) hipLaunchKernelGGL((vt_paged_few_kernel<HP, true, false>), grid, threads, 0, g_vt.stream, job);
-        else if (p.once) hipLaunchKernelGGL((vt_paged_few_kernel<HP, false, true>), grid, threads, 0, g_vt.stream, job);
-        else hipLaunchKernelGGL((vt_paged_few_kernel<HP, false, false>), grid, threads, 0, g_vt.stream, job);
+        if constexpr (HP <= 2) {
+            if (p.wide) hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, false, 2>), grid, threads, 0, g_vt.stream, job);
+        }
+        if (p.wide) { }
+        else if (p.once) hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, true, 1>), grid, threads, 0, g_vt.stream, job);
+        else hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, false, 1>), grid, threads, 0, g_vt.stream, job);
     }
     if constexpr (HP <= 2) {
         if (p.many) {
             pa_job many = job;
             many.items += p.few;
             const dim3 grid((unsigned)heads, (unsigned)p.many);
-            if (f32) hipLaunchKernelGGL((vt_paged_many_kernel<HP, true>), grid, dim3(256), 0, g_vt.stream, many);
-            else hipLaunchKernelGGL((vt_paged_many_kernel<HP, false>), grid, dim3(256), 0, g_vt.stream, many);
+            hipLaunchKernelGGL((vt_paged_many_kernel<HP, F32>), grid, dim3(256), 0, g_vt.stream, many);
         }
     }
 }
@@ -720,15 +765,17 @@ extern "C" int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16,
     const int group = s.n_heads / s.n_kv_heads;
     int page_log = 4;
     while (1 << page_log < s.page_rows) page_log++;
-    const size_t few = (size_t)b->plan.few_slots * s.n_kv_heads * PAGED_FEW_COLS * (s.head_dim + 4) * 4, many = (size_t)b->plan.many_slots * s.n_kv_heads * 4 * (8 * HP + 1) * 1024;
+    const size_t few = (size_t)b->plan.few_slots * s.n_kv_heads * (b->plan.wide ? 32 : 16) * (s.head_dim + 4) * 4, many = (size_t)b->plan.many_slots * s.n_kv_heads * 4 * (8 * HP + 1) * 1024;
     pa_job job = {(const uint16_t *)d_k_pages, (const uint16_t *)d_v_pages, d_Q, d_out, NULL, g_vt.d_mx4_cnt, (const vt_paged_item *)(b->dev + b->at_items),
                   (const int *)(b->dev + b->at_tables), q_stride, s.n_heads, page_log, s.window, vt_divisor_of(group, (long long)b->max_rows * group), scale * 1.44269504f};
     if ((few || many) && !(job.part = (float *)vt_scratch(few > many ? few : many))) return -1;
+#define ATTEND(H) (x_bf16 ? pa_launch<H, false>(job, b->plan, s.n_kv_heads) : pa_launch<H, true>(job, b->plan, s.n_kv_heads))
     switch (HP) {
-    case 1: pa_launch<1>(job, b->plan, s.n_kv_heads, !x_bf16); break;
-    case 2: pa_launch<2>(job, b->plan, s.n_kv_heads, !x_bf16); break;
-    case 3: pa_launch<3>(job, b->plan, s.n_kv_heads, !x_bf16); break;
-    default: pa_launch<4>(job, b->plan, s.n_kv_heads, !x_bf16);
+    case 1: ATTEND(1); break;
+    case 2: ATTEND(2); break;
+    case 3: ATTEND(3); break;
+    default: ATTEND(4);
     }
+#undef ATTEND
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }

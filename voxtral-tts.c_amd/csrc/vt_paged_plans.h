@@ -15,8 +15,7 @@
 #define PAGED_COUNTERS 16384               /* heads times tiles of columns that several workgroups share */
 
 /* Columns are a sequence's new rows times the heads that share a kv head: column c is row c / group, head c % group of the group.
- * Few columns: 16 to a workgroup, whose waves take 32 rows of the cache each in turn.  Many: 128 to a workgroup, 64 rows at a time. */
-#define PAGED_FEW_COLS 16
+ * Few columns: 16 or 32 to a workgroup, whose waves take 32 rows of the cache each in turn.  Many: 128 to a workgroup, 64 rows at a time. */
 #define PAGED_FEW_ROWS 32
 #define PAGED_FEW_WAVES 4
 #define PAGED_MANY_COLS 128
@@ -96,38 +95,59 @@ static inline vt_paged_fault vt_paged_lay_out(const vt_paged_shape &s, int max_s
 
 /* ---- work items --- */
 
-/* items of either kernel (the few's first), parts that they leave; once: the few's rows are read by one workgroup each, more of them than a cache holds */
-struct vt_paged_plan { int few, many, few_slots, many_slots, once; };
+/* items of either kernel (the few's first), parts that they leave; wide: the few's columns go by 32; once: their rows are read by one workgroup each, more of them than a cache holds */
+struct vt_paged_plan { int few, many, few_slots, many_slots, wide, once; };
+
+/* Which kernels a batch goes to: `any`, whether there are sequences for the one for many columns; columns of a workgroup of the other */
+struct vt_paged_kinds { bool any; int few_cols; };
 
 static inline long long vt_paged_max_items(int max_seqs, int max_rows, int group) {
-    return (long long)max_rows * group / PAGED_FEW_COLS + max_seqs + 2 * PAGED_SPLIT_ITEMS;
+    return (long long)max_rows * group / 16 + max_seqs + 2 * PAGED_SPLIT_ITEMS;
 }
 
 /* Which sequences go to the kernel for many columns: those of more than 64 whose heads of up to 128 values leave it registers, where there is enough for it to do, as columns times
- * the rows that they see on average times kv heads times values.  A workgroup of it does twice as much for what it reads, but there are few of them.  Measured, us with the kernel
- * for few columns and for many (fp32 / bf16), 32 heads on 8 of 128: 300 rows behind none (0.18e9) 11 / 10 and 17 / 13, 37 behind 4000 (0.61e9) 21 / 21 and 34 / 26, 450 behind 200 (0.78e9) 22 / 21
- * and 26 / 19, 700 behind none (1.0e9) 27 / 25 and 27 / 19, 200 behind 2000 (1.7e9) 42 / 41 and 38 / 26, 50 behind 16000 (3.3e9) 75 / 74 and 60 / 43; 16 heads of 64: 700 behind none
- * (0.25e9) 11 / 11 and 16 / 13, 512 behind 1500 (0.92e9) 24 / 23 and 25 / 18, 100 behind 500 sixteen times (0.90e9) 28 / 27 and 25 / 18. */
-#define PAGED_MANY_FROM 7e8
+ * the rows that they see on average times kv heads times values, over all of them.  It does twice as much with what it reads, but by few workgroups.  Measured, us with the kernel
+ * for few columns, 32 at a time, and for many (fp32 / bf16), 32 heads on 8 of 128: 450 rows behind 200 (0.8e9) 18 / 16 and 26 / 19, 700 behind none (1.0e9) 24 / 20 and 27 / 19, 200 behind
+ * 2000 (1.7e9) 32 / 24 and 38 / 26, 50 behind 16000 (3.3e9) 52 / 48 and 60 / 43, 512 behind 1500 (3.7e9) 45 / 39 and 49 / 32, 100 behind 500 sixteen times (3.6e9) 59 / 47 and 49 / 29; 16 heads of
+ * 64: 512 behind 1500 (0.9e9) 21 / 17 and 24 / 18.
+ * Else 32 columns to a workgroup, not 16, where there is enough for that, as columns / 16 times rows times kv heads times values (less where every CU has one of 16); 16 and 32 at a time: 37 rows behind 300 (3e6) 7.0 / 6.4 and 9.9 /
+ * 8.2, 100 behind 1000 (27e6) 13 / 13 and 19 / 15, 37 behind 4000 (41e6) 21 / 21 and 23 / 20, 16 behind 300 32 times (40e6) 22 / 22 and 17 / 14, 200 behind 2000 (107e6) 42 / 41 and 32 / 24; 16 heads of 64: 37
+ * behind 4000 (12e6) 14 / 13 and 17 / 16, 512 behind 1500 (57e6) 24 / 23 and 21 / 17. */
+#define PAGED_MANY_FROM 2.5e9
+#define PAGED_WIDE_FROM 45e6
+#define PAGED_WIDE_FULL 30e6
 static inline bool vt_paged_may_be_many(int hp, long long cols) { return hp <= 2 && cols > 64; }
-static inline bool vt_paged_any_many(const vt_paged_shape &s, int n_seqs, const int *past, const int *rows) {
+static inline vt_paged_kinds vt_paged_kinds_of(const vt_paged_shape &s, int n_cu, int n_seqs, const int *past, const int *rows) {
     const int group = s.n_heads / s.n_kv_heads, hp = s.head_dim / 64;
-    double all = 0;
-    for (int i = 0; i < n_seqs; i++)
-        if (vt_paged_may_be_many(hp, (long long)rows[i] * group)) {
-            const double seen = past[i] + 0.5 * rows[i];
-            all += (double)rows[i] * group * (s.window && seen > s.window ? s.window : seen) * s.n_kv_heads * s.head_dim;
-        }
-    return all >= PAGED_MANY_FROM;
-}
-
-/* A kernel's part of a batch: `any`, whether there are sequences for the one for many columns.  Calls f(sequence, c0, first row, end) for every tile of columns. */
-template <class F>
-static inline void vt_paged_tiles(const vt_paged_shape &s, bool any, bool many, int n_seqs, const int *past, const int *rows, F f) {
-    const int group = s.n_heads / s.n_kv_heads, wide = many ? PAGED_MANY_COLS : PAGED_FEW_COLS, hp = s.head_dim / 64;
+    double many = 0, wide = 0, wgs = 0;
+    long long most = 0;
     for (int i = 0; i < n_seqs; i++) {
         const long long cols = (long long)rows[i] * group;
-        if ((any && vt_paged_may_be_many(hp, cols)) != many) continue;
+        const double seen = past[i] + 0.5 * rows[i], each = (s.window && seen > s.window ? s.window : seen) * s.n_kv_heads * s.head_dim;
+        if (vt_paged_may_be_many(hp, cols)) many += (double)cols * each;
+    }
+    vt_paged_kinds k = {many >= PAGED_MANY_FROM, 16};
+    for (int i = 0; i < n_seqs; i++) {
+        const long long cols = (long long)rows[i] * group;
+        const double seen = past[i] + 0.5 * rows[i], each = (s.window && seen > s.window ? s.window : seen) * s.n_kv_heads * s.head_dim;
+        if (k.any && vt_paged_may_be_many(hp, cols)) continue;
+        most = cols > most ? cols : most;
+        if (cols > 16) {
+            wide += (double)((cols + 15) / 16) * each;
+            wgs += (double)((cols + 15) / 16) * s.n_kv_heads;
+        }
+    }
+    if (hp <= 2 && most > 16 && wide >= (wgs >= n_cu ? PAGED_WIDE_FULL : PAGED_WIDE_FROM)) k.few_cols = 32;
+    return k;
+}
+
+/* A kernel's part of a batch.  Calls f(sequence, c0, first row, end) for every tile of columns. */
+template <class F>
+static inline void vt_paged_tiles(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_seqs, const int *past, const int *rows, F f) {
+    const int group = s.n_heads / s.n_kv_heads, wide = many ? PAGED_MANY_COLS : kinds.few_cols, hp = s.head_dim / 64;
+    for (int i = 0; i < n_seqs; i++) {
+        const long long cols = (long long)rows[i] * group;
+        if ((kinds.any && vt_paged_may_be_many(hp, cols)) != many) continue;
         for (long long c0 = 0; c0 < cols; c0 += wide) {
             const long long last = (c0 + wide < cols ? c0 + wide : cols) - 1;
             f(i, (int)c0, vt_paged_first(s.window, past[i], (int)(c0 / group)), past[i] + (int)(last / group) + 1);
@@ -145,15 +165,16 @@ static inline int vt_paged_parts(int first, int end, int unit, int run) {
  * the parts that the last one adds; `tail`: the share of the longest that a launch of more than fit at once ends with.  By head_dim / 64; fitted to 25 batches at every run.  The run that
  * these choose is behind the best one by 2 % on average (many columns: 5 %).  us at some of them: 1531 rows behind none, many columns, in runs of 4 / 8 / 12 / 16 / whole (fp32) 76 / 67
  * / 61 / 65 / 72, 4000 of them 502 / 381 / 350 / 343 / 310, 512 behind 1500 62 / 50 / 54 / 51 / 83; few columns: one row behind 1999 in runs of 1 / 2 / 4 / 8 / 16 7.8 / 8.0 / 9.3 / 13 / 20, behind 65535 of 8 /
- * 16 / 32 / 64 47 / 45 / 53 / 96, 37 behind 4000 of 2 / 6 / 12 / 32 31 / 23 / 21 / 42. */
+ * 16 / 32 / 64 47 / 45 / 53 / 96; 200 rows behind 2000, 32 columns, of 4 / 8 / 16 / whole 51 / 44 / 45 / 32. */
 struct vt_paged_cost { int beside; float fixed, alone, step, part, merge, tail; };
 static const vt_paged_cost vt_paged_few_cost[4] = {{4, 1.3f, 0.27f, 0.75f, 1.6f, 0.12f, 0.27f}, {3, 2.3f, 0.58f, 2.4f, 3.1f, 0.12f, 0.2f}, {2, 2.3f, 0.95f, 2.1f, 4.2f, 0.12f, 0.18f}, {2, 2.3f, 1.35f, 1.8f, 5.2f, 0.11f, 0.16f}};
+static const vt_paged_cost vt_paged_wide_cost[2] = {{3, 1.5f, 0.46f, 0.8f, 2.3f, 0.23f, 0.2f}, {2, 1.6f, 0.59f, 0.95f, 4.4f, 0.06f, 0.08f}};
 static const vt_paged_cost vt_paged_many_cost[2] = {{2, 9.1f, 1.94f, 3.3f, 6.0f, 0.9f, 0.54f}, {2, 5.4f, 2.0f, 3.5f, 4.1f, 1.9f, 0.25f}};
 
-static inline int vt_paged_run(const vt_paged_shape &s, bool any, bool many, int n_cu, int n_seqs, const int *past, const int *rows, int unit) {
-    const vt_paged_cost &c = many ? vt_paged_many_cost[s.head_dim / 64 - 1] : vt_paged_few_cost[s.head_dim / 64 - 1];
+static inline int vt_paged_run(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows, int unit) {
+    const vt_paged_cost &c = (many ? vt_paged_many_cost : kinds.few_cols == 32 ? vt_paged_wide_cost : vt_paged_few_cost)[s.head_dim / 64 - 1];
     long long longest = 1;
-    vt_paged_tiles(s, any, many, n_seqs, past, rows, [&](int, int, int first, int end) {
+    vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int, int, int first, int end) {
         const long long n = vt_paged_parts(first, end, unit, 1);
         longest = n > longest ? n : longest;
     });
@@ -163,7 +184,7 @@ static inline int vt_paged_run(const vt_paged_shape &s, bool any, bool many, int
         const int run = (int)((longest + parts - 1) / parts);
         long long items = 0, extra = 0, split = 0, most = 0, all = 0;
         int late = 0;
-        vt_paged_tiles(s, any, many, n_seqs, past, rows, [&](int, int, int first, int end) {
+        vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int, int, int first, int end) {
             const int n = vt_paged_parts(first, end, unit, 1), p = (n + run - 1) / run, each = (n + p - 1) / p;
             items += p;
             all += n;
@@ -192,11 +213,11 @@ static int vt_paged_longest(const void *a, const void *b) {
 }
 
 /* Items of one kernel into `to`, the longest first; -> how many, and their slots */
-static inline int vt_paged_items(const vt_paged_shape &s, bool any, bool many, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to, int *n_slots) {
+static inline int vt_paged_items(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to, int *n_slots) {
     const int unit = many ? PAGED_MANY_ROWS : PAGED_FEW_ROWS * PAGED_FEW_WAVES, group = s.n_heads / s.n_kv_heads;
-    const int run = vt_paged_run(s, any, many, n_cu, n_seqs, past, rows, unit);
+    const int run = vt_paged_run(s, kinds, many, n_cu, n_seqs, past, rows, unit);
     int n = 0, slots = 0, counters = 0, row = 0, seq = 0;
-    vt_paged_tiles(s, any, many, n_seqs, past, rows, [&](int i, int c0, int first, int end) {
+    vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int i, int c0, int first, int end) {
         while (seq < i) row += rows[seq++];
         const int units = vt_paged_parts(first, end, unit, 1), parts = (units + run - 1) / run, u0 = first / unit;
         for (int p = 0; p < parts; p++) {
@@ -213,15 +234,16 @@ static inline int vt_paged_items(const vt_paged_shape &s, bool any, bool many, i
 
 static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to) {
     vt_paged_plan p;
-    const bool any = vt_paged_any_many(s, n_seqs, past, rows);
-    p.few = vt_paged_items(s, any, false, n_cu, n_seqs, past, rows, starts, to, &p.few_slots);
-    p.many = vt_paged_items(s, any, true, n_cu, n_seqs, past, rows, starts, to + p.few, &p.many_slots);
+    const vt_paged_kinds kinds = vt_paged_kinds_of(s, n_cu, n_seqs, past, rows);
+    p.few = vt_paged_items(s, kinds, false, n_cu, n_seqs, past, rows, starts, to, &p.few_slots);
+    p.many = vt_paged_items(s, kinds, true, n_cu, n_seqs, past, rows, starts, to + p.few, &p.many_slots);
     /* Requests that leave nothing behind in the caches: 65535 rows of 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows, which the caches
      * (32 MB of L2) keep for the next call on them, 6.8 -> 7.2. */
     long long read = 0;
-    p.once = 1;
-    vt_paged_tiles(s, any, false, n_seqs, past, rows, [&](int i, int, int first, int end) {
-        if ((long long)rows[i] * (s.n_heads / s.n_kv_heads) > PAGED_FEW_COLS) p.once = 0;
+    p.wide = kinds.few_cols > 16;
+    p.once = !p.wide;
+    vt_paged_tiles(s, kinds, false, n_seqs, past, rows, [&](int i, int, int first, int end) {
+        if ((long long)rows[i] * (s.n_heads / s.n_kv_heads) > 16) p.once = 0;
         read += end - first;
     });
     if (read * 4 * s.n_kv_heads * s.head_dim < PAGED_CACHED) p.once = 0;
