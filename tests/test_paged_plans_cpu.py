@@ -33,6 +33,7 @@ int main(void) {
         std::vector<vt_paged_item> items(vt_paged_max_items(n_seqs, max_rows, group));
         const vt_paged_plan plan = vt_paged_plan_of(s, 256, n_seqs, past.data(), rows.data(), starts.data(), items.data());
         const vt_paged_kinds kinds = vt_paged_kinds_of(s, 256, n_seqs, past.data(), rows.data());
+        if (plan.wide != (kinds.few_cols == 32) || (plan.once && plan.wide)) { bad++; printf("wide %d once %d\n", plan.wide, plan.once); }
         if (plan.few + plan.many > (int)items.size()) { bad++; printf("items %d %d\n", plan.few, plan.many); }
         /* every column's rows are read once, by the parts of one group, in slots of its own */
         std::vector<long long> want(n_seqs), got(n_seqs);

@@ -21,7 +21,8 @@
 #define PAGED_MANY_COLS 128
 #define PAGED_MANY_ROWS 64
 #define PAGED_MAX_PARTS 64
-#define PAGED_CACHED (32ll << 20)
+#define PAGED_CACHED 32e6                  /* bytes: all L2s */
+#define PAGED_NEAR 256e6                   /* the memory-side cache */
 #define PAGED_SPLIT_ITEMS 4096             /* items that a launch may have beyond one for each tile of columns */
 
 /* What a workgroup does for every kv head: columns c0 .. of a sequence whose new rows are `row` .. of the batch and lie behind `past`
@@ -98,8 +99,9 @@ static inline vt_paged_fault vt_paged_lay_out(const vt_paged_shape &s, int max_s
 /* items of either kernel (the few's first), parts that they leave; wide: the few's columns go by 32; once: their rows are read by one workgroup each, more of them than a cache holds */
 struct vt_paged_plan { int few, many, few_slots, many_slots, wide, once; };
 
-/* Which kernels a batch goes to: `any`, whether there are sequences for the one for many columns; columns of a workgroup of the other */
-struct vt_paged_kinds { bool any; int few_cols; };
+/* Which kernels a batch goes to: `any`, whether there are sequences for the one for many columns; columns of a workgroup of the other, whether its rows are read by one
+ * workgroup only, and their bytes */
+struct vt_paged_kinds { bool any; int few_cols; bool once; double bytes; };
 
 static inline long long vt_paged_max_items(int max_seqs, int max_rows, int group) {
     return (long long)max_rows * group / 16 + max_seqs + 2 * PAGED_SPLIT_ITEMS;
@@ -126,18 +128,20 @@ static inline vt_paged_kinds vt_paged_kinds_of(const vt_paged_shape &s, int n_cu
         const double seen = past[i] + 0.5 * rows[i], each = (s.window && seen > s.window ? s.window : seen) * s.n_kv_heads * s.head_dim;
         if (vt_paged_may_be_many(hp, cols)) many += (double)cols * each;
     }
-    vt_paged_kinds k = {many >= PAGED_MANY_FROM, 16};
+    vt_paged_kinds k = {many >= PAGED_MANY_FROM, 16, false, 0};
     for (int i = 0; i < n_seqs; i++) {
         const long long cols = (long long)rows[i] * group;
         const double seen = past[i] + 0.5 * rows[i], each = (s.window && seen > s.window ? s.window : seen) * s.n_kv_heads * s.head_dim;
         if (k.any && vt_paged_may_be_many(hp, cols)) continue;
         most = cols > most ? cols : most;
+        k.bytes += ((double)past[i] + rows[i] - vt_paged_first(s.window, past[i], 0)) * 4 * s.n_kv_heads * s.head_dim;
         if (cols > 16) {
             wide += (double)((cols + 15) / 16) * each;
             wgs += (double)((cols + 15) / 16) * s.n_kv_heads;
         }
     }
     if (hp <= 2 && most > 16 && wide >= (wgs >= n_cu ? PAGED_WIDE_FULL : PAGED_WIDE_FROM)) k.few_cols = 32;
+    k.once = most <= 16;
     return k;
 }
 
@@ -162,17 +166,19 @@ static inline int vt_paged_parts(int first, int end, int unit, int run) {
 }
 
 /* What a workgroup takes: `fixed` us, `step` for a unit of its rows, alone on its CU and with `beside` of them on it, `part` more where it leaves a part, and `merge` for each of
- * the parts that the last one adds; `tail`: the share of the longest that a launch of more than fit at once ends with.  By head_dim / 64; fitted to 25 batches at every run.  The run that
+ * the parts that the last one adds; `tail`: the share of the longest that a launch of more than fit at once ends with.  By head_dim / 64; fitted to 25 to 30 batches at every run.  The run that
  * these choose is behind the best one by 2 % on average (many columns: 5 %).  us at some of them: 1531 rows behind none, many columns, in runs of 4 / 8 / 12 / 16 / whole (fp32) 76 / 67
  * / 61 / 65 / 72, 4000 of them 502 / 381 / 350 / 343 / 310, 512 behind 1500 62 / 50 / 54 / 51 / 83; few columns: one row behind 1999 in runs of 1 / 2 / 4 / 8 / 16 7.8 / 8.0 / 9.3 / 13 / 20, behind 65535 of 8 /
  * 16 / 32 / 64 47 / 45 / 53 / 96; 200 rows behind 2000, 32 columns, of 4 / 8 / 16 / whole 51 / 44 / 45 / 32. */
 struct vt_paged_cost { int beside; float fixed, alone, step, part, merge, tail; };
-static const vt_paged_cost vt_paged_few_cost[4] = {{4, 1.3f, 0.27f, 0.75f, 1.6f, 0.12f, 0.27f}, {3, 2.3f, 0.58f, 2.4f, 3.1f, 0.12f, 0.2f}, {2, 2.3f, 0.95f, 2.1f, 4.2f, 0.12f, 0.18f}, {2, 2.3f, 1.35f, 1.8f, 5.2f, 0.11f, 0.16f}};
+static const vt_paged_cost vt_paged_few_cost[4] = {{4, 2.0f, 0.41f, 2.7f, 1.55f, 0.18f, 0.26f}, {3, 2.8f, 0.98f, 3.5f, 2.1f, 0.13f, 0.09f}, {2, 1.3f, 1.75f, 1.9f, 3.9f, 0.1f, 0.25f}, {2, 2.8f, 2.7f, 5.7f, 9.4f, 0.09f, 0.1f}};
 static const vt_paged_cost vt_paged_wide_cost[2] = {{3, 1.5f, 0.46f, 0.8f, 2.3f, 0.23f, 0.2f}, {2, 1.6f, 0.59f, 0.95f, 4.4f, 0.06f, 0.08f}};
 static const vt_paged_cost vt_paged_many_cost[2] = {{2, 9.1f, 1.94f, 3.3f, 6.0f, 0.9f, 0.54f}, {2, 5.4f, 2.0f, 3.5f, 4.1f, 1.9f, 0.25f}};
 
 static inline int vt_paged_run(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows, int unit) {
-    const vt_paged_cost &c = (many ? vt_paged_many_cost : kinds.few_cols == 32 ? vt_paged_wide_cost : vt_paged_few_cost)[s.head_dim / 64 - 1];
+    vt_paged_cost c = (many ? vt_paged_many_cost : kinds.few_cols == 32 ? vt_paged_wide_cost : vt_paged_few_cost)[s.head_dim / 64 - 1];
+    /* rows that come from memory come as slowly to a workgroup alone: 33 queries behind 4000 rows each, in runs of 4 / 12 / whole 98 / 102 / 132 us */
+    if (!many && kinds.bytes > PAGED_NEAR) c.alone = c.step;
     long long longest = 1;
     vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int, int, int first, int end) {
         const long long n = vt_paged_parts(first, end, unit, 1);
@@ -215,6 +221,8 @@ static int vt_paged_longest(const void *a, const void *b) {
 /* Items of one kernel into `to`, the longest first; -> how many, and their slots */
 static inline int vt_paged_items(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to, int *n_slots) {
     const int unit = many ? PAGED_MANY_ROWS : PAGED_FEW_ROWS * PAGED_FEW_WAVES, group = s.n_heads / s.n_kv_heads;
+    *n_slots = 0;
+    if (many && !kinds.any) return 0;
     const int run = vt_paged_run(s, kinds, many, n_cu, n_seqs, past, rows, unit);
     int n = 0, slots = 0, counters = 0, row = 0, seq = 0;
     vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int i, int c0, int first, int end) {
@@ -233,20 +241,14 @@ static inline int vt_paged_items(const vt_paged_shape &s, const vt_paged_kinds &
 }
 
 static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to) {
-    vt_paged_plan p;
+    vt_paged_plan p = {0, 0, 0, 0, 0, 0};
     const vt_paged_kinds kinds = vt_paged_kinds_of(s, n_cu, n_seqs, past, rows);
     p.few = vt_paged_items(s, kinds, false, n_cu, n_seqs, past, rows, starts, to, &p.few_slots);
     p.many = vt_paged_items(s, kinds, true, n_cu, n_seqs, past, rows, starts, to + p.few, &p.many_slots);
+    p.wide = kinds.few_cols > 16;
     /* Requests that leave nothing behind in the caches: 65535 rows of 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows, which the caches
      * (32 MB of L2) keep for the next call on them, 6.8 -> 7.2. */
-    long long read = 0;
-    p.wide = kinds.few_cols > 16;
-    p.once = !p.wide;
-    vt_paged_tiles(s, kinds, false, n_seqs, past, rows, [&](int i, int, int first, int end) {
-        if ((long long)rows[i] * (s.n_heads / s.n_kv_heads) > 16) p.once = 0;
-        read += end - first;
-    });
-    if (read * 4 * s.n_kv_heads * s.head_dim < PAGED_CACHED) p.once = 0;
+    p.once = kinds.once && kinds.bytes >= PAGED_CACHED;
     return p;
 }
 
