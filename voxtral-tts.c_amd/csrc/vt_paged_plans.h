@@ -6,6 +6,7 @@
 #define VT_PAGED_PLANS_H
 
 #include <limits.h>
+#include <math.h>
 #include <stdint.h>
 #include <stdlib.h>
 
@@ -22,7 +23,6 @@
 #define PAGED_MANY_ROWS 64
 #define PAGED_MAX_PARTS 64
 #define PAGED_CACHED 32e6                  /* bytes: all L2s */
-#define PAGED_NEAR 256e6                   /* the memory-side cache */
 #define PAGED_SPLIT_ITEMS 4096             /* items that a launch may have beyond one for each tile of columns */
 
 /* What a workgroup does for every kv head: columns c0 .. of a sequence whose new rows are `row` .. of the batch and lie behind `past`
@@ -167,18 +167,16 @@ static inline int vt_paged_parts(int first, int end, int unit, int run) {
 
 /* What a workgroup takes: `fixed` us, `step` for a unit of its rows, alone on its CU and with `beside` of them on it, `part` more where it leaves a part, and `merge` for each of
  * the parts that the last one adds; `tail`: the share of the longest that a launch of more than fit at once ends with.  By head_dim / 64; fitted to 25 to 30 batches at every run.  The run that
- * these choose is behind the best one by 2 % on average (many columns: 5 %).  us at some of them: 1531 rows behind none, many columns, in runs of 4 / 8 / 12 / 16 / whole (fp32) 76 / 67
+ * these choose is behind the best one by 1 to 2 % on average, 10 at the worst.  us at some of them: 1531 rows behind none, many columns, in runs of 4 / 8 / 12 / 16 / whole (fp32) 76 / 67
  * / 61 / 65 / 72, 4000 of them 502 / 381 / 350 / 343 / 310, 512 behind 1500 62 / 50 / 54 / 51 / 83; few columns: one row behind 1999 in runs of 1 / 2 / 4 / 8 / 16 7.8 / 8.0 / 9.3 / 13 / 20, behind 65535 of 8 /
  * 16 / 32 / 64 47 / 45 / 53 / 96; 200 rows behind 2000, 32 columns, of 4 / 8 / 16 / whole 51 / 44 / 45 / 32. */
 struct vt_paged_cost { int beside; float fixed, alone, step, part, merge, tail; };
-static const vt_paged_cost vt_paged_few_cost[4] = {{4, 2.0f, 0.41f, 2.7f, 1.55f, 0.18f, 0.26f}, {3, 2.8f, 0.98f, 3.5f, 2.1f, 0.13f, 0.09f}, {2, 1.3f, 1.75f, 1.9f, 3.9f, 0.1f, 0.25f}, {2, 2.8f, 2.7f, 5.7f, 9.4f, 0.09f, 0.1f}};
-static const vt_paged_cost vt_paged_wide_cost[2] = {{3, 1.5f, 0.46f, 0.8f, 2.3f, 0.23f, 0.2f}, {2, 1.6f, 0.59f, 0.95f, 4.4f, 0.06f, 0.08f}};
-static const vt_paged_cost vt_paged_many_cost[2] = {{2, 9.1f, 1.94f, 3.3f, 6.0f, 0.9f, 0.54f}, {2, 5.4f, 2.0f, 3.5f, 4.1f, 1.9f, 0.25f}};
+static const vt_paged_cost vt_paged_few_cost[4] = {{4, 1.1f, 0.8f, 2.55f, 2.85f, 0.35f, 0.37f}, {3, 2.7f, 0.95f, 3.2f, 2.6f, 0.12f, 0.11f}, {2, 1.2f, 1.04f, 1.93f, 1.9f, 0.08f, 0.31f}, {2, 5.1f, 1.2f, 2.8f, 3.9f, 0.07f, 0.29f}};
+static const vt_paged_cost vt_paged_wide_cost[2] = {{3, 1.4f, 0.32f, 0.7f, 2.5f, 0.16f, 0.39f}, {2, 0.85f, 0.42f, 1.09f, 4.85f, 0.07f, 0.08f}};
+static const vt_paged_cost vt_paged_many_cost[2] = {{2, 7.9f, 1.9f, 3.0f, 5.0f, 1.0f, 0.45f}, {2, 9.25f, 2.2f, 3.8f, 3.6f, 2.2f, 0.24f}};
 
 static inline int vt_paged_run(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows, int unit) {
-    vt_paged_cost c = (many ? vt_paged_many_cost : kinds.few_cols == 32 ? vt_paged_wide_cost : vt_paged_few_cost)[s.head_dim / 64 - 1];
-    /* rows that come from memory come as slowly to a workgroup alone: 33 queries behind 4000 rows each, in runs of 4 / 12 / whole 98 / 102 / 132 us */
-    if (!many && kinds.bytes > PAGED_NEAR) c.alone = c.step;
+    const vt_paged_cost &c = (many ? vt_paged_many_cost : kinds.few_cols == 32 ? vt_paged_wide_cost : vt_paged_few_cost)[s.head_dim / 64 - 1];
     long long longest = 1;
     vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int, int, int first, int end) {
         const long long n = vt_paged_parts(first, end, unit, 1);
@@ -199,7 +197,7 @@ static inline int vt_paged_run(const vt_paged_shape &s, const vt_paged_kinds &ki
         });
         if (extra > PAGED_SPLIT_ITEMS || split * s.n_kv_heads > PAGED_COUNTERS) break;
         const double wgs = (double)items * s.n_kv_heads, room = (double)n_cu * c.beside;
-        const double share = wgs < n_cu ? 0.0 : wgs < room ? (wgs - n_cu) / (room - n_cu) : 1.0;
+        const double full = ceil(wgs / n_cu) - 1, share = full < c.beside - 1 ? full / (c.beside - 1) : 1.0;          /* of the CU that has most of them */
         const double one = c.fixed + most * (c.alone + (c.step - c.alone) * share) + late * c.part;
         const double sum = (items * c.fixed + all * c.step + extra * c.part) * s.n_kv_heads / room + (wgs > room ? c.tail * one : 0.0);
         const double us = (one > sum ? one : sum) + (split ? c.merge * parts : 0.0);
