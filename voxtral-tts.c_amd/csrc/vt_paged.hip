@@ -168,16 +168,16 @@ extern "C" int tts_hip_rotary_turns(double *d_turns, int rot_dim, double theta, 
 }
 
 /* ---- heads: norm, turn, store ------------------------------------------------------------------------------------
- * A lane has a unit of four pairs of a head, 2^log lanes a head, and makes the angles once for the HEADS heads that it walks: angles are
- * 160 of the 200 instructions that a unit takes.  (2 p, 2 p + 1) is pair p in both layouts where p does not turn.  Bound by the launch for a few rows, by memory
- * for many. */
+ * A lane has a unit of four pairs of a head, 2^log lanes a head, and makes the angles once for the HEADS heads that it walks: angles are more than half of the instructions that a
+ * unit takes.  (2 p, 2 p + 1) is pair p in both layouts where p does not turn.  Bound by the launch for a few rows (1 to 226 rows of 32 heads 3.8 to 4.1 us a call, 2.5 to 3.8 of them the
+ * kernel's); 1531 rows of 32 heads 7.5 us, 25 MB at 3.3 TB/s. */
 struct turn_job {
     const void *x, *x2;                                  /* K and V for pages */
     void *out, *out2;
     const int *pos, *place;
     const double *turns;
     const float *gain;
-    float magnitude, eps;
+    float magnitude, eps, inv_hd;
     int n, heads, hd, x_stride, out_stride, rot_half;    /* n: rows times sets of heads; rot_half: 2 rot + half */
     int lanes_log;
     vt_divisor sets;                                     /* sets of heads of a row */
@@ -264,6 +264,17 @@ static __device__ __forceinline__ void turn_store(void *out, long long at, int h
     }
 }
 
+/* sum over 2^log lanes that lie together, the same in each of them */
+static __device__ __forceinline__ float turn_sum(float v, int log) {
+    if (log > 0) v += vt_dpp<0xB1>(v);
+    if (log > 1) v += vt_dpp<0x4E>(v);
+    if (log > 2) v += vt_dpp<0x141>(v);
+    if (log > 3) v += vt_dpp<0x140>(v);
+    if (log > 4) { const f32x2 r = vt_swap16(v, v); v = r.x + r.y; }
+    if (log > 5) { const f32x2 r = vt_swap32(v, v); v = r.x + r.y; }
+    return v;
+}
+
 /* PAGES: blockIdx.y 0 turns K into its pages, 1 takes V into its own as it is */
 template <bool BF16, bool WIDE, bool PAGES, int HEADS>
 __global__ void __launch_bounds__(256) vt_turn_kernel(turn_job a) {
@@ -297,13 +308,7 @@ __global__ void __launch_bounds__(256) vt_turn_kernel(turn_job a) {
     float g[4], gb[4];
     const bool norm = a.gain && !values;
     if (norm) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int pr = min(4 * u + e, a.hd / 2 - 1);
-            const bool far = half && 2 * pr < rot;
-            g[e] = a.gain[far ? pr : 2 * pr];
-            gb[e] = a.gain[far ? pr + rot / 2 : 2 * pr + 1];
-        }
+        turn_load<false, WIDE>(a.gain, 0, a.hd, mine ? u : 0, rot, half, g, gb);
     }
     long long to = 0;
     if constexpr (PAGES) {
@@ -318,8 +323,8 @@ __global__ void __launch_bounds__(256) vt_turn_kernel(turn_job a) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) sum = fmaf(q[k][e], q[k][e], fmaf(p[k][e], p[k][e], sum));
             }
-            for (int w = 1; w < G; w *= 2) sum += __shfl_xor(sum, w);
-            const float f = 1.f / sqrtf(sum / (float)a.hd + a.eps);
+            sum = turn_sum(sum, a.lanes_log);
+            const float f = rsqrtf(fmaf(sum, a.inv_hd, a.eps));
 #pragma unroll
             for (int e = 0; e < 4; e++) { p[k][e] = p[k][e] * f * g[e]; q[k][e] = q[k][e] * f * gb[e]; }
         }
@@ -349,7 +354,8 @@ static int turn_ok(const char *who, const tts_hip_rotary_t *how, int head_dim) {
     return 1;
 }
 
-/* heads that a lane walks: one until every CU has eight waves of them (us for 32 heads of 128 fp32 values with 1 / 4: see the launch) */
+/* Heads that a lane walks: two from where every CU has 16 waves of units on (us at one / two / four of them: 1531 rows of 32 heads of 128 bf16 values, normed, 8.8 / 7.5 / 7.6, into pages 1531 rows of
+ * 8 fp32 ones 5.1 / 5.4 / 5.9 and 4000 bf16 ones 8.7 / 7.8 / 7.9). */
 template <bool PAGES>
 static void turn_launch(turn_job &a, int rows, int bf16, int aligned) {
     int log = 0;
@@ -358,8 +364,8 @@ static void turn_launch(turn_job &a, int rows, int bf16, int aligned) {
     const int rot = a.rot_half >> 1, half = a.rot_half & 1;
     const bool wide = aligned && a.hd % 8 == 0 && (!half || rot % 8 == 0);
     const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
-    const bool four = a.heads >= 4 && (((long long)rows * a.heads) << log) > 2048ll * n_cu;
-    const int each = four ? 4 : 1, sets = (a.heads + each - 1) / each, most = (int)((0x7fffffffll >> log) / sets);
+    const bool two = a.heads >= 2 && (((long long)rows * a.heads) << log) > 1024ll * n_cu;
+    const int each = two ? 2 : 1, sets = (a.heads + each - 1) / each, most = (int)((0x7fffffffll >> log) / sets);
     const int all = rows;
     const turn_job whole = a;
     for (int at = 0; at < all; at += most) {             /* rows of a launch: their lanes are counted in 31 bits */
@@ -374,8 +380,8 @@ static void turn_launch(turn_job &a, int rows, int bf16, int aligned) {
         a.sets = vt_divisor_of(sets, (long long)n * sets);
         const dim3 grid((unsigned)((((long long)a.n << log) + 255) / 256), PAGES ? 2 : 1);
 #define TURN(B, W, H) hipLaunchKernelGGL((vt_turn_kernel<B, W, PAGES, H>), grid, dim3(256), 0, g_vt.stream, a)
-        if (bf16) { if (wide) { if (four) TURN(true, true, 4); else TURN(true, true, 1); } else { if (four) TURN(true, false, 4); else TURN(true, false, 1); } }
-        else { if (wide) { if (four) TURN(false, true, 4); else TURN(false, true, 1); } else { if (four) TURN(false, false, 4); else TURN(false, false, 1); } }
+        if (bf16) { if (wide) { if (two) TURN(true, true, 2); else TURN(true, true, 1); } else { if (two) TURN(true, false, 2); else TURN(true, false, 1); } }
+        else { if (wide) { if (two) TURN(false, true, 2); else TURN(false, true, 1); } else { if (two) TURN(false, false, 2); else TURN(false, false, 1); } }
 #undef TURN
     }
 }
@@ -397,9 +403,9 @@ extern "C" int tts_hip_rotary(void *d_out, const void *d_x, int x_bf16, int rows
     if (how->rot_dim && (!d_positions || ((uintptr_t)d_positions & 3))) { vt_set_error("%s: no positions", who); return -1; }
     if (!vt_mx4_ready(who)) return -1;
     if (rows == 0) return 0;
-    turn_job a = {d_x, NULL, d_out, NULL, d_positions, NULL, how->d_turns, how->d_gain, how->magnitude, how->eps, 0, n_heads, head_dim, x_stride, out_stride,
+    turn_job a = {d_x, NULL, d_out, NULL, d_positions, NULL, how->d_turns, how->d_gain, how->magnitude, how->eps, 1.f / head_dim, 0, n_heads, head_dim, x_stride, out_stride,
                   2 * how->rot_dim + how->half, 0, {0, 1}};
-    const int aligned = ((((uintptr_t)d_out | (uintptr_t)d_x) & (4 * size - 1)) | (x_stride & 3) | (out_stride & 3)) == 0;
+    const int aligned = ((((uintptr_t)d_out | (uintptr_t)d_x) & (4 * size - 1)) | (x_stride & 3) | (out_stride & 3) | ((uintptr_t)how->d_gain & 15)) == 0;
     turn_launch<false>(a, rows, x_bf16, aligned);
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
@@ -420,9 +426,9 @@ extern "C" int tts_hip_paged_append(const tts_hip_paged_t *b, void *d_k_pages, v
     if (!vt_paged_ready(who, b)) return -1;
     if (b->n_rows == 0) return 0;
     turn_job a = {d_K, d_V, d_k_pages, d_v_pages, (const int *)b->dev, (const int *)(b->dev + b->at_place), how ? how->d_turns : NULL, how ? how->d_gain : NULL,
-                  how ? how->magnitude : 1.f, how ? how->eps : 0.f, 0, b->shape.n_kv_heads, b->shape.head_dim, stride, b->shape.page_rows,
+                  how ? how->magnitude : 1.f, how ? how->eps : 0.f, 1.f / b->shape.head_dim, 0, b->shape.n_kv_heads, b->shape.head_dim, stride, b->shape.page_rows,
                   how ? 2 * how->rot_dim + how->half : 0, 0, {0, 1}};
-    const int aligned = ((((uintptr_t)d_K | (uintptr_t)d_V) & (4 * size - 1)) | (stride & 3)) == 0;
+    const int aligned = ((((uintptr_t)d_K | (uintptr_t)d_V) & (4 * size - 1)) | (stride & 3) | (how ? (uintptr_t)how->d_gain & 15 : 0)) == 0;
     turn_launch<true>(a, b->n_rows, x_bf16, aligned);
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
