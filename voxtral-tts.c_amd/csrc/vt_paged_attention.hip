@@ -415,6 +415,10 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
  * 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95. */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 
+/* fp32: the compiler keeps to the order that is written, in which an instruction's operands are asked for just ahead of it and no more of them wait in registers than there are; bf16 has
+ * registers for its own order (four prompts in a window 112.0 us as written, 108.8 so) */
+template <bool F32> static __device__ __forceinline__ void pa_here() { if constexpr (F32) __builtin_amdgcn_sched_barrier(0); }
+
 template <int HP, bool F32>
 __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     constexpr int HD = 64 * HP, ROW = 2 * HD, WAVES = 4, DT = 2 * HP, KS = 4 * HP, PIECES = HD / 8;
@@ -482,7 +486,7 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     pa_f32x16 o[DT];
 #pragma unroll
     for (int i = 0; i < DT; i++) o[i] = pa_f32x16{};
-    /* addresses in LDS: one for all of K's pieces and one for all of V's, which differ from them in bits of their own.  (Through an empty asm in each unit: else each piece's, for each
+    /* addresses in LDS: one for all of K's pieces and one for all of V's, which differ from them in bits of their own.  (fp32: through an empty asm in each unit, else each piece's, for each
      * buffer, is kept in a register.) */
     const int k_base = n * ROW + (g ^ (n & SWAP)) * 16, r4 = (n & 15) >> 2;
     const int v_base = (4 * g + r4) * ROW + (v_swap(r4) + 2 * (n >> 4) + ((n & 3) >> 1)) * 16 + (n & 1) * 8;
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
             top = -INFINITY;
         }
         int k_from = k_base, v_from = v_base;
-        asm volatile("" : "+v"(k_from), "+v"(v_from));
+        if constexpr (F32) asm volatile("" : "+v"(k_from), "+v"(v_from));
         u32x4 w4[2][NP];
         auto weigh = [&](int e) __attribute__((always_inline)) {
             const float p0 = pa_weight<F32>(s[2 * e], m, a.scale), p1 = pa_weight<F32>(s[2 * e + 1], m, a.scale);
@@ -580,7 +584,7 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
         u32x4 v[2 * DT];
 #pragma unroll
         for (int ks = 0; ks < AHEAD; ks++) k[ks] = read_k(kb, khalf, ks, k_from);
-        __builtin_amdgcn_sched_barrier(0);
+        pa_here<F32>();
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             const int then = ks + AHEAD;
@@ -593,11 +597,11 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
 #pragma unroll
                 for (int e = EARLY * (ks - BEFORE) / (KS - BEFORE); e < EARLY * (ks - BEFORE + 1) / (KS - BEFORE); e++) weigh(e);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            pa_here<F32>();
         }
         hide(u + 1, next);
         top = next[0];
-        __builtin_amdgcn_sched_barrier(0);
+        pa_here<F32>();
 #pragma unroll
         for (int x = 0; x < 2 * DT; x++) {               /* 16 rows a step: elements 8 st .. of the scores */
             const int st = x / DT, i = x % DT;
@@ -612,7 +616,7 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
 #pragma unroll
                 for (int e = 16 * i / DT; e < 16 * (i + 1) / DT; e += 2) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, next[e]), next[e + 1]);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            pa_here<F32>();
         }
     };
     pa_f32x16 sa, sb;
