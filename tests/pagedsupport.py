@@ -120,7 +120,8 @@ class Cache:
         return np.concatenate([np.arange(p, p + r) for r, p in zip(self.rows, self.past)] or [np.zeros(0)]).astype(np.int32)
 
     def some(self):
-        """Rows of the batch that are compared where it has many: of each sequence the first and last 20, those around its wave and workgroup borders, and some others."""
+        """Rows of the batch that are compared where it has many: of each sequence the first and last 20, those around its wave and workgroup borders, and
+        some others."""
         keep, at = np.zeros(sum(self.rows), bool), 0
         for r in self.rows:
             for edge in (0, 32, 128, r // 2, r):
@@ -130,8 +131,8 @@ class Cache:
         return keep
 
     def attend(self, q, scale, keep=None):
-        """q [rows, heads, head_dim] -> results in 64 bits, the weighted sum of |v|, and the largest sum of |q k| scale that a query meets; NaN where it sees, in
-        that value, a value that is not finite"""
+        """q [rows, heads, head_dim] -> results in 64 bits, the weighted sum of |v|, and the largest sum of |q k| scale that a query meets; NaN where it
+        sees, in that value, a value that is not finite"""
         out, size, most = np.zeros(q.shape), np.zeros(q.shape), 0.0
         at, group = 0, self.heads // self.kv_heads
         for i, (r, p) in enumerate(zip(self.rows, self.past)):
@@ -175,7 +176,8 @@ def attention(cache, q, bf16, scale, q_gap=0):
     x[:, :width] = bits16(q).reshape(rows, -1) if bf16 else q.reshape(rows, -1)
     dq, do = Dev(lib, x), Dev(lib, np.zeros((rows, width), x.dtype), behind=4096)
     try:
-        assert lib.tts_hip_paged_attention(do.ptr, dq.ptr, int(bf16), width + q_gap if q_gap else 0, cache.batch.ptr, cache.dev["k"].ptr, cache.dev["v"].ptr, scale) == 0, lib.tts_hip_last_error()
+        assert lib.tts_hip_paged_attention(do.ptr, dq.ptr, int(bf16), width + q_gap if q_gap else 0, cache.batch.ptr, cache.dev["k"].ptr, cache.dev["v"].ptr,
+                                           scale) == 0, lib.tts_hip_last_error()
         got = do.get()
     finally:
         dq.free()
@@ -193,13 +195,12 @@ def is_many(cache, i):
 
 
 def check(cache, got, want, size, most, bf16, keep=None):
-    """Elementwise by arithmetic, and fp32 by its norm too.
-
-    A score is the sum of 3 head_dim products (1: bf16) of bf16 values, exact, in fp32 that cuts: each of at most 3 head_dim / 8 additions is off by 2^-23 of what is
-    summed so far, which `most` bounds; q times scale and its planes are off by 2^-24 and 2^-25 of it, or a bf16 query's score times scale by 2^-24.  A weight is off by as much, relative to itself, by 2^-22
-    for the difference to the maximum and the exponential, and by the same again through the sum; sums of weights and results add 2^-23 of themselves for
-    each of (row count / 8) steps at the worst, in practice a few.  bf16: a weight's rounding is 2^-8, at most, in the kernel for many columns, and 2^-16 in the other; a result's 2^-8.
-    By norm: errors of single scores are independent, sqrt(3 head_dim / 16) 2^-24 times a few: 5e-7."""
+    """Elementwise by arithmetic, and fp32 by its norm too.  A score is the sum of 3 head_dim products (1: bf16) of bf16 values, exact, in fp32 that cuts:
+    each of at most 3 head_dim / 8 additions is off by 2^-23 of what is summed so far, which `most` bounds; q times scale and its planes are off by 2^-24
+    and 2^-25 of it, or a bf16 query's score times scale by 2^-24.  A weight is off by as much, relative to itself, by 2^-22 for the difference to the
+    maximum and the exponential, and by the same again through the sum; sums of weights and results add 2^-23 of themselves for each of (row count / 8)
+    steps at the worst, in practice a few.  bf16: a weight's rounding is 2^-8, at most, in the kernel for many columns, and 2^-16 in the other; a result's
+    2^-8.  By norm: errors of single scores are independent, sqrt(3 head_dim / 16) 2^-24 times a few: 5e-7."""
     score = (3 * cache.hd / 8 + 3) * 2.0 ** -23 * most
     rel = np.full(got.shape[0], 2 * score + 64 * 2.0 ** -23)
     if bf16:

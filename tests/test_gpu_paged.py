@@ -27,7 +27,9 @@ def normal(rng, shape, bf16):
 
 # ---- rotary positions --------------------------------------------------------------------------
 
-@pytest.mark.parametrize("rot,theta,factor,original,low,high", [(128, 1e6, 1.0, 0, 1, 32), (64, 1e4, 8.0, 8192, 1, 32), (2, 5e5, 4.0, 0, 1, 2), (512, 1e6, 32.0, 131072, 0.5, 64), (26, 10.0, 0.5, 100, -3, 3)])
+@pytest.mark.parametrize("rot,theta,factor,original,low,high",
+                         [(128, 1e6, 1.0, 0, 1, 32), (64, 1e4, 8.0, 8192, 1, 32), (2, 5e5, 4.0, 0, 1, 2), (512, 1e6, 32.0, 131072, 0.5, 64),
+                          (26, 10.0, 0.5, 100, -3, 3)])
 def test_turns(hip, rot, theta, factor, original, low, high):
     d = P.Dev(hip.lib, np.zeros(rot // 2), behind=64)
     assert hip.lib.tts_hip_rotary_turns(d.ptr, rot, theta, factor, original, low, high) == 0
@@ -37,9 +39,9 @@ def test_turns(hip, rot, theta, factor, original, low, high):
 
 ROTARY = [  # rows, heads, head_dim, rot, half, norm, gaps (out, x), shift (values from a multiple of 16 bytes)
     (1, 32, 128, 128, 0, False, (0, 0), 0), (37, 32, 128, 128, 1, True, (0, 2048), 0), (3, 6, 128, 64, 0, True, (4, 8), 0), (5, 3, 64, 32, 1, False, (0, 0), 0),
-    (2, 5, 192, 192, 1, True, (0, 0), 0), (9, 7, 256, 128, 0, True, (0, 0), 0), (4, 2, 512, 512, 1, True, (0, 0), 0), (6, 3, 96, 52, 1, True, (0, 0), 0), (6, 3, 96, 52, 0, False, (0, 0), 0),
-    (3, 1, 2, 2, 1, True, (0, 0), 0), (3, 4, 10, 6, 1, False, (1, 3), 1), (70, 5, 80, 80, 1, True, (0, 0), 1), (4, 9, 128, 0, 0, True, (0, 0), 0), (300, 64, 128, 128, 1, True, (0, 0), 0),
-    (1100, 33, 64, 64, 0, False, (64, 0), 0),
+    (2, 5, 192, 192, 1, True, (0, 0), 0), (9, 7, 256, 128, 0, True, (0, 0), 0), (4, 2, 512, 512, 1, True, (0, 0), 0), (6, 3, 96, 52, 1, True, (0, 0), 0),
+    (6, 3, 96, 52, 0, False, (0, 0), 0), (3, 1, 2, 2, 1, True, (0, 0), 0), (3, 4, 10, 6, 1, False, (1, 3), 1), (70, 5, 80, 80, 1, True, (0, 0), 1),
+    (4, 9, 128, 0, 0, True, (0, 0), 0), (300, 64, 128, 128, 1, True, (0, 0), 0), (1100, 33, 64, 64, 0, False, (64, 0), 0),
 ]
 
 
@@ -60,17 +62,20 @@ def test_rotary(hip, rows, heads, hd, rot, half, norm, gaps, shift, bf16):
     raw = np.zeros(wide.size + shift, wide.dtype)
     raw[shift:] = wide.ravel()
     old = np.full(rows * (width + gaps[0]) + shift, 77, wide.dtype)
-    dx, do, dt, dg, dp = P.Dev(hip.lib, raw), P.Dev(hip.lib, old, behind=256), P.Dev(hip.lib, np.concatenate((t, [np.nan]))), P.Dev(hip.lib, gain), P.Dev(hip.lib, pos)
+    dx, do, dt = P.Dev(hip.lib, raw), P.Dev(hip.lib, old, behind=256), P.Dev(hip.lib, np.concatenate((t, [np.nan])))
+    dg, dp = P.Dev(hip.lib, gain), P.Dev(hip.lib, pos)
     how = P.how(hip, dt.ptr if rot else None, rot, half, dg.ptr if norm else None, 1e-5, 1.25)
     args = (bf16, rows, heads, hd)
-    assert hip.lib.tts_hip_rotary(do.ptr + shift * size, dx.ptr + shift * size, *args, width + gaps[0] if gaps[0] else 0, width + gaps[1] if gaps[1] else 0, dp.ptr if rot else None, how) == 0, hip.lib.tts_hip_last_error()
+    assert hip.lib.tts_hip_rotary(do.ptr + shift * size, dx.ptr + shift * size, *args, width + gaps[0] if gaps[0] else 0, width + gaps[1] if gaps[1] else 0,
+                                  dp.ptr if rot else None, how) == 0, hip.lib.tts_hip_last_error()
     out = do.get()
     assert (out[:shift] == 77).all()
     out = out[shift:].reshape(rows, -1)
     assert (out[:, width:] == 77).all()                                                             # the room between rows
     got = (P.value16(out[:, :width]) if bf16 else out[:, :width]).reshape(x.shape).astype(np.float64)
     want, both = P.turned(x, pos, t, half, gain if norm else None, 1e-5, 1.25)
-    # cosine and sine to 2 ulp of 1 and the rest of the angle to 2^-24 of a step, two products and a sum, times the magnitude: 2^-23 each; a norm adds the sum of head_dim / 8 squares and five operations
+    # cosine and sine to 2 ulp of 1 and the rest of the angle to 2^-24 of a step, two products and a sum, times the magnitude: 2^-23 each; a norm adds the sum of
+    # head_dim / 8 squares and five operations
     rel = 8 * 2.0 ** -23 + ((hd / 8 + 8) * 2.0 ** -24 if norm else 0)
     tol = rel * both + (2.0 ** -8 * (np.abs(want) + rel * both) if bf16 else 0)
     assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / np.maximum(tol, 1e-300)).max())
@@ -104,7 +109,8 @@ def test_rotary_agrees_with_apply_rope(hip):
 @pytest.mark.parametrize("bf16", [0, 1])
 @pytest.mark.parametrize("layout,batch,page,rot,half,norm,gap", [
     ((32, 8, 128), "1@301", 16, 128, 0, False, 0), ((32, 8, 128), "37@5 1@16 0@3 1@15 20@0", 16, 128, 1, True, 4096), ((16, 16, 64), "300@40", 64, 32, 0, True, 0),
-    ((6, 2, 192), "33@31 1@0", 32, 190, 1, False, 3), ((12, 4, 256), "5@250 100@0", 256, 256, 1, True, 8), ((14, 2, 64), "17@100", 1024, None, 0, False, 0), ((32, 8, 128), "700@9 400@0", 16, 128, 0, True, 0)])
+    ((6, 2, 192), "33@31 1@0", 32, 190, 1, False, 3), ((12, 4, 256), "5@250 100@0", 256, 256, 1, True, 8), ((14, 2, 64), "17@100", 1024, None, 0, False, 0),
+    ((32, 8, 128), "700@9 400@0", 16, 128, 0, True, 0)])
 def test_append(hip, layout, batch, page, rot, half, norm, gap, bf16):
     heads, kv, hd = layout
     c = P.Cache(hip, batch, page, heads, kv, hd, seed=3)
@@ -119,7 +125,8 @@ def test_append(hip, layout, batch, page, rot, half, norm, gap, bf16):
     t = P.turns(rot, 1e6) if rot else np.zeros(0)
     dk, dv, dt, dg = (P.Dev(hip.lib, a) for a in (*wide, t, gain))
     how = None if rot is None else P.how(hip, dt.ptr, rot, half, dg.ptr if norm else None)
-    assert hip.lib.tts_hip_paged_append(c.batch.ptr, c.dev["k"].ptr, c.dev["v"].ptr, dk.ptr, dv.ptr, bf16, width + gap if gap else 0, how) == 0, hip.lib.tts_hip_last_error()
+    assert hip.lib.tts_hip_paged_append(c.batch.ptr, c.dev["k"].ptr, c.dev["v"].ptr, dk.ptr, dv.ptr, bf16, width + gap if gap else 0,
+                                        how) == 0, hip.lib.tts_hip_last_error()
     got_k, got_v = c.download()
     pos = c.positions()
     pages = np.concatenate([c.tables[i][np.arange(p, p + r) // page] for i, (r, p) in enumerate(zip(c.rows, c.past))])
@@ -162,12 +169,13 @@ def test_attention(hip, batch, page, window, layout, bf16):
 
 
 MANY = [  # layout, batch, page, window: enough for the kernel for many columns
-    ((32, 8, 128), "1300@0 3@50", 16, 0), ((32, 8, 128), "130@500 1@700 64@64 0@9 900@450", 64, 0), ((32, 8, 128), "7000@0", 16, 90), ((32, 8, 128), "37@9000 100@4000", 32, 0),
-    ((16, 16, 64), "333@3700 900@1100 1@40 700@0", 256, 0), ((16, 16, 64), "65@36000 300@2000", 16, 0), ((8, 1, 128), "300@9000", 16, 0), ((8, 1, 128), "5300@100 17@800", 32, 500), ((8, 1, 128), "10000@33", 64, 260),
-    ((14, 2, 64), "2000@800", 1024, 0), ((20, 1, 64), "1500@733 9@9", 16, 0)]
+    ((32, 8, 128), "1300@0 3@50", 16, 0), ((32, 8, 128), "130@500 1@700 64@64 0@9 900@450", 64, 0), ((32, 8, 128), "7000@0", 16, 90),
+    ((32, 8, 128), "37@9000 100@4000", 32, 0), ((16, 16, 64), "333@3700 900@1100 1@40 700@0", 256, 0), ((16, 16, 64), "65@36000 300@2000", 16, 0),
+    ((8, 1, 128), "300@9000", 16, 0), ((8, 1, 128), "5300@100 17@800", 32, 500), ((8, 1, 128), "10000@33", 64, 260), ((14, 2, 64), "2000@800", 1024, 0),
+    ((20, 1, 64), "1500@733 9@9", 16, 0)]
 WIDE = [  # enough for 32 columns at a time
-    ((32, 8, 128), "37@5100 1@300", 16, 0), ((32, 8, 128), "300@700 5@5 0@1", 64, 650), ((32, 8, 128), "90@1111 7@2000", 32, 1000), ((16, 16, 64), "512@1500", 16, 0), ((20, 1, 64), "100@4000 2@9000", 256, 0),
-    ((8, 1, 128), "70@9999", 16, 0)]
+    ((32, 8, 128), "37@5100 1@300", 16, 0), ((32, 8, 128), "300@700 5@5 0@1", 64, 650), ((32, 8, 128), "90@1111 7@2000", 32, 1000),
+    ((16, 16, 64), "512@1500", 16, 0), ((20, 1, 64), "100@4000 2@9000", 256, 0), ((8, 1, 128), "70@9999", 16, 0)]
 
 
 def large(hip, layout, batch, page, window, bf16, scale=None, size=1.0):
@@ -199,11 +207,25 @@ def test_attention_of_32_columns_at_a_time(hip, layout, batch, page, window, bf1
 
 
 @pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("layout,batch,page,window", [((4096, 1, 64), "1@40 2@9", 16, 0), ((1, 1, 256), "300@5 1@2", 1 << 20, 0), ((100, 1, 128), "3@100", 64, 17),
+                                                      ((7, 7, 192), "20@0", 16, 0)])
+def test_attention_of_other_layouts(hip, layout, batch, page, window, bf16):
+    test_attention(hip, batch, page, window, layout, bf16)
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("layout,n,apart,window", [((24, 3, 64), 200, 1, 0), ((8, 2, 128), 300, 11, 2000)])
+def test_attention_of_many_sequences(hip, layout, n, apart, window, bf16):
+    test_attention(hip, " ".join(f"1@{apart * i}" for i in range(n)), 16, window, layout, bf16)
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
 @pytest.mark.parametrize("layout", [(8, 2, 128), (6, 2, 192), (16, 2, 64)])
-@pytest.mark.parametrize("batch,window", [("40@100", 0), ("9@7", 0), ("40@100 1@200", 30), ("300@10", 40), ("200@3000", 0), ("2000@800", 0), ("7500@10", 300), ("3700@0 1@500", 600), ("25000@0", 100)])
+@pytest.mark.parametrize("batch,window", [("40@100", 0), ("9@7", 0), ("40@100 1@200", 30), ("300@10", 40), ("200@3000", 0), ("2000@800", 0), ("7500@10", 300),
+                                          ("3700@0 1@500", 600), ("25000@0", 100)])
 def test_what_a_query_does_not_see_changes_nothing(hip, batch, window, layout, bf16):
-    """Infinities and NaN in keys and values: who sees a key's NaN answers NaN, who sees a value's in that value; nobody else notices.  Who sees a key's infinity answers NaN
-    where its score is +infinity or no number, and may where it is -infinity, a weight of 0."""
+    """Infinities and NaN in keys and values: who sees a key's NaN answers NaN, who sees a value's in that value; nobody else notices.  Who sees a key's
+    infinity answers NaN where its score is +infinity or no number, and may where it is -infinity, a weight of 0."""
     c = P.Cache(hip, batch, 16, *layout, window=window, seed=1)
     c.fill()
     rows, past = c.rows[0], c.past[0]
@@ -288,6 +310,25 @@ def test_pages_behind_4_gib(hip):
     c.free()
 
 
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_more_items_than_a_grid_has(hip, bf16):
+    """Tiles of columns past 65535, the most that a grid's second dimension has: the rows around that place."""
+    heads, hd, rows, w = 4, 256, 262144 + 600, 3                  # four columns a row, 16 to a tile
+    c = P.Cache(hip, f"{rows}@0", 1 << 14, heads, 1, hd, window=w, seed=5, spare=0)
+    c.fill(size=0.5)
+    c.upload()
+    rng = np.random.default_rng(12)
+    block = normal(rng, (4096, heads, hd), bf16)
+    q = np.tile(block, (-(-rows // 4096), 1, 1))[:rows]
+    got = P.attention(c, q, bf16, 0.0625)
+    keep = np.zeros(rows, bool)
+    for at in (0, 262140, rows):
+        keep[max(0, at - 100):at + 100] = True
+    assert np.isfinite(got).all()
+    assert P.check(c, got, *c.attend(q, 0.0625, keep), bf16, keep)
+    c.free()
+
+
 def test_an_empty_batch_does_nothing(hip):
     c = P.Cache(hip, "0@5 0@0", 16, 8, 2, 64, seed=4)
     c.upload()
@@ -316,8 +357,8 @@ def test_a_refused_batch_leaves_none(hip):
 
 @pytest.mark.parametrize("bf16", [0, 1])
 def test_prompts_and_steps_as_a_program_runs_them(hip, bf16):
-    """A layer's attention of three utterances: prompts in chunks, then steps of all of them, from one matrix q|k|v, on one handle.  Each step's cache and results against 64
-    bits, from the cache that the library wrote."""
+    """A layer's attention of three utterances: prompts in chunks, then steps of all of them, from one matrix q|k|v, on one handle.  Each step's cache and
+    results against 64 bits, from the cache that the library wrote."""
     heads, kv, hd, page = 8, 2, 128, 16
     width, rng, lib = (heads + 2 * kv) * hd, np.random.default_rng(11), hip.lib
     c = P.Cache(hip, "90@0 70@0 8@0", page, heads, kv, hd, seed=6)
@@ -346,7 +387,8 @@ def test_prompts_and_steps_as_a_program_runs_them(hip, bf16):
         pos = c.positions()
         pages = np.concatenate([c.tables[i][np.arange(p, p + r) // page] for i, (r, p) in enumerate(zip(rows, past))])
         k = x[:, heads * hd:(heads + kv) * hd].reshape(-1, kv, hd)
-        for new, old, g in ((P.value16(np.ascontiguousarray(k_bits[pages, :, pos % page])), k, gain[1]), (q.reshape(-1, heads, hd), x[:, :heads * hd].reshape(-1, heads, hd), gain[0])):
+        for new, old, g in ((P.value16(np.ascontiguousarray(k_bits[pages, :, pos % page])), k, gain[1]),
+                            (q.reshape(-1, heads, hd), x[:, :heads * hd].reshape(-1, heads, hd), gain[0])):
             want, both = P.turned(old, pos, t, 1, g, 1e-5)
             rel = 8 * 2.0 ** -23 + (hd / 8 + 8) * 2.0 ** -24
             rounded = bf16 or new.shape[1] == kv

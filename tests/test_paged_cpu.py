@@ -38,13 +38,16 @@ def batch():
     pkg.lib().tts_hip_paged_free(b)
 
 
-@pytest.mark.parametrize("other", [{"n_pages": 0}, {"page_rows": 8}, {"page_rows": 48}, {"page_rows": 1 << 21}, {"page_rows": -16}, {"n_kv_heads": 0}, {"n_heads": 33}, {"n_heads": 0}, {"n_heads": -32},
-                                   {"head_dim": 32}, {"head_dim": 96}, {"head_dim": 320}, {"window": -1}, {"n_heads": 4097, "n_kv_heads": 1}, {"n_heads": 1 << 17, "n_kv_heads": 1 << 17}])
+@pytest.mark.parametrize("other", [{"n_pages": 0}, {"page_rows": 8}, {"page_rows": 48}, {"page_rows": 1 << 21}, {"page_rows": -16}, {"n_kv_heads": 0},
+                                   {"n_heads": 33}, {"n_heads": 0}, {"n_heads": -32},
+                                   {"head_dim": 32}, {"head_dim": 96}, {"head_dim": 320}, {"window": -1}, {"n_heads": 4097, "n_kv_heads": 1},
+                                   {"n_heads": 1 << 17, "n_kv_heads": 1 << 17}])
 def test_create_refuses_a_shape(other):
     refused("tts_hip_paged_create", shape(**other), 3, 64, 10, answer=None)
 
 
-@pytest.mark.parametrize("seqs,rows,table", [(0, 64, 10), (3, 0, 10), (3, 64, 0), (-1, 64, 10), (3, (1 << 22) + 1, 10), ((1 << 22) + 1, 64, 10), (3, 64, (1 << 28) + 1)])
+@pytest.mark.parametrize("seqs,rows,table", [(0, 64, 10), (3, 0, 10), (3, 64, 0), (-1, 64, 10), (3, (1 << 22) + 1, 10), ((1 << 22) + 1, 64, 10),
+                                             (3, 64, (1 << 28) + 1)])
 def test_create_refuses_sizes(seqs, rows, table):
     refused("tts_hip_paged_create", shape(), seqs, rows, table, answer=None)
 
@@ -59,9 +62,11 @@ def ints(*v):
 
 
 @pytest.mark.parametrize("n,past,rows,tables,stride,why", [
-    (-1, (0,), (1,), (1,), 1, "sequences"), (4, (0,) * 4, (1,) * 4, (1, 2, 3, 4), 1, "sequences"), (1, (0,), (1,), (1,), -1, "sequences"), (1, (-1,), (1,), (1,), 1, "rows behind"),
-    (1, (0,), (-1,), (1,), 1, "rows behind"), (1, (1 << 30,), (1,), (1,), 1, "rows behind"), (1, (0,), (65,), (1, 2, 3, 4, 5), 5, "new rows"), (1, (16,), (1,), (1,), 1, "pages"),
-    (2, (95, 95), (1, 1), tuple(range(6)) + (0, 1, 2, 3, 4, 6), 6, "pages"), (1, (0,), (1,), (10,), 1, "page 0"), (1, (16,), (1,), (-1, 2), 2, "page 0"), (2, (3, 7), (1, 1), (4, 4), 1, "twice")])
+    (-1, (0,), (1,), (1,), 1, "sequences"), (4, (0,) * 4, (1,) * 4, (1, 2, 3, 4), 1, "sequences"), (1, (0,), (1,), (1,), -1, "sequences"),
+    (1, (-1,), (1,), (1,), 1, "rows behind"), (1, (0,), (-1,), (1,), 1, "rows behind"), (1, (1 << 30,), (1,), (1,), 1, "rows behind"),
+    (1, (0,), (65,), (1, 2, 3, 4, 5), 5, "new rows"), (1, (16,), (1,), (1,), 1, "pages"),
+    (2, (95, 95), (1, 1), tuple(range(6)) + (0, 1, 2, 3, 4, 6), 6, "pages"), (1, (0,), (1,), (10,), 1, "page 0"), (1, (16,), (1,), (-1, 2), 2, "page 0"),
+    (2, (3, 7), (1, 1), (4, 4), 1, "twice")])
 def test_set_refuses(batch, n, past, rows, tables, stride, why):
     past, rows, tables = ints(*past), ints(*rows), ints(*tables)
     assert why in refused("tts_hip_paged_set", batch, n, past.ctypes.data, rows.ctypes.data, tables.ctypes.data, stride)
@@ -83,8 +88,10 @@ def test_a_batch_needs_a_context(batch):
     lib.tts_hip_paged_free(None)
 
 
-@pytest.mark.parametrize("rot,theta,factor,original,low,high", [(0, 1e6, 1, 0, 1, 32), (3, 1e6, 1, 0, 1, 32), (514, 1e6, 1, 0, 1, 32), (64, 0, 1, 0, 1, 32), (64, NAN, 1, 0, 1, 32), (64, INF, 1, 0, 1, 32), (64, 1e6, 0, 0, 1, 32),
-                                                                  (64, 1e6, -2, 0, 1, 32), (64, 1e6, 1, -1, 1, 32), (64, 1e6, 1, 0, 2, 2), (64, 1e6, 1, 0, NAN, 2), (64, 1e6, 1, 0, 1, INF)])
+@pytest.mark.parametrize("rot,theta,factor,original,low,high",
+                         [(0, 1e6, 1, 0, 1, 32), (3, 1e6, 1, 0, 1, 32), (514, 1e6, 1, 0, 1, 32), (64, 0, 1, 0, 1, 32), (64, NAN, 1, 0, 1, 32),
+                          (64, INF, 1, 0, 1, 32), (64, 1e6, 0, 0, 1, 32), (64, 1e6, -2, 0, 1, 32), (64, 1e6, 1, -1, 1, 32), (64, 1e6, 1, 0, 2, 2),
+                          (64, 1e6, 1, 0, NAN, 2), (64, 1e6, 1, 0, 1, INF)])
 def test_turns_refuses(rot, theta, factor, original, low, high):
     refused("tts_hip_rotary_turns", P, rot, theta, factor, original, low, high)
 
@@ -101,7 +108,8 @@ def how(**other):
     return C.byref(h)
 
 
-BAD_TURNS = [{"rot_dim": -2}, {"rot_dim": 3}, {"rot_dim": 130}, {"half": 2}, {"half": -1}, {"d_turns": None}, {"d_turns": P + 4}, {"magnitude": NAN}, {"magnitude": INF}, {"d_gain": P + 2}, {"d_gain": P, "eps": -1.0}, {"d_gain": P, "eps": NAN}]
+BAD_TURNS = [{"rot_dim": -2}, {"rot_dim": 3}, {"rot_dim": 130}, {"half": 2}, {"half": -1}, {"d_turns": None}, {"d_turns": P + 4}, {"magnitude": NAN},
+             {"magnitude": INF}, {"d_gain": P + 2}, {"d_gain": P, "eps": -1.0}, {"d_gain": P, "eps": NAN}]
 
 
 @pytest.mark.parametrize("other", BAD_TURNS)
@@ -110,23 +118,29 @@ def test_bad_turns_are_refused(batch, other):
     refused("tts_hip_paged_append", batch, P, Q, R, S, 0, 0, how(**other))
 
 
-@pytest.mark.parametrize("args", [(None, Q, 0, 1, 32, 128, 0, 0, R), (P, None, 0, 1, 32, 128, 0, 0, R), (P + 2, Q, 0, 1, 32, 128, 0, 0, R), (P, Q + 1, 1, 1, 32, 128, 0, 0, R), (P, Q, 0, -1, 32, 128, 0, 0, R), (P, Q, 0, 1, 0, 128, 0, 0, R),
-                                  (P, Q, 0, 1, 32, 0, 0, 0, R), (P, Q, 0, 1, 32, 129, 0, 0, R), (P, Q, 0, 1, 32, 514, 0, 0, R), (P, Q, 0, 1, 32, 128, 4095, 0, R), (P, Q, 0, 1, 32, 128, 0, 4095, R), (P, Q, 0, 1, 32, 128, 0, -4096, R),
-                                  (P, Q, 0, 1, 32, 128, 0, 0, None), (P, Q, 0, 1, 32, 128, 0, 0, R + 2), (P, Q, 0, (1 << 30) + 1, 32, 128, 0, 0, R), (P, Q, 0, 1, 1 << 23, 128, 0, 0, R)])
+@pytest.mark.parametrize("args", [(None, Q, 0, 1, 32, 128, 0, 0, R), (P, None, 0, 1, 32, 128, 0, 0, R), (P + 2, Q, 0, 1, 32, 128, 0, 0, R),
+                                  (P, Q + 1, 1, 1, 32, 128, 0, 0, R), (P, Q, 0, -1, 32, 128, 0, 0, R), (P, Q, 0, 1, 0, 128, 0, 0, R),
+                                  (P, Q, 0, 1, 32, 0, 0, 0, R), (P, Q, 0, 1, 32, 129, 0, 0, R), (P, Q, 0, 1, 32, 514, 0, 0, R),
+                                  (P, Q, 0, 1, 32, 128, 4095, 0, R), (P, Q, 0, 1, 32, 128, 0, 4095, R), (P, Q, 0, 1, 32, 128, 0, -4096, R),
+                                  (P, Q, 0, 1, 32, 128, 0, 0, None), (P, Q, 0, 1, 32, 128, 0, 0, R + 2), (P, Q, 0, (1 << 30) + 1, 32, 128, 0, 0, R),
+                                  (P, Q, 0, 1, 1 << 23, 128, 0, 0, R)])
 def test_rotary_refuses(args):
     refused("tts_hip_rotary", *args, how())
     refused("tts_hip_rotary", P, Q, 0, 1, 32, 128, 0, 0, R, None)
 
 
-@pytest.mark.parametrize("args", [(None, Q, R, S, 0, 0), (P, None, R, S, 0, 0), (P, Q, None, S, 0, 0), (P, Q, R, None, 0, 0), (P + 8, Q, R, S, 0, 0), (P, Q + 2, R, S, 0, 0), (P, Q, R + 2, S, 0, 0), (P, Q, R, S + 1, 1, 0),
+@pytest.mark.parametrize("args", [(None, Q, R, S, 0, 0), (P, None, R, S, 0, 0), (P, Q, None, S, 0, 0), (P, Q, R, None, 0, 0), (P + 8, Q, R, S, 0, 0),
+                                  (P, Q + 2, R, S, 0, 0), (P, Q, R + 2, S, 0, 0), (P, Q, R, S + 1, 1, 0),
                                   (P, Q, R, S, 0, 1023), (P, Q, R, S, 0, -1024)])
 def test_append_refuses(batch, args):
     refused("tts_hip_paged_append", batch, *args, None)
     refused("tts_hip_paged_append", None, P, Q, R, S, 0, 0, None)
 
 
-@pytest.mark.parametrize("out,q,stride,k,v,scale", [(None, Q, 0, R, S, 1.0), (P, None, 0, R, S, 1.0), (P, Q, 0, None, S, 1.0), (P, Q, 0, R, None, 1.0), (P + 8, Q, 0, R, S, 1.0), (P, Q + 4, 0, R, S, 1.0), (P, Q, 0, R + 8, S, 1.0),
-                                                    (P, Q, 4095, R, S, 1.0), (P, Q, 4100, R, S, 1.0), (P, Q, 0, R, S, 0.0), (P, Q, 0, R, S, -1.0), (P, Q, 0, R, S, NAN), (P, Q, 0, R, S, INF)])
+@pytest.mark.parametrize("out,q,stride,k,v,scale", [(None, Q, 0, R, S, 1.0), (P, None, 0, R, S, 1.0), (P, Q, 0, None, S, 1.0), (P, Q, 0, R, None, 1.0),
+                                                    (P + 8, Q, 0, R, S, 1.0), (P, Q + 4, 0, R, S, 1.0), (P, Q, 0, R + 8, S, 1.0),
+                                                    (P, Q, 4095, R, S, 1.0), (P, Q, 4100, R, S, 1.0), (P, Q, 0, R, S, 0.0), (P, Q, 0, R, S, -1.0),
+                                                    (P, Q, 0, R, S, NAN), (P, Q, 0, R, S, INF)])
 def test_attention_refuses(batch, out, q, stride, k, v, scale):
     refused("tts_hip_paged_attention", out, q, 0, stride, batch, k, v, scale)
     refused("tts_hip_paged_attention", P, Q, 0, 0, None, R, S, 1.0)

@@ -28,7 +28,8 @@ int main(void) {
         for (size_t i = 0; i < tables.size(); i++) tables[i] = (int)i % s.n_pages;
         int n_rows = 0, n_table = 0;
         vt_paged_rows to = {pos.data(), place.data(), out.data(), starts.data(), written.data()};
-        const vt_paged_fault f = vt_paged_lay_out(s, n_seqs, max_rows, n_seqs * pages, n_seqs, past.data(), rows.data(), tables.data(), pages, to, &n_rows, &n_table);
+        const vt_paged_fault f = vt_paged_lay_out(s, n_seqs, max_rows, n_seqs * pages, n_seqs, past.data(), rows.data(), tables.data(), pages, to, &n_rows,
+                                                  &n_table);
         if (vt_paged_shape_bad(s) || f.what) { bad++; printf("refused %d\n", f.what); continue; }
         std::vector<vt_paged_item> items(vt_paged_max_items(n_seqs, max_rows, group));
         const vt_paged_plan plan = vt_paged_plan_of(s, 256, n_seqs, past.data(), rows.data(), starts.data(), items.data());
@@ -38,7 +39,8 @@ int main(void) {
         /* every column's rows are read once, by the parts of one group, in slots of its own */
         std::vector<long long> want(n_seqs), got(n_seqs);
         for (int k = 0; k < 2; k++) {
-            const int from = k ? plan.few : 0, n = k ? plan.many : plan.few, cols = k ? PAGED_MANY_COLS : kinds.few_cols, unit = k ? 64 : 32, n_slots = k ? plan.many_slots : plan.few_slots;
+            const int from = k ? plan.few : 0, n = k ? plan.many : plan.few, cols = k ? PAGED_MANY_COLS : kinds.few_cols;
+            const int unit = k ? 64 : 32, n_slots = k ? plan.many_slots : plan.few_slots;
             std::vector<char> slot(n_slots);
             std::vector<int> left(PAGED_COUNTERS);
             for (int j = from; j < from + n; j++) {
@@ -48,10 +50,14 @@ int main(void) {
                 if (i == n_seqs || it.cols != rows[i] * group || it.table != starts[i]) { bad++; printf("no sequence\n"); break; }
                 const int c1 = it.c0 + cols < it.cols ? it.c0 + cols : it.cols, q0 = it.c0 / group, q1 = (c1 - 1) / group;
                 const int first = s.window && past[i] + q0 >= s.window ? past[i] + q0 - s.window + 1 : 0, end = past[i] + q1 + 1;
-                const bool wrong = it.c0 % cols || it.c0 >= it.cols || it.lo < first || it.end > end || it.lo >= it.end || (it.lo % unit && it.lo != first) || (it.end % unit && it.end != end) ||
-                                   it.parts < 1 || it.parts > PAGED_MAX_PARTS || it.part < 0 || it.part >= it.parts || (it.part == 0 && it.lo != first) || (it.part == it.parts - 1 && it.end != end) ||
-                                   it.end - 1 >= past[i] + rows[i] || (it.end - 1) / page_rows + it.table >= n_table || (j > from && it.end - it.lo > items[j - 1].end - items[j - 1].lo);
-                if (wrong && bad++ < 5) printf("item %d of %d: columns %d of %d, rows %d .. %d of %d .. %d, part %d of %d\n", j, n, it.c0, it.cols, it.lo, it.end, first, end, it.part, it.parts);
+                const bool off = it.c0 % cols || it.c0 >= it.cols || it.lo < first || it.end > end || it.lo >= it.end;
+                const bool torn = (it.lo % unit && it.lo != first) || (it.end % unit && it.end != end);
+                const bool unshared = it.parts < 1 || it.parts > PAGED_MAX_PARTS || it.part < 0 || it.part >= it.parts ||
+                                      (it.part == 0 && it.lo != first) || (it.part == it.parts - 1 && it.end != end);
+                const bool unknown = it.end - 1 >= past[i] + rows[i] || (it.end - 1) / page_rows + it.table >= n_table;
+                const bool wrong = off || torn || unshared || unknown || (j > from && it.end - it.lo > items[j - 1].end - items[j - 1].lo);
+                if (wrong && bad++ < 5) printf("item %d of %d: columns %d of %d, rows %d .. %d of %d .. %d, part %d of %d\n", j, n, it.c0, it.cols, it.lo, it.end,
+                                               first, end, it.part, it.parts);
                 got[i] += (long long)(c1 - it.c0) * (it.end - it.lo);
                 if (it.part == 0) want[i] += (long long)(c1 - it.c0) * (end - first);
                 if (it.parts > 1) {
@@ -126,8 +132,10 @@ int main(void) {
         const vt_paged_fault f = vt_paged_lay_out(k.s, 3, 64, 10, k.n_seqs, k.past, k.rows, k.tables[0], 4, to, &n, &m);
         if (f.what != k.what) { bad++; printf("case %d: %d instead of %d\n", (int)(&k - c), f.what, k.what); }
     }
-    const vt_paged_shape shapes[] = {{0, 16, 32, 8, 128, 0}, {1, 8, 32, 8, 128, 0}, {1, 24, 32, 8, 128, 0}, {1, 1 << 21, 32, 8, 128, 0}, {1, 16, 32, 8, 96, 0}, {1, 16, 32, 8, 320, 0}, {1, 16, 32, 0, 128, 0},
-                                     {1, 16, 33, 8, 128, 0}, {1, 16, 0, 8, 128, 0}, {1, 16, 32, 8, 128, -1}, {1, 16, 4097, 1, 128, 0}, {1, 16, 65536, 65536, 64, 0}, {1, -16, 32, 8, 128, 0}};
+    const vt_paged_shape shapes[] = {{0, 16, 32, 8, 128, 0}, {1, 8, 32, 8, 128, 0}, {1, 24, 32, 8, 128, 0}, {1, 1 << 21, 32, 8, 128, 0}, {1, 16, 32, 8, 96, 0},
+                                     {1, 16, 32, 8, 320, 0}, {1, 16, 32, 0, 128, 0},
+                                     {1, 16, 33, 8, 128, 0}, {1, 16, 0, 8, 128, 0}, {1, 16, 32, 8, 128, -1}, {1, 16, 4097, 1, 128, 0},
+                                     {1, 16, 65536, 65536, 64, 0}, {1, -16, 32, 8, 128, 0}};
     for (const auto &x : shapes) if (!vt_paged_shape_bad(x)) { bad++; printf("shape %d\n", (int)(&x - shapes)); }
     printf("%d\n", bad);
     return 0;

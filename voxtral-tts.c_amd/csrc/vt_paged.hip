@@ -1,9 +1,8 @@
 /*
- * vt_paged.hip - several sequences over one paged key/value cache: the batch's handle, rotary positions (with the norm of each
- * head in the same pass), and keys and values into pages.  The attention is in vt_paged_attention.hip.
+ * vt_paged.hip - several sequences over one paged key/value cache: the batch's handle, rotary positions (with the norm of each head in the same pass), and
+ * keys and values into pages.  The attention is in vt_paged_attention.hip.
  *
- * A pool is [n_pages, n_kv_heads, page_rows, head_dim] bf16, one for K and one for V: what one head's attention reads of a page is one
- * piece of memory.
+ * A pool is [n_pages, n_kv_heads, page_rows, head_dim] bf16, one for K and one for V: what one head's attention reads of a page is one piece of memory.
  */
 #include "vt_paged.h"
 #include "vt_device.h"
@@ -22,7 +21,8 @@ extern "C" tts_hip_paged_t *tts_hip_paged_create(const tts_hip_paged_shape_t *sh
     if (!shape) { vt_set_error("%s: no shape", who); return NULL; }
     const vt_paged_shape s = {shape->n_pages, shape->page_rows, shape->n_heads, shape->n_kv_heads, shape->head_dim, shape->window};
     if (const char *why = vt_paged_shape_bad(s)) {
-        vt_set_error("%s: %d pages of %d rows, %d heads on %d of %d, window %d: %s", who, s.n_pages, s.page_rows, s.n_heads, s.n_kv_heads, s.head_dim, s.window, why);
+        vt_set_error("%s: %d pages of %d rows, %d heads on %d of %d, window %d: %s", who, s.n_pages, s.page_rows, s.n_heads, s.n_kv_heads, s.head_dim, s.window,
+                     why);
         return NULL;
     }
     const int group = s.n_heads / s.n_kv_heads;
@@ -45,10 +45,8 @@ extern "C" tts_hip_paged_t *tts_hip_paged_create(const tts_hip_paged_shape_t *sh
     b->max_table = max_table;
     b->max_items = (int)vt_paged_max_items(max_seqs, max_rows, group);
     b->device = b->n_seqs = -1;
-    b->at_place = paged_up(sizeof(int) * (size_t)max_rows);
-    b->at_tables = b->at_place + paged_up(2 * sizeof(int) * (size_t)max_rows);
-    b->at_items = b->at_tables + paged_up(sizeof(int) * (size_t)max_table);
-    b->bytes = b->at_items + sizeof(vt_paged_item) * (size_t)b->max_items;
+    b->described = paged_up(sizeof(int) * (size_t)max_rows) + paged_up(2 * sizeof(int) * (size_t)max_rows) + paged_up(sizeof(int) * (size_t)max_table);
+    b->bytes = b->described + sizeof(vt_paged_item) * (size_t)b->max_items;
     b->starts = own;
     b->written = own + max_seqs;
     return b;
@@ -103,12 +101,19 @@ extern "C" int tts_hip_paged_set(tts_hip_paged_t *b, int n_seqs, const int *past
     if (n_seqs > 0 && (!past || !rows || !tables)) { vt_set_error("%s: a NULL pointer", who); return -1; }
     const bool first = b->device < 0;
     unsigned char *host = b->host;
-    if (first && !(host = (unsigned char *)malloc(b->at_items))) { vt_set_error("%s: out of host memory", who); return -1; }
+    if (first && !(host = (unsigned char *)malloc(b->described))) { vt_set_error("%s: out of host memory", who); return -1; }
     /* `host` may still be on its way from the last call */
     if (!first && vt_check(hipEventSynchronize(b->copied), who)) return -1;
+    /* one piece of memory, one copy: what comes first is as long as these rows need */
+    long long some = 0;
+    for (int i = 0; i < n_seqs && i < b->max_seqs && some < b->max_rows; i++) some += rows[i] > 0 ? rows[i] : 0;
+    if (some > b->max_rows) some = b->max_rows;
+    b->at_place = paged_up(sizeof(int) * (size_t)some);
+    b->at_tables = b->at_place + paged_up(2 * sizeof(int) * (size_t)some);
     vt_paged_rows to = {(int *)host, (int *)(host + b->at_place), (int *)(host + b->at_tables), b->starts, b->written};
     int n_rows = 0, n_table = 0;
     const vt_paged_fault f = vt_paged_lay_out(b->shape, b->max_seqs, b->max_rows, b->max_table, n_seqs, past, rows, tables, table_stride, to, &n_rows, &n_table);
+    b->at_items = b->at_tables + paged_up(sizeof(int) * (size_t)n_table);
     int bad = f.what != PAGED_OK;
     if (bad) paged_say(who, b, f, past, rows, n_seqs, table_stride);
     bad = bad || !vt_mx4_ready(who) || paged_memory(who, b);
@@ -118,13 +123,8 @@ extern "C" int tts_hip_paged_set(tts_hip_paged_t *b, int n_seqs, const int *past
     }
     if (bad) return -1;
     b->plan = vt_paged_plan_of(b->shape, g_vt.n_cu > 0 ? g_vt.n_cu : 256, n_seqs, past, rows, b->starts, (vt_paged_item *)(b->host + b->at_items));
-    b->most_pos = 0;
-    for (int i = 0; i < n_seqs; i++)
-        if (rows[i] && past[i] + rows[i] > b->most_pos) b->most_pos = past[i] + rows[i];
-    const struct { size_t at, bytes; } parts[] = {{0, sizeof(int) * (size_t)n_rows}, {b->at_place, 2 * sizeof(int) * (size_t)n_rows},
-                                                   {b->at_tables, sizeof(int) * (size_t)n_table}, {b->at_items, sizeof(vt_paged_item) * (size_t)(b->plan.few + b->plan.many)}};
-    for (const auto &p : parts)
-        if (p.bytes && vt_check(hipMemcpyAsync(b->dev + p.at, b->host + p.at, p.bytes, hipMemcpyHostToDevice, g_vt.stream), who)) return -1;
+    const size_t all = b->at_items + sizeof(vt_paged_item) * (size_t)(b->plan.few + b->plan.many);
+    if (n_rows && vt_check(hipMemcpyAsync(b->dev, b->host, all, hipMemcpyHostToDevice, g_vt.stream), who)) return -1;
     if (vt_check(hipEventRecord(b->copied, g_vt.stream), who)) return -1;
     b->n_rows = n_rows;
     b->n_seqs = n_seqs;
@@ -144,9 +144,9 @@ extern "C" const int *tts_hip_paged_positions(const tts_hip_paged_t *b) {
     return vt_paged_ready(who, b) ? (const int *)b->dev : NULL;
 }
 
-/* ---- positions --------------------------------------------------------------------------------------------------
- * Pair i of a head turns by 2 pi position turns[i].  The product is made in 64 bits and only what is left of it below one turn goes on in
- * fp32, in two parts: the angle is right to 2^-24 or so however far the position (in fp32 it would be off by 0.03 at position 10^6). */
+/* ---- positions -------------------------------------------------------------------------------------------------- Pair i of a head turns by 2 pi position
+ * turns[i].  The product is made in 64 bits and only what is left of it below one turn goes on in fp32, in two parts: the angle is right to 2^-24 or so
+ * however far the position (in fp32 it would be off by 0.03 at position 10^6). */
 __global__ void __launch_bounds__(256) vt_rotary_turns_kernel(double *turns, int pairs, double theta, double factor, double original, double low, double high) {
     const int i = (int)(blockIdx.x * 256 + threadIdx.x);
     if (i >= pairs) return;
@@ -157,20 +157,24 @@ __global__ void __launch_bounds__(256) vt_rotary_turns_kernel(double *turns, int
 
 extern "C" int tts_hip_rotary_turns(double *d_turns, int rot_dim, double theta, double factor, int original_rows, double low_turns, double high_turns) {
     static const char who[] = "tts_hip_rotary_turns";
-    if (!d_turns || ((uintptr_t)d_turns & 7) || rot_dim < 2 || rot_dim > 512 || rot_dim % 2) { vt_set_error("%s: %d values that turn (2 .. 512, even)", who, rot_dim); return -1; }
+    if (!d_turns || ((uintptr_t)d_turns & 7) || rot_dim < 2 || rot_dim > 512 || rot_dim % 2) {
+        vt_set_error("%s: %d values that turn (2 .. 512, even)", who, rot_dim);
+        return -1;
+    }
     if (!(theta > 0) || !(factor > 0) || isinf(theta) || isinf(factor) || original_rows < 0 || !(low_turns < high_turns) || isinf(low_turns) || isinf(high_turns)) {
         vt_set_error("%s: theta %g, factor %g, %d rows, between %g and %g turns", who, theta, factor, original_rows, low_turns, high_turns);
         return -1;
     }
     if (!vt_mx4_ready(who)) return -1;
-    hipLaunchKernelGGL(vt_rotary_turns_kernel, dim3(1), dim3(256), 0, g_vt.stream, d_turns, rot_dim / 2, theta, factor, (double)original_rows, low_turns, high_turns);
+    hipLaunchKernelGGL(vt_rotary_turns_kernel, dim3(1), dim3(256), 0, g_vt.stream, d_turns, rot_dim / 2, theta, factor, (double)original_rows, low_turns,
+                       high_turns);
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
 
-/* ---- heads: norm, turn, store ------------------------------------------------------------------------------------
- * A lane has a unit of four pairs of a head, 2^log lanes a head, and makes the angles once for the HEADS heads that it walks: angles are more than half of the instructions that a
- * unit takes.  (2 p, 2 p + 1) is pair p in both layouts where p does not turn.  Bound by the launch for a few rows (1 to 226 rows of 32 heads 3.8 to 4.1 us a call, 2.5 to 3.8 of them the
- * kernel's); 1531 rows of 32 heads 7.5 us, 25 MB at 3.3 TB/s. */
+/* ---- heads: norm, turn, store ------------------------------------------------------------------------------------ A lane has a unit of four pairs of a
+ * head, 2^log lanes a head, and makes the angles once for the HEADS heads that it walks: angles are more than half of the instructions that a unit takes.
+ * (2 p, 2 p + 1) is pair p in both layouts where p does not turn.  Bound by the launch for a few rows (1 to 226 rows of 32 heads 3.8 to 4.1 us a call, 2.5
+ * to 3.8 of them the kernel's); 1531 rows of 32 heads 7.5 us, 25 MB at 3.3 TB/s. */
 struct turn_job {
     const void *x, *x2;                                  /* K and V for pages */
     void *out, *out2;
@@ -339,7 +343,8 @@ __global__ void __launch_bounds__(256) vt_turn_kernel(turn_job a) {
         }
         const int h = h0 + k;
         if (mine && h < a.heads)
-            turn_store<OUT16, WIDE>(values ? a.out2 : a.out, PAGES ? to + (long long)h * a.out_stride * a.hd : (long long)row * a.out_stride + h * a.hd, a.hd, u, rot, half, p[k], q[k]);
+            turn_store<OUT16, WIDE>(values ? a.out2 : a.out, PAGES ? to + (long long)h * a.out_stride * a.hd : (long long)row * a.out_stride + h * a.hd, a.hd, u,
+                                    rot, half, p[k], q[k]);
     }
 }
 
@@ -349,13 +354,19 @@ static int turn_ok(const char *who, const tts_hip_rotary_t *how, int head_dim) {
         vt_set_error("%s: %d of %d values turn, half %d", who, how->rot_dim, head_dim, how->half);
         return 0;
     }
-    if (how->rot_dim && (!how->d_turns || ((uintptr_t)how->d_turns & 7) || !isfinite(how->magnitude))) { vt_set_error("%s: no turns, or a magnitude that is no number", who); return 0; }
-    if (how->d_gain && (((uintptr_t)how->d_gain & 3) || !(how->eps >= 0) || isinf(how->eps))) { vt_set_error("%s: gains of a norm, eps %g", who, how->eps); return 0; }
+    if (how->rot_dim && (!how->d_turns || ((uintptr_t)how->d_turns & 7) || !isfinite(how->magnitude))) {
+        vt_set_error("%s: no turns, or a magnitude that is no number", who);
+        return 0;
+    }
+    if (how->d_gain && (((uintptr_t)how->d_gain & 3) || !(how->eps >= 0) || isinf(how->eps))) {
+        vt_set_error("%s: gains of a norm, eps %g", who, how->eps);
+        return 0;
+    }
     return 1;
 }
 
-/* Heads that a lane walks: two from where every CU has 16 waves of units on (us at one / two / four of them: 1531 rows of 32 heads of 128 bf16 values, normed, 8.8 / 7.5 / 7.6, into pages 1531 rows of
- * 8 fp32 ones 5.1 / 5.4 / 5.9 and 4000 bf16 ones 8.7 / 7.8 / 7.9). */
+/* Heads that a lane walks: two from where every CU has 16 waves of units on (us at one / two / four of them: 1531 rows of 32 heads of 128 bf16 values,
+ * normed, 8.8 / 7.5 / 7.6, into pages 1531 rows of 8 fp32 ones 5.1 / 5.4 / 5.9 and 4000 bf16 ones 8.7 / 7.8 / 7.9). */
 template <bool PAGES>
 static void turn_launch(turn_job &a, int rows, int bf16, int aligned) {
     int log = 0;
@@ -390,7 +401,10 @@ extern "C" int tts_hip_rotary(void *d_out, const void *d_x, int x_bf16, int rows
                               const tts_hip_rotary_t *how) {
     static const char who[] = "tts_hip_rotary";
     const int size = x_bf16 ? 2 : 4;
-    if (!how || !d_out || !d_x || (((uintptr_t)d_out | (uintptr_t)d_x) & (size - 1))) { vt_set_error("%s: a NULL pointer, or values that do not lie on %d bytes", who, size); return -1; }
+    if (!how || !d_out || !d_x || (((uintptr_t)d_out | (uintptr_t)d_x) & (size - 1))) {
+        vt_set_error("%s: a NULL pointer, or values that do not lie on %d bytes", who, size);
+        return -1;
+    }
     if (head_dim < 2 || head_dim > 512 || head_dim % 2 || n_heads < 1 || rows < 0 || rows > 1 << 30 || (long long)n_heads * head_dim > 1 << 29) {
         vt_set_error("%s: %d rows of %d heads of %d values (2 .. 512, even)", who, rows, n_heads, head_dim);
         return -1;
@@ -403,7 +417,8 @@ extern "C" int tts_hip_rotary(void *d_out, const void *d_x, int x_bf16, int rows
     if (how->rot_dim && (!d_positions || ((uintptr_t)d_positions & 3))) { vt_set_error("%s: no positions", who); return -1; }
     if (!vt_mx4_ready(who)) return -1;
     if (rows == 0) return 0;
-    turn_job a = {d_x, NULL, d_out, NULL, d_positions, NULL, how->d_turns, how->d_gain, how->magnitude, how->eps, 1.f / head_dim, 0, n_heads, head_dim, x_stride, out_stride,
+    turn_job a = {d_x, NULL, d_out, NULL, d_positions, NULL, how->d_turns, how->d_gain, how->magnitude, how->eps, 1.f / head_dim, 0, n_heads, head_dim, x_stride,
+                  out_stride,
                   2 * how->rot_dim + how->half, 0, {0, 1}};
     const int aligned = ((((uintptr_t)d_out | (uintptr_t)d_x) & (4 * size - 1)) | (x_stride & 3) | (out_stride & 3) | ((uintptr_t)how->d_gain & 15)) == 0;
     turn_launch<false>(a, rows, x_bf16, aligned);

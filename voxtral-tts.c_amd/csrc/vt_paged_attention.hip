@@ -1,16 +1,16 @@
 /*
  * vt_paged_attention.hip - attention of a batch's new rows over a paged cache of bf16 keys and values (vt_paged.h).
  *
- * The queries of the heads that share a kv head are columns (vt_paged_plans.h).  Scores are S^T[row][column] = K Q^T and results O^T[value][column] = V^T P^T on
- * the bf16 matrix instructions: keys and values as they lie, queries and weights as planes that each hold 8 bits of what the one before leaves, smallest
+ * The queries of the heads that share a kv head are columns (vt_paged_plans.h).  Scores are S^T[row][column] = K Q^T and results O^T[value][column] = V^T P^T
+ * on the bf16 matrix instructions: keys and values as they lie, queries and weights as planes that each hold 8 bits of what the one before leaves, smallest
  * first: three make fp32 of fp32, one is a bf16 query itself.  A lane holds the same column of S^T and of O^T, and the order of the rows inside an
- * instruction is free, so that weights go from one product to the next in their registers.  Maximum, sum and results of a column are fp32, one pass over the rows with
- * the running maximum.
+ * instruction is free, so that weights go from one product to the next in their registers.  Maximum, sum and results of a column are fp32, one pass over the
+ * rows with the running maximum.
  *
  * What a column does not see: a hidden score is -infinity whatever the key holds.  A hidden value's weight is 0, but 0 times an infinity or NaN would be NaN,
- * so that where rows at hand are hidden from some column and a value among them is not finite, the value counts as 0, and a product of its own, with ones as the
- * weights of what a column sees, tells which results are NaN.  Rows behind a sequence's last are never read: requests have the size of the rows
- * that are there, and the rest is zeros.
+ * so that where rows at hand are hidden from some column and a value among them is not finite, the value counts as 0, and a product of its own, with ones as
+ * the weights of what a column sees, tells which results are NaN.  Rows behind a sequence's last are never read: requests have the size of the rows that are
+ * there, and the rest is zeros.
  */
 #include "vt_paged.h"
 #include "vt_device.h"
@@ -87,16 +87,23 @@ static __device__ __forceinline__ void pa_store4(void *out, size_t at, const f32
 
 /* pairs of bf16 of which one is not finite */
 typedef unsigned short pa_u16x2 __attribute__((ext_vector_type(2)));
-static __device__ __forceinline__ pa_u16x2 pa_larger(pa_u16x2 most, unsigned w) { return __builtin_elementwise_max(most, __builtin_bit_cast(pa_u16x2, w & 0x7fff7fffu)); }
+static __device__ __forceinline__ pa_u16x2 pa_larger(pa_u16x2 most, unsigned w) {
+    return __builtin_elementwise_max(most, __builtin_bit_cast(pa_u16x2, w & 0x7fff7fffu));
+}
 static __device__ __forceinline__ bool pa_not_finite(pa_u16x2 most) { return max((int)most.x, (int)most.y) >= 0x7f80; }
 /* such values as ones, others as zeros; and the other way round, they as zeros */
-static __device__ __forceinline__ unsigned pa_marks(unsigned w) { return ((w & 0x7f80u) == 0x7f80u ? 0x3f80u : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0x3f800000u : 0u); }
-static __device__ __forceinline__ unsigned pa_finite(unsigned w) { return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u); }
+static __device__ __forceinline__ unsigned pa_marks(unsigned w) {
+    return ((w & 0x7f80u) == 0x7f80u ? 0x3f80u : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0x3f800000u : 0u);
+}
+static __device__ __forceinline__ unsigned pa_finite(unsigned w) {
+    return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+}
 
 static __device__ __forceinline__ float pa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-/* A column's weights are relative to m, which follows the largest score only where that is further above than this: weights up to 2^8 are as exact as ones below 1,
- * and what was summed so far is scaled anew in the first tile and hardly ever after it (with 32 columns to a wave one of them has a new largest score in nearly every tile). */
+/* A column's weights are relative to m, which follows the largest score only where that is further above than this: weights up to 2^8 are as exact as ones
+ * below 1, and what was summed so far is scaled anew in the first tile and hardly ever after it (with 32 columns to a wave one of them has a new largest
+ * score in nearly every tile). */
 #define PA_SLACK 8.f
 template <bool F32>
 static __device__ __forceinline__ float pa_weight(float s, float m, float scale) { return pa_exp2(F32 ? s - m : fmaf(s, scale, -m)); }
@@ -120,11 +127,12 @@ static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, in
     return pa_rows_of(table[pa_entry(at, lo, end, page_log)], at, lo, end, page_log, heads, head, row_bytes);
 }
 
-/* ---- few columns -------------------------------------------------------------------------------------------------
- * A wave has 32 rows of K and V in registers at a time, asks for the next as soon as these are used, and waits for nobody; the waves of a workgroup,
- * and then the workgroups that share the columns' rows, add their parts in a fixed order, the last workgroup to arrive those of all.  K is the A operand of 16 x 16 x 32, a lane's 16
- * bytes from its own row.  V's rows are its columns: a lane loads CD values each of the eight rows that it has weights of, 16 lanes a whole row, and pairs of rows are
- * put together two values at a time.  Queries, the same for all waves, wait in LDS as operands.  ONCE: no other workgroup reads these rows, and there are more than a cache holds. */
+/* ---- few columns ------------------------------------------------------------------------------------------------- A wave has 32 rows of K and V in
+ * registers at a time, asks for the next as soon as these are used, and waits for nobody; the waves of a workgroup, and then the workgroups that share the
+ * columns' rows, add their parts in a fixed order, the last workgroup to arrive those of all.  K is the A operand of 16 x 16 x 32, a lane's 16 bytes from
+ * its own row.  V's rows are its columns: a lane loads CD values each of the eight rows that it has weights of, 16 lanes a whole row, and pairs of rows are
+ * put together two values at a time.  Queries, the same for all waves, wait in LDS as operands.  ONCE: no other workgroup reads these rows, and there are
+ * more than a cache holds. */
 template <int HP, bool F32, bool ONCE, int CT>
 __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(pa_job a) {
     constexpr int HD = 64 * HP, ROW = 2 * HD, KS = 2 * HP, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4, WAVES = PAGED_FEW_WAVES;
@@ -134,7 +142,8 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
     __shared__ int last;
     static_assert(sizeof area >= KS * NQ * CT * 1024, "operands");
     u32x4 *queries = reinterpret_cast<u32x4 *>(area);
-    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4, h = (int)blockIdx.x, heads = (int)gridDim.x;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int h = (int)blockIdx.x, heads = (int)gridDim.x;
     const vt_paged_item it = pa_item(a.items);
     const pa_const_int *table = (const pa_const_int *)(uintptr_t)(a.tables + it.table);
     const int base = it.lo & ~(PAGED_FEW_ROWS - 1), tiles = (it.end - base + PAGED_FEW_ROWS - 1) / PAGED_FEW_ROWS;
@@ -204,7 +213,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
         for (int p = 0; p < NQ; p++) queries[(y * NQ + p) * 64 + lane] = q[p];
     }
     const int q_first = it.past + vt_div(it.c0, a.group), q_last = it.past + vt_div(it.c0 + nc - 1, a.group);
-    const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);       /* rows that every column sees */
+    const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);      /* that every column sees */
     float m[2], l[2];
     f32x4 o[CT][CHUNKS * CD];
 #pragma unroll
@@ -299,7 +308,8 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
                     for (int i = 0; i < CD; i++) {
                         u32x4 v4;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) v4[e] = pa_marks(__builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u));
+                        for (int e = 0; e < 4; e++)
+                            v4[e] = pa_marks(__builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u));
                         const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(ones), (f32x4{0.f, 0.f, 0.f, 0.f}), 0, 0, 0);
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[c][ch * CD + i][e] = hit[e] > 0.f ? NAN : o[c][ch * CD + i][e];
@@ -320,10 +330,13 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
 #pragma unroll
                 for (int e = 0; e < 4; e++) v4[e] = __builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--) o[0][ch * CD + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[0][p]), o[0][ch * CD + i], 0, 0, 0);
+                for (int p = NP - 1; p >= 0; p--)
+                    o[0][ch * CD + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[0][p]), o[0][ch * CD + i], 0, 0, 0);
                 if constexpr (CT == 2) {                 /* (also where there is no second: a branch for each would cost more) */
 #pragma unroll
-                    for (int p = NP - 1; p >= 0; p--) o[CT - 1][ch * CD + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[CT - 1][p]), o[CT - 1][ch * CD + i], 0, 0, 0);
+                    for (int p = NP - 1; p >= 0; p--)
+                        o[CT - 1][ch * CD + i] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[CT - 1][p]), o[CT - 1][ch * CD + i], 0, 0, 0);
                 }
             }
         ask_v();
@@ -399,7 +412,8 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
         for (int k0 = 0; k0 < it.parts; k0 += 16) {      /* parts past the last: the last again, times 0 */
             f32x4 p[16];
 #pragma unroll
-            for (int k = 0; k < 16; k++) p[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(pd, from + min(k0 + k, it.parts - 1) * (COLS * OD * 4), 0, 16));
+            for (int k = 0; k < 16; k++)
+                p[k] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(pd, from + min(k0 + k, it.parts - 1) * (COLS * OD * 4), 0, 16));
 #pragma unroll
             for (int k = 0; k < 16; k++) v = v + p[k] * wt[col][k0 + k];
         }
@@ -408,15 +422,17 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
 }
 
 /* ---- many columns ------------------------------------------------------------------------------------------------
- * A workgroup has 128 columns, a wave 32, and goes through its rows 64 at a time, 16 of them each wave's to ask for, by requests that write LDS.  K's rows are the A operand of
+ * A workgroup has 128 columns, a wave 32, and goes through its rows 64 at a time, 16 of them each wave's to ask for, by requests that write LDS.  K's rows are the
+ * A operand of
  * 32 x 32 x 16 as they lie; of V, whose rows are that operand's columns, the transposing reads of LDS give a lane four rows' values of one column.
  *
- * A unit is 32 rows.  While unit u's weights are made and multiplied, the matrix cores make unit u + 1's scores, so that K's tiles lie half a tile behind V's: beside V's rows
+ * A unit is 32 rows.  While unit u's weights are made and multiplied, the matrix cores make unit u + 1's scores, so that K's tiles lie half a tile behind V's:
+ * beside V's rows
  * 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95. */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 
-/* fp32: the compiler keeps to the order that is written, in which an instruction's operands are asked for just ahead of it and no more of them wait in registers than there are; bf16 has
- * registers for its own order (four prompts in a window 112.0 us as written, 108.8 so) */
+/* fp32: the compiler keeps to the order that is written, in which an instruction's operands are asked for just ahead of it and no more of them wait in
+ * registers than there are; bf16 has registers for its own order (four prompts in a window 112.0 us as written, 108.8 so) */
 template <bool F32> static __device__ __forceinline__ void pa_here() { if constexpr (F32) __builtin_amdgcn_sched_barrier(0); }
 
 template <int HP, bool F32>
@@ -425,28 +441,31 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 1, KB = 64 * ROW;
     /* objects of their own: a read waits for the requests that write the same one */
     __shared__ __attribute__((aligned(16))) unsigned char k0[KB], k1[KB], v0[KB], v1[KB];
-    /* Tiles with rows that some column does not see: at most 3 where the columns' rows begin to be seen and 3 where they end (fewer queries than 128 apart), or 5 with a window of less */
+    /* Tiles with rows that some column does not see: at most 3 where the columns' rows begin to be seen and 3 where they end (fewer queries than 128
+     * apart), or 5 with a window of less */
     constexpr int EDGES = 6;
     __shared__ unsigned marks[EDGES][64][DT];            /* of such a tile the values that are not finite, 32 of a row's to a word; where there are any: .. */
     __shared__ int odd[EDGES][WAVES], last;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5, h = (int)blockIdx.x, heads = (int)gridDim.x;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5;
+    const int h = (int)blockIdx.x, heads = (int)gridDim.x;
     const vt_paged_item it = pa_item(a.items);
     const pa_const_int *table = (const pa_const_int *)(uintptr_t)(a.tables + it.table);
     const int w0 = it.c0 + 32 * wave, wc = min(w0 + 32, it.cols) - w0;                   /* this wave's columns: none, perhaps */
     const int cc = min(w0 + n, it.cols - 1), qi = vt_div(cc, a.group), pos = it.past + qi;
     const int see_lo = max(a.window && pos >= a.window ? pos - a.window + 1 : 0, it.lo), see_hi = min(pos + 1, it.end);
     const int q_first = it.past + vt_div(min(w0, it.cols - 1), a.group), q_last = it.past + vt_div(min(w0 + 31, it.cols - 1), a.group);
-    const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);     /* rows that every column of the wave sees */
+    const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);    /* that every column of the wave sees */
     const int any_lo = a.window && q_first >= a.window ? q_first - a.window + 1 : 0, any_hi = wc > 0 ? min(q_last + 1, it.end) : 0;   /* .. that any does */
     const int wg_last = it.past + vt_div(min(it.c0 + PAGED_MANY_COLS, it.cols) - 1, a.group);
-    const int wg_lo = max(a.window && wg_last >= a.window ? wg_last - a.window + 1 : 0, it.lo), wg_hi = min(it.past + vt_div(it.c0, a.group) + 1, it.end);         /* rows that every column sees */
+    const int wg_lo = max(a.window && wg_last >= a.window ? wg_last - a.window + 1 : 0, it.lo);             /* rows that every column sees */
+    const int wg_hi = min(it.past + vt_div(it.c0, a.group) + 1, it.end);
     const int base = it.lo & ~(PAGED_MANY_ROWS - 1), tiles = (it.end - base + PAGED_MANY_ROWS - 1) / PAGED_MANY_ROWS;
     const size_t head_at = (size_t)h * a.group.d + (cc - qi * a.group.d);
     u32x4 raw[KS][2];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) pa_query_load<F32>(a.Q, (size_t)(it.row + qi) * a.q_stride + head_at * HD + 16 * ks + 8 * g, raw[ks]);
-    /* Pieces of 16 bytes change places within a row, so that what is read at once lies in different banks: K's with the row's last bits, so that 16 (8) rows' same piece do; V's fours of
-     * them, so that four rows' same 64 bytes do. */
+    /* Pieces of 16 bytes change places within a row, so that what is read at once lies in different banks: K's with the row's last bits, so that 16 (8)
+     * rows' same piece do; V's fours of them, so that four rows' same 64 bytes do. */
     constexpr int SWAP = PIECES - 1;
     auto v_swap = [](int r) { return HP == 1 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
     int k_at[4], v_at[4];                                /* DT of them (with that size the host pass drops the kernel) */
@@ -486,8 +505,8 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     pa_f32x16 o[DT];
 #pragma unroll
     for (int i = 0; i < DT; i++) o[i] = pa_f32x16{};
-    /* addresses in LDS: one for all of K's pieces and one for all of V's, which differ from them in bits of their own.  (fp32: through an empty asm in each unit, else each piece's, for each
-     * buffer, is kept in a register.) */
+    /* addresses in LDS: one for all of K's pieces and one for all of V's, which differ from them in bits of their own.  (fp32: through an empty asm in each
+     * unit, else each piece's, for each buffer, is kept in a register.) */
     const int k_base = n * ROW + (g ^ (n & SWAP)) * 16, r4 = (n & 15) >> 2;
     const int v_base = (4 * g + r4) * ROW + (v_swap(r4) + 2 * (n >> 4) + ((n & 3) >> 1)) * 16 + (n & 1) * 8;
     auto read_k = [&](const unsigned char *kb, int half, int ks, int from) __attribute__((always_inline)) {
@@ -556,8 +575,8 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
         __syncthreads();
         edges++;
     };
-    /* pairs of weights that are made beside the scores; the others beside the first products with values.  An instruction takes the matrix cores 32 cycles, a pair 50 (fp32, with
-     * three times the instructions: 90) of the vector unit. */
+    /* pairs of weights that are made beside the scores; the others beside the first products with values.  An instruction takes the matrix cores 32 cycles,
+     * a pair 50 (fp32, with three times the instructions: 90) of the vector unit. */
     constexpr int EARLY = F32 ? 8 : HP == 1 ? 6 : 5, AHEAD = F32 ? 1 : 3, BEFORE = F32 ? 1 : 2;
     /* (AHEAD: operands that are asked for ahead of their instruction; BEFORE: those in front of what depends on the maximum) */
     float top = -INFINITY;                               /* the largest score of the unit at hand, in a lane's rows */
@@ -614,7 +633,8 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
                 for (int e = EARLY + (8 - EARLY) * i / DT; e < EARLY + (8 - EARLY) * (i + 1) / DT; e++) weigh(e);
             } else {
 #pragma unroll
-                for (int e = 16 * i / DT; e < 16 * (i + 1) / DT; e += 2) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, next[e]), next[e + 1]);
+                for (int e = 16 * i / DT; e < 16 * (i + 1) / DT; e += 2)
+                    top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, next[e]), next[e + 1]);
             }
             pa_here<F32>();
         }
@@ -731,28 +751,33 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     }
 }
 
-template <int HP, bool F32>
-static void pa_launch(const pa_job &job, const vt_paged_plan &p, int heads) {
-    if (p.few) {
-        const dim3 grid((unsigned)heads, (unsigned)p.few), threads(64 * PAGED_FEW_WAVES);
-        if constexpr (HP <= 2) {
-            if (p.wide) hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, false, 2>), grid, threads, 0, g_vt.stream, job);
-        }
-        if (p.wide) { }
-        else if (p.once) hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, true, 1>), grid, threads, 0, g_vt.stream, job);
-        else hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, false, 1>), grid, threads, 0, g_vt.stream, job);
-    }
-    if constexpr (HP <= 2) {
-        if (p.many) {
-            pa_job many = job;
-            many.items += p.few;
-            const dim3 grid((unsigned)heads, (unsigned)p.many);
-            hipLaunchKernelGGL((vt_paged_many_kernel<HP, F32>), grid, dim3(256), 0, g_vt.stream, many);
-        }
+/* items are the grid's second dimension, of at most 65535 */
+template <class F>
+static void pa_items(const pa_job &job, int from, int n, int heads, F launch) {
+    for (int at = 0; at < n; at += 65535) {
+        pa_job part = job;
+        part.items = job.items + from + at;
+        launch(part, dim3((unsigned)heads, (unsigned)(n - at < 65535 ? n - at : 65535)));
     }
 }
 
-extern "C" int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16, int q_stride, const tts_hip_paged_t *b, const void *d_k_pages, const void *d_v_pages, float scale) {
+template <int HP, bool F32>
+static void pa_launch(const pa_job &job, const vt_paged_plan &p, int heads) {
+    pa_items(job, 0, p.few, heads, [&](const pa_job &a, const dim3 &grid) {
+        const dim3 threads(64 * PAGED_FEW_WAVES);
+        if constexpr (HP <= 2) {
+            if (p.wide) { hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, false, 2>), grid, threads, 0, g_vt.stream, a); return; }
+        }
+        if (p.once) hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, true, 1>), grid, threads, 0, g_vt.stream, a);
+        else hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, false, 1>), grid, threads, 0, g_vt.stream, a);
+    });
+    if constexpr (HP <= 2)
+        pa_items(job, p.few, p.many, heads,
+                 [](const pa_job &a, const dim3 &grid) { hipLaunchKernelGGL((vt_paged_many_kernel<HP, F32>), grid, dim3(256), 0, g_vt.stream, a); });
+}
+
+extern "C" int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16, int q_stride, const tts_hip_paged_t *b, const void *d_k_pages,
+                                       const void *d_v_pages, float scale) {
     static const char who[] = "tts_hip_paged_attention";
     if (!b) { vt_set_error("%s: no batch", who); return -1; }
     if (!d_out || !d_Q || !d_k_pages || !d_v_pages || (((uintptr_t)d_out | (uintptr_t)d_Q | (uintptr_t)d_k_pages | (uintptr_t)d_v_pages) & 15)) {
@@ -769,9 +794,11 @@ extern "C" int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16,
     const int group = s.n_heads / s.n_kv_heads;
     int page_log = 4;
     while (1 << page_log < s.page_rows) page_log++;
-    const size_t few = (size_t)b->plan.few_slots * s.n_kv_heads * (b->plan.wide ? 32 : 16) * (s.head_dim + 4) * 4, many = (size_t)b->plan.many_slots * s.n_kv_heads * 4 * (8 * HP + 1) * 1024;
+    const size_t few = (size_t)b->plan.few_slots * s.n_kv_heads * (b->plan.wide ? 32 : 16) * (s.head_dim + 4) * 4;
+    const size_t many = (size_t)b->plan.many_slots * s.n_kv_heads * 4 * (8 * HP + 1) * 1024;
     pa_job job = {(const uint16_t *)d_k_pages, (const uint16_t *)d_v_pages, d_Q, d_out, NULL, g_vt.d_mx4_cnt, (const vt_paged_item *)(b->dev + b->at_items),
-                  (const int *)(b->dev + b->at_tables), q_stride, s.n_heads, page_log, s.window, vt_divisor_of(group, (long long)b->max_rows * group), scale * 1.44269504f};
+                  (const int *)(b->dev + b->at_tables), q_stride, s.n_heads, page_log, s.window, vt_divisor_of(group, (long long)b->max_rows * group),
+                  scale * 1.44269504f};
     if ((few || many) && !(job.part = (float *)vt_scratch(few > many ? few : many))) return -1;
 #define ATTEND(H) (x_bf16 ? pa_launch<H, false>(job, b->plan, s.n_kv_heads) : pa_launch<H, true>(job, b->plan, s.n_kv_heads))
     switch (HP) {

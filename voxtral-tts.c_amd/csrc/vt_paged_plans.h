@@ -1,6 +1,6 @@
 /*
- * vt_paged_plans.h - a batch of sequences over a paged cache (vt_paged.hip): what is refused, and the attention's work items from
- * shapes and the number of CUs.  Host code without HIP, so that a host test can walk it.
+ * vt_paged_plans.h - a batch of sequences over a paged cache (vt_paged.hip): what is refused, and the attention's work items from shapes and the number of
+ * CUs.  Host code without HIP, so that a host test can walk it.
  */
 #ifndef VT_PAGED_PLANS_H
 #define VT_PAGED_PLANS_H
@@ -15,8 +15,8 @@
 #define PAGED_MAX_GROUP 4096               /* heads on a kv head */
 #define PAGED_COUNTERS 16384               /* heads times tiles of columns that several workgroups share */
 
-/* Columns are a sequence's new rows times the heads that share a kv head: column c is row c / group, head c % group of the group.
- * Few columns: 16 or 32 to a workgroup, whose waves take 32 rows of the cache each in turn.  Many: 128 to a workgroup, 64 rows at a time. */
+/* Columns are a sequence's new rows times the heads that share a kv head: column c is row c / group, head c % group of the group. Few columns: 16 or 32 to
+ * a workgroup, whose waves take 32 rows of the cache each in turn.  Many: 128 to a workgroup, 64 rows at a time. */
 #define PAGED_FEW_ROWS 32
 #define PAGED_FEW_WAVES 4
 #define PAGED_MANY_COLS 128
@@ -25,8 +25,8 @@
 #define PAGED_CACHED 32e6                  /* bytes: all L2s */
 #define PAGED_SPLIT_ITEMS 4096             /* items that a launch may have beyond one for each tile of columns */
 
-/* What a workgroup does for every kv head: columns c0 .. of a sequence whose new rows are `row` .. of the batch and lie behind `past`
- * rows, over the cache's rows lo .. end - 1; `parts` of them make up the columns' result, in slots `slot` .. */
+/* What a workgroup does for every kv head: columns c0 .. of a sequence whose new rows are `row` .. of the batch and lie behind `past` rows, over the
+ * cache's rows lo .. end - 1; `parts` of them make up the columns' result, in slots `slot` .. */
 struct vt_paged_item { int row, past, cols, table, c0, lo, end, slot, part, parts, counter, spare; };
 
 struct vt_paged_shape { int n_pages, page_rows, n_heads, n_kv_heads, head_dim, window; };
@@ -51,8 +51,8 @@ static int vt_paged_by_value(const void *a, const void *b) {
     return x < y ? -1 : x > y;
 }
 
-/* The batch as the kernels read it: of each new row its position, page and row in the page, of each sequence its pages' numbers one behind
- * the other from `starts` on. */
+/* The batch as the kernels read it: of each new row its position, page and row in the page, of each sequence its pages' numbers one behind the other from
+ * `starts` on. */
 struct vt_paged_rows { int *pos, *place, *tables, *starts, *written; };
 
 enum { PAGED_OK, PAGED_COUNT, PAGED_SEQUENCE, PAGED_TOO_MANY_ROWS, PAGED_TABLE, PAGED_PAGE, PAGED_WRITTEN };
@@ -96,25 +96,27 @@ static inline vt_paged_fault vt_paged_lay_out(const vt_paged_shape &s, int max_s
 
 /* ---- work items --- */
 
-/* items of either kernel (the few's first), parts that they leave; wide: the few's columns go by 32; once: their rows are read by one workgroup each, more of them than a cache holds */
+/* items of either kernel (the few's first), parts that they leave; wide: the few's columns go by 32; once: their rows are read by one workgroup each, more
+ * of them than a cache holds */
 struct vt_paged_plan { int few, many, few_slots, many_slots, wide, once; };
 
-/* Which kernels a batch goes to: `any`, whether there are sequences for the one for many columns; columns of a workgroup of the other, whether its rows are read by one
- * workgroup only, and their bytes */
+/* Which kernels a batch goes to: `any`, whether there are sequences for the one for many columns; columns of a workgroup of the other, whether its rows are
+ * read by one workgroup only, and their bytes */
 struct vt_paged_kinds { bool any; int few_cols; bool once; double bytes; };
 
 static inline long long vt_paged_max_items(int max_seqs, int max_rows, int group) {
     return (long long)max_rows * group / 16 + max_seqs + 2 * PAGED_SPLIT_ITEMS;
 }
 
-/* Which sequences go to the kernel for many columns: those of more than 64 whose heads of up to 128 values leave it registers, where there is enough for it to do, as columns times
- * the rows that they see on average times kv heads times values, over all of them.  It does twice as much with what it reads, but by few workgroups.  Measured, us with the kernel
- * for few columns, 32 at a time, and for many (fp32 / bf16), 32 heads on 8 of 128: 450 rows behind 200 (0.8e9) 18 / 16 and 26 / 19, 700 behind none (1.0e9) 24 / 20 and 27 / 19, 200 behind
- * 2000 (1.7e9) 32 / 24 and 38 / 26, 50 behind 16000 (3.3e9) 52 / 48 and 60 / 43, 512 behind 1500 (3.7e9) 45 / 39 and 49 / 32, 100 behind 500 sixteen times (3.6e9) 59 / 47 and 49 / 29; 16 heads of
- * 64: 512 behind 1500 (0.9e9) 21 / 17 and 24 / 18.
- * Else 32 columns to a workgroup, not 16, where there is enough for that, as columns / 16 times rows times kv heads times values (less where every CU has one of 16); 16 and 32 at a time: 37 rows behind 300 (3e6) 7.0 / 6.4 and 9.9 /
- * 8.2, 100 behind 1000 (27e6) 13 / 13 and 19 / 15, 37 behind 4000 (41e6) 21 / 21 and 23 / 20, 16 behind 300 32 times (40e6) 22 / 22 and 17 / 14, 200 behind 2000 (107e6) 42 / 41 and 32 / 24; 16 heads of 64: 37
- * behind 4000 (12e6) 14 / 13 and 17 / 16, 512 behind 1500 (57e6) 24 / 23 and 21 / 17. */
+/* Which sequences go to the kernel for many columns: those of more than 64 whose heads of up to 128 values leave it registers, where there is enough for it
+ * to do, as columns times the rows that they see on average times kv heads times values, over all of them.  It does twice as much with what it reads, but
+ * by few workgroups.  Measured, us with the kernel for few columns, 32 at a time, and for many (fp32 / bf16), 32 heads on 8 of 128: 450 rows behind 200
+ * (0.8e9) 18 / 16 and 26 / 19, 700 behind none (1.0e9) 24 / 20 and 27 / 19, 200 behind 2000 (1.7e9) 32 / 24 and 38 / 26, 50 behind 16000 (3.3e9) 52 / 48
+ * and 60 / 43, 512 behind 1500 (3.7e9) 45 / 39 and 49 / 32, 100 behind 500 sixteen times (3.6e9) 59 / 47 and 49 / 29; 16 heads of 64: 512 behind 1500
+ * (0.9e9) 21 / 17 and 24 / 18. Else 32 columns to a workgroup, not 16, where there is enough for that, as columns / 16 times rows times kv heads times
+ * values (less where every CU has one of 16); 16 and 32 at a time: 37 rows behind 300 (3e6) 7.0 / 6.4 and 9.9 / 8.2, 100 behind 1000 (27e6) 13 / 13 and 19
+ * / 15, 37 behind 4000 (41e6) 21 / 21 and 23 / 20, 16 behind 300 32 times (40e6) 22 / 22 and 17 / 14, 200 behind 2000 (107e6) 42 / 41 and 32 / 24; 16 heads
+ * of 64: 37 behind 4000 (12e6) 14 / 13 and 17 / 16, 512 behind 1500 (57e6) 24 / 23 and 21 / 17. */
 #define PAGED_MANY_FROM 2.5e9
 #define PAGED_WIDE_FROM 45e6
 #define PAGED_WIDE_FULL 30e6
@@ -165,13 +167,15 @@ static inline int vt_paged_parts(int first, int end, int unit, int run) {
     return (int)((units + run - 1) / run);
 }
 
-/* What a workgroup takes: `fixed` us, `step` for a unit of its rows, alone on its CU and with `beside` of them on it, `part` more where it leaves a part, and `merge` for each of
- * the parts that the last one adds; `tail`: the share of the longest that a launch of more than fit at once ends with.  By head_dim / 64; fitted to 25 to 30 batches at every run.  The run that
- * these choose is behind the best one by 1 to 2 % on average, 10 at the worst.  us at some of them: 1531 rows behind none, many columns, in runs of 4 / 8 / 12 / 16 / whole (fp32) 76 / 67
- * / 61 / 65 / 72, 4000 of them 502 / 381 / 350 / 343 / 310, 512 behind 1500 62 / 50 / 54 / 51 / 83; few columns: one row behind 1999 in runs of 1 / 2 / 4 / 8 / 16 7.8 / 8.0 / 9.3 / 13 / 20, behind 65535 of 8 /
- * 16 / 32 / 64 47 / 45 / 53 / 96; 200 rows behind 2000, 32 columns, of 4 / 8 / 16 / whole 51 / 44 / 45 / 32. */
+/* What a workgroup takes: `fixed` us, `step` for a unit of its rows, alone on its CU and with `beside` of them on it, `part` more where it leaves a part,
+ * and `merge` for each of the parts that the last one adds; `tail`: the share of the longest that a launch of more than fit at once ends with.  By head_dim
+ * / 64; fitted to 25 to 30 batches at every run.  The run that these choose is behind the best one by 1 to 2 % on average, 10 at the worst.  us at some of
+ * them: 1531 rows behind none, many columns, in runs of 4 / 8 / 12 / 16 / whole (fp32) 76 / 67 / 61 / 65 / 72, 4000 of them 502 / 381 / 350 / 343 / 310,
+ * 512 behind 1500 62 / 50 / 54 / 51 / 83; few columns: one row behind 1999 in runs of 1 / 2 / 4 / 8 / 16 7.8 / 8.0 / 9.3 / 13 / 20, behind 65535 of 8 / 16
+ * / 32 / 64 47 / 45 / 53 / 96; 200 rows behind 2000, 32 columns, of 4 / 8 / 16 / whole 51 / 44 / 45 / 32. */
 struct vt_paged_cost { int beside; float fixed, alone, step, part, merge, tail; };
-static const vt_paged_cost vt_paged_few_cost[4] = {{4, 1.1f, 0.8f, 2.55f, 2.85f, 0.35f, 0.37f}, {3, 2.7f, 0.95f, 3.2f, 2.6f, 0.12f, 0.11f}, {2, 1.2f, 1.04f, 1.93f, 1.9f, 0.08f, 0.31f}, {2, 5.1f, 1.2f, 2.8f, 3.9f, 0.07f, 0.29f}};
+static const vt_paged_cost vt_paged_few_cost[4] = {{4, 1.1f, 0.8f, 2.55f, 2.85f, 0.35f, 0.37f}, {3, 2.7f, 0.95f, 3.2f, 2.6f, 0.12f, 0.11f},
+                                                   {2, 1.2f, 1.04f, 1.93f, 1.9f, 0.08f, 0.31f}, {2, 5.1f, 1.2f, 2.8f, 3.9f, 0.07f, 0.29f}};
 static const vt_paged_cost vt_paged_wide_cost[2] = {{3, 1.4f, 0.32f, 0.7f, 2.5f, 0.16f, 0.39f}, {2, 0.85f, 0.42f, 1.09f, 4.85f, 0.07f, 0.08f}};
 static const vt_paged_cost vt_paged_many_cost[2] = {{2, 7.9f, 1.9f, 3.0f, 5.0f, 1.0f, 0.45f}, {2, 9.25f, 2.2f, 3.8f, 3.6f, 2.2f, 0.24f}};
 
@@ -184,7 +188,7 @@ static inline int vt_paged_run(const vt_paged_shape &s, const vt_paged_kinds &ki
     });
     int best = (int)longest;
     double least = 1e300;
-    for (int parts = 1; parts <= PAGED_MAX_PARTS; parts++) {
+    for (int parts = 1; parts <= PAGED_MAX_PARTS; parts += parts < 16 ? 1 : parts / 8) {
         const int run = (int)((longest + parts - 1) / parts);
         long long items = 0, extra = 0, split = 0, most = 0, all = 0;
         int late = 0;
@@ -217,7 +221,8 @@ static int vt_paged_longest(const void *a, const void *b) {
 }
 
 /* Items of one kernel into `to`, the longest first; -> how many, and their slots */
-static inline int vt_paged_items(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to, int *n_slots) {
+static inline int vt_paged_items(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows,
+                                 const int *starts, vt_paged_item *to, int *n_slots) {
     const int unit = many ? PAGED_MANY_ROWS : PAGED_FEW_ROWS * PAGED_FEW_WAVES, group = s.n_heads / s.n_kv_heads;
     *n_slots = 0;
     if (many && !kinds.any) return 0;
@@ -244,8 +249,8 @@ static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, int n_cu, 
     p.few = vt_paged_items(s, kinds, false, n_cu, n_seqs, past, rows, starts, to, &p.few_slots);
     p.many = vt_paged_items(s, kinds, true, n_cu, n_seqs, past, rows, starts, to + p.few, &p.many_slots);
     p.wide = kinds.few_cols > 16;
-    /* Requests that leave nothing behind in the caches: 65535 rows of 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows, which the caches
-     * (32 MB of L2) keep for the next call on them, 6.8 -> 7.2. */
+    /* Requests that leave nothing behind in the caches: 65535 rows of 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows, which the
+     * caches (32 MB of L2) keep for the next call on them, 6.8 -> 7.2. */
     p.once = kinds.once && kinds.bytes >= PAGED_CACHED;
     return p;
 }
