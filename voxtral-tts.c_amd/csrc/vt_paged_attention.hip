@@ -15,6 +15,7 @@
 #include "vt_paged.h"
 #include "vt_device.h"
 #include "vt_requests.h"
+#include "vt_mx4_plans.h"
 
 #include <math.h>
 
@@ -35,6 +36,7 @@ struct pa_job {
     float scale;                                         /* times log2 e */
 };
 static_assert(sizeof(pa_job) <= 104, "arguments");
+static_assert(PAGED_COUNTERS <= VT_MX4_COUNTERS, "counters");
 
 static __device__ __forceinline__ pa_bf16x8 pa_operand(const u32x4 &w) { return __builtin_bit_cast(pa_bf16x8, w); }
 
@@ -110,10 +112,10 @@ static __device__ __forceinline__ float pa_weight(float s, float m, float scale)
 
 /* What the batch's description holds is the same for a whole workgroup: scalar loads, which the kernel's own stores cannot touch */
 typedef __attribute__((address_space(4))) const int pa_const_int;
-static __device__ __forceinline__ vt_paged_item pa_item(const vt_paged_item *items) {
+static __device__ __forceinline__ vt_paged_item pa_item(const vt_paged_item *items, int at) {
     static_assert(sizeof(vt_paged_item) == 48, "words");
-    const pa_const_int *w = (const pa_const_int *)(uintptr_t)(items + blockIdx.y);
-    return vt_paged_item{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9], w[10], 0};
+    const pa_const_int *w = (const pa_const_int *)(uintptr_t)(items + at);
+    return vt_paged_item{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9], w[10], w[11]};
 }
 
 /* 16 rows from `at` on, a multiple of 16, of those lo .. end - 1: where they lie, and the bytes of them that are there */
@@ -127,24 +129,30 @@ static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, in
     return pa_rows_of(table[pa_entry(at, lo, end, page_log)], at, lo, end, page_log, heads, head, row_bytes);
 }
 
-/* ---- few columns ------------------------------------------------------------------------------------------------- A wave has 32 rows of K and V in
- * registers at a time, asks for the next as soon as these are used, and waits for nobody; the waves of a workgroup, and then the workgroups that share the
- * columns' rows, add their parts in a fixed order, the last workgroup to arrive those of all.  K is the A operand of 16 x 16 x 32, a lane's 16 bytes from
- * its own row.  V's rows are its columns: a lane loads CD values each of the eight rows that it has weights of, 16 lanes a whole row, and pairs of rows are
- * put together two values at a time.  Queries, the same for all waves, wait in LDS as operands.  ONCE: no other workgroup reads these rows, and there are
- * more than a cache holds. */
-template <int HP, bool F32, bool ONCE, int CT>
-__global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(pa_job a) {
+/* ---- few columns ----
+ * A wave has 32 rows of K and V in registers at a time, asks for the next as soon as these are used, and waits for nobody; the waves of a workgroup, and then
+ * the workgroups that share the columns' rows, add their parts in a fixed order, the last workgroup to arrive those of all.  K is the A operand of 16 x 16 x
+ * 32, a lane's 16 bytes from its own row.  V's rows are its columns: a lane loads CD values each of the eight rows that it has weights of, 16 lanes a whole
+ * row, and pairs of rows are put together two values at a time.  Queries, the same for all waves, wait in LDS as operands.  ONCE: no other workgroup reads
+ * these rows, and there are more than a cache holds.
+ *
+ * Rows are read as they lie and once for 16 or 32 columns, so that memory bounds a long cache: one query behind 65535 rows of 8 x 128, 268 MB, 44 us
+ * (6.1 TB/s), steps of 64 sequences of 118000 rows, 483 MB, 82 us (5.9 TB/s).  A short one is bound by what follows on each other in a workgroup - its
+ * item, its table, queries and rows, a part's store, counter and merge: one query behind 1999 rows 8 us a call with 4 for the launch. */
+template <int HP, bool F32, int CT>
+struct pa_few_sizes {
+    static constexpr int OD = 64 * HP + 4, COLS = 16 * CT, QUERIES = 2 * HP * (F32 ? 3 : 1) * CT * 1024, AREA = COLS * OD * 4, ML = PAGED_FEW_WAVES * COLS * 8,
+                         WT = COLS * PAGED_MAX_PARTS * 4;
+};
+/* LDS: `queries`, and after the last product area(k), wave k's part; ml beside both, wt where nothing is once the parts have left */
+template <int HP, bool F32, bool ONCE, int CT, class AREA>
+static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *queries, AREA area, float (*ml)[16 * CT][2],
+                                              float (*wt)[PAGED_MAX_PARTS], int &last) {
     constexpr int HD = 64 * HP, ROW = 2 * HD, KS = 2 * HP, CD = HP % 2 ? 4 : 8, CHUNKS = HD / (16 * CD), OD = HD + 4, WAVES = PAGED_FEW_WAVES;
     constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 2, COLS = 16 * CT, HOW = ONCE ? 2 /* nt */ : 0;
-    __shared__ __attribute__((aligned(16))) float area[WAVES][COLS][OD];                /* the queries' operands, then the waves' parts */
-    __shared__ float ml[WAVES][COLS][2], wt[COLS][PAGED_MAX_PARTS];
-    __shared__ int last;
-    static_assert(sizeof area >= KS * NQ * CT * 1024, "operands");
-    u32x4 *queries = reinterpret_cast<u32x4 *>(area);
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     const int h = (int)blockIdx.x, heads = (int)gridDim.x;
-    const vt_paged_item it = pa_item(a.items);
+    const vt_paged_item it = pa_item(a.items, item);
     const pa_const_int *table = (const pa_const_int *)(uintptr_t)(a.tables + it.table);
     const int base = it.lo & ~(PAGED_FEW_ROWS - 1), tiles = (it.end - base + PAGED_FEW_ROWS - 1) / PAGED_FEW_ROWS;
     u32x4 k[2][KS];
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
 #pragma unroll
         for (int k = 0; k < WAVES; k++) L[c] = fmaf(ml[k][col][1], pa_exp2(ml[k][col][0] - M[c]), L[c]);
         const float f = L[c] == 0.f && it.parts > 1 ? 0.f : pa_exp2(m[c] - M[c]) / L[c];
-        float *to = &area[wave][col][4 * g * CD];
+        float *to = area(wave) + col * OD + 4 * g * CD;
 #pragma unroll
         for (int ch = 0; ch < CHUNKS; ch++)
 #pragma unroll
@@ -379,7 +387,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
         const int col = e / (HD / 4), d = 4 * (e - col * (HD / 4));
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < WAVES; k++) v = v + *reinterpret_cast<const f32x4 *>(&area[k][col][d]);
+        for (int k = 0; k < WAVES; k++) v = v + *reinterpret_cast<const f32x4 *>(area(k) + col * OD + d);
         if (it.parts == 1) result(col, d, v);
         else {
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), pd, ((it.part * COLS + col) * OD + 4 + d) * 4, 0, 16 /* sc1 */);
@@ -421,40 +429,41 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
     }
 }
 
-/* ---- many columns ------------------------------------------------------------------------------------------------
- * A workgroup has 128 columns, a wave 32, and goes through its rows 64 at a time, 16 of them each wave's to ask for, by requests that write LDS.  K's rows are the
- * A operand of
- * 32 x 32 x 16 as they lie; of V, whose rows are that operand's columns, the transposing reads of LDS give a lane four rows' values of one column.
+/* ---- many columns ----
+ * A workgroup has 128 columns, a wave 32, and goes through its rows 64 at a time, 16 of them each wave's to ask for, by requests that write LDS.  K's rows are
+ * the A operand of 32 x 32 x 16 as they lie; of V, whose rows are that operand's columns, the transposing reads of LDS give a lane four rows' values of one
+ * column.
  *
  * A unit is 32 rows.  While unit u's weights are made and multiplied, the matrix cores make unit u + 1's scores, so that K's tiles lie half a tile behind V's:
- * beside V's rows
- * 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95. */
+ * beside V's rows 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95.
+ *
+ * Matrix instructions bound it, and for bf16 the vector unit beside them, which has two values' weights to make for each: 4000 rows behind none of 32 heads of
+ * 128 fp32 (three planes of queries and of weights, 393 G multiplications and additions) 316 us, the rate of a large matrix product, bf16 155 us; 1531 rows fp32 61 us, of which the first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a
+ * window of 2048 bf16 109 us.  Matrix cores busy 64 and 47 % of the time. */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 
 /* fp32: the compiler keeps to the order that is written, in which an instruction's operands are asked for just ahead of it and no more of them wait in
  * registers than there are; bf16 has registers for its own order (four prompts in a window 112.0 us as written, 108.8 so) */
 template <bool F32> static __device__ __forceinline__ void pa_here() { if constexpr (F32) __builtin_amdgcn_sched_barrier(0); }
 
+/* Tiles with rows that some column does not see: at most 3 where the columns' rows begin to be seen and 3 where they end (fewer queries than 128 apart), or 5
+ * with a window of less.  `marks`: of such a tile the values that are not finite, 32 of a row's to a word; `odd`: where there are any. */
+#define PA_EDGES 6
 template <int HP, bool F32>
-__global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
-    constexpr int HD = 64 * HP, ROW = 2 * HD, WAVES = 4, DT = 2 * HP, KS = 4 * HP, PIECES = HD / 8;
-    constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 1, KB = 64 * ROW;
-    /* objects of their own: a read waits for the requests that write the same one */
-    __shared__ __attribute__((aligned(16))) unsigned char k0[KB], k1[KB], v0[KB], v1[KB];
-    /* Tiles with rows that some column does not see: at most 3 where the columns' rows begin to be seen and 3 where they end (fewer queries than 128
-     * apart), or 5 with a window of less */
-    constexpr int EDGES = 6;
-    __shared__ unsigned marks[EDGES][64][DT];            /* of such a tile the values that are not finite, 32 of a row's to a word; where there are any: .. */
-    __shared__ int odd[EDGES][WAVES], last;
+static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsigned char *k0, unsigned char *k1, unsigned char *v0, unsigned char *v1,
+                                               unsigned (*marks)[64][2 * HP], int (*odd)[4], int &last) {
+    constexpr int HD = 64 * HP, ROW = 2 * HD, WAVES = 4, DT = 2 * HP, KS = 4 * HP, PIECES = HD / 8, EDGES = PA_EDGES;
+    constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 1;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5;
     const int h = (int)blockIdx.x, heads = (int)gridDim.x;
-    const vt_paged_item it = pa_item(a.items);
+    const vt_paged_item it = pa_item(a.items, item);
     const pa_const_int *table = (const pa_const_int *)(uintptr_t)(a.tables + it.table);
     const int w0 = it.c0 + 32 * wave, wc = min(w0 + 32, it.cols) - w0;                   /* this wave's columns: none, perhaps */
     const int cc = min(w0 + n, it.cols - 1), qi = vt_div(cc, a.group), pos = it.past + qi;
     const int see_lo = max(a.window && pos >= a.window ? pos - a.window + 1 : 0, it.lo), see_hi = min(pos + 1, it.end);
     const int q_first = it.past + vt_div(min(w0, it.cols - 1), a.group), q_last = it.past + vt_div(min(w0 + 31, it.cols - 1), a.group);
-    const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);    /* that every column of the wave sees */
+    const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo);          /* rows that every column of the wave sees */
+    const int all_hi = min(q_first + 1, it.end);
     const int any_lo = a.window && q_first >= a.window ? q_first - a.window + 1 : 0, any_hi = wc > 0 ? min(q_last + 1, it.end) : 0;   /* .. that any does */
     const int wg_last = it.past + vt_div(min(it.c0 + PAGED_MANY_COLS, it.cols) - 1, a.group);
     const int wg_lo = max(a.window && wg_last >= a.window ? wg_last - a.window + 1 : 0, it.lo);             /* rows that every column sees */
@@ -751,6 +760,45 @@ __global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
     }
 }
 
+template <int HP, bool F32, bool ONCE, int CT>
+__global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(pa_job a) {
+    typedef pa_few_sizes<HP, F32, CT> S;
+    __shared__ __attribute__((aligned(16))) float area[PAGED_FEW_WAVES][S::COLS][S::OD];
+    __shared__ float ml[PAGED_FEW_WAVES][S::COLS][2], wt[S::COLS][PAGED_MAX_PARTS];
+    __shared__ int last;
+    static_assert(sizeof area >= S::QUERIES, "operands");
+    pa_few<HP, F32, ONCE, CT>(a, (int)blockIdx.y, reinterpret_cast<u32x4 *>(area), [&](int k) { return &area[k][0][0]; }, ml, wt, last);
+}
+
+/* objects of their own: a read waits for the requests that write the same one */
+#define PA_MANY_LDS(HP)                                                                                                               \
+    __shared__ __attribute__((aligned(16))) unsigned char k0[64 * 128 * HP], k1[64 * 128 * HP], v0[64 * 128 * HP], v1[64 * 128 * HP]; \
+    __shared__ __attribute__((aligned(16))) unsigned marks[PA_EDGES][64][2 * HP];                                                     \
+    __shared__ int odd[PA_EDGES][4], last;
+
+template <int HP, bool F32>
+__global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
+    PA_MANY_LDS(HP)
+    pa_many<HP, F32>(a, (int)blockIdx.y, k0, k1, v0, v1, marks, odd, last);
+}
+
+/* Prompts and steps in one launch, an item either kernel's work: what reads memory and what multiplies share the CUs.  One behind the other / so: 512 rows
+ * behind 1500 with 31 steps behind up to 1999 bf16 59 / 42 us, with steps behind 60 to 9000 71 / 53 (fp32 88 / 72), 300 behind 6000 with three behind 10000
+ * to 30000 90 / 72. */
+template <int HP, bool F32, bool ONCE>
+__global__ void __launch_bounds__(256, 2) vt_paged_both_kernel(pa_job a) {
+    typedef pa_few_sizes<HP, F32, 1> S;
+    PA_MANY_LDS(HP)
+    static_assert(S::QUERIES <= sizeof k0 && S::AREA <= sizeof k0 && S::ML <= sizeof marks && S::WT <= sizeof k0, "LDS");
+    const int y = (int)blockIdx.y;
+    if (pa_item(a.items, y).many) pa_many<HP, F32>(a, y, k0, k1, v0, v1, marks, odd, last);
+    else
+        pa_few<HP, F32, ONCE, 1>(a, y, reinterpret_cast<u32x4 *>(k0),
+                                 [&](int k) { return reinterpret_cast<float *>(k == 0 ? k0 : k == 1 ? k1 : k == 2 ? v0 : v1); },
+                                 reinterpret_cast<float (*)[16][2]>(marks),
+                                 reinterpret_cast<float (*)[PAGED_MAX_PARTS]>(k0), last);
+}
+
 /* items are the grid's second dimension, of at most 65535 */
 template <class F>
 static void pa_items(const pa_job &job, int from, int n, int heads, F launch) {
@@ -763,6 +811,14 @@ static void pa_items(const pa_job &job, int from, int n, int heads, F launch) {
 
 template <int HP, bool F32>
 static void pa_launch(const pa_job &job, const vt_paged_plan &p, int heads) {
+    if constexpr (HP <= 2) {
+        if (p.both) {
+            const dim3 grid((unsigned)heads, (unsigned)(p.few + p.many));
+            if (p.once) hipLaunchKernelGGL((vt_paged_both_kernel<HP, F32, true>), grid, dim3(256), 0, g_vt.stream, job);
+            else hipLaunchKernelGGL((vt_paged_both_kernel<HP, F32, false>), grid, dim3(256), 0, g_vt.stream, job);
+            return;
+        }
+    }
     pa_items(job, 0, p.few, heads, [&](const pa_job &a, const dim3 &grid) {
         const dim3 threads(64 * PAGED_FEW_WAVES);
         if constexpr (HP <= 2) {
@@ -794,13 +850,13 @@ extern "C" int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16,
     const int group = s.n_heads / s.n_kv_heads;
     int page_log = 4;
     while (1 << page_log < s.page_rows) page_log++;
-    const size_t few = (size_t)b->plan.few_slots * s.n_kv_heads * (b->plan.wide ? 32 : 16) * (s.head_dim + 4) * 4;
-    const size_t many = (size_t)b->plan.many_slots * s.n_kv_heads * 4 * (8 * HP + 1) * 1024;
+    const vt_paged_plan &p = b->plan;
+    const long long few = p.few_slots * vt_paged_few_part(s, p.wide ? 32 : 16), many = p.many_slots ? (p.many_slot + p.many_slots) * vt_paged_many_part(s) : 0;
     pa_job job = {(const uint16_t *)d_k_pages, (const uint16_t *)d_v_pages, d_Q, d_out, NULL, g_vt.d_mx4_cnt, (const vt_paged_item *)(b->dev + b->at_items),
                   (const int *)(b->dev + b->at_tables), q_stride, s.n_heads, page_log, s.window, vt_divisor_of(group, (long long)b->max_rows * group),
                   scale * 1.44269504f};
-    if ((few || many) && !(job.part = (float *)vt_scratch(few > many ? few : many))) return -1;
-#define ATTEND(H) (x_bf16 ? pa_launch<H, false>(job, b->plan, s.n_kv_heads) : pa_launch<H, true>(job, b->plan, s.n_kv_heads))
+    if ((few || many) && !(job.part = (float *)vt_scratch((size_t)(few > many ? few : many) * s.n_kv_heads))) return -1;
+#define ATTEND(H) (x_bf16 ? pa_launch<H, false>(job, p, s.n_kv_heads) : pa_launch<H, true>(job, p, s.n_kv_heads))
     switch (HP) {
     case 1: ATTEND(1); break;
     case 2: ATTEND(2); break;

@@ -27,7 +27,7 @@
 
 /* What a workgroup does for every kv head: columns c0 .. of a sequence whose new rows are `row` .. of the batch and lie behind `past` rows, over the
  * cache's rows lo .. end - 1; `parts` of them make up the columns' result, in slots `slot` .. */
-struct vt_paged_item { int row, past, cols, table, c0, lo, end, slot, part, parts, counter, spare; };
+struct vt_paged_item { int row, past, cols, table, c0, lo, end, slot, part, parts, counter, many; };
 
 struct vt_paged_shape { int n_pages, page_rows, n_heads, n_kv_heads, head_dim, window; };
 
@@ -98,7 +98,7 @@ static inline vt_paged_fault vt_paged_lay_out(const vt_paged_shape &s, int max_s
 
 /* items of either kernel (the few's first), parts that they leave; wide: the few's columns go by 32; once: their rows are read by one workgroup each, more
  * of them than a cache holds */
-struct vt_paged_plan { int few, many, few_slots, many_slots, wide, once; };
+struct vt_paged_plan { int few, many, few_slots, many_slot, many_slots, wide, once, both; };
 
 /* Which kernels a batch goes to: `any`, whether there are sequences for the one for many columns; columns of a workgroup of the other, whether its rows are
  * read by one workgroup only, and their bytes */
@@ -179,17 +179,27 @@ static const vt_paged_cost vt_paged_few_cost[4] = {{4, 1.1f, 0.8f, 2.55f, 2.85f,
 static const vt_paged_cost vt_paged_wide_cost[2] = {{3, 1.4f, 0.32f, 0.7f, 2.5f, 0.16f, 0.39f}, {2, 0.85f, 0.42f, 1.09f, 4.85f, 0.07f, 0.08f}};
 static const vt_paged_cost vt_paged_many_cost[2] = {{2, 7.9f, 1.9f, 3.0f, 5.0f, 1.0f, 0.45f}, {2, 9.25f, 2.2f, 3.8f, 3.6f, 2.2f, 0.24f}};
 
-static inline int vt_paged_run(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows, int unit) {
-    const vt_paged_cost &c = (many ? vt_paged_many_cost : kinds.few_cols == 32 ? vt_paged_wide_cost : vt_paged_few_cost)[s.head_dim / 64 - 1];
-    long long longest = 1;
-    vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int, int, int first, int end) {
-        const long long n = vt_paged_parts(first, end, unit, 1);
-        longest = n > longest ? n : longest;
-    });
-    int best = (int)longest;
-    double least = 1e300;
-    for (int parts = 1; parts <= PAGED_MAX_PARTS; parts += parts < 16 ? 1 : parts / 8) {
+static const vt_paged_cost &vt_paged_cost_of(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many) {
+    return (many ? vt_paged_many_cost : kinds.few_cols == 32 ? vt_paged_wide_cost : vt_paged_few_cost)[s.head_dim / 64 - 1];
+}
+
+/* A kernel's part of a batch in runs of `run` units at most: its workgroups and their units, us of all of them; the longest one's units, whether it leaves a
+ * part; us of the merge */
+struct vt_paged_try { int run; double wgs, units, all, most, late, merge; };
+#define PAGED_TRIES 40
+static inline int vt_paged_tries(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_seqs, const int *past, const int *rows, vt_paged_try *to) {
+    const int unit = many ? PAGED_MANY_ROWS : PAGED_FEW_ROWS * PAGED_FEW_WAVES;
+    const vt_paged_cost &c = vt_paged_cost_of(s, kinds, many);
+    long long longest = 0;
+    if (!many || kinds.any)
+        vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int, int, int first, int end) {
+            const long long n = vt_paged_parts(first, end, unit, 1);
+            longest = n > longest ? n : longest;
+        });
+    int tries = 0;
+    for (int parts = 1; longest && parts <= PAGED_MAX_PARTS; parts += parts < 16 ? 1 : parts / 8) {
         const int run = (int)((longest + parts - 1) / parts);
+        if (tries && to[tries - 1].run == run) continue;
         long long items = 0, extra = 0, split = 0, most = 0, all = 0;
         int late = 0;
         vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int, int, int first, int end) {
@@ -199,16 +209,46 @@ static inline int vt_paged_run(const vt_paged_shape &s, const vt_paged_kinds &ki
             if (p > 1) { extra += p; split++; }
             if (each > most || (each == most && p > 1)) { late = p > 1; most = each; }
         });
-        if (extra > PAGED_SPLIT_ITEMS || split * s.n_kv_heads > PAGED_COUNTERS) break;
-        const double wgs = (double)items * s.n_kv_heads, room = (double)n_cu * c.beside;
-        const double full = ceil(wgs / n_cu) - 1, share = full < c.beside - 1 ? full / (c.beside - 1) : 1.0;          /* of the CU that has most of them */
-        const double one = c.fixed + most * (c.alone + (c.step - c.alone) * share) + late * c.part;
-        const double sum = (items * c.fixed + all * c.step + extra * c.part) * s.n_kv_heads / room + (wgs > room ? c.tail * one : 0.0);
-        const double us = (one > sum ? one : sum) + (split ? c.merge * parts : 0.0);
-        if (us < least) { least = us; best = run; }
+        if (extra > PAGED_SPLIT_ITEMS || split > PAGED_COUNTERS / 2 / s.n_kv_heads) break;
+        const double heads = s.n_kv_heads, us = (double)items * c.fixed + (double)all * c.step + (double)extra * c.part;
+        to[tries++] = vt_paged_try{run, items * heads, all * heads, us * heads, (double)most, (double)late, split ? c.merge * parts : 0.0};
         if (run == 1) break;
     }
-    return best;
+    return tries;
+}
+/* us of the longest one, by the share of the CU that has most of them; `slow`: a unit's time by what else is there */
+static inline double vt_paged_one(const vt_paged_cost &c, const vt_paged_try &t, int n_cu, double slow) {
+    const double full = ceil(t.wgs / n_cu) - 1, share = full < c.beside - 1 ? full / (c.beside - 1) : 1.0;
+    return c.fixed + t.most * slow * (c.alone + (c.step - c.alone) * share) + t.late * c.part;
+}
+
+/* The runs of both kernels.  In one launch they share the CUs: a workgroup of many columns runs better beside one of few than beside another, and fewer of them
+ * that leave no parts do best.  The factors are fitted to 30 pairs of runs of nine batches; the pair that they choose is behind the best one by 1 % on average. */
+static inline void vt_paged_runs(const vt_paged_shape &s, const vt_paged_kinds &kinds, int n_cu, int n_seqs, const int *past, const int *rows, int *runs) {
+    vt_paged_try t[2][PAGED_TRIES];
+    int n[2];
+    for (int k = 0; k < 2; k++) {
+        n[k] = vt_paged_tries(s, kinds, k, n_seqs, past, rows, t[k]);
+        const vt_paged_cost &c = vt_paged_cost_of(s, kinds, k && kinds.any);
+        double least = 1e300;
+        runs[k] = 1;
+        for (int i = 0; i < n[k]; i++) {
+            const double room = (double)n_cu * c.beside, one = vt_paged_one(c, t[k][i], n_cu, 1);
+            const double sum = t[k][i].all / room + (t[k][i].wgs > room ? c.tail * one : 0.0), us = (one > sum ? one : sum) + t[k][i].merge;
+            if (us < least) { least = us; runs[k] = t[k][i].run; }
+        }
+    }
+    if (!n[0] || !n[1] || kinds.few_cols != 16) return;
+    const vt_paged_cost &c = vt_paged_cost_of(s, kinds, false), &d = vt_paged_cost_of(s, kinds, true);
+    double least = 1e300;
+    for (int i = 0; i < n[0]; i++)
+        for (int j = 0; j < n[1]; j++) {
+            const vt_paged_try &x = t[0][i], &y = t[1][j];
+            const double a = c.fixed + 0.8 * x.most * c.step + x.late * c.part, b = vt_paged_one(d, y, n_cu, 0.65), one = a > b ? a : b;
+            const double sum = (0.9 * x.all + y.all - 0.45 * y.units * d.step) / (2 * n_cu) + (x.wgs + y.wgs > 2 * n_cu ? 0.1 * (a < b ? a : b) : 0.0);
+            const double us = (one > sum ? one : sum) + 0.15 * a + (x.merge > y.merge ? x.merge : y.merge);
+            if (us < least) { least = us; runs[0] = x.run; runs[1] = y.run; }
+        }
 }
 
 static int vt_paged_longest(const void *a, const void *b) {
@@ -220,37 +260,54 @@ static int vt_paged_longest(const void *a, const void *b) {
     return x->part < y->part ? -1 : x->part > y->part;
 }
 
+/* .. of both kernels: the few's units, of 128 rows, take about as long as the many's, of 64 */
+static int vt_paged_slowest(const void *a, const void *b) {
+    const vt_paged_item *x = (const vt_paged_item *)a, *y = (const vt_paged_item *)b;
+    const int n = (x->end - x->lo) << x->many, m = (y->end - y->lo) << y->many;
+    if (n != m) return n > m ? -1 : 1;
+    return x->many != y->many ? (x->many ? -1 : 1) : vt_paged_longest(a, b);
+}
+
 /* Items of one kernel into `to`, the longest first; -> how many, and their slots */
-static inline int vt_paged_items(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_cu, int n_seqs, const int *past, const int *rows,
-                                 const int *starts, vt_paged_item *to, int *n_slots) {
+static inline int vt_paged_items(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int run, int n_seqs, const int *past, const int *rows,
+                                 const int *starts, vt_paged_item *to, int slot, int *n_slots) {
     const int unit = many ? PAGED_MANY_ROWS : PAGED_FEW_ROWS * PAGED_FEW_WAVES, group = s.n_heads / s.n_kv_heads;
     *n_slots = 0;
     if (many && !kinds.any) return 0;
-    const int run = vt_paged_run(s, kinds, many, n_cu, n_seqs, past, rows, unit);
-    int n = 0, slots = 0, counters = 0, row = 0, seq = 0;
+    int n = 0, slots = slot, counters = many ? PAGED_COUNTERS / 2 / s.n_kv_heads : 0, row = 0, seq = 0;
     vt_paged_tiles(s, kinds, many, n_seqs, past, rows, [&](int i, int c0, int first, int end) {
         while (seq < i) row += rows[seq++];
         const int units = vt_paged_parts(first, end, unit, 1), parts = (units + run - 1) / run, u0 = first / unit;
         for (int p = 0; p < parts; p++) {
             const int from = (int)((long long)units * p / parts), till = (int)((long long)units * (p + 1) / parts);
             to[n++] = vt_paged_item{row, past[i], rows[i] * group, starts[i], c0, p ? (u0 + from) * unit : first, p + 1 < parts ? (u0 + till) * unit : end,
-                                    slots, p, parts, counters, 0};
+                                    slots, p, parts, counters, many};
         }
         if (parts > 1) { slots += parts; counters++; }
     });
     qsort(to, n, sizeof *to, vt_paged_longest);
-    *n_slots = slots;
+    *n_slots = slots - slot;
     return n;
 }
 
+/* bytes of a part of one head */
+static inline long long vt_paged_few_part(const vt_paged_shape &s, int cols) { return (long long)cols * (s.head_dim + 4) * 4; }
+static inline long long vt_paged_many_part(const vt_paged_shape &s) { return 4ll * (s.head_dim / 8 + 1) * 1024; }
+
 static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to) {
-    vt_paged_plan p = {0, 0, 0, 0, 0, 0};
+    vt_paged_plan p = {0, 0, 0, 0, 0, 0, 0, 0};
     const vt_paged_kinds kinds = vt_paged_kinds_of(s, n_cu, n_seqs, past, rows);
-    p.few = vt_paged_items(s, kinds, false, n_cu, n_seqs, past, rows, starts, to, &p.few_slots);
-    p.many = vt_paged_items(s, kinds, true, n_cu, n_seqs, past, rows, starts, to + p.few, &p.many_slots);
+    int runs[2];
+    vt_paged_runs(s, kinds, n_cu, n_seqs, past, rows, runs);
+    p.few = vt_paged_items(s, kinds, false, runs[0], n_seqs, past, rows, starts, to, 0, &p.few_slots);
+    const long long part = vt_paged_few_part(s, kinds.few_cols) * p.few_slots, each = vt_paged_many_part(s);
+    p.many_slot = (int)((part + each - 1) / each);
+    p.many = vt_paged_items(s, kinds, true, runs[1], n_seqs, past, rows, starts, to + p.few, p.many_slot, &p.many_slots);
+    p.both = p.few && p.many && p.few + p.many <= 65535 && kinds.few_cols == 16;
+    if (p.both) qsort(to, p.few + p.many, sizeof *to, vt_paged_slowest);
     p.wide = kinds.few_cols > 16;
     /* Requests that leave nothing behind in the caches: 65535 rows of 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows, which the
-     * caches (32 MB of L2) keep for the next call on them, 6.8 -> 7.2. */
+     * caches (32 MB of L2) keep for the next call on them, 6.8 -> 7.2.  Beside a prompt as well: 31 sequences 43.4 -> 41.3, three of 10000 to 30000 76 -> 72. */
     p.once = kinds.once && kinds.bytes >= PAGED_CACHED;
     return p;
 }
