@@ -430,14 +430,17 @@ int tts_hip_rotary(void *d_out, const void *d_x, int x_bf16, int rows, int n_hea
 int tts_hip_paged_append(const tts_hip_paged_t *batch, void *d_k_pages, void *d_v_pages, const void *d_K, const void *d_V, int x_bf16,
                          int stride, const tts_hip_rotary_t *how);
 /* Causal attention of the new rows over their sequences: the query at position p sees the rows 0 .. p, or the last `window` of them, its own
- * among them (append first).  Q [rows, n_heads * head_dim], q_stride values from row to row (0: dense, else a multiple of 8), out dense and of Q's type, both on 16 bytes;
- * they do not overlap.  scale > 0.  What a query does not see changes nothing in its result, whatever it holds: rows of its pages behind the
- * last one are not even read.  A query with an infinity or a NaN in it, and one that sees a key with a NaN, gives NaN; a key's infinity
- * makes NaN too, or, where the score is -infinity, may leave the key without weight.  A value's infinity or NaN that a
- * query sees makes that value of its result infinite or NaN.  Sums and softmax statistics are fp32.  fp32: queries (times scale) and
- * weights enter to 24 bits, results are off by some 1e-7 of their norm; a score that leaves fp32 makes NaN.  bf16: a weight is rounded to bf16 once for more
- * than 64 queries times heads on a kv head, and results once.  Where several workgroups share a sequence's rows their parts meet in the library's work
- * area, which grows by allocation when a call needs more than any before it and stays. */
+ * among them (append first).  Q [rows, n_heads * head_dim], q_stride values from row to row (0: dense, else a multiple of 8), out dense and of
+ * Q's type, both on 16 bytes; they do not overlap.  scale > 0.
+ * What a query does not see changes nothing in its result, whatever it holds: rows of its pages behind the last one are not even read.  A query
+ * with an infinity or a NaN in it, and one that sees a key with a NaN, gives NaN; a key's infinity makes NaN too, or, where the score is
+ * -infinity, may leave the key without weight.  A value's infinity or NaN that a query sees makes that value of its result infinite or NaN.
+ * Sums and softmax statistics are fp32, and what leaves them on the way (scores, or values times more than 2^8 of weight) gives NaN or infinity;
+ * products below 2^-126 may count as 0.  fp32: queries times scale and weights enter to 24 bits, results are off by some 1e-7 of their norm.
+ * bf16: where a call has enough queries for the matrix kernel a weight is rounded to bf16 once, else to 16 bits, and results once.  A call's
+ * results are the same bits each time; beside other sequences in the batch the same query's may differ by these roundings, as the kernel and
+ * the parts that its rows are read in are chosen for the batch.  Where several workgroups share a sequence's rows their parts meet in the
+ * library's work area, which grows by allocation when a call needs more than any before it and stays. */
 int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16, int q_stride, const tts_hip_paged_t *batch, const void *d_k_pages,
                             const void *d_v_pages, float scale);
 
