@@ -185,13 +185,13 @@ def attention(cache, q, bf16, scale, q_gap=0):
     return (value16(got) if bf16 else got).reshape(q.shape)
 
 
-def is_many(cache, i):
+def is_many(cache, i, bf16):
     """The kernel that rounds a bf16 batch's weights to bf16 (vt_paged_any_many)."""
     group = cache.heads // cache.kv_heads
-    if cache.hd > 128:
+    if cache.hd > 128 and not (cache.hd == 256 and bf16):
         return False
     all_of_them = sum(r * group * min(p + r / 2, cache.window or math.inf) * cache.kv_heads * cache.hd for r, p in zip(cache.rows, cache.past) if r * group > 64)
-    return all_of_them >= 2.5e9 and cache.rows[i] * group > 64
+    return all_of_them >= (2.5e9 if cache.hd <= 128 else 1.3e9) and cache.rows[i] * group > 64
 
 
 def check(cache, got, want, size, most, bf16, keep=None):
@@ -206,7 +206,7 @@ def check(cache, got, want, size, most, bf16, keep=None):
     if bf16:
         at = 0
         for i, r in enumerate(cache.rows):
-            rel[at:at + r] += 2.0 ** -8 if is_many(cache, i) else 2.0 ** -16
+            rel[at:at + r] += 2.0 ** -8 if is_many(cache, i, bf16) else 2.0 ** -16
             at += r
     if keep is not None:
         got, want, size, rel = got[keep], want[keep], size[keep], rel[keep]

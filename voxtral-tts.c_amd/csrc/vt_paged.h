@@ -18,7 +18,8 @@ struct tts_hip_paged {
     int *starts, *written;
     /* the batch, and how it is worked on; n_seqs -1: none yet */
     int n_seqs, n_rows;
-    vt_paged_plan plan;
+    vt_paged_plan plan[2];               /* for fp32 and bf16 queries */
+    int bf16_items;                      /* the second one's first item */
 };
 
 int vt_paged_ready(const char *who, const tts_hip_paged *b);      /* a batch of this context's device; else an error */

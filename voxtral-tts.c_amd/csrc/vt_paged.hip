@@ -43,7 +43,7 @@ extern "C" tts_hip_paged_t *tts_hip_paged_create(const tts_hip_paged_shape_t *sh
     b->max_seqs = max_seqs;
     b->max_rows = max_rows;
     b->max_table = max_table;
-    b->max_items = (int)vt_paged_max_items(max_seqs, max_rows, group);
+    b->max_items = (int)vt_paged_max_items(max_seqs, max_rows, group) << vt_paged_type_matters(s);
     b->device = b->n_seqs = -1;
     b->described = paged_up(sizeof(int) * (size_t)max_rows) + paged_up(2 * sizeof(int) * (size_t)max_rows) + paged_up(sizeof(int) * (size_t)max_table);
     b->bytes = b->described + sizeof(vt_paged_item) * (size_t)b->max_items;
@@ -122,8 +122,17 @@ extern "C" int tts_hip_paged_set(tts_hip_paged_t *b, int n_seqs, const int *past
         free(host);
     }
     if (bad) return -1;
-    b->plan = vt_paged_plan_of(b->shape, g_vt.n_cu > 0 ? g_vt.n_cu : 256, n_seqs, past, rows, b->starts, (vt_paged_item *)(b->host + b->at_items));
-    const size_t all = b->at_items + sizeof(vt_paged_item) * (size_t)(b->plan.few + b->plan.many);
+    vt_paged_item *items = (vt_paged_item *)(b->host + b->at_items);
+    const int n_cu = g_vt.n_cu > 0 ? g_vt.n_cu : 256;
+    b->plan[0] = b->plan[1] = vt_paged_plan_of(b->shape, false, n_cu, n_seqs, past, rows, b->starts, items);
+    int n_items = b->plan[0].few + b->plan[0].many;
+    b->bf16_items = 0;
+    if (vt_paged_type_matters(b->shape)) {
+        b->bf16_items = n_items;
+        b->plan[1] = vt_paged_plan_of(b->shape, true, n_cu, n_seqs, past, rows, b->starts, items + n_items);
+        n_items += b->plan[1].few + b->plan[1].many;
+    }
+    const size_t all = b->at_items + sizeof(vt_paged_item) * (size_t)n_items;
     if (n_rows && vt_check(hipMemcpyAsync(b->dev, b->host, all, hipMemcpyHostToDevice, g_vt.stream), who)) return -1;
     if (vt_check(hipEventRecord(b->copied, g_vt.stream), who)) return -1;
     b->n_rows = n_rows;

@@ -430,16 +430,18 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
 }
 
 /* ---- many columns ----
- * A workgroup has 128 columns, a wave 32, and goes through its rows 64 at a time, 16 of them each wave's to ask for, by requests that write LDS.  K's rows are
- * the A operand of 32 x 32 x 16 as they lie; of V, whose rows are that operand's columns, the transposing reads of LDS give a lane four rows' values of one
- * column.
+ * A workgroup has 128 columns, a wave 32, and goes through its rows 64 at a time, 16 of them each wave's to ask for, by requests that write LDS.  K's rows
+ * are the A operand of 32 x 32 x 16 as they lie; of V, whose rows are that operand's columns, the transposing reads of LDS give a lane four rows' values of
+ * one column.
  *
- * A unit is 32 rows.  While unit u's weights are made and multiplied, the matrix cores make unit u + 1's scores, so that K's tiles lie half a tile behind V's:
- * beside V's rows 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95.
+ * A unit is 32 rows.  While unit u's weights are made and multiplied, the matrix cores make unit u + 1's scores, so that K's tiles lie half a tile behind
+ * V's: beside V's rows 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95.
  *
- * Matrix instructions bound it, and for bf16 the vector unit beside them, which has two values' weights to make for each: 4000 rows behind none of 32 heads of
- * 128 fp32 (three planes of queries and of weights, 393 G multiplications and additions) 316 us, the rate of a large matrix product, bf16 155 us; 1531 rows fp32 61 us, of which the first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a
- * window of 2048 bf16 109 us.  Matrix cores busy 64 and 47 % of the time. */
+ * Matrix instructions bound it, and for bf16 the vector unit beside them, which has two values' weights to make for each: 4000 rows behind none of 32 heads
+ * of 128 fp32 (three planes of queries and of weights, 393 G multiplications and additions) 316 us, the rate of a large matrix product, bf16 155 us; 1531
+ * rows fp32 61 us, of which the first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a window of 2048 bf16 109 us.  Matrix cores
+ * busy 64 and 47 % of the time.  Heads of 256 bf16 values have one workgroup to a CU, for its LDS and registers: 3000 rows of 12 on 4 behind none 117 us
+ * (55 G). */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 
 /* fp32: the compiler keeps to the order that is written, in which an instruction's operands are asked for just ahead of it and no more of them wait in
@@ -475,9 +477,9 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
     for (int ks = 0; ks < KS; ks++) pa_query_load<F32>(a.Q, (size_t)(it.row + qi) * a.q_stride + head_at * HD + 16 * ks + 8 * g, raw[ks]);
     /* Pieces of 16 bytes change places within a row, so that what is read at once lies in different banks: K's with the row's last bits, so that 16 (8)
      * rows' same piece do; V's fours of them, so that four rows' same 64 bytes do. */
-    constexpr int SWAP = PIECES - 1;
+    constexpr int SWAP = PIECES < 16 ? PIECES - 1 : 15;
     auto v_swap = [](int r) { return HP == 1 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); };
-    int k_at[4], v_at[4];                                /* DT of them (with that size the host pass drops the kernel) */
+    int k_at[8], v_at[8];                                /* DT of them (with that size the host pass drops the kernel) */
 #pragma unroll
     for (int d = 0; d < DT; d++) {
         const int u = d * 64 + lane, r = u / PIECES;
@@ -497,7 +499,7 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
     auto v_place = [&](int t) __attribute__((always_inline)) {
         return pa_rows_of(__builtin_amdgcn_readlane(v_page, t & 63), base + 64 * t + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW);
     };
-    auto load = [&](const uint16_t *pool, const pa_rows &at, const int (&from)[4], unsigned char *to) __attribute__((always_inline)) {
+    auto load = [&](const uint16_t *pool, const pa_rows &at, const int (&from)[8], unsigned char *to) __attribute__((always_inline)) {
         const __amdgpu_buffer_rsrc_t d = vt_buffer(pool + at.row * HD, at.bytes);
 #pragma unroll
         for (int i = 0; i < DT; i++)
@@ -777,7 +779,7 @@ __global__ void __launch_bounds__(64 * PAGED_FEW_WAVES, 2) vt_paged_few_kernel(p
     __shared__ int odd[PA_EDGES][4], last;
 
 template <int HP, bool F32>
-__global__ void __launch_bounds__(256, 2) vt_paged_many_kernel(pa_job a) {
+__global__ void __launch_bounds__(256, HP <= 2 ? 2 : 1) vt_paged_many_kernel(pa_job a) {
     PA_MANY_LDS(HP)
     pa_many<HP, F32>(a, (int)blockIdx.y, k0, k1, v0, v1, marks, odd, last);
 }
@@ -827,7 +829,7 @@ static void pa_launch(const pa_job &job, const vt_paged_plan &p, int heads) {
         if (p.once) hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, true, 1>), grid, threads, 0, g_vt.stream, a);
         else hipLaunchKernelGGL((vt_paged_few_kernel<HP, F32, false, 1>), grid, threads, 0, g_vt.stream, a);
     });
-    if constexpr (HP <= 2)
+    if constexpr (HP <= 2 || (HP == 4 && !F32))
         pa_items(job, p.few, p.many, heads,
                  [](const pa_job &a, const dim3 &grid) { hipLaunchKernelGGL((vt_paged_many_kernel<HP, F32>), grid, dim3(256), 0, g_vt.stream, a); });
 }
@@ -850,10 +852,11 @@ extern "C" int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16,
     const int group = s.n_heads / s.n_kv_heads;
     int page_log = 4;
     while (1 << page_log < s.page_rows) page_log++;
-    const vt_paged_plan &p = b->plan;
+    const vt_paged_plan &p = b->plan[x_bf16 != 0];
     const long long few = p.few_slots * vt_paged_few_part(s, p.wide ? 32 : 16), many = p.many_slots ? (p.many_slot + p.many_slots) * vt_paged_many_part(s) : 0;
-    pa_job job = {(const uint16_t *)d_k_pages, (const uint16_t *)d_v_pages, d_Q, d_out, NULL, g_vt.d_mx4_cnt, (const vt_paged_item *)(b->dev + b->at_items),
-                  (const int *)(b->dev + b->at_tables), q_stride, s.n_heads, page_log, s.window, vt_divisor_of(group, (long long)b->max_rows * group),
+    pa_job job = {(const uint16_t *)d_k_pages, (const uint16_t *)d_v_pages, d_Q, d_out, NULL, g_vt.d_mx4_cnt,
+                  (const vt_paged_item *)(b->dev + b->at_items) + (x_bf16 ? b->bf16_items : 0), (const int *)(b->dev + b->at_tables),
+                  q_stride, s.n_heads, page_log, s.window, vt_divisor_of(group, (long long)b->max_rows * group),
                   scale * 1.44269504f};
     if ((few || many) && !(job.part = (float *)vt_scratch((size_t)(few > many ? few : many) * s.n_kv_heads))) return -1;
 #define ATTEND(H) (x_bf16 ? pa_launch<H, false>(job, p, s.n_kv_heads) : pa_launch<H, true>(job, p, s.n_kv_heads))

@@ -108,20 +108,27 @@ static inline long long vt_paged_max_items(int max_seqs, int max_rows, int group
     return (long long)max_rows * group / 16 + max_seqs + 2 * PAGED_SPLIT_ITEMS;
 }
 
-/* Which sequences go to the kernel for many columns: those of more than 64 whose heads of up to 128 values leave it registers, where there is enough for it
- * to do, as columns times the rows that they see on average times kv heads times values, over all of them.  It does twice as much with what it reads, but
- * by few workgroups.  Measured, us with the kernel for few columns, 32 at a time, and for many (fp32 / bf16), 32 heads on 8 of 128: 450 rows behind 200
- * (0.8e9) 18 / 16 and 26 / 19, 700 behind none (1.0e9) 24 / 20 and 27 / 19, 200 behind 2000 (1.7e9) 32 / 24 and 38 / 26, 50 behind 16000 (3.3e9) 52 / 48
- * and 60 / 43, 512 behind 1500 (3.7e9) 45 / 39 and 49 / 32, 100 behind 500 sixteen times (3.6e9) 59 / 47 and 49 / 29; 16 heads of 64: 512 behind 1500
- * (0.9e9) 21 / 17 and 24 / 18. Else 32 columns to a workgroup, not 16, where there is enough for that, as columns / 16 times rows times kv heads times
- * values (less where every CU has one of 16); 16 and 32 at a time: 37 rows behind 300 (3e6) 7.0 / 6.4 and 9.9 / 8.2, 100 behind 1000 (27e6) 13 / 13 and 19
- * / 15, 37 behind 4000 (41e6) 21 / 21 and 23 / 20, 16 behind 300 32 times (40e6) 22 / 22 and 17 / 14, 200 behind 2000 (107e6) 42 / 41 and 32 / 24; 16 heads
- * of 64: 37 behind 4000 (12e6) 14 / 13 and 17 / 16, 512 behind 1500 (57e6) 24 / 23 and 21 / 17. */
+/* Which sequences go to the kernel for many columns: those of more than 64, where there is enough for it to do, as columns times the rows that they see on
+ * average times kv heads times values, over all of them.  It does twice as much with what it reads, but by few workgroups.  Measured, us with the kernel
+ * for few columns, 32 at a time, and for many (fp32 / bf16), 32 heads on 8 of 128: 450 rows behind 200 (0.8e9) 18 / 16 and 26 / 19, 700 behind none (1.0e9)
+ * 24 / 20 and 27 / 19, 200 behind 2000 (1.7e9) 32 / 24 and 38 / 26, 50 behind 16000 (3.3e9) 52 / 48 and 60 / 43, 512 behind 1500 (3.7e9) 45 / 39 and 49 /
+ * 32, 100 behind 500 sixteen times (3.6e9) 59 / 47 and 49 / 29; 16 heads of 64: 512 behind 1500 (0.9e9) 21 / 17 and 24 / 18.  Heads of 256 values leave it
+ * registers if they are bf16: 12 on 4, 300 behind 1000 (1.1e9) 28 and 33, 1000 behind none (1.5e9) 38 and 31, 200 behind 3000 (1.9e9) 50 and 43, 512 behind
+ * 1500 (2.8e9) 69 and 40, 3000 behind none (14e9) 247 and 117; fp32 it keeps some in memory and 3000 take 250 and 344.  Heads of 192 do not lie as it reads
+ * them.
+ *
+ * Else 32 columns to a workgroup, not 16, where there is enough for that, as columns / 16 times rows times kv heads times values (less where every CU has
+ * one of 16); 16 and 32 at a time: 37 rows behind 300 (3e6) 7.0 / 6.4 and 9.9 / 8.2, 100 behind 1000 (27e6) 13 / 13 and 19 / 15, 37 behind 4000 (41e6) 21 /
+ * 21 and 23 / 20, 16 behind 300 32 times (40e6) 22 / 22 and 17 / 14, 200 behind 2000 (107e6) 42 / 41 and 32 / 24; 16 heads of 64: 37 behind 4000 (12e6) 14
+ * / 13 and 17 / 16, 512 behind 1500 (57e6) 24 / 23 and 21 / 17. */
 #define PAGED_MANY_FROM 2.5e9
+#define PAGED_MANY_FROM_256 1.3e9
 #define PAGED_WIDE_FROM 45e6
 #define PAGED_WIDE_FULL 30e6
-static inline bool vt_paged_may_be_many(int hp, long long cols) { return hp <= 2 && cols > 64; }
-static inline vt_paged_kinds vt_paged_kinds_of(const vt_paged_shape &s, int n_cu, int n_seqs, const int *past, const int *rows) {
+static inline bool vt_paged_may_be_many(int hp, long long cols) { return hp != 3 && cols > 64; }
+/* .. and both kernels be one launch's */
+static inline bool vt_paged_may_be_both(const vt_paged_shape &s, const vt_paged_kinds &kinds) { return s.head_dim <= 128 && kinds.few_cols == 16; }
+static inline vt_paged_kinds vt_paged_kinds_of(const vt_paged_shape &s, bool bf16, int n_cu, int n_seqs, const int *past, const int *rows) {
     const int group = s.n_heads / s.n_kv_heads, hp = s.head_dim / 64;
     double many = 0, wide = 0, wgs = 0;
     long long most = 0;
@@ -130,7 +137,7 @@ static inline vt_paged_kinds vt_paged_kinds_of(const vt_paged_shape &s, int n_cu
         const double seen = past[i] + 0.5 * rows[i], each = (s.window && seen > s.window ? s.window : seen) * s.n_kv_heads * s.head_dim;
         if (vt_paged_may_be_many(hp, cols)) many += (double)cols * each;
     }
-    vt_paged_kinds k = {many >= PAGED_MANY_FROM, 16, false, 0};
+    vt_paged_kinds k = {hp <= 2 ? many >= PAGED_MANY_FROM : bf16 && many >= PAGED_MANY_FROM_256, 16, false, 0};
     for (int i = 0; i < n_seqs; i++) {
         const long long cols = (long long)rows[i] * group;
         const double seen = past[i] + 0.5 * rows[i], each = (s.window && seen > s.window ? s.window : seen) * s.n_kv_heads * s.head_dim;
@@ -177,14 +184,15 @@ struct vt_paged_cost { int beside; float fixed, alone, step, part, merge, tail; 
 static const vt_paged_cost vt_paged_few_cost[4] = {{4, 1.1f, 0.8f, 2.55f, 2.85f, 0.35f, 0.37f}, {3, 2.7f, 0.95f, 3.2f, 2.6f, 0.12f, 0.11f},
                                                    {2, 1.2f, 1.04f, 1.93f, 1.9f, 0.08f, 0.31f}, {2, 5.1f, 1.2f, 2.8f, 3.9f, 0.07f, 0.29f}};
 static const vt_paged_cost vt_paged_wide_cost[2] = {{3, 1.4f, 0.32f, 0.7f, 2.5f, 0.16f, 0.39f}, {2, 0.85f, 0.42f, 1.09f, 4.85f, 0.07f, 0.08f}};
-static const vt_paged_cost vt_paged_many_cost[2] = {{2, 7.9f, 1.9f, 3.0f, 5.0f, 1.0f, 0.45f}, {2, 9.25f, 2.2f, 3.8f, 3.6f, 2.2f, 0.24f}};
+static const vt_paged_cost vt_paged_many_cost[4] = {{2, 7.9f, 1.9f, 3.0f, 5.0f, 1.0f, 0.45f}, {2, 9.25f, 2.2f, 3.8f, 3.6f, 2.2f, 0.24f}, {},
+                                                    {1, 8.5f, 2.57f, 2.57f, 5.0f, 1.0f, 0.24f}};
 
 static const vt_paged_cost &vt_paged_cost_of(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many) {
     return (many ? vt_paged_many_cost : kinds.few_cols == 32 ? vt_paged_wide_cost : vt_paged_few_cost)[s.head_dim / 64 - 1];
 }
 
-/* A kernel's part of a batch in runs of `run` units at most: its workgroups and their units, us of all of them; the longest one's units, whether it leaves a
- * part; us of the merge */
+/* A kernel's part of a batch in runs of `run` units at most: its workgroups and their units, us of all of them; the longest one's units, whether it leaves
+ * a part; us of the merge */
 struct vt_paged_try { int run; double wgs, units, all, most, late, merge; };
 #define PAGED_TRIES 40
 static inline int vt_paged_tries(const vt_paged_shape &s, const vt_paged_kinds &kinds, bool many, int n_seqs, const int *past, const int *rows, vt_paged_try *to) {
@@ -222,8 +230,9 @@ static inline double vt_paged_one(const vt_paged_cost &c, const vt_paged_try &t,
     return c.fixed + t.most * slow * (c.alone + (c.step - c.alone) * share) + t.late * c.part;
 }
 
-/* The runs of both kernels.  In one launch they share the CUs: a workgroup of many columns runs better beside one of few than beside another, and fewer of them
- * that leave no parts do best.  The factors are fitted to 30 pairs of runs of nine batches; the pair that they choose is behind the best one by 1 % on average. */
+/* The runs of both kernels.  In one launch they share the CUs: a workgroup of many columns runs better beside one of few than beside another, and fewer of
+ * them that leave no parts do best.  The factors are fitted to 30 pairs of runs of nine batches; the pair that they choose is behind the best one by 1 % on
+ * average. */
 static inline void vt_paged_runs(const vt_paged_shape &s, const vt_paged_kinds &kinds, int n_cu, int n_seqs, const int *past, const int *rows, int *runs) {
     vt_paged_try t[2][PAGED_TRIES];
     int n[2];
@@ -238,7 +247,7 @@ static inline void vt_paged_runs(const vt_paged_shape &s, const vt_paged_kinds &
             if (us < least) { least = us; runs[k] = t[k][i].run; }
         }
     }
-    if (!n[0] || !n[1] || kinds.few_cols != 16) return;
+    if (!n[0] || !n[1] || !vt_paged_may_be_both(s, kinds)) return;
     const vt_paged_cost &c = vt_paged_cost_of(s, kinds, false), &d = vt_paged_cost_of(s, kinds, true);
     double least = 1e300;
     for (int i = 0; i < n[0]; i++)
@@ -294,20 +303,24 @@ static inline int vt_paged_items(const vt_paged_shape &s, const vt_paged_kinds &
 static inline long long vt_paged_few_part(const vt_paged_shape &s, int cols) { return (long long)cols * (s.head_dim + 4) * 4; }
 static inline long long vt_paged_many_part(const vt_paged_shape &s) { return 4ll * (s.head_dim / 8 + 1) * 1024; }
 
-static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts, vt_paged_item *to) {
+/* bf16: the queries' type, which a batch does not know: two plans where it matters */
+static inline bool vt_paged_type_matters(const vt_paged_shape &s) { return s.head_dim == 256; }
+static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, bool bf16, int n_cu, int n_seqs, const int *past, const int *rows, const int *starts,
+                                             vt_paged_item *to) {
     vt_paged_plan p = {0, 0, 0, 0, 0, 0, 0, 0};
-    const vt_paged_kinds kinds = vt_paged_kinds_of(s, n_cu, n_seqs, past, rows);
+    const vt_paged_kinds kinds = vt_paged_kinds_of(s, bf16, n_cu, n_seqs, past, rows);
     int runs[2];
     vt_paged_runs(s, kinds, n_cu, n_seqs, past, rows, runs);
     p.few = vt_paged_items(s, kinds, false, runs[0], n_seqs, past, rows, starts, to, 0, &p.few_slots);
     const long long part = vt_paged_few_part(s, kinds.few_cols) * p.few_slots, each = vt_paged_many_part(s);
     p.many_slot = (int)((part + each - 1) / each);
     p.many = vt_paged_items(s, kinds, true, runs[1], n_seqs, past, rows, starts, to + p.few, p.many_slot, &p.many_slots);
-    p.both = p.few && p.many && p.few + p.many <= 65535 && kinds.few_cols == 16;
+    p.both = p.few && p.many && p.few + p.many <= 65535 && vt_paged_may_be_both(s, kinds);
     if (p.both) qsort(to, p.few + p.many, sizeof *to, vt_paged_slowest);
     p.wide = kinds.few_cols > 16;
     /* Requests that leave nothing behind in the caches: 65535 rows of 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows, which the
-     * caches (32 MB of L2) keep for the next call on them, 6.8 -> 7.2.  Beside a prompt as well: 31 sequences 43.4 -> 41.3, three of 10000 to 30000 76 -> 72. */
+     * caches (32 MB of L2) keep for the next call on them, 6.8 -> 7.2.  Beside a prompt as well: 31 sequences 43.4 -> 41.3, three of 10000 to 30000 76 ->
+     * 72. */
     p.once = kinds.once && kinds.bytes >= PAGED_CACHED;
     return p;
 }
