@@ -186,7 +186,7 @@ def attention(cache, q, bf16, scale, q_gap=0):
 
 
 def is_many(cache, i, bf16):
-    """The kernel that rounds a bf16 batch's weights to bf16 (vt_paged_any_many)."""
+    """The kernel that rounds a bf16 batch's weights to bf16 (vt_paged_kinds_of)."""
     group = cache.heads // cache.kv_heads
     if cache.hd > 128 and not (cache.hd == 256 and bf16):
         return False
