@@ -438,14 +438,15 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
  * V's: beside V's rows 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95.
  *
  * Matrix instructions bound it, and for bf16 the vector unit beside them, which has two values' weights to make for each: 4000 rows behind none of 32 heads
- * of 128 fp32 (three planes of queries and of weights, 393 G multiplications and additions) 316 us, the rate of a large matrix product, bf16 155 us; 1531
- * rows fp32 61 us, of which the first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a window of 2048 bf16 109 us.  Matrix cores
- * busy 64 and 47 % of the time.  Heads of 256 bf16 values have one workgroup to a CU, for its LDS and registers: 3000 rows of 12 on 4 behind none 117 us
+ * of 128 fp32 (three planes of queries and of weights, 393 G multiplications and additions) 316 us, the rate of a large matrix product, bf16 152 us; 1531
+ * rows fp32 61 us, of which the first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a window of 2048 bf16 107 us.  Matrix cores
+ * busy 64 and 47 % of the time.  Heads of 256 bf16 values have one workgroup to a CU, for its LDS and registers: 3000 rows of 12 on 4 behind none 115 us
  * (55 G). */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 
 /* fp32: the compiler keeps to the order that is written, in which an instruction's operands are asked for just ahead of it and no more of them wait in
- * registers than there are; bf16 has registers for its own order (four prompts in a window 112.0 us as written, 108.8 so) */
+ * registers than there are; bf16 has registers for its own order (four prompts in a window 112.0 us as written, 108.8 so, 107 with the weights held ahead
+ * of the branch) */
 template <bool F32> static __device__ __forceinline__ void pa_here() { if constexpr (F32) __builtin_amdgcn_sched_barrier(0); }
 
 /* Tiles with rows that some column does not see: at most 3 where the columns' rows begin to be seen and 3 where they end (fewer queries than 128 apart), or 5
@@ -628,6 +629,11 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
                 for (int e = EARLY * (ks - BEFORE) / (KS - BEFORE); e < EARLY * (ks - BEFORE + 1) / (KS - BEFORE); e++) weigh(e);
             }
             pa_here<F32>();
+        }
+        if constexpr (!F32) {                            /* else the compiler moves them behind hide's branch, where no scores are made */
+#pragma unroll
+            for (int e = 0; e < EARLY; e++) asm volatile("" : "+v"(w4[e >> 2][0][e & 3]));
+            asm volatile("" : "+v"(l));
         }
         hide(u + 1, next);
         top = next[0];
