@@ -104,6 +104,34 @@ def test_rotary_agrees_with_apply_rope(hip):
         d.free()
 
 
+@pytest.mark.parametrize("width", [128, 26])                      # rows on four values, and not
+def test_what_does_not_turn_is_passed_on(hip, width):
+    """Every bf16 there is, and fp32 of every exponent, through a call that turns nothing, and as values into pages: the same bits, a NaN as a NaN."""
+    every = np.arange(65536, dtype=np.uint32)
+    for bits, bf16 in ((every.astype(np.uint16), 1), (every << 16 | every[::-1] ^ 0x5A5A, 0)):
+        bits = bits[:len(bits) // (2 * width) * 2 * width]
+        dx, do = P.Dev(hip.lib, bits), P.Dev(hip.lib, np.zeros_like(bits))
+        assert hip.lib.tts_hip_rotary(do.ptr, dx.ptr, bf16, len(bits) // (2 * width), 2, width, 0, 0, None, P.how(hip, None, 0, 0)) == 0
+        value = lambda b: P.value16(b) if bf16 else b.view(np.float32)
+        out, nan = do.get(), np.isnan(value(bits))
+        assert np.array_equal(out[~nan], bits[~nan]) and np.isnan(value(out)[nan]).all() and nan.any()
+        for d in (dx, do):
+            d.free()
+    if width != 128:
+        return
+    c = P.Cache(hip, "256@0", 16, 8, 2, 128)
+    c.upload()
+    bits = every.astype(np.uint16).reshape(256, 2, 128)
+    dx = P.Dev(hip.lib, bits)
+    assert hip.lib.tts_hip_paged_append(c.batch.ptr, c.dev["k"].ptr, c.dev["v"].ptr, dx.ptr, dx.ptr, 1, 0, None) == 0
+    pos = np.arange(256)
+    for pool in c.download():
+        out, nan = pool[c.tables[0][pos // 16], :, pos % 16], np.isnan(P.value16(bits))
+        assert np.array_equal(out[~nan], bits[~nan]) and np.isnan(P.value16(np.ascontiguousarray(out))[nan]).all()
+    dx.free()
+    c.free()
+
+
 # ---- keys and values into pages ----------------------------------------------------------------
 
 @pytest.mark.parametrize("bf16", [0, 1])

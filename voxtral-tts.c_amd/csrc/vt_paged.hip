@@ -153,9 +153,9 @@ extern "C" const int *tts_hip_paged_positions(const tts_hip_paged_t *b) {
     return vt_paged_ready(who, b) ? (const int *)b->dev : NULL;
 }
 
-/* ---- positions -------------------------------------------------------------------------------------------------- Pair i of a head turns by 2 pi position
- * turns[i].  The product is made in 64 bits and only what is left of it below one turn goes on in fp32, in two parts: the angle is right to 2^-24 or so
- * however far the position (in fp32 it would be off by 0.03 at position 10^6). */
+/* ---- positions ----
+ * Pair i of a head turns by 2 pi position turns[i].  The product is made in 64 bits and only what is left of it below one turn goes on in fp32, in two
+ * parts: the angle is right to 2^-24 or so however far the position (in fp32 it would be off by 0.03 at position 10^6). */
 __global__ void __launch_bounds__(256) vt_rotary_turns_kernel(double *turns, int pairs, double theta, double factor, double original, double low, double high) {
     const int i = (int)(blockIdx.x * 256 + threadIdx.x);
     if (i >= pairs) return;
@@ -180,10 +180,10 @@ extern "C" int tts_hip_rotary_turns(double *d_turns, int rot_dim, double theta, 
     return vt_check(hipGetLastError(), who) ? -1 : 0;
 }
 
-/* ---- heads: norm, turn, store ------------------------------------------------------------------------------------ A lane has a unit of four pairs of a
- * head, 2^log lanes a head, and makes the angles once for the HEADS heads that it walks: angles are more than half of the instructions that a unit takes.
- * (2 p, 2 p + 1) is pair p in both layouts where p does not turn.  Bound by the launch for a few rows (1 to 226 rows of 32 heads 3.8 to 4.1 us a call, 2.5
- * to 3.8 of them the kernel's); 1531 rows of 32 heads 7.5 us, 25 MB at 3.3 TB/s. */
+/* ---- heads: norm, turn, store ----
+ * A lane has a unit of four pairs of a head, 2^log lanes a head, and makes the angles once for the HEADS heads that it walks: angles are more than half of
+ * the instructions that a unit takes.  (2 p, 2 p + 1) is pair p in both layouts where p does not turn.  Bound by the launch for a few rows (1 to 226 rows of
+ * 32 heads 3.8 to 4.3 us a call, 2.5 to 3.8 of them the kernel's); 1531 rows of 32 heads 7.5 us, 25 MB at 3.3 TB/s. */
 struct turn_job {
     const void *x, *x2;                                  /* K and V for pages */
     void *out, *out2;
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(256) vt_turn_kernel(turn_job a) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float v = p[k][e], w = q[k][e];
-                const bool turn = 8 * u + 2 * e < rot;
+                const bool turn = 8 * u + 2 * e < rot;           /* what does not is passed on as it is */
                 p[k][e] = turn ? fmaf(v, c[e], -(w * s[e])) : v;
                 q[k][e] = turn ? fmaf(v, s[e], w * c[e]) : w;
             }
@@ -357,7 +357,6 @@ __global__ void __launch_bounds__(256) vt_turn_kernel(turn_job a) {
     }
 }
 
-/* what does not turn is passed on bit for bit, also where it shares a unit with what does */
 static int turn_ok(const char *who, const tts_hip_rotary_t *how, int head_dim) {
     if (how->rot_dim < 0 || how->rot_dim > head_dim || how->rot_dim % 2 || (how->half != 0 && how->half != 1)) {
         vt_set_error("%s: %d of %d values turn, half %d", who, how->rot_dim, head_dim, how->half);
@@ -427,8 +426,7 @@ extern "C" int tts_hip_rotary(void *d_out, const void *d_x, int x_bf16, int rows
     if (!vt_mx4_ready(who)) return -1;
     if (rows == 0) return 0;
     turn_job a = {d_x, NULL, d_out, NULL, d_positions, NULL, how->d_turns, how->d_gain, how->magnitude, how->eps, 1.f / head_dim, 0, n_heads, head_dim, x_stride,
-                  out_stride,
-                  2 * how->rot_dim + how->half, 0, {0, 1}};
+                  out_stride, 2 * how->rot_dim + how->half, 0, {0, 1}};
     const int aligned = ((((uintptr_t)d_out | (uintptr_t)d_x) & (4 * size - 1)) | (x_stride & 3) | (out_stride & 3) | ((uintptr_t)how->d_gain & 15)) == 0;
     turn_launch<false>(a, rows, x_bf16, aligned);
     return vt_check(hipGetLastError(), who) ? -1 : 0;
