@@ -1,0 +1,50 @@
+"""What the operators over a paged cache promise of a result's bits, range and rounding, at the places where a kernel that is right on ordinary numbers can
+fall short: weights of bf16 calls, scores that only a neighbour in the same wave sees, values near the end of the range, positions near 2^31, shared pages."""
+import math
+
+import numpy as np
+import pytest
+
+import hipsupport as H
+import pagedsupport as P
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    h = H.Hip(kv_max=8)
+    yield h
+    h.close()
+
+
+def normal(rng, shape, bf16):
+    x = rng.standard_normal(shape, np.float32)
+    return P.value16(P.bits16(x)) if bf16 else x
+
+
+MANY = [((32, 8, 128), "1300@0 3@50", 16, 0), ((32, 8, 128), "130@500 1@700 64@64 0@9 900@450", 64, 0), ((32, 8, 128), "2500@1000 1@3000 2@100", 32, 1200),
+        ((16, 16, 64), "333@3700 900@1100 1@40 700@0", 256, 0), ((14, 2, 64), "2000@800", 1024, 0), ((12, 4, 256), "1700@30 1@5 40@900", 16, 0)]
+
+
+@pytest.mark.parametrize("layout,batch,page,window", MANY)
+def test_a_bf16_result_is_rounded_and_little_else(hip, layout, batch, page, window):
+    """Queries of many columns in bf16: weights enter to 16 bits.  A value's error is its own rounding, of at most half a step h = 2^-8 of the power of two
+    below it and uniform within, so that over many values the squares add up to h^2 / 3 each.  Weights (2^-17 of each, independent: 4e-6 of the norm), scores
+    (1e-6) and sums are far below 2 % of that; a weight rounded to bf16 (2^-8 / sqrt 3 times 0.74) would be another 80 % beside it."""
+    c = P.Cache(hip, batch, page, *layout, window=window, seed=len(batch))
+    c.fill()
+    c.upload()
+    q = normal(np.random.default_rng(7), (sum(c.rows), layout[0], layout[2]), 1)
+    scale, keep = 1 / math.sqrt(layout[2]), c.some()
+    assert any(P.is_many(c, i, 1) for i in range(len(c.rows)))
+    got = P.attention(c, q, 1, scale)[keep].astype(np.float64)
+    want, size, most = c.attend(q, scale, keep)
+    want, size = want[keep], size[keep]
+    off = got - want
+    half = 2.0 ** (np.floor(np.log2(np.abs(want))) - 8)
+    rel = 2 * (3 * c.hd / 8 + 3) * 2.0 ** -23 * most + 64 * 2.0 ** -23 + 2.0 ** -16
+    # the next power of two is nearer than rel to some results: twice the half step there
+    assert (np.abs(off) <= 2.0 ** -8 * (np.abs(want) + rel * size) + rel * size).all()
+    assert math.sqrt((off ** 2).sum()) <= 1.02 * math.sqrt((half ** 2).sum() / 3)
+    c.free()

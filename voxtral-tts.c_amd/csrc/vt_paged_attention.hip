@@ -3,7 +3,7 @@
  *
  * The queries of the heads that share a kv head are columns (vt_paged_plans.h).  Scores are S^T[row][column] = K Q^T and results O^T[value][column] = V^T P^T
  * on the bf16 matrix instructions: keys and values as they lie, queries and weights as planes that each hold 8 bits of what the one before leaves, smallest
- * first: three make fp32 of fp32, one is a bf16 query itself.  A lane holds the same column of S^T and of O^T, and the order of the rows inside an
+ * first: three make fp32 of fp32, one is a bf16 query itself, whose weights are two: 16 bits, so that its result's rounding is what is seen of them.  A lane holds the same column of S^T and of O^T, and the order of the rows inside an
  * instruction is free, so that weights go from one product to the next in their registers.  Maximum, sum and results of a column are fp32, one pass over the
  * rows with the running maximum.
  *
@@ -438,15 +438,15 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
  * V's: beside V's rows 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95.
  *
  * Matrix instructions bound it, and for bf16 the vector unit beside them, which has two values' weights to make for each: 4000 rows behind none of 32 heads
- * of 128 fp32 (three planes of queries and of weights, 393 G multiplications and additions) 316 us, the rate of a large matrix product, bf16 152 us; 1531
- * rows fp32 61 us, of which the first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a window of 2048 bf16 107 us.  Matrix cores
- * busy 64 and 47 % of the time.  Heads of 256 bf16 values have one workgroup to a CU, for its LDS and registers: 3000 rows of 12 on 4 behind none 115 us
- * (55 G). */
+ * of 128 fp32 (three planes of queries and of weights, 393 G multiplications and additions) 316 us, the rate of a large matrix product, bf16 (two planes of
+ * weights, 197 G) 193 us; 1531 rows fp32 61 us, of which the first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a window of 2048
+ * bf16 137 us.  Heads of 256 bf16 values have one workgroup to a CU, for its LDS and registers: 3000 rows of 12 on 4 behind none 130 us (83 G).  With weights
+ * of one plane these three take 153, 107 and 115 us, and a result is off by 2.1e-3 of its norm instead of the 1.6e-3 that its own rounding leaves. */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 
 /* fp32: the compiler keeps to the order that is written, in which an instruction's operands are asked for just ahead of it and no more of them wait in
- * registers than there are; bf16 has registers for its own order (four prompts in a window 112.0 us as written, 108.8 so, 107 with the weights held ahead
- * of the branch) */
+ * registers than there are; bf16 has registers for its own order (four prompts in a window 142.0 us as written, 140.4 so, 138.6 with the weights held
+ * ahead of the branch) */
 template <bool F32> static __device__ __forceinline__ void pa_here() { if constexpr (F32) __builtin_amdgcn_sched_barrier(0); }
 
 /* Tiles with rows that some column does not see: at most 3 where the columns' rows begin to be seen and 3 where they end (fewer queries than 128 apart), or 5
@@ -456,7 +456,7 @@ template <int HP, bool F32>
 static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsigned char *k0, unsigned char *k1, unsigned char *v0, unsigned char *v1,
                                                unsigned (*marks)[64][2 * HP], int (*odd)[4], int &last) {
     constexpr int HD = 64 * HP, ROW = 2 * HD, WAVES = 4, DT = 2 * HP, KS = 4 * HP, PIECES = HD / 8, EDGES = PA_EDGES;
-    constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 1;
+    constexpr int NQ = F32 ? 3 : 1, NP = F32 ? 3 : 2;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5;
     const int h = (int)blockIdx.x, heads = (int)gridDim.x;
     const vt_paged_item it = pa_item(a.items, item);
@@ -588,7 +588,7 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
         edges++;
     };
     /* pairs of weights that are made beside the scores; the others beside the first products with values.  An instruction takes the matrix cores 32 cycles,
-     * a pair 50 (fp32, with three times the instructions: 90) of the vector unit. */
+     * a pair 70 (fp32, with twice the instructions: 90) of the vector unit. */
     constexpr int EARLY = F32 ? 8 : HP == 1 ? 6 : 5, AHEAD = F32 ? 1 : 3, BEFORE = F32 ? 1 : 2;
     /* (AHEAD: operands that are asked for ahead of their instruction; BEFORE: those in front of what depends on the maximum) */
     float top = -INFINITY;                               /* the largest score of the unit at hand, in a lane's rows */
@@ -632,7 +632,9 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
         }
         if constexpr (!F32) {                            /* else the compiler moves them behind hide's branch, where no scores are made */
 #pragma unroll
-            for (int e = 0; e < EARLY; e++) asm volatile("" : "+v"(w4[e >> 2][0][e & 3]));
+            for (int e = 0; e < EARLY; e++)
+#pragma unroll
+                for (int p = 0; p < NP; p++) asm volatile("" : "+v"(w4[e >> 2][p][e & 3]));
             asm volatile("" : "+v"(l));
         }
         hide(u + 1, next);

@@ -109,13 +109,14 @@ static inline long long vt_paged_max_items(int max_seqs, int max_rows, int group
 }
 
 /* Which sequences go to the kernel for many columns: those of more than 64, where there is enough for it to do, as columns times the rows that they see on
- * average times kv heads times values, over all of them.  It does twice as much with what it reads, but by few workgroups.  Measured, us with the kernel
- * for few columns, 32 at a time, and for many (fp32 / bf16), 32 heads on 8 of 128: 450 rows behind 200 (0.8e9) 18 / 16 and 26 / 19, 700 behind none (1.0e9)
- * 24 / 20 and 27 / 19, 200 behind 2000 (1.7e9) 32 / 24 and 38 / 26, 50 behind 16000 (3.3e9) 52 / 48 and 60 / 43, 512 behind 1500 (3.7e9) 45 / 39 and 49 /
- * 32, 100 behind 500 sixteen times (3.6e9) 59 / 47 and 49 / 29; 16 heads of 64: 512 behind 1500 (0.9e9) 21 / 17 and 24 / 18.  Heads of 256 values leave it
- * registers if they are bf16: 12 on 4, 300 behind 1000 (1.1e9) 28 and 33, 1000 behind none (1.5e9) 38 and 31, 200 behind 3000 (1.9e9) 50 and 43, 512 behind
- * 1500 (2.8e9) 69 and 40, 3000 behind none (14e9) 247 and 117; fp32 it keeps some in memory and 3000 take 250 and 344.  Heads of 192 do not lie as it reads
- * them.
+ * average times kv heads times values, over all of them.  It does more with what it reads, but by few workgroups.  Measured, us with the kernel for few
+ * columns, 32 at a time, and for many (fp32 / bf16), 32 heads on 8 of 128: 450 rows behind 200 (0.8e9) 18 / 16 and 26 / 20, 700 behind none (1.0e9) 25 / 21
+ * and 27 / 20, 200 behind 2000 (1.7e9) 33 / 25 and 35 / 26, 50 behind 16000 (3.3e9) 61 / 48 and 64 / 47, 100 behind 500 sixteen times (3.6e9) 60 / 46 and
+ * 51 / 34, 512 behind 1500 (3.7e9) 46 / 39 and 50 / 36; 16 heads of 64: 512 behind 1500 (0.9e9) 21 / 17 and 25 / 20.  One figure serves both types: fp32
+ * calls of one sequence would do better by 5 to 10 % from 3e9 on with the other kernel up to about 4e9, several sequences of the same figure worse by 18.
+ * Heads of 256 values leave it registers if they are bf16: 12 on 4, 300 behind 1000 (1.1e9) 28 and 34, 1000 behind none (1.5e9) 38 and 33, 200 behind 3000
+ * (1.9e9) 50 and 45, 512 behind 1500 (2.8e9) 69 and 42, 3000 behind none (14e9) 245 and 130; fp32 it keeps some in memory and 3000 take 250 and 344.  Heads
+ * of 192 do not lie as it reads them.
  *
  * Else 32 columns to a workgroup, not 16, where there is enough for that, as columns / 16 times rows times kv heads times values (less where every CU has
  * one of 16); 16 and 32 at a time: 37 rows behind 300 (3e6) 7.0 / 6.4 and 9.9 / 8.2, 100 behind 1000 (27e6) 13 / 13 and 19 / 15, 37 behind 4000 (41e6) 21 /
