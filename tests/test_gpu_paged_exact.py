@@ -48,3 +48,39 @@ def test_a_bf16_result_is_rounded_and_little_else(hip, layout, batch, page, wind
     assert (np.abs(off) <= 2.0 ** -8 * (np.abs(want) + rel * size) + rel * size).all()
     assert math.sqrt((off ** 2).sum()) <= 1.02 * math.sqrt((half ** 2).sum() / 3)
     c.free()
+
+
+# layout, batch, page: few columns in parts, few with a wave's rows behind one another, 32 at a time, many in one part and in several, and both in one launch
+NEIGHBOURS = [((32, 8, 128), "3@700", 16), ((8, 1, 128), "7@1500", 32), ((32, 8, 128), " ".join(["4@900"] * 40), 16), ((24, 3, 64), " ".join(["9@700"] * 50), 64),
+              ((6, 2, 192), " ".join(["5@600"] * 70), 16), ((16, 2, 256), " ".join(["3@800"] * 60), 16), ((32, 8, 128), "300@700 5@5", 64),
+              ((16, 16, 64), "512@1500", 16), ((32, 8, 128), "1300@0", 16), ((32, 8, 128), "90@2500 600@1500", 64), ((32, 8, 128), "600@1500 1@2000 2@777", 64),
+              ((14, 2, 64), "2000@800", 1024), ((12, 4, 256), "1700@30", 16)]
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("layout,batch,page", NEIGHBOURS)
+def test_keys_that_a_query_does_not_see_leave_its_bits(hip, layout, batch, page, bf16):
+    """Queries share waves and tiles with later ones of their sequence.  Keys that only those see - scores far above the others', infinities, NaN - and values
+    there change no bit of what came before."""
+    c = P.Cache(hip, batch, page, *layout, seed=len(batch))
+    c.fill()
+    q = normal(np.random.default_rng(7), (sum(c.rows), layout[0], layout[2]), bf16)
+    scale, results = 2 / math.sqrt(layout[2]), []
+    first = [max(1, (r - 1) // 2 | 1) if r > 1 else r for r in c.rows]                  # queries from this one on see what changes
+    before = np.concatenate([np.arange(r) < f for r, f in zip(c.rows, first)])
+    for what in ("as it is", "far", "infinite", "NaN"):
+        for pool, odd in ((c.k, 0x7F80), (c.v, 0xFF80)):
+            for i, t in enumerate(c.tables):
+                p = np.arange(c.past[i] + first[i], c.past[i] + c.rows[i])
+                x = c.rng.standard_normal((len(p), layout[1], layout[2]), np.float32) * 30
+                pool[t[p // page], :, p % page] = P.bits16(x) if what == "far" else odd if what == "infinite" else P.NAN16 if what == "NaN" else P.bits16(x / 30)
+        c.upload()
+        results.append(P.attention(c, q, bf16, scale))
+        for d in c.dev.values():
+            d.free()
+    c.dev = {}
+    assert np.isfinite(results[0]).all() and before.any()
+    for other in results[1:]:
+        assert np.array_equal(other[before], results[0][before])
+        assert len(before) == before.sum() or not np.array_equal(other[~before], results[0][~before])
+    c.free()

@@ -105,8 +105,17 @@ static __device__ __forceinline__ float pa_exp2(float x) { return __builtin_amdg
 
 /* A column's weights are relative to m, which follows the largest score only where that is further above than this: weights up to 2^8 are as exact as ones
  * below 1, and what was summed so far is scaled anew in the first tile and hardly ever after it (with 32 columns to a wave one of them has a new largest
- * score in nearly every tile). */
+ * score in nearly every tile).  The wave goes there together, but a column's m stays unless its own score is far above: what another column sees is none of
+ * its business. */
 #define PA_SLACK 8.f
+static __device__ __forceinline__ bool pa_far(float top, float m) { return __any(!(top <= m + PA_SLACK)); }
+/* -> what the column's sums are scaled by; a NaN stays one */
+static __device__ __forceinline__ float pa_follow(float top, float &m) {
+    if (top <= m + PA_SLACK) return 1.f;
+    const float before = m;
+    m = __builtin_elementwise_maximum(top, before);
+    return pa_exp2(before - m);
+}
 template <bool F32>
 static __device__ __forceinline__ float pa_weight(float s, float m, float scale) { return pa_exp2(F32 ? s - m : fmaf(s, scale, -m)); }
 
@@ -286,13 +295,11 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
                 top = __builtin_elementwise_maximum(r.x, r.y);
             }
             if constexpr (!F32) top = top * a.scale;
-            if (__any(!(top <= m[c] + PA_SLACK))) {
-                top = __builtin_elementwise_maximum(top, m[c]);
-                const float less = pa_exp2(m[c] - top);
+            if (pa_far(top, m[c])) {
+                const float less = pa_follow(top, m[c]);
                 l[c] *= less;
 #pragma unroll
                 for (int i = 0; i < CHUNKS * CD; i++) o[c][i] = o[c][i] * less;
-                m[c] = top;
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -543,13 +550,11 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
     auto follow = [&](float top) __attribute__((always_inline)) {         /* the running maximum; a NaN stays one: who sees it answers NaN */
         { const f32x2 r = vt_swap32(top, top); top = __builtin_elementwise_maximum(r.x, r.y); }
         if constexpr (!F32) top = top * a.scale;
-        if (__any(!(top <= m + PA_SLACK))) {
-            top = __builtin_elementwise_maximum(top, m);
-            const float less = pa_exp2(m - top);
+        if (pa_far(top, m)) {
+            const float less = pa_follow(top, m);
             l *= less;
 #pragma unroll
             for (int i = 0; i < DT; i++) o[i] = o[i] * less;
-            m = top;
         }
     };
     /* Where rows of a V tile are hidden from some column, values that are not finite become 0, and are remembered.  All waves come here or none. */
