@@ -436,11 +436,13 @@ int tts_hip_paged_append(const tts_hip_paged_t *batch, void *d_k_pages, void *d_
  * What a query does not see changes nothing in its result, whatever it holds: rows of its pages behind the last one are not even read.  A query
  * with an infinity or a NaN in it, and one that sees a key with a NaN, gives NaN; a key's infinity makes NaN too, or, where the score is
  * -infinity, may leave the key without weight.  A value's infinity or NaN that a query sees makes that value of its result infinite or NaN.
- * Sums and softmax statistics are fp32, and what leaves them on the way (scores, or values times more than 2^8 of weight) gives NaN or infinity;
- * products below 2^-126 may count as 0.  fp32: queries times scale and weights enter to 24 bits, results are off by some 1e-7 of their norm.
- * bf16: weights enter to 16 bits, and results are rounded once.  A call's results are the same bits each time; beside other sequences in the
- * batch the same query's may differ by these roundings, as the kernel and the parts that its rows are read in are chosen for the batch.  Where several workgroups share a sequence's rows their parts meet in the
- * library's work area, which grows by allocation when a call needs more than any before it and stays. */
+ * Sums and softmax statistics are fp32.  A score that leaves that gives NaN or infinity, and a value times its weight below 2^-126 may count as 0.
+ * A mean of finite values is finite: a query whose sums leave fp32 is summed once more with smaller weights (and what counts as 0 is then below
+ * 2^-86).  fp32: queries times scale and weights enter to 24 bits, results are off by some 1e-7 of their norm.  bf16: weights enter to 16 bits, and
+ * results are rounded once.  A call's results are the same bits each time; beside other sequences in the batch the same query's may differ by
+ * these roundings, as the kernel and the parts that its rows are read in are chosen for the batch.  Where several workgroups share a
+ * sequence's rows their parts meet in the library's work area, which grows by allocation when a call needs more than any before it and
+ * stays. */
 int tts_hip_paged_attention(void *d_out, const void *d_Q, int x_bf16, int q_stride, const tts_hip_paged_t *batch, const void *d_k_pages,
                             const void *d_v_pages, float scale);
 

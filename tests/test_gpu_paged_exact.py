@@ -84,3 +84,40 @@ def test_keys_that_a_query_does_not_see_leave_its_bits(hip, layout, batch, page,
         assert np.array_equal(other[before], results[0][before])
         assert len(before) == before.sum() or not np.array_equal(other[~before], results[0][~before])
     c.free()
+
+
+RANGE = NEIGHBOURS + [((32, 8, 128), "1@0 1@1999 1@40", 16), ((8, 1, 128), "1@20000", 256), ((4, 4, 192), "37@300", 16), ((8, 1, 128), "5300@100", 32),
+                      ((32, 8, 128), "1@9000 1500@100", 16)]
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("alike", [True, False])
+@pytest.mark.parametrize("layout,batch,page", RANGE)
+def test_a_mean_is_finite_where_its_values_are(hip, layout, batch, page, alike, bf16):
+    """Values up to the largest that bf16 has, over as many rows as there are: what a query answers is a mean of them, however large their sum; from the queries
+    on that see the large ones, and without a bit's change for the others in their waves.  Weights are then relative to up to 2^40 times the largest one, and
+    the difference to it is off by 2^-19 (of a number below 64, half a step) times log 2: 2^-19 beside what pagedsupport.check counts."""
+    c = P.Cache(hip, batch, page, *layout, seed=len(batch))
+    c.fill()
+    q = normal(np.random.default_rng(7), (sum(c.rows), layout[0], layout[2]), bf16) * np.float32(0 if alike else 1)
+    scale, keep = 1 / math.sqrt(layout[2]), c.some()
+    c.upload()
+    ordinary = P.attention(c, q, bf16, scale)
+    for d in c.dev.values():
+        d.free()
+    first = [r // 3 for r in c.rows]                             # queries from this one on see large values, in the first half of their heads
+    for i, t in enumerate(c.tables):
+        p = np.arange(c.past[i] + first[i] if c.rows[i] > 1 else 0, c.past[i] + c.rows[i])
+        x = c.rng.standard_normal((len(p), layout[1], layout[2] // 2), np.float32)
+        x = 3.3e38 * np.clip(1 - 0.01 * np.abs(x), 0.9, 1) if alike else np.clip(x, -1.65, 1.65) * 2e38
+        c.v[t[p // page], :, p % page, :layout[2] // 2] = P.bits16(x)
+    c.upload()
+    got = P.attention(c, q, bf16, scale)
+    assert np.isfinite(got).all()
+    want, size, most = c.attend(q, scale, keep)
+    rel = 2 * (3 * c.hd / 8 + 3) * 2.0 ** -23 * most + 64 * 2.0 ** -23 + 2.0 ** -19 + (2.0 ** -16 if bf16 else 0)
+    off, tol = np.abs(got - want)[keep], (rel * size + (2.0 ** -8 * (np.abs(want) + rel * size) if bf16 else 0))[keep]
+    assert (off <= tol).all(), float((off / tol).max())
+    before = np.concatenate([np.arange(r) < (f if r > 1 else 0) for r, f in zip(c.rows, first)])
+    assert np.array_equal(got[before], ordinary[before])
+    c.free()

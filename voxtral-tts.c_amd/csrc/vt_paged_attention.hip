@@ -3,9 +3,9 @@
  *
  * The queries of the heads that share a kv head are columns (vt_paged_plans.h).  Scores are S^T[row][column] = K Q^T and results O^T[value][column] = V^T P^T
  * on the bf16 matrix instructions: keys and values as they lie, queries and weights as planes that each hold 8 bits of what the one before leaves, smallest
- * first: three make fp32 of fp32, one is a bf16 query itself, whose weights are two: 16 bits, so that its result's rounding is what is seen of them.  A lane holds the same column of S^T and of O^T, and the order of the rows inside an
- * instruction is free, so that weights go from one product to the next in their registers.  Maximum, sum and results of a column are fp32, one pass over the
- * rows with the running maximum.
+ * first: three make fp32 of fp32, one is a bf16 query itself, whose weights are two: 16 bits, so that its result's rounding is what is seen of them.  A lane
+ * holds the same column of S^T and of O^T, and the order of the rows inside an instruction is free, so that weights go from one product to the next in their
+ * registers.  Maximum, sum and results of a column are fp32, one pass over the rows with the running maximum.
  *
  * What a column does not see: a hidden score is -infinity whatever the key holds.  A hidden value's weight is 0, but 0 times an infinity or NaN would be NaN,
  * so that where rows at hand are hidden from some column and a value among them is not finite, the value counts as 0, and a product of its own, with ones as
@@ -118,6 +118,24 @@ static __device__ __forceinline__ float pa_follow(float top, float &m) {
 }
 template <bool F32>
 static __device__ __forceinline__ float pa_weight(float s, float m, float scale) { return pa_exp2(F32 ? s - m : fmaf(s, scale, -m)); }
+
+/* Sums that leave fp32 although their mean does not: a column's weights are relative to its m, up to 2^8 each and as many as there are rows, so that values
+ * above 2^120 over the number of rows may do that.  A column whose results are not finite is summed once more with an m so much further up that all its
+ * weights come to less than 1; its neighbours' m stays, and with it every bit of theirs.  (Not everybody's from the start: a product of such a weight with
+ * a value is lost below 2^-126, and a score's difference to m loses bits.  A column that answers NaN or infinity anyway is summed twice.)  The look and what
+ * the second copy of the loop does to the first's registers: one query behind 1999 rows 7.94 -> 8.06 us, 1531 behind none bf16 40.4 -> 40.5, heads of 256
+ * 3000 rows 128 -> 134. */
+static __device__ __forceinline__ float pa_largest(float so_far, const f32x4 &v) {       /* a NaN stays one */
+    so_far = __builtin_elementwise_maximum(__builtin_elementwise_maximum(so_far, fabsf(v.x)), fabsf(v.y));
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(so_far, fabsf(v.z)), fabsf(v.w));
+}
+template <int COLS> static __device__ __forceinline__ unsigned long long pa_same_columns(unsigned long long lanes) {      /* all lanes of a column that one is of */
+    lanes |= lanes >> 32 | lanes << 32;
+    return COLS == 16 ? lanes | lanes >> 16 | lanes << 48 : lanes;
+}
+static __device__ __forceinline__ float pa_lift(unsigned long long over, int rows) {
+    return over >> __lane_id() & 1 ? (float)(9 + 32 - __clz(rows)) : 0.f;
+}
 
 /* What the batch's description holds is the same for a whole workgroup: scalar loads, which the kernel's own stores cannot touch */
 typedef __attribute__((address_space(4))) const int pa_const_int;
@@ -233,6 +251,8 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
     const int all_lo = max(a.window && q_last >= a.window ? q_last - a.window + 1 : 0, it.lo), all_hi = min(q_first + 1, it.end);      /* that every column sees */
     float m[2], l[2];
     f32x4 o[CT][CHUNKS * CD];
+    __syncthreads();
+    auto sums = [&](const unsigned long long (&over)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         m[c] = -3.402823466e38f;                         /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
@@ -240,7 +260,6 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
 #pragma unroll
         for (int i = 0; i < CHUNKS * CD; i++) o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    __syncthreads();
 #pragma unroll 1
     for (int t = wave; t < tiles; t += WAVES) {
         const int first = base + PAGED_FEW_ROWS * t;
@@ -295,6 +314,7 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
                 top = __builtin_elementwise_maximum(r.x, r.y);
             }
             if constexpr (!F32) top = top * a.scale;
+            if (over[c]) top += pa_lift(over[c], it.end - it.lo);
             if (pa_far(top, m[c])) {
                 const float less = pa_follow(top, m[c]);
                 l[c] *= less;
@@ -355,6 +375,23 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
                 }
             }
         ask_v();
+    }
+    };
+    unsigned long long over[2] = {0, 0};
+    sums({0, 0});
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        if (c && !two) break;
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < CHUNKS * CD; i++) most = pa_largest(most, o[c][i]);
+        over[c] = pa_same_columns<16>(__ballot(!(most < INFINITY)));
+    }
+    if (__builtin_expect((over[0] | over[1]) != 0, 0)) { /* rare */
+        place(wave);
+        ask_k();
+        ask_v();
+        sums(over);
     }
     /* The waves' parts, each times its share of the sum of weights: a mean of values */
 #pragma unroll
@@ -513,17 +550,19 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
         for (int i = 0; i < DT; i++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void *)(to + wave * 16 * ROW + i * 1024), 16, from[i], 0, 0, 0);
     };
-    pages(0);
-    load(a.K, pa_place(table, base - 32 + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW), k_at, k1);
-    load(a.V, v_place(0), v_at, v0);
-    load(a.K, k_place(0), k_at, k0);
+    auto first_tiles = [&]() __attribute__((always_inline)) {
+        pages(0);
+        load(a.K, pa_place(table, base - 32 + 16 * wave, it.lo, it.end, a.page_log, heads, h, ROW), k_at, k1);
+        load(a.V, v_place(0), v_at, v0);
+        load(a.K, k_place(0), k_at, k0);
+    };
+    first_tiles();
     u32x4 q[KS][NQ];                                     /* (made while the first tiles are on their way) */
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) pa_query_planes<F32, NQ>(raw[ks], a.scale, q[ks]);
-    float m = -3.402823466e38f, l = 0.f;
+    float m, l;
     pa_f32x16 o[DT];
-#pragma unroll
-    for (int i = 0; i < DT; i++) o[i] = pa_f32x16{};
+    unsigned long long over = 0;
     /* addresses in LDS: one for all of K's pieces and one for all of V's, which differ from them in bits of their own.  (fp32: through an empty asm in each
      * unit, else each piece's, for each buffer, is kept in a register.) */
     const int k_base = n * ROW + (g ^ (n & SWAP)) * 16, r4 = (n & 15) >> 2;
@@ -550,6 +589,7 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
     auto follow = [&](float top) __attribute__((always_inline)) {         /* the running maximum; a NaN stays one: who sees it answers NaN */
         { const f32x2 r = vt_swap32(top, top); top = __builtin_elementwise_maximum(r.x, r.y); }
         if constexpr (!F32) top = top * a.scale;
+        if (over) top += pa_lift(over, it.end - it.lo);
         if (pa_far(top, m)) {
             const float less = pa_follow(top, m);
             l *= less;
@@ -558,7 +598,7 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
         }
     };
     /* Where rows of a V tile are hidden from some column, values that are not finite become 0, and are remembered.  All waves come here or none. */
-    int edges = 0;                                       /* tiles that were looked at: the first ones up to the rows that all columns see, and the last ones */
+    int edges;                                           /* tiles that were looked at: the first ones up to the rows that all columns see, and the last ones */
     auto look = [&](int t, unsigned char *vb) __attribute__((always_inline)) {
         if ((base + 64 * t >= wg_lo && base + 64 * t + 64 <= wg_hi) || edges == EDGES) return;
         pa_u16x2 most = {0, 0};
@@ -596,7 +636,7 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
      * a pair 70 (fp32, with twice the instructions: 90) of the vector unit. */
     constexpr int EARLY = F32 ? 8 : HP == 1 ? 6 : 5, AHEAD = F32 ? 1 : 3, BEFORE = F32 ? 1 : 2;
     /* (AHEAD: operands that are asked for ahead of their instruction; BEFORE: those in front of what depends on the maximum) */
-    float top = -INFINITY;                               /* the largest score of the unit at hand, in a lane's rows */
+    float top;                                           /* the largest score of the unit at hand, in a lane's rows */
     auto unit = [&](int u, const unsigned char *kb, int khalf, pa_f32x16 &next, pa_f32x16 &s, const unsigned char *vb, int vhalf) __attribute__((always_inline)) {
         if (!visible(u)) {
             if (!visible(u + 1)) return;
@@ -664,21 +704,6 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
         }
     };
     pa_f32x16 sa, sb;
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
-    if (visible(0)) {                                    /* the first unit's scores */
-        sa = pa_f32x16{};
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const pa_bf16x8 k = read_k(k1, 1, ks, k_base);
-#pragma unroll
-            for (int p = NQ - 1; p >= 0; p--) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, pa_operand(q[ks][p]), sa, 0, 0, 0);
-        }
-        hide(0, sa);
-#pragma unroll
-        for (int v = 0; v < 16; v++) top = __builtin_elementwise_maximum(top, sa[v]);
-    }
-    __syncthreads();
     auto step = [&](int t, const unsigned char *kb, unsigned char *vb, unsigned char *k_to, unsigned char *v_to) __attribute__((always_inline)) {
         if (t + 1 < tiles) {
             if (((t + 1) & 63) == 0) pages(t + 1);
@@ -691,11 +716,50 @@ static __device__ __forceinline__ void pa_many(const pa_job &a, int item, unsign
         __builtin_amdgcn_s_waitcnt(0x0f70);              /* the next tiles have arrived */
         __syncthreads();
     };
+    auto sums = [&]() __attribute__((always_inline)) {
+        m = -3.402823466e38f;
+        l = 0.f;
+        top = -INFINITY;
+        edges = 0;
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[i] = pa_f32x16{};
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __syncthreads();
+        if (visible(0)) {                                /* the first unit's scores */
+            sa = pa_f32x16{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const pa_bf16x8 k = read_k(k1, 1, ks, k_base);
+#pragma unroll
+                for (int p = NQ - 1; p >= 0; p--) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, pa_operand(q[ks][p]), sa, 0, 0, 0);
+            }
+            hide(0, sa);
+#pragma unroll
+            for (int v = 0; v < 16; v++) top = __builtin_elementwise_maximum(top, sa[v]);
+        }
+        __syncthreads();
 #pragma unroll 1
-    for (int t = 0; t < tiles; t += 2) {
-        step(t, k0, v0, k1, v1);
-        if (t + 1 >= tiles) break;
-        step(t + 1, k1, v1, k0, v0);
+        for (int t = 0; t < tiles; t += 2) {
+            step(t, k0, v0, k1, v1);
+            if (t + 1 >= tiles) break;
+            step(t + 1, k1, v1, k0, v0);
+        }
+    };
+    if (tid == 0) last = 0;
+    sums();
+    {
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) most = pa_largest(most, f32x4{o[i][v], o[i][v + 1], o[i][v + 2], o[i][v + 3]});
+        over = pa_same_columns<32>(__ballot(!(most < INFINITY)));
+        if (over && lane == 0) last = 1;
+        __syncthreads();
+    }
+    if (__builtin_expect(last, 0)) {                     /* rare; all waves go, for their requests and barriers */
+        first_tiles();
+        sums();
     }
     { const f32x2 r = vt_swap32(l, l); l = r.x + r.y; }
     {
