@@ -157,6 +157,21 @@ class Hip:
         return codes, x
 
 
+def _int32(x, what):
+    """A vector of whole numbers as the library reads them."""
+    a = np.asarray(x)
+    if a.ndim != 1:
+        raise ValueError(f"{what}: not a vector")
+    try:
+        with np.errstate(invalid="ignore"):
+            b = np.ascontiguousarray(a, np.int32)
+    except OverflowError:
+        b = None
+    if b is None or not np.array_equal(a, b):
+        raise ValueError(f"{what}: not whole numbers of 32 bits")
+    return b
+
+
 class PagedBatch:
     """A batch of sequences over a paged cache (tts_hip_paged_t): the handle, and what the calls read of it."""
 
@@ -169,8 +184,11 @@ class PagedBatch:
             raise ValueError(self.lib.tts_hip_last_error().decode())
 
     def set(self, past, rows, tables):
-        """Sequence i has rows[i] new rows behind past[i] and the pages tables[i]; 0, or -1 where the library refuses."""
-        past, rows = np.ascontiguousarray(past, np.int32), np.ascontiguousarray(rows, np.int32)
+        """Sequence i has rows[i] new rows behind past[i] and the pages tables[i]; 0, or -1 where the library refuses.  ValueError where these are not of
+        one length, or not whole numbers of 32 bits."""
+        past, rows, tables = _int32(past, "past"), _int32(rows, "rows"), [_int32(t, f"pages of sequence {i}") for i, t in enumerate(tables)]
+        if not len(past) == len(rows) == len(tables):
+            raise ValueError(f"{len(past)} sequences with {len(rows)} numbers of rows and {len(tables)} tables")
         wide = np.full((len(tables), max([1] + [len(t) for t in tables])), -1, np.int32)
         for i, t in enumerate(tables):
             wide[i, :len(t)] = t
