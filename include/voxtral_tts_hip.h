@@ -416,13 +416,13 @@ typedef struct {
 
 /* d_turns[i] = theta^(-2 i / rot_dim) / 2 pi for i < rot_dim / 2, stretched by `factor` (1: not): a pair that makes fewer than low_turns
  * turns in original_rows positions is divided by it, one that makes more than high_turns is not, in between the share goes with the turns.  original_rows 0
- * and a low_turns above 0 divide all of them. */
+ * and a low_turns above 0 divide all of them.  Each is right to some 2^-52, an angle of it to 2^-24 at positions of 2^28 and 2^-21 at 2^31. */
 int tts_hip_rotary_turns(double *d_turns, int rot_dim, double theta, double factor, int original_rows, double low_turns, double high_turns);
 /* x [rows, n_heads, head_dim] -> out of the same type, x_stride and out_stride values from row to row (0: dense); row r at position
  * d_positions[r] (any int; device).  out may be x with the same stride, else they do not overlap.  Any alignment that the type allows; rows on
- * four values, head_dim a multiple of 8 and, with half, rot_dim too are fastest.  head_dim even, 2 .. 512.  Angles are as exact as fp32 holds them at
- * any position, sums fp32, bf16 results are rounded once.  Values that do not turn and are not normed come out bit for bit, a NaN as
- * a NaN. */
+ * four values, head_dim a multiple of 8 and, with half, rot_dim too are fastest.  head_dim even, 2 .. 512.  Angles, position times the turns
+ * given, are as exact as fp32 holds them at any position, sums fp32, bf16 results are rounded once.  Values that do not turn and are not normed
+ * come out bit for bit, a NaN as a NaN. */
 int tts_hip_rotary(void *d_out, const void *d_x, int x_bf16, int rows, int n_heads, int head_dim, int out_stride, int x_stride,
                    const int *d_positions, const tts_hip_rotary_t *how);
 

@@ -1,5 +1,6 @@
 """What the operators over a paged cache promise of a result's bits, range and rounding, at the places where a kernel that is right on ordinary numbers can
 fall short: weights of bf16 calls, scores that only a neighbour in the same wave sees, values near the end of the range, positions near 2^31, shared pages."""
+from fractions import Fraction
 import math
 
 import numpy as np
@@ -121,3 +122,32 @@ def test_a_mean_is_finite_where_its_values_are(hip, layout, batch, page, alike, 
     before = np.concatenate([np.arange(r) < (f if r > 1 else 0) for r, f in zip(c.rows, first)])
     assert np.array_equal(got[before], ordinary[before])
     c.free()
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("most", [0.16, 40.0, 5e5])
+def test_angles_are_those_of_the_turns_given(hip, most, half, norm):
+    """Position times turn in whole numbers of any length, of which the fraction is an angle: at the ends of int, and for turns of many whole ones a position.
+    (A product rounded to 64 bits is off by up to 2^-25 of a turn at 2^31 times 0.16, by 1/8 at 2^31 times 5e5.)"""
+    rows, heads, hd = 12, 3, 64
+    rng = np.random.default_rng(11)
+    pos = np.array([2 ** 31 - 1, -2 ** 31, 2 ** 31 - 2, 2 ** 30 + 12345, -2 ** 29 - 1, 2 ** 28 + 1, 10 ** 6 + 7, 4097, 1, 0, -1, -77], np.int32)
+    t = most * rng.random(hd // 2)
+    left = np.array([[float((Fraction(int(p)) * Fraction(float(f)) + Fraction(1, 2)) % 1 - Fraction(1, 2)) for f in t] for p in pos])
+    x = rng.standard_normal((rows, heads, hd), np.float32)
+    gain = 1 + 0.1 * rng.standard_normal(hd).astype(np.float32)
+    dx, do, dt, dg, dp = (P.Dev(hip.lib, a) for a in (x, np.zeros_like(x), t, gain, pos))
+    assert hip.lib.tts_hip_rotary(do.ptr, dx.ptr, 0, rows, heads, hd, 0, 0, dp.ptr, P.how(hip, dt.ptr, hd, half, dg.ptr if norm else None)) == 0
+    y = x.astype(np.float64)
+    if norm:
+        y = y / np.sqrt((y * y).mean(-1, keepdims=True) + float(np.float32(1e-5))) * gain
+    a, b = (y[..., :hd // 2], y[..., hd // 2:]) if half else (y[..., 0::2], y[..., 1::2])
+    c, s = np.cos(2 * math.pi * left)[:, None], np.sin(2 * math.pi * left)[:, None]
+    got = do.get().astype(np.float64)
+    u, v = (got[..., :hd // 2], got[..., hd // 2:]) if half else (got[..., 0::2], got[..., 1::2])
+    # cosine and sine to 2 ulp of 1, the rest of the angle to 2^-24 of a step, two products and a sum: 2^-23 each; a norm adds its sum and five operations
+    tol = (8 * 2.0 ** -23 + ((hd / 8 + 8) * 2.0 ** -24 if norm else 0)) * (np.abs(a) + np.abs(b))
+    assert (np.abs(u - (a * c - b * s)) <= tol).all() and (np.abs(v - (a * s + b * c)) <= tol).all()
+    for d in (dx, do, dt, dg, dp):
+        d.free()

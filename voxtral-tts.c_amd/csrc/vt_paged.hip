@@ -154,8 +154,9 @@ extern "C" const int *tts_hip_paged_positions(const tts_hip_paged_t *b) {
 }
 
 /* ---- positions ----
- * Pair i of a head turns by 2 pi position turns[i].  The product is made in 64 bits and only what is left of it below one turn goes on in fp32, in two
- * parts: the angle is right to 2^-24 or so however far the position (in fp32 it would be off by 0.03 at position 10^6). */
+ * Pair i of a head turns by 2 pi position turns[i].  The product is made in 64 bits, with what that rounds away, and only what is left of it below one turn
+ * goes on in fp32, in two parts: the angle is that of these turns to 2^-24 or so however far the position (in fp32 it would be off by 0.03 at position 10^6).
+ * The turns themselves are made here to some 2^-52: what is left of the formula's angle is off by that times the position, 2^-24 at 2^28, 2^-21 at 2^31. */
 __global__ void __launch_bounds__(256) vt_rotary_turns_kernel(double *turns, int pairs, double theta, double factor, double original, double low, double high) {
     const int i = (int)(blockIdx.x * 256 + threadIdx.x);
     if (i >= pairs) return;
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(256) vt_turn_kernel(turn_job a) {
         const double pos = (double)a.pos[row];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const double t = pos * a.turns[min(4 * u + e, rot / 2 - 1)], left = t - rint(t);
+            const double f = a.turns[min(4 * u + e, rot / 2 - 1)], t = pos * f, left = t - rint(t) + fma(pos, f, -t);
             const float near = (float)left, more = (float)(left - (double)near) * 6.28318531f;
             float sn, cs;
             sincospif(2.f * near, &sn, &cs);
