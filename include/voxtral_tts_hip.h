@@ -416,7 +416,9 @@ typedef struct {
 
 /* d_turns[i] = theta^(-2 i / rot_dim) / 2 pi for i < rot_dim / 2, stretched by `factor` (1: not): a pair that makes fewer than low_turns
  * turns in original_rows positions is divided by it, one that makes more than high_turns is not, in between the share goes with the turns.  original_rows 0
- * and a low_turns above 0 divide all of them.  Each is right to some 2^-52, an angle of it to 2^-24 at positions of 2^28 and 2^-21 at 2^31. */
+ * and a low_turns above 0 divide all of them.  Each is right to some 2^-52, an angle of it to 2^-24 at positions of 2^28 and 2^-21 at 2^31.
+ * The share goes with the turns themselves.  Models are also trained with one that goes with the pair's number i between two bounds: for such
+ * a model, or with any other rule, a program fills d_turns itself. */
 int tts_hip_rotary_turns(double *d_turns, int rot_dim, double theta, double factor, int original_rows, double low_turns, double high_turns);
 /* x [rows, n_heads, head_dim] -> out of the same type, x_stride and out_stride values from row to row (0: dense); row r at position
  * d_positions[r] (any int; device).  out may be x with the same stride, else they do not overlap.  Any alignment that the type allows; rows on
