@@ -151,3 +151,30 @@ def test_angles_are_those_of_the_turns_given(hip, most, half, norm):
     assert (np.abs(u - (a * c - b * s)) <= tol).all() and (np.abs(v - (a * s + b * c)) <= tol).all()
     for d in (dx, do, dt, dg, dp):
         d.free()
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("layout,batch,page,common,window", [
+    ((32, 8, 128), " ".join(["1@700"] * 64), 16, 30, 0), ((32, 8, 128), "1@2000 1@640 37@900 1@641", 32, 20, 0), ((16, 16, 64), "300@1500 1@5000 9@1500", 64, 23, 0),
+    ((32, 8, 128), "600@1500 1@1500 2@1600 1@9000", 16, 93, 1000), ((12, 4, 256), "3@300 1@700", 256, 1, 0), ((32, 8, 128), "1@9000 1@9000 1@9000", 16, 562, 0)])
+def test_sequences_that_share_pages(hip, layout, batch, page, common, window, bf16):
+    """A common beginning of `common` pages that all read, steps and prompts, and what follows it of each."""
+    c = P.Cache(hip, batch, page, *layout, window=window, seed=len(batch))
+    c.tables = [np.concatenate((c.tables[0][:common], t[common:])) for t in c.tables]
+    assert all(p >= common * page for p in c.past) and c.batch.set(c.past, c.rows, c.tables) == 0
+    c.fill()
+    c.upload()
+    q = normal(np.random.default_rng(7), (sum(c.rows), layout[0], layout[2]), bf16)
+    scale, keep = 1 / math.sqrt(layout[2]), c.some()
+    got = P.attention(c, q, bf16, scale)
+    assert np.isfinite(got).all() and P.check(c, got, *c.attend(q, scale, keep), bf16, keep)
+    x = normal(np.random.default_rng(8), (sum(c.rows), layout[1], layout[2]), bf16)
+    d = P.Dev(hip.lib, P.bits16(x) if bf16 else x)
+    assert hip.lib.tts_hip_paged_append(c.batch.ptr, c.dev["k"].ptr, c.dev["v"].ptr, d.ptr, d.ptr, bf16, 0, None) == 0
+    pos = c.positions()
+    pages = np.concatenate([t[np.arange(p, p + r) // page] for t, r, p in zip(c.tables, c.rows, c.past)])
+    for pool, new in zip((c.k, c.v), c.download()):
+        pool[pages, :, pos % page] = P.bits16(x)
+        assert np.array_equal(new, pool)                                                # the common pages are as they were
+    d.free()
+    c.free()

@@ -16,6 +16,7 @@ struct tts_hip_paged {
     size_t at_place, at_tables, at_items, described, bytes;
     hipEvent_t copied;                   /* the last batch has left `host` */
     int *starts, *written;
+    unsigned long long *seen;            /* a bit for each page, 0 between calls */
     /* the batch, and how it is worked on; n_seqs -1: none yet */
     int n_seqs, n_rows;
     vt_paged_plan plan[2];               /* for fp32 and bf16 queries */

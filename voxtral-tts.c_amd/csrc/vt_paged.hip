@@ -33,10 +33,12 @@ extern "C" tts_hip_paged_t *tts_hip_paged_create(const tts_hip_paged_shape_t *sh
     }
     tts_hip_paged *b = new (std::nothrow) tts_hip_paged();
     int *own = (int *)malloc(sizeof(int) * ((size_t)max_seqs + max_rows));
-    if (!b || !own) {
+    unsigned long long *seen = (unsigned long long *)calloc((size_t)s.n_pages / 64 + 1, sizeof *seen);
+    if (!b || !own || !seen) {
         vt_set_error("%s: out of host memory", who);
         delete b;
         free(own);
+        free(seen);
         return NULL;
     }
     b->shape = s;
@@ -49,6 +51,7 @@ extern "C" tts_hip_paged_t *tts_hip_paged_create(const tts_hip_paged_shape_t *sh
     b->bytes = b->described + sizeof(vt_paged_item) * (size_t)b->max_items;
     b->starts = own;
     b->written = own + max_seqs;
+    b->seen = seen;
     return b;
 }
 
@@ -65,6 +68,7 @@ extern "C" void tts_hip_paged_free(tts_hip_paged_t *b) {
         if (before != b->device) (void)hipSetDevice(before);
     }
     free(b->starts);
+    free(b->seen);
     delete b;
 }
 
@@ -132,6 +136,7 @@ extern "C" int tts_hip_paged_set(tts_hip_paged_t *b, int n_seqs, const int *past
         b->plan[1] = vt_paged_plan_of(b->shape, true, n_cu, n_seqs, past, rows, b->starts, items + n_items);
         n_items += b->plan[1].few + b->plan[1].many;
     }
+    vt_paged_once(b->plan, 2, b->shape, n_seqs, past, rows, b->starts, (const int *)(b->host + b->at_tables), b->seen);
     const size_t all = b->at_items + sizeof(vt_paged_item) * (size_t)n_items;
     if (n_rows && vt_check(hipMemcpyAsync(b->dev, b->host, all, hipMemcpyHostToDevice, g_vt.stream), who)) return -1;
     if (vt_check(hipEventRecord(b->copied, g_vt.stream), who)) return -1;

@@ -160,8 +160,8 @@ static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, in
  * A wave has 32 rows of K and V in registers at a time, asks for the next as soon as these are used, and waits for nobody; the waves of a workgroup, and then
  * the workgroups that share the columns' rows, add their parts in a fixed order, the last workgroup to arrive those of all.  K is the A operand of 16 x 16 x
  * 32, a lane's 16 bytes from its own row.  V's rows are its columns: a lane loads CD values each of the eight rows that it has weights of, 16 lanes a whole
- * row, and pairs of rows are put together two values at a time.  Queries, the same for all waves, wait in LDS as operands.  ONCE: no other workgroup reads
- * these rows, and there are more than a cache holds.
+ * row, and pairs of rows are put together two values at a time.  Queries, the same for all waves, wait in LDS as operands.  ONCE: other workgroups
+ * read few of these rows, and there are more than a cache holds.
  *
  * Rows are read as they lie and once for 16 or 32 columns, so that memory bounds a long cache: one query behind 65535 rows of 8 x 128, 268 MB, 44 us
  * (6.1 TB/s), steps of 64 sequences of 118000 rows, 483 MB, 82 us (5.9 TB/s).  A short one is bound by what follows on each other in a workgroup - its

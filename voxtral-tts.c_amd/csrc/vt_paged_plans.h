@@ -96,12 +96,12 @@ static inline vt_paged_fault vt_paged_lay_out(const vt_paged_shape &s, int max_s
 
 /* ---- work items --- */
 
-/* items of either kernel (the few's first), parts that they leave; wide: the few's columns go by 32; once: their rows are read by one workgroup each, more
- * of them than a cache holds */
+/* items of either kernel (the few's first), parts that they leave; wide: the few's columns go by 32; once: their rows are read by one workgroup each, but for
+ * pages that sequences share (vt_paged_once), more of them than a cache holds */
 struct vt_paged_plan { int few, many, few_slots, many_slot, many_slots, wide, once, both; };
 
-/* Which kernels a batch goes to: `any`, whether there are sequences for the one for many columns; columns of a workgroup of the other, whether its rows are
- * read by one workgroup only, and their bytes */
+/* Which kernels a batch goes to: `any`, whether there are sequences for the one for many columns; columns of a workgroup of the other, whether one workgroup
+ * reads a sequence's rows, and their bytes */
 struct vt_paged_kinds { bool any; int few_cols; bool once; double bytes; };
 
 static inline long long vt_paged_max_items(int max_seqs, int max_rows, int group) {
@@ -319,11 +319,41 @@ static inline vt_paged_plan vt_paged_plan_of(const vt_paged_shape &s, bool bf16,
     p.both = p.few && p.many && p.few + p.many <= 65535 && vt_paged_may_be_both(s, kinds);
     if (p.both) qsort(to, p.few + p.many, sizeof *to, vt_paged_slowest);
     p.wide = kinds.few_cols > 16;
-    /* Requests that leave nothing behind in the caches: 65535 rows of 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows, which the
-     * caches (32 MB of L2) keep for the next call on them, 6.8 -> 7.2.  Beside a prompt as well: 31 sequences 43.4 -> 41.3, three of 10000 to 30000 76 ->
-     * 72. */
     p.once = kinds.once && kinds.bytes >= PAGED_CACHED;
     return p;
+}
+
+/* Requests that leave nothing behind in the caches, for rows that nobody reads again and that the caches (32 MB of L2) do not keep for the next call: 65535 rows of
+ * 8 x 128 53.6 -> 48.2 us, 64 sequences of 118000 91.6 -> 83.4; but 300 rows 6.8 -> 7.2.  Beside a prompt as well: 31 sequences 43.4 -> 41.3, three of 10000 to
+ * 30000 76 -> 72.  Sequences may share pages that they read, a common beginning, and with such requests each fetches these for itself.  us without and with
+ * them, steps of 64 sequences on c common rows and r of their own, share of the rows read that another one has read before: c 4000, r 1 (98 %) 73.6 / 83.1,
+ * c 4000, r 1000 (79 %) 114 / 124, c 1000, r 1000 (49 %) 61.6 / 61.5, c 1000, r 4000 (20 %) 189 / 179, none 90 / 82; 16 sequences c 8000, r 4000 (62 %) 79 /
+ * 92; 256 sequences c 512, r 512 (50 %) 118 / 125. */
+#define PAGED_AGAIN 0.33
+/* What is left of `once` in n plans of a batch that vt_paged_lay_out has laid out.  `seen`: a bit for each page of the pool, all 0 before and after. */
+static inline void vt_paged_once(vt_paged_plan *plans, int n, const vt_paged_shape &s, int n_seqs, const int *past, const int *rows, const int *starts,
+                                 const int *tables, unsigned long long *seen) {
+    int once = 0, log = 0;
+    for (int i = 0; i < n; i++) once |= plans[i].once;
+    if (!once) return;
+    while (1 << log < s.page_rows) log++;
+    long long all = 0, again = 0;
+    for (int clear = 0; clear < 2; clear++)
+        for (int i = 0; i < n_seqs; i++) {
+            if (rows[i] == 0) continue;
+            const int first = vt_paged_first(s.window, past[i], 0) >> log, last = (past[i] + rows[i] - 1) >> log;
+            for (int p = first; p <= last; p++) {
+                const int page = tables[starts[i] + p];
+                unsigned long long *word = seen + page / 64, bit = 1ull << (page & 63);
+                if (clear) { *word = 0; continue; }
+                all++;
+                again += (*word & bit) != 0;
+                *word |= bit;
+            }
+        }
+    const double bytes = (double)(all - again) * s.page_rows * 4 * s.n_kv_heads * s.head_dim;
+    if ((double)again <= PAGED_AGAIN * (double)all && bytes >= PAGED_CACHED) return;
+    for (int i = 0; i < n; i++) plans[i].once = 0;
 }
 
 #endif /* VT_PAGED_PLANS_H */
