@@ -56,3 +56,21 @@ int main(void) {
 def test_rows_that_others_read_too():
     out = P.run(SHARED)
     assert out.splitlines()[-1] == "0", out
+
+
+LONGEST = r"""
+#include <stdio.h>
+#include "vt_paged_plans.h"
+int main(void) {
+    /* row, past, cols, table, c0, lo, end, slot, part, parts, counter, many */
+    vt_paged_item it[] = {{0, 100, 16, 0, 0, 0, 101, 0, 0, 1, 0, 0}, {1, (1 << 30) - 1, 128, 0, 0, 0, 1 << 30, 0, 0, 1, 0, 1},
+                          {2, (1 << 30) - 2, 16, 0, 0, 0, (1 << 30) - 1, 0, 0, 1, 0, 0}, {3, 700, 128, 0, 0, 0, 701, 0, 0, 1, 0, 1}};
+    qsort(it, 4, sizeof *it, vt_paged_slowest);
+    for (const auto &x : it) printf("%d ", x.row);
+    return 0;
+}
+"""
+
+
+def test_the_longest_comes_first_at_any_length():
+    assert P.run(LONGEST).split() == ["1", "2", "3", "0"]

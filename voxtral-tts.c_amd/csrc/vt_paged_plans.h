@@ -273,7 +273,7 @@ static int vt_paged_longest(const void *a, const void *b) {
 /* .. of both kernels: the few's units, of 128 rows, take about as long as the many's, of 64 */
 static int vt_paged_slowest(const void *a, const void *b) {
     const vt_paged_item *x = (const vt_paged_item *)a, *y = (const vt_paged_item *)b;
-    const int n = (x->end - x->lo) << x->many, m = (y->end - y->lo) << y->many;
+    const long long n = (long long)(x->end - x->lo) << x->many, m = (long long)(y->end - y->lo) << y->many;
     if (n != m) return n > m ? -1 : 1;
     return x->many != y->many ? (x->many ? -1 : 1) : vt_paged_longest(a, b);
 }
