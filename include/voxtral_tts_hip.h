@@ -397,8 +397,10 @@ tts_hip_paged_t *tts_hip_paged_create(const tts_hip_paged_shape_t *shape, int ma
 void tts_hip_paged_free(tts_hip_paged_t *batch);
 /* The batch to come: sequence i has rows[i] new rows (none is allowed) behind past[i] cached ones and the pages tables[i * table_stride] ..,
  * host memory that is read during the call.  Page numbers are checked, up to 2^30 rows a sequence; entries of pages that no new row sees are not looked at.
- * Sequences may share pages that they read; a page that new rows go into twice is refused.  The description is on its way to the device when the call returns,
- * behind everything that was queued before; a refused one leaves the handle without a batch. */
+ * Sequences may share pages that they read; a page that new rows go into twice is refused.  The description is on its way to the device when the
+ * call returns, behind everything that was queued before; a refused one leaves the handle without a batch.  The call waits for the copy of the
+ * handle's last description, and so for what was queued ahead of that one; beside that it takes the host some 6 us for a few sequences,
+ * 27 for 64 of them and 120 for 32768 new rows. */
 int tts_hip_paged_set(tts_hip_paged_t *batch, int n_seqs, const int *past, const int *rows, const int *tables, int table_stride);
 /* The new rows' positions, one after the other (device memory of the handle), for tts_hip_rotary; NULL: no batch. */
 const int *tts_hip_paged_positions(const tts_hip_paged_t *batch);
