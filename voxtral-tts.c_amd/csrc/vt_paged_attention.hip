@@ -164,7 +164,7 @@ static __device__ __forceinline__ pa_rows pa_place(const pa_const_int *table, in
  * read few of these rows, and there are more than a cache holds.
  *
  * Rows are read as they lie and once for 16 or 32 columns, so that memory bounds a long cache: one query behind 65535 rows of 8 x 128, 268 MB, 44 us
- * (6.1 TB/s), steps of 64 sequences of 118000 rows, 483 MB, 82 us (5.9 TB/s).  A short one is bound by what follows on each other in a workgroup - its
+ * (6.1 TB/s), steps of 64 sequences of 118000 rows, 483 MB, 83 us (5.8 TB/s).  A short one is bound by what follows on each other in a workgroup - its
  * item, its table, queries and rows, a part's store, counter and merge: one query behind 1999 rows 8 us a call with 4 for the launch. */
 template <int HP, bool F32, int CT>
 struct pa_few_sizes {
@@ -254,128 +254,128 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
     __syncthreads();
     auto sums = [&](const unsigned long long (&over)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < CT; c++) {
-        m[c] = -3.402823466e38f;                         /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
-        l[c] = 0.f;
+        for (int c = 0; c < CT; c++) {
+            m[c] = -3.402823466e38f;                         /* finite: with nothing seen yet a hidden score's weight is exp2(-inf) all the same */
+            l[c] = 0.f;
 #pragma unroll
-        for (int i = 0; i < CHUNKS * CD; i++) o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+            for (int i = 0; i < CHUNKS * CD; i++) o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll 1
-    for (int t = wave; t < tiles; t += WAVES) {
-        const int first = base + PAGED_FEW_ROWS * t;
-        const bool hidden = first < all_lo || first + PAGED_FEW_ROWS > all_hi;
-        place(t + WAVES);
-        int own = lane;                                  /* (through an empty asm: else the queries are kept in registers after all) */
-        asm volatile("" : "+v"(own));
-        f32x4 s[CT][2];
-#pragma unroll
-        for (int c = 0; c < CT; c++) {
-            s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (c && !two) break;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int p = NQ - 1; p >= 0; p--) {
-                    const pa_bf16x8 q = pa_operand(queries[((ks * CT + c) * NQ + p) * 64 + own]);
-#pragma unroll
-                    for (int kt = 0; kt < 2; kt++) s[c][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(k[kt][ks]), q, s[c][kt], 0, 0, 0);
-                }
-        }
-        ask_k();
-        auto sees = [&](int c, int kt, int v) { const int key = first + 16 * kt + 4 * g + v; return key >= see_lo[c] && key < see_hi[c]; };
-        bool bad = false;
-        if (hidden) {
-#pragma unroll
-            for (int c = 0; c < CT; c++)
-#pragma unroll
-                for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++) s[c][kt][v] = sees(c, kt, v) ? s[c][kt][v] : -INFINITY;
-            pa_u16x2 most = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int ch = 0; ch < CHUNKS; ch++)
-#pragma unroll
-                    for (int e = 0; e < CD / 2; e++) most = pa_larger(most, v[j][ch][e]);
-            bad = __any(pa_not_finite(most));
-        }
-        u32x4 w4[CT][NP];
-#pragma unroll
-        for (int c = 0; c < CT; c++) {
-            if (c && !two) break;
-            float top = __builtin_elementwise_maximum(s[c][0][0], s[c][1][0]);                /* a NaN stays one: who sees it answers NaN */
-#pragma unroll
-            for (int v = 1; v < 4; v++) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[c][0][v]), s[c][1][v]);
-            {
-                f32x2 r = vt_swap16(top, top);
-                top = __builtin_elementwise_maximum(r.x, r.y);
-                r = vt_swap32(top, top);
-                top = __builtin_elementwise_maximum(r.x, r.y);
-            }
-            if constexpr (!F32) top = top * a.scale;
-            if (over[c]) top += pa_lift(over[c], it.end - it.lo);
-            if (pa_far(top, m[c])) {
-                const float less = pa_follow(top, m[c]);
-                l[c] *= less;
-#pragma unroll
-                for (int i = 0; i < CHUNKS * CD; i++) o[c][i] = o[c][i] * less;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float p0 = pa_weight<F32>(s[c][e >> 1][2 * (e & 1)], m[c], a.scale), p1 = pa_weight<F32>(s[c][e >> 1][2 * (e & 1) + 1], m[c], a.scale);
-                l[c] += p0 + p1;
-                unsigned w[NP];
-                pa_planes2<NP>(p0, p1, w);
-#pragma unroll
-                for (int p = 0; p < NP; p++) w4[c][p][e] = w[p];
-            }
-        }
-        if (bad) {                                       /* rare */
+        for (int t = wave; t < tiles; t += WAVES) {
+            const int first = base + PAGED_FEW_ROWS * t;
+            const bool hidden = first < all_lo || first + PAGED_FEW_ROWS > all_hi;
+            place(t + WAVES);
+            int own = lane;                                  /* (through an empty asm: else the queries are kept in registers after all) */
+            asm volatile("" : "+v"(own));
+            f32x4 s[CT][2];
 #pragma unroll
             for (int c = 0; c < CT; c++) {
-                u32x4 ones;
+                s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (c && !two) break;
 #pragma unroll
-                for (int e = 0; e < 4; e++) ones[e] = (sees(c, e >> 1, 2 * (e & 1)) ? 0x3f80u : 0u) | (sees(c, e >> 1, 2 * (e & 1) + 1) ? 0x3f800000u : 0u);
+                for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int ch = 0; ch < CHUNKS; ch++)
+                    for (int p = NQ - 1; p >= 0; p--) {
+                        const pa_bf16x8 q = pa_operand(queries[((ks * CT + c) * NQ + p) * 64 + own]);
 #pragma unroll
-                    for (int i = 0; i < CD; i++) {
-                        u32x4 v4;
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            v4[e] = pa_marks(__builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u));
-                        const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(ones), (f32x4{0.f, 0.f, 0.f, 0.f}), 0, 0, 0);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[c][ch * CD + i][e] = hit[e] > 0.f ? NAN : o[c][ch * CD + i][e];
+                        for (int kt = 0; kt < 2; kt++) s[c][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(k[kt][ks]), q, s[c][kt], 0, 0, 0);
                     }
             }
+            ask_k();
+            auto sees = [&](int c, int kt, int v) { const int key = first + 16 * kt + 4 * g + v; return key >= see_lo[c] && key < see_hi[c]; };
+            bool bad = false;
+            if (hidden) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
+                for (int c = 0; c < CT; c++)
 #pragma unroll
-                for (int ch = 0; ch < CHUNKS; ch++)
+                    for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-                    for (int e = 0; e < CD / 2; e++) v[j][ch][e] = pa_finite(v[j][ch][e]);
-        }
+                        for (int v = 0; v < 4; v++) s[c][kt][v] = sees(c, kt, v) ? s[c][kt][v] : -INFINITY;
+                pa_u16x2 most = {0, 0};
 #pragma unroll
-        for (int ch = 0; ch < CHUNKS; ch++)
+                for (int j = 0; j < 8; j++)
 #pragma unroll
-            for (int i = 0; i < CD; i++) {
-                u32x4 v4;
+                    for (int ch = 0; ch < CHUNKS; ch++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) v4[e] = __builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                        for (int e = 0; e < CD / 2; e++) most = pa_larger(most, v[j][ch][e]);
+                bad = __any(pa_not_finite(most));
+            }
+            u32x4 w4[CT][NP];
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--)
-                    o[0][ch * CD + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[0][p]), o[0][ch * CD + i], 0, 0, 0);
-                if constexpr (CT == 2) {                 /* (also where there is no second: a branch for each would cost more) */
+            for (int c = 0; c < CT; c++) {
+                if (c && !two) break;
+                float top = __builtin_elementwise_maximum(s[c][0][0], s[c][1][0]);                /* a NaN stays one: who sees it answers NaN */
 #pragma unroll
-                    for (int p = NP - 1; p >= 0; p--)
-                        o[CT - 1][ch * CD + i] =
-                            __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[CT - 1][p]), o[CT - 1][ch * CD + i], 0, 0, 0);
+                for (int v = 1; v < 4; v++) top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, s[c][0][v]), s[c][1][v]);
+                {
+                    f32x2 r = vt_swap16(top, top);
+                    top = __builtin_elementwise_maximum(r.x, r.y);
+                    r = vt_swap32(top, top);
+                    top = __builtin_elementwise_maximum(r.x, r.y);
+                }
+                if constexpr (!F32) top = top * a.scale;
+                if (over[c]) top += pa_lift(over[c], it.end - it.lo);
+                if (pa_far(top, m[c])) {
+                    const float less = pa_follow(top, m[c]);
+                    l[c] *= less;
+#pragma unroll
+                    for (int i = 0; i < CHUNKS * CD; i++) o[c][i] = o[c][i] * less;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p0 = pa_weight<F32>(s[c][e >> 1][2 * (e & 1)], m[c], a.scale), p1 = pa_weight<F32>(s[c][e >> 1][2 * (e & 1) + 1], m[c], a.scale);
+                    l[c] += p0 + p1;
+                    unsigned w[NP];
+                    pa_planes2<NP>(p0, p1, w);
+#pragma unroll
+                    for (int p = 0; p < NP; p++) w4[c][p][e] = w[p];
                 }
             }
-        ask_v();
-    }
+            if (bad) {                                       /* rare */
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    u32x4 ones;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) ones[e] = (sees(c, e >> 1, 2 * (e & 1)) ? 0x3f80u : 0u) | (sees(c, e >> 1, 2 * (e & 1) + 1) ? 0x3f800000u : 0u);
+#pragma unroll
+                    for (int ch = 0; ch < CHUNKS; ch++)
+#pragma unroll
+                        for (int i = 0; i < CD; i++) {
+                            u32x4 v4;
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                v4[e] = pa_marks(__builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u));
+                            const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(ones), (f32x4{0.f, 0.f, 0.f, 0.f}), 0, 0, 0);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[c][ch * CD + i][e] = hit[e] > 0.f ? NAN : o[c][ch * CD + i][e];
+                        }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int ch = 0; ch < CHUNKS; ch++)
+#pragma unroll
+                        for (int e = 0; e < CD / 2; e++) v[j][ch][e] = pa_finite(v[j][ch][e]);
+            }
+#pragma unroll
+            for (int ch = 0; ch < CHUNKS; ch++)
+#pragma unroll
+                for (int i = 0; i < CD; i++) {
+                    u32x4 v4;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v4[e] = __builtin_amdgcn_perm(v[2 * e + 1][ch][i / 2], v[2 * e][ch][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; p--)
+                        o[0][ch * CD + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[0][p]), o[0][ch * CD + i], 0, 0, 0);
+                    if constexpr (CT == 2) {                 /* (also where there is no second: a branch for each would cost more) */
+#pragma unroll
+                        for (int p = NP - 1; p >= 0; p--)
+                            o[CT - 1][ch * CD + i] =
+                                __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa_operand(v4), pa_operand(w4[CT - 1][p]), o[CT - 1][ch * CD + i], 0, 0, 0);
+                    }
+                }
+            ask_v();
+        }
     };
     unsigned long long over[2] = {0, 0};
     sums({0, 0});
@@ -481,11 +481,12 @@ static __device__ __forceinline__ void pa_few(const pa_job &a, int item, u32x4 *
  * A unit is 32 rows.  While unit u's weights are made and multiplied, the matrix cores make unit u + 1's scores, so that K's tiles lie half a tile behind
  * V's: beside V's rows 64 t .. 64 t + 63 stand K's 64 t + 32 .. 64 t + 95.
  *
- * Matrix instructions bound it, and for bf16 the vector unit beside them, which has two values' weights to make for each: 4000 rows behind none of 32 heads
- * of 128 fp32 (three planes of queries and of weights, 393 G multiplications and additions) 316 us, the rate of a large matrix product, bf16 (two planes of
- * weights, 197 G) 193 us; 1531 rows fp32 61 us, of which the first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a window of 2048
- * bf16 137 us.  Heads of 256 bf16 values have one workgroup to a CU, for its LDS and registers: 3000 rows of 12 on 4 behind none 130 us (83 G).  With weights
- * of one plane these three take 153, 107 and 115 us, and a result is off by 2.1e-3 of its norm instead of the 1.6e-3 that its own rounding leaves. */
+ * Matrix instructions bound it, and for bf16 the vector unit beside them, which has two values' weights to make for each: with two waves to a SIMD they overlap
+ * little (busy 49 and 39 % of the time; 62 and 35 in fp32).  4000 rows behind none of 32 heads of 128 fp32 (three planes of queries and of weights, 393 G
+ * multiplications and additions) 316 us, the rate of a large matrix product, bf16 (two planes of weights, 197 G) 193 us; 1531 rows fp32 61 us, of which the
+ * first tiles' way and the parts' end are 15; four prompts of 226 to 2000 rows in a window of 2048 bf16 137 us.  Heads of 256 bf16 values have one workgroup
+ * to a CU, for its LDS and registers: 3000 rows of 12 on 4 behind none 134 us (83 G).  With weights of one plane these three take 153, 107 and 115 us, and a
+ * result is off by 2.1e-3 of its norm instead of the 1.6e-3 that its own rounding leaves. */
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 
 /* fp32: the compiler keeps to the order that is written, in which an instruction's operands are asked for just ahead of it and no more of them wait in
